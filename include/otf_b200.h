@@ -441,6 +441,130 @@ OTF_API int otf_attn_decode_noalloc(const void* q, const void* k_cache, const vo
                                     void* out, float scale, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                     int64_t max_pos, void* stream);
 
+/*
+ * A key/value cache in pages, for sequences of different lengths (no counterpart in the
+ * reference, whose runner keeps HF's contiguous cache of one sequence,
+ * otf_llm/run_symmetric_2bit.py:150-187; otf_attn_rope_decode_batch is the contiguous form).
+ * Token s of sequence b lies in page page_table[b * ld_table + s / page_size] at place
+ * s % page_size: its key for KV head h is the head_dim values at k_pages + page * page_stride +
+ * place * token_stride + h * head_stride (elements), its value the same in v_pages.  Both pools
+ * are 16-byte aligned and the strides multiples of 8, so pages may hold [token, head, dim] or
+ * [head, token, dim].  lengths[b] counts the tokens cached before a call; a negative length
+ * marks a place of the batch without a sequence, which every call leaves as it is.
+ * dtype: OTF_DTYPE_F16 or OTF_DTYPE_BF16 (queries and outputs have the cache's type).
+ * head_dim 64 or 128; at most 4096 sequences; max_pages * page_size below 2^31.
+ * A sequence whose tokens do not fit in max_pages pages, or (in otf_paged_append and
+ * otf_paged_evict) a token whose page is not in [0, n_pages), is left out: nothing of it is
+ * written and the otf_device_error flag is raised.  In otf_paged_attn tokens of such a page
+ * read as zeros, and the flag is raised.
+ */
+typedef struct otf_paged_cache {
+  void* k_pages;
+  void* v_pages;
+  int64_t page_stride, token_stride, head_stride;
+  int64_t n_pages, page_size, kv_heads, head_dim;
+  const int32_t* page_table; /* device int32 [batch, ld_table] */
+  int64_t ld_table, max_pages;
+  const int32_t* lengths;    /* device int32 [batch] */
+  int64_t batch;
+  int32_t dtype;
+} otf_paged_cache;
+
+/*
+ * Rotary positions.  The first rot_dim values of a head turn by position * frequency:
+ * pairs (i, i + rot_dim / 2), or (2i, 2i + 1) when interleaved, become
+ * factor * (x c - y s, y c + x s); the others stay.  turns: device double [rot_dim / 2], the
+ * frequencies divided by 2 pi, so that scaled frequencies need no other form and angles of
+ * far positions keep 64 bits until they are reduced to one turn.  rot_dim even, 0..head_dim.
+ */
+typedef struct otf_rotary {
+  const double* turns;
+  int64_t rot_dim;
+  float factor;
+  int32_t interleaved;
+} otf_rotary;
+
+/*
+ * New tokens enter the cache: their queries and keys turned, keys and values written.
+ * q: [n, heads, head_dim] with row stride ldq (heads next to one another), written to q_out
+ * (which may be q); k, v: [n, kv_heads, head_dim] with row strides ldk, ldv.  q may be NULL
+ * (keys and values alone).  Sequence b has the rows [starts[b], starts[b + 1]) (device int32
+ * [batch + 1], starts[0] = 0), or with starts NULL n / batch rows each; its t-th row becomes
+ * token lengths[b] + t.  Rows behind the last sequence are left as they were.  positions
+ * (device int32 [n], may be NULL): the rows' rotary positions, where they are not those
+ * tokens' places (after otf_paged_evict).  rotary may be NULL (nothing turns).  The pointers
+ * are 16-byte aligned, the strides multiples of 8.  lengths is not advanced.  Arithmetic in
+ * fp32, one rounding.  The pages that new tokens enter belong to one sequence each.
+ * Beside otf_rope_kv, which turns whole heads of one position by fp16 tables.
+ */
+OTF_API int otf_paged_append(const otf_paged_cache* cache, const otf_rotary* rotary, const void* q, int64_t ldq,
+                             void* q_out, int64_t ldqo, int64_t heads, const void* k, int64_t ldk, const void* v,
+                             int64_t ldv, const int32_t* starts, const int32_t* positions, int64_t n, void* stream);
+
+/*
+ * Attention of the `tokens` (1..16) newest tokens of every sequence over its pages: row
+ * b * tokens + t of q ([batch * tokens, heads, head_dim], row stride ldq) sees the tokens
+ * 0 .. lengths[b] + t (its own key among them: otf_paged_append ran before, lengths not yet
+ * advanced) and out (row stride ldo) = softmax(scale q k) v, query head j reading KV head
+ * j / (heads / kv_heads).  What a row does not see does not reach it, whatever it holds.
+ * weights (fp32 [batch, kv_heads, ldw], may be NULL; ldw >= max_pages * page_size):
+ * weights[b, h, s] += the softmax weight that token s received from the rows and query heads of
+ * KV head h, for otf_paged_evict.  Scores, sums and outputs in fp32, joined over the parts of
+ * the cache in a fixed order.  workspace: otf_paged_attn_workspace_bytes(...), 256-byte aligned,
+ * need not be cleared; two calls that may run at the same time need one each.
+ */
+OTF_API int64_t otf_paged_attn_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                               int64_t tokens, int64_t max_tokens, int with_weights);
+OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* q, int64_t ldq, int64_t heads, int64_t tokens,
+                           float scale, void* out, int64_t ldo, float* weights, int64_t ldw, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
+/*
+ * Eviction: every sequence longer than `budget` tokens is cut to it, for each KV head by
+ * itself: the `recent` last tokens stay (0 <= recent <= budget), and of the others the
+ * budget - recent of the largest weights (ties: the lower place; a NaN counts as the largest).
+ * The order stays.  kept: int32 [batch, kv_heads, budget], the places kept, then -1.  The kept
+ * keys and values go to the same head's tokens 0, 1, ... of `to`, whose page_table holds pages
+ * that hold nothing of `from`, or all the same pages in the same order: then from's pools,
+ * table and lengths are given again and the cache is cut in place.  `to` has from's geometry
+ * (kv_heads, head_dim, batch, dtype, page_size) and room for budget tokens.  weights (fp32
+ * [batch, kv_heads, ldw]) go along to weights_out ([batch, kv_heads, ldw_out], may be weights),
+ * zero behind the kept ones (in place: up to the old length).  lengths_out[b] = min(lengths[b],
+ * budget).  Sequences within the budget are carried over whole.
+ */
+OTF_API int otf_paged_evict(const otf_paged_cache* from, const otf_paged_cache* to, const float* weights, int64_t ldw,
+                            float* weights_out, int64_t ldw_out, int64_t budget, int64_t recent, int32_t* kept,
+                            int32_t* lengths_out, void* stream);
+
+/*
+ * Verification of drafted tokens: with p = softmax(target / temperature) and q =
+ * softmax(draft / temperature) the j-th drafted token d is taken while uniforms[b, j] * q(d) <
+ * p(d); the first one that is not is replaced by a token of max(p - q, 0), and behind the last
+ * one a token of p follows, drawn as the largest w_i / noise[b, i] (noise: exponentially
+ * distributed random numbers; ties: the lower index).  temperature 0: a token is taken while it
+ * is the target's first largest logit, and that follows.
+ * target: fp32, row (b, j) at target + b * target_seq + j * ld_target, drafts + 1 rows of vocab
+ * values each; draft the same with drafts rows, or NULL: the drafted tokens were certain
+ * (looked up, or a greedy draft's), q = 1 at them.  tokens: int64 [batch, ld_tokens];
+ * uniforms: fp32 [batch, ld_uniforms]; noise: fp32 [batch, ld_noise] (both may be NULL when
+ * every temperature is 0).  temperatures: device fp32 [batch], or NULL: `temperature` for all.
+ * counts: device int32 [batch], the drafted tokens of each sequence (0..drafts), or NULL: all
+ * have `drafts` (0..32).  out_tokens: int64 [batch, drafts + 1], the taken tokens, the drawn
+ * one, then -1; accepted: int32 [batch].  Temperatures are 0 or in 1e-20 .. 1e20; a NaN among
+ * the logits is never the largest.  A sequence without a token of positive weight, or
+ * with a count or temperature out of range, gets -1 and raises the otf_device_error flag; so
+ * does a drafted token outside the vocabulary, which is refused.  Where max(p - q, 0) holds
+ * nothing, p is drawn from.  workspace: otf_verify_workspace_bytes(...), 256-byte aligned, need
+ * not be cleared, one per call at a time.  Beside otf_i8_head_argmax, the greedy pick of one row.
+ */
+OTF_API int64_t otf_verify_workspace_bytes(int64_t batch, int64_t drafts, int64_t vocab);
+OTF_API int otf_verify_drafts(const float* target, int64_t target_seq, int64_t ld_target, const float* draft,
+                              int64_t draft_seq, int64_t ld_draft, const int64_t* tokens, int64_t ld_tokens,
+                              const float* uniforms, int64_t ld_uniforms, const float* noise, int64_t ld_noise,
+                              const float* temperatures, float temperature, const int32_t* counts,
+                              int64_t* out_tokens, int32_t* accepted, int64_t batch, int64_t drafts, int64_t vocab,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

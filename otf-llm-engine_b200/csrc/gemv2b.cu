@@ -1924,6 +1924,8 @@ int ar_device_error(int clear);                 // tp_ar.cu
 int mk_device_error(int clear);                 // decode_step.cu
 int attn_device_error(int clear);               // attention.cu
 int head_device_error(int clear);               // int8_ops.cu
+int paged_device_error(int clear);              // paged.cu
+int verify_device_error(int clear);             // verify.cu
 
 static int num_sms() {
   static thread_local int cached[64] = {};
@@ -2519,6 +2521,8 @@ extern "C" OTF_API int otf_device_error(int clear) {
   const int x = mk_device_error(clear);
   const int a = attn_device_error(clear);
   const int h = head_device_error(clear);
-  if (w < 0 || x < 0 || a < 0 || h < 0) return -1;
-  return v | w | x | a | h;
+  const int p = paged_device_error(clear);
+  const int d = verify_device_error(clear);
+  if (w < 0 || x < 0 || a < 0 || h < 0 || p < 0 || d < 0) return -1;
+  return v | w | x | a | h | p | d;
 }

@@ -77,6 +77,21 @@ class DecodeDims(ctypes.Structure):
                 ("group_size", ctypes.c_int64), ("eps", ctypes.c_float), ("codebook", ctypes.c_float * 4)]
 
 
+class PagedCache(ctypes.Structure):
+    """Mirror of `otf_paged_cache`."""
+    _fields_ = [("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p), ("page_stride", ctypes.c_int64),
+                ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("n_pages", ctypes.c_int64),
+                ("page_size", ctypes.c_int64), ("kv_heads", ctypes.c_int64), ("head_dim", ctypes.c_int64),
+                ("page_table", ctypes.c_void_p), ("ld_table", ctypes.c_int64), ("max_pages", ctypes.c_int64),
+                ("lengths", ctypes.c_void_p), ("batch", ctypes.c_int64), ("dtype", ctypes.c_int32)]
+
+
+class RotaryArgs(ctypes.Structure):
+    """Mirror of `otf_rotary`."""
+    _fields_ = [("turns", ctypes.c_void_p), ("rot_dim", ctypes.c_int64), ("factor", ctypes.c_float),
+                ("interleaved", ctypes.c_int32)]
+
+
 # Names exported by the library; kept in step with include/otf_b200.h.
 EXPORTS = (
     "otf_version",
@@ -112,6 +127,12 @@ EXPORTS = (
     "otf_attn_rope_decode_batch",
     "otf_pos_advance_batch",
     "otf_attn_prefill",
+    "otf_paged_append",
+    "otf_paged_attn_workspace_bytes",
+    "otf_paged_attn",
+    "otf_paged_evict",
+    "otf_verify_workspace_bytes",
+    "otf_verify_drafts",
 )
 
 
@@ -198,6 +219,21 @@ def lib() -> ctypes.CDLL:
     L.otf2b_quantize.argtypes = [vp, i32, i64, i64, i64, i64, vp, i64, vp, vp, i64, vp, i64, vp, i64, vp, i64, vp,
                                  vp]
     L.otf2b_quantize.restype = i32
+    cache = ctypes.POINTER(PagedCache)
+    L.otf_paged_append.argtypes = [cache, ctypes.POINTER(RotaryArgs), vp, i64, vp, i64, i64, vp, i64, vp, i64, vp, vp,
+                                   i64, vp]
+    L.otf_paged_append.restype = i32
+    L.otf_paged_attn_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i64, i32]
+    L.otf_paged_attn_workspace_bytes.restype = i64
+    L.otf_paged_attn.argtypes = [cache, vp, i64, i64, i64, ctypes.c_float, vp, i64, vp, i64, vp, i64, vp]
+    L.otf_paged_attn.restype = i32
+    L.otf_paged_evict.argtypes = [cache, cache, vp, i64, vp, i64, i64, i64, vp, vp, vp]
+    L.otf_paged_evict.restype = i32
+    L.otf_verify_workspace_bytes.argtypes = [i64, i64, i64]
+    L.otf_verify_workspace_bytes.restype = i64
+    L.otf_verify_drafts.argtypes = [vp, i64, i64, vp, i64, i64, vp, i64, vp, i64, vp, i64, vp, ctypes.c_float, vp, vp,
+                                    vp, i64, i64, i64, vp, i64, vp]
+    L.otf_verify_drafts.restype = i32
     _lib = L
     return L
 

@@ -1,0 +1,353 @@
+"""A key/value cache in pages for sequences of different lengths, on the native kernels.
+
+``PagedKVCache`` holds one layer's pages: ``append`` turns new queries and keys by their rotary
+positions and writes keys and values into the pages, ``attend`` is the attention of one or a few
+new tokens per sequence over them, ``evict`` cuts long sequences to a budget by accumulated
+attention weight.  ``Rotary`` holds the frequencies (whole heads or a part of them, half or
+interleaved layout, plain or scaled for long contexts).
+
+The contiguous caches of ``decode_model`` keep one fixed length per sequence; the reference keeps
+HF's cache of one sequence (otf_llm/run_symmetric_2bit.py:150-187).
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from . import _native
+
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1}
+MAX_NEW_TOKENS = 16
+
+_SCALING_KEYS = {
+    "default": (),
+    "linear": ("factor",),
+    "llama3": ("factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings"),
+    "yarn": ("factor", "original_max_position_embeddings"),
+}
+_SCALING_OPTIONAL = {"yarn": ("attention_factor", "beta_fast", "beta_slow")}
+
+
+def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling: Optional[dict] = None
+                     ) -> Tuple[torch.Tensor, float]:
+    """Rotary frequencies in radians per position (float64 [rot_dim / 2], on the CPU) and the factor
+    on the turned values.  ``scaling``: None, or a dict as HF configurations hold it in
+    ``rope_scaling``, with ``rope_type`` "default", "linear", "llama3" or "yarn" and its numbers."""
+    if rot_dim < 0 or rot_dim % 2:
+        raise ValueError(f"rot_dim must be even and not negative, got {rot_dim}")
+    if not theta > 0:
+        raise ValueError(f"theta must be positive, got {theta}")
+    i = torch.arange(0, rot_dim, 2, dtype=torch.float64)
+    f = float(theta) ** (-i / max(rot_dim, 1))
+    if scaling is None:
+        return f, 1.0
+    kind = scaling.get("rope_type", scaling.get("type"))
+    if kind not in _SCALING_KEYS:
+        raise ValueError(f"rope_type must be one of {sorted(_SCALING_KEYS)}, got {kind!r}")
+    need, may = _SCALING_KEYS[kind], _SCALING_OPTIONAL.get(kind, ())
+    missing = [k for k in need if scaling.get(k) is None]
+    unknown = [k for k in scaling if k not in need + may + ("rope_type", "type", "rope_theta")]
+    if missing or unknown:
+        raise ValueError(f"rope_type {kind!r}: missing {missing}, not supported {unknown}")
+    if kind == "default":
+        return f, 1.0
+    factor = float(scaling["factor"])
+    if not factor > 0:
+        raise ValueError(f"factor must be positive, got {factor}")
+    if kind == "linear":
+        return f / factor, 1.0
+    context = float(scaling["original_max_position_embeddings"])
+    if kind == "llama3":
+        low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        if not 0 < low < high:
+            raise ValueError("low_freq_factor must be positive and below high_freq_factor")
+        turns = context * f / (2 * math.pi)                 # over the original context
+        mix = ((turns - low) / (high - low)).clamp(0, 1)
+        return f * mix + f / factor * (1 - mix), 1.0
+    attention = scaling.get("attention_factor")
+    if attention is None:
+        attention = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+
+    def place(turns: float) -> float:                       # the pair that turns so often over the context
+        return rot_dim * math.log(context / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+    low = max(math.floor(place(float(scaling.get("beta_fast") or 32.0))), 0)
+    high = min(math.ceil(place(float(scaling.get("beta_slow") or 1.0))), rot_dim - 1)
+    ramp = ((i / 2 - low) / ((high - low) if high != low else 0.001)).clamp(0, 1)
+    return f * (1 - ramp) + f / factor * ramp, float(attention)
+
+
+class Rotary:
+    """Rotary positions of the first ``rot_dim`` values of every head (all of them by default):
+    pairs (i, i + rot_dim / 2), or (2i, 2i + 1) if ``interleaved``.  See ``rope_frequencies``."""
+
+    def __init__(self, head_dim: int, *, rot_dim: Optional[int] = None, theta: float = 10000.0,
+                 scaling: Optional[dict] = None, interleaved: bool = False, device="cuda"):
+        rot_dim = head_dim if rot_dim is None else int(rot_dim)
+        if not 0 <= rot_dim <= head_dim:
+            raise ValueError(f"rot_dim {rot_dim} outside 0..{head_dim}")
+        self.head_dim, self.rot_dim, self.interleaved = int(head_dim), rot_dim, bool(interleaved)
+        self.frequencies, self.factor = rope_frequencies(rot_dim, theta, scaling)
+        self.turns = (self.frequencies / (2 * math.pi)).to(device)
+        a = _native.RotaryArgs()
+        a.turns, a.rot_dim = self.turns.data_ptr() if rot_dim else None, rot_dim
+        a.factor, a.interleaved = self.factor, int(self.interleaved)
+        self._args = a
+        self._ref = ctypes.byref(a)
+
+
+class PagedKVCache:
+    """One layer's keys and values in pages.
+
+    k_pages, v_pages: fp16 or bf16 [n_pages, page_size, kv_heads, head_dim] with the same strides
+    and unit inner stride (a transposed view of [n_pages, kv_heads, page_size, head_dim] will do);
+    page_table: int32 [batch, max_pages], whose row b names the pages of sequence b in order;
+    lengths: int32 [batch], the tokens that each sequence has cached, negative for a place
+    without a sequence (left as it is by every call).  The tensors stay the caller's: pages are
+    handed out by writing the table, and ``advance`` counts a step's tokens once every layer has
+    appended them (layers may share table and lengths).
+
+    Sequences that do not fit, and pages outside the pool, are left out on the device and raise
+    the ``_native.device_error`` flag (see include/otf_b200.h)."""
+
+    def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor):
+        for name, t in (("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table), ("lengths", lengths)):
+            _native._need_cuda(t, name)
+            if t.device != k_pages.device:
+                raise ValueError(f"{name} is on {t.device}, k_pages on {k_pages.device}")
+        if k_pages.dtype not in _DTYPES or v_pages.dtype != k_pages.dtype:
+            raise TypeError(f"pages must be fp16 or bf16 both, got {k_pages.dtype} and {v_pages.dtype}")
+        if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride():
+            raise ValueError("k_pages and v_pages must be [n_pages, page_size, kv_heads, head_dim] with equal strides")
+        n, page, heads, dim = k_pages.shape
+        if dim not in (64, 128):
+            raise ValueError(f"head_dim must be 64 or 128, got {dim}")
+        if n == 0 or page == 0 or heads == 0:
+            raise ValueError(f"empty pages {tuple(k_pages.shape)}")
+        stride = [s if e > 1 else dim for e, s in zip(k_pages.shape[:3], k_pages.stride()[:3])]
+        if k_pages.stride(3) != 1 or any(s % 8 or s < 0 for s in stride) or k_pages.data_ptr() % 16 or \
+                v_pages.data_ptr() % 16 or any(s < dim for s in stride[1:]):
+            raise ValueError(f"pages need 16-byte aligned rows and a unit inner stride, got strides {k_pages.stride()}")
+        if page_table.dtype != torch.int32 or lengths.dtype != torch.int32:
+            raise TypeError("page_table and lengths must be int32")
+        if page_table.dim() != 2 or page_table.shape[1] == 0 or page_table.stride(1) != 1:
+            raise ValueError("page_table must be a row-major [batch, max_pages] tensor")
+        if lengths.shape != page_table.shape[:1] or lengths.shape[0] == 0 or not lengths.is_contiguous():
+            raise ValueError(f"lengths must be a contiguous [{page_table.shape[0]}] vector")
+        self.k_pages, self.v_pages, self.page_table, self.lengths = k_pages, v_pages, page_table, lengths
+        self.device, self.dtype = k_pages.device, k_pages.dtype
+        self.page_size, self.kv_heads, self.head_dim = page, heads, dim
+        self.batch, self.max_pages = page_table.shape
+        self.capacity = self.max_pages * page
+        c = _native.PagedCache()
+        c.k_pages, c.v_pages = k_pages.data_ptr(), v_pages.data_ptr()
+        c.page_stride, c.token_stride, c.head_stride = stride
+        c.n_pages, c.page_size, c.kv_heads, c.head_dim = n, page, heads, dim
+        c.page_table, c.max_pages = page_table.data_ptr(), self.max_pages
+        c.ld_table = page_table.stride(0) if self.batch > 1 else max(page_table.stride(0), self.max_pages)
+        c.lengths, c.batch, c.dtype = lengths.data_ptr(), self.batch, _DTYPES[self.dtype]
+        self._args = c
+        self._ref = ctypes.byref(c)
+
+    @classmethod
+    def allocate(cls, n_pages: int, page_size: int, kv_heads: int, head_dim: int, page_table: torch.Tensor,
+                 lengths: torch.Tensor, dtype: torch.dtype = torch.float16) -> "PagedKVCache":
+        """A cache of new zeroed pages [n_pages, page_size, kv_heads, head_dim] under the given table."""
+        k, v = (torch.zeros(n_pages, page_size, kv_heads, head_dim, dtype=dtype, device=page_table.device)
+                for _ in range(2))
+        return cls(k, v, page_table, lengths)
+
+    def _heads(self, t: torch.Tensor, name: str, heads: Optional[int] = None) -> int:
+        """Check [rows, heads, head_dim] values whose heads lie next to one another; the row stride."""
+        if t.device != self.device or t.dtype != self.dtype:
+            raise ValueError(f"{name} must be {self.dtype} on {self.device}, got {t.dtype} on {t.device}")
+        d = self.head_dim
+        if t.dim() != 3 or t.shape[2] != d or (heads is not None and t.shape[1] != heads) or t.shape[1] == 0:
+            raise ValueError(f"{name} must be [rows, {heads or 'heads'}, {d}], got {tuple(t.shape)}")
+        row, head, one = t.stride()
+        if one != 1 or (head != d and t.shape[1] > 1):
+            raise ValueError(f"{name} needs its heads next to one another, got strides {t.stride()}")
+        if t.shape[0] <= 1:
+            row = t.shape[1] * d
+        if row % 8 or row < t.shape[1] * d or t.data_ptr() % 16:
+            raise ValueError(f"{name} needs 16-byte aligned rows that do not overlap, got strides {t.stride()}")
+        return row
+
+    def _vector(self, t: torch.Tensor, name: str, n: int) -> ctypes.c_void_p:
+        if t.device != self.device or t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 [{n}] vector on {self.device}")
+        return t.data_ptr()
+
+    def append(self, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, rotary: Optional[Rotary] = None, *,
+               starts: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+               q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+        """New tokens enter the cache (otf_paged_append).
+
+        q [n, heads, head_dim] (or None), k and v [n, kv_heads, head_dim]: rows of new tokens, e.g.
+        parts of a fused projection's output.  Sequence b has the rows starts[b] .. starts[b + 1] - 1
+        (int32 [batch + 1] on the device), or n / batch each; its t-th becomes token lengths[b] + t,
+        and turns by that position, or by positions[row] (int32 [n]) where places and positions
+        differ (after ``evict``).  Returns the turned queries, in ``q_out`` (which may be q) or a new
+        tensor.  Rows behind the last sequence are left as they were, as are those of a negative
+        length.  ``lengths`` is not advanced."""
+        n = k.shape[0]
+        ldk = self._heads(k, "k", self.kv_heads)
+        ldv = self._heads(v, "v", self.kv_heads)
+        if v.shape[0] != n:
+            raise ValueError(f"v has {v.shape[0]} rows, k {n}")
+        ldq = ldo = heads = 0
+        if q is not None:
+            ldq = self._heads(q, "q")
+            heads = q.shape[1]
+            if q.shape[0] != n:
+                raise ValueError(f"q has {q.shape[0]} rows, k {n}")
+            if q_out is None:
+                q_out = torch.empty((n, heads, self.head_dim), dtype=self.dtype, device=self.device)
+                ldo = heads * self.head_dim
+            else:
+                ldo = self._heads(q_out, "q_out", heads)
+                if q_out.shape[0] != n:
+                    raise ValueError(f"q_out has {q_out.shape[0]} rows, k {n}")
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        if starts is None and n % self.batch:
+            raise ValueError(f"{n} rows do not divide among {self.batch} sequences; give starts")
+        if rotary is not None and (rotary.head_dim != self.head_dim or rotary.turns.device != self.device):
+            raise ValueError(f"rotary is for heads of {rotary.head_dim} on {rotary.turns.device}")
+        if n:
+            with _on(self.device):
+                st = _native.lib().otf_paged_append(
+                    self._ref, None if rotary is None else rotary._ref, None if q is None else q.data_ptr(), ldq,
+                    None if q is None else q_out.data_ptr(), ldo, heads, k.data_ptr(), ldk, v.data_ptr(), ldv,
+                    None if starts is None else self._vector(starts, "starts", self.batch + 1),
+                    None if positions is None else self._vector(positions, "positions", n), n, _stream(self.device))
+            _native._check(st, "otf_paged_append")
+        return q_out
+
+    def attend(self, q: torch.Tensor, *, scale: Optional[float] = None, weights: Optional[torch.Tensor] = None,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of the newest tokens over the cache (otf_paged_attn).
+
+        q: [batch, heads, head_dim], or [batch, tokens, heads, head_dim] with the 1 to 16 newest
+        tokens of every sequence (all of them appended, ``lengths`` not yet advanced): row t of
+        sequence b sees the tokens 0 .. lengths[b] + t.  ``scale`` defaults to head_dim ** -0.5.
+        ``weights`` (fp32 [batch, kv_heads, at least capacity], contiguous): to every token's entry
+        is added the softmax weight that it received from the rows and the query heads of that KV
+        head.  Returns ``out``, of q's shape (rows of negative lengths are left as they were)."""
+        shape = q.shape
+        if q.dim() == 3:
+            tokens, rows = 1, q
+        elif q.dim() == 4:
+            tokens = shape[1]
+            rows = q.flatten(0, 1) if q.is_contiguous() else self._flat(q, "q")
+        else:
+            raise ValueError(f"q must have 3 or 4 dimensions, got {tuple(shape)}")
+        if shape[0] != self.batch or not 1 <= tokens <= MAX_NEW_TOKENS:
+            raise ValueError(f"q must hold 1 to {MAX_NEW_TOKENS} tokens of {self.batch} sequences, got {tuple(shape)}")
+        ldq = self._heads(rows, "q")
+        heads = rows.shape[1]
+        if heads % self.kv_heads:
+            raise ValueError(f"{heads} query heads over {self.kv_heads} KV heads")
+        if out is None:
+            out = torch.empty(shape, dtype=self.dtype, device=self.device)
+            ldo = heads * self.head_dim
+        else:
+            if out.shape != shape:
+                raise ValueError(f"out must have q's shape {tuple(shape)}, got {tuple(out.shape)}")
+            ldo = self._heads(out if out.dim() == 3 else self._flat(out, "out"), "out", heads)
+        ldw = 0
+        if weights is not None:
+            ldw = self._weights(weights, "weights", self.capacity)
+        L = _native.lib()
+        n = L.otf_paged_attn_workspace_bytes(self.batch, heads, self.kv_heads, self.head_dim, tokens, self.capacity,
+                                             0 if weights is None else 1)
+        if n < 0:
+            raise ValueError("shape not supported by otf_paged_attn")
+        # from the caching allocator, for this call alone: calls on two streams, or in two captured
+        # graphs, share nothing
+        ws = torch.empty(n, dtype=torch.uint8, device=self.device)
+        with _on(self.device):
+            st = L.otf_paged_attn(self._ref, rows.data_ptr(), ldq, heads, tokens,
+                                  self.head_dim ** -0.5 if scale is None else float(scale), out.data_ptr(), ldo,
+                                  None if weights is None else weights.data_ptr(), ldw, ws.data_ptr(), n,
+                                  _stream(self.device))
+        _native._check(st, "otf_paged_attn")
+        return out
+
+    def evict(self, weights: torch.Tensor, budget: int, recent: int, *, to: Optional["PagedKVCache"] = None,
+              weights_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Cut every sequence longer than ``budget`` tokens to it (otf_paged_evict), for each KV head
+        by itself: the ``recent`` last tokens stay, and of the others those of the largest
+        ``weights`` (as ``attend`` adds them up; ties: the earlier token), in their order.
+
+        In place by default: pages, ``weights`` and ``lengths`` of this cache are cut, and a
+        sequence's pages behind its first budget / page_size (rounded up) may be handed on.  With
+        ``to``, a cache of the same geometry whose table names other pages, the kept tokens go there
+        (its ``lengths`` are set, and ``weights_out``, fp32 [batch, kv_heads, at least budget], is
+        written), and this one stays as it is.  Returns int32 [batch, kv_heads, budget]: the
+        places that were kept, then -1."""
+        ldw = self._weights(weights, "weights", self.capacity)
+        budget, recent = int(budget), int(recent)
+        if to is None:
+            if weights_out is not None:
+                raise ValueError("weights_out without to: in place, weights are cut themselves")
+            to, weights_out = self, weights
+        elif weights_out is None:
+            raise ValueError("weights_out is needed with to")
+        elif weights_out.data_ptr() == weights.data_ptr() or to.k_pages.data_ptr() == self.v_pages.data_ptr():
+            raise ValueError("weights_out and to's pages must not be the source's")
+        if (to.batch, to.kv_heads, to.head_dim, to.page_size, to.dtype, to.device) != \
+                (self.batch, self.kv_heads, self.head_dim, self.page_size, self.dtype, self.device):
+            raise ValueError("to must have this cache's batch, heads, page size, type and device")
+        if not 0 < budget <= to.capacity or not 0 <= recent <= budget:
+            raise ValueError(f"budget {budget} (of {to.capacity}) and recent {recent} do not fit")
+        ldo = self._weights(weights_out, "weights_out", budget)
+        kept = torch.empty((self.batch, self.kv_heads, budget), dtype=torch.int32, device=self.device)
+        with _on(self.device):
+            st = _native.lib().otf_paged_evict(self._ref, to._ref, weights.data_ptr(), ldw, weights_out.data_ptr(),
+                                               ldo, budget, recent, kept.data_ptr(), to.lengths.data_ptr(),
+                                               _stream(self.device))
+        _native._check(st, "otf_paged_evict")
+        return kept
+
+    def advance(self, tokens: int = 1) -> None:
+        """lengths += tokens, where there is a sequence."""
+        self.lengths.add_(self.lengths.ge(0).to(torch.int32), alpha=int(tokens))
+
+    def _weights(self, t: torch.Tensor, name: str, least: int) -> int:
+        if t.device != self.device or t.dtype != torch.float32 or t.dim() != 3 or not t.is_contiguous() or \
+                t.shape[:2] != (self.batch, self.kv_heads) or t.shape[2] < least:
+            raise ValueError(f"{name} must be contiguous fp32 [{self.batch}, {self.kv_heads}, at least {least}] on "
+                             f"{self.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        return t.shape[2]
+
+    @staticmethod
+    def _flat(t: torch.Tensor, name: str) -> torch.Tensor:
+        """[batch, tokens, heads, dim] as rows, without a copy."""
+        if t.shape[0] > 1 and t.shape[1] > 1 and t.stride(0) != t.shape[1] * t.stride(1):
+            raise ValueError(f"{name} needs evenly strided rows, got strides {t.stride()}")
+        row = t.stride(1) if t.shape[1] > 1 else t.stride(0)
+        return t.as_strided((t.shape[0] * t.shape[1], t.shape[2], t.shape[3]), (row, t.stride(2), t.stride(3)))
+
+
+class _Same:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *a):
+        return False
+
+
+_SAME = _Same()
+
+
+def _on(dev: torch.device):
+    """The device made current, where it is not already."""
+    return _SAME if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _stream(dev: torch.device) -> int:
+    return torch.cuda.current_stream(dev).cuda_stream

@@ -1,0 +1,518 @@
+"""The paged key/value cache against its definitions in 64 bits: append with rotary positions,
+attention of one or a few new tokens, eviction, and all of them together."""
+import math
+
+import pytest
+import torch
+
+import paged_oracle as ref
+
+pytestmark = pytest.mark.gpu
+TYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+def make(dev, lengths, page, kv, dim, dtype, order="token", room=None, seed=0, spare=2, fill=float("nan")):
+    """A cache whose pages hold `fill` but for the tokens there are, under a shuffled table with
+    entries that name no page behind each sequence's room."""
+    from otf_llm.paged import PagedKVCache
+    g = torch.Generator().manual_seed(seed)
+    room = room or [max(n, 1) for n in lengths]
+    need = [-(-r // page) for r in room]
+    n_pages, most = sum(need) + spare, max(need) + 1
+    shape = (n_pages, page, kv, dim) if order == "token" else (n_pages, kv, page, dim)
+    pools = [torch.full(shape, fill, dtype=dtype) for _ in range(2)]
+    if order == "head":
+        pools = [p.transpose(1, 2) for p in pools]
+    ids = torch.randperm(n_pages, generator=g).tolist()
+    table = torch.full((len(lengths), most), -7, dtype=torch.int32)
+    for b, n in enumerate(need):
+        for j in range(n):
+            table[b, j] = ids.pop()
+    for b, n in enumerate(lengths):
+        for s in range(max(n, 0)):
+            for pool in pools:
+                pool[ref.place(table, page, b, s)] = torch.randn(kv, dim, generator=g).to(dtype)
+    on = [p.to(dev) if order == "token" else p.transpose(1, 2).contiguous().to(dev).transpose(1, 2) for p in pools]
+    cache = PagedKVCache(on[0], on[1], table.to(dev), torch.tensor(lengths, dtype=torch.int32, device=dev))
+    return cache, pools, table, g
+
+
+def flag():
+    from otf_llm import _native
+    torch.cuda.synchronize()
+    return _native.device_error(clear=True)
+
+
+def same(a, b):
+    """Equal bits, NaN included."""
+    return torch.equal(a.contiguous().view(torch.int16), b.contiguous().view(torch.int16))
+
+
+# ---- append -----------------------------------------------------------------------------------
+
+
+def check_append(cuda_dev, lengths, new, page, heads, kv, dim, rot, interleaved, scaling, dtype, order, uniform,
+                 positions=None, in_place=False, extra=0, seed=1):
+    from otf_llm.paged import Rotary
+    cache, pools, table, g = make(cuda_dev, lengths, page, kv, dim, dtype, order, seed=seed,
+                                  room=[max(n, 0) + t + 1 for n, t in zip(lengths, new)])
+    n = sum(new)
+    qkv = torch.randn(n + extra, heads + 2 * kv, dim, generator=g).to(dtype)
+    dq = qkv.to(cuda_dev)
+    q, k, v = dq.split([heads, kv, kv], dim=1)
+    rotary = Rotary(dim, rot_dim=rot, theta=10000.0, scaling=scaling, interleaved=interleaved, device=cuda_dev)
+    starts = None if uniform else torch.tensor([0] + new).cumsum(0).to(torch.int32).to(cuda_dev)
+    pos = None if positions is None else torch.tensor(positions, dtype=torch.int32, device=cuda_dev)
+    out = q if in_place else torch.full((n + extra, heads, dim), 7.0, dtype=dtype, device=cuda_dev)
+    got = cache.append(q, k, v, rotary, starts=starts, positions=pos, q_out=out)
+    assert got is out and flag() == 0
+    want_q = (qkv[:, :heads] if in_place else torch.full((n + extra, heads, dim), 7.0)).double()
+    tol_q = torch.zeros_like(want_q)
+    want_k, want_v = pools[0].clone(), pools[1].clone()
+    row, u = 0, torch.finfo(dtype).eps / 2
+    f, factor = rotary.frequencies, rotary.factor
+    k_got, v_got = cache.k_pages.cpu(), cache.v_pages.cpu()
+    for b, t in enumerate(new):
+        for j in range(t):
+            if lengths[b] >= 0:
+                s = lengths[b] + j
+                p = positions[row] if positions is not None else s
+                at = ref.place(table, page, b, s)
+                # c and s within 2^-21 (the angle's last bit of a turn, and sincospi's), two
+                # products and a sum in fp32, one rounding
+                for x, want, tol in ((qkv[row, :heads], want_q[row], tol_q[row]), (qkv[row, heads:heads + kv], None, None)):
+                    y = ref.rotate(x, p, f, factor, rot, interleaved)
+                    most = u * y.abs() + 2.0 ** -20 * factor * x.double().abs().amax() + torch.finfo(dtype).tiny * u
+                    if want is not None:
+                        want.copy_(y)
+                        tol.copy_(most)
+                        if rot < dim:
+                            tol[:, rot:] = 0
+                    else:
+                        if rot < dim:
+                            most[:, rot:] = 0
+                        assert bool(((k_got[at].double() - y).abs() <= most).all()), (b, j)
+                        want_k[at] = k_got[at]
+                want_v[at] = qkv[row, heads + kv:]
+            row += 1
+    assert bool(((out.cpu().double() - want_q).abs() <= tol_q).all())
+    assert same(k_got, want_k) and same(v_got, want_v)      # nothing else was written
+
+
+APPEND = [
+    ([0], [1], 16, 1, 1, 64, 64, False, "none"),
+    ([5, 0, -1, 33], [1, 1, 1, 1], 16, 8, 2, 128, 128, False, "none"),
+    ([0, 7, 100], [9, 0, 40], 20, 6, 2, 64, 32, True, "linear"),
+    ([3, 0], [17, 5], 1, 28, 4, 128, 24, False, "yarn"),
+    ([250, 1], [3, 30], 3, 5, 5, 128, 128, True, "llama3"),
+    ([15, 16], [2, 2], 8, 64, 8, 64, 0, False, "none"),
+    ([2, 9, -3, 40], [4, 6, 2, 3], 128, 16, 1, 128, 10, True, "none"),
+    ([1], [70], 64, 32, 32, 64, 6, False, "linear"),
+]
+SCALING = {"none": None, "linear": {"rope_type": "linear", "factor": 4.0},
+           "llama3": {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+                      "original_max_position_embeddings": 64},
+           "yarn": {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 128}}
+
+
+@pytest.mark.parametrize("dtype,order", [("fp16", "token"), ("bf16", "head")])
+@pytest.mark.parametrize("lengths,new,page,heads,kv,dim,rot,interleaved,scaling", APPEND)
+def test_append_matches_definition(lengths, new, page, heads, kv, dim, rot, interleaved, scaling, dtype, order, cuda_dev):
+    check_append(cuda_dev, lengths, new, page, heads, kv, dim, rot, interleaved, SCALING[scaling], TYPES[dtype], order,
+                 uniform=False, extra=2)
+
+
+def test_append_uniform_rows_in_place_and_given_positions(cuda_dev):
+    check_append(cuda_dev, [4, 0, 19], [3, 3, 3], 16, 8, 2, 128, 64, False, None, torch.float16, "token", uniform=True,
+                 in_place=True)
+    check_append(cuda_dev, [4, 0, 19], [1, 1, 1], 16, 8, 2, 64, 64, True, None, torch.bfloat16, "token", uniform=True,
+                 positions=[1000003, -5, 2 ** 31 - 1])
+
+
+def test_append_many_sequences(cuda_dev):
+    lengths = [(7 * b) % 23 for b in range(75)]
+    check_append(cuda_dev, lengths, [b % 3 for b in range(75)], 8, 2, 1, 64, 64, False, None, torch.float16, "token",
+                 uniform=False, extra=1)
+
+
+def test_append_keys_and_values_alone_and_nothing_turned(cuda_dev):
+    cache, pools, table, g = make(cuda_dev, [3, 0], 4, 2, 64, torch.float16, room=[8, 8])
+    k, v = torch.randn(4, 2, 64, generator=g).half(), torch.randn(4, 2, 64, generator=g).half()
+    assert cache.append(None, k.to(cuda_dev), v.to(cuda_dev)) is None
+    kp, vp = cache.k_pages.cpu(), cache.v_pages.cpu()
+    for row, (b, s) in enumerate(((0, 3), (0, 4), (1, 0), (1, 1))):
+        at = ref.place(table, 4, b, s)
+        assert torch.equal(kp[at], k[row]) and torch.equal(vp[at], v[row])
+    assert flag() == 0
+    assert cache.append(None, k[:0].to(cuda_dev), v[:0].to(cuda_dev)) is None
+
+
+def test_append_leaves_out_what_has_no_place(cuda_dev):
+    from otf_llm.paged import Rotary
+    cache, pools, table, g = make(cuda_dev, [2, 30, 5], 16, 2, 64, torch.float16, room=[16, 32, 16])
+    cache.page_table[2, 0] = 10 ** 6                       # a page outside the pool
+    q, k, v = (torch.randn(9, h, 64, generator=g).half().to(cuda_dev) for h in (4, 2, 2))
+    before = cache.k_pages.clone()
+    cap = cache.capacity
+    cache.lengths[1] = cap - 1                             # its second and third token do not fit
+    cache.page_table[1] = int(table[1, 0])
+    out = torch.full_like(q, 7.0)
+    cache.append(q, k, v, Rotary(64, device=cuda_dev), q_out=out)
+    assert flag() == 1
+    assert not bool((out[:4] == 7.0).any()) and bool((out[4:] == 7.0).all())
+    changed = (cache.k_pages.cpu().view(torch.int16) != before.cpu().view(torch.int16)).any(-1).any(-1)
+    assert changed.nonzero().tolist() == sorted([[int(table[0, 0]), 2], [int(table[0, 0]), 3], [int(table[0, 0]), 4],
+                                                 [int(table[1, 0]), (cap - 1) % 16]])
+
+
+# ---- attend -----------------------------------------------------------------------------------
+
+
+def check_attend(cuda_dev, totals, tokens, page, heads, kv, dim, dtype, order="token", weights=False, scale=None, seed=2,
+                 spread=1.0, prepare=None):
+    cache, pools, table, g = make(cuda_dev, totals, page, kv, dim, dtype, order, seed=seed)
+    if prepare is not None:
+        prepare(cache, pools, table)
+    cache.lengths.copy_(torch.tensor([n - tokens if n > 0 else -1 for n in totals], dtype=torch.int32))
+    q = (torch.randn(len(totals), tokens, heads, dim, generator=g) * spread).to(dtype)
+    out = torch.full((len(totals), tokens, heads, dim), 7.0, dtype=dtype, device=cuda_dev)
+    w0 = w = None
+    if weights:
+        w0 = torch.rand(len(totals), kv, cache.capacity, generator=g)
+        w = w0.to(cuda_dev)
+    got = cache.attend(q.to(cuda_dev), weights=w, out=out, scale=scale)
+    assert got is out and flag() == 0
+    out = out.cpu().double()
+    want_w = w0.double() if weights else None
+    tol_w = want_w * 2.0 ** -22 if weights else None
+    for b, n in enumerate(totals):
+        if n <= 0:
+            assert bool((out[b] == 7.0).all())
+            continue
+        k, v = (ref.gather(p, table, b, n) for p in pools)
+        for t in range(tokens):
+            m = n - tokens + t + 1
+            y, p, mass, size = ref.attend(q[b, t], k[:m], v[:m], dim ** -0.5 if scale is None else scale)
+            tol = ref.attend_tolerance(y, mass, size, dim, dtype)
+            off = (out[b, t] - y).abs() - tol
+            assert bool((off <= 0).all()), (b, t, float(off.max()), float((out[b, t] - y).abs().max()))
+            if weights:
+                rep = heads // kv
+                want_w[b, :, :m] += p.view(kv, rep, m).sum(1)
+                tol_w[b, :, :m] += (p * (size * 2.0 ** -14 + 2.0 ** -18)).view(kv, rep, m).sum(1) + 2.0 ** -40
+    if weights:
+        off = (w.cpu().double() - want_w).abs() - tol_w
+        assert bool((off <= 0).all()), float(off.max())
+    return cache, q
+
+
+ATTEND = [
+    ([1], 1, 16, 1, 1, 64),
+    ([1, 2, 15, 16, 17, 31, 32, 33], 1, 16, 8, 2, 128),
+    ([700], 1, 16, 32, 8, 128),
+    ([0, 300, 0, 5], 1, 20, 6, 2, 64),
+    ([129, 127, 128, 64, 65], 1, 1, 28, 4, 128),
+    ([513, 40], 1, 3, 48, 1, 64),
+    ([260, 7], 1, 128, 16, 16, 128),
+    ([5, 6, 64, 200], 5, 16, 8, 2, 128),
+    ([16, 17, 200], 16, 20, 4, 4, 64),
+    ([300, 8], 8, 16, 64, 8, 128),
+    ([2, 90], 2, 8, 40, 8, 64),
+    ([1100, 3], 3, 64, 71, 1, 128),
+]
+
+
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("dtype,order", [("fp16", "token"), ("bf16", "head")])
+@pytest.mark.parametrize("totals,tokens,page,heads,kv,dim", ATTEND)
+def test_attend_matches_definition(totals, tokens, page, heads, kv, dim, dtype, order, weights, cuda_dev):
+    check_attend(cuda_dev, totals, tokens, page, heads, kv, dim, TYPES[dtype], order, weights)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_attend_peaked_and_flat_scores(dtype, cuda_dev):
+    check_attend(cuda_dev, [500, 33], 1, 16, 8, 2, 128, TYPES[dtype], spread=30.0)      # one key takes nearly all
+    check_attend(cuda_dev, [3000], 2, 16, 8, 2, 64, TYPES[dtype], spread=0.0, weights=True)  # all equal
+    check_attend(cuda_dev, [90], 1, 16, 8, 2, 128, TYPES[dtype], scale=-0.3)
+
+
+def test_attend_many_sequences_and_long_ones(cuda_dev):
+    check_attend(cuda_dev, [1 + (37 * b) % 90 for b in range(150)], 1, 16, 4, 2, 64, torch.float16)
+    check_attend(cuda_dev, [9000, 1, 40], 1, 64, 4, 1, 64, torch.float16, weights=True)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_attend_rows_do_not_see_later_tokens(bad, dtype, cuda_dev):
+    """The newest tokens hold `bad`: rows before them stay finite and right, rows that see them do not."""
+    dt = TYPES[dtype]
+    totals, tokens, page, heads, kv, dim = [40, 5, 129], 4, 16, 6, 2, 64
+    cache, pools, table, g = make(cuda_dev, totals, page, kv, dim, dt)
+    for b, n in enumerate(totals):
+        for pool, on in zip(pools, (cache.k_pages, cache.v_pages)):
+            for s in (n - 2, n - 1):
+                pool[ref.place(table, page, b, s)] = bad
+                on[ref.place(table, page, b, s)] = bad
+    cache.lengths.sub_(tokens)
+    q = torch.randn(len(totals), tokens, heads, dim, generator=g).to(dt)
+    w = torch.zeros(len(totals), kv, cache.capacity, device=cuda_dev)
+    out = cache.attend(q.to(cuda_dev), weights=w).cpu().double()
+    for b, n in enumerate(totals):
+        k, v = (ref.gather(p, table, b, n) for p in pools)
+        for t in range(tokens - 2):
+            m = n - tokens + t + 1
+            y, p, mass, size = ref.attend(q[b, t], k[:m], v[:m], dim ** -0.5)
+            assert bool(((out[b, t] - y).abs() <= ref.attend_tolerance(y, mass, size, dim, dt)).all())
+        finite = bool(torch.isfinite(out[b, tokens - 1]).all())
+        assert not finite
+
+
+def test_attend_reads_bad_pages_as_zeros_and_raises_the_flag(cuda_dev):
+    cache, pools, table, g = make(cuda_dev, [40, 20], 16, 2, 64, torch.float16)
+    cache.page_table[0, 1] = -1
+    cache.lengths.sub_(1)
+    q = torch.randn(2, 4, 64, generator=g).half()
+    out = cache.attend(q.to(cuda_dev)).cpu().double()
+    assert flag() == 1
+    k, v = (ref.gather(p, torch.where(table < 0, 0, table), 0, 40) for p in pools)
+    k[16:32], v[16:32] = 0, 0
+    y, p, mass, size = ref.attend(q[0], k, v, 0.125)
+    assert bool(((out[0] - y).abs() <= ref.attend_tolerance(y, mass, size, 64, torch.float16)).all())
+    # a sequence longer than its table is left out whole, the other one is not
+    cache.page_table.copy_(table)
+    cache.lengths[0] = cache.capacity
+    out = torch.full_like(q, 7.0).to(cuda_dev)
+    cache.attend(q.to(cuda_dev), out=out)
+    assert flag() == 1
+    assert bool((out[0] == 7.0).all()) and not bool((out[1] == 7.0).any())
+
+
+def test_attend_strided_queries_and_outputs(cuda_dev):
+    cache, pools, table, g = make(cuda_dev, [33, 50], 16, 2, 64, torch.float16)
+    cache.lengths.sub_(3)
+    wide = torch.randn(2, 3, 12, 64, generator=g).half().to(cuda_dev)
+    q = wide[:, :, 2:10]
+    room = torch.zeros(2, 3, 16, 64, dtype=torch.float16, device=cuda_dev)
+    out = cache.attend(q, out=room[:, :, 4:12])
+    assert torch.equal(out, cache.attend(q.contiguous()))
+    assert not bool(room[:, :, :4].any()) and not bool(room[:, :, 12:].any())
+
+
+def test_offsets_beyond_32_bits(cuda_dev):
+    """A pool of over 2^31 values a side: the used pages lie at its end."""
+    from otf_llm.paged import PagedKVCache
+    n, page, kv, dim = 135000, 16, 8, 128
+    k, v = (torch.empty(n, page, kv, dim, dtype=torch.float16, device=cuda_dev) for _ in range(2))
+    table = torch.tensor([[n - 1, n - 4, n - 2]], dtype=torch.int32, device=cuda_dev)
+    cache = PagedKVCache(k, v, table, torch.zeros(1, dtype=torch.int32, device=cuda_dev))
+    g = torch.Generator().manual_seed(3)
+    kk, vv = torch.randn(40, kv, dim, generator=g).half(), torch.randn(40, kv, dim, generator=g).half()
+    cache.append(None, kk.to(cuda_dev), vv.to(cuda_dev))
+    q = torch.randn(1, 16, dim, generator=g).half()
+    cache.lengths.fill_(39)
+    out = cache.attend(q.to(cuda_dev)).cpu().double()
+    y, p, mass, size = ref.attend(q[0], kk.double(), vv.double(), dim ** -0.5)
+    assert bool(((out[0] - y).abs() <= ref.attend_tolerance(y, mass, size, dim, torch.float16)).all())
+    cache.lengths.fill_(40)
+    w = torch.rand(1, kv, cache.capacity, generator=g)
+    kept = cache.evict(w.to(cuda_dev), 20, 4)
+    for h in range(kv):
+        keep = ref.evict(w[0, h], 40, 20, 4)
+        assert kept[0, h].tolist() == keep
+        at = [ref.place(table, page, 0, s) for s in range(20)]
+        assert torch.equal(torch.stack([k[a][h] for a in at]).cpu(), kk[keep, h])
+    assert flag() == 0
+
+
+# ---- evict ------------------------------------------------------------------------------------
+
+
+def check_evict(cuda_dev, lengths, budget, recent, page, kv, dim, dtype, order, apart, weights=None, seed=4):
+    from otf_llm.paged import PagedKVCache
+    cache, pools, table, g = make(cuda_dev, lengths, page, kv, dim, dtype, order, seed=seed,
+                                  room=[max(n, budget) for n in lengths])
+    w = torch.rand(len(lengths), kv, cache.capacity, generator=g) ** 4
+    w[w < 0.05] = 0.0
+    if weights is not None:
+        weights(w)
+    dw = w.to(cuda_dev)
+    if apart:
+        to, to_pools, to_table, _ = make(cuda_dev, [0] * len(lengths), page, kv, dim, dtype, "token", seed=seed + 1,
+                                         room=[budget] * len(lengths))
+        wo = torch.full((len(lengths), kv, budget + 5), 9.0, device=cuda_dev)
+        kept = cache.evict(dw, budget, recent, to=to, weights_out=wo)
+        assert same(cache.k_pages.cpu(), pools[0]) and cache.lengths.tolist() == lengths
+        assert torch.equal(dw.cpu().view(torch.int32), w.view(torch.int32))
+    else:
+        to, to_pools, to_table, wo = cache, [p.clone() for p in pools], table, dw
+        kept = cache.evict(dw, budget, recent)
+    assert flag() == 0
+    kept = kept.cpu()
+    want = [p.clone() for p in to_pools]
+    want_w = torch.zeros_like(wo.cpu()) if apart else w.clone()
+    for b, n in enumerate(lengths):
+        for h in range(kv):
+            keep = ref.evict(w[b, h], max(n, 0), budget, recent)
+            assert kept[b, h].tolist() == keep + [-1] * (budget - len(keep)), (b, h)
+            if n < 0:
+                if apart:
+                    want_w[b, h] = 9.0
+                continue
+            if not apart and n > budget:
+                want_w[b, h, :n] = 0
+            for j, s in enumerate(keep):
+                for side in (0, 1):
+                    at, src = ref.place(to_table, page, b, j), ref.place(table, page, b, s)
+                    want[side][at[0], at[1], h] = pools[side][src[0], src[1], h]
+                want_w[b, h, j] = w[b, h, s]
+    assert to.lengths.tolist() == [min(n, budget) for n in lengths]
+    assert same(to.k_pages.cpu(), want[0]) and same(to.v_pages.cpu(), want[1])
+    assert torch.equal(wo.cpu().view(torch.int32), want_w.view(torch.int32))
+
+
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("lengths,budget,recent,page,kv,dim,dtype,order", [
+    ([1], 1, 0, 16, 1, 64, "fp16", "token"),
+    ([100, 30, 31, 29, 0, -1], 30, 8, 16, 2, 64, "fp16", "token"),
+    ([77, 200], 64, 64, 20, 3, 128, "bf16", "head"),
+    ([300], 7, 0, 1, 2, 128, "fp16", "head"),
+    ([1500, 40], 1100, 3, 128, 1, 64, "bf16", "token"),
+    ([260, 33], 32, 1, 3, 2, 64, "fp16", "token"),
+])
+def test_evict_matches_definition(lengths, budget, recent, page, kv, dim, dtype, order, apart, cuda_dev):
+    check_evict(cuda_dev, lengths, budget, recent, page, kv, dim, TYPES[dtype], order, apart)
+
+
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("kind", ["equal", "zero", "signs", "odd", "rising", "falling", "tiny"])
+def test_evict_ties_and_odd_weights(kind, apart, cuda_dev):
+    def weights(w):
+        n = w.shape[2]
+        if kind == "equal":
+            w.fill_(0.25)
+        elif kind == "zero":
+            w.zero_()
+            w[..., ::2] = -0.0
+        elif kind == "signs":
+            w.sub_(0.3)
+        elif kind == "odd":
+            w[..., 5::7] = float("nan")
+            w[..., 3::11] = float("inf")
+            w[..., 4::13] = -float("inf")
+        elif kind == "rising":
+            w.copy_(torch.arange(n).float().expand_as(w))
+        elif kind == "falling":
+            w.copy_(-torch.arange(n).float().expand_as(w))
+        else:
+            w.mul_(1e-42)                                   # subnormal
+    check_evict(cuda_dev, [150, 40, 64], 40, 5, 16, 2, 64, torch.float16, "token", apart, weights)
+
+
+def test_evict_long_sequence(cuda_dev):
+    check_evict(cuda_dev, [5000], 700, 100, 64, 2, 64, torch.float16, "token", False)
+
+
+# ---- graphs, streams, all together ----------------------------------------------------------------
+
+
+def test_two_captured_graphs_and_another_stream(cuda_dev):
+    """Two graphs of attend calls and an eager call on a third stream run at the same time and agree
+    with calls one after another."""
+    caches = [make(cuda_dev, [400 + 50 * i, 30, 777], 16, 2, 64, torch.float16, seed=10 + i) for i in range(3)]
+    qs = [torch.randn(3, 8, 64, generator=c[3]).half().to(cuda_dev) for c in caches]
+    want = []
+    for (c, *_), q in zip(caches, qs):
+        c.lengths.sub_(1)
+        w = torch.zeros(3, 2, c.capacity, device=cuda_dev)
+        want.append((c.attend(q, weights=w), w))
+    outs = [(torch.zeros_like(q), torch.zeros_like(w)) for q, (_, w) in zip(qs, want)]
+    torch.cuda.synchronize()
+    graphs = []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            for _ in range(4):
+                outs[i][1].zero_()
+                caches[i][0].attend(qs[i], weights=outs[i][1], out=outs[i][0])
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        with torch.cuda.stream(streams[2]):
+            outs[2][1].zero_()
+            caches[2][0].attend(qs[2], weights=outs[2][1], out=outs[2][0])
+    torch.cuda.synchronize()
+    for (o, w), (wo, ww) in zip(outs, want):
+        assert torch.equal(o, wo) and torch.equal(w, ww)
+    assert flag() == 0
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_prompt_decode_evict_verify_together(dtype, cuda_dev):
+    """Prompts enter the cache, tokens are decoded with weights kept, the cache is cut in place, decoding
+    goes on at the old positions, and drafted tokens are scored and verified, against the same
+    steps in 64 bits on what the cache holds."""
+    from otf_llm.paged import Rotary
+    from otf_llm.speculative import verify_drafts
+    dt, heads, kv, dim, page = TYPES[dtype], 8, 2, 64, 16
+    prompts = [50, 9, 31]
+    cache, pools, table, g = make(cuda_dev, [0, 0, 0], page, kv, dim, dt, room=[96] * 3, fill=0.0)
+    rotary = Rotary(dim, rot_dim=32, theta=10000.0, device=cuda_dev)
+    starts = torch.tensor([0, 50, 59, 90], dtype=torch.int32, device=cuda_dev)
+
+    def rows(n):
+        return [torch.randn(n, h, dim, generator=g).to(dt).to(cuda_dev) for h in (heads, kv, kv)]
+    q, k, v = rows(90)
+    cache.append(q, k, v, rotary, starts=starts)
+    cache.lengths.copy_(torch.tensor(prompts, dtype=torch.int32))
+    weights = torch.zeros(3, kv, cache.capacity, device=cuda_dev)
+    seen = list(prompts)
+    sums = torch.zeros(3, kv, cache.capacity, dtype=torch.float64)
+
+    def step(tokens):
+        q, k, v = rows(3 * tokens)
+        pos = torch.tensor([n + t for n in seen for t in range(tokens)], dtype=torch.int32, device=cuda_dev)
+        q = cache.append(q, k, v, rotary, positions=pos)
+        out = cache.attend(q.view(3, tokens, heads, dim), weights=weights)
+        kp, vp = cache.k_pages.cpu(), cache.v_pages.cpu()
+        for b, n in enumerate(cache.lengths.tolist()):
+            kk, vv = ref.gather(kp, table, b, n + tokens), ref.gather(vp, table, b, n + tokens)
+            for t in range(tokens):
+                m = n + t + 1
+                y, p, mass, size = ref.attend(q[b * tokens + t].cpu(), kk[:m], vv[:m], dim ** -0.5)
+                off = (out[b, t].cpu().double() - y).abs()
+                assert bool((off <= ref.attend_tolerance(y, mass, size, dim, dt)).all())
+                sums[b, :, :m] += p.view(kv, -1, m).sum(1)
+        cache.advance(tokens)
+        for b in range(3):
+            seen[b] += tokens
+        return out
+
+    for _ in range(4):
+        step(1)
+    assert float((weights.cpu().double() - sums).abs().max()) < 1e-4
+    kept = cache.evict(weights, 24, 6).cpu()
+    assert cache.lengths.tolist() == [24, 13, 24]
+    for b in (0, 2):
+        for h in range(kv):
+            keep = kept[b, h].tolist()
+            assert keep[-6:] == list(range(seen[b] - 6, seen[b])) and keep == sorted(set(keep))
+            sums[b, h, :24] = sums[b, h, keep].clone()
+            sums[b, h, 24:] = 0
+    assert float((weights.cpu().double() - sums).abs().max()) < 1e-4
+    step(1)
+    out = step(4)
+    vocab = 500
+    mat = torch.randn(heads * dim, vocab, generator=g).to(cuda_dev)
+    logits = out.float().reshape(3, 4, -1) @ mat
+    tokens = logits[:, :3].argmax(2)
+    tokens[1, 1] = (tokens[1, 1] + 1) % vocab
+    got, accepted = verify_drafts(logits, tokens, temperature=0.0)
+    assert accepted.tolist() == [3, 1, 3]
+    best = logits.argmax(2)
+    assert got[1].tolist() == [int(tokens[1, 0]), int(best[1, 1]), -1, -1]
+    assert got[0].tolist() == tokens[0].tolist() + [int(best[0, 3])]
+    assert flag() == 0

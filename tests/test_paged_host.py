@@ -1,0 +1,147 @@
+"""The paged cache and the verification of drafts without a GPU: frequencies, refusals."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+INVALID, UNSUPPORTED = 1, 2
+
+
+def test_frequencies_match_hf_definitions():
+    from transformers import LlamaConfig
+    from transformers.modeling_rope_utils import ROPE_INIT_FUNCTIONS
+
+    from otf_llm.paged import rope_frequencies
+    for scaling in ({"rope_type": "linear", "factor": 4.0},
+                    {"rope_type": "llama3", "factor": 32.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+                     "original_max_position_embeddings": 8192},
+                    {"rope_type": "yarn", "factor": 16.0, "original_max_position_embeddings": 4096}):
+        cfg = LlamaConfig(hidden_size=512, num_attention_heads=4, head_dim=128, max_position_embeddings=131072,
+                          rope_parameters=dict(scaling, rope_theta=500000.0))
+        want, factor = ROPE_INIT_FUNCTIONS[scaling["rope_type"]](cfg, "cpu")
+        got, mine = rope_frequencies(128, 500000.0, scaling)
+        assert got.dtype == torch.float64
+        # HF computes in fp32, powers and ramps among it
+        assert torch.allclose(got.float(), want, rtol=2e-5, atol=0) and math.isclose(mine, factor, rel_tol=1e-12)
+    plain, one = rope_frequencies(128, 500000.0)
+    assert one == 1.0 and torch.equal(plain, 500000.0 ** (-torch.arange(0, 128, 2, dtype=torch.float64) / 128))
+
+
+def test_frequencies_refuse_what_they_do_not_know():
+    from otf_llm.paged import rope_frequencies
+    for bad in ({"rope_type": "dynamic", "factor": 2.0}, {"rope_type": "linear"}, {"factor": 2.0},
+                {"rope_type": "linear", "factor": -1.0}, {"rope_type": "linear", "factor": 2.0, "mscale": 1.0},
+                {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 4.0, "high_freq_factor": 1.0,
+                 "original_max_position_embeddings": 8192}):
+        with pytest.raises(ValueError):
+            rope_frequencies(64, 10000.0, bad)
+    for rot, theta in ((63, 1e4), (-2, 1e4), (64, 0.0)):
+        with pytest.raises(ValueError):
+            rope_frequencies(rot, theta)
+    assert rope_frequencies(0)[0].numel() == 0
+
+
+def test_no_cpu_cache():
+    from otf_llm.paged import PagedKVCache
+    from otf_llm.speculative import verify_drafts
+    k = torch.zeros(2, 16, 1, 64, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        PagedKVCache(k, k.clone(), torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        verify_drafts(torch.zeros(1, 1, 8), torch.zeros(1, 0, dtype=torch.int64), temperature=0.0)
+
+
+FAKE = 1 << 20          # never read: every case is refused before anything runs
+
+
+def cache(**other):
+    from otf_llm import _native as N
+    c = N.PagedCache()
+    given = dict(k_pages=FAKE, v_pages=FAKE, page_stride=16 * 2 * 64, token_stride=128, head_stride=64, n_pages=10,
+                 page_size=16, kv_heads=2, head_dim=64, page_table=FAKE, ld_table=4, max_pages=4, lengths=FAKE, batch=3,
+                 dtype=0)
+    given.update(other)
+    for k, v in given.items():
+        setattr(c, k, v)
+    return c
+
+
+BAD_CACHES = [(dict(k_pages=None), INVALID), (dict(lengths=None), INVALID), (dict(page_table=None), INVALID),
+              (dict(dtype=2), UNSUPPORTED), (dict(head_dim=96), UNSUPPORTED), (dict(batch=0), INVALID),
+              (dict(batch=4097), UNSUPPORTED), (dict(page_size=0), INVALID), (dict(n_pages=0), INVALID),
+              (dict(kv_heads=0), INVALID), (dict(ld_table=3), INVALID), (dict(k_pages=FAKE + 8), INVALID),
+              (dict(token_stride=132), INVALID), (dict(head_stride=56), INVALID), (dict(page_stride=-8), INVALID),
+              (dict(max_pages=1 << 30, ld_table=1 << 30), UNSUPPORTED)]
+
+
+@pytest.mark.parametrize("other,status", BAD_CACHES)
+def test_abi_refuses_bad_caches(other, status):
+    from otf_llm import _native as N
+    L, ref = N.lib(), ctypes.byref(cache(**other))
+    good = ctypes.byref(cache())
+    assert L.otf_paged_append(ref, None, None, 0, None, 0, 0, FAKE, 128, FAKE, 128, None, None, 3, None) == status
+    assert L.otf_paged_attn(ref, FAKE, 256, 4, 1, 1.0, FAKE, 256, None, 0, FAKE, 1 << 40, None) == status
+    assert L.otf_paged_evict(ref, good, FAKE, 64, FAKE, 64, 8, 2, FAKE, FAKE, None) == status
+    assert L.otf_paged_evict(good, ref, FAKE, 64, FAKE, 64, 8, 2, FAKE, FAKE, None) == status
+
+
+def test_abi_refuses_bad_arguments():
+    from otf_llm import _native as N
+    L, c = N.lib(), ctypes.byref(cache())
+    rot = N.RotaryArgs()
+    rot.turns, rot.rot_dim, rot.factor = FAKE, 64, 1.0
+
+    def append(q=FAKE, ldq=256, qo=FAKE, ldqo=256, heads=4, k=FAKE, ldk=128, v=FAKE, ldv=128, starts=None, n=3, r=rot):
+        return L.otf_paged_append(c, ctypes.byref(r) if r is not None else None, q, ldq, qo, ldqo, heads, k, ldk, v, ldv,
+                                  starts, None, n, None)
+    for bad in (dict(n=4), dict(n=-1), dict(ldq=255), dict(ldq=128), dict(qo=None), dict(heads=0), dict(k=None),
+                dict(ldk=64), dict(v=FAKE + 2), dict(ldv=129)):
+        assert append(**bad) == INVALID, bad
+    assert append(n=0) == 0
+    for dims in (63, 66, -2):
+        r = N.RotaryArgs()
+        r.turns, r.rot_dim = FAKE, dims
+        assert append(r=r) == INVALID
+    r = N.RotaryArgs()
+    r.turns, r.rot_dim = None, 32
+    assert append(r=r) == INVALID
+
+    def attn(q=FAKE, ldq=256, heads=4, tokens=1, out=FAKE, ldo=256, w=None, ldw=0, ws=FAKE, n=1 << 40):
+        return L.otf_paged_attn(c, q, ldq, heads, tokens, 1.0, out, ldo, w, ldw, ws, n, None)
+    for bad in (dict(q=None), dict(out=None), dict(heads=3), dict(heads=0), dict(tokens=0), dict(ldq=248), dict(ldo=250),
+                dict(w=FAKE, ldw=63), dict(ws=None), dict(ws=FAKE + 16), dict(n=0)):
+        assert attn(**bad) == INVALID, bad
+    assert attn(tokens=17) == UNSUPPORTED
+    assert L.otf_paged_attn_workspace_bytes(3, 4, 2, 64, 1, 64, 0) > 0
+    for bad in ((0, 4, 2, 64, 1, 64, 0), (3, 5, 2, 64, 1, 64, 0), (3, 4, 2, 64, 17, 64, 0), (3, 4, 2, 64, 1, 0, 1)):
+        assert L.otf_paged_attn_workspace_bytes(*bad) == -1
+
+    def evict(to=None, w=FAKE, ldw=64, wo=FAKE, ldwo=64, budget=8, recent=2, kept=FAKE, out=FAKE):
+        return L.otf_paged_evict(c, ctypes.byref(to) if to is not None else c, w, ldw, wo, ldwo, budget, recent, kept,
+                                 out, None)
+    for bad in (dict(w=None), dict(wo=None), dict(kept=None), dict(out=None), dict(budget=0), dict(budget=65),
+                dict(recent=9), dict(recent=-1), dict(ldw=63), dict(ldwo=32), dict(wo=FAKE + 1024, ldwo=7),
+                dict(to=cache(head_dim=128, head_stride=128, token_stride=256)), dict(to=cache(dtype=1)),
+                dict(to=cache(page_size=8)), dict(to=cache(batch=2))):
+        assert evict(**bad) == INVALID, bad
+
+
+def test_abi_refuses_bad_verifications():
+    from otf_llm import _native as N
+    L = N.lib()
+    n = L.otf_verify_workspace_bytes(2, 3, 100)
+    assert n > 0
+    for bad in ((0, 3, 100), (2, -1, 100), (2, 33, 100), (2, 3, 0)):
+        assert L.otf_verify_workspace_bytes(*bad) == -1
+
+    def verify(t=FAKE, ts=400, ldt=100, d=None, ds=0, ldd=0, tok=FAKE, ldtok=3, u=FAKE, ldu=3, e=FAKE, lde=100, temp=1.0,
+               out=FAKE, acc=FAKE, batch=2, drafts=3, vocab=100, ws=FAKE, size=n):
+        return L.otf_verify_drafts(t, ts, ldt, d, ds, ldd, tok, ldtok, u, ldu, e, lde, None, temp, None, out, acc, batch,
+                                   drafts, vocab, ws, size, None)
+    for bad in (dict(t=None), dict(ldt=99), dict(d=FAKE, ldd=99), dict(tok=None), dict(ldtok=2), dict(u=None),
+                dict(ldu=2), dict(e=None), dict(lde=99), dict(temp=-1.0), dict(temp=float("nan")),
+                dict(temp=float("inf")), dict(temp=1e-30), dict(out=None), dict(acc=None), dict(batch=0),
+                dict(drafts=-1), dict(vocab=0), dict(ws=None), dict(ws=FAKE + 8), dict(size=n - 1)):
+        assert verify(**bad) == INVALID, bad
+    assert verify(drafts=33, ldtok=33, ldu=33) == UNSUPPORTED
