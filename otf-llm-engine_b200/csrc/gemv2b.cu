@@ -1925,6 +1925,7 @@ int mk_device_error(int clear);                 // decode_step.cu
 int attn_device_error(int clear);               // attention.cu
 int head_device_error(int clear);               // int8_ops.cu
 int paged_device_error(int clear);              // paged.cu
+int paged_attn_device_error(int clear);         // paged_attn.cu
 int verify_device_error(int clear);             // verify.cu
 
 static int num_sms() {
@@ -2522,7 +2523,8 @@ extern "C" OTF_API int otf_device_error(int clear) {
   const int a = attn_device_error(clear);
   const int h = head_device_error(clear);
   const int p = paged_device_error(clear);
+  const int c = paged_attn_device_error(clear);
   const int d = verify_device_error(clear);
-  if (w < 0 || x < 0 || a < 0 || h < 0 || p < 0 || d < 0) return -1;
-  return v | w | x | a | h | p | d;
+  if (w < 0 || x < 0 || a < 0 || h < 0 || p < 0 || c < 0 || d < 0) return -1;
+  return v | w | x | a | h | p | c | d;
 }

@@ -1,11 +1,9 @@
-// A key/value cache in pages: rotary positions and the write of new tokens (otf_paged_append),
-// attention of a few new tokens per sequence over the pages (otf_paged_attn), and the cut of
-// long sequences to a budget (otf_paged_evict).  Layout and rules: include/otf_b200.h.
-#include <cuda_bf16.h>
-
+// A key/value cache in pages: rotary positions and the write of new tokens (otf_paged_append) and
+// the cut of long sequences to a budget (otf_paged_evict); the attention that reads it is in
+// paged_attn.cu.  Layout and rules: include/otf_b200.h.
 #include <algorithm>
 
-#include "otf_common.cuh"
+#include "paged.cuh"
 
 namespace otf {
 
@@ -13,32 +11,9 @@ int set_cuda_error(cudaError_t e);  // capi.cu
 int check_device();                 // capi.cu
 int paged_device_error(int clear);  // read (and optionally clear) the flag below
 
-constexpr int kPagedMaxBatch = 4096;
-constexpr int kPagedMaxTokens = 16;  // new tokens of a sequence in one attention call
-
 // Set when a sequence does not fit its pages or names a page outside the pool.
 __device__ int g_paged_device_error;
 __device__ __forceinline__ void report_bad_page() { atomicExch(&g_paged_device_error, 1); }
-
-// otf_paged_cache as the kernels take it.
-struct PagedView {
-  uint16_t* k;
-  uint16_t* v;
-  int64_t page_stride, token_stride, head_stride;
-  const int* table;
-  int64_t ld_table;
-  const int* lengths;
-  int n_pages, page_size, capacity, kv_heads, batch;
-};
-
-template <bool BF>
-__device__ __forceinline__ float to_f(uint16_t v) {
-  return BF ? __bfloat162float(__ushort_as_bfloat16(v)) : h2f(v);
-}
-template <bool BF>
-__device__ __forceinline__ uint16_t from_f(float v) {
-  return BF ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : f2h(v);
-}
 
 // The sequence of row `row` under the row ranges starts[0..batch], found by a warp: as many
 // sequences end at or before it.  batch when the row lies behind the last sequence.
@@ -126,97 +101,6 @@ __global__ void __launch_bounds__(256) k_paged_append(PagedView c, const double*
     const int h = e / D, i = e - h * D;
     c.v[at + h * c.head_stride + i] = v[row * ldv + (int64_t)h * D + i];
   }
-}
-
-// One CTA per (query head, row): scores and the softmax over all cached tokens, warp by warp.
-template <bool BF, int D>
-__global__ void __launch_bounds__(256) k_paged_attn_plain(PagedView c, const uint16_t* q, int64_t ldq, int heads,
-                                                          int tokens, float scale, uint16_t* out, int64_t ldo,
-                                                          float* stats) {
-  constexpr int PL = D / 32, W = 8;
-  __shared__ float s_m[W], s_l[W], s_o[W][D];
-  pdl_trigger();
-  pdl_wait();
-  const int h = blockIdx.x, row = blockIdx.y, b = row / tokens, t = row - b * tokens;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int len = c.lengths[b];
-  if (len < 0) return;
-  if ((int64_t)len + tokens > c.capacity) {
-    if (threadIdx.x == 0) report_bad_page();
-    return;
-  }
-  const int g = h / (heads / c.kv_heads);
-  float qv[PL], o[PL], m = -INFINITY, l = 0.0f;
-#pragma unroll
-  for (int i = 0; i < PL; ++i) {
-    qv[i] = to_f<BF>(q[row * ldq + (int64_t)h * D + lane * PL + i]);
-    o[i] = 0.0f;
-  }
-  for (int s = warp; s <= len + t; s += W) {
-    const int page = c.table[b * c.ld_table + s / c.page_size];
-    const bool ok = page >= 0 && page < c.n_pages;
-    if (!ok && lane == 0) report_bad_page();
-    const int64_t at = (ok ? page : 0) * c.page_stride + (s % c.page_size) * c.token_stride + g * c.head_stride + lane * PL;
-    float d = 0.0f, vv[PL];
-#pragma unroll
-    for (int i = 0; i < PL; ++i) {
-      d = fmaf(qv[i], ok ? to_f<BF>(c.k[at + i]) : 0.0f, d);
-      vv[i] = ok ? to_f<BF>(c.v[at + i]) : 0.0f;
-    }
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
-    d *= scale;
-    const float mn = fmaxf(m, d), corr = m == -INFINITY ? 0.0f : expf(m - mn);
-    const float p = d == -INFINITY ? 0.0f : expf(d - mn);  // a NaN stays one
-    l = l * corr + p;
-#pragma unroll
-    for (int i = 0; i < PL; ++i) o[i] = o[i] * corr + p * vv[i];
-    m = mn;
-  }
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < PL; ++i) s_o[warp][lane * PL + i] = o[i];
-  __syncthreads();
-  float mm = -INFINITY, ll = 0.0f;
-  for (int w = 0; w < W; ++w) mm = fmaxf(mm, s_m[w]);
-  for (int w = 0; w < W; ++w) ll += s_l[w] == 0.0f ? 0.0f : s_l[w] * expf(s_m[w] - mm);
-  for (int i = threadIdx.x; i < D; i += blockDim.x) {
-    float a = 0.0f;
-    for (int w = 0; w < W; ++w) a += s_l[w] == 0.0f ? 0.0f : s_o[w][i] * expf(s_m[w] - mm);
-    out[row * ldo + (int64_t)h * D + i] = from_f<BF>(a / ll);
-  }
-  if (threadIdx.x == 0 && stats) stats[(int64_t)row * heads + h] = mm + logf(ll);
-}
-
-// weights[b, g, s] += sum over the rows and query heads of exp(score - log-sum): one thread per token.
-template <bool BF, int D>
-__global__ void __launch_bounds__(256) k_paged_weights_plain(PagedView c, const uint16_t* q, int64_t ldq, int heads,
-                                                             int tokens, float scale, const float* stats,
-                                                             float* weights, int64_t ldw) {
-  pdl_trigger();
-  pdl_wait();
-  const int g = blockIdx.y, b = blockIdx.z;
-  const int s = blockIdx.x * blockDim.x + threadIdx.x;
-  const int len = c.lengths[b];
-  if (len < 0 || (int64_t)len + tokens > c.capacity || s >= len + tokens) return;
-  const int page = c.table[b * c.ld_table + s / c.page_size];
-  const bool ok = page >= 0 && page < c.n_pages;
-  const uint16_t* kr = c.k + (ok ? page : 0) * c.page_stride + (s % c.page_size) * c.token_stride + g * c.head_stride;
-  const int rep = heads / c.kv_heads;
-  float sum = 0.0f;
-  for (int t = max(0, s - len); t < tokens; ++t) {
-    const int row = b * tokens + t;
-    for (int r = 0; r < rep; ++r) {
-      const int h = g * rep + r;
-      float d = 0.0f;
-      for (int i = 0; i < D; ++i) d = fmaf(to_f<BF>(q[row * ldq + (int64_t)h * D + i]), ok ? to_f<BF>(kr[i]) : 0.0f, d);
-      sum += expf(d * scale - stats[(int64_t)row * heads + h]);
-    }
-  }
-  weights[((int64_t)b * c.kv_heads + g) * ldw + s] += sum;
 }
 
 // ---- eviction -------------------------------------------------------------------------------
@@ -377,32 +261,6 @@ __global__ void __launch_bounds__(256) k_evict_move(PagedView from, PagedView to
   }
 }
 
-// ---- host -----------------------------------------------------------------------------------
-
-static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
-// The view of a cache, or why there is none.
-static int view_of(const otf_paged_cache* c, PagedView& v) {
-  if (!c || !c->k_pages || !c->v_pages || !c->page_table || !c->lengths) return OTF_ERR_INVALID;
-  if (c->dtype != OTF_DTYPE_F16 && c->dtype != OTF_DTYPE_BF16) return OTF_ERR_UNSUPPORTED;
-  if (c->head_dim != 64 && c->head_dim != 128) return OTF_ERR_UNSUPPORTED;
-  if (c->batch <= 0 || c->kv_heads <= 0 || c->page_size <= 0 || c->max_pages <= 0 || c->n_pages <= 0)
-    return OTF_ERR_INVALID;
-  if (c->batch > kPagedMaxBatch || c->kv_heads > 1024 || c->n_pages > INT32_MAX || c->page_size > INT32_MAX ||
-      c->max_pages > INT32_MAX || c->max_pages * c->page_size > INT32_MAX)
-    return OTF_ERR_UNSUPPORTED;
-  if (c->ld_table < c->max_pages) return OTF_ERR_INVALID;
-  if (!aligned16(c->k_pages) || !aligned16(c->v_pages) || c->page_stride % 8 || c->token_stride % 8 ||
-      c->head_stride % 8 || c->page_stride < 0 || c->token_stride < c->head_dim || c->head_stride < c->head_dim)
-    return OTF_ERR_INVALID;
-  v = PagedView{static_cast<uint16_t*>(c->k_pages), static_cast<uint16_t*>(c->v_pages), c->page_stride,
-                c->token_stride, c->head_stride, c->page_table, c->ld_table, c->lengths, (int)c->n_pages,
-                (int)c->page_size, (int)(c->max_pages * c->page_size), (int)c->kv_heads, (int)c->batch};
-  return OTF_OK;
-}
-
-static bool rows16(const void* p, int64_t ld, int64_t cols) { return p && aligned16(p) && ld % 8 == 0 && ld >= cols; }
-
 }  // namespace otf
 
 using otf::check_device;
@@ -448,50 +306,6 @@ extern "C" OTF_API int otf_paged_append(const otf_paged_cache* cache, const otf_
       rot, rot ? rotary->factor : 1.0f, rot ? (int)rotary->interleaved : 0, static_cast<const uint16_t*>(q), ldq,
       static_cast<uint16_t*>(q_out), ldqo, (int)heads, static_cast<const uint16_t*>(k), ldk,
       static_cast<const uint16_t*>(v), ldv, starts, positions, (int)(n / c.batch), (int)D));
-}
-
-extern "C" OTF_API int64_t otf_paged_attn_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads,
-                                                          int64_t head_dim, int64_t tokens, int64_t max_tokens,
-                                                          int with_weights) {
-  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || head_dim <= 0 || tokens <= 0 ||
-      tokens > otf::kPagedMaxTokens || max_tokens <= 0)
-    return -1;
-  (void)with_weights;
-  return otf::align_up(batch * tokens * heads * 4, 256);
-}
-
-extern "C" OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* q, int64_t ldq, int64_t heads,
-                                      int64_t tokens, float scale, void* out, int64_t ldo, float* weights,
-                                      int64_t ldw, void* workspace, int64_t workspace_bytes, void* stream) {
-  otf::PagedView c;
-  int st = otf::view_of(cache, c);
-  if (st != OTF_OK) return st;
-  const int64_t D = cache->head_dim;
-  if (heads <= 0 || heads > 65535 || heads % c.kv_heads || tokens <= 0) return OTF_ERR_INVALID;
-  if (tokens > otf::kPagedMaxTokens) return OTF_ERR_UNSUPPORTED;
-  if (!otf::rows16(q, ldq, heads * D) || !otf::rows16(out, ldo, heads * D)) return OTF_ERR_INVALID;
-  if (weights && ldw < c.capacity) return OTF_ERR_INVALID;
-  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
-      workspace_bytes < otf_paged_attn_workspace_bytes(c.batch, heads, c.kv_heads, D, tokens, c.capacity, !!weights))
-    return OTF_ERR_INVALID;
-  st = check_device();
-  if (st != OTF_OK) return st;
-  const bool bf = cache->dtype == OTF_DTYPE_BF16;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  float* stats = static_cast<float*>(workspace);
-  const dim3 grid((unsigned)heads, (unsigned)(c.batch * tokens));
-  const auto* qq = static_cast<const uint16_t*>(q);
-  auto* oo = static_cast<uint16_t*>(out);
-  auto* ka = D == 128 ? (bf ? otf::k_paged_attn_plain<true, 128> : otf::k_paged_attn_plain<false, 128>)
-                      : (bf ? otf::k_paged_attn_plain<true, 64> : otf::k_paged_attn_plain<false, 64>);
-  cudaError_t e = otf::launch_pdl(ka, grid, dim3(256), 0, s, 1u, c, qq, ldq, (int)heads, (int)tokens, scale, oo, ldo,
-                                  stats);
-  if (e != cudaSuccess || !weights) return set_cuda_error(e);
-  auto* kw = D == 128 ? (bf ? otf::k_paged_weights_plain<true, 128> : otf::k_paged_weights_plain<false, 128>)
-                      : (bf ? otf::k_paged_weights_plain<true, 64> : otf::k_paged_weights_plain<false, 64>);
-  return set_cuda_error(otf::launch_pdl(kw, dim3((unsigned)((c.capacity + 255) / 256), (unsigned)c.kv_heads, (unsigned)c.batch),
-                                        dim3(256), 0, s, 1u, c, qq, ldq, (int)heads, (int)tokens, scale,
-                                        (const float*)stats, weights, ldw));
 }
 
 extern "C" OTF_API int otf_paged_evict(const otf_paged_cache* from, const otf_paged_cache* to, const float* weights,

@@ -1,0 +1,670 @@
+// Attention of a few new tokens per sequence over a key/value cache in pages (otf_paged_attn).
+//
+// Mathematics.  For a query row r of a KV head, with s_j = scale log2(e) q_r k_j, one pass over the
+// cached tokens keeps the running maximum m, l = sum_j 2^(s_j - m) and o = sum_j 2^(s_j - m) v_j,
+// rescaled when m grows; out = o / l.  Parts (m, l, o) of disjoint token ranges join as
+// M = max m, L = sum l 2^(m - M), O = sum o 2^(m - M).
+//
+// Bound: the keys and values are read once, 2 x head_dim x 2 bytes per token and KV head; the
+// products are 4 x head_dim x rows flops on them, below the matrix pipe's rate up to some tens
+// of rows.  So the aim is to keep enough loads in flight on every SM.
+//
+// Split.  An item is a (sequence, KV head, block of 16 or 32 query rows); its tokens that every
+// row sees (0 .. length) are cut into chunks, and all items' chunks, in order, are dealt out evenly
+// to a fixed grid in contiguous runs, whatever the lengths are: a run may cross items, and an
+// item may be shared by several CTAs, which then leave parts that a second kernel joins in order.
+// Neither launch depends on lengths (they are read on the device), so a step can be captured.
+//
+// Inside a CTA each warp is on its own: it takes 16 (head_dim 64: 32) tokens of every chunk through its
+// own ring of shared-memory stages, filled by 16-byte asynchronous copies some chunks ahead and
+// across items, and runs q k and p v on m16n8k16 matrix instructions, the row block's queries
+// held in registers.  The warps meet only at an item's end.
+//
+// The tokens - 1 newest keys, which not every row sees, are added row by row at the item's end on
+// plain arithmetic, so that the loop needs no causal mask and a row cannot be reached by what
+// later tokens hold.
+#include <algorithm>
+#include <map>
+#include <mutex>
+#include <utility>
+
+#include "paged.cuh"
+
+namespace otf {
+
+int set_cuda_error(cudaError_t e);       // capi.cu
+int check_device();                      // capi.cu
+int paged_attn_device_error(int clear);  // read (and optionally clear) the flag below
+
+constexpr int kPaWarps = 4;
+constexpr int kPaThreads = kPaWarps * 32;
+constexpr int kPaStages = 3;
+constexpr int kPaStage = 8192;  // bytes of a warp's stage: its tokens' keys, then values
+constexpr int kPaGrid = 296;    // two CTAs on each of 148 SMs
+
+// Set when a sequence does not fit its pages or names a page outside the pool.
+__device__ int g_paged_attn_device_error;
+__device__ __forceinline__ void report_bad_attn_page() { atomicExch(&g_paged_attn_device_error, 1); }
+
+// Division of numbers below 2^31 by a fixed one.
+struct FastDiv {
+  uint32_t mul, shift, d;
+};
+static FastDiv fast_div(uint32_t d) {
+  uint32_t l = 0;
+  while ((1ull << l) < d) ++l;
+  return FastDiv{(uint32_t)(((1ull << 32) * ((1ull << l) - d)) / d + 1), l, d};
+}
+__device__ __forceinline__ uint32_t operator/(uint32_t n, const FastDiv& f) {
+  return (__umulhi(f.mul, n) + n) >> f.shift;
+}
+
+struct AttnArgs {
+  PagedView c;
+  FastDiv page;
+  const uint16_t* q;
+  int64_t ldq;
+  uint16_t* out;
+  int64_t ldo;
+  float scale;         // with log2(e)
+  int rep, tokens;     // query heads per KV head, new tokens per sequence
+  int rows, blocks;    // rep x tokens rows in so many row blocks
+  int64_t* prefix;     // [batch + 1] chunks before each sequence
+  float* part;         // [2 x grid][rows of a block][head_dim + 2]
+  float* lse;          // [batch, kv_heads, rows] log2 of the sum, when weights are wanted
+  float* scores;       // [batch, kv_heads, rows, ld_scores] likewise
+  int64_t ld_scores;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <bool BF>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (BF)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr) : "memory");
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  return (uint32_t)from_f<BF>(lo) | ((uint32_t)from_f<BF>(hi) << 16);
+}
+
+// 2^8 on fp16 probabilities: the largest is 256, and what lies 2^-32 below it still counts.
+template <bool BF>
+constexpr float kProbShift = BF ? 0.0f : 8.0f;
+
+// Where a walk over the chunks stands: sequence, item (KV head and row block) and chunk.
+struct Walk {
+  int b, item, chunk, chunks;
+};
+
+template <int D>
+struct Tile {
+  static constexpr int keys = D == 128 ? 16 : 32;   // of a warp's stage
+  static constexpr int chunk = keys * kPaWarps;
+  static constexpr int pieces = D / 8;              // 16-byte pieces of a row
+  static constexpr int rows = 32 / pieces;          // rows that a warp's copy instruction covers
+};
+
+template <int D>
+__device__ __forceinline__ int chunks_of(int len) {
+  return (len + 1 + Tile<D>::chunk - 1) / Tile<D>::chunk;  // none when len is -1
+}
+
+template <bool BF, int D, int MT>
+__global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
+  constexpr int KT = Tile<D>::keys, CH = Tile<D>::chunk, NS = kPaStages, PL = D / 32, RB = 16 * MT;
+  extern __shared__ __align__(128) unsigned char smem[];
+  float* s_m = reinterpret_cast<float*>(smem + kPaWarps * NS * kPaStage);
+  float* s_l = s_m + kPaWarps * RB;
+  int* s_len = reinterpret_cast<int*>(s_l + kPaWarps * RB);
+  __shared__ int64_t s_sum[kPaWarps];
+  __shared__ Walk s_walk;
+  pdl_trigger();
+  pdl_wait();
+  const PagedView& c = a.c;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int items = c.kv_heads * a.blocks;
+
+  // the lengths, and this CTA's run of chunks [u0, u1) of all items' chunks
+  int64_t sum = 0;
+  for (int b = tid; b < c.batch; b += kPaThreads) {
+    int len = c.lengths[b];
+    if (len >= 0 && (int64_t)len + a.tokens > c.capacity) {
+      if (blockIdx.x == 0) report_bad_attn_page();
+      len = -1;
+    }
+    s_len[b] = max(len, -1);
+    sum += (int64_t)chunks_of<D>(max(len, -1)) * items;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) s_sum[warp] = sum;
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < kPaWarps; ++w) total += s_sum[w];
+  const int64_t ctas = min((int64_t)kPaGrid, total);  // every one of them has a chunk at least
+  const int64_t u0 = blockIdx.x < ctas ? blockIdx.x * total / ctas : total;
+  const int64_t u1 = blockIdx.x < ctas ? (blockIdx.x + 1) * total / ctas : total;
+  if (warp == 0 && (u0 < u1 || blockIdx.x == 0)) {
+    int64_t base = 0;
+    for (int b0 = 0; b0 < c.batch; b0 += 32) {
+      const int b = b0 + lane;
+      const int n = b < c.batch ? chunks_of<D>(s_len[b]) : 0;
+      const int64_t mine = (int64_t)n * items;
+      int64_t inc = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += x;
+      }
+      const int64_t first = base + inc - mine;
+      if (u0 >= first && u0 < first + mine) {
+        const int at = (int)(u0 - first);
+        s_walk = Walk{b, at / n, at % n, n};
+      }
+      if (blockIdx.x == 0 && b < c.batch) {
+        a.prefix[b] = first;
+        if (b == c.batch - 1) a.prefix[c.batch] = total;
+      }
+      base += __shfl_sync(0xffffffffu, inc, 31);
+    }
+  }
+  __syncthreads();
+  if (u0 >= u1) return;
+
+  auto advance = [&](Walk& w) {
+    if (++w.chunk < w.chunks) return;
+    w.chunk = 0;
+    if (++w.item < items) return;
+    w.item = 0;
+    do ++w.b;
+    while (w.b < c.batch && s_len[w.b] < 0);
+    w.chunks = w.b < c.batch ? chunks_of<D>(s_len[w.b]) : 1;
+  };
+
+  // this lane's token of the walk's chunk: the offset of its page row (its head's rows lie
+  // head_stride apart), -1 where there is none
+  auto token_at = [&](const Walk& w, bool there) -> int64_t {
+    const int key = w.chunk * CH + warp * KT + lane;
+    if (!there || lane >= KT || key > s_len[w.b]) return -1;
+    const uint32_t at = (uint32_t)key / a.page;
+    const int page = c.table[w.b * c.ld_table + at];
+    if (page < 0 || page >= c.n_pages) {
+      report_bad_attn_page();
+      return -1;
+    }
+    return page * c.page_stride + (int64_t)(key - (int)(at * a.page.d)) * c.token_stride;
+  };
+  const uint32_t ring = smem_u32(smem) + warp * NS * kPaStage;
+  const int my_row = lane / Tile<D>::pieces, my_piece = lane % Tile<D>::pieces;
+  auto fetch = [&](const Walk& w, int64_t offset, int slot) {
+    const int64_t head = (int64_t)(w.item / a.blocks) * c.head_stride + my_piece * 8;
+    const uint32_t dst = ring + slot * kPaStage;
+#pragma unroll
+    for (int i = 0; i < KT / Tile<D>::rows; ++i) {
+      const int r = i * Tile<D>::rows + my_row;
+      const int64_t off = __shfl_sync(0xffffffffu, offset, r);
+      const bool ok = off >= 0;
+      const int64_t at = ok ? off + head : 0;
+      const uint32_t to = dst + r * (D * 2) + ((my_piece ^ (r & 7)) << 4);
+      cp_async16(to, c.k + at, ok ? 16u : 0u);
+      cp_async16(to + KT * D * 2, c.v + at, ok ? 16u : 0u);
+    }
+  };
+
+  Walk get = s_walk, load = s_walk;
+  int64_t u_load = u0;
+  int64_t next = token_at(load, true);
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i) {
+    if (u_load < u1) {
+      fetch(load, next, i);
+      advance(load);
+      next = token_at(load, ++u_load < u1);
+    }
+    cp_async_commit();
+  }
+
+  uint32_t qf[MT][D / 16][4];
+  float o[MT][D / 8][4], m[MT][2], l[MT][2];
+  int64_t begin = u0 - get.chunk;  // this item's first chunk
+  bool fresh = true;
+  int slot = 0;
+  for (int64_t u = u0; u < u1; ++u) {
+    const int g = get.item / a.blocks, rb = get.item - g * a.blocks;
+    const int len = s_len[get.b];
+    if (fresh) {
+      fresh = false;
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = rb * RB + t * 16 + h * 8 + (lane >> 2);
+          const int tok = r / a.rep;
+          const uint32_t* x = reinterpret_cast<const uint32_t*>(a.q + ((int64_t)get.b * a.tokens + tok) * a.ldq +
+                                                                (int64_t)(g * a.rep + r - tok * a.rep) * D) + (lane & 3);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            qf[t][k][h] = r < a.rows ? x[k * 8] : 0u;
+            qf[t][k][h + 2] = r < a.rows ? x[k * 8 + 4] : 0u;
+          }
+          m[t][h] = -INFINITY;
+          l[t][h] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[t][j][i] = 0.0f;
+      }
+    }
+    cp_async_wait<NS - 2>();
+    __syncwarp();
+    {  // the stage read one round ago takes the chunk NS - 1 ahead
+      if (u_load < u1) {
+        fetch(load, next, slot == 0 ? NS - 1 : slot - 1);
+        advance(load);
+        next = token_at(load, ++u_load < u1);
+      }
+      cp_async_commit();
+    }
+    const int key0 = get.chunk * CH + warp * KT;
+    if (key0 <= len) {
+      const uint32_t kb = ring + slot * kPaStage, vb = kb + KT * D * 2;
+      float s[MT][KT / 8][4];
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int n = 0; n < KT / 8; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[t][n][i] = 0.0f;
+      const int lrow = lane & 7, lmat = lane >> 3;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+        for (int n = 0; n < KT / 16; ++n) {
+          const int row = n * 16 + (lmat >> 1) * 8 + lrow;
+          uint32_t b0, b1, b2, b3;
+          ldmatrix_x4(kb + row * (D * 2) + (((k * 2 + (lmat & 1)) ^ lrow) << 4), b0, b1, b2, b3);
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            mma16816<BF>(s[t][2 * n], qf[t][k], b0, b1);
+            mma16816<BF>(s[t][2 * n + 1], qf[t][k], b2, b3);
+          }
+        }
+      const bool edge = key0 + KT > len + 1;
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        float mx[2] = {m[t][0], m[t][1]};
+#pragma unroll
+        for (int n = 0; n < KT / 8; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float x = s[t][n][i] * a.scale;
+            if (edge && key0 + n * 8 + (lane & 3) * 2 + (i & 1) > len) x = -INFINITY;
+            s[t][n][i] = x;
+            mx[i >> 1] = fmaxf(mx[i >> 1], x);
+          }
+        if (a.scores) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = rb * RB + t * 16 + h * 8 + (lane >> 2);
+            if (r < a.rows) {
+              float* to = a.scores + (((int64_t)get.b * c.kv_heads + g) * a.rows + r) * a.ld_scores + key0 + (lane & 3) * 2;
+#pragma unroll
+              for (int n = 0; n < KT / 8; ++n)
+                if (key0 + n * 8 <= len)  // ld_scores covers whole groups of 8
+                  *reinterpret_cast<float2*>(to + n * 8) = make_float2(s[t][n][2 * h], s[t][n][2 * h + 1]);
+            }
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+        }
+        if (__any_sync(0xffffffffu, mx[0] != m[t][0] || mx[1] != m[t][1])) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float f = m[t][h] == -INFINITY ? 0.0f : ex2(m[t][h] - mx[h]);
+            l[t][h] *= f;
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j) {
+              o[t][j][2 * h] *= f;
+              o[t][j][2 * h + 1] *= f;
+            }
+            m[t][h] = mx[h];
+          }
+        }
+        const float z[2] = {kProbShift<BF> - (m[t][0] == -INFINITY ? 0.0f : m[t][0]),
+                            kProbShift<BF> - (m[t][1] == -INFINITY ? 0.0f : m[t][1])};
+#pragma unroll
+        for (int n = 0; n < KT / 8; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[t][n][i] = ex2(s[t][n][i] + z[i >> 1]);
+            l[t][i >> 1] += s[t][n][i];
+          }
+      }
+      uint32_t p[MT][KT / 16][4];
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int n = 0; n < KT / 16; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            p[t][n][i] = pack2<BF>(s[t][2 * n + (i >> 1)][2 * (i & 1)], s[t][2 * n + (i >> 1)][2 * (i & 1) + 1]);
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+        for (int n = 0; n < KT / 16; ++n) {
+          const int row = n * 16 + (lmat & 1) * 8 + lrow;
+          uint32_t b0, b1, b2, b3;
+          ldmatrix_x4_trans(vb + row * (D * 2) + (((j * 2 + (lmat >> 1)) ^ lrow) << 4), b0, b1, b2, b3);
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            mma16816<BF>(o[t][2 * j], p[t][n], b0, b1);
+            mma16816<BF>(o[t][2 * j + 1], p[t][n], b2, b3);
+          }
+        }
+    }
+    const bool last = get.chunk + 1 == get.chunks;
+    if (last || u + 1 == u1) {
+      // The item's end in this run: the warps' parts join, through the stage just read.
+      const bool whole = last && begin >= u0;
+      float* mine = reinterpret_cast<float*>(smem + warp * NS * kPaStage + slot * kPaStage);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x = l[t][h];
+          x += __shfl_xor_sync(0xffffffffu, x, 1);
+          x += __shfl_xor_sync(0xffffffffu, x, 2);
+          const int r = h * 8 + (lane >> 2);
+          if ((lane & 3) == 0) {
+            s_m[warp * RB + r] = m[t][h];
+            s_l[warp * RB + r] = x;
+          }
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j)  // columns turned by the row, against bank conflicts
+            *reinterpret_cast<float2*>(mine + r * D + ((j * 8 + (lane & 3) * 2) ^ ((r & 3) << 3))) =
+                make_float2(o[t][j][2 * h], o[t][j][2 * h + 1]);
+        }
+        __syncthreads();
+        for (int r = warp; r < 16; r += kPaWarps) {
+          const int rr = rb * RB + t * 16 + r;
+          if (rr >= a.rows) break;
+          float M = -INFINITY, L = 0.0f, acc[PL];
+#pragma unroll
+          for (int i = 0; i < PL; ++i) acc[i] = 0.0f;
+#pragma unroll
+          for (int w = 0; w < kPaWarps; ++w) M = fmaxf(M, s_m[w * RB + r]);
+#pragma unroll
+          for (int w = 0; w < kPaWarps; ++w) {
+            const float lw = s_l[w * RB + r];
+            const float f = lw == 0.0f ? 0.0f : ex2(s_m[w * RB + r] - M);
+            const float* x = reinterpret_cast<const float*>(smem + w * NS * kPaStage + slot * kPaStage) + r * D +
+                             ((lane * PL) ^ ((r & 3) << 3));
+            if (lw != 0.0f) {
+              L = fmaf(lw, f, L);
+#pragma unroll
+              for (int i = 0; i < PL; ++i) acc[i] = fmaf(x[i], f, acc[i]);
+            }
+          }
+          const int tok = rr / a.rep, head = g * a.rep + rr - tok * a.rep;
+          const int64_t row = (int64_t)get.b * a.tokens + tok;
+          if (last && a.tokens > 1) {  // the newest tokens, as far as this row sees them
+            float qv[PL];
+#pragma unroll
+            for (int i = 0; i < PL; ++i) qv[i] = to_f<BF>(a.q[row * a.ldq + (int64_t)head * D + lane * PL + i]);
+            float* sc = a.scores ? a.scores + (((int64_t)get.b * c.kv_heads + g) * a.rows + rr) * a.ld_scores : nullptr;
+            for (int key = len + 1; key < len + a.tokens; ++key) {
+              if (key > len + tok) {
+                if (sc && lane == 0) sc[key] = -INFINITY;
+                continue;
+              }
+              const uint32_t at = (uint32_t)key / a.page;
+              const int page = c.table[get.b * c.ld_table + at];
+              const bool ok = page >= 0 && page < c.n_pages;
+              if (!ok) report_bad_attn_page();
+              const int64_t off = (ok ? page : 0) * c.page_stride +
+                                  (int64_t)(key - (int)(at * a.page.d)) * c.token_stride + g * c.head_stride + lane * PL;
+              float d = 0.0f, vv[PL];
+#pragma unroll
+              for (int i = 0; i < PL; ++i) {
+                d = fmaf(qv[i], ok ? to_f<BF>(c.k[off + i]) : 0.0f, d);
+                vv[i] = ok ? to_f<BF>(c.v[off + i]) : 0.0f;
+              }
+#pragma unroll
+              for (int x = 16; x > 0; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
+              d *= a.scale;
+              if (sc && lane == 0) sc[key] = d;
+              const float mn = fmaxf(M, d), f = M == -INFINITY ? 0.0f : ex2(M - mn);
+              const float pr = d == -INFINITY ? 0.0f : ex2(d - mn + kProbShift<BF>);
+              L = L * f + pr;
+#pragma unroll
+              for (int i = 0; i < PL; ++i) acc[i] = acc[i] * f + (d == -INFINITY ? 0.0f : pr * vv[i]);
+              M = mn;
+            }
+          }
+          if (whole) {
+            uint16_t* y = a.out + row * a.ldo + (int64_t)head * D + lane * PL;
+#pragma unroll
+            for (int i = 0; i < PL; ++i) y[i] = from_f<BF>(acc[i] / L);
+            if (a.lse && lane == 0)
+              a.lse[((int64_t)get.b * c.kv_heads + g) * a.rows + rr] = M + log2f(L) - kProbShift<BF>;
+          } else {
+            float* y = a.part + ((int64_t)(2 * blockIdx.x + (begin >= u0 && begin != u0 ? 1 : 0)) * RB + t * 16 + r) * (D + 2);
+#pragma unroll
+            for (int i = 0; i < PL; ++i) y[2 + lane * PL + i] = acc[i];
+            if (lane == 0) {
+              y[0] = M;
+              y[1] = L;
+            }
+          }
+        }
+        __syncthreads();  // before the stages are filled again, or the next 16 rows come
+      }
+      fresh = true;
+    }
+    if (last) begin = u + 1;
+    advance(get);
+    slot = slot + 1 == NS ? 0 : slot + 1;
+  }
+  cp_async_wait<0>();
+}
+
+// The parts of an item that several CTAs shared, joined in the cache's order: grid (items, row
+// groups), a warp per row.
+template <bool BF, int D>
+__global__ void __launch_bounds__(128) k_paged_attn_join(AttnArgs a, int RB) {
+  constexpr int PL = D / 32;
+  pdl_trigger();
+  pdl_wait();
+  const PagedView& c = a.c;
+  const int items = c.kv_heads * a.blocks;
+  const int b = blockIdx.x / items, item = blockIdx.x - b * items, g = item / a.blocks, rb = item - g * a.blocks;
+  const int lane = threadIdx.x & 31, r = blockIdx.y * 4 + (threadIdx.x >> 5), rr = rb * RB + r;
+  if (r >= RB || rr >= a.rows) return;
+  const int64_t p0 = a.prefix[b], n = (a.prefix[b + 1] - p0) / items, total = a.prefix[c.batch];
+  if (n == 0) return;
+  const int64_t c0 = p0 + item * n, c1 = c0 + n;
+  const int64_t ctas = min((int64_t)kPaGrid, total);
+  const int i0 = (int)(((c0 + 1) * ctas - 1) / total), i1 = (int)((c1 * ctas - 1) / total);
+  if (i0 == i1) return;  // one CTA had it whole
+  const int second = i0 * total / ctas == c0 ? 0 : 1;  // the item is not the first of CTA i0's run
+  auto part = [&](int i) { return a.part + ((int64_t)(2 * i + (i == i0 ? second : 0)) * RB + r) * (D + 2); };
+  float M = -INFINITY;
+  for (int i = i0 + lane; i <= i1; i += 32) M = fmaxf(M, part(i)[0]);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+  float L = 0.0f, acc[PL];
+#pragma unroll
+  for (int i = 0; i < PL; ++i) acc[i] = 0.0f;
+#pragma unroll 4
+  for (int i = i0; i <= i1; ++i) {
+    const float* x = part(i);
+    const float li = x[1], f = li == 0.0f ? 0.0f : ex2(x[0] - M);
+    if (li != 0.0f) {
+      L = fmaf(li, f, L);
+#pragma unroll
+      for (int j = 0; j < PL; ++j) acc[j] = fmaf(x[2 + lane * PL + j], f, acc[j]);
+    }
+  }
+  const int tok = rr / a.rep, head = g * a.rep + rr - tok * a.rep;
+  uint16_t* y = a.out + ((int64_t)b * a.tokens + tok) * a.ldo + (int64_t)head * D + lane * PL;
+#pragma unroll
+  for (int i = 0; i < PL; ++i) y[i] = from_f<BF>(acc[i] / L);
+  if (a.lse && lane == 0) a.lse[((int64_t)b * c.kv_heads + g) * a.rows + rr] = M + log2f(L) - kProbShift<BF>;
+}
+
+// weights[b, g, s] += sum over the item rows of 2^(score - lse).  One thread per token, rows in order.
+__global__ void __launch_bounds__(256) k_paged_attn_weights(AttnArgs a, float* weights, int64_t ldw) {
+  pdl_trigger();
+  pdl_wait();
+  const PagedView& c = a.c;
+  const int g = blockIdx.y, b = blockIdx.z, s = blockIdx.x * 256 + threadIdx.x;
+  const int len = c.lengths[b];
+  if (len < 0 || (int64_t)len + a.tokens > c.capacity || s >= len + a.tokens) return;
+  const int64_t item = (int64_t)b * c.kv_heads + g;
+  const float* x = a.scores + item * a.rows * a.ld_scores + s;
+  const float* lse = a.lse + item * a.rows;
+  float sum = 0.0f;
+#pragma unroll 8
+  for (int r = 0; r < a.rows; ++r) {
+    const float v = x[r * a.ld_scores];
+    sum += v == -INFINITY ? 0.0f : ex2(v - lse[r]);
+  }
+  weights[item * ldw + s] += sum;
+}
+
+// Bytes of the workspace's parts, in order.
+struct AttnSpace {
+  int64_t prefix, part, lse, scores, ld_scores;
+  int64_t bytes() const { return prefix + part + lse + scores; }
+};
+static AttnSpace attn_space(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t tokens, int64_t max_tokens,
+                            bool weights) {
+  AttnSpace s;
+  const int64_t rows = heads / kv_heads * tokens, RB = rows <= 16 ? 16 : 32;
+  s.prefix = align_up((batch + 1) * 8, 256);
+  s.part = align_up(2 * kPaGrid * RB * (D + 2) * 4, 256);
+  s.ld_scores = align_up(max_tokens, 8);
+  s.lse = weights ? align_up(batch * kv_heads * rows * 4, 256) : 0;
+  s.scores = weights ? align_up(batch * kv_heads * rows * s.ld_scores * 4, 256) : 0;
+  return s;
+}
+
+template <bool BF, int D>
+static cudaError_t launch_attn(const AttnArgs& a, float* weights, int64_t ldw, cudaStream_t s) {
+  const int RB = a.rows <= 16 ? 16 : 32;
+  auto* k = RB == 16 ? k_paged_attn<BF, D, 1> : k_paged_attn<BF, D, 2>;
+  const size_t dyn = (size_t)kPaWarps * kPaStages * kPaStage + (size_t)kPaWarps * RB * 8 + (size_t)a.c.batch * 4;
+  {
+    // the shared-memory opt-in, once per kernel and device, for the largest batch
+    static std::mutex mu;
+    static std::map<std::pair<const void*, int>, bool> done;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    std::lock_guard<std::mutex> lock(mu);
+    bool& have = done[std::make_pair(reinterpret_cast<const void*>(k), dev)];
+    if (!have) {
+      e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               kPaWarps * kPaStages * kPaStage + kPaWarps * 32 * 8 + kPagedMaxBatch * 4);
+      if (e != cudaSuccess) return e;
+      have = true;
+    }
+  }
+  cudaError_t e = launch_pdl(k, dim3(kPaGrid), dim3(kPaThreads), dyn, s, 1u, a);
+  if (e != cudaSuccess) return e;
+  e = launch_pdl(k_paged_attn_join<BF, D>, dim3((unsigned)(a.c.batch * a.c.kv_heads * a.blocks), (unsigned)(std::min(a.rows, RB) + 3) / 4),
+                 dim3(128), 0, s, 1u, a, RB);
+  if (e != cudaSuccess || !weights) return e;
+  return launch_pdl(k_paged_attn_weights,
+                    dim3((unsigned)((a.c.capacity + 255) / 256), (unsigned)a.c.kv_heads, (unsigned)a.c.batch), dim3(256), 0,
+                    s, 1u, a, weights, ldw);
+}
+
+}  // namespace otf
+
+using otf::check_device;
+using otf::set_cuda_error;
+
+int otf::paged_attn_device_error(int clear) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, otf::g_paged_attn_device_error, sizeof(int)) != cudaSuccess) {
+    set_cuda_error(cudaGetLastError());
+    return -1;
+  }
+  if (clear && v) {
+    const int z = 0;
+    cudaMemcpyToSymbol(otf::g_paged_attn_device_error, &z, sizeof(int));
+  }
+  return v;
+}
+
+extern "C" OTF_API int64_t otf_paged_attn_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads,
+                                                          int64_t head_dim, int64_t tokens, int64_t max_tokens,
+                                                          int with_weights) {
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || head_dim <= 0 || tokens <= 0 ||
+      tokens > otf::kPagedMaxTokens || max_tokens <= 0)
+    return -1;
+  return otf::attn_space(batch, heads, kv_heads, head_dim, tokens, max_tokens, with_weights != 0).bytes();
+}
+
+extern "C" OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* q, int64_t ldq, int64_t heads,
+                                      int64_t tokens, float scale, void* out, int64_t ldo, float* weights,
+                                      int64_t ldw, void* workspace, int64_t workspace_bytes, void* stream) {
+  otf::AttnArgs a = {};
+  int st = otf::view_of(cache, a.c);
+  if (st != OTF_OK) return st;
+  const int64_t D = cache->head_dim;
+  if (heads <= 0 || heads % a.c.kv_heads || tokens <= 0) return OTF_ERR_INVALID;
+  if (tokens > otf::kPagedMaxTokens || heads > 65535) return OTF_ERR_UNSUPPORTED;
+  if (!otf::rows16(q, ldq, heads * D) || !otf::rows16(out, ldo, heads * D)) return OTF_ERR_INVALID;
+  if (weights && ldw < a.c.capacity) return OTF_ERR_INVALID;
+  const otf::AttnSpace space = otf::attn_space(a.c.batch, heads, a.c.kv_heads, D, tokens, a.c.capacity, weights != nullptr);
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < space.bytes())
+    return OTF_ERR_INVALID;
+  st = check_device();
+  if (st != OTF_OK) return st;
+  a.page = otf::fast_div((uint32_t)a.c.page_size);
+  a.q = static_cast<const uint16_t*>(q);
+  a.ldq = ldq;
+  a.out = static_cast<uint16_t*>(out);
+  a.ldo = ldo;
+  a.scale = scale * 1.4426950408889634f;
+  a.rep = (int)(heads / a.c.kv_heads);
+  a.tokens = (int)tokens;
+  a.rows = (int)(a.rep * tokens);
+  a.blocks = a.rows <= 16 ? 1 : (a.rows + 31) / 32;
+  char* w = static_cast<char*>(workspace);
+  a.prefix = reinterpret_cast<int64_t*>(w);
+  a.part = reinterpret_cast<float*>(w + space.prefix);
+  if (weights) {
+    a.lse = reinterpret_cast<float*>(w + space.prefix + space.part);
+    a.scores = reinterpret_cast<float*>(w + space.prefix + space.part + space.lse);
+    a.ld_scores = space.ld_scores;
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool bf = cache->dtype == OTF_DTYPE_BF16;
+  const cudaError_t e = D == 128 ? (bf ? otf::launch_attn<true, 128>(a, weights, ldw, s) : otf::launch_attn<false, 128>(a, weights, ldw, s))
+                                 : (bf ? otf::launch_attn<true, 64>(a, weights, ldw, s) : otf::launch_attn<false, 64>(a, weights, ldw, s));
+  return set_cuda_error(e);
+}
