@@ -36,7 +36,13 @@ struct __align__(16) RowPart {
 __device__ __forceinline__ float exp_scaled(float d, float c_hi, float c_lo) {
   const float n = fmaxf(rintf(d * c_hi), -160.0f);
   const float r = fmaf(d, c_lo, fmaf(d, c_hi, -n));
-  return d == -INFINITY ? 0.0f : ldexpf(exp2f(r), (int)n);
+  return d > -INFINITY ? ldexpf(exp2f(r), (int)n) : 0.0f;  // 0 for a NaN too
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // 0, or from 1e-20 on (log2(e) / T and its product with a difference of logits stay finite).
@@ -46,14 +52,29 @@ __device__ __forceinline__ float temperature_of(const float* temperatures, float
   return temperatures ? temperatures[b] : temperature;
 }
 
-// Grid (segments, rows): rows are the batch x (drafts + 1) of the target, then the draft's.
+// Four consecutive logits of a row, -inf behind its end.  Rows that are not 16-byte aligned are read
+// value by value by the same threads, so that a row's sums do not depend on where it lies.
+__device__ __forceinline__ float4 logits4(const float* x, int i, int end, bool aligned) {
+  if (aligned && i + 4 <= end) return __ldcs(reinterpret_cast<const float4*>(x + i));
+  float4 v;
+  v.x = i < end ? __ldcs(x + i) : -INFINITY;
+  v.y = i + 1 < end ? __ldcs(x + i + 1) : -INFINITY;
+  v.z = i + 2 < end ? __ldcs(x + i + 2) : -INFINITY;
+  v.w = i + 3 < end ? __ldcs(x + i + 3) : -INFINITY;
+  return v;
+}
+
+// One pass over the logits: grid (segments, rows), the rows being the batch x (drafts + 1) of the
+// target, then the draft's.  A thread holds its 32 values in registers: their maximum, then the
+// sum of exponentials under it, joined over the CTA.  Memory-bound, 5 instructions per logit.
 __global__ void __launch_bounds__(kVerifyThreads) k_verify_rows(const float* target, int64_t tseq, int64_t ldt,
                                                                 const float* draft, int64_t dseq, int64_t ldd,
                                                                 const float* temperatures, float temperature,
                                                                 const int* counts, int batch, int drafts, int vocab,
                                                                 RowPart* parts) {
-  __shared__ float s_m[8], s_s[8];
-  __shared__ int s_i[8];
+  constexpr int N = kVerifySeg / (4 * kVerifyThreads), W = kVerifyThreads / 32;
+  __shared__ float s_m[W], s_s[W];
+  __shared__ int s_i[W];
   pdl_trigger();
   pdl_wait();
   const int row = blockIdx.y, trows = batch * (drafts + 1);
@@ -65,88 +86,144 @@ __global__ void __launch_bounds__(kVerifyThreads) k_verify_rows(const float* tar
   const int count = counts ? counts[b] : drafts;
   if (of_target ? j > count : (j >= count || T == 0.0f)) return;  // a row that nothing asks for
   const float* x = of_target ? target + b * tseq + j * ldt : draft + b * dseq + j * ldd;
-  const int i0 = blockIdx.x * kVerifySeg, i1 = min(vocab, i0 + kVerifySeg);
+  const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  const int i0 = blockIdx.x * kVerifySeg + 4 * threadIdx.x;
+  float4 v[N];
+#pragma unroll
+  for (int z = 0; z < N; ++z) v[z] = logits4(x, i0 + z * 4 * kVerifyThreads, vocab, aligned);
+  float m = -INFINITY;  // a NaN is never the largest
+#pragma unroll
+  for (int z = 0; z < N; ++z) m = fmaxf(m, fmaxf(fmaxf(v[z].x, v[z].y), fmaxf(v[z].z, v[z].w)));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float s = 0.0f;
+  int at = INT_MAX;
+  if (T == 0.0f) {
+#pragma unroll
+    for (int z = N - 1; z >= 0; --z) {
+      const float e[4] = {v[z].x, v[z].y, v[z].z, v[z].w};
+#pragma unroll
+      for (int w = 3; w >= 0; --w) {
+        const int i = i0 + z * 4 * kVerifyThreads + w;
+        if (e[w] == m && i < vocab) at = i;
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
+      const int a2 = __shfl_xor_sync(0xffffffffu, at, o);
+      if (m2 > m || (m2 == m && a2 < at)) {
+        m = m2;
+        at = a2;
+      }
+    }
+    if (lane == 0) {
+      s_m[warp] = m;
+      s_i[warp] = at;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < W; ++w)
+        if (s_m[w] > m || (s_m[w] == m && s_i[w] < at)) {
+          m = s_m[w];
+          at = s_i[w];
+        }
+      parts[(int64_t)row * gridDim.x + blockIdx.x] = RowPart{m, 0.0f, at, 0};
+    }
+    return;
+  }
   const float c_hi = (float)(1.4426950408889634 / (double)T);
   const float c_lo = (float)(1.4426950408889634 / (double)T - (double)c_hi);
-  float m = -INFINITY, s = 0.0f;
-  int at = INT_MAX;
-  for (int i = i0 + threadIdx.x; i < i1; i += kVerifyThreads)
-    if (x[i] > m || (at == INT_MAX && x[i] == x[i])) {  // a NaN is never the largest
-      m = x[i];
-      at = i;
-    }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  auto better = [](float m1, int i1_, float m2, int i2_) { return m1 > m2 || (m1 == m2 && i1_ < i2_); };
+  auto term = [&](float x, float max) {  // 0 for -inf and NaN (the maximum drops a NaN)
+    const float d = x - max;
+    return ex2(fmaxf(fmaf(d, c_hi, d * c_lo), -200.0f));
+  };
+  const float mt = m == -INFINITY ? 0.0f : m;  // nothing but -inf: the sum is 0
+#pragma unroll
+  for (int z = 0; z < N; ++z)
+    if (i0 + z * 4 * kVerifyThreads < vocab)
+      s += (term(v[z].x, mt) + term(v[z].y, mt)) + (term(v[z].z, mt) + term(v[z].w, mt));
+  auto join = [&](float m2, float s2) {
+    const float M = fmaxf(m, m2);
+    if (M != -INFINITY) s = s * term(m, M) + s2 * term(m2, M);  // else both are 0
+    m = M;
+  };
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
-    const int a2 = __shfl_xor_sync(0xffffffffu, at, o);
-    if (better(m2, a2, m, at)) {
-      m = m2;
-      at = a2;
-    }
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    join(m2, s2);
   }
   if (lane == 0) {
     s_m[warp] = m;
-    s_i[warp] = at;
+    s_s[warp] = s;
   }
   __syncthreads();
-  for (int w = 0; w < 8; ++w)
-    if (better(s_m[w], s_i[w], m, at)) {
-      m = s_m[w];
-      at = s_i[w];
-    }
-  if (T != 0.0f && m != -INFINITY)
-    for (int i = i0 + threadIdx.x; i < i1; i += kVerifyThreads) s += exp_scaled(x[i] - m, c_hi, c_lo);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (lane == 0) s_s[warp] = s;
-  __syncthreads();
   if (threadIdx.x == 0) {
-    s = 0.0f;
-    for (int w = 0; w < 8; ++w) s += s_s[w];
-    parts[(int64_t)row * gridDim.x + blockIdx.x] = RowPart{m, s, at, 0};
+    for (int w = 1; w < W; ++w) join(s_m[w], s_s[w]);
+    parts[(int64_t)row * gridDim.x + blockIdx.x] = RowPart{m, s, INT_MAX, 0};
   }
 }
 
-// One CTA per sequence: the rows' parts joined, the drafted tokens taken or refused, the draw.
-__global__ void __launch_bounds__(1024) k_verify_pick(const float* target, int64_t tseq, int64_t ldt,
-                                                      const float* draft, int64_t dseq, int64_t ldd,
-                                                      const int64_t* tokens, int64_t ldtok, const float* uniforms,
-                                                      int64_t ldu, const float* noise, int64_t ldn,
-                                                      const float* temperatures, float temperature, const int* counts,
-                                                      int64_t* out, int* accepted, int batch, int drafts, int vocab,
-                                                      const RowPart* parts, int segs) {
-  __shared__ double s_max[2 * kVerifyMaxDrafts + 1], s_sum[2 * kVerifyMaxDrafts + 1];
+// A race's leader: the largest w / e and its index, of what the draft leaves of p and of p itself.
+struct Leader {
+  float best[2];
+  int at[2];
+  __device__ __forceinline__ void take(int z, float score, int i) {
+    if (score > best[z] || (score == best[z] && i < at[z])) {
+      best[z] = score;
+      at[z] = i;
+    }
+  }
+};
+
+// A cluster of kPickCluster CTAs per sequence.  Every CTA joins the rows' parts and follows the
+// drafted tokens (a few hundred numbers); the race over the vocabulary is cut among them, and
+// their leaders meet in rank 0 through distributed shared memory.
+constexpr int kPickCluster = 8;
+constexpr int kPickThreads = 512;
+
+__global__ void __launch_bounds__(kPickThreads) k_verify_pick(const float* target, int64_t tseq, int64_t ldt,
+                                                              const float* draft, int64_t dseq, int64_t ldd,
+                                                              const int64_t* tokens, int64_t ldtok, const float* uniforms,
+                                                              int64_t ldu, const float* noise, int64_t ldn,
+                                                              const float* temperatures, float temperature, const int* counts,
+                                                              int64_t* out, int* accepted, int batch, int drafts, int vocab,
+                                                              const RowPart* parts, int segs) {
+  constexpr int W = kPickThreads / 32;
+  __shared__ double s_sum[2 * kVerifyMaxDrafts + 1];
+  __shared__ float s_max[2 * kVerifyMaxDrafts + 1];
   __shared__ int s_at[kVerifyMaxDrafts + 1];
   __shared__ int s_taken;
-  __shared__ float s_best[2][32];
-  __shared__ int s_idx[2][32];
+  __shared__ __align__(16) Leader s_lead[W];
+  __shared__ __align__(16) Leader s_all[kPickCluster];
   pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int b = blockIdx.x / kPickCluster, rank = (int)cluster_ctarank(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const float T = temperature_of(temperatures, temperature, b);
   const int count = counts ? counts[b] : drafts;
   if (count < 0 || count > drafts || !temperature_ok(T) || (T > 0.0f && (!noise || (count && !uniforms)))) {
-    for (int j = tid; j <= drafts; j += blockDim.x) out[(int64_t)b * (drafts + 1) + j] = -1;
+    if (rank) return;  // as all the others do
+    for (int j = tid; j <= drafts; j += kPickThreads) out[(int64_t)b * (drafts + 1) + j] = -1;
     if (tid == 0) {
       accepted[b] = 0;
       atomicExch(&g_verify_device_error, 1);
     }
     return;
   }
+  if (T == 0.0f && rank) return;  // no race
   const bool drafted = draft != nullptr && T > 0.0f;
-  for (int r = warp; r < count + 1 + (drafted ? count : 0); r += 32) {
+  for (int r = warp; r < count + 1 + (drafted ? count : 0); r += W) {
     const int64_t row = r <= count ? (int64_t)b * (drafts + 1) + r
                                    : (int64_t)batch * (drafts + 1) + (int64_t)b * drafts + (r - count - 1);
     const RowPart* p = parts + row * segs;
     float m = -INFINITY;
     int at = INT_MAX;
-    for (int i = lane; i < segs; i += 32)
-      if (p[i].max > m || (p[i].max == m && p[i].at < at)) {
-        m = p[i].max;
-        at = p[i].at;
+    for (int i = lane; i < segs; i += 32) {
+      const RowPart q = p[i];
+      if (q.max > m || (q.max == m && q.at < at)) {
+        m = q.max;
+        at = q.at;
       }
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
@@ -158,8 +235,10 @@ __global__ void __launch_bounds__(1024) k_verify_pick(const float* target, int64
     }
     double s = 0.0;
     if (T > 0.0f)
-      for (int i = lane; i < segs; i += 32)
-        if (p[i].max != -INFINITY) s += (double)p[i].sum * exp(((double)p[i].max - (double)m) / (double)T);
+      for (int i = lane; i < segs; i += 32) {
+        const RowPart q = p[i];
+        if (q.sum != 0.0f) s += (double)q.sum * exp(((double)q.max - (double)m) / (double)T);
+      }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (lane == 0) {
@@ -175,15 +254,16 @@ __global__ void __launch_bounds__(1024) k_verify_pick(const float* target, int64
     if (lane < count) {
       const int64_t d = tokens[b * ldtok + lane];
       if (d < 0 || d >= vocab) {
-        atomicExch(&g_verify_device_error, 1);
+        if (rank == 0) atomicExch(&g_verify_device_error, 1);
       } else if (T == 0.0f) {
         take = d == s_at[lane];
       } else {
-        const double p = exp(((double)target[b * tseq + lane * ldt + d] - s_max[lane]) / (double)T) / s_sum[lane];
+        const double p = exp(((double)target[b * tseq + lane * ldt + d] - (double)s_max[lane]) / (double)T) / s_sum[lane];
         double q = 1.0;
         if (drafted)
-          q = exp(((double)draft[b * dseq + lane * ldd + d] - s_max[drafts + 1 + lane]) / (double)T) /
+          q = exp(((double)draft[b * dseq + lane * ldd + d] - (double)s_max[drafts + 1 + lane]) / (double)T) /
               s_sum[drafts + 1 + lane];
+        if (!(q >= 0.0)) q = 0.0;  // a NaN
         take = (double)uniforms[b * ldu + lane] * q < p;
       }
     }
@@ -199,28 +279,30 @@ __global__ void __launch_bounds__(1024) k_verify_pick(const float* target, int64
     const bool refused = taken < count;
     const float* x = target + b * tseq + taken * ldt;
     const float* y = drafted && refused ? draft + b * dseq + taken * ldd : nullptr;
-    const float xm = (float)s_max[taken], xi = (float)(1.0 / s_sum[taken]);
-    const float ym = y ? (float)s_max[drafts + 1 + taken] : 0.0f, yi = y ? (float)(1.0 / s_sum[drafts + 1 + taken]) : 0.0f;
+    const float* e = noise + b * ldn;
+    const bool ax = (reinterpret_cast<uintptr_t>(x) & 15) == 0, ay = (reinterpret_cast<uintptr_t>(y) & 15) == 0,
+               ae = (reinterpret_cast<uintptr_t>(e) & 15) == 0;
+    const float xm = s_max[taken], xi = (float)(1.0 / s_sum[taken]);
+    const float ym = y ? s_max[drafts + 1 + taken] : 0.0f, yi = y ? (float)(1.0 / s_sum[drafts + 1 + taken]) : 0.0f;
     const int64_t out_of = refused && !drafted ? tokens[b * ldtok + taken] : -1;
     const float c_hi = (float)(1.4426950408889634 / (double)T);
     const float c_lo = (float)(1.4426950408889634 / (double)T - (double)c_hi);
-    // the race of what is left of p, and of p itself for where nothing is left
-    float best[2] = {0.0f, 0.0f};
-    int idx[2] = {INT_MAX, INT_MAX};
-    for (int i = tid; i < vocab; i += blockDim.x) {
-      const float e = noise[b * ldn + i];
-      // products that round by themselves: equal rows leave exactly nothing
-      const float p = __fmul_rn(exp_scaled(x[i] - xm, c_hi, c_lo), xi);
-      float left = p;
-      if (y) left = __fsub_rn(p, __fmul_rn(exp_scaled(y[i] - ym, c_hi, c_lo), yi));
-      if (i == out_of) left = 0.0f;
-      const float w[2] = {left, p};
+    Leader lead = {{0.0f, 0.0f}, {INT_MAX, INT_MAX}};
+    for (int i = 4 * (rank * kPickThreads + tid); i < vocab; i += 4 * kPickThreads * kPickCluster) {
+      const float4 vx = logits4(x, i, vocab, ax), ve = logits4(e, i, vocab, ae);
+      float4 vy = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (y) vy = logits4(y, i, vocab, ay);
+      const float fx[4] = {vx.x, vx.y, vx.z, vx.w}, fy[4] = {vy.x, vy.y, vy.z, vy.w}, fe[4] = {ve.x, ve.y, ve.z, ve.w};
 #pragma unroll
-      for (int z = 0; z < 2; ++z) {
-        const float sc = w[z] > 0.0f ? w[z] / e : 0.0f;
-        if (sc > best[z]) {
-          best[z] = sc;
-          idx[z] = i;
+      for (int z = 0; z < 4; ++z) {
+        // products that round by themselves: equal rows leave exactly nothing
+        const float p = __fmul_rn(exp_scaled(fx[z] - xm, c_hi, c_lo), xi);
+        float left = p;
+        if (y) left = __fsub_rn(p, __fmul_rn(exp_scaled(fy[z] - ym, c_hi, c_lo), yi));
+        if (i + z == out_of) left = 0.0f;
+        if (i + z < vocab && p > 0.0f) {
+          lead.take(1, p / fe[z], i + z);
+          if (left > 0.0f) lead.take(0, left / fe[z], i + z);
         }
       }
     }
@@ -228,31 +310,30 @@ __global__ void __launch_bounds__(1024) k_verify_pick(const float* target, int64
     for (int z = 0; z < 2; ++z) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
-        const float s2 = __shfl_xor_sync(0xffffffffu, best[z], o);
-        const int i2 = __shfl_xor_sync(0xffffffffu, idx[z], o);
-        if (s2 > best[z] || (s2 == best[z] && i2 < idx[z])) {
-          best[z] = s2;
-          idx[z] = i2;
-        }
-      }
-      if (lane == 0) {
-        s_best[z][warp] = best[z];
-        s_idx[z][warp] = idx[z];
+        const float s2 = __shfl_xor_sync(0xffffffffu, lead.best[z], o);
+        const int i2 = __shfl_xor_sync(0xffffffffu, lead.at[z], o);
+        lead.take(z, s2, i2);
       }
     }
+    if (lane == 0) s_lead[warp] = lead;
     __syncthreads();
+    cluster_sync_all();  // rank 0 runs
+    if (tid == 0) {
+      for (int w = 1; w < W; ++w)
+        for (int z = 0; z < 2; ++z) lead.take(z, s_lead[w].best[z], s_lead[w].at[z]);
+      const uint32_t to = mapa_shared(smem_u32(&s_all[rank]), 0);
+      st_cluster_v2(to, __float_as_uint(lead.best[0]), __float_as_uint(lead.best[1]));
+      st_cluster_v2(to + 8, (uint32_t)lead.at[0], (uint32_t)lead.at[1]);
+    }
+    cluster_sync_all();
+    if (rank) return;
     for (int z = 0; z < 2 && last < 0; ++z) {
-      float bs = 0.0f;
-      int bi = INT_MAX;
-      for (int w = 0; w < 32; ++w)
-        if (s_best[z][w] > bs || (s_best[z][w] == bs && s_idx[z][w] < bi)) {
-          bs = s_best[z][w];
-          bi = s_idx[z][w];
-        }
-      if (bi != INT_MAX) last = bi;
+      Leader w = s_all[0];
+      for (int k = 1; k < kPickCluster; ++k) w.take(z, s_all[k].best[z], s_all[k].at[z]);
+      if (w.at[z] != INT_MAX) last = w.at[z];
     }
   }
-  for (int j = tid; j <= drafts; j += blockDim.x)
+  for (int j = tid; j <= drafts; j += kPickThreads)
     out[(int64_t)b * (drafts + 1) + j] = last < 0 || j > taken ? -1 : j < taken ? tokens[b * ldtok + j] : last;
   if (tid == 0) {
     accepted[b] = last < 0 ? 0 : taken;
@@ -316,7 +397,8 @@ extern "C" OTF_API int otf_verify_drafts(const float* target, int64_t target_seq
                                   0, s, 1u, target, target_seq, ld_target, draft, draft_seq, ld_draft, temperatures,
                                   temperature, counts, (int)batch, (int)drafts, (int)vocab, parts);
   if (e != cudaSuccess) return set_cuda_error(e);
-  return set_cuda_error(otf::launch_pdl(otf::k_verify_pick, dim3((unsigned)batch), dim3(1024), 0, s, 1u, target,
+  return set_cuda_error(otf::launch_pdl(otf::k_verify_pick, dim3((unsigned)batch * otf::kPickCluster),
+                                        dim3(otf::kPickThreads), 0, s, (unsigned)otf::kPickCluster, target,
                                         target_seq, ld_target, draft, draft_seq, ld_draft, tokens, ld_tokens, uniforms,
                                         ld_uniforms, noise, ld_noise, temperatures, temperature, counts, out_tokens,
                                         accepted, (int)batch, (int)drafts, (int)vocab, (const otf::RowPart*)parts,

@@ -85,6 +85,18 @@ def test_verify_masked_logits(cuda_dev):
     check(cuda_dev, target, torch.full((4, 3), 4242), None, uniforms, noise, 0.9)
 
 
+def test_verify_nan_logits_count_as_masked(cuda_dev):
+    from otf_llm.speculative import verify_drafts
+    target, tokens, draft, uniforms, noise = (t.to(cuda_dev) for t in inputs(4, 3, 9001, True, seed=13))
+    target[:, :, 1::3], draft[:, :, 2::5] = float("nan"), float("nan")
+    for temperature in (0.0, 0.8):
+        rest = dict(uniforms=uniforms, noise=noise, temperature=temperature)
+        got = verify_drafts(target, tokens, draft_logits=draft, **rest)
+        want = verify_drafts(target.nan_to_num(nan=-float("inf")), tokens,
+                             draft_logits=draft.nan_to_num(nan=-float("inf")), **rest)
+        assert flag() == 0 and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_verify_equal_distributions(cuda_dev):
     """Draft and target the same: all taken; one refused all the same (u = 1 cannot be below) leaves nothing
     of p - q, and p is drawn from."""
