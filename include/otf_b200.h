@@ -525,8 +525,8 @@ OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* q, int64_t 
  * budget - recent of the largest weights (ties: the lower place; a NaN counts as the largest).
  * The order stays.  kept: int32 [batch, kv_heads, budget], the places kept, then -1.  The kept
  * keys and values go to the same head's tokens 0, 1, ... of `to`, whose page_table holds pages
- * that hold nothing of `from`, or all the same pages in the same order: then from's pools,
- * table and lengths are given again and the cache is cut in place.  `to` has from's geometry
+ * that hold nothing of `from` (in the same pools or others); or from's pools, table, weights and
+ * lengths are given again, and the cache is cut in place.  `to` has from's geometry
  * (kv_heads, head_dim, batch, dtype, page_size) and room for budget tokens.  weights (fp32
  * [batch, kv_heads, ldw]) go along to weights_out ([batch, kv_heads, ldw_out], may be weights),
  * zero behind the kept ones (in place: up to the old length).  lengths_out[b] = min(lengths[b],
@@ -551,7 +551,7 @@ OTF_API int otf_paged_evict(const otf_paged_cache* from, const otf_paged_cache* 
  * counts: device int32 [batch], the drafted tokens of each sequence (0..drafts), or NULL: all
  * have `drafts` (0..32).  out_tokens: int64 [batch, drafts + 1], the taken tokens, the drawn
  * one, then -1; accepted: int32 [batch].  Temperatures are 0 or in 1e-20 .. 1e20; a NaN among
- * the logits is never the largest.  A sequence without a token of positive weight, or
+ * the logits counts as -inf.  A sequence without a token of positive weight, or
  * with a count or temperature out of range, gets -1 and raises the otf_device_error flag; so
  * does a drafted token outside the vocabulary, which is refused.  Where max(p - q, 0) holds
  * nothing, p is drawn from.  workspace: otf_verify_workspace_bytes(...), 256-byte aligned, need

@@ -27,66 +27,142 @@ __device__ __forceinline__ int sequence_of(const int* starts, int batch, int row
   return b;
 }
 
-// Rotary positions and the cache write, one CTA per row.
-template <bool BF>
-__global__ void __launch_bounds__(256) k_paged_append(PagedView c, const double* turns, int rot, float factor,
-                                                      int interleaved, const uint16_t* q, int64_t ldq, uint16_t* qo,
-                                                      int64_t ldqo, int heads, const uint16_t* k, int64_t ldk,
-                                                      const uint16_t* v, int64_t ldv, const int* starts,
-                                                      const int* positions, int per, int D) {
-  __shared__ float s_c[64], s_s[64];
-  pdl_trigger();
-  pdl_wait();
+// What k_paged_append gets beside the cache.
+struct AppendArgs {
+  PagedView c;
+  const double* turns;
+  int rot, interleaved;
+  float factor;
+  const uint16_t* q;
+  uint16_t* qo;
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t ldq, ldqo, ldk, ldv;
+  int heads;  // 0: keys and values alone
+  const int* starts;
+  const int* positions;
+  int per;    // rows of a sequence, without starts
+};
+
+// Where a row goes: the offset of its token's page row, or -1 (all threads agree).  The rotary
+// position's sines and cosines go to s_c and s_s.
+__device__ __forceinline__ int64_t append_place(const AppendArgs& a, float* s_c, float* s_s) {
+  const PagedView& c = a.c;
   const int row = blockIdx.x, tid = threadIdx.x;
-  const int b = starts ? sequence_of(starts, c.batch, row) : row / per;
-  if (b >= c.batch) return;  // behind the last sequence
-  const int t = row - (starts ? starts[b] : b * per);
+  const int b = a.starts ? sequence_of(a.starts, c.batch, row) : row / a.per;
+  if (b >= c.batch) return -1;  // behind the last sequence
+  const int t = row - (a.starts ? a.starts[b] : b * a.per);
   const int len = c.lengths[b];
-  if (len < 0) return;  // no sequence in this place
+  if (len < 0) return -1;  // no sequence in this place
   const int64_t slot = (int64_t)len + t;
   if (t < 0 || slot >= c.capacity) {
     if (tid == 0) report_bad_page();
-    return;
+    return -1;
   }
   const int page = c.table[b * c.ld_table + slot / c.page_size];
   if (page < 0 || page >= c.n_pages) {
     if (tid == 0) report_bad_page();
-    return;
+    return -1;
   }
-  const int half = rot / 2;
-  if (tid < half) {
-    double turn = (double)(positions ? positions[row] : (int)slot) * turns[tid];
+  if (tid < a.rot / 2) {
+    // the angle in turns, 64 bits until the whole turns are gone: what is left keeps 2^-25 of a turn
+    double turn = (double)(a.positions ? a.positions[row] : (int)slot) * a.turns[tid];
     turn -= rint(turn);
     float sn, cs;
     sincospif(2.0f * (float)turn, &sn, &cs);
-    s_c[tid] = cs * factor;
-    s_s[tid] = sn * factor;
+    s_c[tid] = cs * a.factor;
+    s_s[tid] = sn * a.factor;
   }
+  return page * c.page_stride + (slot % c.page_size) * c.token_stride;
+}
+
+// Rotary positions and the cache write, one CTA per row, in units of two 16-byte pieces whose
+// values turn together: pieces i and i + rot / 16 of a head (half layout), or 2i and 2i + 1.
+// Memory-bound: a row is read and written once.  The values are requested before the row's place
+// in the cache and its angles are known, kAppendBatch units at a time.
+constexpr int kAppendThreads = 128;
+constexpr int kAppendBatch = 5;
+
+template <bool BF, int D>
+__global__ void __launch_bounds__(kAppendThreads) k_paged_append(AppendArgs a) {
+  constexpr int UH = D / 16;  // units of a head
+  __shared__ __align__(16) float s_c[64], s_s[64];
+  pdl_trigger();
+  pdl_wait();
+  const PagedView& c = a.c;
+  const int64_t row = blockIdx.x;
+  const int nq = a.heads * UH, nk = c.kv_heads * UH, units = nq + 2 * nk, turning = a.rot / 16;
+  const int second = a.interleaved ? 0 : turning;
+  int64_t at = 0;
+  for (int u0 = 0; u0 < units; u0 += kAppendBatch * kAppendThreads) {
+    uint4 x[kAppendBatch][2];
+#pragma unroll
+    for (int j = 0; j < kAppendBatch; ++j) {
+      const int u = u0 + j * kAppendThreads + threadIdx.x;
+      if (u < units) {
+        const uint16_t* src = u < nq        ? a.q + row * a.ldq + (int64_t)(u / UH) * D
+                              : u < nq + nk ? a.k + row * a.ldk + (int64_t)((u - nq) / UH) * D
+                                            : a.v + row * a.ldv + (int64_t)((u - nq - nk) / UH) * D;
+        const int i = u % UH;
+        const bool halves = second && i < turning && u < nq + nk;
+        x[j][0] = *reinterpret_cast<const uint4*>(src + (halves ? i : 2 * i) * 8);
+        x[j][1] = *reinterpret_cast<const uint4*>(src + (halves ? i + second : 2 * i + 1) * 8);
+      }
+    }
+    if (u0 == 0) {
+      at = append_place(a, s_c, s_s);
+      if (at < 0) return;
+      __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < kAppendBatch; ++j) {
+      const int u = u0 + j * kAppendThreads + threadIdx.x;
+      if (u >= units) break;
+      const int i = u % UH;
+      uint16_t* dst = u < nq        ? a.qo + row * a.ldqo + (int64_t)(u / UH) * D
+                      : u < nq + nk ? c.k + at + (int64_t)((u - nq) / UH) * c.head_stride
+                                    : c.v + at + (int64_t)((u - nq - nk) / UH) * c.head_stride;
+      const bool turn = i < turning && u < nq + nk, halves = second && turn;
+      if (turn) {
+        uint16_t* e = reinterpret_cast<uint16_t*>(x[j]);
+#pragma unroll
+        for (int z = 0; z < 8; ++z) {
+          const float cs = s_c[8 * i + z], sn = s_s[8 * i + z];
+          const float fa = to_f<BF>(halves ? e[z] : e[2 * z]), fb = to_f<BF>(halves ? e[z + 8] : e[2 * z + 1]);
+          const uint16_t ra = from_f<BF>(fa * cs - fb * sn), rb = from_f<BF>(fb * cs + fa * sn);
+          if (halves) {
+            e[z] = ra;
+            e[z + 8] = rb;
+          } else {
+            e[2 * z] = ra;
+            e[2 * z + 1] = rb;
+          }
+        }
+      }
+      *reinterpret_cast<uint4*>(dst + (halves ? i : 2 * i) * 8) = x[j][0];
+      *reinterpret_cast<uint4*>(dst + (halves ? i + second : 2 * i + 1) * 8) = x[j][1];
+    }
+  }
+}
+
+// The same for a rot that is no multiple of 16, value by value.
+template <bool BF>
+__global__ void __launch_bounds__(256) k_paged_append_any(AppendArgs a, int D) {
+  __shared__ float s_c[64], s_s[64];
+  pdl_trigger();
+  pdl_wait();
+  const PagedView& c = a.c;
+  const int64_t row = blockIdx.x;
+  const int64_t at = append_place(a, s_c, s_s);
+  if (at < 0) return;
   __syncthreads();
-  const int64_t at = page * c.page_stride + (slot % c.page_size) * c.token_stride;
-  const int pairs = D / 2;
-  const int turning = (q ? heads : 0) + c.kv_heads;
-  for (int e = tid; e < turning * pairs; e += blockDim.x) {
-    int h = e / pairs;
-    const int i = e - h * pairs;
-    const uint16_t* x;
-    uint16_t* y;
-    if (q && h < heads) {
-      x = q + row * ldq + (int64_t)h * D;
-      y = qo + row * ldqo + (int64_t)h * D;
-    } else {
-      if (q) h -= heads;
-      x = k + row * ldk + (int64_t)h * D;
-      y = c.k + at + h * c.head_stride;
-    }
-    int i0, i1;
-    if (i < half) {
-      i0 = interleaved ? 2 * i : i;
-      i1 = interleaved ? 2 * i + 1 : i + half;
-    } else {
-      i0 = 2 * i;
-      i1 = 2 * i + 1;
-    }
+  const int pairs = D / 2, half = a.rot / 2;
+  for (int e = threadIdx.x; e < (a.heads + c.kv_heads) * pairs; e += blockDim.x) {
+    const int h = e / pairs, i = e - h * pairs;
+    const uint16_t* x = h < a.heads ? a.q + row * a.ldq + (int64_t)h * D : a.k + row * a.ldk + (int64_t)(h - a.heads) * D;
+    uint16_t* y = h < a.heads ? a.qo + row * a.ldqo + (int64_t)h * D : c.k + at + (h - a.heads) * c.head_stride;
+    const bool halves = i < half && !a.interleaved;
+    const int i0 = halves ? i : 2 * i, i1 = halves ? i + half : 2 * i + 1;
     const uint16_t xa = x[i0], xb = x[i1];
     if (i < half) {
       const float fa = to_f<BF>(xa), fb = to_f<BF>(xb);
@@ -97,9 +173,9 @@ __global__ void __launch_bounds__(256) k_paged_append(PagedView c, const double*
       y[i1] = xb;
     }
   }
-  for (int e = tid; e < c.kv_heads * D; e += blockDim.x) {
+  for (int e = threadIdx.x; e < c.kv_heads * D; e += blockDim.x) {
     const int h = e / D, i = e - h * D;
-    c.v[at + h * c.head_stride + i] = v[row * ldv + (int64_t)h * D + i];
+    c.v[at + h * c.head_stride + i] = a.v[row * a.ldv + (int64_t)h * D + i];
   }
 }
 
@@ -113,152 +189,302 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-constexpr int kEvictThreads = 1024;
+constexpr int kEvictThreads = 512;
+constexpr int kEvictCluster = 8;     // CTAs that may share one (sequence, KV head)
+constexpr int kEvictSlice = 4096;    // weights that a CTA takes before others join it
 
-// One CTA per (sequence, KV head): the k-th largest key by four rounds of 8 bits, then the kept
-// places in order.  Weights move downwards only, tile by tile, so they may be cut in place.
+// Which places stay: a cluster per (sequence, KV head), each CTA a contiguous slice of the n
+// weights that are not among the recent ones.  Four rounds of 8 bits find the k-th largest key
+// (each round: counts of the slice's keys in shared memory, summed over the cluster through
+// distributed shared memory), then every CTA, knowing how many kept keys lie before its slice,
+// writes its places in order.  Of the keys equal to the k-th largest the first ones stay.
+// The weights are read from L2 in every round: latency of the rounds bounds it, not bytes.
 __global__ void __launch_bounds__(kEvictThreads) k_evict_select(const int* lengths, int kv_heads, int capacity,
-                                                                const float* weights, int64_t ldw, float* wout,
-                                                                int64_t ldwo, int budget, int recent, int* kept) {
-  __shared__ int s_hist[256];
-  __shared__ int s_need;
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_g[32], s_e[32];
+                                                                const float* weights, int64_t ldw, int budget,
+                                                                int recent, int* kept, int ctas) {
+  constexpr int W = kEvictThreads / 32;
+  __shared__ int s_hist[4][256];
+  __shared__ int s_sum[256];
+  __shared__ int s_cut[2];       // this round's digit, and how many keys of it are needed
+  __shared__ int s_count[2];     // the slice's keys above and at the limit
+  __shared__ int s_g[W], s_e[W];
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int b = blockIdx.x / kv_heads;
-  const float* w = weights + (int64_t)blockIdx.x * ldw;
-  float* wo = wout + (int64_t)blockIdx.x * ldwo;
-  int* keep = kept + (int64_t)blockIdx.x * budget;
+  const int rank = ctas > 1 ? (int)cluster_ctarank() : 0;
+  const int pair = blockIdx.x / ctas, b = pair / kv_heads;
+  const float* w = weights + (int64_t)pair * ldw;
+  int* keep = kept + (int64_t)pair * budget;
   int len = lengths[b];
-  if (len > capacity || len > ldw) {
+  if (len > capacity) {
     if (tid == 0) report_bad_page();
     len = -1;
   }
-  if (len < 0) {
-    for (int i = tid; i < budget; i += kEvictThreads) keep[i] = -1;
-    return;
-  }
-  const bool in_place = wout == weights;
-  if (len <= budget) {
-    for (int i = tid; i < budget; i += kEvictThreads) keep[i] = i < len ? i : -1;
-    if (!in_place)
-      for (int64_t i = tid; i < ldwo; i += kEvictThreads) wo[i] = i < len ? w[i] : 0.0f;
+  if (len <= budget) {  // the whole cluster returns
+    for (int i = rank * kEvictThreads + tid; i < budget; i += ctas * kEvictThreads) keep[i] = i < len ? i : -1;
     return;
   }
   const int n = len - recent, k = budget - recent;
-  if (tid == 0) {
-    s_prefix = 0u;
-    s_need = k;
-  }
-  uint32_t mask = 0u;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) s_hist[tid] = 0;
-    __syncthreads();
-    const uint32_t prefix = s_prefix;
-    for (int i = tid; i < n; i += kEvictThreads) {
+  for (int i = rank * kEvictThreads + tid; i < recent; i += ctas * kEvictThreads) keep[k + i] = n + i;
+  if (k == 0) return;
+  const int per = (n + ctas - 1) / ctas, i0 = min(n, rank * per), i1 = min(n, i0 + per);
+  for (int i = tid; i < 4 * 256; i += kEvictThreads) (&s_hist[0][0])[i] = 0;
+  if (tid < 2) s_count[tid] = 0;
+  __syncthreads();
+  uint32_t limit = 0u, mask = 0u;
+  int need = k;
+#pragma unroll 1
+  for (int round = 0; round < 4; ++round) {
+    const int shift = 24 - 8 * round;
+#pragma unroll 4
+    for (int i = i0 + tid; i < i1; i += kEvictThreads) {
       const uint32_t u = weight_key(w[i]);
-      if ((u & mask) == prefix) atomicAdd(&s_hist[(u >> shift) & 255u], 1);
+      if ((u & mask) == limit) atomicAdd(&s_hist[round][(u >> shift) & 255u], 1);
+    }
+    if (ctas > 1) cluster_sync_all(); else __syncthreads();
+    if (tid < 256) {
+      int sum = 0;
+      if (ctas > 1) {
+        const uint32_t at = smem_u32(&s_hist[round][tid]);
+        for (int r = 0; r < ctas; ++r) sum += ld_cluster_s32(mapa_shared(at, r));
+      } else {
+        sum = s_hist[round][tid];
+      }
+      s_sum[tid] = sum;
     }
     __syncthreads();
-    if (tid == 0) {
-      int need = s_need, bin = 255;
-      while (bin > 0 && s_hist[bin] < need) need -= s_hist[bin--];
-      s_need = need;
-      s_prefix = prefix | ((uint32_t)bin << shift);
+    if (warp == 0) {  // lane l holds the digits 255 - 8 l and the seven below
+      int c[8], mine = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mine += c[i] = s_sum[255 - 8 * lane - i];
+      int before = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += x;
+      }
+      before -= mine;
+      if (before < need && before + mine >= need) {
+        int i = 0;
+        while (before + c[i] < need) before += c[i++];
+        s_cut[0] = 255 - 8 * lane - i;
+        s_cut[1] = need - before;
+      }
     }
+    __syncthreads();
+    limit |= (uint32_t)s_cut[0] << shift;
+    need = s_cut[1];
     mask |= 255u << shift;
-    __syncthreads();
   }
-  const uint32_t limit = s_prefix;
-  const int need = s_need;  // of the keys equal to the limit, the first ones
-  int g0 = 0, e0 = 0;
-  for (int base = 0; base < n; base += kEvictThreads) {
+  int above = 0, equal = 0;
+#pragma unroll 4
+  for (int i = i0 + tid; i < i1; i += kEvictThreads) {
+    const uint32_t u = weight_key(w[i]);
+    above += u > limit;
+    equal += u == limit;
+  }
+  above = __reduce_add_sync(0xffffffffu, above);
+  equal = __reduce_add_sync(0xffffffffu, equal);
+  if (lane == 0) {
+    atomicAdd(&s_count[0], above);
+    atomicAdd(&s_count[1], equal);
+  }
+  int g0 = 0, e0 = 0;  // kept keys above the limit, and keys at it, before this tile
+  if (ctas > 1) {
+    cluster_sync_all();
+    for (int r = 0; r < rank; ++r) {
+      g0 += ld_cluster_s32(mapa_shared(smem_u32(&s_count[0]), r));
+      e0 += ld_cluster_s32(mapa_shared(smem_u32(&s_count[1]), r));
+    }
+    cluster_sync_all();  // no CTA leaves while another reads its counts
+  }
+  for (int base = i0; base < i1; base += kEvictThreads) {
     const int i = base + tid;
-    const float x = i < n ? w[i] : 0.0f;
-    const uint32_t u = weight_key(x);
-    const bool gt = k > 0 && i < n && u > limit, eq = k > 0 && i < n && u == limit;
+    const uint32_t u = i < i1 ? weight_key(w[i]) : 0u;
+    const bool gt = i < i1 && u > limit, eq = i < i1 && u == limit;
     const unsigned bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
     if (lane == 0) {
       s_g[warp] = __popc(bg);
       s_e[warp] = __popc(be);
     }
-    __syncthreads();  // the tile's weights are read, its counts there
+    __syncthreads();
     int g = g0, e = e0;
-    for (int i2 = 0; i2 < 32; ++i2) {
-      if (i2 < warp) {
-        g += s_g[i2];
-        e += s_e[i2];
+#pragma unroll
+    for (int x = 0; x < W; ++x) {
+      if (x < warp) {
+        g += s_g[x];
+        e += s_e[x];
       }
-      g0 += s_g[i2];
-      e0 += s_e[i2];
+      g0 += s_g[x];
+      e0 += s_e[x];
     }
     const unsigned below = (1u << lane) - 1u;
     g += __popc(bg & below);
     e += __popc(be & below);
-    if (gt || (eq && e < need)) {
-      const int at = g + min(e, need);
-      keep[at] = i;
-      wo[at] = x;
-    }
+    if (gt || (eq && e < need)) keep[g + min(e, need)] = i;
     __syncthreads();
   }
-  for (int base = 0; base < recent; base += kEvictThreads) {
-    const int i = base + tid;
-    const float x = i < recent ? w[n + i] : 0.0f;
-    __syncthreads();
-    if (i < recent) {
-      keep[k + i] = n + i;
-      wo[k + i] = x;
-    }
-    __syncthreads();
-  }
-  const int64_t end = in_place ? len : ldwo;
-  for (int64_t i = budget + tid; i < end; i += kEvictThreads) wo[i] = 0.0f;
 }
 
-// One CTA per (sequence, KV head, keys or values): the kept rows move to the front, 16 at a
-// time in order.  A row's place never rises, so a step's rows are read before any row of the
-// step or of a later one is overwritten, and the pages may be the same.
-__global__ void __launch_bounds__(256) k_evict_move(PagedView from, PagedView to, const int* kept, int budget, int D,
-                                                    int* lengths_out) {
+// The kept rows' keys, values and weights, where source and target are apart: grid (pairs, tiles
+// of kMoveRows kept places).  One pass, memory-bound; a row's place is looked up by the threads
+// that move it.
+constexpr int kMoveRows = 64;
+
+struct MoveArgs {
+  PagedView from, to;
+  const int* kept;
+  const float* weights;
+  float* wout;
+  int64_t ldw, ldwo;
+  int budget;
+  int* lengths_out;
+};
+
+// Offset of a sequence's token in a pool, -1 (and the flag) when its page is not in it.
+__device__ __forceinline__ int64_t token_offset(const PagedView& c, int b, int s) {
+  const int at = s / c.page_size;
+  const int page = c.table[b * c.ld_table + at];
+  if (page < 0 || page >= c.n_pages) {
+    report_bad_page();
+    return -1;
+  }
+  return page * c.page_stride + (int64_t)(s - at * c.page_size) * c.token_stride;
+}
+
+__device__ __forceinline__ void set_length(const MoveArgs& a, int b) {
+  const int len = a.from.lengths[b];
+  a.lengths_out[b] = len > a.from.capacity ? len : min(len, a.budget);
+}
+
+template <int D>
+__global__ void __launch_bounds__(256) k_evict_copy(MoveArgs a) {
+  constexpr int P = D / 8, R = 256 / P, N = kMoveRows / R;
+  __shared__ int64_t s_from[kMoveRows], s_to[kMoveRows];
   pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.x / from.kv_heads, g = blockIdx.x - b * from.kv_heads;
-  const uint16_t* src = blockIdx.y ? from.v : from.k;
-  uint16_t* dst = blockIdx.y ? to.v : to.k;
-  const int* keep = kept + (int64_t)blockIdx.x * budget;
-  const int pieces = D / 8, rows = 256 / pieces;
-  const int r = threadIdx.x / pieces, piece = threadIdx.x - r * pieces;
-  for (int base = 0; base < budget; base += rows) {
-    const int j = base + r;
-    const int s = j < budget ? keep[j] : -1;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    bool ok = s >= 0;
-    if (ok) {
-      const int p = from.table[b * from.ld_table + s / from.page_size];
-      ok = p >= 0 && p < from.n_pages;
-      if (ok)
-        x = *reinterpret_cast<const uint4*>(src + p * from.page_stride + (s % from.page_size) * from.token_stride +
-                                            g * from.head_stride + piece * 8);
-    }
-    __syncthreads();
+  const int pair = blockIdx.x, b = pair / a.from.kv_heads, g = pair - b * a.from.kv_heads, tid = threadIdx.x;
+  const int base = blockIdx.y * kMoveRows;
+  const int* keep = a.kept + (int64_t)pair * a.budget;
+  if (a.from.lengths[b] < 0 || a.from.lengths[b] > a.from.capacity) {
+    if (g == 0 && blockIdx.y == 0 && tid == 0) set_length(a, b);
+    return;
+  }
+  if (tid < kMoveRows) {
+    const int j = base + tid, s = j < a.budget ? keep[j] : -1;
+    int64_t x = -1, y = -1;
     if (s >= 0) {
-      const int p = to.table[b * to.ld_table + j / to.page_size];
-      if (p < 0 || p >= to.n_pages) ok = false;
-      if (ok)
-        *reinterpret_cast<uint4*>(dst + p * to.page_stride + (j % to.page_size) * to.token_stride +
-                                  g * to.head_stride + piece * 8) = x;
-      else
-        report_bad_page();
+      a.wout[pair * a.ldwo + j] = a.weights[pair * a.ldw + s];
+      x = token_offset(a.from, b, s);
+      y = token_offset(a.to, b, j);
+    } else if (j < a.budget) {
+      a.wout[pair * a.ldwo + j] = 0.0f;
+    }
+    s_from[tid] = y < 0 ? -1 : x;
+    s_to[tid] = y;
+  }
+  if (blockIdx.y == 0)
+    for (int64_t i = a.budget + tid; i < a.ldwo; i += 256) a.wout[pair * a.ldwo + i] = 0.0f;
+  __syncthreads();
+  const int r = tid / P, piece = tid - r * P;
+  uint4 x[N][2];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int64_t at = s_from[i * R + r];
+    if (at >= 0) {
+      const int64_t o = at + g * a.from.head_stride + piece * 8;
+      x[i][0] = ld_stream16(a.from.k + o);
+      x[i][1] = ld_stream16(a.from.v + o);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (s_from[i * R + r] >= 0) {
+      const int64_t o = s_to[i * R + r] + g * a.to.head_stride + piece * 8;
+      *reinterpret_cast<uint4*>(a.to.k + o) = x[i][0];
+      *reinterpret_cast<uint4*>(a.to.v + o) = x[i][1];
+    }
+  if (g == 0 && blockIdx.y == 0 && tid == 0) set_length(a, b);
+}
+
+// The same in place: a CTA per (pair, keys / values, 64-byte column of the rows), or for a pair's
+// weights, goes through the kept places in order, a tile of 256 at a time.  A row never moves to
+// a higher place, so what a tile overwrites lies before all rows that later tiles read, and
+// the next tile's rows can be requested before this one's are written; only within a tile must
+// every row be read (the barrier) before one is written.  Rows that stay where they are are skipped.
+__global__ void __launch_bounds__(128) k_evict_shift(MoveArgs a, int columns) {
+  constexpr int N = 8, R = 32, T = N * R;  // rows of a thread, of the CTA at once, of a tile
+  pdl_trigger();
+  pdl_wait();
+  const int pair = blockIdx.x, b = pair / a.from.kv_heads, g = pair - b * a.from.kv_heads, tid = threadIdx.x;
+  const int len = a.from.lengths[b];
+  if (len <= a.budget || len > a.from.capacity) return;  // nothing moves
+  const int* keep = a.kept + (int64_t)pair * a.budget;
+  if ((int)blockIdx.y == 2 * columns) {
+    float* w = a.wout + pair * a.ldwo;
+    for (int base = 0; base < a.budget; base += N * 128) {
+      float x[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int j = base + i * 128 + tid;
+        x[i] = j < a.budget ? w[keep[j]] : 0.0f;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int j = base + i * 128 + tid;
+        if (j < a.budget) w[j] = x[i];
+      }
     }
     __syncthreads();
+    for (int i = a.budget + tid; i < len; i += 128) w[i] = 0.0f;
+    return;
   }
-  if (g == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
-    const int len = from.lengths[b];
-    lengths_out[b] = len > from.capacity ? len : min(len, budget);
+  uint16_t* pool = ((int)blockIdx.y < columns ? a.from.k : a.from.v) + g * a.from.head_stride +
+                   ((int)blockIdx.y % columns) * 32 + (tid & 3) * 8;
+  const int r = tid >> 2;
+  struct Rows {
+    uint4 x[N];
+    int64_t to[N];
+  };
+  auto load = [&](int base, Rows& v) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int j = base + i * R + r;
+      const int s = j < a.budget ? keep[j] : j;
+      v.to[i] = -1;
+      if (s != j) {
+        const int64_t at = token_offset(a.from, b, s);
+        if (at >= 0) {
+          v.to[i] = token_offset(a.from, b, j);
+          v.x[i] = *reinterpret_cast<const uint4*>(pool + at);
+        }
+      }
+    }
+  };
+  auto store = [&](const Rows& v) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (v.to[i] >= 0) *reinterpret_cast<uint4*>(pool + v.to[i]) = v.x[i];
+  };
+  Rows even, odd;
+  load(0, even);
+  for (int base = 0; base < a.budget; base += 2 * T) {
+    load(base + T, odd);
+    __syncthreads();
+    store(even);
+    if (base + T >= a.budget) break;
+    load(base + 2 * T, even);
+    __syncthreads();
+    store(odd);
   }
+}
+
+// In place the lengths change when nobody reads them any more.
+__global__ void k_evict_lengths(MoveArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  for (int b = blockIdx.x * blockDim.x + threadIdx.x; b < a.from.batch; b += gridDim.x * blockDim.x) set_length(a, b);
 }
 
 }  // namespace otf
@@ -300,12 +526,32 @@ extern "C" OTF_API int otf_paged_append(const otf_paged_cache* cache, const otf_
   }
   st = check_device();
   if (st != OTF_OK) return st;
-  auto* kern = cache->dtype == OTF_DTYPE_BF16 ? otf::k_paged_append<true> : otf::k_paged_append<false>;
-  return set_cuda_error(otf::launch_pdl(
-      kern, dim3((unsigned)n), dim3(256), 0, static_cast<cudaStream_t>(stream), 1u, c, rot ? rotary->turns : nullptr,
-      rot, rot ? rotary->factor : 1.0f, rot ? (int)rotary->interleaved : 0, static_cast<const uint16_t*>(q), ldq,
-      static_cast<uint16_t*>(q_out), ldqo, (int)heads, static_cast<const uint16_t*>(k), ldk,
-      static_cast<const uint16_t*>(v), ldv, starts, positions, (int)(n / c.batch), (int)D));
+  otf::AppendArgs a = {c,
+                       rot ? rotary->turns : nullptr,
+                       rot,
+                       rot ? (int)(rotary->interleaved != 0) : 0,
+                       rot ? rotary->factor : 1.0f,
+                       static_cast<const uint16_t*>(q),
+                       static_cast<uint16_t*>(q_out),
+                       static_cast<const uint16_t*>(k),
+                       static_cast<const uint16_t*>(v),
+                       ldq,
+                       ldqo,
+                       ldk,
+                       ldv,
+                       q ? (int)heads : 0,
+                       starts,
+                       positions,
+                       (int)(n / c.batch)};
+  const bool bf = cache->dtype == OTF_DTYPE_BF16;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const dim3 grid((unsigned)n);
+  if (rot % 16)
+    return set_cuda_error(otf::launch_pdl(bf ? otf::k_paged_append_any<true> : otf::k_paged_append_any<false>, grid,
+                                          dim3(256), 0, s, 1u, a, (int)D));
+  auto* kern = D == 128 ? (bf ? otf::k_paged_append<true, 128> : otf::k_paged_append<false, 128>)
+                        : (bf ? otf::k_paged_append<true, 64> : otf::k_paged_append<false, 64>);
+  return set_cuda_error(otf::launch_pdl(kern, grid, dim3(otf::kAppendThreads), 0, s, 1u, a));
 }
 
 extern "C" OTF_API int otf_paged_evict(const otf_paged_cache* from, const otf_paged_cache* to, const float* weights,
@@ -323,12 +569,28 @@ extern "C" OTF_API int otf_paged_evict(const otf_paged_cache* from, const otf_pa
   if (ldw < f.capacity || ldw_out < budget || (weights == weights_out && ldw != ldw_out)) return OTF_ERR_INVALID;
   st = check_device();
   if (st != OTF_OK) return st;
+  if (budget > 65535ll * otf::kMoveRows) return OTF_ERR_UNSUPPORTED;
+  // cut in place: the same pools under the same table, and the weights and lengths with them
+  const bool in_place = to->page_table == from->page_table && to->k_pages == from->k_pages && to->v_pages == from->v_pages;
+  if (in_place != (weights == weights_out) || in_place != (lengths_out == from->lengths)) return OTF_ERR_INVALID;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned pairs = (unsigned)(f.batch * f.kv_heads);
-  cudaError_t e = otf::launch_pdl(otf::k_evict_select, dim3(pairs), dim3(otf::kEvictThreads), 0, s, 1u, f.lengths,
-                                  f.kv_heads, f.capacity, weights, ldw, weights_out, ldw_out, (int)budget, (int)recent,
-                                  kept);
+  const int64_t pairs = f.batch * (int64_t)f.kv_heads;
+  // CTAs per (sequence, KV head): one for every kEvictSlice weights that there can be, while that
+  // leaves less than two CTAs per SM
+  int ctas = 1;
+  while (ctas < otf::kEvictCluster && (int64_t)ctas * otf::kEvictSlice < f.capacity && pairs * ctas <= 148) ctas *= 2;
+  cudaError_t e = otf::launch_pdl(otf::k_evict_select, dim3((unsigned)(pairs * ctas)), dim3(otf::kEvictThreads), 0, s,
+                                  (unsigned)ctas, f.lengths, f.kv_heads, f.capacity, weights, ldw, (int)budget,
+                                  (int)recent, kept, ctas);
   if (e != cudaSuccess) return set_cuda_error(e);
-  return set_cuda_error(otf::launch_pdl(otf::k_evict_move, dim3(pairs, 2), dim3(256), 0, s, 1u, f, t,
-                                        (const int*)kept, (int)budget, (int)from->head_dim, lengths_out));
+  const otf::MoveArgs a = {f, t, kept, weights, weights_out, ldw, ldw_out, (int)budget, lengths_out};
+  if (in_place) {
+    const int columns = (int)(from->head_dim / 32);
+    e = otf::launch_pdl(otf::k_evict_shift, dim3((unsigned)pairs, 2 * columns + 1), dim3(128), 0, s, 1u, a, columns);
+    if (e != cudaSuccess) return set_cuda_error(e);
+    return set_cuda_error(otf::launch_pdl(otf::k_evict_lengths, dim3((unsigned)((f.batch + 255) / 256)), dim3(256), 0, s, 1u, a));
+  }
+  const int64_t tiles = (budget + otf::kMoveRows - 1) / otf::kMoveRows;
+  return set_cuda_error(otf::launch_pdl(from->head_dim == 128 ? otf::k_evict_copy<128> : otf::k_evict_copy<64>,
+                                        dim3((unsigned)pairs, (unsigned)tiles), dim3(256), 0, s, 1u, a));
 }

@@ -297,8 +297,9 @@ class PagedKVCache:
             to, weights_out = self, weights
         elif weights_out is None:
             raise ValueError("weights_out is needed with to")
-        elif weights_out.data_ptr() == weights.data_ptr() or to.k_pages.data_ptr() == self.v_pages.data_ptr():
-            raise ValueError("weights_out and to's pages must not be the source's")
+        elif weights_out.data_ptr() == weights.data_ptr() or to.lengths.data_ptr() == self.lengths.data_ptr() or \
+                to.page_table.data_ptr() == self.page_table.data_ptr():
+            raise ValueError("to's table, lengths and weights must not be this cache's (leave to out to cut in place)")
         if (to.batch, to.kv_heads, to.head_dim, to.page_size, to.dtype, to.device) != \
                 (self.batch, self.kv_heads, self.head_dim, self.page_size, self.dtype, self.device):
             raise ValueError("to must have this cache's batch, heads, page size, type and device")
