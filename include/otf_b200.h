@@ -555,7 +555,7 @@ OTF_API int otf_paged_evict(const otf_paged_cache* from, const otf_paged_cache* 
  * with a count or temperature out of range, gets -1 and raises the otf_device_error flag; so
  * does a drafted token outside the vocabulary, which is refused.  Where max(p - q, 0) holds
  * nothing, p is drawn from.  workspace: otf_verify_workspace_bytes(...), 256-byte aligned, need
- * not be cleared, one per call at a time.  Beside otf_i8_head_argmax, the greedy pick of one row.
+ * not be cleared, one per call at a time; at most 65535 sequences.  Beside otf_i8_head_argmax, the greedy pick of one row.
  */
 OTF_API int64_t otf_verify_workspace_bytes(int64_t batch, int64_t drafts, int64_t vocab);
 OTF_API int otf_verify_drafts(const float* target, int64_t target_seq, int64_t ld_target, const float* draft,

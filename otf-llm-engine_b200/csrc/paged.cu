@@ -79,7 +79,8 @@ __device__ __forceinline__ int64_t append_place(const AppendArgs& a, float* s_c,
 // Rotary positions and the cache write, one CTA per row, in units of two 16-byte pieces whose
 // values turn together: pieces i and i + rot / 16 of a head (half layout), or 2i and 2i + 1.
 // Memory-bound: a row is read and written once.  The values are requested before the row's place
-// in the cache and its angles are known, kAppendBatch units at a time.
+// in the cache and its angles are known, kAppendBatch units at a time; a thread has the same i in
+// every head, whose 8 sines and cosines it keeps in registers.
 constexpr int kAppendThreads = 128;
 constexpr int kAppendBatch = 5;
 
@@ -91,56 +92,64 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(AppendArgs a) {
   pdl_wait();
   const PagedView& c = a.c;
   const int64_t row = blockIdx.x;
-  const int nq = a.heads * UH, nk = c.kv_heads * UH, units = nq + 2 * nk, turning = a.rot / 16;
-  const int second = a.interleaved ? 0 : turning;
+  const int heads = a.heads + 2 * c.kv_heads, i = threadIdx.x % UH;
+  const bool turns = i < a.rot / 16, halves = turns && !a.interleaved;
+  const int p0 = halves ? i * 8 : i * 16, p1 = halves ? i * 8 + a.rot / 2 : i * 16 + 8;
+  const int v0 = i * 16;  // values never turn: whole 32-byte units
+  float cs[8], sn[8];
   int64_t at = 0;
-  for (int u0 = 0; u0 < units; u0 += kAppendBatch * kAppendThreads) {
+  constexpr int HC = kAppendThreads / UH;  // heads that the CTA covers at once
+  for (int h0 = 0; h0 < heads; h0 += kAppendBatch * HC) {
     uint4 x[kAppendBatch][2];
 #pragma unroll
     for (int j = 0; j < kAppendBatch; ++j) {
-      const int u = u0 + j * kAppendThreads + threadIdx.x;
-      if (u < units) {
-        const uint16_t* src = u < nq        ? a.q + row * a.ldq + (int64_t)(u / UH) * D
-                              : u < nq + nk ? a.k + row * a.ldk + (int64_t)((u - nq) / UH) * D
-                                            : a.v + row * a.ldv + (int64_t)((u - nq - nk) / UH) * D;
-        const int i = u % UH;
-        const bool halves = second && i < turning && u < nq + nk;
-        x[j][0] = *reinterpret_cast<const uint4*>(src + (halves ? i : 2 * i) * 8);
-        x[j][1] = *reinterpret_cast<const uint4*>(src + (halves ? i + second : 2 * i + 1) * 8);
+      const int h = h0 + j * HC + (int)threadIdx.x / UH;
+      if (h < heads) {
+        const bool is_v = h >= a.heads + c.kv_heads;
+        const uint16_t* src = h < a.heads ? a.q + row * a.ldq + (int64_t)h * D
+                              : is_v      ? a.v + row * a.ldv + (int64_t)(h - a.heads - c.kv_heads) * D
+                                          : a.k + row * a.ldk + (int64_t)(h - a.heads) * D;
+        x[j][0] = *reinterpret_cast<const uint4*>(src + (is_v ? v0 : p0));
+        x[j][1] = *reinterpret_cast<const uint4*>(src + (is_v ? v0 + 8 : p1));
       }
     }
-    if (u0 == 0) {
+    if (h0 == 0) {
       at = append_place(a, s_c, s_s);
       if (at < 0) return;
       __syncthreads();
+      if (turns)
+#pragma unroll
+        for (int z = 0; z < 8; ++z) {
+          cs[z] = s_c[8 * i + z];
+          sn[z] = s_s[8 * i + z];
+        }
     }
 #pragma unroll
     for (int j = 0; j < kAppendBatch; ++j) {
-      const int u = u0 + j * kAppendThreads + threadIdx.x;
-      if (u >= units) break;
-      const int i = u % UH;
-      uint16_t* dst = u < nq        ? a.qo + row * a.ldqo + (int64_t)(u / UH) * D
-                      : u < nq + nk ? c.k + at + (int64_t)((u - nq) / UH) * c.head_stride
-                                    : c.v + at + (int64_t)((u - nq - nk) / UH) * c.head_stride;
-      const bool turn = i < turning && u < nq + nk, halves = second && turn;
-      if (turn) {
-        uint16_t* e = reinterpret_cast<uint16_t*>(x[j]);
+      const int h = h0 + j * HC + (int)threadIdx.x / UH;
+      if (h >= heads) break;
+      const bool is_v = h >= a.heads + c.kv_heads;
+      uint16_t* dst = h < a.heads ? a.qo + row * a.ldqo + (int64_t)h * D
+                      : is_v      ? c.v + at + (int64_t)(h - a.heads - c.kv_heads) * c.head_stride
+                                  : c.k + at + (int64_t)(h - a.heads) * c.head_stride;
+      if (turns && !is_v) {
+        uint32_t* w0 = reinterpret_cast<uint32_t*>(&x[j][0]);
+        uint32_t* w1 = reinterpret_cast<uint32_t*>(&x[j][1]);
 #pragma unroll
-        for (int z = 0; z < 8; ++z) {
-          const float cs = s_c[8 * i + z], sn = s_s[8 * i + z];
-          const float fa = to_f<BF>(halves ? e[z] : e[2 * z]), fb = to_f<BF>(halves ? e[z + 8] : e[2 * z + 1]);
-          const uint16_t ra = from_f<BF>(fa * cs - fb * sn), rb = from_f<BF>(fb * cs + fa * sn);
-          if (halves) {
-            e[z] = ra;
-            e[z + 8] = rb;
-          } else {
-            e[2 * z] = ra;
-            e[2 * z + 1] = rb;
+        for (int z = 0; z < 4; ++z) {
+          if (halves) {  // pairs (w0, w1) place by place
+            const float2 u = unpack2<BF>(w0[z]), v = unpack2<BF>(w1[z]);
+            w0[z] = pack2<BF>(u.x * cs[2 * z] - v.x * sn[2 * z], u.y * cs[2 * z + 1] - v.y * sn[2 * z + 1]);
+            w1[z] = pack2<BF>(v.x * cs[2 * z] + u.x * sn[2 * z], v.y * cs[2 * z + 1] + u.y * sn[2 * z + 1]);
+          } else {       // pairs within a word, four in each piece
+            const float2 u = unpack2<BF>(w0[z]), v = unpack2<BF>(w1[z]);
+            w0[z] = pack2<BF>(u.x * cs[z] - u.y * sn[z], u.y * cs[z] + u.x * sn[z]);
+            w1[z] = pack2<BF>(v.x * cs[z + 4] - v.y * sn[z + 4], v.y * cs[z + 4] + v.x * sn[z + 4]);
           }
         }
       }
-      *reinterpret_cast<uint4*>(dst + (halves ? i : 2 * i) * 8) = x[j][0];
-      *reinterpret_cast<uint4*>(dst + (halves ? i + second : 2 * i + 1) * 8) = x[j][1];
+      *reinterpret_cast<uint4*>(dst + (is_v ? v0 : p0)) = x[j][0];
+      *reinterpret_cast<uint4*>(dst + (is_v ? v0 + 8 : p1)) = x[j][1];
     }
   }
 }
@@ -190,24 +199,28 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 constexpr int kEvictThreads = 512;
+constexpr int kEvictKeys = 16;       // weights of a thread
+constexpr int kEvictStrip = kEvictThreads * kEvictKeys;
 constexpr int kEvictCluster = 8;     // CTAs that may share one (sequence, KV head)
 constexpr int kEvictSlice = 4096;    // weights that a CTA takes before others join it
 
 // Which places stay: a cluster per (sequence, KV head), each CTA a contiguous slice of the n
-// weights that are not among the recent ones.  Four rounds of 8 bits find the k-th largest key
-// (each round: counts of the slice's keys in shared memory, summed over the cluster through
-// distributed shared memory), then every CTA, knowing how many kept keys lie before its slice,
-// writes its places in order.  Of the keys equal to the k-th largest the first ones stay.
-// The weights are read from L2 in every round: latency of the rounds bounds it, not bytes.
+// weights that are not among the recent ones, a thread 16 neighbours.  Four rounds of 8 bits
+// find the k-th largest key (each round: counts of the slice's keys in shared memory, summed over
+// the cluster through distributed shared memory); then every CTA, knowing how many kept keys
+// lie before its slice, writes its places in order.  Of the keys equal to the k-th largest the
+// first ones stay.  Bound by the rounds' latencies, not by bytes: ONE holds the keys of a
+// slice of up to kEvictStrip in registers through all rounds, longer ones are read again (from L2).
+template <bool ONE>
 __global__ void __launch_bounds__(kEvictThreads) k_evict_select(const int* lengths, int kv_heads, int capacity,
                                                                 const float* weights, int64_t ldw, int budget,
                                                                 int recent, int* kept, int ctas) {
-  constexpr int W = kEvictThreads / 32;
+  constexpr int W = kEvictThreads / 32, V = kEvictKeys;
   __shared__ int s_hist[4][256];
   __shared__ int s_sum[256];
-  __shared__ int s_cut[2];       // this round's digit, and how many keys of it are needed
-  __shared__ int s_count[2];     // the slice's keys above and at the limit
-  __shared__ int s_g[W], s_e[W];
+  __shared__ int s_cut[2];    // this round's digit, and how many keys of it are needed
+  __shared__ int s_count[2];  // the slice's keys above and at the limit
+  __shared__ uint32_t s_warp[W];
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -227,7 +240,31 @@ __global__ void __launch_bounds__(kEvictThreads) k_evict_select(const int* lengt
   const int n = len - recent, k = budget - recent;
   for (int i = rank * kEvictThreads + tid; i < recent; i += ctas * kEvictThreads) keep[k + i] = n + i;
   if (k == 0) return;
-  const int per = (n + ctas - 1) / ctas, i0 = min(n, rank * per), i1 = min(n, i0 + per);
+  const int per = ((n + ctas - 1) / ctas + 3) & ~3, i0 = min(n, rank * per), i1 = min(n, i0 + per);
+  const bool aligned = (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+  // this thread's keys of the strip from `base` on: u[0 .. there)
+  uint32_t u[V];
+  auto load = [&](int base) -> int {
+    const int i = base + tid * V, there = max(0, min(V, i1 - i));
+#pragma unroll
+    for (int z = 0; z < V; z += 4) {
+      float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (aligned && z + 4 <= there) {
+        x = *reinterpret_cast<const float4*>(w + i + z);
+      } else {
+        if (z < there) x.x = w[i + z];
+        if (z + 1 < there) x.y = w[i + z + 1];
+        if (z + 2 < there) x.z = w[i + z + 2];
+        if (z + 3 < there) x.w = w[i + z + 3];
+      }
+      u[z] = weight_key(x.x);
+      u[z + 1] = weight_key(x.y);
+      u[z + 2] = weight_key(x.z);
+      u[z + 3] = weight_key(x.w);
+    }
+    return there;
+  };
+  int there = ONE ? load(i0) : 0;
   for (int i = tid; i < 4 * 256; i += kEvictThreads) (&s_hist[0][0])[i] = 0;
   if (tid < 2) s_count[tid] = 0;
   __syncthreads();
@@ -236,10 +273,11 @@ __global__ void __launch_bounds__(kEvictThreads) k_evict_select(const int* lengt
 #pragma unroll 1
   for (int round = 0; round < 4; ++round) {
     const int shift = 24 - 8 * round;
-#pragma unroll 4
-    for (int i = i0 + tid; i < i1; i += kEvictThreads) {
-      const uint32_t u = weight_key(w[i]);
-      if ((u & mask) == limit) atomicAdd(&s_hist[round][(u >> shift) & 255u], 1);
+    for (int base = i0; base < i1; base += kEvictStrip) {
+      if (!ONE) there = load(base);
+#pragma unroll
+      for (int z = 0; z < V; ++z)
+        if (z < there && (u[z] & mask) == limit) atomicAdd(&s_hist[round][(u[z] >> shift) & 255u], 1);
     }
     if (ctas > 1) cluster_sync_all(); else __syncthreads();
     if (tid < 256) {
@@ -265,10 +303,16 @@ __global__ void __launch_bounds__(kEvictThreads) k_evict_select(const int* lengt
       }
       before -= mine;
       if (before < need && before + mine >= need) {
-        int i = 0;
-        while (before + c[i] < need) before += c[i++];
-        s_cut[0] = 255 - 8 * lane - i;
-        s_cut[1] = need - before;
+        bool found = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (!found && before + c[i] >= need) {
+            found = true;
+            s_cut[0] = 255 - 8 * lane - i;
+            s_cut[1] = need - before;
+          }
+          before += c[i];
+        }
       }
     }
     __syncthreads();
@@ -276,54 +320,69 @@ __global__ void __launch_bounds__(kEvictThreads) k_evict_select(const int* lengt
     need = s_cut[1];
     mask |= 255u << shift;
   }
-  int above = 0, equal = 0;
-#pragma unroll 4
-  for (int i = i0 + tid; i < i1; i += kEvictThreads) {
-    const uint32_t u = weight_key(w[i]);
-    above += u > limit;
-    equal += u == limit;
-  }
-  above = __reduce_add_sync(0xffffffffu, above);
-  equal = __reduce_add_sync(0xffffffffu, equal);
-  if (lane == 0) {
-    atomicAdd(&s_count[0], above);
-    atomicAdd(&s_count[1], equal);
-  }
-  int g0 = 0, e0 = 0;  // kept keys above the limit, and keys at it, before this tile
+  // keys above the limit in the low, at it in the high half
+  auto count = [&] {
+    uint32_t c = 0;
+#pragma unroll
+    for (int z = 0; z < V; ++z)
+      if (z < there) c += u[z] > limit ? 1u : u[z] == limit ? 0x10000u : 0u;
+    return c;
+  };
+  uint32_t mine = 0;
+  int g0 = 0, e0 = 0;  // kept keys above the limit, and keys at it, before this strip
   if (ctas > 1) {
+    int above = 0, equal = 0;
+    for (int base = i0; base < i1; base += kEvictStrip) {
+      if (!ONE) there = load(base);
+      mine = count();
+      above += mine & 0xffffu;
+      equal += mine >> 16;
+    }
+    above = __reduce_add_sync(0xffffffffu, above);
+    equal = __reduce_add_sync(0xffffffffu, equal);
+    if (lane == 0) {
+      atomicAdd(&s_count[0], above);
+      atomicAdd(&s_count[1], equal);
+    }
+    __syncwarp();
     cluster_sync_all();
     for (int r = 0; r < rank; ++r) {
       g0 += ld_cluster_s32(mapa_shared(smem_u32(&s_count[0]), r));
       e0 += ld_cluster_s32(mapa_shared(smem_u32(&s_count[1]), r));
     }
-    cluster_sync_all();  // no CTA leaves while another reads its counts
   }
-  for (int base = i0; base < i1; base += kEvictThreads) {
-    const int i = base + tid;
-    const uint32_t u = i < i1 ? weight_key(w[i]) : 0u;
-    const bool gt = i < i1 && u > limit, eq = i < i1 && u == limit;
-    const unsigned bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
-    if (lane == 0) {
-      s_g[warp] = __popc(bg);
-      s_e[warp] = __popc(be);
+  for (int base = i0; base < i1; base += kEvictStrip) {
+    if (!ONE) there = load(base);
+    mine = count();
+    uint32_t inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += x;
     }
+    if (lane == 31) s_warp[warp] = inc;
     __syncthreads();
-    int g = g0, e = e0;
+    uint32_t before = 0, all = 0;
 #pragma unroll
     for (int x = 0; x < W; ++x) {
-      if (x < warp) {
-        g += s_g[x];
-        e += s_e[x];
-      }
-      g0 += s_g[x];
-      e0 += s_e[x];
+      if (x == warp) before = all;
+      all += s_warp[x];
     }
-    const unsigned below = (1u << lane) - 1u;
-    g += __popc(bg & below);
-    e += __popc(be & below);
-    if (gt || (eq && e < need)) keep[g + min(e, need)] = i;
+    before += inc - mine;
+    int g = g0 + (int)(before & 0xffffu), e = e0 + (int)(before >> 16);
+#pragma unroll
+    for (int z = 0; z < V; ++z)
+      if (z < there) {
+        const bool eq = u[z] == limit;
+        if (u[z] > limit || (eq && e < need)) keep[g + min(e, need)] = base + tid * V + z;
+        g += u[z] > limit;
+        e += eq;
+      }
+    g0 += (int)(all & 0xffffu);
+    e0 += (int)(all >> 16);
     __syncthreads();
   }
+  if (ctas > 1) cluster_sync_all();  // no CTA leaves while another reads its counts
 }
 
 // The kept rows' keys, values and weights, where source and target are apart: grid (pairs, tiles
@@ -579,7 +638,8 @@ extern "C" OTF_API int otf_paged_evict(const otf_paged_cache* from, const otf_pa
   // leaves less than two CTAs per SM
   int ctas = 1;
   while (ctas < otf::kEvictCluster && (int64_t)ctas * otf::kEvictSlice < f.capacity && pairs * ctas <= 148) ctas *= 2;
-  cudaError_t e = otf::launch_pdl(otf::k_evict_select, dim3((unsigned)(pairs * ctas)), dim3(otf::kEvictThreads), 0, s,
+  const bool one = (((f.capacity + ctas - 1) / ctas + 3) & ~3) <= otf::kEvictStrip;
+  cudaError_t e = otf::launch_pdl(one ? otf::k_evict_select<true> : otf::k_evict_select<false>, dim3((unsigned)(pairs * ctas)), dim3(otf::kEvictThreads), 0, s,
                                   (unsigned)ctas, f.lengths, f.kv_heads, f.capacity, weights, ldw, (int)budget,
                                   (int)recent, kept, ctas);
   if (e != cudaSuccess) return set_cuda_error(e);

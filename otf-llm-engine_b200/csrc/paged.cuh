@@ -30,6 +30,22 @@ __device__ __forceinline__ uint16_t from_f(float v) {
   return BF ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : f2h(v);
 }
 
+// Two values as they lie next to one another in memory.
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if (BF) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <bool BF>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  return BF ? make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u))
+            : __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // The view of a cache, or why there is none.

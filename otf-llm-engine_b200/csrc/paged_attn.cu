@@ -70,7 +70,8 @@ struct AttnArgs {
   int rep, tokens;     // query heads per KV head, new tokens per sequence
   int rows, blocks;    // rep x tokens rows in so many row blocks
   int64_t* prefix;     // [batch + 1] chunks before each sequence
-  float* part;         // [2 x grid][rows of a block][head_dim + 2]
+  float* part;         // [2 x grid][rows of a block][head_dim]: o of a part
+  float2* part_ml;     // [2 x grid][rows of a block]: its m and l
   float* lse;          // [batch, kv_heads, rows] log2 of the sum, when weights are wanted
   float* scores;       // [batch, kv_heads, rows, ld_scores] likewise
   int64_t ld_scores;
@@ -97,9 +98,20 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t& r0, u
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr) : "memory");
 }
-template <bool BF>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  return (uint32_t)from_f<BF>(lo) | ((uint32_t)from_f<BF>(hi) << 16);
+// PL consecutive values of a row to fp32, and back.
+template <bool BF, int PL>
+__device__ __forceinline__ void load_row(const uint16_t* x, float (&v)[PL]) {
+#pragma unroll
+  for (int i = 0; i < PL / 2; ++i) {
+    const float2 w = unpack2<BF>(reinterpret_cast<const uint32_t*>(x)[i]);
+    v[2 * i] = w.x;
+    v[2 * i + 1] = w.y;
+  }
+}
+template <bool BF, int PL>
+__device__ __forceinline__ void store_row(uint16_t* y, const float (&v)[PL], float f) {
+#pragma unroll
+  for (int i = 0; i < PL / 2; ++i) reinterpret_cast<uint32_t*>(y)[i] = pack2<BF>(v[2 * i] * f, v[2 * i + 1] * f);
 }
 
 // 2^8 on fp16 probabilities: the largest is 256, and what lies 2^-32 below it still counts.
@@ -130,7 +142,8 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
   extern __shared__ __align__(128) unsigned char smem[];
   float* s_m = reinterpret_cast<float*>(smem + kPaWarps * NS * kPaStage);
   float* s_l = s_m + kPaWarps * RB;
-  int* s_len = reinterpret_cast<int*>(s_l + kPaWarps * RB);
+  uint16_t* s_tail = reinterpret_cast<uint16_t*>(s_l + kPaWarps * RB);  // [tokens - 1][keys, values][D]
+  int* s_len = reinterpret_cast<int*>(s_tail + (a.tokens - 1) * 2 * D);
   __shared__ int64_t s_sum[kPaWarps];
   __shared__ Walk s_walk;
   pdl_trigger();
@@ -387,6 +400,21 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
       // The item's end in this run: the warps' parts join, through the stage just read.
       const bool whole = last && begin >= u0;
       float* mine = reinterpret_cast<float*>(smem + warp * NS * kPaStage + slot * kPaStage);
+      if (last)  // the newest tokens, all requested together
+        for (int e = tid; e < (a.tokens - 1) * 2 * (D / 8); e += kPaThreads) {
+          const int piece = e % (D / 8), side = e / (D / 8) & 1, i = e / (D / 4);
+          const int key = len + 1 + i;
+          const uint32_t at = (uint32_t)key / a.page;
+          const int page = c.table[get.b * c.ld_table + at];
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (page >= 0 && page < c.n_pages)
+            x = *reinterpret_cast<const uint4*>((side ? c.v : c.k) + page * c.page_stride +
+                                                (int64_t)(key - (int)(at * a.page.d)) * c.token_stride +
+                                                g * c.head_stride + piece * 8);
+          else
+            report_bad_attn_page();
+          *reinterpret_cast<uint4*>(s_tail + (i * 2 + side) * D + piece * 8) = x;
+        }
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
         __syncwarp();
@@ -430,52 +458,39 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
           const int64_t row = (int64_t)get.b * a.tokens + tok;
           if (last && a.tokens > 1) {  // the newest tokens, as far as this row sees them
             float qv[PL];
-#pragma unroll
-            for (int i = 0; i < PL; ++i) qv[i] = to_f<BF>(a.q[row * a.ldq + (int64_t)head * D + lane * PL + i]);
+            load_row<BF, PL>(a.q + row * a.ldq + (int64_t)head * D + lane * PL, qv);
             float* sc = a.scores ? a.scores + (((int64_t)get.b * c.kv_heads + g) * a.rows + rr) * a.ld_scores : nullptr;
-            for (int key = len + 1; key < len + a.tokens; ++key) {
-              if (key > len + tok) {
-                if (sc && lane == 0) sc[key] = -INFINITY;
+            for (int i = 0; i < a.tokens - 1; ++i) {
+              if (i >= tok) {
+                if (sc && lane == 0) sc[len + 1 + i] = -INFINITY;
                 continue;
               }
-              const uint32_t at = (uint32_t)key / a.page;
-              const int page = c.table[get.b * c.ld_table + at];
-              const bool ok = page >= 0 && page < c.n_pages;
-              if (!ok) report_bad_attn_page();
-              const int64_t off = (ok ? page : 0) * c.page_stride +
-                                  (int64_t)(key - (int)(at * a.page.d)) * c.token_stride + g * c.head_stride + lane * PL;
-              float d = 0.0f, vv[PL];
+              float kv[PL], vv[PL], d = 0.0f;
+              load_row<BF, PL>(s_tail + i * 2 * D + lane * PL, kv);
+              load_row<BF, PL>(s_tail + (i * 2 + 1) * D + lane * PL, vv);
 #pragma unroll
-              for (int i = 0; i < PL; ++i) {
-                d = fmaf(qv[i], ok ? to_f<BF>(c.k[off + i]) : 0.0f, d);
-                vv[i] = ok ? to_f<BF>(c.v[off + i]) : 0.0f;
-              }
+              for (int j = 0; j < PL; ++j) d = fmaf(qv[j], kv[j], d);
 #pragma unroll
               for (int x = 16; x > 0; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
               d *= a.scale;
-              if (sc && lane == 0) sc[key] = d;
+              if (sc && lane == 0) sc[len + 1 + i] = d;
               const float mn = fmaxf(M, d), f = M == -INFINITY ? 0.0f : ex2(M - mn);
               const float pr = d == -INFINITY ? 0.0f : ex2(d - mn + kProbShift<BF>);
               L = L * f + pr;
 #pragma unroll
-              for (int i = 0; i < PL; ++i) acc[i] = acc[i] * f + (d == -INFINITY ? 0.0f : pr * vv[i]);
+              for (int j = 0; j < PL; ++j) acc[j] = acc[j] * f + (d == -INFINITY ? 0.0f : pr * vv[j]);
               M = mn;
             }
           }
           if (whole) {
-            uint16_t* y = a.out + row * a.ldo + (int64_t)head * D + lane * PL;
-#pragma unroll
-            for (int i = 0; i < PL; ++i) y[i] = from_f<BF>(acc[i] / L);
+            store_row<BF, PL>(a.out + row * a.ldo + (int64_t)head * D + lane * PL, acc, 1.0f / L);
             if (a.lse && lane == 0)
               a.lse[((int64_t)get.b * c.kv_heads + g) * a.rows + rr] = M + log2f(L) - kProbShift<BF>;
           } else {
-            float* y = a.part + ((int64_t)(2 * blockIdx.x + (begin >= u0 && begin != u0 ? 1 : 0)) * RB + t * 16 + r) * (D + 2);
+            const int64_t at = (int64_t)(2 * blockIdx.x + (begin > u0 ? 1 : 0)) * RB + t * 16 + r;
 #pragma unroll
-            for (int i = 0; i < PL; ++i) y[2 + lane * PL + i] = acc[i];
-            if (lane == 0) {
-              y[0] = M;
-              y[1] = L;
-            }
+            for (int i = 0; i < PL; ++i) a.part[at * D + lane * PL + i] = acc[i];
+            if (lane == 0) a.part_ml[at] = make_float2(M, L);
           }
         }
         __syncthreads();  // before the stages are filled again, or the next 16 rows come
@@ -501,35 +516,53 @@ __global__ void __launch_bounds__(128) k_paged_attn_join(AttnArgs a, int RB) {
   const int b = blockIdx.x / items, item = blockIdx.x - b * items, g = item / a.blocks, rb = item - g * a.blocks;
   const int lane = threadIdx.x & 31, r = blockIdx.y * 4 + (threadIdx.x >> 5), rr = rb * RB + r;
   if (r >= RB || rr >= a.rows) return;
-  const int64_t p0 = a.prefix[b], n = (a.prefix[b + 1] - p0) / items, total = a.prefix[c.batch];
-  if (n == 0) return;
-  const int64_t c0 = p0 + item * n, c1 = c0 + n;
+  const int64_t p0 = a.prefix[b], p1 = a.prefix[b + 1], total = a.prefix[c.batch];
+  if (p0 == p1) return;
+  // the CTAs whose runs meet the item's chunks [c0, c1): 32-bit divisions where they do
   const int64_t ctas = min((int64_t)kPaGrid, total);
-  const int i0 = (int)(((c0 + 1) * ctas - 1) / total), i1 = (int)((c1 * ctas - 1) / total);
+  int i0, i1, second;
+  if (total < (1 << 23)) {
+    const uint32_t n = (uint32_t)(p1 - p0) / items, c0 = (uint32_t)p0 + item * n, t = (uint32_t)total, u = (uint32_t)ctas;
+    i0 = (int)(((c0 + 1) * u - 1) / t);
+    i1 = (int)(((c0 + n) * u - 1) / t);
+    second = i0 * t / u == c0 ? 0 : 1;
+  } else {
+    const int64_t n = (p1 - p0) / items, c0 = p0 + item * n;
+    i0 = (int)(((c0 + 1) * ctas - 1) / total);
+    i1 = (int)(((c0 + n) * ctas - 1) / total);
+    second = i0 * total / ctas == c0 ? 0 : 1;
+  }
   if (i0 == i1) return;  // one CTA had it whole
-  const int second = i0 * total / ctas == c0 ? 0 : 1;  // the item is not the first of CTA i0's run
-  auto part = [&](int i) { return a.part + ((int64_t)(2 * i + (i == i0 ? second : 0)) * RB + r) * (D + 2); };
-  float M = -INFINITY;
-  for (int i = i0 + lane; i <= i1; i += 32) M = fmaxf(M, part(i)[0]);
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-  float L = 0.0f, acc[PL];
+  // a part is the first of its CTA's run, but the item's first part may be the second of one
+  auto part = [&](int i) { return (int64_t)(2 * i + (i == i0 ? second : 0)) * RB + r; };
+  float M = -INFINITY, L = 0.0f, acc[PL];
 #pragma unroll
   for (int i = 0; i < PL; ++i) acc[i] = 0.0f;
-#pragma unroll 4
-  for (int i = i0; i <= i1; ++i) {
-    const float* x = part(i);
-    const float li = x[1], f = li == 0.0f ? 0.0f : ex2(x[0] - M);
-    if (li != 0.0f) {
-      L = fmaf(li, f, L);
+  for (int i = i0 + lane; i <= i1; i += 32) M = fmaxf(M, a.part_ml[part(i)].x);
 #pragma unroll
-      for (int j = 0; j < PL; ++j) acc[j] = fmaf(x[2 + lane * PL + j], f, acc[j]);
+  for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+  for (int base = i0; base <= i1; base += 32) {
+    float f = 0.0f;  // a lane holds one part's factor
+    if (base + lane <= i1) {
+      const float2 ml = a.part_ml[part(base + lane)];
+      if (ml.y != 0.0f) {
+        f = ex2(ml.x - M);
+        L = fmaf(ml.y, f, L);
+      }
+    }
+    const int n = min(32, i1 + 1 - base);
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const float w = __shfl_sync(0xffffffffu, f, i);
+      const float* x = a.part + part(base + i) * D + lane * PL;
+#pragma unroll
+      for (int j = 0; j < PL; ++j) acc[j] = fmaf(x[j], w, acc[j]);
     }
   }
-  const int tok = rr / a.rep, head = g * a.rep + rr - tok * a.rep;
-  uint16_t* y = a.out + ((int64_t)b * a.tokens + tok) * a.ldo + (int64_t)head * D + lane * PL;
 #pragma unroll
-  for (int i = 0; i < PL; ++i) y[i] = from_f<BF>(acc[i] / L);
+  for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+  const int tok = rr / a.rep, head = g * a.rep + rr - tok * a.rep;
+  store_row<BF, PL>(a.out + ((int64_t)b * a.tokens + tok) * a.ldo + (int64_t)head * D + lane * PL, acc, 1.0f / L);
   if (a.lse && lane == 0) a.lse[((int64_t)b * c.kv_heads + g) * a.rows + rr] = M + log2f(L) - kProbShift<BF>;
 }
 
@@ -555,15 +588,16 @@ __global__ void __launch_bounds__(256) k_paged_attn_weights(AttnArgs a, float* w
 
 // Bytes of the workspace's parts, in order.
 struct AttnSpace {
-  int64_t prefix, part, lse, scores, ld_scores;
-  int64_t bytes() const { return prefix + part + lse + scores; }
+  int64_t prefix, part, part_ml, lse, scores, ld_scores;
+  int64_t bytes() const { return prefix + part + part_ml + lse + scores; }
 };
 static AttnSpace attn_space(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t tokens, int64_t max_tokens,
                             bool weights) {
   AttnSpace s;
   const int64_t rows = heads / kv_heads * tokens, RB = rows <= 16 ? 16 : 32;
   s.prefix = align_up((batch + 1) * 8, 256);
-  s.part = align_up(2 * kPaGrid * RB * (D + 2) * 4, 256);
+  s.part = align_up(2 * kPaGrid * RB * D * 4, 256);
+  s.part_ml = align_up(2 * kPaGrid * RB * 8, 256);
   s.ld_scores = align_up(max_tokens, 8);
   s.lse = weights ? align_up(batch * kv_heads * rows * 4, 256) : 0;
   s.scores = weights ? align_up(batch * kv_heads * rows * s.ld_scores * 4, 256) : 0;
@@ -574,7 +608,8 @@ template <bool BF, int D>
 static cudaError_t launch_attn(const AttnArgs& a, float* weights, int64_t ldw, cudaStream_t s) {
   const int RB = a.rows <= 16 ? 16 : 32;
   auto* k = RB == 16 ? k_paged_attn<BF, D, 1> : k_paged_attn<BF, D, 2>;
-  const size_t dyn = (size_t)kPaWarps * kPaStages * kPaStage + (size_t)kPaWarps * RB * 8 + (size_t)a.c.batch * 4;
+  const size_t dyn = (size_t)kPaWarps * kPaStages * kPaStage + (size_t)kPaWarps * RB * 8 +
+                     (size_t)(a.tokens - 1) * 4 * D + (size_t)a.c.batch * 4;
   {
     // the shared-memory opt-in, once per kernel and device, for the largest batch
     static std::mutex mu;
@@ -586,7 +621,8 @@ static cudaError_t launch_attn(const AttnArgs& a, float* weights, int64_t ldw, c
     bool& have = done[std::make_pair(reinterpret_cast<const void*>(k), dev)];
     if (!have) {
       e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               kPaWarps * kPaStages * kPaStage + kPaWarps * 32 * 8 + kPagedMaxBatch * 4);
+                               kPaWarps * kPaStages * kPaStage + kPaWarps * 32 * 8 + (kPagedMaxTokens - 1) * 4 * D +
+                                   kPagedMaxBatch * 4);
       if (e != cudaSuccess) return e;
       have = true;
     }
@@ -656,10 +692,12 @@ extern "C" OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* 
   a.blocks = a.rows <= 16 ? 1 : (a.rows + 31) / 32;
   char* w = static_cast<char*>(workspace);
   a.prefix = reinterpret_cast<int64_t*>(w);
-  a.part = reinterpret_cast<float*>(w + space.prefix);
+  a.part = reinterpret_cast<float*>(w += space.prefix);
+  a.part_ml = reinterpret_cast<float2*>(w += space.part);
+  w += space.part_ml;
   if (weights) {
-    a.lse = reinterpret_cast<float*>(w + space.prefix + space.part);
-    a.scores = reinterpret_cast<float*>(w + space.prefix + space.part + space.lse);
+    a.lse = reinterpret_cast<float*>(w);
+    a.scores = reinterpret_cast<float*>(w + space.lse);
     a.ld_scores = space.ld_scores;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -30,6 +30,12 @@ struct __align__(16) RowPart {
   int at, pad;
 };
 
+// What the draw of a sequence needs: the row it is of, the rows' maxima and 1 / sums, log2(e) / T.
+struct __align__(16) Pick {
+  int taken, refused, drafted, out_of;  // taken -1: nothing to draw
+  float xm, xi, ym, yi, c_hi, c_lo, pad[2];
+};
+
 // exp(d / T) for d <= 0, with c = log2(e) / T in two floats: the exponent is split into its
 // nearest whole number and a rest that keeps the product's low bits, so that the relative error
 // stays near 2^-22 for small results too (d c alone, rounded, is off by d c 2^-24).
@@ -48,10 +54,6 @@ __device__ __forceinline__ float ex2(float x) {
 // 0, or from 1e-20 on (log2(e) / T and its product with a difference of logits stay finite).
 __host__ __device__ __forceinline__ bool temperature_ok(float T) { return T == 0.0f || (T >= 1e-20f && T <= 1e20f); }
 
-__device__ __forceinline__ float temperature_of(const float* temperatures, float temperature, int b) {
-  return temperatures ? temperatures[b] : temperature;
-}
-
 // Four consecutive logits of a row, -inf behind its end.  Rows that are not 16-byte aligned are read
 // value by value by the same threads, so that a row's sums do not depend on where it lies.
 __device__ __forceinline__ float4 logits4(const float* x, int i, int end, bool aligned) {
@@ -64,161 +66,180 @@ __device__ __forceinline__ float4 logits4(const float* x, int i, int end, bool a
   return v;
 }
 
-// One pass over the logits: grid (segments, rows), the rows being the batch x (drafts + 1) of the
-// target, then the draft's.  A thread holds its 32 values in registers: their maximum, then the
-// sum of exponentials under it, joined over the CTA.  Memory-bound, 5 instructions per logit.
-__global__ void __launch_bounds__(kVerifyThreads) k_verify_rows(const float* target, int64_t tseq, int64_t ldt,
-                                                                const float* draft, int64_t dseq, int64_t ldd,
-                                                                const float* temperatures, float temperature,
-                                                                const int* counts, int batch, int drafts, int vocab,
-                                                                RowPart* parts) {
+// The logits' place, and what every kernel asks about a sequence.
+struct VerifyArgs {
+  const float* target;
+  const float* draft;  // or null
+  int64_t tseq, ldt, dseq, ldd;
+  const int64_t* tokens;
+  int64_t ldtok;
+  const float* uniforms;
+  int64_t ldu;
+  const float* noise;
+  int64_t ldn;
+  const float* temperatures;
+  float temperature;
+  const int* counts;
+  int64_t* out;
+  int* accepted;
+  int drafts, vocab, segs;
+  RowPart* parts;  // [batch][2 drafts + 1: the target's rows, then the draft's][segs]
+  Pick* picks;     // [batch]
+
+  __device__ __forceinline__ float temp(int b) const { return temperatures ? temperatures[b] : temperature; }
+  __device__ __forceinline__ int count(int b) const { return counts ? counts[b] : drafts; }
+  // row r of the count + 1 target rows and then count draft rows that sequence b needs
+  __device__ __forceinline__ int rows(int b, int n, float T) const {
+    return n < 0 || n > drafts ? 0 : n + 1 + (draft && T > 0.0f ? n : 0);
+  }
+  __device__ __forceinline__ const float* row(int b, int n, int r) const {
+    return r <= n ? target + b * tseq + r * ldt : draft + b * dseq + (r - n - 1) * ldd;
+  }
+  __device__ __forceinline__ int64_t part(int b, int n, int r) const {
+    return ((int64_t)b * (2 * drafts + 1) + (r <= n ? r : drafts + r - n)) * segs;
+  }
+};
+
+// One pass over the logits: grid (segments, row groups, batch).  A thread holds its 32 values of a row's
+// segment in registers: their maximum, then the sum of exponentials under it, joined over the CTA.
+// Memory-bound, 7 instructions per logit.  A CTA goes through its group's rows, so that rows that
+// a sequence with fewer drafted tokens does not have cost nothing.
+__global__ void __launch_bounds__(kVerifyThreads) k_verify_rows(VerifyArgs a) {
   constexpr int N = kVerifySeg / (4 * kVerifyThreads), W = kVerifyThreads / 32;
   __shared__ float s_m[W], s_s[W];
   __shared__ int s_i[W];
   pdl_trigger();
   pdl_wait();
-  const int row = blockIdx.y, trows = batch * (drafts + 1);
-  const bool of_target = row < trows;
-  const int per = of_target ? drafts + 1 : drafts;
-  const int r = of_target ? row : row - trows;
-  const int b = r / per, j = r - b * per;
-  const float T = temperature_of(temperatures, temperature, b);
-  const int count = counts ? counts[b] : drafts;
-  if (of_target ? j > count : (j >= count || T == 0.0f)) return;  // a row that nothing asks for
-  const float* x = of_target ? target + b * tseq + j * ldt : draft + b * dseq + j * ldd;
-  const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  const int b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float T = a.temp(b);
+  const int n = a.count(b), rows = a.rows(b, n, T);
   const int i0 = blockIdx.x * kVerifySeg + 4 * threadIdx.x;
-  float4 v[N];
-#pragma unroll
-  for (int z = 0; z < N; ++z) v[z] = logits4(x, i0 + z * 4 * kVerifyThreads, vocab, aligned);
-  float m = -INFINITY;  // a NaN is never the largest
-#pragma unroll
-  for (int z = 0; z < N; ++z) m = fmaxf(m, fmaxf(fmaxf(v[z].x, v[z].y), fmaxf(v[z].z, v[z].w)));
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float s = 0.0f;
-  int at = INT_MAX;
-  if (T == 0.0f) {
-#pragma unroll
-    for (int z = N - 1; z >= 0; --z) {
-      const float e[4] = {v[z].x, v[z].y, v[z].z, v[z].w};
-#pragma unroll
-      for (int w = 3; w >= 0; --w) {
-        const int i = i0 + z * 4 * kVerifyThreads + w;
-        if (e[w] == m && i < vocab) at = i;
-      }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
-      const int a2 = __shfl_xor_sync(0xffffffffu, at, o);
-      if (m2 > m || (m2 == m && a2 < at)) {
-        m = m2;
-        at = a2;
-      }
-    }
-    if (lane == 0) {
-      s_m[warp] = m;
-      s_i[warp] = at;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int w = 1; w < W; ++w)
-        if (s_m[w] > m || (s_m[w] == m && s_i[w] < at)) {
-          m = s_m[w];
-          at = s_i[w];
-        }
-      parts[(int64_t)row * gridDim.x + blockIdx.x] = RowPart{m, 0.0f, at, 0};
-    }
-    return;
-  }
   const float c_hi = (float)(1.4426950408889634 / (double)T);
   const float c_lo = (float)(1.4426950408889634 / (double)T - (double)c_hi);
   auto term = [&](float x, float max) {  // 0 for -inf and NaN (the maximum drops a NaN)
     const float d = x - max;
     return ex2(fmaxf(fmaf(d, c_hi, d * c_lo), -200.0f));
   };
-  const float mt = m == -INFINITY ? 0.0f : m;  // nothing but -inf: the sum is 0
+  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+    const float* x = a.row(b, n, r);
+    RowPart* to = a.parts + a.part(b, n, r) + blockIdx.x;
+    const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+    float4 v[N];
 #pragma unroll
-  for (int z = 0; z < N; ++z)
-    if (i0 + z * 4 * kVerifyThreads < vocab)
-      s += (term(v[z].x, mt) + term(v[z].y, mt)) + (term(v[z].z, mt) + term(v[z].w, mt));
-  auto join = [&](float m2, float s2) {
-    const float M = fmaxf(m, m2);
-    if (M != -INFINITY) s = s * term(m, M) + s2 * term(m2, M);  // else both are 0
-    m = M;
-  };
+    for (int z = 0; z < N; ++z) v[z] = logits4(x, i0 + z * 4 * kVerifyThreads, a.vocab, aligned);
+    float m = -INFINITY;  // a NaN is never the largest
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-    join(m2, s2);
-  }
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_s[warp] = s;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < W; ++w) join(s_m[w], s_s[w]);
-    parts[(int64_t)row * gridDim.x + blockIdx.x] = RowPart{m, s, INT_MAX, 0};
+    for (int z = 0; z < N; ++z) m = fmaxf(m, fmaxf(fmaxf(v[z].x, v[z].y), fmaxf(v[z].z, v[z].w)));
+    if (T == 0.0f) {
+      int at = INT_MAX;
+#pragma unroll
+      for (int z = N - 1; z >= 0; --z) {
+        const float e[4] = {v[z].x, v[z].y, v[z].z, v[z].w};
+#pragma unroll
+        for (int w = 3; w >= 0; --w) {
+          const int i = i0 + z * 4 * kVerifyThreads + w;
+          if (e[w] == m && i < a.vocab) at = i;
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
+        const int a2 = __shfl_xor_sync(0xffffffffu, at, o);
+        if (m2 > m || (m2 == m && a2 < at)) {
+          m = m2;
+          at = a2;
+        }
+      }
+      __syncthreads();  // the row before is done with
+      if (lane == 0) {
+        s_m[warp] = m;
+        s_i[warp] = at;
+      }
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        for (int w = 1; w < W; ++w)
+          if (s_m[w] > m || (s_m[w] == m && s_i[w] < at)) {
+            m = s_m[w];
+            at = s_i[w];
+          }
+        *to = RowPart{m, 0.0f, at, 0};
+      }
+      continue;
+    }
+    const float mt = m == -INFINITY ? 0.0f : m;  // nothing but -inf: the sum is 0
+    float s = 0.0f;
+#pragma unroll
+    for (int z = 0; z < N; ++z)
+      if (i0 + z * 4 * kVerifyThreads < a.vocab)
+        s += (term(v[z].x, mt) + term(v[z].y, mt)) + (term(v[z].z, mt) + term(v[z].w, mt));
+    auto join = [&](float m2, float s2) {
+      const float M = fmaxf(m, m2);
+      if (M != -INFINITY) s = s * term(m, M) + s2 * term(m2, M);  // else both are 0
+      m = M;
+    };
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+      join(m2, s2);
+    }
+    __syncthreads();
+    if (lane == 0) {
+      s_m[warp] = m;
+      s_s[warp] = s;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < W; ++w) join(s_m[w], s_s[w]);
+      *to = RowPart{m, s, INT_MAX, 0};
+    }
   }
 }
 
-// A race's leader: the largest w / e and its index, of what the draft leaves of p and of p itself.
-struct Leader {
-  float best[2];
-  int at[2];
-  __device__ __forceinline__ void take(int z, float score, int i) {
-    if (score > best[z] || (score == best[z] && i < at[z])) {
-      best[z] = score;
-      at[z] = i;
-    }
+__device__ __forceinline__ void write_tokens(const VerifyArgs& a, int b, int taken, int64_t last, int tid, int threads) {
+  for (int j = tid; j <= a.drafts; j += threads)
+    a.out[(int64_t)b * (a.drafts + 1) + j] = last < 0 || j > taken ? -1 : j < taken ? a.tokens[b * a.ldtok + j] : last;
+  if (tid == 0) {
+    a.accepted[b] = last < 0 ? 0 : taken;
+    if (last < 0) atomicExch(&g_verify_device_error, 1);
   }
-};
+}
 
-// A cluster of kPickCluster CTAs per sequence.  Every CTA joins the rows' parts and follows the
-// drafted tokens (a few hundred numbers); the race over the vocabulary is cut among them, and
-// their leaders meet in rank 0 through distributed shared memory.
-constexpr int kPickCluster = 8;
-constexpr int kPickThreads = 512;
-
-__global__ void __launch_bounds__(kPickThreads) k_verify_pick(const float* target, int64_t tseq, int64_t ldt,
-                                                              const float* draft, int64_t dseq, int64_t ldd,
-                                                              const int64_t* tokens, int64_t ldtok, const float* uniforms,
-                                                              int64_t ldu, const float* noise, int64_t ldn,
-                                                              const float* temperatures, float temperature, const int* counts,
-                                                              int64_t* out, int* accepted, int batch, int drafts, int vocab,
-                                                              const RowPart* parts, int segs) {
-  constexpr int W = kPickThreads / 32;
+// A CTA per sequence: the rows' parts joined (a warp per row), the drafted tokens followed, and what
+// the draw needs left in picks[b]; with temperature 0 that is all.  Latency-bound: the tokens and
+// their logits are requested before the parts are joined.
+__global__ void __launch_bounds__(256) k_verify_pick(VerifyArgs a) {
   __shared__ double s_sum[2 * kVerifyMaxDrafts + 1];
   __shared__ float s_max[2 * kVerifyMaxDrafts + 1];
   __shared__ int s_at[kVerifyMaxDrafts + 1];
-  __shared__ int s_taken;
-  __shared__ __align__(16) Leader s_lead[W];
-  __shared__ __align__(16) Leader s_all[kPickCluster];
   pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.x / kPickCluster, rank = (int)cluster_ctarank(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const float T = temperature_of(temperatures, temperature, b);
-  const int count = counts ? counts[b] : drafts;
-  if (count < 0 || count > drafts || !temperature_ok(T) || (T > 0.0f && (!noise || (count && !uniforms)))) {
-    if (rank) return;  // as all the others do
-    for (int j = tid; j <= drafts; j += kPickThreads) out[(int64_t)b * (drafts + 1) + j] = -1;
-    if (tid == 0) {
-      accepted[b] = 0;
-      atomicExch(&g_verify_device_error, 1);
-    }
+  const int b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const float T = a.temp(b);
+  const int n = a.count(b), rows = a.rows(b, n, T);
+  if (rows == 0 || !temperature_ok(T) || (T > 0.0f && (!a.noise || (n && !a.uniforms)))) {
+    if (tid == 0) a.picks[b].taken = -1;
+    write_tokens(a, b, 0, -1, tid, 256);
     return;
   }
-  if (T == 0.0f && rank) return;  // no race
-  const bool drafted = draft != nullptr && T > 0.0f;
-  for (int r = warp; r < count + 1 + (drafted ? count : 0); r += W) {
-    const int64_t row = r <= count ? (int64_t)b * (drafts + 1) + r
-                                   : (int64_t)batch * (drafts + 1) + (int64_t)b * drafts + (r - count - 1);
-    const RowPart* p = parts + row * segs;
+  const bool drafted = rows > n + 1;
+  float xd = 0.0f, yd = 0.0f, u = 0.0f;
+  int64_t d = -1;
+  if (warp == 0 && lane < n) {
+    d = a.tokens[b * a.ldtok + lane];
+    if (d >= 0 && d < a.vocab && T > 0.0f) {
+      xd = a.target[b * a.tseq + lane * a.ldt + d];
+      if (drafted) yd = a.draft[b * a.dseq + lane * a.ldd + d];
+      u = a.uniforms[b * a.ldu + lane];
+    }
+  }
+  for (int r = warp; r < rows; r += 8) {
+    const RowPart* p = a.parts + a.part(b, n, r);
     float m = -INFINITY;
     int at = INT_MAX;
-    for (int i = lane; i < segs; i += 32) {
-      const RowPart q = p[i];
+    RowPart first = {-INFINITY, 0.0f, INT_MAX, 0};
+    if (lane < a.segs) first = p[lane];
+    for (int i = lane; i < a.segs; i += 32) {
+      const RowPart q = i == lane ? first : p[i];
       if (q.max > m || (q.max == m && q.at < at)) {
         m = q.max;
         at = q.at;
@@ -235,110 +256,154 @@ __global__ void __launch_bounds__(kPickThreads) k_verify_pick(const float* targe
     }
     double s = 0.0;
     if (T > 0.0f)
-      for (int i = lane; i < segs; i += 32) {
-        const RowPart q = p[i];
+      for (int i = lane; i < a.segs; i += 32) {
+        const RowPart q = i == lane ? first : p[i];
         if (q.sum != 0.0f) s += (double)q.sum * exp(((double)q.max - (double)m) / (double)T);
       }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (lane == 0) {
-      const int to = r <= count ? r : drafts + 1 + (r - count - 1);
+      const int to = r <= n ? r : a.drafts + r - n;
       s_max[to] = m;
       s_sum[to] = s;
-      if (r <= count) s_at[r] = at;
+      if (r <= n) s_at[r] = at;
     }
   }
   __syncthreads();
-  if (warp == 0) {
-    bool take = false;
-    if (lane < count) {
-      const int64_t d = tokens[b * ldtok + lane];
-      if (d < 0 || d >= vocab) {
-        if (rank == 0) atomicExch(&g_verify_device_error, 1);
-      } else if (T == 0.0f) {
-        take = d == s_at[lane];
-      } else {
-        const double p = exp(((double)target[b * tseq + lane * ldt + d] - (double)s_max[lane]) / (double)T) / s_sum[lane];
-        double q = 1.0;
-        if (drafted)
-          q = exp(((double)draft[b * dseq + lane * ldd + d] - (double)s_max[drafts + 1 + lane]) / (double)T) /
-              s_sum[drafts + 1 + lane];
+  if (warp) return;
+  bool take = false;
+  if (lane < n) {
+    if (d < 0 || d >= a.vocab) {
+      atomicExch(&g_verify_device_error, 1);
+    } else if (T == 0.0f) {
+      take = d == s_at[lane];
+    } else {
+      const double p = exp(((double)xd - (double)s_max[lane]) / (double)T) / s_sum[lane];
+      double q = 1.0;
+      if (drafted) {
+        q = exp(((double)yd - (double)s_max[a.drafts + 1 + lane]) / (double)T) / s_sum[a.drafts + 1 + lane];
         if (!(q >= 0.0)) q = 0.0;  // a NaN
-        take = (double)uniforms[b * ldu + lane] * q < p;
       }
+      take = (double)u * q < p;
     }
-    const unsigned no = ~__ballot_sync(0xffffffffu, take);
-    if (lane == 0) s_taken = no ? __ffs((int)no) - 1 : 32;
   }
-  __syncthreads();
-  const int taken = min(s_taken, count);
-  int64_t last = -1;
+  const unsigned no = ~__ballot_sync(0xffffffffu, take);
+  const int taken = no ? min(__ffs((int)no) - 1, n) : n;
   if (T == 0.0f) {
-    last = s_at[taken] == INT_MAX ? -1 : s_at[taken];
-  } else {
-    const bool refused = taken < count;
-    const float* x = target + b * tseq + taken * ldt;
-    const float* y = drafted && refused ? draft + b * dseq + taken * ldd : nullptr;
-    const float* e = noise + b * ldn;
-    const bool ax = (reinterpret_cast<uintptr_t>(x) & 15) == 0, ay = (reinterpret_cast<uintptr_t>(y) & 15) == 0,
-               ae = (reinterpret_cast<uintptr_t>(e) & 15) == 0;
-    const float xm = s_max[taken], xi = (float)(1.0 / s_sum[taken]);
-    const float ym = y ? s_max[drafts + 1 + taken] : 0.0f, yi = y ? (float)(1.0 / s_sum[drafts + 1 + taken]) : 0.0f;
-    const int64_t out_of = refused && !drafted ? tokens[b * ldtok + taken] : -1;
-    const float c_hi = (float)(1.4426950408889634 / (double)T);
-    const float c_lo = (float)(1.4426950408889634 / (double)T - (double)c_hi);
-    Leader lead = {{0.0f, 0.0f}, {INT_MAX, INT_MAX}};
-    for (int i = 4 * (rank * kPickThreads + tid); i < vocab; i += 4 * kPickThreads * kPickCluster) {
-      const float4 vx = logits4(x, i, vocab, ax), ve = logits4(e, i, vocab, ae);
+    write_tokens(a, b, taken, s_at[taken] == INT_MAX ? -1 : s_at[taken], lane, 32);
+    if (lane == 0) a.picks[b].taken = -1;
+    return;
+  }
+  const bool refused = taken < n;
+  const int64_t out_of = __shfl_sync(0xffffffffu, d, min(taken, 31));
+  if (lane == 0) {
+    Pick k;
+    k.taken = taken;
+    k.refused = refused;
+    k.drafted = drafted && refused;
+    k.out_of = refused && !drafted && out_of >= 0 && out_of < a.vocab ? (int)out_of : -1;
+    k.xm = s_max[taken];
+    k.xi = (float)(1.0 / s_sum[taken]);
+    k.ym = k.drafted ? s_max[a.drafts + 1 + taken] : 0.0f;
+    k.yi = k.drafted ? (float)(1.0 / s_sum[a.drafts + 1 + taken]) : 0.0f;
+    const double c = 1.4426950408889634 / (double)T;
+    k.c_hi = (float)c;
+    k.c_lo = (float)(c - (double)k.c_hi);
+    a.picks[b] = k;
+  }
+}
+
+// The leader of the race: the largest w / e, and its index.
+struct __align__(8) Leader {
+  float best;
+  int at;
+  __device__ __forceinline__ void take(float score, int i) {
+    if (score > best || (score == best && i < at)) {
+      best = score;
+      at = i;
+    }
+  }
+};
+
+// The draw: a cluster of kRaceCluster CTAs per sequence, the vocabulary cut among them, their leaders
+// exchanged through distributed shared memory.  An entry is weighed with the hardware's exponential
+// first, whose error is far below the margin 2^-16; only what may beat its warp's leader by then is
+// computed with care (some 10 entries of a warp), so the loop stays near 25 instructions per entry.
+constexpr int kRaceCluster = 8;
+constexpr int kRaceThreads = 256;
+
+__global__ void __launch_bounds__(kRaceThreads) k_verify_race(VerifyArgs a) {
+  constexpr int W = kRaceThreads / 32;
+  __shared__ Leader s_lead[W];
+  __shared__ Leader s_all[2][kRaceCluster];
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.x / kRaceCluster, rank = (int)cluster_ctarank(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Pick k = a.picks[b];
+  if (k.taken < 0) return;  // done already; the whole cluster returns
+  cluster_arrive_relaxed();
+  const float* x = a.target + b * a.tseq + k.taken * a.ldt;
+  const float* e = a.noise + b * a.ldn;
+  const bool ax = (reinterpret_cast<uintptr_t>(x) & 15) == 0, ae = (reinterpret_cast<uintptr_t>(e) & 15) == 0;
+  const float* y = k.drafted ? a.draft + b * a.dseq + k.taken * a.ldd : nullptr;
+  int out_of = k.out_of;
+  int64_t last = -1;
+  for (int pass = 0;; ++pass) {  // a second one where nothing of p - q is left: p itself
+    const bool ay = (reinterpret_cast<uintptr_t>(y) & 15) == 0;
+    Leader lead = {0.0f, INT_MAX};
+    float bar = 0.0f;  // the warp's leader
+#pragma unroll 4
+    for (int i0 = 4 * (rank * kRaceThreads + warp * 32); i0 < a.vocab; i0 += 4 * kRaceThreads * kRaceCluster) {
+      const int i = i0 + 4 * lane;
+      const float4 vx = logits4(x, i, a.vocab, ax), ve = logits4(e, i, a.vocab, ae);
       float4 vy = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (y) vy = logits4(y, i, vocab, ay);
+      if (y) vy = logits4(y, i, a.vocab, ay);
       const float fx[4] = {vx.x, vx.y, vx.z, vx.w}, fy[4] = {vy.x, vy.y, vy.z, vy.w}, fe[4] = {ve.x, ve.y, ve.z, ve.w};
+      bool may[4], any = false;
 #pragma unroll
       for (int z = 0; z < 4; ++z) {
-        // products that round by themselves: equal rows leave exactly nothing
-        const float p = __fmul_rn(exp_scaled(fx[z] - xm, c_hi, c_lo), xi);
-        float left = p;
-        if (y) left = __fsub_rn(p, __fmul_rn(exp_scaled(fy[z] - ym, c_hi, c_lo), yi));
-        if (i + z == out_of) left = 0.0f;
-        if (i + z < vocab && p > 0.0f) {
-          lead.take(1, p / fe[z], i + z);
-          if (left > 0.0f) lead.take(0, left / fe[z], i + z);
-        }
+        const float dx = fx[z] - k.xm, dy = fy[z] - k.ym;
+        const float p = ex2(fmaxf(fmaf(dx, k.c_hi, dx * k.c_lo), -200.0f)) * k.xi;
+        float q = 0.0f;
+        if (y) q = ex2(fmaxf(fmaf(dy, k.c_hi, dy * k.c_lo), -200.0f)) * k.yi;
+        may[z] = fmaf(p + q, 0x1p-16f, p - q) > bar * fe[z] && i + z != out_of && i + z < a.vocab;
+        any |= may[z];
+      }
+      if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+        for (int z = 0; z < 4; ++z)
+          if (may[z]) {
+            // products that round by themselves: equal rows leave exactly nothing
+            float w = __fmul_rn(exp_scaled(fx[z] - k.xm, k.c_hi, k.c_lo), k.xi);
+            if (y) w = __fsub_rn(w, __fmul_rn(exp_scaled(fy[z] - k.ym, k.c_hi, k.c_lo), k.yi));
+            if (w > 0.0f) lead.take(w / fe[z], i + z);
+          }
+        bar = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(lead.best)));
       }
     }
 #pragma unroll
-    for (int z = 0; z < 2; ++z) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const float s2 = __shfl_xor_sync(0xffffffffu, lead.best[z], o);
-        const int i2 = __shfl_xor_sync(0xffffffffu, lead.at[z], o);
-        lead.take(z, s2, i2);
-      }
+    for (int o = 16; o > 0; o >>= 1) {
+      const float s2 = __shfl_xor_sync(0xffffffffu, lead.best, o);
+      const int i2 = __shfl_xor_sync(0xffffffffu, lead.at, o);
+      lead.take(s2, i2);
     }
     if (lane == 0) s_lead[warp] = lead;
     __syncthreads();
-    cluster_sync_all();  // rank 0 runs
-    if (tid == 0) {
-      for (int w = 1; w < W; ++w)
-        for (int z = 0; z < 2; ++z) lead.take(z, s_lead[w].best[z], s_lead[w].at[z]);
-      const uint32_t to = mapa_shared(smem_u32(&s_all[rank]), 0);
-      st_cluster_v2(to, __float_as_uint(lead.best[0]), __float_as_uint(lead.best[1]));
-      st_cluster_v2(to + 8, (uint32_t)lead.at[0], (uint32_t)lead.at[1]);
+    if (pass == 0) cluster_wait();  // all CTAs of the cluster run
+    if (tid < kRaceCluster) {
+      for (int w = 0; w < W; ++w) lead.take(s_lead[w].best, s_lead[w].at);
+      st_cluster_v2(mapa_shared(smem_u32(&s_all[pass][rank]), tid), __float_as_uint(lead.best), (uint32_t)lead.at);
     }
+    __syncwarp();
     cluster_sync_all();
-    if (rank) return;
-    for (int z = 0; z < 2 && last < 0; ++z) {
-      Leader w = s_all[0];
-      for (int k = 1; k < kPickCluster; ++k) w.take(z, s_all[k].best[z], s_all[k].at[z]);
-      if (w.at[z] != INT_MAX) last = w.at[z];
-    }
+    Leader all = s_all[pass][0];
+    for (int r = 1; r < kRaceCluster; ++r) all.take(s_all[pass][r].best, s_all[pass][r].at);
+    if (all.at != INT_MAX) last = all.at;
+    if (last >= 0 || pass == 1 || !k.refused) break;
+    y = nullptr;
+    out_of = -1;
   }
-  for (int j = tid; j <= drafts; j += kPickThreads)
-    out[(int64_t)b * (drafts + 1) + j] = last < 0 || j > taken ? -1 : j < taken ? tokens[b * ldtok + j] : last;
-  if (tid == 0) {
-    accepted[b] = last < 0 ? 0 : taken;
-    if (last < 0) atomicExch(&g_verify_device_error, 1);
-  }
+  if (rank == 0) write_tokens(a, b, k.taken, last, tid, kRaceThreads);
 }
 
 }  // namespace otf
@@ -362,7 +427,8 @@ int otf::verify_device_error(int clear) {
 extern "C" OTF_API int64_t otf_verify_workspace_bytes(int64_t batch, int64_t drafts, int64_t vocab) {
   if (batch <= 0 || drafts < 0 || drafts > otf::kVerifyMaxDrafts || vocab <= 0 || vocab > INT32_MAX / 2) return -1;
   const int64_t segs = (vocab + otf::kVerifySeg - 1) / otf::kVerifySeg;
-  return otf::align_up(batch * (2 * drafts + 1) * segs * (int64_t)sizeof(otf::RowPart), 256);
+  return otf::align_up(batch * (int64_t)sizeof(otf::Pick), 256) +
+         otf::align_up(batch * (2 * drafts + 1) * segs * (int64_t)sizeof(otf::RowPart), 256);
 }
 
 extern "C" OTF_API int otf_verify_drafts(const float* target, int64_t target_seq, int64_t ld_target,
@@ -374,7 +440,7 @@ extern "C" OTF_API int otf_verify_drafts(const float* target, int64_t target_seq
                                          int64_t vocab, void* workspace, int64_t workspace_bytes, void* stream) {
   if (!target || !out_tokens || !accepted || !workspace || batch <= 0 || drafts < 0 || vocab <= 0)
     return OTF_ERR_INVALID;
-  if (drafts > otf::kVerifyMaxDrafts || vocab > INT32_MAX / 2 || batch > 65535 / (2 * drafts + 1))
+  if (drafts > otf::kVerifyMaxDrafts || vocab > INT32_MAX / 2 || batch > 65535)
     return OTF_ERR_UNSUPPORTED;
   if (drafts > 0 && (!tokens || ld_tokens < drafts || (uniforms && ld_uniforms < drafts))) return OTF_ERR_INVALID;
   if (ld_target < vocab || target_seq < 0 || (noise && ld_noise < vocab)) return OTF_ERR_INVALID;
@@ -388,19 +454,39 @@ extern "C" OTF_API int otf_verify_drafts(const float* target, int64_t target_seq
     return OTF_ERR_INVALID;
   int st = check_device();
   if (st != OTF_OK) return st;
-  if (drafts == 0) draft = nullptr;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int segs = (int)((vocab + otf::kVerifySeg - 1) / otf::kVerifySeg);
-  auto* parts = static_cast<otf::RowPart*>(workspace);
-  const int64_t rows = batch * (drafts + 1) + (draft ? batch * drafts : 0);
-  cudaError_t e = otf::launch_pdl(otf::k_verify_rows, dim3((unsigned)segs, (unsigned)rows), dim3(otf::kVerifyThreads),
-                                  0, s, 1u, target, target_seq, ld_target, draft, draft_seq, ld_draft, temperatures,
-                                  temperature, counts, (int)batch, (int)drafts, (int)vocab, parts);
+  char* w = static_cast<char*>(workspace);
+  const otf::VerifyArgs a = {target,
+                             drafts ? draft : nullptr,
+                             target_seq,
+                             ld_target,
+                             draft_seq,
+                             ld_draft,
+                             tokens,
+                             ld_tokens,
+                             uniforms,
+                             ld_uniforms,
+                             noise,
+                             ld_noise,
+                             temperatures,
+                             temperature,
+                             counts,
+                             out_tokens,
+                             accepted,
+                             (int)drafts,
+                             (int)vocab,
+                             segs,
+                             reinterpret_cast<otf::RowPart*>(w + otf::align_up(batch * (int64_t)sizeof(otf::Pick), 256)),
+                             reinterpret_cast<otf::Pick*>(w)};
+  // row groups: one per row while all of their CTAs fit the GPU at once, else 4
+  const int64_t rows = drafts + 1 + (a.draft ? drafts : 0);
+  const int64_t groups = std::min<int64_t>(rows, batch * segs * rows <= 4 * 148 ? rows : 4);
+  cudaError_t e = otf::launch_pdl(otf::k_verify_rows, dim3((unsigned)segs, (unsigned)groups, (unsigned)batch),
+                                  dim3(otf::kVerifyThreads), 0, s, 1u, a);
   if (e != cudaSuccess) return set_cuda_error(e);
-  return set_cuda_error(otf::launch_pdl(otf::k_verify_pick, dim3((unsigned)batch * otf::kPickCluster),
-                                        dim3(otf::kPickThreads), 0, s, (unsigned)otf::kPickCluster, target,
-                                        target_seq, ld_target, draft, draft_seq, ld_draft, tokens, ld_tokens, uniforms,
-                                        ld_uniforms, noise, ld_noise, temperatures, temperature, counts, out_tokens,
-                                        accepted, (int)batch, (int)drafts, (int)vocab, (const otf::RowPart*)parts,
-                                        segs));
+  e = otf::launch_pdl(otf::k_verify_pick, dim3((unsigned)batch), dim3(256), 0, s, 1u, a);
+  if (e != cudaSuccess || (!temperatures && temperature == 0.0f)) return set_cuda_error(e);
+  return set_cuda_error(otf::launch_pdl(otf::k_verify_race, dim3((unsigned)batch * otf::kRaceCluster),
+                                        dim3(otf::kRaceThreads), 0, s, (unsigned)otf::kRaceCluster, a));
 }
