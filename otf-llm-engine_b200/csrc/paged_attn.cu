@@ -118,14 +118,21 @@ __device__ __forceinline__ void store_row(uint16_t* y, const float (&v)[PL], flo
 template <bool BF>
 constexpr float kProbShift = BF ? 0.0f : 8.0f;
 
-// Where a walk over the chunks stands: sequence, item (KV head and row block) and chunk.
+// Work is dealt out in units: a chunk is one, and an item's start and end cost about as much as
+// kPaItemUnits more (queries fetched, warps joined), which short items would otherwise pile up in one CTA.
+constexpr int kPaItemUnits = 2;
+
+// Where a walk over a CTA's run stands: sequence, item (KV head and row block), chunk, and the
+// units left (a chunk is there while they are positive).
 struct Walk {
   int b, item, chunk, chunks;
+  int64_t left;
 };
 
 template <int D>
 struct Tile {
   static constexpr int keys = D == 128 ? 16 : 32;   // of a warp's stage
+  static constexpr int groups = keys / 16;
   static constexpr int chunk = keys * kPaWarps;
   static constexpr int pieces = D / 8;              // 16-byte pieces of a row
   static constexpr int rows = 32 / pieces;          // rows that a warp's copy instruction covers
@@ -135,14 +142,21 @@ template <int D>
 __device__ __forceinline__ int chunks_of(int len) {
   return (len + 1 + Tile<D>::chunk - 1) / Tile<D>::chunk;  // none when len is -1
 }
+template <int D>
+__device__ __forceinline__ int64_t units_of(int len, int items) {
+  return len < 0 ? 0 : (int64_t)(chunks_of<D>(len) + kPaItemUnits) * items;
+}
 
-template <bool BF, int D, int MT>
+// ALIGNED: a page holds a multiple of 16 tokens, so that 16 neighbours from a multiple of 16 on lie
+// in one page and one look-up serves them; otherwise every lane looks up its own token.
+template <bool BF, int D, int MT, bool ALIGNED>
 __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
-  constexpr int KT = Tile<D>::keys, CH = Tile<D>::chunk, NS = kPaStages, PL = D / 32, RB = 16 * MT;
-  extern __shared__ __align__(128) unsigned char smem[];
-  float* s_m = reinterpret_cast<float*>(smem + kPaWarps * NS * kPaStage);
-  float* s_l = s_m + kPaWarps * RB;
-  uint16_t* s_tail = reinterpret_cast<uint16_t*>(s_l + kPaWarps * RB);  // [tokens - 1][keys, values][D]
+  constexpr int KT = Tile<D>::keys, CH = Tile<D>::chunk, NS = kPaStages, RB = 16 * MT, G = Tile<D>::groups;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  unsigned char* s_q = smem + kPaWarps * NS * kPaStage;  // [RB][D] when it does not fit the registers
+  float* s_m = reinterpret_cast<float*>(s_q + (MT > 1 ? RB * D * 2 : 0));
+  float* s_l = s_m + kPaWarps * 16;
+  uint16_t* s_tail = reinterpret_cast<uint16_t*>(s_l + kPaWarps * 16);  // [tokens - 1][keys, values][D]
   int* s_len = reinterpret_cast<int*>(s_tail + (a.tokens - 1) * 2 * D);
   __shared__ int64_t s_sum[kPaWarps];
   __shared__ Walk s_walk;
@@ -152,16 +166,16 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int items = c.kv_heads * a.blocks;
 
-  // the lengths, and this CTA's run of chunks [u0, u1) of all items' chunks
+  // the lengths, and this CTA's run of units [u0, u1)
   int64_t sum = 0;
   for (int b = tid; b < c.batch; b += kPaThreads) {
-    int len = c.lengths[b];
-    if (len >= 0 && (int64_t)len + a.tokens > c.capacity) {
+    int len = max(c.lengths[b], -1);
+    if ((int64_t)len + a.tokens > c.capacity) {
       if (blockIdx.x == 0) report_bad_attn_page();
       len = -1;
     }
-    s_len[b] = max(len, -1);
-    sum += (int64_t)chunks_of<D>(max(len, -1)) * items;
+    s_len[b] = len;
+    sum += units_of<D>(len, items);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -170,7 +184,7 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
   int64_t total = 0;
 #pragma unroll
   for (int w = 0; w < kPaWarps; ++w) total += s_sum[w];
-  const int64_t ctas = min((int64_t)kPaGrid, total);  // every one of them has a chunk at least
+  const int64_t ctas = min((int64_t)kPaGrid, total);
   const int64_t u0 = blockIdx.x < ctas ? blockIdx.x * total / ctas : total;
   const int64_t u1 = blockIdx.x < ctas ? (blockIdx.x + 1) * total / ctas : total;
   if (warp == 0 && (u0 < u1 || blockIdx.x == 0)) {
@@ -178,7 +192,7 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
     for (int b0 = 0; b0 < c.batch; b0 += 32) {
       const int b = b0 + lane;
       const int n = b < c.batch ? chunks_of<D>(s_len[b]) : 0;
-      const int64_t mine = (int64_t)n * items;
+      const int64_t mine = b < c.batch ? units_of<D>(s_len[b], items) : 0;
       int64_t inc = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -187,8 +201,8 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
       }
       const int64_t first = base + inc - mine;
       if (u0 >= first && u0 < first + mine) {
-        const int at = (int)(u0 - first);
-        s_walk = Walk{b, at / n, at % n, n};
+        const int at = (int)(u0 - first), item = at / (n + kPaItemUnits), x = at - item * (n + kPaItemUnits);
+        s_walk = Walk{b, item, max(0, x - kPaItemUnits), n, u1 - u0 - max(0, kPaItemUnits - x)};
       }
       if (blockIdx.x == 0 && b < c.batch) {
         a.prefix[b] = first;
@@ -198,87 +212,129 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
     }
   }
   __syncthreads();
-  if (u0 >= u1) return;
+  if (u0 >= u1 || s_walk.left <= 0) return;
 
   auto advance = [&](Walk& w) {
+    --w.left;
     if (++w.chunk < w.chunks) return;
+    w.left -= kPaItemUnits;
     w.chunk = 0;
-    if (++w.item < items) return;
+    if (++w.item < items || w.left <= 0) return;
     w.item = 0;
     do ++w.b;
     while (w.b < c.batch && s_len[w.b] < 0);
-    w.chunks = w.b < c.batch ? chunks_of<D>(s_len[w.b]) : 1;
+    if (w.b < c.batch) w.chunks = chunks_of<D>(s_len[w.b]);
   };
 
-  // this lane's token of the walk's chunk: the offset of its page row (its head's rows lie
-  // head_stride apart), -1 where there is none
-  auto token_at = [&](const Walk& w, bool there) -> int64_t {
-    const int key = w.chunk * CH + warp * KT + lane;
-    if (!there || lane >= KT || key > s_len[w.b]) return -1;
-    const uint32_t at = (uint32_t)key / a.page;
-    const int page = c.table[w.b * c.ld_table + at];
-    if (page < 0 || page >= c.n_pages) {
-      report_bad_attn_page();
-      return -1;
+  // Offsets in the pools of the walk's chunk for this warp: of each group of 16 tokens (ALIGNED), or
+  // of the lane's token; -1 where there is none.
+  struct Places {
+    int64_t at[ALIGNED ? G : 1];
+  };
+  auto places = [&](const Walk& w) {
+    Places p;
+#pragma unroll
+    for (int g = 0; g < (ALIGNED ? G : 1); ++g) {
+      const int key = w.chunk * CH + warp * KT + (ALIGNED ? g * 16 : lane);
+      p.at[g] = -1;
+      if (w.left > 0 && (ALIGNED || lane < KT) && key <= s_len[w.b]) {
+        const uint32_t in = (uint32_t)key / a.page;
+        const int page = c.table[w.b * c.ld_table + in];
+        if (page >= 0 && page < c.n_pages)
+          p.at[g] = page * c.page_stride + (int64_t)(key - (int)(in * a.page.d)) * c.token_stride;
+        else
+          report_bad_attn_page();
+      }
     }
-    return page * c.page_stride + (int64_t)(key - (int)(at * a.page.d)) * c.token_stride;
+    return p;
   };
   const uint32_t ring = smem_u32(smem) + warp * NS * kPaStage;
   const int my_row = lane / Tile<D>::pieces, my_piece = lane % Tile<D>::pieces;
-  auto fetch = [&](const Walk& w, int64_t offset, int slot) {
-    const int64_t head = (int64_t)(w.item / a.blocks) * c.head_stride + my_piece * 8;
+  const int64_t v_from_k = c.v - c.k, my_off = my_row * c.token_stride + my_piece * 8;
+  auto fetch = [&](const Walk& w, const Places& p, int slot) {
+    const int64_t head = (int64_t)(w.item / a.blocks) * c.head_stride;
     const uint32_t dst = ring + slot * kPaStage;
+    const int there = s_len[w.b] + 1 - (w.chunk * CH + warp * KT);  // tokens of the tile that there are
 #pragma unroll
     for (int i = 0; i < KT / Tile<D>::rows; ++i) {
       const int r = i * Tile<D>::rows + my_row;
-      const int64_t off = __shfl_sync(0xffffffffu, offset, r);
-      const bool ok = off >= 0;
-      const int64_t at = ok ? off + head : 0;
+      const uint16_t* x;
+      bool ok;
+      if (ALIGNED) {
+        constexpr int per = 16 / Tile<D>::rows;  // instructions of a group
+        ok = r < there && p.at[i / per] >= 0;
+        x = c.k + p.at[i / per] + head + my_off + (int64_t)((i % per) * Tile<D>::rows) * c.token_stride;
+      } else {
+        const int64_t off = __shfl_sync(0xffffffffu, p.at[0], r);
+        ok = off >= 0;
+        x = c.k + off + head + my_piece * 8;
+      }
+      if (!ok) x = c.k;  // an address, not read
       const uint32_t to = dst + r * (D * 2) + ((my_piece ^ (r & 7)) << 4);
-      cp_async16(to, c.k + at, ok ? 16u : 0u);
-      cp_async16(to + KT * D * 2, c.v + at, ok ? 16u : 0u);
+      cp_async16(to, x, ok ? 16u : 0u);
+      cp_async16(to + KT * D * 2, ok ? x + v_from_k : x, ok ? 16u : 0u);
     }
   };
 
   Walk get = s_walk, load = s_walk;
-  int64_t u_load = u0;
-  int64_t next = token_at(load, true);
+  Places next = places(load);
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) {
-    if (u_load < u1) {
+    if (load.left > 0) {
       fetch(load, next, i);
       advance(load);
-      next = token_at(load, ++u_load < u1);
+      next = places(load);
     }
     cp_async_commit();
   }
 
-  uint32_t qf[MT][D / 16][4];
+  uint32_t qf[D / 16][4];
   float o[MT][D / 8][4], m[MT][2], l[MT][2];
-  int64_t begin = u0 - get.chunk;  // this item's first chunk
+  const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;  // on q, so that a larger product weighs more
+  const float scale = fabsf(a.scale);
+  const int lrow = lane & 7, lmat = lane >> 3;
+  const uint32_t k_lane = ((lmat >> 1) * 8 + lrow) * (D * 2) + (((lmat & 1) ^ lrow) << 4);
+  const uint32_t v_lane = ((lmat & 1) * 8 + lrow) * (D * 2) + (((lmat >> 1) ^ lrow) << 4);
+  const uint32_t q_lane = smem_u32(s_q) + v_lane;  // a query's fragment has the values' order of matrices
+  int parts = 0, began = get.chunk, slot = 0;
   bool fresh = true;
-  int slot = 0;
-  for (int64_t u = u0; u < u1; ++u) {
+  while (get.left > 0) {
     const int g = get.item / a.blocks, rb = get.item - g * a.blocks;
     const int len = s_len[get.b];
     if (fresh) {
       fresh = false;
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
+      // the row block's queries: matrix fragments in registers, or (two matrices high, where the
+      // outputs take the registers) rows in shared memory for ldmatrix
+      if (MT == 1) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int r = rb * RB + t * 16 + h * 8 + (lane >> 2);
+          const int r = rb * RB + h * 8 + (lane >> 2);
           const int tok = r / a.rep;
           const uint32_t* x = reinterpret_cast<const uint32_t*>(a.q + ((int64_t)get.b * a.tokens + tok) * a.ldq +
                                                                 (int64_t)(g * a.rep + r - tok * a.rep) * D) + (lane & 3);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
-            qf[t][k][h] = r < a.rows ? x[k * 8] : 0u;
-            qf[t][k][h + 2] = r < a.rows ? x[k * 8 + 4] : 0u;
+            qf[k][h] = r < a.rows ? x[k * 8] ^ sign : 0u;
+            qf[k][h + 2] = r < a.rows ? x[k * 8 + 4] ^ sign : 0u;
           }
-          m[t][h] = -INFINITY;
-          l[t][h] = 0.0f;
         }
+      } else {
+#pragma unroll
+        for (int e = tid; e < RB * D / 8; e += kPaThreads) {
+          const int w = e / (D / 8), piece = e % (D / 8), r = rb * RB + w, tok = r / a.rep;
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (r < a.rows)
+            x = *reinterpret_cast<const uint4*>(a.q + ((int64_t)get.b * a.tokens + tok) * a.ldq +
+                                                (int64_t)(g * a.rep + r - tok * a.rep) * D + piece * 8);
+          *reinterpret_cast<uint4*>(s_q + w * D * 2 + ((piece ^ (w & 7)) << 4)) =
+              make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
+        }
+        __syncthreads();
+      }
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        m[t][0] = m[t][1] = -INFINITY;
+        l[t][0] = l[t][1] = 0.0f;
 #pragma unroll
         for (int j = 0; j < D / 8; ++j)
 #pragma unroll
@@ -287,17 +343,16 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
     }
     cp_async_wait<NS - 2>();
     __syncwarp();
-    {  // the stage read one round ago takes the chunk NS - 1 ahead
-      if (u_load < u1) {
-        fetch(load, next, slot == 0 ? NS - 1 : slot - 1);
-        advance(load);
-        next = token_at(load, ++u_load < u1);
-      }
-      cp_async_commit();
+    // the stage read one round ago takes the chunk NS - 1 ahead
+    if (load.left > 0) {
+      fetch(load, next, slot == 0 ? NS - 1 : slot - 1);
+      advance(load);
+      next = places(load);
     }
+    cp_async_commit();
     const int key0 = get.chunk * CH + warp * KT;
     if (key0 <= len) {
-      const uint32_t kb = ring + slot * kPaStage, vb = kb + KT * D * 2;
+      const uint32_t kb = ring + slot * kPaStage + k_lane, vb = ring + slot * kPaStage + KT * D * 2 + v_lane;
       float s[MT][KT / 8][4];
 #pragma unroll
       for (int t = 0; t < MT; ++t)
@@ -305,34 +360,39 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
         for (int n = 0; n < KT / 8; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[t][n][i] = 0.0f;
-      const int lrow = lane & 7, lmat = lane >> 3;
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k)
+      for (int k = 0; k < D / 16; ++k) {
+        uint32_t qk[MT][4];
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+          if (MT == 1)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) qk[t][i] = qf[k][i];
+          else
+            ldmatrix_x4((q_lane ^ (k << 5)) + t * 16 * D * 2, qk[t][0], qk[t][1], qk[t][2], qk[t][3]);
 #pragma unroll
         for (int n = 0; n < KT / 16; ++n) {
-          const int row = n * 16 + (lmat >> 1) * 8 + lrow;
           uint32_t b0, b1, b2, b3;
-          ldmatrix_x4(kb + row * (D * 2) + (((k * 2 + (lmat & 1)) ^ lrow) << 4), b0, b1, b2, b3);
+          ldmatrix_x4((kb ^ (k << 5)) + n * 16 * D * 2, b0, b1, b2, b3);
 #pragma unroll
           for (int t = 0; t < MT; ++t) {
-            mma16816<BF>(s[t][2 * n], qf[t][k], b0, b1);
-            mma16816<BF>(s[t][2 * n + 1], qf[t][k], b2, b3);
+            mma16816<BF>(s[t][2 * n], qk[t], b0, b1);
+            mma16816<BF>(s[t][2 * n + 1], qk[t], b2, b3);
           }
         }
-      const bool edge = key0 + KT > len + 1;
+      }
+      if (key0 + KT > len + 1) {
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        float mx[2] = {m[t][0], m[t][1]};
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int n = 0; n < KT / 8; ++n)
+          for (int n = 0; n < KT / 8; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float x = s[t][n][i] * a.scale;
-            if (edge && key0 + n * 8 + (lane & 3) * 2 + (i & 1) > len) x = -INFINITY;
-            s[t][n][i] = x;
-            mx[i >> 1] = fmaxf(mx[i >> 1], x);
-          }
-        if (a.scores) {
+            for (int i = 0; i < 4; ++i)
+              if (key0 + n * 8 + (lane & 3) * 2 + (i & 1) > len) s[t][n][i] = -INFINITY;
+      }
+      if (a.scores) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int r = rb * RB + t * 16 + h * 8 + (lane >> 2);
@@ -341,19 +401,29 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
 #pragma unroll
               for (int n = 0; n < KT / 8; ++n)
                 if (key0 + n * 8 <= len)  // ld_scores covers whole groups of 8
-                  *reinterpret_cast<float2*>(to + n * 8) = make_float2(s[t][n][2 * h], s[t][n][2 * h + 1]);
+                  *reinterpret_cast<float2*>(to + n * 8) = make_float2(s[t][n][2 * h] * scale, s[t][n][2 * h + 1] * scale);
             }
           }
+      }
+      uint32_t p[MT][KT / 16][4];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        float mx[2] = {-INFINITY, -INFINITY};  // of the products, before the scale
+#pragma unroll
+        for (int n = 0; n < KT / 8; ++n) {
+          mx[0] = fmaxf(mx[0], fmaxf(s[t][n][0], s[t][n][1]));
+          mx[1] = fmaxf(mx[1], fmaxf(s[t][n][2], s[t][n][3]));
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
           mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+          mx[h] = fmaxf(mx[h], m[t][h]);
         }
         if (__any_sync(0xffffffffu, mx[0] != m[t][0] || mx[1] != m[t][1])) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float f = m[t][h] == -INFINITY ? 0.0f : ex2(m[t][h] - mx[h]);
+            const float f = m[t][h] == -INFINITY ? 0.0f : ex2((m[t][h] - mx[h]) * scale);
             l[t][h] *= f;
 #pragma unroll
             for (int j = 0; j < D / 8; ++j) {
@@ -363,31 +433,25 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
             m[t][h] = mx[h];
           }
         }
-        const float z[2] = {kProbShift<BF> - (m[t][0] == -INFINITY ? 0.0f : m[t][0]),
-                            kProbShift<BF> - (m[t][1] == -INFINITY ? 0.0f : m[t][1])};
+        // 2^(scale (s - m) + shift): one multiply-add and one exponential per entry
+        const float z[2] = {kProbShift<BF> - (m[t][0] == -INFINITY ? 0.0f : m[t][0] * scale),
+                            kProbShift<BF> - (m[t][1] == -INFINITY ? 0.0f : m[t][1] * scale)};
 #pragma unroll
-        for (int n = 0; n < KT / 8; ++n)
+        for (int n = 0; n < KT / 8; ++n) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            s[t][n][i] = ex2(s[t][n][i] + z[i >> 1]);
-            l[t][i >> 1] += s[t][n][i];
-          }
+          for (int i = 0; i < 4; ++i) s[t][n][i] = ex2(fmaf(s[t][n][i], scale, z[i >> 1]));
+          l[t][0] += s[t][n][0] + s[t][n][1];
+          l[t][1] += s[t][n][2] + s[t][n][3];
+          p[t][n >> 1][(n & 1) * 2] = pack2<BF>(s[t][n][0], s[t][n][1]);
+          p[t][n >> 1][(n & 1) * 2 + 1] = pack2<BF>(s[t][n][2], s[t][n][3]);
+        }
       }
-      uint32_t p[MT][KT / 16][4];
-#pragma unroll
-      for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int n = 0; n < KT / 16; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            p[t][n][i] = pack2<BF>(s[t][2 * n + (i >> 1)][2 * (i & 1)], s[t][2 * n + (i >> 1)][2 * (i & 1) + 1]);
 #pragma unroll
       for (int j = 0; j < D / 16; ++j)
 #pragma unroll
         for (int n = 0; n < KT / 16; ++n) {
-          const int row = n * 16 + (lmat & 1) * 8 + lrow;
           uint32_t b0, b1, b2, b3;
-          ldmatrix_x4_trans(vb + row * (D * 2) + (((j * 2 + (lmat >> 1)) ^ lrow) << 4), b0, b1, b2, b3);
+          ldmatrix_x4_trans((vb ^ (j << 5)) + n * 16 * D * 2, b0, b1, b2, b3);
 #pragma unroll
           for (int t = 0; t < MT; ++t) {
             mma16816<BF>(o[t][2 * j], p[t][n], b0, b1);
@@ -395,17 +459,20 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
           }
         }
     }
-    const bool last = get.chunk + 1 == get.chunks;
-    if (last || u + 1 == u1) {
-      // The item's end in this run: the warps' parts join, through the stage just read.
-      const bool whole = last && begin >= u0;
+    const Walk now = get;
+    const bool last = now.chunk + 1 == now.chunks;
+    advance(get);
+    if (last || get.left <= 0) {
+      // The item's end in this run: the warps' parts join, through the stage just read, all 16 rows
+      // of a block at once: 8 threads per row, each the 4 values from j * 32 + 4 * part on.
+      const bool whole = last && began == 0;
       float* mine = reinterpret_cast<float*>(smem + warp * NS * kPaStage + slot * kPaStage);
-      if (last)  // the newest tokens, all requested together
+      if (last)  // the newest tokens
         for (int e = tid; e < (a.tokens - 1) * 2 * (D / 8); e += kPaThreads) {
           const int piece = e % (D / 8), side = e / (D / 8) & 1, i = e / (D / 4);
           const int key = len + 1 + i;
           const uint32_t at = (uint32_t)key / a.page;
-          const int page = c.table[get.b * c.ld_table + at];
+          const int page = c.table[now.b * c.ld_table + at];
           uint4 x = make_uint4(0, 0, 0, 0);
           if (page >= 0 && page < c.n_pages)
             x = *reinterpret_cast<const uint4*>((side ? c.v : c.k) + page * c.page_stride +
@@ -415,126 +482,146 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
             report_bad_attn_page();
           *reinterpret_cast<uint4*>(s_tail + (i * 2 + side) * D + piece * 8) = x;
         }
+      const int r = tid >> 3, part = tid & 7;
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
+        const int rr = rb * RB + t * 16 + r;
+        const int tok = rr / a.rep, head = g * a.rep + rr - tok * a.rep;
+        const int64_t row = (int64_t)now.b * a.tokens + tok;
+        float qv[D / 32][4];
+        if (last && a.tokens > 1 && rr < a.rows)
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j) load_row<BF, 4>(a.q + row * a.ldq + (int64_t)head * D + j * 32 + part * 4, qv[j]);
         __syncwarp();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float x = l[t][h];
           x += __shfl_xor_sync(0xffffffffu, x, 1);
           x += __shfl_xor_sync(0xffffffffu, x, 2);
-          const int r = h * 8 + (lane >> 2);
+          const int w = h * 8 + (lane >> 2);
           if ((lane & 3) == 0) {
-            s_m[warp * RB + r] = m[t][h];
-            s_l[warp * RB + r] = x;
+            s_m[warp * 16 + w] = m[t][h] * scale;
+            s_l[warp * 16 + w] = x;
           }
 #pragma unroll
           for (int j = 0; j < D / 8; ++j)  // columns turned by the row, against bank conflicts
-            *reinterpret_cast<float2*>(mine + r * D + ((j * 8 + (lane & 3) * 2) ^ ((r & 3) << 3))) =
+            *reinterpret_cast<float2*>(mine + w * D + ((j * 8 + (lane & 3) * 2) ^ ((w & 3) << 3))) =
                 make_float2(o[t][j][2 * h], o[t][j][2 * h + 1]);
         }
         __syncthreads();
-        for (int r = warp; r < 16; r += kPaWarps) {
-          const int rr = rb * RB + t * 16 + r;
-          if (rr >= a.rows) break;
-          float M = -INFINITY, L = 0.0f, acc[PL];
+        float M = -INFINITY, L = 0.0f, acc[D / 32][4];
 #pragma unroll
-          for (int i = 0; i < PL; ++i) acc[i] = 0.0f;
+        for (int w = 0; w < kPaWarps; ++w) M = fmaxf(M, s_m[w * 16 + r]);
 #pragma unroll
-          for (int w = 0; w < kPaWarps; ++w) M = fmaxf(M, s_m[w * RB + r]);
+        for (int j = 0; j < D / 32; ++j)
 #pragma unroll
-          for (int w = 0; w < kPaWarps; ++w) {
-            const float lw = s_l[w * RB + r];
-            const float f = lw == 0.0f ? 0.0f : ex2(s_m[w * RB + r] - M);
-            const float* x = reinterpret_cast<const float*>(smem + w * NS * kPaStage + slot * kPaStage) + r * D +
-                             ((lane * PL) ^ ((r & 3) << 3));
-            if (lw != 0.0f) {
-              L = fmaf(lw, f, L);
+          for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
 #pragma unroll
-              for (int i = 0; i < PL; ++i) acc[i] = fmaf(x[i], f, acc[i]);
+        for (int w = 0; w < kPaWarps; ++w) {
+          const float lw = s_l[w * 16 + r];
+          const float f = lw == 0.0f ? 0.0f : ex2(s_m[w * 16 + r] - M);
+          const float* x = reinterpret_cast<const float*>(smem + w * NS * kPaStage + slot * kPaStage) + r * D;
+          if (lw != 0.0f) {
+            L = fmaf(lw, f, L);
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+              const float4 y = *reinterpret_cast<const float4*>(x + ((j * 32 + part * 4) ^ ((r & 3) << 3)));
+              acc[j][0] = fmaf(y.x, f, acc[j][0]);
+              acc[j][1] = fmaf(y.y, f, acc[j][1]);
+              acc[j][2] = fmaf(y.z, f, acc[j][2]);
+              acc[j][3] = fmaf(y.w, f, acc[j][3]);
             }
           }
-          const int tok = rr / a.rep, head = g * a.rep + rr - tok * a.rep;
-          const int64_t row = (int64_t)get.b * a.tokens + tok;
-          if (last && a.tokens > 1) {  // the newest tokens, as far as this row sees them
-            float qv[PL];
-            load_row<BF, PL>(a.q + row * a.ldq + (int64_t)head * D + lane * PL, qv);
-            float* sc = a.scores ? a.scores + (((int64_t)get.b * c.kv_heads + g) * a.rows + rr) * a.ld_scores : nullptr;
-            for (int i = 0; i < a.tokens - 1; ++i) {
-              if (i >= tok) {
-                if (sc && lane == 0) sc[len + 1 + i] = -INFINITY;
-                continue;
-              }
-              float kv[PL], vv[PL], d = 0.0f;
-              load_row<BF, PL>(s_tail + i * 2 * D + lane * PL, kv);
-              load_row<BF, PL>(s_tail + (i * 2 + 1) * D + lane * PL, vv);
+        }
+        if (last && a.tokens > 1) {  // the newest tokens, as far as a row sees them
+          float* sc = a.scores && rr < a.rows && part == 0
+                          ? a.scores + (((int64_t)now.b * c.kv_heads + g) * a.rows + rr) * a.ld_scores + len + 1
+                          : nullptr;
+          for (int i = 0; i < a.tokens - 1; ++i) {
+            float d = 0.0f, vv[D / 32][4];
 #pragma unroll
-              for (int j = 0; j < PL; ++j) d = fmaf(qv[j], kv[j], d);
+            for (int j = 0; j < D / 32; ++j) {
+              float kv[4];
+              load_row<BF, 4>(s_tail + i * 2 * D + j * 32 + part * 4, kv);
+              load_row<BF, 4>(s_tail + (i * 2 + 1) * D + j * 32 + part * 4, vv[j]);
 #pragma unroll
-              for (int x = 16; x > 0; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
-              d *= a.scale;
-              if (sc && lane == 0) sc[len + 1 + i] = d;
-              const float mn = fmaxf(M, d), f = M == -INFINITY ? 0.0f : ex2(M - mn);
-              const float pr = d == -INFINITY ? 0.0f : ex2(d - mn + kProbShift<BF>);
+              for (int z = 0; z < 4; ++z) d = fmaf(qv[j][z], kv[z], d);
+            }
+#pragma unroll
+            for (int x = 4; x > 0; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
+            d = i < tok ? d * a.scale : -INFINITY;
+            if (sc) sc[i] = d;
+            if (d != -INFINITY) {
+              const float mn = fmaxf(M, d), f = M == -INFINITY ? 0.0f : ex2(M - mn), pr = ex2(d - mn + kProbShift<BF>);
               L = L * f + pr;
 #pragma unroll
-              for (int j = 0; j < PL; ++j) acc[j] = acc[j] * f + (d == -INFINITY ? 0.0f : pr * vv[j]);
+              for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+                for (int z = 0; z < 4; ++z) acc[j][z] = fmaf(pr, vv[j][z], acc[j][z] * f);
               M = mn;
             }
           }
+        }
+        if (rr < a.rows) {
           if (whole) {
-            store_row<BF, PL>(a.out + row * a.ldo + (int64_t)head * D + lane * PL, acc, 1.0f / L);
-            if (a.lse && lane == 0)
-              a.lse[((int64_t)get.b * c.kv_heads + g) * a.rows + rr] = M + log2f(L) - kProbShift<BF>;
-          } else {
-            const int64_t at = (int64_t)(2 * blockIdx.x + (begin > u0 ? 1 : 0)) * RB + t * 16 + r;
 #pragma unroll
-            for (int i = 0; i < PL; ++i) a.part[at * D + lane * PL + i] = acc[i];
-            if (lane == 0) a.part_ml[at] = make_float2(M, L);
+            for (int j = 0; j < D / 32; ++j)
+              store_row<BF, 4>(a.out + row * a.ldo + (int64_t)head * D + j * 32 + part * 4, acc[j], 1.0f / L);
+            if (a.lse && part == 0)
+              a.lse[((int64_t)now.b * c.kv_heads + g) * a.rows + rr] = M + log2f(L) - kProbShift<BF>;
+          } else {
+            const int64_t at = (int64_t)(2 * blockIdx.x + (parts > 0 ? 1 : 0)) * RB + t * 16 + r;
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j)
+              *reinterpret_cast<float4*>(a.part + at * D + j * 32 + part * 4) =
+                  make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
+            if (part == 0) a.part_ml[at] = make_float2(M, L);
           }
         }
         __syncthreads();  // before the stages are filled again, or the next 16 rows come
       }
+      ++parts;
+      began = 0;
       fresh = true;
     }
-    if (last) begin = u + 1;
-    advance(get);
     slot = slot + 1 == NS ? 0 : slot + 1;
   }
   cp_async_wait<0>();
 }
 
 // The parts of an item that several CTAs shared, joined in the cache's order: grid (items, row
-// groups), a warp per row.
+// groups), a warp per row.  Latency-bound: the parts' m and l come together, then eight parts at a
+// time.  40 registers, so that its CTAs find room beside the last of the attention's.
 template <bool BF, int D>
-__global__ void __launch_bounds__(128) k_paged_attn_join(AttnArgs a, int RB) {
+__global__ void __launch_bounds__(128, 12) k_paged_attn_join(AttnArgs a, int RB) {
   constexpr int PL = D / 32;
   pdl_trigger();
-  pdl_wait();
   const PagedView& c = a.c;
   const int items = c.kv_heads * a.blocks;
   const int b = blockIdx.x / items, item = blockIdx.x - b * items, g = item / a.blocks, rb = item - g * a.blocks;
   const int lane = threadIdx.x & 31, r = blockIdx.y * 4 + (threadIdx.x >> 5), rr = rb * RB + r;
+  pdl_wait();
   if (r >= RB || rr >= a.rows) return;
   const int64_t p0 = a.prefix[b], p1 = a.prefix[b + 1], total = a.prefix[c.batch];
   if (p0 == p1) return;
-  // the CTAs whose runs meet the item's chunks [c0, c1): 32-bit divisions where they do
+  // the CTAs whose runs meet the item's chunks, units [c0, c1) behind its kPaItemUnits: 32-bit
+  // divisions where they do; and whether the item is not the first of CTA i0's run
   const int64_t ctas = min((int64_t)kPaGrid, total);
-  int i0, i1, second;
+  int i0, i1;
+  bool second;
   if (total < (1 << 23)) {
-    const uint32_t n = (uint32_t)(p1 - p0) / items, c0 = (uint32_t)p0 + item * n, t = (uint32_t)total, u = (uint32_t)ctas;
-    i0 = (int)(((c0 + 1) * u - 1) / t);
-    i1 = (int)(((c0 + n) * u - 1) / t);
-    second = i0 * t / u == c0 ? 0 : 1;
+    const uint32_t n = (uint32_t)(p1 - p0) / items, at = (uint32_t)p0 + item * n, t = (uint32_t)total, u = (uint32_t)ctas;
+    i0 = (int)(((at + kPaItemUnits + 1) * u - 1) / t);
+    i1 = (int)(((at + n) * u - 1) / t);
+    second = i0 * t / u < at;
   } else {
-    const int64_t n = (p1 - p0) / items, c0 = p0 + item * n;
-    i0 = (int)(((c0 + 1) * ctas - 1) / total);
-    i1 = (int)(((c0 + n) * ctas - 1) / total);
-    second = i0 * total / ctas == c0 ? 0 : 1;
+    const int64_t n = (p1 - p0) / items, at = p0 + item * n;
+    i0 = (int)(((at + kPaItemUnits + 1) * ctas - 1) / total);
+    i1 = (int)(((at + n) * ctas - 1) / total);
+    second = i0 * total / ctas < at;
   }
   if (i0 == i1) return;  // one CTA had it whole
-  // a part is the first of its CTA's run, but the item's first part may be the second of one
-  auto part = [&](int i) { return (int64_t)(2 * i + (i == i0 ? second : 0)) * RB + r; };
+  auto part = [&](int i) { return (2 * i + (i == i0 && second ? 1 : 0)) * RB + r; };
   float M = -INFINITY, L = 0.0f, acc[PL];
 #pragma unroll
   for (int i = 0; i < PL; ++i) acc[i] = 0.0f;
@@ -551,12 +638,21 @@ __global__ void __launch_bounds__(128) k_paged_attn_join(AttnArgs a, int RB) {
       }
     }
     const int n = min(32, i1 + 1 - base);
-#pragma unroll 8
+#pragma unroll 4
     for (int i = 0; i < n; ++i) {
       const float w = __shfl_sync(0xffffffffu, f, i);
-      const float* x = a.part + part(base + i) * D + lane * PL;
-#pragma unroll
-      for (int j = 0; j < PL; ++j) acc[j] = fmaf(x[j], w, acc[j]);
+      const float* x = a.part + (int64_t)part(base + i) * D + lane * PL;
+      if (D == 128) {
+        const float4 y = *reinterpret_cast<const float4*>(x);
+        acc[0] = fmaf(y.x, w, acc[0]);
+        acc[1] = fmaf(y.y, w, acc[1]);
+        acc[PL - 2] = fmaf(y.z, w, acc[PL - 2]);
+        acc[PL - 1] = fmaf(y.w, w, acc[PL - 1]);
+      } else {
+        const float2 y = *reinterpret_cast<const float2*>(x);
+        acc[0] = fmaf(y.x, w, acc[0]);
+        acc[1] = fmaf(y.y, w, acc[1]);
+      }
     }
   }
 #pragma unroll
@@ -607,8 +703,10 @@ static AttnSpace attn_space(int64_t batch, int64_t heads, int64_t kv_heads, int6
 template <bool BF, int D>
 static cudaError_t launch_attn(const AttnArgs& a, float* weights, int64_t ldw, cudaStream_t s) {
   const int RB = a.rows <= 16 ? 16 : 32;
-  auto* k = RB == 16 ? k_paged_attn<BF, D, 1> : k_paged_attn<BF, D, 2>;
-  const size_t dyn = (size_t)kPaWarps * kPaStages * kPaStage + (size_t)kPaWarps * RB * 8 +
+  const bool aligned = a.c.page_size % 16 == 0;
+  auto* k = RB == 16 ? (aligned ? k_paged_attn<BF, D, 1, true> : k_paged_attn<BF, D, 1, false>)
+                     : (aligned ? k_paged_attn<BF, D, 2, true> : k_paged_attn<BF, D, 2, false>);
+  const size_t dyn = (size_t)kPaWarps * kPaStages * kPaStage + (size_t)kPaWarps * 16 * 8 + (RB > 16 ? RB * D * 2 : 0) +
                      (size_t)(a.tokens - 1) * 4 * D + (size_t)a.c.batch * 4;
   {
     // the shared-memory opt-in, once per kernel and device, for the largest batch
@@ -621,7 +719,7 @@ static cudaError_t launch_attn(const AttnArgs& a, float* weights, int64_t ldw, c
     bool& have = done[std::make_pair(reinterpret_cast<const void*>(k), dev)];
     if (!have) {
       e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               kPaWarps * kPaStages * kPaStage + kPaWarps * 32 * 8 + (kPagedMaxTokens - 1) * 4 * D +
+                               kPaWarps * kPaStages * kPaStage + kPaWarps * 16 * 8 + 32 * D * 2 + (kPagedMaxTokens - 1) * 4 * D +
                                    kPagedMaxBatch * 4);
       if (e != cudaSuccess) return e;
       have = true;
