@@ -92,6 +92,7 @@ class Rotary:
         self.head_dim, self.rot_dim, self.interleaved = int(head_dim), rot_dim, bool(interleaved)
         self.frequencies, self.factor = rope_frequencies(rot_dim, theta, scaling)
         self.turns = (self.frequencies / (2 * math.pi)).to(device)
+        self.device = self.turns.device
         a = _native.RotaryArgs()
         a.turns, a.rot_dim = self.turns.data_ptr() if rot_dim else None, rot_dim
         a.factor, a.interleaved = self.factor, int(self.interleaved)
@@ -142,6 +143,7 @@ class PagedKVCache:
         self.page_size, self.kv_heads, self.head_dim = page, heads, dim
         self.batch, self.max_pages = page_table.shape
         self.capacity = self.max_pages * page
+        self._scale = dim ** -0.5
         c = _native.PagedCache()
         c.k_pages, c.v_pages = k_pages.data_ptr(), v_pages.data_ptr()
         c.page_stride, c.token_stride, c.head_stride = stride
@@ -151,6 +153,10 @@ class PagedKVCache:
         c.lengths, c.batch, c.dtype = lengths.data_ptr(), self.batch, _DTYPES[self.dtype]
         self._args = c
         self._ref = ctypes.byref(c)
+        # shapes and strides of earlier calls' arguments, with what their checks found: a decode
+        # loop's calls differ in addresses alone
+        self._append_plans: dict = {}
+        self._attend_plans: dict = {}
 
     @classmethod
     def allocate(cls, n_pages: int, page_size: int, kv_heads: int, head_dim: int, page_table: torch.Tensor,
@@ -161,9 +167,8 @@ class PagedKVCache:
         return cls(k, v, page_table, lengths)
 
     def _heads(self, t: torch.Tensor, name: str, heads: Optional[int] = None) -> int:
-        """Check [rows, heads, head_dim] values whose heads lie next to one another; the row stride."""
-        if t.device != self.device or t.dtype != self.dtype:
-            raise ValueError(f"{name} must be {self.dtype} on {self.device}, got {t.dtype} on {t.device}")
+        """Check the shape and strides of [rows, heads, head_dim] values whose heads lie next to one
+        another; the row stride."""
         d = self.head_dim
         if t.dim() != 3 or t.shape[2] != d or (heads is not None and t.shape[1] != heads) or t.shape[1] == 0:
             raise ValueError(f"{name} must be [rows, {heads or 'heads'}, {d}], got {tuple(t.shape)}")
@@ -172,11 +177,18 @@ class PagedKVCache:
             raise ValueError(f"{name} needs its heads next to one another, got strides {t.stride()}")
         if t.shape[0] <= 1:
             row = t.shape[1] * d
-        if row % 8 or row < t.shape[1] * d or t.data_ptr() % 16:
+        if row % 8 or row < t.shape[1] * d:
             raise ValueError(f"{name} needs 16-byte aligned rows that do not overlap, got strides {t.stride()}")
         return row
 
-    def _vector(self, t: torch.Tensor, name: str, n: int) -> ctypes.c_void_p:
+    def _values(self, t: torch.Tensor, name: str) -> int:
+        """The address of values of the cache's type on its device."""
+        p = t.data_ptr()
+        if t.dtype is not self.dtype or t.device != self.device or p & 15:
+            raise ValueError(f"{name} must be 16-byte aligned {self.dtype} on {self.device}, got {t.dtype} on {t.device}")
+        return p
+
+    def _vector(self, t: torch.Tensor, name: str, n: int) -> int:
         if t.device != self.device or t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous int32 [{n}] vector on {self.device}")
         return t.data_ptr()
@@ -193,39 +205,57 @@ class PagedKVCache:
         differ (after ``evict``).  Returns the turned queries, in ``q_out`` (which may be q) or a new
         tensor.  Rows behind the last sequence are left as they were, as are those of a negative
         length.  ``lengths`` is not advanced."""
-        n = k.shape[0]
-        ldk = self._heads(k, "k", self.kv_heads)
-        ldv = self._heads(v, "v", self.kv_heads)
-        if v.shape[0] != n:
-            raise ValueError(f"v has {v.shape[0]} rows, k {n}")
-        ldq = ldo = heads = 0
+        key = (None if q is None else (q.shape, q.stride()), k.shape, k.stride(), v.shape, v.stride())
+        plan = self._append_plans.get(key)
+        if plan is None:
+            plan = self._remember(self._append_plans, key, self._plan_append(q, k, v))
+        n, heads, ldq, ldk, ldv = plan
+        pk, pv = self._values(k, "k"), self._values(v, "v")
+        pq = po = ps = pp = None
+        ldo = 0
         if q is not None:
-            ldq = self._heads(q, "q")
-            heads = q.shape[1]
-            if q.shape[0] != n:
-                raise ValueError(f"q has {q.shape[0]} rows, k {n}")
+            pq, ldo = self._values(q, "q"), heads * self.head_dim
             if q_out is None:
-                q_out = torch.empty((n, heads, self.head_dim), dtype=self.dtype, device=self.device)
-                ldo = heads * self.head_dim
+                q_out = torch.empty_like(q)
             else:
+                if q_out.shape != q.shape:
+                    raise ValueError(f"q_out must have q's shape {tuple(q.shape)}, got {tuple(q_out.shape)}")
                 ldo = self._heads(q_out, "q_out", heads)
-                if q_out.shape[0] != n:
-                    raise ValueError(f"q_out has {q_out.shape[0]} rows, k {n}")
+            po = self._values(q_out, "q_out")
         elif q_out is not None:
             raise ValueError("q_out without q")
-        if starts is None and n % self.batch:
+        if starts is not None:
+            ps = self._vector(starts, "starts", self.batch + 1)
+        elif n % self.batch:
             raise ValueError(f"{n} rows do not divide among {self.batch} sequences; give starts")
-        if rotary is not None and (rotary.head_dim != self.head_dim or rotary.turns.device != self.device):
-            raise ValueError(f"rotary is for heads of {rotary.head_dim} on {rotary.turns.device}")
+        if positions is not None:
+            pp = self._vector(positions, "positions", n)
+        if rotary is not None and (rotary.head_dim != self.head_dim or rotary.device != self.device):
+            raise ValueError(f"rotary is for heads of {rotary.head_dim} on {rotary.device}")
         if n:
             with _on(self.device):
-                st = _native.lib().otf_paged_append(
-                    self._ref, None if rotary is None else rotary._ref, None if q is None else q.data_ptr(), ldq,
-                    None if q is None else q_out.data_ptr(), ldo, heads, k.data_ptr(), ldk, v.data_ptr(), ldv,
-                    None if starts is None else self._vector(starts, "starts", self.batch + 1),
-                    None if positions is None else self._vector(positions, "positions", n), n, _stream(self.device))
-            _native._check(st, "otf_paged_append")
+                st = _native.lib().otf_paged_append(self._ref, None if rotary is None else rotary._ref, pq, ldq, po, ldo,
+                                                    heads, pk, ldk, pv, ldv, ps, pp, n, _stream(self.device))
+            if st:
+                _native._check(st, "otf_paged_append")
         return q_out
+
+    def _plan_append(self, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor) -> tuple:
+        ldk, ldv = self._heads(k, "k", self.kv_heads), self._heads(v, "v", self.kv_heads)
+        n, heads, ldq = k.shape[0], 0, 0
+        if q is not None:
+            ldq, heads = self._heads(q, "q"), q.shape[1]
+        for name, t in (("v", v), ("q", q)):
+            if t is not None and t.shape[0] != n:
+                raise ValueError(f"{name} has {t.shape[0]} rows, k {n}")
+        return n, heads, ldq, ldk, ldv
+
+    @staticmethod
+    def _remember(plans: dict, key: tuple, plan: tuple) -> tuple:
+        if len(plans) >= 256:                               # prompts come in many lengths
+            plans.clear()
+        plans[key] = plan
+        return plan
 
     def attend(self, q: torch.Tensor, *, scale: Optional[float] = None, weights: Optional[torch.Tensor] = None,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -237,45 +267,51 @@ class PagedKVCache:
         ``weights`` (fp32 [batch, kv_heads, at least capacity], contiguous): to every token's entry
         is added the softmax weight that it received from the rows and the query heads of that KV
         head.  Returns ``out``, of q's shape (rows of negative lengths are left as they were)."""
-        shape = q.shape
-        if q.dim() == 3:
-            tokens, rows = 1, q
-        elif q.dim() == 4:
-            tokens = shape[1]
-            rows = q.flatten(0, 1) if q.is_contiguous() else self._flat(q, "q")
-        else:
-            raise ValueError(f"q must have 3 or 4 dimensions, got {tuple(shape)}")
-        if shape[0] != self.batch or not 1 <= tokens <= MAX_NEW_TOKENS:
-            raise ValueError(f"q must hold 1 to {MAX_NEW_TOKENS} tokens of {self.batch} sequences, got {tuple(shape)}")
-        ldq = self._heads(rows, "q")
-        heads = rows.shape[1]
-        if heads % self.kv_heads:
-            raise ValueError(f"{heads} query heads over {self.kv_heads} KV heads")
+        key = (q.shape, q.stride(), weights is None)
+        plan = self._attend_plans.get(key)
+        if plan is None:
+            plan = self._remember(self._attend_plans, key, self._plan_attend(q, weights))
+        tokens, heads, ldq, bytes_ = plan
+        pq, ldo = self._values(q, "q"), heads * self.head_dim
         if out is None:
-            out = torch.empty(shape, dtype=self.dtype, device=self.device)
-            ldo = heads * self.head_dim
+            out = torch.empty_like(q)
         else:
-            if out.shape != shape:
-                raise ValueError(f"out must have q's shape {tuple(shape)}, got {tuple(out.shape)}")
-            ldo = self._heads(out if out.dim() == 3 else self._flat(out, "out"), "out", heads)
-        ldw = 0
+            if out.shape != q.shape:
+                raise ValueError(f"out must have q's shape {tuple(q.shape)}, got {tuple(out.shape)}")
+            ldo = self._heads(self._flat(out, "out"), "out", heads)
+        po = self._values(out, "out")
+        if po == pq:
+            raise ValueError("out must not be q")
+        pw, ldw = None, 0
         if weights is not None:
             ldw = self._weights(weights, "weights", self.capacity)
-        L = _native.lib()
-        n = L.otf_paged_attn_workspace_bytes(self.batch, heads, self.kv_heads, self.head_dim, tokens, self.capacity,
-                                             0 if weights is None else 1)
-        if n < 0:
-            raise ValueError("shape not supported by otf_paged_attn")
+            pw = weights.data_ptr()
         # from the caching allocator, for this call alone: calls on two streams, or in two captured
         # graphs, share nothing
-        ws = torch.empty(n, dtype=torch.uint8, device=self.device)
+        ws = torch.empty(bytes_, dtype=torch.uint8, device=self.device)
         with _on(self.device):
-            st = L.otf_paged_attn(self._ref, rows.data_ptr(), ldq, heads, tokens,
-                                  self.head_dim ** -0.5 if scale is None else float(scale), out.data_ptr(), ldo,
-                                  None if weights is None else weights.data_ptr(), ldw, ws.data_ptr(), n,
-                                  _stream(self.device))
-        _native._check(st, "otf_paged_attn")
+            st = _native.lib().otf_paged_attn(self._ref, pq, ldq, heads, tokens,
+                                              self._scale if scale is None else float(scale), po, ldo, pw, ldw,
+                                              ws.data_ptr(), bytes_, _stream(self.device))
+        if st:
+            _native._check(st, "otf_paged_attn")
         return out
+
+    def _plan_attend(self, q: torch.Tensor, weights: Optional[torch.Tensor]) -> tuple:
+        if q.dim() not in (3, 4):
+            raise ValueError(f"q must have 3 or 4 dimensions, got {tuple(q.shape)}")
+        tokens = q.shape[1] if q.dim() == 4 else 1
+        if q.shape[0] != self.batch or not 1 <= tokens <= MAX_NEW_TOKENS:
+            raise ValueError(f"q must hold 1 to {MAX_NEW_TOKENS} tokens of {self.batch} sequences, got {tuple(q.shape)}")
+        rows = self._flat(q, "q")
+        ldq, heads = self._heads(rows, "q"), rows.shape[1]
+        if heads % self.kv_heads:
+            raise ValueError(f"{heads} query heads over {self.kv_heads} KV heads")
+        n = _native.lib().otf_paged_attn_workspace_bytes(self.batch, heads, self.kv_heads, self.head_dim, tokens,
+                                                         self.capacity, 0 if weights is None else 1)
+        if n < 0:
+            raise ValueError("shape not supported by otf_paged_attn")
+        return tokens, heads, ldq, n
 
     def evict(self, weights: torch.Tensor, budget: int, recent: int, *, to: Optional["PagedKVCache"] = None,
               weights_out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -328,6 +364,8 @@ class PagedKVCache:
     @staticmethod
     def _flat(t: torch.Tensor, name: str) -> torch.Tensor:
         """[batch, tokens, heads, dim] as rows, without a copy."""
+        if t.dim() == 3:
+            return t
         if t.shape[0] > 1 and t.shape[1] > 1 and t.stride(0) != t.shape[1] * t.stride(1):
             raise ValueError(f"{name} needs evenly strided rows, got strides {t.stride()}")
         row = t.stride(1) if t.shape[1] > 1 else t.stride(0)
@@ -351,4 +389,5 @@ def _on(dev: torch.device):
 
 
 def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    """The device's current stream, without the Stream object that torch.cuda.current_stream makes."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)

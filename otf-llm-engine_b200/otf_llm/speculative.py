@@ -18,21 +18,6 @@ from .paged import _on, _stream
 MAX_DRAFTS = 32
 
 
-def _rows3(t: torch.Tensor, name: str, shape, dev) -> Tuple[int, int]:
-    """Check fp32 [batch, rows, vocab] values with a unit inner stride; (sequence stride, row stride)."""
-    if t.device != dev or t.dtype != torch.float32 or tuple(t.shape) != shape or (t.stride(2) != 1 and shape[2] > 1):
-        raise ValueError(f"{name} must be fp32 {list(shape)} with a unit inner stride on {dev}, got {t.dtype} "
-                         f"{list(t.shape)} with strides {t.stride()} on {t.device}")
-    return (t.stride(0) if shape[0] > 1 else 0), (t.stride(1) if shape[1] > 1 else shape[2])
-
-
-def _rows2(t: torch.Tensor, name: str, dtype, shape, dev) -> int:
-    if t.device != dev or t.dtype != dtype or tuple(t.shape) != shape or (t.stride(1) != 1 and shape[1] > 1):
-        raise ValueError(f"{name} must be {dtype} {list(shape)} with a unit inner stride on {dev}, got {t.dtype} "
-                         f"{list(t.shape)} with strides {t.stride()} on {t.device}")
-    return t.stride(0) if shape[0] > 1 else shape[1]
-
-
 def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, *,
                   draft_logits: Optional[torch.Tensor] = None, uniforms: Optional[torch.Tensor] = None,
                   noise: Optional[torch.Tensor] = None, temperature: Union[float, torch.Tensor] = 1.0,
@@ -50,49 +35,93 @@ def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, *,
 
     Returns (tokens int64 [batch, drafts + 1]: the taken ones, the one that follows, then -1;
     accepted int32 [batch])."""
-    _native._need_cuda(target_logits, "target_logits")
-    dev = target_logits.device
-    if target_logits.dim() != 3 or target_logits.shape[0] == 0 or target_logits.shape[2] == 0:
-        raise ValueError(f"target_logits must be [batch, drafts + 1, vocab], got {list(target_logits.shape)}")
-    batch, drafts, vocab = target_logits.shape[0], target_logits.shape[1] - 1, target_logits.shape[2]
-    if not 0 <= drafts <= MAX_DRAFTS:
-        raise ValueError(f"0 to {MAX_DRAFTS} drafted tokens, got {drafts}")
-    seq_t, ld_t = _rows3(target_logits, "target_logits", (batch, drafts + 1, vocab), dev)
-    ld_tok = _rows2(draft_tokens, "draft_tokens", torch.int64, (batch, drafts), dev)
-    seq_d = ld_d = ld_u = ld_n = 0
+    key = (target_logits.device, target_logits.shape, target_logits.stride(), draft_tokens.shape, draft_tokens.stride(),
+           None if draft_logits is None else (draft_logits.shape, draft_logits.stride()),
+           None if uniforms is None else (uniforms.shape, uniforms.stride()),
+           None if noise is None else (noise.shape, noise.stride()))
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _plan(target_logits, draft_tokens, draft_logits, uniforms, noise)
+        if len(_plans) >= 256:
+            _plans.clear()
+        _plans[key] = plan
+    dev, batch, drafts, vocab, seq_t, ld_t, ld_tok, seq_d, ld_d, ld_u, ld_n, bytes_ = plan
+    pt, ptok = _address(target_logits, "target_logits", _F32, dev), _address(draft_tokens, "draft_tokens", torch.int64, dev)
+    pd = pu = pn = each = pc = None
+    one = 0.0
     if draft_logits is not None:
-        seq_d, ld_d = _rows3(draft_logits, "draft_logits", (batch, drafts, vocab), dev)
+        pd = _address(draft_logits, "draft_logits", _F32, dev)
     if uniforms is not None:
-        ld_u = _rows2(uniforms, "uniforms", torch.float32, (batch, drafts), dev)
+        pu = _address(uniforms, "uniforms", _F32, dev)
     if noise is not None:
-        ld_n = _rows2(noise, "noise", torch.float32, (batch, vocab), dev)
-    each, one = None, 0.0
+        pn = _address(noise, "noise", _F32, dev)
     if isinstance(temperature, torch.Tensor):
-        _rows2(temperature.view(1, -1), "temperature", torch.float32, (1, batch), dev)
-        each = temperature.data_ptr()
-        if noise is None or (drafts and uniforms is None):
-            raise ValueError("temperatures of each sequence need uniforms and noise")
+        each = _vector(temperature, "temperature", _F32, batch, dev)
     else:
         one = float(temperature)
         if not (one == 0.0 or 1e-20 <= one <= 1e20):
             raise ValueError(f"temperature must be 0, or positive and finite, got {one}")
-        if one > 0 and (noise is None or (drafts and uniforms is None)):
-            raise ValueError("a temperature above 0 needs uniforms and noise")
+    if (pn is None or (drafts and pu is None)) and (each is not None or one > 0):
+        raise ValueError("a temperature above 0 needs uniforms and noise")
     if counts is not None:
-        _rows2(counts.view(1, -1), "counts", torch.int32, (1, batch), dev)
+        pc = _vector(counts, "counts", torch.int32, batch, dev)
     tokens = torch.empty((batch, drafts + 1), dtype=torch.int64, device=dev)
     accepted = torch.empty(batch, dtype=torch.int32, device=dev)
-    L = _native.lib()
-    n = L.otf_verify_workspace_bytes(batch, drafts, vocab)
+    ws = torch.empty(bytes_, dtype=torch.uint8, device=dev)     # for this call alone, on its stream
+    with _on(dev):
+        st = _native.lib().otf_verify_drafts(pt, seq_t, ld_t, pd, seq_d, ld_d, ptok, ld_tok, pu, ld_u, pn, ld_n, each, one,
+                                             pc, tokens.data_ptr(), accepted.data_ptr(), batch, drafts, vocab,
+                                             ws.data_ptr(), bytes_, _stream(dev))
+    if st:
+        _native._check(st, "otf_verify_drafts")
+    return tokens, accepted
+
+
+_F32 = torch.float32
+# shapes and strides of earlier calls' arguments, with what their checks found
+_plans: dict = {}
+
+
+def _address(t: torch.Tensor, name: str, dtype: torch.dtype, dev: torch.device) -> int:
+    if t.dtype is not dtype or t.device != dev:
+        raise ValueError(f"{name} must be {dtype} on {dev}, got {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+def _vector(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, dev: torch.device) -> int:
+    if t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous [{n}] vector, got {list(t.shape)} with strides {t.stride()}")
+    return _address(t, name, dtype, dev)
+
+
+def _rows(t: torch.Tensor, name: str, shape: Tuple[int, ...]) -> Tuple[int, ...]:
+    """The strides of all dimensions but the last, whose values lie next to one another."""
+    if tuple(t.shape) != shape or (t.stride(-1) != 1 and shape[-1] > 1):
+        raise ValueError(f"{name} must be {list(shape)} with a unit inner stride, got {list(t.shape)} with strides "
+                         f"{t.stride()}")
+    if len(shape) == 2:
+        return (t.stride(0) if shape[0] > 1 else shape[1],)
+    return (t.stride(0) if shape[0] > 1 else 0), (t.stride(1) if shape[1] > 1 else shape[2])
+
+
+def _plan(target: torch.Tensor, tokens: torch.Tensor, draft: Optional[torch.Tensor], uniforms: Optional[torch.Tensor],
+          noise: Optional[torch.Tensor]) -> tuple:
+    _native._need_cuda(target, "target_logits")
+    if target.dim() != 3 or target.shape[0] == 0 or target.shape[1] == 0 or target.shape[2] == 0:
+        raise ValueError(f"target_logits must be [batch, drafts + 1, vocab], got {list(target.shape)}")
+    batch, drafts, vocab = target.shape[0], target.shape[1] - 1, target.shape[2]
+    if drafts > MAX_DRAFTS:
+        raise ValueError(f"0 to {MAX_DRAFTS} drafted tokens, got {drafts}")
+    seq_t, ld_t = _rows(target, "target_logits", (batch, drafts + 1, vocab))
+    ld_tok, = _rows(tokens, "draft_tokens", (batch, drafts))
+    seq_d = ld_d = ld_u = ld_n = 0
+    if draft is not None:
+        seq_d, ld_d = _rows(draft, "draft_logits", (batch, drafts, vocab))
+    if uniforms is not None:
+        ld_u, = _rows(uniforms, "uniforms", (batch, drafts))
+    if noise is not None:
+        ld_n, = _rows(noise, "noise", (batch, vocab))
+    n = _native.lib().otf_verify_workspace_bytes(batch, drafts, vocab)
     if n < 0:
         raise ValueError("shape not supported by otf_verify_drafts")
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        st = L.otf_verify_drafts(target_logits.data_ptr(), seq_t, ld_t,
-                                 None if draft_logits is None else draft_logits.data_ptr(), seq_d, ld_d,
-                                 draft_tokens.data_ptr(), ld_tok, None if uniforms is None else uniforms.data_ptr(),
-                                 ld_u, None if noise is None else noise.data_ptr(), ld_n, each, one,
-                                 None if counts is None else counts.data_ptr(), tokens.data_ptr(), accepted.data_ptr(),
-                                 batch, drafts, vocab, ws.data_ptr(), n, _stream(dev))
-    _native._check(st, "otf_verify_drafts")
-    return tokens, accepted
+    return target.device, batch, drafts, vocab, seq_t, ld_t, ld_tok, seq_d, ld_d, ld_u, ld_n, n
