@@ -114,7 +114,10 @@ __device__ __forceinline__ void store_row(uint16_t* y, const float (&v)[PL], flo
   for (int i = 0; i < PL / 2; ++i) reinterpret_cast<uint32_t*>(y)[i] = pack2<BF>(v[2 * i] * f, v[2 * i + 1] * f);
 }
 
-// 2^8 on fp16 probabilities: the largest is 256, and what lies 2^-32 below it still counts.
+// The running reference m of a row follows its maximum only when a score rises 2^7 above it, which
+// saves the reductions and rescalings of most steps: probabilities reach 2^(shift + 7), 2^15 in
+// fp16, and what lies 2^-32 below the reference still counts there.
+constexpr float kHeadroom = 7.0f;
 template <bool BF>
 constexpr float kProbShift = BF ? 0.0f : 8.0f;
 
@@ -408,42 +411,53 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
       uint32_t p[MT][KT / 16][4];
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
-        float mx[2] = {-INFINITY, -INFINITY};  // of the products, before the scale
+        // the exponents scale s - m + shift against the reference m; where one of them leaves the
+        // headroom (or a row has no reference yet) m becomes the true maximum so far
+        float e[KT / 8][4], top[2] = {-INFINITY, -INFINITY};
+        auto exponents = [&] {
+          const float z[2] = {kProbShift<BF> - (m[t][0] == -INFINITY ? 0.0f : m[t][0]),
+                              kProbShift<BF> - (m[t][1] == -INFINITY ? 0.0f : m[t][1])};
+#pragma unroll
+          for (int n = 0; n < KT / 8; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[n][i] = fmaf(s[t][n][i], scale, z[i >> 1]);
+        };
+        exponents();
 #pragma unroll
         for (int n = 0; n < KT / 8; ++n) {
-          mx[0] = fmaxf(mx[0], fmaxf(s[t][n][0], s[t][n][1]));
-          mx[1] = fmaxf(mx[1], fmaxf(s[t][n][2], s[t][n][3]));
+          top[0] = fmaxf(top[0], fmaxf(e[n][0], e[n][1]));
+          top[1] = fmaxf(top[1], fmaxf(e[n][2], e[n][3]));
         }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-          mx[h] = fmaxf(mx[h], m[t][h]);
-        }
-        if (__any_sync(0xffffffffu, mx[0] != m[t][0] || mx[1] != m[t][1])) {
+        const bool grow = top[0] > (m[t][0] == -INFINITY ? -INFINITY : kProbShift<BF> + kHeadroom) ||
+                          top[1] > (m[t][1] == -INFINITY ? -INFINITY : kProbShift<BF> + kHeadroom);
+        if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float f = m[t][h] == -INFINITY ? 0.0f : ex2((m[t][h] - mx[h]) * scale);
+            float mx = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < KT / 8; ++n) mx = fmaxf(mx, fmaxf(s[t][n][2 * h], s[t][n][2 * h + 1]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            mx = fmaxf(mx * scale, m[t][h]);
+            const float f = m[t][h] == -INFINITY ? 0.0f : ex2(m[t][h] - mx);
             l[t][h] *= f;
 #pragma unroll
             for (int j = 0; j < D / 8; ++j) {
               o[t][j][2 * h] *= f;
               o[t][j][2 * h + 1] *= f;
             }
-            m[t][h] = mx[h];
+            m[t][h] = mx;
           }
+          exponents();
         }
-        // 2^(scale (s - m) + shift): one multiply-add and one exponential per entry
-        const float z[2] = {kProbShift<BF> - (m[t][0] == -INFINITY ? 0.0f : m[t][0] * scale),
-                            kProbShift<BF> - (m[t][1] == -INFINITY ? 0.0f : m[t][1] * scale)};
 #pragma unroll
         for (int n = 0; n < KT / 8; ++n) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[t][n][i] = ex2(fmaf(s[t][n][i], scale, z[i >> 1]));
-          l[t][0] += s[t][n][0] + s[t][n][1];
-          l[t][1] += s[t][n][2] + s[t][n][3];
-          p[t][n >> 1][(n & 1) * 2] = pack2<BF>(s[t][n][0], s[t][n][1]);
-          p[t][n >> 1][(n & 1) * 2 + 1] = pack2<BF>(s[t][n][2], s[t][n][3]);
+          for (int i = 0; i < 4; ++i) e[n][i] = ex2(e[n][i]);
+          l[t][0] += e[n][0] + e[n][1];
+          l[t][1] += e[n][2] + e[n][3];
+          p[t][n >> 1][(n & 1) * 2] = pack2<BF>(e[n][0], e[n][1]);
+          p[t][n >> 1][(n & 1) * 2 + 1] = pack2<BF>(e[n][2], e[n][3]);
         }
       }
 #pragma unroll
@@ -500,7 +514,7 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
           x += __shfl_xor_sync(0xffffffffu, x, 2);
           const int w = h * 8 + (lane >> 2);
           if ((lane & 3) == 0) {
-            s_m[warp * 16 + w] = m[t][h] * scale;
+            s_m[warp * 16 + w] = m[t][h];
             s_l[warp * 16 + w] = x;
           }
 #pragma unroll
@@ -589,19 +603,27 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
   cp_async_wait<0>();
 }
 
-// The parts of an item that several CTAs shared, joined in the cache's order: grid (items, row
-// groups), a warp per row.  Latency-bound: the parts' m and l come together, then eight parts at a
-// time.  40 registers, so that its CTAs find room beside the last of the attention's.
+// The parts of an item that several CTAs shared, joined in the cache's order: grid (items, groups of 4
+// rows).  Latency-bound: a warp finds one row's M, L and its parts' factors, then every warp adds up a
+// quarter of the parts for all four rows, so that the loads of many parts are in flight.
+constexpr int kJoinWarps = 4;
+
 template <bool BF, int D>
-__global__ void __launch_bounds__(128, 12) k_paged_attn_join(AttnArgs a, int RB) {
-  constexpr int PL = D / 32;
+__global__ void __launch_bounds__(kJoinWarps * 32) k_paged_attn_join(AttnArgs a, int RB) {
+  constexpr int PL = D / 32, W = kJoinWarps;
+  __shared__ float s_f[W][kPaGrid];
+  __shared__ float s_l[W], s_m[W];
+  __shared__ __align__(16) float s_o[W][W][D];
   pdl_trigger();
   const PagedView& c = a.c;
   const int items = c.kv_heads * a.blocks;
   const int b = blockIdx.x / items, item = blockIdx.x - b * items, g = item / a.blocks, rb = item - g * a.blocks;
-  const int lane = threadIdx.x & 31, r = blockIdx.y * 4 + (threadIdx.x >> 5), rr = rb * RB + r;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r0 = blockIdx.y * W;
+  if (rb * RB + r0 >= a.rows) {
+    pdl_wait();
+    return;
+  }
   pdl_wait();
-  if (r >= RB || rr >= a.rows) return;
   const int64_t p0 = a.prefix[b], p1 = a.prefix[b + 1], total = a.prefix[c.batch];
   if (p0 == p1) return;
   // the CTAs whose runs meet the item's chunks, units [c0, c1) behind its kPaItemUnits: 32-bit
@@ -621,45 +643,66 @@ __global__ void __launch_bounds__(128, 12) k_paged_attn_join(AttnArgs a, int RB)
     second = i0 * total / ctas < at;
   }
   if (i0 == i1) return;  // one CTA had it whole
-  auto part = [&](int i) { return (2 * i + (i == i0 && second ? 1 : 0)) * RB + r; };
-  float M = -INFINITY, L = 0.0f, acc[PL];
+  const int n = i1 + 1 - i0;
+  auto part = [&](int i) { return (2 * (i0 + i) + (i == 0 && second ? 1 : 0)) * RB + r0; };
+  {
+    float M = -INFINITY, L = 0.0f;
+    for (int i = lane; i < n; i += 32) M = fmaxf(M, a.part_ml[part(i) + warp].x);
 #pragma unroll
-  for (int i = 0; i < PL; ++i) acc[i] = 0.0f;
-  for (int i = i0 + lane; i <= i1; i += 32) M = fmaxf(M, a.part_ml[part(i)].x);
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-  for (int base = i0; base <= i1; base += 32) {
-    float f = 0.0f;  // a lane holds one part's factor
-    if (base + lane <= i1) {
-      const float2 ml = a.part_ml[part(base + lane)];
-      if (ml.y != 0.0f) {
-        f = ex2(ml.x - M);
-        L = fmaf(ml.y, f, L);
-      }
+    for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+    for (int i = lane; i < n; i += 32) {
+      const float2 ml = a.part_ml[part(i) + warp];
+      const float f = ml.y == 0.0f ? 0.0f : ex2(ml.x - M);
+      s_f[warp][i] = f;
+      L = fmaf(ml.y, f, L);
     }
-    const int n = min(32, i1 + 1 - base);
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float w = __shfl_sync(0xffffffffu, f, i);
-      const float* x = a.part + (int64_t)part(base + i) * D + lane * PL;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+    if (lane == 0) {
+      s_m[warp] = M;
+      s_l[warp] = L;
+    }
+  }
+  __syncthreads();
+  float acc[W][PL];
+#pragma unroll
+  for (int r = 0; r < W; ++r)
+#pragma unroll
+    for (int j = 0; j < PL; ++j) acc[r][j] = 0.0f;
+#pragma unroll 2
+  for (int i = warp; i < n; i += W) {
+    const float* x = a.part + (int64_t)part(i) * D + lane * PL;
+#pragma unroll
+    for (int r = 0; r < W; ++r) {
+      const float f = s_f[r][i];
       if (D == 128) {
-        const float4 y = *reinterpret_cast<const float4*>(x);
-        acc[0] = fmaf(y.x, w, acc[0]);
-        acc[1] = fmaf(y.y, w, acc[1]);
-        acc[PL - 2] = fmaf(y.z, w, acc[PL - 2]);
-        acc[PL - 1] = fmaf(y.w, w, acc[PL - 1]);
+        const float4 y = *reinterpret_cast<const float4*>(x + r * D);
+        acc[r][0] = fmaf(y.x, f, acc[r][0]);
+        acc[r][1] = fmaf(y.y, f, acc[r][1]);
+        acc[r][PL - 2] = fmaf(y.z, f, acc[r][PL - 2]);
+        acc[r][PL - 1] = fmaf(y.w, f, acc[r][PL - 1]);
       } else {
-        const float2 y = *reinterpret_cast<const float2*>(x);
-        acc[0] = fmaf(y.x, w, acc[0]);
-        acc[1] = fmaf(y.y, w, acc[1]);
+        const float2 y = *reinterpret_cast<const float2*>(x + r * D);
+        acc[r][0] = fmaf(y.x, f, acc[r][0]);
+        acc[r][1] = fmaf(y.y, f, acc[r][1]);
       }
     }
   }
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+  for (int r = 0; r < W; ++r)
+#pragma unroll
+    for (int j = 0; j < PL; ++j) s_o[warp][r][lane * PL + j] = acc[r][j];
+  __syncthreads();
+  const int rr = rb * RB + r0 + warp;
+  if (rr >= a.rows) return;
+  float sum[PL];
+#pragma unroll
+  for (int j = 0; j < PL; ++j)
+    sum[j] = (s_o[0][warp][lane * PL + j] + s_o[1][warp][lane * PL + j]) +
+             (s_o[2][warp][lane * PL + j] + s_o[3][warp][lane * PL + j]);
   const int tok = rr / a.rep, head = g * a.rep + rr - tok * a.rep;
-  store_row<BF, PL>(a.out + ((int64_t)b * a.tokens + tok) * a.ldo + (int64_t)head * D + lane * PL, acc, 1.0f / L);
-  if (a.lse && lane == 0) a.lse[((int64_t)b * c.kv_heads + g) * a.rows + rr] = M + log2f(L) - kProbShift<BF>;
+  store_row<BF, PL>(a.out + ((int64_t)b * a.tokens + tok) * a.ldo + (int64_t)head * D + lane * PL, sum, 1.0f / s_l[warp]);
+  if (a.lse && lane == 0) a.lse[((int64_t)b * c.kv_heads + g) * a.rows + rr] = s_m[warp] + log2f(s_l[warp]) - kProbShift<BF>;
 }
 
 // weights[b, g, s] += sum over the item rows of 2^(score - lse).  One thread per token, rows in order.
