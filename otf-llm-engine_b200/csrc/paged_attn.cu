@@ -603,29 +603,25 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
   cp_async_wait<0>();
 }
 
-// The parts of an item that several CTAs shared, joined in the cache's order: grid (items, groups of 4
-// rows).  Latency-bound: a warp finds one row's M, L and its parts' factors, then every warp adds up a
-// quarter of the parts for all four rows, so that the loads of many parts are in flight.
+// The parts of an item that several CTAs shared, joined in the cache's order: grid (items, rows / rows
+// of a CTA), WR of the CTA's four warps on a row, each adding up every WR-th part.  Latency-bound:
+// after the parts' m and l come their o, eight in flight per warp.
 constexpr int kJoinWarps = 4;
 
-template <bool BF, int D>
+template <bool BF, int D, int WR>
 __global__ void __launch_bounds__(kJoinWarps * 32) k_paged_attn_join(AttnArgs a, int RB) {
   constexpr int PL = D / 32, W = kJoinWarps;
-  __shared__ float s_f[W][kPaGrid];
-  __shared__ float s_l[W], s_m[W];
-  __shared__ __align__(16) float s_o[W][W][D];
+  __shared__ float s_l[W];
+  __shared__ __align__(16) float s_o[WR > 1 ? W : 1][D];
   pdl_trigger();
   const PagedView& c = a.c;
   const int items = c.kv_heads * a.blocks;
   const int b = blockIdx.x / items, item = blockIdx.x - b * items, g = item / a.blocks, rb = item - g * a.blocks;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r0 = blockIdx.y * W;
-  if (rb * RB + r0 >= a.rows) {
-    pdl_wait();
-    return;
-  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WR;
+  const int r = blockIdx.y * (W / WR) + warp / WR, rr = rb * RB + r;
   pdl_wait();
   const int64_t p0 = a.prefix[b], p1 = a.prefix[b + 1], total = a.prefix[c.batch];
-  if (p0 == p1) return;
+  if (p0 == p1 || rr >= a.rows) return;  // with WR > 1 the whole CTA
   // the CTAs whose runs meet the item's chunks, units [c0, c1) behind its kPaItemUnits: 32-bit
   // divisions where they do; and whether the item is not the first of CTA i0's run
   const int64_t ctas = min((int64_t)kPaGrid, total);
@@ -644,65 +640,66 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_paged_attn_join(AttnArgs a,
   }
   if (i0 == i1) return;  // one CTA had it whole
   const int n = i1 + 1 - i0;
-  auto part = [&](int i) { return (2 * (i0 + i) + (i == 0 && second ? 1 : 0)) * RB + r0; };
-  {
-    float M = -INFINITY, L = 0.0f;
-    for (int i = lane; i < n; i += 32) M = fmaxf(M, a.part_ml[part(i) + warp].x);
+  auto part = [&](int i) { return (2 * (i0 + i) + (i == 0 && second ? 1 : 0)) * RB + r; };
+  float M = -INFINITY, L = 0.0f, acc[PL];
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-    for (int i = lane; i < n; i += 32) {
-      const float2 ml = a.part_ml[part(i) + warp];
-      const float f = ml.y == 0.0f ? 0.0f : ex2(ml.x - M);
-      s_f[warp][i] = f;
+  for (int j = 0; j < PL; ++j) acc[j] = 0.0f;
+#pragma unroll 4
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, a.part_ml[part(i)].x);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+  for (int base = sub; base < n; base += 8 * WR) {
+    float x[8][PL], f = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = base + k * WR;
+      const float* y = a.part + (int64_t)part(min(i, n - 1)) * D + lane * PL;
+      if (D == 128) {
+        const float4 z = *reinterpret_cast<const float4*>(y);
+        x[k][0] = z.x;
+        x[k][1] = z.y;
+        x[k][PL - 2] = z.z;
+        x[k][PL - 1] = z.w;
+      } else {
+        const float2 z = *reinterpret_cast<const float2*>(y);
+        x[k][0] = z.x;
+        x[k][1] = z.y;
+      }
+    }
+    if (lane < 8 && base + lane * WR < n) {  // lane k holds the factor of the k-th of them
+      const float2 ml = a.part_ml[part(base + lane * WR)];
+      f = ml.y == 0.0f ? 0.0f : ex2(ml.x - M);
       L = fmaf(ml.y, f, L);
     }
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
-    if (lane == 0) {
-      s_m[warp] = M;
-      s_l[warp] = L;
-    }
-  }
-  __syncthreads();
-  float acc[W][PL];
+    for (int k = 0; k < 8; ++k) {
+      const float w = __shfl_sync(0xffffffffu, f, k);
+      if (base + k * WR < n)
 #pragma unroll
-  for (int r = 0; r < W; ++r)
-#pragma unroll
-    for (int j = 0; j < PL; ++j) acc[r][j] = 0.0f;
-#pragma unroll 2
-  for (int i = warp; i < n; i += W) {
-    const float* x = a.part + (int64_t)part(i) * D + lane * PL;
-#pragma unroll
-    for (int r = 0; r < W; ++r) {
-      const float f = s_f[r][i];
-      if (D == 128) {
-        const float4 y = *reinterpret_cast<const float4*>(x + r * D);
-        acc[r][0] = fmaf(y.x, f, acc[r][0]);
-        acc[r][1] = fmaf(y.y, f, acc[r][1]);
-        acc[r][PL - 2] = fmaf(y.z, f, acc[r][PL - 2]);
-        acc[r][PL - 1] = fmaf(y.w, f, acc[r][PL - 1]);
-      } else {
-        const float2 y = *reinterpret_cast<const float2*>(x + r * D);
-        acc[r][0] = fmaf(y.x, f, acc[r][0]);
-        acc[r][1] = fmaf(y.y, f, acc[r][1]);
-      }
+        for (int j = 0; j < PL; ++j) acc[j] = fmaf(x[k][j], w, acc[j]);
     }
   }
 #pragma unroll
-  for (int r = 0; r < W; ++r)
+  for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+  if (WR > 1) {
+    if (lane == 0) s_l[warp] = L;
 #pragma unroll
-    for (int j = 0; j < PL; ++j) s_o[warp][r][lane * PL + j] = acc[r][j];
-  __syncthreads();
-  const int rr = rb * RB + r0 + warp;
-  if (rr >= a.rows) return;
-  float sum[PL];
+    for (int j = 0; j < PL; ++j) s_o[warp % (WR > 1 ? W : 1)][lane * PL + j] = acc[j];
+    __syncthreads();
+    if (sub) return;
+    L = 0.0f;
 #pragma unroll
-  for (int j = 0; j < PL; ++j)
-    sum[j] = (s_o[0][warp][lane * PL + j] + s_o[1][warp][lane * PL + j]) +
-             (s_o[2][warp][lane * PL + j] + s_o[3][warp][lane * PL + j]);
+    for (int j = 0; j < PL; ++j) acc[j] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WR; ++w) {
+      L += s_l[warp + w];
+#pragma unroll
+      for (int j = 0; j < PL; ++j) acc[j] += s_o[(warp + w) % (WR > 1 ? W : 1)][lane * PL + j];
+    }
+  }
   const int tok = rr / a.rep, head = g * a.rep + rr - tok * a.rep;
-  store_row<BF, PL>(a.out + ((int64_t)b * a.tokens + tok) * a.ldo + (int64_t)head * D + lane * PL, sum, 1.0f / s_l[warp]);
-  if (a.lse && lane == 0) a.lse[((int64_t)b * c.kv_heads + g) * a.rows + rr] = s_m[warp] + log2f(s_l[warp]) - kProbShift<BF>;
+  store_row<BF, PL>(a.out + ((int64_t)b * a.tokens + tok) * a.ldo + (int64_t)head * D + lane * PL, acc, 1.0f / L);
+  if (a.lse && lane == 0) a.lse[((int64_t)b * c.kv_heads + g) * a.rows + rr] = M + log2f(L) - kProbShift<BF>;
 }
 
 // weights[b, g, s] += sum over the item rows of 2^(score - lse).  One thread per token, rows in order.
@@ -770,8 +767,15 @@ static cudaError_t launch_attn(const AttnArgs& a, float* weights, int64_t ldw, c
   }
   cudaError_t e = launch_pdl(k, dim3(kPaGrid), dim3(kPaThreads), dyn, s, 1u, a);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(k_paged_attn_join<BF, D>, dim3((unsigned)(a.c.batch * a.c.kv_heads * a.blocks), (unsigned)(std::min(a.rows, RB) + 3) / 4),
-                 dim3(128), 0, s, 1u, a, RB);
+  // Few rows are shared by many CTAs each: a join CTA per row, its four warps on a quarter of the parts
+  // each; many rows by few: a warp per row.
+  const int64_t items = (int64_t)a.c.batch * a.c.kv_heads * a.blocks;
+  const int rows = std::min(a.rows, RB);
+  if (items * rows <= kPaGrid * 4)
+    e = launch_pdl(k_paged_attn_join<BF, D, 4>, dim3((unsigned)items, (unsigned)rows), dim3(kJoinWarps * 32), 0, s, 1u, a, RB);
+  else
+    e = launch_pdl(k_paged_attn_join<BF, D, 1>, dim3((unsigned)items, (unsigned)(rows + 3) / 4), dim3(kJoinWarps * 32), 0, s,
+                   1u, a, RB);
   if (e != cudaSuccess || !weights) return e;
   return launch_pdl(k_paged_attn_weights,
                     dim3((unsigned)((a.c.capacity + 255) / 256), (unsigned)a.c.kv_heads, (unsigned)a.c.batch), dim3(256), 0,
