@@ -202,12 +202,12 @@ constexpr int kEvictThreads = 512;
 constexpr int kEvictKeys = 16;       // weights of a thread
 constexpr int kEvictStrip = kEvictThreads * kEvictKeys;
 constexpr int kEvictCluster = 8;     // CTAs that may share one (sequence, KV head)
-constexpr int kEvictSlice = 4096;    // weights that a CTA takes before others join it
+constexpr int kEvictBins = 2048;     // 11, 11 and 10 bits in three rounds
 
 // Which places stay: a cluster per (sequence, KV head), each CTA a contiguous slice of the n
-// weights that are not among the recent ones, a thread 16 neighbours.  Four rounds of 8 bits
-// find the k-th largest key (each round: counts of the slice's keys in shared memory, summed over
-// the cluster through distributed shared memory); then every CTA, knowing how many kept keys
+// weights that are not among the recent ones, a thread 16 neighbours.  Three rounds of 11,
+// 11 and 10 bits find the k-th largest key (each round: counts of the slice's keys in shared memory,
+// summed over the cluster through distributed shared memory); then every CTA, knowing how many kept keys
 // lie before its slice, writes its places in order.  Of the keys equal to the k-th largest the
 // first ones stay.  Bound by the rounds' latencies, not by bytes: ONE holds the keys of a
 // slice of up to kEvictStrip in registers through all rounds, longer ones are read again (from L2).
@@ -216,11 +216,10 @@ __global__ void __launch_bounds__(kEvictThreads) k_evict_select(const int* lengt
                                                                 const float* weights, int64_t ldw, int budget,
                                                                 int recent, int* kept, int ctas) {
   constexpr int W = kEvictThreads / 32, V = kEvictKeys;
-  __shared__ int s_hist[4][256];
-  __shared__ int s_sum[256];
+  __shared__ __align__(16) int s_hist[3][kEvictBins];
   __shared__ int s_cut[2];    // this round's digit, and how many keys of it are needed
   __shared__ int s_count[2];  // the slice's keys above and at the limit
-  __shared__ uint32_t s_warp[W];
+  __shared__ int s_warp[W];
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -265,60 +264,69 @@ __global__ void __launch_bounds__(kEvictThreads) k_evict_select(const int* lengt
     return there;
   };
   int there = ONE ? load(i0) : 0;
-  for (int i = tid; i < 4 * 256; i += kEvictThreads) (&s_hist[0][0])[i] = 0;
+  for (int i = tid; i < 3 * kEvictBins / 4; i += kEvictThreads)
+    reinterpret_cast<int4*>(&s_hist[0][0])[i] = make_int4(0, 0, 0, 0);
   if (tid < 2) s_count[tid] = 0;
   __syncthreads();
   uint32_t limit = 0u, mask = 0u;
   int need = k;
 #pragma unroll 1
-  for (int round = 0; round < 4; ++round) {
-    const int shift = 24 - 8 * round;
+  for (int round = 0; round < 3; ++round) {
+    const int shift = round == 0 ? 21 : round == 1 ? 10 : 0;
+    const uint32_t bits = round == 2 ? 1023u : 2047u;
     for (int base = i0; base < i1; base += kEvictStrip) {
       if (!ONE) there = load(base);
 #pragma unroll
       for (int z = 0; z < V; ++z)
-        if (z < there && (u[z] & mask) == limit) atomicAdd(&s_hist[round][(u[z] >> shift) & 255u], 1);
+        if (z < there && (u[z] & mask) == limit) atomicAdd(&s_hist[round][(u[z] >> shift) & bits], 1);
     }
     if (ctas > 1) cluster_sync_all(); else __syncthreads();
-    if (tid < 256) {
-      int sum = 0;
-      if (ctas > 1) {
-        const uint32_t at = smem_u32(&s_hist[round][tid]);
-        for (int r = 0; r < ctas; ++r) sum += ld_cluster_s32(mapa_shared(at, r));
-      } else {
-        sum = s_hist[round][tid];
-      }
-      s_sum[tid] = sum;
-    }
-    __syncthreads();
-    if (warp == 0) {  // lane l holds the digits 255 - 8 l and the seven below
-      int c[8], mine = 0;
+    // thread t: the 4 digits from kEvictBins - 1 - 4 t downwards
+    int4 c = make_int4(0, 0, 0, 0);
+    const int* mine = &s_hist[round][kEvictBins - 4 - 4 * tid];
+    if (ctas > 1) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mine += c[i] = s_sum[255 - 8 * lane - i];
-      int before = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += x;
-      }
-      before -= mine;
-      if (before < need && before + mine >= need) {
-        bool found = false;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (!found && before + c[i] >= need) {
-            found = true;
-            s_cut[0] = 255 - 8 * lane - i;
-            s_cut[1] = need - before;
-          }
-          before += c[i];
+      for (int r = 0; r < kEvictCluster; ++r)
+        if (r < ctas) {
+          const int4 x = ld_cluster_v4(mapa_shared(smem_u32(mine), r));
+          c.x += x.x;
+          c.y += x.y;
+          c.z += x.z;
+          c.w += x.w;
         }
+    } else {
+      c = *reinterpret_cast<const int4*>(mine);
+    }
+    const int all = (c.x + c.y) + (c.z + c.w);
+    int before = all;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += x;
+    }
+    if (lane == 31) s_warp[warp] = before;
+    __syncthreads();
+    before -= all;
+#pragma unroll
+    for (int x = 0; x < W; ++x)
+      if (x < warp) before += s_warp[x];
+    if (before < need && before + all >= need) {  // one thread's
+      const int d[4] = {c.w, c.z, c.y, c.x};
+      bool found = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (!found && before + d[i] >= need) {
+          found = true;
+          s_cut[0] = kEvictBins - 1 - 4 * tid - i;
+          s_cut[1] = need - before;
+        }
+        before += d[i];
       }
     }
     __syncthreads();
     limit |= (uint32_t)s_cut[0] << shift;
     need = s_cut[1];
-    mask |= 255u << shift;
+    mask |= bits << shift;
   }
   // keys above the limit in the low, at it in the high half
   auto count = [&] {
@@ -360,13 +368,13 @@ __global__ void __launch_bounds__(kEvictThreads) k_evict_select(const int* lengt
       const uint32_t x = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += x;
     }
-    if (lane == 31) s_warp[warp] = inc;
+    if (lane == 31) s_warp[warp] = (int)inc;
     __syncthreads();
     uint32_t before = 0, all = 0;
 #pragma unroll
     for (int x = 0; x < W; ++x) {
       if (x == warp) before = all;
-      all += s_warp[x];
+      all += (uint32_t)s_warp[x];
     }
     before += inc - mine;
     int g = g0 + (int)(before & 0xffffu), e = e0 + (int)(before >> 16);
@@ -634,10 +642,10 @@ extern "C" OTF_API int otf_paged_evict(const otf_paged_cache* from, const otf_pa
   if (in_place != (weights == weights_out) || in_place != (lengths_out == from->lengths)) return OTF_ERR_INVALID;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t pairs = f.batch * (int64_t)f.kv_heads;
-  // CTAs per (sequence, KV head): one for every kEvictSlice weights that there can be, while that
-  // leaves less than two CTAs per SM
+  // CTAs per (sequence, KV head): as many as hold the weights that there can be in registers, while
+  // that leaves less than two CTAs per SM
   int ctas = 1;
-  while (ctas < otf::kEvictCluster && (int64_t)ctas * otf::kEvictSlice < f.capacity && pairs * ctas <= 148) ctas *= 2;
+  while (ctas < otf::kEvictCluster && (int64_t)ctas * otf::kEvictStrip < f.capacity && pairs * ctas <= 148) ctas *= 2;
   const bool one = (((f.capacity + ctas - 1) / ctas + 3) & ~3) <= otf::kEvictStrip;
   cudaError_t e = otf::launch_pdl(one ? otf::k_evict_select<true> : otf::k_evict_select<false>, dim3((unsigned)(pairs * ctas)), dim3(otf::kEvictThreads), 0, s,
                                   (unsigned)ctas, f.lengths, f.kv_heads, f.capacity, weights, ldw, (int)budget,

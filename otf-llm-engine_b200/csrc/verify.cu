@@ -17,13 +17,13 @@ int check_device();                  // capi.cu
 int verify_device_error(int clear);  // read (and optionally clear) the flag below
 
 constexpr int kVerifyMaxDrafts = 32;
-constexpr int kVerifySeg = 8192;     // logits of a row that one CTA reads
+constexpr int kVerifySeg = 1024;     // logits of a row that one warp reads
 constexpr int kVerifyThreads = 256;
 
 // Set when a sequence has no token to draw, or an argument on the device is out of range.
 __device__ int g_verify_device_error;
 
-// What one CTA found in its part of a row: the largest logit, its first index, and the sum of
+// What one warp found in its part of a row: the largest logit, its first index, and the sum of
 // exp((x - max) / T).
 struct __align__(16) RowPart {
   float max, sum;
@@ -100,98 +100,56 @@ struct VerifyArgs {
   }
 };
 
-// One pass over the logits: grid (segments, row groups, batch).  A thread holds its 32 values of a row's
-// segment in registers: their maximum, then the sum of exponentials under it, joined over the CTA.
-// Memory-bound, 7 instructions per logit.  A CTA goes through its group's rows, so that rows that
-// a sequence with fewer drafted tokens does not have cost nothing.
+// One pass over the logits: grid (blocks of 8 segments, row groups, batch), a warp per segment.  A lane
+// holds its 32 values of a row's segment in registers: the warp's maximum, then the sum of
+// exponentials under it.  Memory-bound, 7 instructions per logit; the warps of a CTA never meet.  A
+// CTA goes through its group's rows, so that rows that a sequence with fewer drafted tokens does
+// not have cost nothing.
 __global__ void __launch_bounds__(kVerifyThreads) k_verify_rows(VerifyArgs a) {
-  constexpr int N = kVerifySeg / (4 * kVerifyThreads), W = kVerifyThreads / 32;
-  __shared__ float s_m[W], s_s[W];
-  __shared__ int s_i[W];
+  constexpr int N = kVerifySeg / 128;
   pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.z, lane = threadIdx.x & 31, seg = blockIdx.x * (kVerifyThreads / 32) + (threadIdx.x >> 5);
+  if (seg >= a.segs) return;
   const float T = a.temp(b);
   const int n = a.count(b), rows = a.rows(b, n, T);
-  const int i0 = blockIdx.x * kVerifySeg + 4 * threadIdx.x;
+  const int i0 = seg * kVerifySeg + 4 * lane;
   const float c_hi = (float)(1.4426950408889634 / (double)T);
   const float c_lo = (float)(1.4426950408889634 / (double)T - (double)c_hi);
-  auto term = [&](float x, float max) {  // 0 for -inf and NaN (the maximum drops a NaN)
-    const float d = x - max;
-    return ex2(fmaxf(fmaf(d, c_hi, d * c_lo), -200.0f));
-  };
   for (int r = blockIdx.y; r < rows; r += gridDim.y) {
     const float* x = a.row(b, n, r);
-    RowPart* to = a.parts + a.part(b, n, r) + blockIdx.x;
     const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
     float4 v[N];
 #pragma unroll
-    for (int z = 0; z < N; ++z) v[z] = logits4(x, i0 + z * 4 * kVerifyThreads, a.vocab, aligned);
+    for (int z = 0; z < N; ++z) v[z] = logits4(x, i0 + z * 128, a.vocab, aligned);
     float m = -INFINITY;  // a NaN is never the largest
 #pragma unroll
     for (int z = 0; z < N; ++z) m = fmaxf(m, fmaxf(fmaxf(v[z].x, v[z].y), fmaxf(v[z].z, v[z].w)));
-    if (T == 0.0f) {
-      int at = INT_MAX;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float s = 0.0f;
+    int at = INT_MAX;
+    if (T == 0.0f) {  // the first of the largest
 #pragma unroll
       for (int z = N - 1; z >= 0; --z) {
         const float e[4] = {v[z].x, v[z].y, v[z].z, v[z].w};
 #pragma unroll
-        for (int w = 3; w >= 0; --w) {
-          const int i = i0 + z * 4 * kVerifyThreads + w;
-          if (e[w] == m && i < a.vocab) at = i;
-        }
+        for (int w = 3; w >= 0; --w)
+          if (e[w] == m && i0 + z * 128 + w < a.vocab) at = i0 + z * 128 + w;
       }
+      at = __reduce_min_sync(0xffffffffu, at);
+    } else {
+      const float mt = m == -INFINITY ? 0.0f : m;  // nothing but -inf: the sum is 0
+      auto term = [&](float x) {  // 0 for -inf and NaN (the maximum drops a NaN)
+        const float d = x - mt;
+        return ex2(fmaxf(fmaf(d, c_hi, d * c_lo), -200.0f));
+      };
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
-        const int a2 = __shfl_xor_sync(0xffffffffu, at, o);
-        if (m2 > m || (m2 == m && a2 < at)) {
-          m = m2;
-          at = a2;
-        }
-      }
-      __syncthreads();  // the row before is done with
-      if (lane == 0) {
-        s_m[warp] = m;
-        s_i[warp] = at;
-      }
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        for (int w = 1; w < W; ++w)
-          if (s_m[w] > m || (s_m[w] == m && s_i[w] < at)) {
-            m = s_m[w];
-            at = s_i[w];
-          }
-        *to = RowPart{m, 0.0f, at, 0};
-      }
-      continue;
-    }
-    const float mt = m == -INFINITY ? 0.0f : m;  // nothing but -inf: the sum is 0
-    float s = 0.0f;
+      for (int z = 0; z < N; ++z) s += (term(v[z].x) + term(v[z].y)) + (term(v[z].z) + term(v[z].w));
 #pragma unroll
-    for (int z = 0; z < N; ++z)
-      if (i0 + z * 4 * kVerifyThreads < a.vocab)
-        s += (term(v[z].x, mt) + term(v[z].y, mt)) + (term(v[z].z, mt) + term(v[z].w, mt));
-    auto join = [&](float m2, float s2) {
-      const float M = fmaxf(m, m2);
-      if (M != -INFINITY) s = s * term(m, M) + s2 * term(m2, M);  // else both are 0
-      m = M;
-    };
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-      join(m2, s2);
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     }
-    __syncthreads();
-    if (lane == 0) {
-      s_m[warp] = m;
-      s_s[warp] = s;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int w = 1; w < W; ++w) join(s_m[w], s_s[w]);
-      *to = RowPart{m, s, INT_MAX, 0};
-    }
+    if (lane == 0) a.parts[a.part(b, n, r) + seg] = RowPart{m, s, at, 0};
   }
 }
 
@@ -207,7 +165,9 @@ __device__ __forceinline__ void write_tokens(const VerifyArgs& a, int b, int tak
 // A CTA per sequence: the rows' parts joined (a warp per row), the drafted tokens followed, and what
 // the draw needs left in picks[b]; with temperature 0 that is all.  Latency-bound: the tokens and
 // their logits are requested before the parts are joined.
-__global__ void __launch_bounds__(256) k_verify_pick(VerifyArgs a) {
+constexpr int kPickThreads = 512;
+
+__global__ void __launch_bounds__(kPickThreads) k_verify_pick(VerifyArgs a) {
   __shared__ double s_sum[2 * kVerifyMaxDrafts + 1];
   __shared__ float s_max[2 * kVerifyMaxDrafts + 1];
   __shared__ int s_at[kVerifyMaxDrafts + 1];
@@ -218,7 +178,7 @@ __global__ void __launch_bounds__(256) k_verify_pick(VerifyArgs a) {
   const int n = a.count(b), rows = a.rows(b, n, T);
   if (rows == 0 || !temperature_ok(T) || (T > 0.0f && (!a.noise || (n && !a.uniforms)))) {
     if (tid == 0) a.picks[b].taken = -1;
-    write_tokens(a, b, 0, -1, tid, 256);
+    write_tokens(a, b, 0, -1, tid, kPickThreads);
     return;
   }
   const bool drafted = rows > n + 1;
@@ -232,36 +192,42 @@ __global__ void __launch_bounds__(256) k_verify_pick(VerifyArgs a) {
       u = a.uniforms[b * a.ldu + lane];
     }
   }
-  for (int r = warp; r < rows; r += 8) {
+  const double c = T > 0.0f ? 1.4426950408889634 / (double)T : 0.0;
+  const float c_hi = (float)c, c_lo = (float)(c - (double)c_hi);
+  for (int r = warp; r < rows; r += kPickThreads / 32) {
     const RowPart* p = a.parts + a.part(b, n, r);
+    constexpr int U = 4;  // a lane's parts of 128 segments, requested together
     float m = -INFINITY;
     int at = INT_MAX;
-    RowPart first = {-INFINITY, 0.0f, INT_MAX, 0};
-    if (lane < a.segs) first = p[lane];
-    for (int i = lane; i < a.segs; i += 32) {
-      const RowPart q = i == lane ? first : p[i];
-      if (q.max > m || (q.max == m && q.at < at)) {
-        m = q.max;
-        at = q.at;
+    RowPart q[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) q[k] = lane + 32 * k < a.segs ? p[lane + 32 * k] : RowPart{-INFINITY, 0.0f, INT_MAX, 0};
+    auto top = [&](const RowPart& x) {
+      if (x.max > m || (x.max == m && x.at < at)) {
+        m = x.max;
+        at = x.at;
       }
-    }
+    };
+#pragma unroll
+    for (int k = 0; k < U; ++k) top(q[k]);
+    for (int i = lane + 32 * U; i < a.segs; i += 32) top(p[i]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
       const int a2 = __shfl_xor_sync(0xffffffffu, at, o);
-      if (m2 > m || (m2 == m && a2 < at)) {
-        m = m2;
-        at = a2;
-      }
+      top(RowPart{m2, 0.0f, a2, 0});
     }
     double s = 0.0;
-    if (T > 0.0f)
-      for (int i = lane; i < a.segs; i += 32) {
-        const RowPart q = i == lane ? first : p[i];
-        if (q.sum != 0.0f) s += (double)q.sum * exp(((double)q.max - (double)m) / (double)T);
-      }
+    if (T > 0.0f) {
+      auto add = [&](const RowPart& x) {
+        if (x.sum != 0.0f) s += (double)(x.sum * exp_scaled(x.max - m, c_hi, c_lo));
+      };
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      for (int k = 0; k < U; ++k) add(q[k]);
+      for (int i = lane + 32 * U; i < a.segs; i += 32) add(p[i]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    }
     if (lane == 0) {
       const int to = r <= n ? r : a.drafts + r - n;
       s_max[to] = m;
@@ -306,9 +272,8 @@ __global__ void __launch_bounds__(256) k_verify_pick(VerifyArgs a) {
     k.xi = (float)(1.0 / s_sum[taken]);
     k.ym = k.drafted ? s_max[a.drafts + 1 + taken] : 0.0f;
     k.yi = k.drafted ? (float)(1.0 / s_sum[a.drafts + 1 + taken]) : 0.0f;
-    const double c = 1.4426950408889634 / (double)T;
-    k.c_hi = (float)c;
-    k.c_lo = (float)(c - (double)k.c_hi);
+    k.c_hi = c_hi;
+    k.c_lo = c_lo;
     a.picks[b] = k;
   }
 }
@@ -325,20 +290,22 @@ struct __align__(8) Leader {
   }
 };
 
-// The draw: a cluster of kRaceCluster CTAs per sequence, the vocabulary cut among them, their leaders
+// The draw: a cluster of `ctas` CTAs per sequence, the vocabulary cut among them, their leaders
 // exchanged through distributed shared memory.  An entry is weighed with the hardware's exponential
 // first, whose error is far below the margin 2^-16; only what may beat its warp's leader by then is
 // computed with care (some 10 entries of a warp), so the loop stays near 25 instructions per entry.
+// A thread requests kRaceBatch pieces of each row before it uses them.
 constexpr int kRaceCluster = 8;
 constexpr int kRaceThreads = 256;
+constexpr int kRaceBatch = 4;
 
-__global__ void __launch_bounds__(kRaceThreads) k_verify_race(VerifyArgs a) {
-  constexpr int W = kRaceThreads / 32;
+__global__ void __launch_bounds__(kRaceThreads, 2) k_verify_race(VerifyArgs a, int ctas) {
+  constexpr int W = kRaceThreads / 32, U = kRaceBatch;
   __shared__ Leader s_lead[W];
   __shared__ Leader s_all[2][kRaceCluster];
   pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.x / kRaceCluster, rank = (int)cluster_ctarank(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int b = blockIdx.x / ctas, rank = blockIdx.x - b * ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Pick k = a.picks[b];
   if (k.taken < 0) return;  // done already; the whole cluster returns
   cluster_arrive_relaxed();
@@ -348,37 +315,46 @@ __global__ void __launch_bounds__(kRaceThreads) k_verify_race(VerifyArgs a) {
   const float* y = k.drafted ? a.draft + b * a.dseq + k.taken * a.ldd : nullptr;
   int out_of = k.out_of;
   int64_t last = -1;
+  const int step = 4 * kRaceThreads * ctas;
   for (int pass = 0;; ++pass) {  // a second one where nothing of p - q is left: p itself
     const bool ay = (reinterpret_cast<uintptr_t>(y) & 15) == 0;
     Leader lead = {0.0f, INT_MAX};
     float bar = 0.0f;  // the warp's leader
-#pragma unroll 4
-    for (int i0 = 4 * (rank * kRaceThreads + warp * 32); i0 < a.vocab; i0 += 4 * kRaceThreads * kRaceCluster) {
-      const int i = i0 + 4 * lane;
-      const float4 vx = logits4(x, i, a.vocab, ax), ve = logits4(e, i, a.vocab, ae);
-      float4 vy = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (y) vy = logits4(y, i, a.vocab, ay);
-      const float fx[4] = {vx.x, vx.y, vx.z, vx.w}, fy[4] = {vy.x, vy.y, vy.z, vy.w}, fe[4] = {ve.x, ve.y, ve.z, ve.w};
-      bool may[4], any = false;
+    for (int i0 = 4 * (rank * kRaceThreads + warp * 32); i0 < a.vocab; i0 += U * step) {
+      float4 vx[U], ve[U], vy[U];
 #pragma unroll
-      for (int z = 0; z < 4; ++z) {
-        const float dx = fx[z] - k.xm, dy = fy[z] - k.ym;
-        const float p = ex2(fmaxf(fmaf(dx, k.c_hi, dx * k.c_lo), -200.0f)) * k.xi;
-        float q = 0.0f;
-        if (y) q = ex2(fmaxf(fmaf(dy, k.c_hi, dy * k.c_lo), -200.0f)) * k.yi;
-        may[z] = fmaf(p + q, 0x1p-16f, p - q) > bar * fe[z] && i + z != out_of && i + z < a.vocab;
-        any |= may[z];
+      for (int j = 0; j < U; ++j) {
+        const int i = min(i0 + j * step, a.vocab) + 4 * lane;  // behind the end: -inf without a read
+        vx[j] = logits4(x, i, a.vocab, ax);
+        ve[j] = logits4(e, i, a.vocab, ae);
+        vy[j] = y ? logits4(y, i, a.vocab, ay) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       }
-      if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
-        for (int z = 0; z < 4; ++z)
-          if (may[z]) {
-            // products that round by themselves: equal rows leave exactly nothing
-            float w = __fmul_rn(exp_scaled(fx[z] - k.xm, k.c_hi, k.c_lo), k.xi);
-            if (y) w = __fsub_rn(w, __fmul_rn(exp_scaled(fy[z] - k.ym, k.c_hi, k.c_lo), k.yi));
-            if (w > 0.0f) lead.take(w / fe[z], i + z);
-          }
-        bar = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(lead.best)));
+      for (int j = 0; j < U; ++j) {
+        const int i = min(i0 + j * step, a.vocab) + 4 * lane;
+        const float fx[4] = {vx[j].x, vx[j].y, vx[j].z, vx[j].w}, fy[4] = {vy[j].x, vy[j].y, vy[j].z, vy[j].w},
+                    fe[4] = {ve[j].x, ve[j].y, ve[j].z, ve[j].w};
+        bool may[4], any = false;
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          const float dx = fx[z] - k.xm, dy = fy[z] - k.ym;
+          const float p = ex2(fmaxf(fmaf(dx, k.c_hi, dx * k.c_lo), -200.0f)) * k.xi;
+          float q = 0.0f;
+          if (y) q = ex2(fmaxf(fmaf(dy, k.c_hi, dy * k.c_lo), -200.0f)) * k.yi;
+          may[z] = fmaf(p + q, 0x1p-16f, p - q) > bar * fe[z] && i + z != out_of && i + z < a.vocab;
+          any |= may[z];
+        }
+        if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+          for (int z = 0; z < 4; ++z)
+            if (may[z]) {
+              // products that round by themselves: equal rows leave exactly nothing
+              float w = __fmul_rn(exp_scaled(fx[z] - k.xm, k.c_hi, k.c_lo), k.xi);
+              if (y) w = __fsub_rn(w, __fmul_rn(exp_scaled(fy[z] - k.ym, k.c_hi, k.c_lo), k.yi));
+              if (w > 0.0f) lead.take(w / fe[z], i + z);
+            }
+          bar = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(lead.best)));
+        }
       }
     }
 #pragma unroll
@@ -390,14 +366,14 @@ __global__ void __launch_bounds__(kRaceThreads) k_verify_race(VerifyArgs a) {
     if (lane == 0) s_lead[warp] = lead;
     __syncthreads();
     if (pass == 0) cluster_wait();  // all CTAs of the cluster run
-    if (tid < kRaceCluster) {
+    if (tid < ctas) {
       for (int w = 0; w < W; ++w) lead.take(s_lead[w].best, s_lead[w].at);
       st_cluster_v2(mapa_shared(smem_u32(&s_all[pass][rank]), tid), __float_as_uint(lead.best), (uint32_t)lead.at);
     }
     __syncwarp();
     cluster_sync_all();
     Leader all = s_all[pass][0];
-    for (int r = 1; r < kRaceCluster; ++r) all.take(s_all[pass][r].best, s_all[pass][r].at);
+    for (int r = 1; r < ctas; ++r) all.take(s_all[pass][r].best, s_all[pass][r].at);
     if (all.at != INT_MAX) last = all.at;
     if (last >= 0 || pass == 1 || !k.refused) break;
     y = nullptr;
@@ -481,12 +457,16 @@ extern "C" OTF_API int otf_verify_drafts(const float* target, int64_t target_seq
                              reinterpret_cast<otf::Pick*>(w)};
   // row groups: one per row while all of their CTAs fit the GPU at once, else 4
   const int64_t rows = drafts + 1 + (a.draft ? drafts : 0);
-  const int64_t groups = std::min<int64_t>(rows, batch * segs * rows <= 4 * 148 ? rows : 4);
-  cudaError_t e = otf::launch_pdl(otf::k_verify_rows, dim3((unsigned)segs, (unsigned)groups, (unsigned)batch),
+  const int64_t blocks = (segs + 7) / 8;
+  const int64_t groups = std::min<int64_t>(rows, batch * blocks * rows <= 4 * 148 ? rows : 4);
+  cudaError_t e = otf::launch_pdl(otf::k_verify_rows, dim3((unsigned)blocks, (unsigned)groups, (unsigned)batch),
                                   dim3(otf::kVerifyThreads), 0, s, 1u, a);
   if (e != cudaSuccess) return set_cuda_error(e);
-  e = otf::launch_pdl(otf::k_verify_pick, dim3((unsigned)batch), dim3(256), 0, s, 1u, a);
+  e = otf::launch_pdl(otf::k_verify_pick, dim3((unsigned)batch), dim3(otf::kPickThreads), 0, s, 1u, a);
   if (e != cudaSuccess || (!temperatures && temperature == 0.0f)) return set_cuda_error(e);
-  return set_cuda_error(otf::launch_pdl(otf::k_verify_race, dim3((unsigned)batch * otf::kRaceCluster),
-                                        dim3(otf::kRaceThreads), 0, s, (unsigned)otf::kRaceCluster, a));
+  // CTAs per sequence: as many as all run at once, two on an SM
+  int ctas = otf::kRaceCluster;
+  while (ctas > 1 && batch * ctas > 2 * 148) ctas /= 2;
+  return set_cuda_error(otf::launch_pdl(otf::k_verify_race, dim3((unsigned)(batch * ctas)), dim3(otf::kRaceThreads), 0, s,
+                                        (unsigned)ctas, a, ctas));
 }
