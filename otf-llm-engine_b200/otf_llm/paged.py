@@ -233,11 +233,8 @@ class PagedKVCache:
         if rotary is not None and (rotary.head_dim != self.head_dim or rotary.device != self.device):
             raise ValueError(f"rotary is for heads of {rotary.head_dim} on {rotary.device}")
         if n:
-            with _on(self.device):
-                st = _native.lib().otf_paged_append(self._ref, None if rotary is None else rotary._ref, pq, ldq, po, ldo,
-                                                    heads, pk, ldk, pv, ldv, ps, pp, n, _stream(self.device))
-            if st:
-                _native._check(st, "otf_paged_append")
+            _call("otf_paged_append", self.device, self._ref, None if rotary is None else rotary._ref, pq, ldq, po, ldo,
+                  heads, pk, ldk, pv, ldv, ps, pp, n)
         return q_out
 
     def _plan_append(self, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor) -> tuple:
@@ -289,12 +286,8 @@ class PagedKVCache:
         # from the caching allocator, for this call alone: calls on two streams, or in two captured
         # graphs, share nothing
         ws = torch.empty(bytes_, dtype=torch.uint8, device=self.device)
-        with _on(self.device):
-            st = _native.lib().otf_paged_attn(self._ref, pq, ldq, heads, tokens,
-                                              self._scale if scale is None else float(scale), po, ldo, pw, ldw,
-                                              ws.data_ptr(), bytes_, _stream(self.device))
-        if st:
-            _native._check(st, "otf_paged_attn")
+        _call("otf_paged_attn", self.device, self._ref, pq, ldq, heads, tokens,
+              self._scale if scale is None else float(scale), po, ldo, pw, ldw, ws.data_ptr(), bytes_)
         return out
 
     def _plan_attend(self, q: torch.Tensor, weights: Optional[torch.Tensor]) -> tuple:
@@ -343,11 +336,8 @@ class PagedKVCache:
             raise ValueError(f"budget {budget} (of {to.capacity}) and recent {recent} do not fit")
         ldo = self._weights(weights_out, "weights_out", budget)
         kept = torch.empty((self.batch, self.kv_heads, budget), dtype=torch.int32, device=self.device)
-        with _on(self.device):
-            st = _native.lib().otf_paged_evict(self._ref, to._ref, weights.data_ptr(), ldw, weights_out.data_ptr(),
-                                               ldo, budget, recent, kept.data_ptr(), to.lengths.data_ptr(),
-                                               _stream(self.device))
-        _native._check(st, "otf_paged_evict")
+        _call("otf_paged_evict", self.device, self._ref, to._ref, weights.data_ptr(), ldw, weights_out.data_ptr(), ldo,
+              budget, recent, kept.data_ptr(), to.lengths.data_ptr())
         return kept
 
     def advance(self, tokens: int = 1) -> None:
@@ -372,22 +362,15 @@ class PagedKVCache:
         return t.as_strided((t.shape[0] * t.shape[1], t.shape[2], t.shape[3]), (row, t.stride(2), t.stride(3)))
 
 
-class _Same:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *a):
-        return False
-
-
-_SAME = _Same()
-
-
-def _on(dev: torch.device):
-    """The device made current, where it is not already."""
-    return _SAME if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
-
-
-def _stream(dev: torch.device) -> int:
-    """The device's current stream, without the Stream object that torch.cuda.current_stream makes."""
-    return torch._C._cuda_getCurrentRawStream(dev.index)
+def _call(name: str, dev: torch.device, *args) -> None:
+    """An entry point of the library with the device current and its current stream as the last
+    argument (the raw handle: torch.cuda.current_stream would make a Stream object)."""
+    fn = getattr(_native.lib(), name)
+    index = dev.index
+    if torch.cuda.current_device() == index:
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if st:
+        _native._check(st, name)

@@ -13,7 +13,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _native
-from .paged import _on, _stream
+from .paged import _call
 
 MAX_DRAFTS = 32
 
@@ -68,12 +68,8 @@ def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, *,
     tokens = torch.empty((batch, drafts + 1), dtype=torch.int64, device=dev)
     accepted = torch.empty(batch, dtype=torch.int32, device=dev)
     ws = torch.empty(bytes_, dtype=torch.uint8, device=dev)     # for this call alone, on its stream
-    with _on(dev):
-        st = _native.lib().otf_verify_drafts(pt, seq_t, ld_t, pd, seq_d, ld_d, ptok, ld_tok, pu, ld_u, pn, ld_n, each, one,
-                                             pc, tokens.data_ptr(), accepted.data_ptr(), batch, drafts, vocab,
-                                             ws.data_ptr(), bytes_, _stream(dev))
-    if st:
-        _native._check(st, "otf_verify_drafts")
+    _call("otf_verify_drafts", dev, pt, seq_t, ld_t, pd, seq_d, ld_d, ptok, ld_tok, pu, ld_u, pn, ld_n, each, one, pc,
+          tokens.data_ptr(), accepted.data_ptr(), batch, drafts, vocab, ws.data_ptr(), bytes_)
     return tokens, accepted
 
 
