@@ -71,7 +71,7 @@ struct AttnArgs {
   int rows, blocks;    // rep x tokens rows in so many row blocks
   int64_t* prefix;     // [batch + 1] chunks before each sequence
   float* part;         // [2 x grid][rows of a block][head_dim]: o of a part
-  float2* part_ml;     // [2 x grid][rows of a block]: its m and l
+  float4* part_ml;     // [2 x grid][rows of a block]: its m, l and unrounded l
   float* lse;          // [batch, kv_heads, rows] log2 of the sum, when weights are wanted
   float* scores;       // [batch, kv_heads, rows, ld_scores] likewise
   int64_t ld_scores;
@@ -159,7 +159,8 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
   unsigned char* s_q = smem + kPaWarps * NS * kPaStage;  // [RB][D] when it does not fit the registers
   float* s_m = reinterpret_cast<float*>(s_q + (MT > 1 ? RB * D * 2 : 0));
   float* s_l = s_m + kPaWarps * 16;
-  uint16_t* s_tail = reinterpret_cast<uint16_t*>(s_l + kPaWarps * 16);  // [tokens - 1][keys, values][D]
+  float* s_exact = s_l + kPaWarps * 16;
+  uint16_t* s_tail = reinterpret_cast<uint16_t*>(s_exact + kPaWarps * 16);  // [tokens - 1][keys, values][D]
   int* s_len = reinterpret_cast<int*>(s_tail + (a.tokens - 1) * 2 * D);
   __shared__ int64_t s_sum[kPaWarps];
   __shared__ Walk s_walk;
@@ -292,7 +293,11 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
   }
 
   uint32_t qf[D / 16][4];
-  float o[MT][D / 8][4], m[MT][2], l[MT][2];
+  float o[MT][D / 8][4], m[MT][2], l[MT][4], exact[MT][2];
+  // a column of ones beside the values: l is the sum of the probabilities as they were rounded, so that a
+  // rounding common to both cancels (one key with all the weight comes out exactly); `exact` sums them
+  // unrounded, for the weights
+  const uint32_t ones = BF ? 0x3F803F80u : 0x3C003C00u;
   const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;  // on q, so that a larger product weighs more
   const float scale = fabsf(a.scale);
   const int lrow = lane & 7, lmat = lane >> 3;
@@ -337,7 +342,7 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
         m[t][0] = m[t][1] = -INFINITY;
-        l[t][0] = l[t][1] = 0.0f;
+        l[t][0] = l[t][1] = l[t][2] = l[t][3] = exact[t][0] = exact[t][1] = 0.0f;
 #pragma unroll
         for (int j = 0; j < D / 8; ++j)
 #pragma unroll
@@ -440,7 +445,9 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             mx = fmaxf(mx * scale, m[t][h]);
             const float f = m[t][h] == -INFINITY ? 0.0f : ex2(m[t][h] - mx);
-            l[t][h] *= f;
+            l[t][2 * h] *= f;
+            l[t][2 * h + 1] *= f;
+            exact[t][h] *= f;
 #pragma unroll
             for (int j = 0; j < D / 8; ++j) {
               o[t][j][2 * h] *= f;
@@ -454,11 +461,17 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
         for (int n = 0; n < KT / 8; ++n) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) e[n][i] = ex2(e[n][i]);
-          l[t][0] += e[n][0] + e[n][1];
-          l[t][1] += e[n][2] + e[n][3];
           p[t][n >> 1][(n & 1) * 2] = pack2<BF>(e[n][0], e[n][1]);
           p[t][n >> 1][(n & 1) * 2 + 1] = pack2<BF>(e[n][2], e[n][3]);
         }
+#pragma unroll
+        for (int n = 0; n < KT / 16; ++n) mma16816<BF>(l[t], p[t][n], ones, ones);
+        if (a.scores)
+#pragma unroll
+          for (int n = 0; n < KT / 8; ++n) {
+            exact[t][0] += e[n][0] + e[n][1];
+            exact[t][1] += e[n][2] + e[n][3];
+          }
       }
 #pragma unroll
       for (int j = 0; j < D / 16; ++j)
@@ -509,13 +522,14 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
         __syncwarp();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float x = l[t][h];
+          const int w = h * 8 + (lane >> 2);
+          float x = exact[t][h];
           x += __shfl_xor_sync(0xffffffffu, x, 1);
           x += __shfl_xor_sync(0xffffffffu, x, 2);
-          const int w = h * 8 + (lane >> 2);
           if ((lane & 3) == 0) {
+            s_exact[warp * 16 + w] = x;
             s_m[warp * 16 + w] = m[t][h];
-            s_l[warp * 16 + w] = x;
+            s_l[warp * 16 + w] = l[t][2 * h];
           }
 #pragma unroll
           for (int j = 0; j < D / 8; ++j)  // columns turned by the row, against bank conflicts
@@ -523,7 +537,7 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
                 make_float2(o[t][j][2 * h], o[t][j][2 * h + 1]);
         }
         __syncthreads();
-        float M = -INFINITY, L = 0.0f, acc[D / 32][4];
+        float M = -INFINITY, L = 0.0f, E = 0.0f, acc[D / 32][4];
 #pragma unroll
         for (int w = 0; w < kPaWarps; ++w) M = fmaxf(M, s_m[w * 16 + r]);
 #pragma unroll
@@ -537,6 +551,7 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
           const float* x = reinterpret_cast<const float*>(smem + w * NS * kPaStage + slot * kPaStage) + r * D;
           if (lw != 0.0f) {
             L = fmaf(lw, f, L);
+            E = fmaf(s_exact[w * 16 + r], f, E);
 #pragma unroll
             for (int j = 0; j < D / 32; ++j) {
               const float4 y = *reinterpret_cast<const float4*>(x + ((j * 32 + part * 4) ^ ((r & 3) << 3)));
@@ -568,6 +583,7 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
             if (d != -INFINITY) {
               const float mn = fmaxf(M, d), f = M == -INFINITY ? 0.0f : ex2(M - mn), pr = ex2(d - mn + kProbShift<BF>);
               L = L * f + pr;
+              E = E * f + pr;
 #pragma unroll
               for (int j = 0; j < D / 32; ++j)
 #pragma unroll
@@ -582,14 +598,14 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
             for (int j = 0; j < D / 32; ++j)
               store_row<BF, 4>(a.out + row * a.ldo + (int64_t)head * D + j * 32 + part * 4, acc[j], 1.0f / L);
             if (a.lse && part == 0)
-              a.lse[((int64_t)now.b * c.kv_heads + g) * a.rows + rr] = M + log2f(L) - kProbShift<BF>;
+              a.lse[((int64_t)now.b * c.kv_heads + g) * a.rows + rr] = M + log2f(E) - kProbShift<BF>;
           } else {
             const int64_t at = (int64_t)(2 * blockIdx.x + (parts > 0 ? 1 : 0)) * RB + t * 16 + r;
 #pragma unroll
             for (int j = 0; j < D / 32; ++j)
               *reinterpret_cast<float4*>(a.part + at * D + j * 32 + part * 4) =
                   make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
-            if (part == 0) a.part_ml[at] = make_float2(M, L);
+            if (part == 0) a.part_ml[at] = make_float4(M, L, E, 0.0f);
           }
         }
         __syncthreads();  // before the stages are filled again, or the next 16 rows come
@@ -611,7 +627,7 @@ constexpr int kJoinWarps = 4;
 template <bool BF, int D, int WR>
 __global__ void __launch_bounds__(kJoinWarps * 32) k_paged_attn_join(AttnArgs a, int RB) {
   constexpr int PL = D / 32, W = kJoinWarps;
-  __shared__ float s_l[W];
+  __shared__ float s_l[W], s_e[W];
   __shared__ __align__(16) float s_o[WR > 1 ? W : 1][D];
   pdl_trigger();
   const PagedView& c = a.c;
@@ -641,7 +657,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_paged_attn_join(AttnArgs a,
   if (i0 == i1) return;  // one CTA had it whole
   const int n = i1 + 1 - i0;
   auto part = [&](int i) { return (2 * (i0 + i) + (i == 0 && second ? 1 : 0)) * RB + r; };
-  float M = -INFINITY, L = 0.0f, acc[PL];
+  float M = -INFINITY, L = 0.0f, E = 0.0f, acc[PL];
 #pragma unroll
   for (int j = 0; j < PL; ++j) acc[j] = 0.0f;
 #pragma unroll 4
@@ -667,9 +683,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_paged_attn_join(AttnArgs a,
       }
     }
     if (lane < 8 && base + lane * WR < n) {  // lane k holds the factor of the k-th of them
-      const float2 ml = a.part_ml[part(base + lane * WR)];
+      const float4 ml = a.part_ml[part(base + lane * WR)];
       f = ml.y == 0.0f ? 0.0f : ex2(ml.x - M);
       L = fmaf(ml.y, f, L);
+      E = fmaf(ml.z, f, E);
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -680,46 +697,66 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_paged_attn_join(AttnArgs a,
     }
   }
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+  for (int x = 16; x > 0; x >>= 1) {
+    L += __shfl_xor_sync(0xffffffffu, L, x);
+    E += __shfl_xor_sync(0xffffffffu, E, x);
+  }
   if (WR > 1) {
-    if (lane == 0) s_l[warp] = L;
+    if (lane == 0) {
+      s_l[warp] = L;
+      s_e[warp] = E;
+    }
 #pragma unroll
     for (int j = 0; j < PL; ++j) s_o[warp % (WR > 1 ? W : 1)][lane * PL + j] = acc[j];
     __syncthreads();
     if (sub) return;
-    L = 0.0f;
+    L = E = 0.0f;
 #pragma unroll
     for (int j = 0; j < PL; ++j) acc[j] = 0.0f;
 #pragma unroll
     for (int w = 0; w < WR; ++w) {
       L += s_l[warp + w];
+      E += s_e[warp + w];
 #pragma unroll
       for (int j = 0; j < PL; ++j) acc[j] += s_o[(warp + w) % (WR > 1 ? W : 1)][lane * PL + j];
     }
   }
   const int tok = rr / a.rep, head = g * a.rep + rr - tok * a.rep;
   store_row<BF, PL>(a.out + ((int64_t)b * a.tokens + tok) * a.ldo + (int64_t)head * D + lane * PL, acc, 1.0f / L);
-  if (a.lse && lane == 0) a.lse[((int64_t)b * c.kv_heads + g) * a.rows + rr] = M + log2f(L) - kProbShift<BF>;
+  if (a.lse && lane == 0) a.lse[((int64_t)b * c.kv_heads + g) * a.rows + rr] = M + log2f(E) - kProbShift<BF>;
 }
 
-// weights[b, g, s] += sum over the item rows of 2^(score - lse).  One thread per token, rows in order.
-__global__ void __launch_bounds__(256) k_paged_attn_weights(AttnArgs a, float* weights, int64_t ldw) {
+// weights[b, g, s] += sum over the item's rows of 2^(score - lse): a thread takes 4 tokens, rows in
+// order.  Memory-bound: the scores are read once, mostly from L2.
+constexpr int kWeightThreads = 128;
+
+__global__ void __launch_bounds__(kWeightThreads) k_paged_attn_weights(AttnArgs a, float* weights, int64_t ldw) {
   pdl_trigger();
   pdl_wait();
   const PagedView& c = a.c;
-  const int g = blockIdx.y, b = blockIdx.z, s = blockIdx.x * 256 + threadIdx.x;
+  const int g = blockIdx.y, b = blockIdx.z, s = 4 * (blockIdx.x * kWeightThreads + threadIdx.x);
   const int len = c.lengths[b];
   if (len < 0 || (int64_t)len + a.tokens > c.capacity || s >= len + a.tokens) return;
   const int64_t item = (int64_t)b * c.kv_heads + g;
   const float* x = a.scores + item * a.rows * a.ld_scores + s;
   const float* lse = a.lse + item * a.rows;
-  float sum = 0.0f;
-#pragma unroll 8
+  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto term = [](float v, float l) { return v == -INFINITY ? 0.0f : ex2(v - l); };
+#pragma unroll 4
   for (int r = 0; r < a.rows; ++r) {
-    const float v = x[r * a.ld_scores];
-    sum += v == -INFINITY ? 0.0f : ex2(v - lse[r]);
+    const float4 v = *reinterpret_cast<const float4*>(x + r * a.ld_scores);
+    const float l = lse[r];
+    sum.x += term(v.x, l);
+    sum.y += term(v.y, l);
+    sum.z += term(v.z, l);
+    sum.w += term(v.w, l);
   }
-  weights[item * ldw + s] += sum;
+  float* w = weights + item * ldw + s;
+  const int n = len + a.tokens - s;  // what lies behind the last token was not written
+  w[0] += sum.x;
+  if (n > 1) w[1] += sum.y;
+  if (n > 2) w[2] += sum.z;
+  if (n > 3) w[3] += sum.w;
 }
 
 // Bytes of the workspace's parts, in order.
@@ -733,7 +770,7 @@ static AttnSpace attn_space(int64_t batch, int64_t heads, int64_t kv_heads, int6
   const int64_t rows = heads / kv_heads * tokens, RB = rows <= 16 ? 16 : 32;
   s.prefix = align_up((batch + 1) * 8, 256);
   s.part = align_up(2 * kPaGrid * RB * D * 4, 256);
-  s.part_ml = align_up(2 * kPaGrid * RB * 8, 256);
+  s.part_ml = align_up(2 * kPaGrid * RB * 16, 256);
   s.ld_scores = align_up(max_tokens, 8);
   s.lse = weights ? align_up(batch * kv_heads * rows * 4, 256) : 0;
   s.scores = weights ? align_up(batch * kv_heads * rows * s.ld_scores * 4, 256) : 0;
@@ -746,7 +783,7 @@ static cudaError_t launch_attn(const AttnArgs& a, float* weights, int64_t ldw, c
   const bool aligned = a.c.page_size % 16 == 0;
   auto* k = RB == 16 ? (aligned ? k_paged_attn<BF, D, 1, true> : k_paged_attn<BF, D, 1, false>)
                      : (aligned ? k_paged_attn<BF, D, 2, true> : k_paged_attn<BF, D, 2, false>);
-  const size_t dyn = (size_t)kPaWarps * kPaStages * kPaStage + (size_t)kPaWarps * 16 * 8 + (RB > 16 ? RB * D * 2 : 0) +
+  const size_t dyn = (size_t)kPaWarps * kPaStages * kPaStage + (size_t)kPaWarps * 16 * 12 + (RB > 16 ? RB * D * 2 : 0) +
                      (size_t)(a.tokens - 1) * 4 * D + (size_t)a.c.batch * 4;
   {
     // the shared-memory opt-in, once per kernel and device, for the largest batch
@@ -759,7 +796,7 @@ static cudaError_t launch_attn(const AttnArgs& a, float* weights, int64_t ldw, c
     bool& have = done[std::make_pair(reinterpret_cast<const void*>(k), dev)];
     if (!have) {
       e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               kPaWarps * kPaStages * kPaStage + kPaWarps * 16 * 8 + 32 * D * 2 + (kPagedMaxTokens - 1) * 4 * D +
+                               kPaWarps * kPaStages * kPaStage + kPaWarps * 16 * 12 + 32 * D * 2 + (kPagedMaxTokens - 1) * 4 * D +
                                    kPagedMaxBatch * 4);
       if (e != cudaSuccess) return e;
       have = true;
@@ -778,7 +815,9 @@ static cudaError_t launch_attn(const AttnArgs& a, float* weights, int64_t ldw, c
                    1u, a, RB);
   if (e != cudaSuccess || !weights) return e;
   return launch_pdl(k_paged_attn_weights,
-                    dim3((unsigned)((a.c.capacity + 255) / 256), (unsigned)a.c.kv_heads, (unsigned)a.c.batch), dim3(256), 0,
+                    dim3((unsigned)((a.c.capacity + 4 * kWeightThreads - 1) / (4 * kWeightThreads)), (unsigned)a.c.kv_heads,
+                         (unsigned)a.c.batch),
+                    dim3(kWeightThreads), 0,
                     s, 1u, a, weights, ldw);
 }
 
@@ -838,7 +877,7 @@ extern "C" OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* 
   char* w = static_cast<char*>(workspace);
   a.prefix = reinterpret_cast<int64_t*>(w);
   a.part = reinterpret_cast<float*>(w += space.prefix);
-  a.part_ml = reinterpret_cast<float2*>(w += space.part);
+  a.part_ml = reinterpret_cast<float4*>(w += space.part);
   w += space.part_ml;
   if (weights) {
     a.lse = reinterpret_cast<float*>(w);
