@@ -554,10 +554,12 @@ OTF_API int otf_paged_evict(const otf_paged_cache* from, const otf_paged_cache* 
  * the logits counts as -inf.  A sequence without a token of positive weight, or
  * with a count or temperature out of range, gets -1 and raises the otf_device_error flag; so
  * does a drafted token outside the vocabulary, which is refused.  Where max(p - q, 0) holds
- * nothing, p is drawn from.  workspace: otf_verify_workspace_bytes(...), 256-byte aligned, need
- * not be cleared, one per call at a time; at most 65535 sequences.  Beside otf_i8_head_argmax, the greedy pick of one row.
+ * nothing, p is drawn from.  At most 65535 sequences and a vocabulary of 2^30.  workspace:
+ * otf_verify_workspace_bytes(...) (0 for small calls, then it may be NULL), 256-byte aligned, need
+ * not be cleared; two calls that may run at the same time need one each.  Beside
+ * otf_i8_head_argmax, the greedy pick of one row.
  */
-OTF_API int64_t otf_verify_workspace_bytes(int64_t batch, int64_t drafts, int64_t vocab);
+OTF_API int64_t otf_verify_workspace_bytes(int64_t batch, int64_t drafts, int64_t vocab, int with_draft);
 OTF_API int otf_verify_drafts(const float* target, int64_t target_seq, int64_t ld_target, const float* draft,
                               int64_t draft_seq, int64_t ld_draft, const int64_t* tokens, int64_t ld_tokens,
                               const float* uniforms, int64_t ld_uniforms, const float* noise, int64_t ld_noise,

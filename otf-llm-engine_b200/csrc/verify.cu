@@ -6,7 +6,18 @@
 // follows.  A draw is argmax_i w_i / e_i with e_i ~ Exp(1) given: the index of the smallest of
 // independent exponential times of rates w_i, which is distributed as w.  Unlike a search in
 // cumulated weights it has no border between neighbours on which a rounding decides.
+//
+// Three steps: (1) every row's maximum, its first index and the sum of exponentials under it, in one
+// pass over the logits (K + 1 rows of the target's, K of the draft's); (2) the drafted tokens, a few
+// hundred numbers per sequence; (3) the race over the one or two rows that it needs.  Memory-bound:
+// the rows are read once, the drawn ones a second time, from L2 where they still are.
+//
+// Few logits take one launch, k_verify: a cluster of CTAs per sequence, the vocabulary cut among them,
+// the steps' results exchanged through distributed shared memory.  Many take three, whose grids
+// fill the GPU in every step whatever the sequences' drafts are: k_verify_rows, k_verify_pick,
+// k_verify_race.  What a step computes is shared, and so is the order of its sums within a row.
 #include <algorithm>
+#include <mutex>
 
 #include "otf_common.cuh"
 
@@ -17,23 +28,33 @@ int check_device();                  // capi.cu
 int verify_device_error(int clear);  // read (and optionally clear) the flag below
 
 constexpr int kVerifyMaxDrafts = 32;
-constexpr int kVerifySeg = 1024;     // logits of a row that one warp reads
+constexpr int kVerifyMaxRows = 2 * kVerifyMaxDrafts + 1;
+constexpr int kVerifySeg = 1024;     // logits that a warp holds at once, 32 a lane
 constexpr int kVerifyThreads = 256;
+constexpr int kVerifyWarps = kVerifyThreads / 32;
+constexpr int kVerifyCluster = 16;   // CTAs of a sequence at most (k_verify)
+constexpr int kPickThreads = 512;
+constexpr int kRaceCluster = 8;      // CTAs of a sequence at most (k_verify_race)
+// Logits of all rows up to which one launch is taken.  Measured, eager calls one after another, one launch
+// against three: 16 sequences x 5 rows of 32000 (2.4M) 14.2 us against 21.0, 32 sequences (4.9M) 16.5
+// against 21.1, 64 (9.8M) 24.2 against 24.4; 4 x 11 rows of 128256 (5.4M) 30.8 against 26.6, 16 x 8
+// (15.7M) 24.9 against 18.4.
+constexpr int64_t kVerifyOneLaunch = 4 << 20;
 
 // Set when a sequence has no token to draw, or an argument on the device is out of range.
 __device__ int g_verify_device_error;
 
-// What one warp found in its part of a row: the largest logit, its first index, and the sum of
+// What is known of a row, or of a part of it: the largest logit, its first index, and the sum of
 // exp((x - max) / T).
 struct __align__(16) RowPart {
   float max, sum;
   int at, pad;
 };
 
-// What the draw of a sequence needs: the row it is of, the rows' maxima and 1 / sums, log2(e) / T.
+// What the draw of a sequence needs: the row it is of, the rows' maxima and 1 / sums.
 struct __align__(16) Pick {
   int taken, refused, drafted, out_of;  // taken -1: nothing to draw
-  float xm, xi, ym, yi, c_hi, c_lo, pad[2];
+  float xm, xi, ym, yi;
 };
 
 // exp(d / T) for d <= 0, with c = log2(e) / T in two floats: the exponent is split into its
@@ -66,7 +87,6 @@ __device__ __forceinline__ float4 logits4(const float* x, int i, int end, bool a
   return v;
 }
 
-// The logits' place, and what every kernel asks about a sequence.
 struct VerifyArgs {
   const float* target;
   const float* draft;  // or null
@@ -82,203 +102,169 @@ struct VerifyArgs {
   const int* counts;
   int64_t* out;
   int* accepted;
-  int drafts, vocab, segs;
+  int drafts, vocab;
+  int slice;       // k_verify: a CTA's part of the vocabulary, a multiple of 4
+  int segs;        // k_verify_rows: segments of a row
   RowPart* parts;  // [batch][2 drafts + 1: the target's rows, then the draft's][segs]
   Pick* picks;     // [batch]
+};
 
-  __device__ __forceinline__ float temp(int b) const { return temperatures ? temperatures[b] : temperature; }
-  __device__ __forceinline__ int count(int b) const { return counts ? counts[b] : drafts; }
-  // row r of the count + 1 target rows and then count draft rows that sequence b needs
-  __device__ __forceinline__ int rows(int b, int n, float T) const {
-    return n < 0 || n > drafts ? 0 : n + 1 + (draft && T > 0.0f ? n : 0);
+// A sequence as the kernels see it.
+struct Sequence {
+  const VerifyArgs& a;
+  int b, n;        // n: its drafted tokens
+  float T, c_hi, c_lo;  // temperature, log2(e) / T in two floats
+  bool ok, drafted;     // drafted: the draft's logits count
+
+  __device__ __forceinline__ Sequence(const VerifyArgs& args, int seq) : a(args), b(seq) {
+    T = a.temperatures ? a.temperatures[b] : a.temperature;
+    n = a.counts ? a.counts[b] : a.drafts;
+    ok = n >= 0 && n <= a.drafts && temperature_ok(T) && (T == 0.0f || (a.noise && (n == 0 || a.uniforms)));
+    drafted = ok && a.draft && T > 0.0f && n > 0;
+    const double c = T > 0.0f ? 1.4426950408889634 / (double)T : 0.0;
+    c_hi = (float)c;
+    c_lo = (float)(c - (double)c_hi);
   }
-  __device__ __forceinline__ const float* row(int b, int n, int r) const {
-    return r <= n ? target + b * tseq + r * ldt : draft + b * dseq + (r - n - 1) * ldd;
+  // rows: the target's 0 .. n, then the draft's
+  __device__ __forceinline__ int rows() const { return !ok ? 0 : n + 1 + (drafted ? n : 0); }
+  __device__ __forceinline__ const float* row(int r) const {
+    return r <= n ? a.target + b * a.tseq + r * a.ldt : a.draft + b * a.dseq + (r - n - 1) * a.ldd;
   }
-  __device__ __forceinline__ int64_t part(int b, int n, int r) const {
-    return ((int64_t)b * (2 * drafts + 1) + (r <= n ? r : drafts + r - n)) * segs;
+  __device__ __forceinline__ RowPart* part(int r) const {
+    return a.parts + ((int64_t)b * (2 * a.drafts + 1) + (r <= n ? r : a.drafts + r - n)) * a.segs;
   }
 };
 
-// One pass over the logits: grid (blocks of 8 segments, row groups, batch), a warp per segment.  A lane
-// holds its 32 values of a row's segment in registers: the warp's maximum, then the sum of
-// exponentials under it.  Memory-bound, 7 instructions per logit; the warps of a CTA never meet.  A
-// CTA goes through its group's rows, so that rows that a sequence with fewer drafted tokens does
-// not have cost nothing.
-__global__ void __launch_bounds__(kVerifyThreads) k_verify_rows(VerifyArgs a) {
-  constexpr int N = kVerifySeg / 128;
-  pdl_trigger();
-  pdl_wait();
-  const int b = blockIdx.z, lane = threadIdx.x & 31, seg = blockIdx.x * (kVerifyThreads / 32) + (threadIdx.x >> 5);
-  if (seg >= a.segs) return;
-  const float T = a.temp(b);
-  const int n = a.count(b), rows = a.rows(b, n, T);
-  const int i0 = seg * kVerifySeg + 4 * lane;
-  const float c_hi = (float)(1.4426950408889634 / (double)T);
-  const float c_lo = (float)(1.4426950408889634 / (double)T - (double)c_hi);
-  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
-    const float* x = a.row(b, n, r);
-    const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-    float4 v[N];
-#pragma unroll
-    for (int z = 0; z < N; ++z) v[z] = logits4(x, i0 + z * 128, a.vocab, aligned);
-    float m = -INFINITY;  // a NaN is never the largest
-#pragma unroll
-    for (int z = 0; z < N; ++z) m = fmaxf(m, fmaxf(fmaxf(v[z].x, v[z].y), fmaxf(v[z].z, v[z].w)));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float s = 0.0f;
-    int at = INT_MAX;
-    if (T == 0.0f) {  // the first of the largest
-#pragma unroll
-      for (int z = N - 1; z >= 0; --z) {
-        const float e[4] = {v[z].x, v[z].y, v[z].z, v[z].w};
-#pragma unroll
-        for (int w = 3; w >= 0; --w)
-          if (e[w] == m && i0 + z * 128 + w < a.vocab) at = i0 + z * 128 + w;
-      }
-      at = __reduce_min_sync(0xffffffffu, at);
-    } else {
-      const float mt = m == -INFINITY ? 0.0f : m;  // nothing but -inf: the sum is 0
-      auto term = [&](float x) {  // 0 for -inf and NaN (the maximum drops a NaN)
-        const float d = x - mt;
-        return ex2(fmaxf(fmaf(d, c_hi, d * c_lo), -200.0f));
-      };
-#pragma unroll
-      for (int z = 0; z < N; ++z) s += (term(v[z].x) + term(v[z].y)) + (term(v[z].z) + term(v[z].w));
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    }
-    if (lane == 0) a.parts[a.part(b, n, r) + seg] = RowPart{m, s, at, 0};
-  }
-}
-
-__device__ __forceinline__ void write_tokens(const VerifyArgs& a, int b, int taken, int64_t last, int tid, int threads) {
+__device__ __forceinline__ void write_tokens(const Sequence& q, int taken, int64_t last, int tid, int threads) {
+  const VerifyArgs& a = q.a;
   for (int j = tid; j <= a.drafts; j += threads)
-    a.out[(int64_t)b * (a.drafts + 1) + j] = last < 0 || j > taken ? -1 : j < taken ? a.tokens[b * a.ldtok + j] : last;
+    a.out[(int64_t)q.b * (a.drafts + 1) + j] =
+        last < 0 || j > taken ? -1 : j < taken ? a.tokens[q.b * a.ldtok + j] : last;
   if (tid == 0) {
-    a.accepted[b] = last < 0 ? 0 : taken;
+    a.accepted[q.b] = last < 0 ? 0 : taken;
     if (last < 0) atomicExch(&g_verify_device_error, 1);
   }
 }
 
-// A CTA per sequence: the rows' parts joined (a warp per row), the drafted tokens followed, and what
-// the draw needs left in picks[b]; with temperature 0 that is all.  Latency-bound: the tokens and
-// their logits are requested before the parts are joined.
-constexpr int kPickThreads = 512;
-
-__global__ void __launch_bounds__(kPickThreads) k_verify_pick(VerifyArgs a) {
-  __shared__ double s_sum[2 * kVerifyMaxDrafts + 1];
-  __shared__ float s_max[2 * kVerifyMaxDrafts + 1];
-  __shared__ int s_at[kVerifyMaxDrafts + 1];
-  pdl_trigger();
-  pdl_wait();
-  const int b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const float T = a.temp(b);
-  const int n = a.count(b), rows = a.rows(b, n, T);
-  if (rows == 0 || !temperature_ok(T) || (T > 0.0f && (!a.noise || (n && !a.uniforms)))) {
-    if (tid == 0) a.picks[b].taken = -1;
-    write_tokens(a, b, 0, -1, tid, kPickThreads);
-    return;
-  }
-  const bool drafted = rows > n + 1;
-  float xd = 0.0f, yd = 0.0f, u = 0.0f;
-  int64_t d = -1;
-  if (warp == 0 && lane < n) {
-    d = a.tokens[b * a.ldtok + lane];
-    if (d >= 0 && d < a.vocab && T > 0.0f) {
-      xd = a.target[b * a.tseq + lane * a.ldt + d];
-      if (drafted) yd = a.draft[b * a.dseq + lane * a.ldd + d];
-      u = a.uniforms[b * a.ldu + lane];
-    }
-  }
-  const double c = T > 0.0f ? 1.4426950408889634 / (double)T : 0.0;
-  const float c_hi = (float)c, c_lo = (float)(c - (double)c_hi);
-  for (int r = warp; r < rows; r += kPickThreads / 32) {
-    const RowPart* p = a.parts + a.part(b, n, r);
-    constexpr int U = 4;  // a lane's parts of 128 segments, requested together
-    float m = -INFINITY;
-    int at = INT_MAX;
-    RowPart q[U];
+// Step 1 for a warp: the 1024 logits of a row from i0 on (none behind `end`), 32 in each lane: their
+// maximum, then the sum of exponentials under it, 7 instructions per logit.  A NaN counts as -inf.
+__device__ __forceinline__ RowPart read_segment(const Sequence& q, const float* x, int i0, int end) {
+  constexpr int N = kVerifySeg / 128;
+  const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  i0 += 4 * (threadIdx.x & 31);
+  float4 v[N];
 #pragma unroll
-    for (int k = 0; k < U; ++k) q[k] = lane + 32 * k < a.segs ? p[lane + 32 * k] : RowPart{-INFINITY, 0.0f, INT_MAX, 0};
-    auto top = [&](const RowPart& x) {
-      if (x.max > m || (x.max == m && x.at < at)) {
-        m = x.max;
-        at = x.at;
-      }
+  for (int z = 0; z < N; ++z) v[z] = logits4(x, i0 + z * 128, end, aligned);
+  float m = -INFINITY;
+#pragma unroll
+  for (int z = 0; z < N; ++z) m = fmaxf(m, fmaxf(fmaxf(v[z].x, v[z].y), fmaxf(v[z].z, v[z].w)));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float s = 0.0f;
+  int at = INT_MAX;
+  if (q.T == 0.0f) {  // the first of the largest
+#pragma unroll
+    for (int z = N - 1; z >= 0; --z) {
+      const float e[4] = {v[z].x, v[z].y, v[z].z, v[z].w};
+#pragma unroll
+      for (int w = 3; w >= 0; --w)
+        if (e[w] == m && i0 + z * 128 + w < end) at = i0 + z * 128 + w;
+    }
+    at = __reduce_min_sync(0xffffffffu, at);
+  } else {
+    const float mt = m == -INFINITY ? 0.0f : m;  // nothing but -inf: the sum is 0
+    auto term = [&](float x) {                   // 0 for -inf and NaN
+      const float d = x - mt;
+      return ex2(fmaxf(fmaf(d, q.c_hi, d * q.c_lo), -200.0f));
     };
 #pragma unroll
-    for (int k = 0; k < U; ++k) top(q[k]);
-    for (int i = lane + 32 * U; i < a.segs; i += 32) top(p[i]);
+    for (int z = 0; z < N; ++z) s += (term(v[z].x) + term(v[z].y)) + (term(v[z].z) + term(v[z].w));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
-      const int a2 = __shfl_xor_sync(0xffffffffu, at, o);
-      top(RowPart{m2, 0.0f, a2, 0});
-    }
-    double s = 0.0;
-    if (T > 0.0f) {
-      auto add = [&](const RowPart& x) {
-        if (x.sum != 0.0f) s += (double)(x.sum * exp_scaled(x.max - m, c_hi, c_lo));
-      };
-#pragma unroll
-      for (int k = 0; k < U; ++k) add(q[k]);
-      for (int i = lane + 32 * U; i < a.segs; i += 32) add(p[i]);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    }
-    if (lane == 0) {
-      const int to = r <= n ? r : a.drafts + r - n;
-      s_max[to] = m;
-      s_sum[to] = s;
-      if (r <= n) s_at[r] = at;
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  }
+  return RowPart{m, s, at, 0};
+}
+
+__device__ __forceinline__ RowPart no_part() { return RowPart{-INFINITY, 0.0f, INT_MAX, 0}; }
+
+// Two parts of a row as one.
+__device__ __forceinline__ RowPart join(const Sequence& q, const RowPart& x, const RowPart& y) {
+  RowPart z = x.max > y.max || (x.max == y.max && x.at < y.at) ? x : y;
+  z.sum = (x.sum != 0.0f ? x.sum * exp_scaled(x.max - z.max, q.c_hi, q.c_lo) : 0.0f) +
+          (y.sum != 0.0f ? y.sum * exp_scaled(y.max - z.max, q.c_hi, q.c_lo) : 0.0f);
+  return z;
+}
+// The parts that `width` neighbouring lanes (a power of two) hold, joined for all of them.
+__device__ __forceinline__ RowPart join_lanes(const Sequence& q, const RowPart& p, int width) {
+  float m = p.max;
+  int at = p.at;
+  for (int o = 1; o < width; o <<= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
+    const int a2 = __shfl_xor_sync(0xffffffffu, at, o);
+    if (m2 > m || (m2 == m && a2 < at)) {
+      m = m2;
+      at = a2;
     }
   }
-  __syncthreads();
-  if (warp) return;
+  float s = p.sum != 0.0f ? p.sum * exp_scaled(p.max - m, q.c_hi, q.c_lo) : 0.0f;
+  for (int o = 1; o < width; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return RowPart{m, s, at, 0};
+}
+
+// Step 2.  A warp's lane j asks for drafted token j and its logits...
+struct Drafted {
+  int64_t token;
+  float x, y, u;
+};
+__device__ __forceinline__ Drafted ask_drafted(const Sequence& q, int j) {
+  const VerifyArgs& a = q.a;
+  Drafted d = {-1, 0.0f, 0.0f, 0.0f};
+  if (j < q.n) {
+    d.token = a.tokens[q.b * a.ldtok + j];
+    if (d.token >= 0 && d.token < a.vocab && q.T > 0.0f) {
+      d.x = a.target[q.b * a.tseq + j * a.ldt + d.token];
+      if (q.drafted) d.y = a.draft[q.b * a.dseq + j * a.ldd + d.token];
+      d.u = a.uniforms[q.b * a.ldu + j];
+    }
+  }
+  return d;
+}
+// ... and follows them, once `row` holds all rows: how many are taken, and what the draw needs.
+__device__ __forceinline__ Pick follow(const Sequence& q, const Drafted& d, const RowPart* row, bool report) {
+  const int j = threadIdx.x & 31, n = q.n;
   bool take = false;
-  if (lane < n) {
-    if (d < 0 || d >= a.vocab) {
-      atomicExch(&g_verify_device_error, 1);
-    } else if (T == 0.0f) {
-      take = d == s_at[lane];
+  if (j < n) {
+    if (d.token < 0 || d.token >= q.a.vocab) {
+      if (report) atomicExch(&g_verify_device_error, 1);
+    } else if (q.T == 0.0f) {
+      take = d.token == row[j].at;
     } else {
-      const double p = exp(((double)xd - (double)s_max[lane]) / (double)T) / s_sum[lane];
-      double q = 1.0;
-      if (drafted) {
-        q = exp(((double)yd - (double)s_max[a.drafts + 1 + lane]) / (double)T) / s_sum[a.drafts + 1 + lane];
-        if (!(q >= 0.0)) q = 0.0;  // a NaN
+      const double p = exp(((double)d.x - (double)row[j].max) / (double)q.T) / (double)row[j].sum;
+      double r = 1.0;
+      if (q.drafted) {
+        r = exp(((double)d.y - (double)row[n + 1 + j].max) / (double)q.T) / (double)row[n + 1 + j].sum;
+        if (!(r >= 0.0)) r = 0.0;  // a NaN
       }
-      take = (double)u * q < p;
+      take = (double)d.u * r < p;
     }
   }
   const unsigned no = ~__ballot_sync(0xffffffffu, take);
-  const int taken = no ? min(__ffs((int)no) - 1, n) : n;
-  if (T == 0.0f) {
-    write_tokens(a, b, taken, s_at[taken] == INT_MAX ? -1 : s_at[taken], lane, 32);
-    if (lane == 0) a.picks[b].taken = -1;
-    return;
-  }
-  const bool refused = taken < n;
-  const int64_t out_of = __shfl_sync(0xffffffffu, d, min(taken, 31));
-  if (lane == 0) {
-    Pick k;
-    k.taken = taken;
-    k.refused = refused;
-    k.drafted = drafted && refused;
-    k.out_of = refused && !drafted && out_of >= 0 && out_of < a.vocab ? (int)out_of : -1;
-    k.xm = s_max[taken];
-    k.xi = (float)(1.0 / s_sum[taken]);
-    k.ym = k.drafted ? s_max[a.drafts + 1 + taken] : 0.0f;
-    k.yi = k.drafted ? (float)(1.0 / s_sum[a.drafts + 1 + taken]) : 0.0f;
-    k.c_hi = c_hi;
-    k.c_lo = c_lo;
-    a.picks[b] = k;
-  }
+  Pick k;
+  k.taken = no ? min(__ffs((int)no) - 1, n) : n;
+  k.refused = k.taken < n;
+  k.drafted = q.drafted && k.refused;
+  const int64_t token = __shfl_sync(0xffffffffu, d.token, min(k.taken, 31));
+  k.out_of = k.refused && !q.drafted && token >= 0 && token < q.a.vocab ? (int)token : -1;
+  k.xm = row[k.taken].max;
+  k.xi = 1.0f / row[k.taken].sum;
+  k.ym = k.drafted ? row[n + 1 + k.taken].max : 0.0f;
+  k.yi = k.drafted ? 1.0f / row[n + 1 + k.taken].sum : 0.0f;
+  return k;
 }
+// With temperature 0 the token that follows, or -1.
+__device__ __forceinline__ int64_t greedy(const RowPart& p) { return p.at == INT_MAX ? -1 : p.at; }
 
-// The leader of the race: the largest w / e, and its index.
+// Step 3.  The leader of the race: the largest w / e, and its index.
 struct __align__(8) Leader {
   float best;
   int at;
@@ -290,82 +276,79 @@ struct __align__(8) Leader {
   }
 };
 
-// The draw: a cluster of `ctas` CTAs per sequence, the vocabulary cut among them, their leaders
-// exchanged through distributed shared memory.  An entry is weighed with the hardware's exponential
-// first, whose error is far below the margin 2^-16; only what may beat its warp's leader by then is
-// computed with care (some 10 entries of a warp), so the loop stays near 25 instructions per entry.
-// A thread requests kRaceBatch pieces of each row before it uses them.
-constexpr int kRaceCluster = 8;
-constexpr int kRaceThreads = 256;
-constexpr int kRaceBatch = 4;
+// A warp's part of the race over entries [i0, end) in pieces of 128, `step` apart, U of them
+// requested at a time.  An entry is weighed with the hardware's exponential first, whose error is
+// far below the margin 2^-16; only what may beat the warp's leader by then is computed with care
+// (some 10 entries), so the loop stays near 25 instructions per entry.  y null: p alone.
+template <int U>
+__device__ __forceinline__ Leader race(const Sequence& q, const Pick& k, const float* y, int out_of, int i0, int end, int step) {
+  const int lane = threadIdx.x & 31;
+  const float* x = q.row(k.taken);
+  const float* e = q.a.noise + q.b * q.a.ldn;
+  const bool ax = (reinterpret_cast<uintptr_t>(x) & 15) == 0, ay = (reinterpret_cast<uintptr_t>(y) & 15) == 0,
+             ae = (reinterpret_cast<uintptr_t>(e) & 15) == 0;
+  Leader lead = {0.0f, INT_MAX};
+  float bar = 0.0f;  // the warp's leader
+  for (; i0 < end; i0 += U * step) {
+    float4 vx[U], ve[U], vy[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int i = min(i0 + j * step, end) + 4 * lane;  // behind the end: -inf without a read
+      vx[j] = logits4(x, i, end, ax);
+      ve[j] = logits4(e, i, end, ae);
+      vy[j] = y ? logits4(y, i, end, ay) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int i = min(i0 + j * step, end) + 4 * lane;
+      const float fx[4] = {vx[j].x, vx[j].y, vx[j].z, vx[j].w}, fy[4] = {vy[j].x, vy[j].y, vy[j].z, vy[j].w},
+                  fe[4] = {ve[j].x, ve[j].y, ve[j].z, ve[j].w};
+      bool may[4], any = false;
+#pragma unroll
+      for (int z = 0; z < 4; ++z) {
+        const float dx = fx[z] - k.xm, dy = fy[z] - k.ym;
+        const float p = ex2(fmaxf(fmaf(dx, q.c_hi, dx * q.c_lo), -200.0f)) * k.xi;
+        float r = 0.0f;
+        if (y) r = ex2(fmaxf(fmaf(dy, q.c_hi, dy * q.c_lo), -200.0f)) * k.yi;
+        may[z] = fmaf(p + r, 0x1p-16f, p - r) > bar * fe[z] && i + z != out_of && i + z < end;
+        any |= may[z];
+      }
+      if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+        for (int z = 0; z < 4; ++z)
+          if (may[z]) {
+            // products that round by themselves: equal rows leave exactly nothing
+            float w = __fmul_rn(exp_scaled(fx[z] - k.xm, q.c_hi, q.c_lo), k.xi);
+            if (y) w = __fsub_rn(w, __fmul_rn(exp_scaled(fy[z] - k.ym, q.c_hi, q.c_lo), k.yi));
+            if (w > 0.0f) lead.take(w / fe[z], i + z);
+          }
+        bar = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(lead.best)));
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float s2 = __shfl_xor_sync(0xffffffffu, lead.best, o);
+    const int i2 = __shfl_xor_sync(0xffffffffu, lead.at, o);
+    lead.take(s2, i2);
+  }
+  return lead;
+}
 
-__global__ void __launch_bounds__(kRaceThreads, 2) k_verify_race(VerifyArgs a, int ctas) {
-  constexpr int W = kRaceThreads / 32, U = kRaceBatch;
+// The race over a cluster: CTA `rank` of `ctas` runs over entries [i0 of its warps, end), the leaders
+// meet in every CTA.  Returns the winner, or -1.  The caller's cluster runs by now.
+template <int U>
+__device__ __forceinline__ int64_t race_cluster(const Sequence& q, const Pick& k, int i0, int end, int step, int rank, int ctas) {
+  constexpr int W = kVerifyWarps;
   __shared__ Leader s_lead[W];
-  __shared__ Leader s_all[2][kRaceCluster];
-  pdl_trigger();
-  pdl_wait();
-  const int b = blockIdx.x / ctas, rank = blockIdx.x - b * ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const Pick k = a.picks[b];
-  if (k.taken < 0) return;  // done already; the whole cluster returns
-  cluster_arrive_relaxed();
-  const float* x = a.target + b * a.tseq + k.taken * a.ldt;
-  const float* e = a.noise + b * a.ldn;
-  const bool ax = (reinterpret_cast<uintptr_t>(x) & 15) == 0, ae = (reinterpret_cast<uintptr_t>(e) & 15) == 0;
-  const float* y = k.drafted ? a.draft + b * a.dseq + k.taken * a.ldd : nullptr;
+  __shared__ Leader s_all[2][kVerifyCluster];
+  const int tid = threadIdx.x;
+  const float* y = k.drafted ? q.row(q.n + 1 + k.taken) : nullptr;
   int out_of = k.out_of;
-  int64_t last = -1;
-  const int step = 4 * kRaceThreads * ctas;
   for (int pass = 0;; ++pass) {  // a second one where nothing of p - q is left: p itself
-    const bool ay = (reinterpret_cast<uintptr_t>(y) & 15) == 0;
-    Leader lead = {0.0f, INT_MAX};
-    float bar = 0.0f;  // the warp's leader
-    for (int i0 = 4 * (rank * kRaceThreads + warp * 32); i0 < a.vocab; i0 += U * step) {
-      float4 vx[U], ve[U], vy[U];
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int i = min(i0 + j * step, a.vocab) + 4 * lane;  // behind the end: -inf without a read
-        vx[j] = logits4(x, i, a.vocab, ax);
-        ve[j] = logits4(e, i, a.vocab, ae);
-        vy[j] = y ? logits4(y, i, a.vocab, ay) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      }
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int i = min(i0 + j * step, a.vocab) + 4 * lane;
-        const float fx[4] = {vx[j].x, vx[j].y, vx[j].z, vx[j].w}, fy[4] = {vy[j].x, vy[j].y, vy[j].z, vy[j].w},
-                    fe[4] = {ve[j].x, ve[j].y, ve[j].z, ve[j].w};
-        bool may[4], any = false;
-#pragma unroll
-        for (int z = 0; z < 4; ++z) {
-          const float dx = fx[z] - k.xm, dy = fy[z] - k.ym;
-          const float p = ex2(fmaxf(fmaf(dx, k.c_hi, dx * k.c_lo), -200.0f)) * k.xi;
-          float q = 0.0f;
-          if (y) q = ex2(fmaxf(fmaf(dy, k.c_hi, dy * k.c_lo), -200.0f)) * k.yi;
-          may[z] = fmaf(p + q, 0x1p-16f, p - q) > bar * fe[z] && i + z != out_of && i + z < a.vocab;
-          any |= may[z];
-        }
-        if (__any_sync(0xffffffffu, any)) {
-#pragma unroll
-          for (int z = 0; z < 4; ++z)
-            if (may[z]) {
-              // products that round by themselves: equal rows leave exactly nothing
-              float w = __fmul_rn(exp_scaled(fx[z] - k.xm, k.c_hi, k.c_lo), k.xi);
-              if (y) w = __fsub_rn(w, __fmul_rn(exp_scaled(fy[z] - k.ym, k.c_hi, k.c_lo), k.yi));
-              if (w > 0.0f) lead.take(w / fe[z], i + z);
-            }
-          bar = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(lead.best)));
-        }
-      }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float s2 = __shfl_xor_sync(0xffffffffu, lead.best, o);
-      const int i2 = __shfl_xor_sync(0xffffffffu, lead.at, o);
-      lead.take(s2, i2);
-    }
-    if (lane == 0) s_lead[warp] = lead;
+    Leader lead = race<U>(q, k, y, out_of, i0, end, step);
+    if ((tid & 31) == 0) s_lead[tid >> 5] = lead;
     __syncthreads();
-    if (pass == 0) cluster_wait();  // all CTAs of the cluster run
     if (tid < ctas) {
       for (int w = 0; w < W; ++w) lead.take(s_lead[w].best, s_lead[w].at);
       st_cluster_v2(mapa_shared(smem_u32(&s_all[pass][rank]), tid), __float_as_uint(lead.best), (uint32_t)lead.at);
@@ -374,13 +357,138 @@ __global__ void __launch_bounds__(kRaceThreads, 2) k_verify_race(VerifyArgs a, i
     cluster_sync_all();
     Leader all = s_all[pass][0];
     for (int r = 1; r < ctas; ++r) all.take(s_all[pass][r].best, s_all[pass][r].at);
-    if (all.at != INT_MAX) last = all.at;
-    if (last >= 0 || pass == 1 || !k.refused) break;
+    if (all.at != INT_MAX) return all.at;
+    if (pass == 1 || !k.refused) return -1;
     y = nullptr;
     out_of = -1;
   }
-  if (rank == 0) write_tokens(a, b, k.taken, last, tid, kRaceThreads);
 }
+
+// All in one launch: a cluster of `ctas` CTAs per sequence.
+__global__ void __launch_bounds__(kVerifyThreads, 3) k_verify(VerifyArgs a, int ctas) {
+  constexpr int W = kVerifyWarps;
+  __shared__ RowPart s_part[kVerifyMaxRows][W];              // this slice's rows, by warp
+  __shared__ RowPart s_cta[kVerifyMaxRows][kVerifyCluster];  // the rows, by CTA
+  __shared__ RowPart s_row[kVerifyMaxRows];
+  __shared__ Pick s_pick;
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.x / ctas, rank = blockIdx.x - b * ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Sequence q(a, b);
+  const int rows = q.rows();
+  if (rows == 0) {
+    if (rank == 0) write_tokens(q, 0, -1, tid, kVerifyThreads);
+    return;  // as the whole cluster does
+  }
+  cluster_arrive_relaxed();
+  Drafted d = {-1, 0.0f, 0.0f, 0.0f};
+  if (warp == 0) d = ask_drafted(q, lane);
+  const int s0 = min(a.vocab, rank * a.slice), s1 = min(a.vocab, s0 + a.slice);
+  // The slice's segments go round `slots` warps, the same ones in every row; several rows at once
+  // where the slice has few segments.
+  const int segs = (a.slice + kVerifySeg - 1) / kVerifySeg;
+  const int slots = segs >= 8 ? 8 : segs >= 4 ? 4 : segs >= 2 ? 2 : 1;
+  for (int r = warp / slots; r < rows; r += W / slots) {
+    const float* x = q.row(r);
+    RowPart p = no_part();
+    for (int seg = warp % slots; seg < segs; seg += slots) p = join(q, p, read_segment(q, x, s0 + seg * kVerifySeg, s1));
+    if (lane == 0) s_part[r][warp % slots] = p;
+  }
+  __syncthreads();
+  cluster_wait();  // all CTAs of the cluster run
+  for (int r = warp; r < rows; r += W) {
+    const RowPart p = join_lanes(q, s_part[r][lane % slots], slots);
+    if (lane < ctas) st_cluster_v4(mapa_shared(smem_u32(&s_cta[r][rank]), lane), p.max, p.sum, p.at);
+  }
+  __syncwarp();
+  cluster_sync_all();
+  for (int r = warp; r < rows; r += W) {
+    const RowPart p = join_lanes(q, s_cta[r][lane % ctas], ctas);
+    if (lane == 0) s_row[r] = p;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const Pick k = follow(q, d, s_row, rank == 0);
+    if (lane == 0) s_pick = k;
+  }
+  __syncthreads();
+  const Pick k = s_pick;
+  const int64_t last = q.T == 0.0f ? greedy(s_row[k.taken])
+                                   : race_cluster<2>(q, k, s0 + 128 * warp, s1, 128 * W, rank, ctas);
+  if (rank == 0) write_tokens(q, k.taken, last, tid, kVerifyThreads);
+}
+
+// Step 1 alone: grid (blocks of 8 segments, row groups, batch), a warp per segment.  The warps of a CTA
+// never meet.  A CTA goes through its group's rows, so that rows that a sequence with fewer
+// drafted tokens does not have cost nothing.
+__global__ void __launch_bounds__(kVerifyThreads, 4) k_verify_rows(VerifyArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  const int seg = blockIdx.x * kVerifyWarps + (threadIdx.x >> 5);
+  if (seg >= a.segs) return;
+  const Sequence q(a, blockIdx.z);
+  const int rows = q.rows();
+  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+    const RowPart p = read_segment(q, q.row(r), seg * kVerifySeg, a.vocab);
+    if ((threadIdx.x & 31) == 0) q.part(r)[seg] = p;
+  }
+}
+
+// Step 2 alone: a CTA per sequence, a warp per row.  Latency-bound.
+__global__ void __launch_bounds__(kPickThreads, 2) k_verify_pick(VerifyArgs a) {
+  __shared__ RowPart s_row[kVerifyMaxRows];
+  pdl_trigger();
+  pdl_wait();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Sequence q(a, blockIdx.x);
+  const int rows = q.rows();
+  if (rows == 0) {
+    if (tid == 0) a.picks[q.b].taken = -1;
+    write_tokens(q, 0, -1, tid, kPickThreads);
+    return;
+  }
+  Drafted d = {-1, 0.0f, 0.0f, 0.0f};
+  if (warp == 0) d = ask_drafted(q, lane);
+  for (int r = warp; r < rows; r += kPickThreads / 32) {
+    constexpr int U = 4;  // a lane's parts of 128 segments, requested together
+    const RowPart* p = q.part(r);
+    RowPart x[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) x[k] = lane + 32 * k < a.segs ? p[lane + 32 * k] : no_part();
+    RowPart z = x[0];
+#pragma unroll
+    for (int k = 1; k < U; ++k) z = join(q, z, x[k]);
+    for (int i = lane + 32 * U; i < a.segs; i += 32) z = join(q, z, p[i]);
+    z = join_lanes(q, z, 32);
+    if (lane == 0) s_row[r] = z;
+  }
+  __syncthreads();
+  if (warp) return;
+  Pick k = follow(q, d, s_row, true);
+  if (q.T == 0.0f) {
+    write_tokens(q, k.taken, greedy(s_row[k.taken]), lane, 32);
+    k.taken = -1;
+  }
+  if (lane == 0) a.picks[q.b] = k;
+}
+
+// Step 3 alone: a cluster of `ctas` CTAs per sequence.
+__global__ void __launch_bounds__(kVerifyThreads, 2) k_verify_race(VerifyArgs a, int ctas) {
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.x / ctas, rank = blockIdx.x - b * ctas;
+  const Pick k = a.picks[b];
+  if (k.taken < 0) return;  // done already; the whole cluster returns
+  cluster_arrive_relaxed();
+  const Sequence q(a, b);
+  cluster_wait();  // all CTAs of the cluster run
+  const int64_t last = race_cluster<4>(q, k, 4 * (rank * kVerifyThreads + (threadIdx.x & ~31)), a.vocab,
+                                       4 * kVerifyThreads * ctas, rank, ctas);
+  if (rank == 0) write_tokens(q, k.taken, last, threadIdx.x, kVerifyThreads);
+}
+
+// One launch, or the workspace of three.
+static bool one_launch(int64_t batch, int64_t rows, int64_t vocab) { return batch * rows <= kVerifyOneLaunch / vocab; }
 
 }  // namespace otf
 
@@ -400,8 +508,10 @@ int otf::verify_device_error(int clear) {
   return v;
 }
 
-extern "C" OTF_API int64_t otf_verify_workspace_bytes(int64_t batch, int64_t drafts, int64_t vocab) {
-  if (batch <= 0 || drafts < 0 || drafts > otf::kVerifyMaxDrafts || vocab <= 0 || vocab > INT32_MAX / 2) return -1;
+extern "C" OTF_API int64_t otf_verify_workspace_bytes(int64_t batch, int64_t drafts, int64_t vocab, int with_draft) {
+  if (batch <= 0 || batch > 65535 || drafts < 0 || drafts > otf::kVerifyMaxDrafts || vocab <= 0 || vocab > (1 << 30))
+    return -1;
+  if (otf::one_launch(batch, drafts + 1 + (with_draft ? drafts : 0), vocab)) return 0;
   const int64_t segs = (vocab + otf::kVerifySeg - 1) / otf::kVerifySeg;
   return otf::align_up(batch * (int64_t)sizeof(otf::Pick), 256) +
          otf::align_up(batch * (2 * drafts + 1) * segs * (int64_t)sizeof(otf::RowPart), 256);
@@ -414,50 +524,71 @@ extern "C" OTF_API int otf_verify_drafts(const float* target, int64_t target_seq
                                          const float* temperatures, float temperature, const int32_t* counts,
                                          int64_t* out_tokens, int32_t* accepted, int64_t batch, int64_t drafts,
                                          int64_t vocab, void* workspace, int64_t workspace_bytes, void* stream) {
-  if (!target || !out_tokens || !accepted || !workspace || batch <= 0 || drafts < 0 || vocab <= 0)
-    return OTF_ERR_INVALID;
-  if (drafts > otf::kVerifyMaxDrafts || vocab > INT32_MAX / 2 || batch > 65535)
-    return OTF_ERR_UNSUPPORTED;
+  if (!target || !out_tokens || !accepted || batch <= 0 || drafts < 0 || vocab <= 0) return OTF_ERR_INVALID;
+  if (drafts > otf::kVerifyMaxDrafts || vocab > (1 << 30) || batch > 65535) return OTF_ERR_UNSUPPORTED;
   if (drafts > 0 && (!tokens || ld_tokens < drafts || (uniforms && ld_uniforms < drafts))) return OTF_ERR_INVALID;
   if (ld_target < vocab || target_seq < 0 || (noise && ld_noise < vocab)) return OTF_ERR_INVALID;
-  if (draft && drafts > 0 && (ld_draft < vocab || draft_seq < 0)) return OTF_ERR_INVALID;
+  if (drafts == 0) draft = nullptr;
+  if (draft && (ld_draft < vocab || draft_seq < 0)) return OTF_ERR_INVALID;
   if (!temperatures) {
     if (!otf::temperature_ok(temperature)) return OTF_ERR_INVALID;
     if (temperature > 0.0f && (!noise || (drafts > 0 && !uniforms))) return OTF_ERR_INVALID;
   }
-  if ((reinterpret_cast<uintptr_t>(workspace) & 255) ||
-      workspace_bytes < otf_verify_workspace_bytes(batch, drafts, vocab))
+  const int64_t bytes = otf_verify_workspace_bytes(batch, drafts, vocab, draft != nullptr);
+  if (bytes > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < bytes))
     return OTF_ERR_INVALID;
   int st = check_device();
   if (st != OTF_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int segs = (int)((vocab + otf::kVerifySeg - 1) / otf::kVerifySeg);
-  char* w = static_cast<char*>(workspace);
-  const otf::VerifyArgs a = {target,
-                             drafts ? draft : nullptr,
-                             target_seq,
-                             ld_target,
-                             draft_seq,
-                             ld_draft,
-                             tokens,
-                             ld_tokens,
-                             uniforms,
-                             ld_uniforms,
-                             noise,
-                             ld_noise,
-                             temperatures,
-                             temperature,
-                             counts,
-                             out_tokens,
-                             accepted,
-                             (int)drafts,
-                             (int)vocab,
-                             segs,
-                             reinterpret_cast<otf::RowPart*>(w + otf::align_up(batch * (int64_t)sizeof(otf::Pick), 256)),
-                             reinterpret_cast<otf::Pick*>(w)};
+  otf::VerifyArgs a = {};
+  a.target = target;
+  a.tseq = target_seq;
+  a.ldt = ld_target;
+  a.draft = draft;
+  a.dseq = draft_seq;
+  a.ldd = ld_draft;
+  a.tokens = tokens;
+  a.ldtok = ld_tokens;
+  a.uniforms = uniforms;
+  a.ldu = ld_uniforms;
+  a.noise = noise;
+  a.ldn = ld_noise;
+  a.temperatures = temperatures;
+  a.temperature = temperature;
+  a.counts = counts;
+  a.out = out_tokens;
+  a.accepted = accepted;
+  a.drafts = (int)drafts;
+  a.vocab = (int)vocab;
+  if (bytes == 0) {
+    {
+      // clusters of 16 are beyond the portable size: allowed once per device
+      static std::mutex mu;
+      static bool done[64] = {};
+      int dev = 0;
+      cudaError_t e = cudaGetDevice(&dev);
+      if (e != cudaSuccess) return set_cuda_error(e);
+      std::lock_guard<std::mutex> lock(mu);
+      if (dev < 0 || dev >= 64 || !done[dev]) {
+        e = cudaFuncSetAttribute(otf::k_verify, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return set_cuda_error(e);
+        if (dev >= 0 && dev < 64) done[dev] = true;
+      }
+    }
+    // CTAs per sequence: 16 (of such clusters 14 run at once), 8, or as many as all run at once, three
+    // on an SM; no more than the vocabulary has segments
+    int ctas = batch <= 8 ? 16 : 8;
+    while (ctas > 1 && (batch * ctas > 3 * 148 || (int64_t)(ctas - 1) * otf::kVerifySeg >= vocab)) ctas /= 2;
+    a.slice = (int)(((vocab + ctas - 1) / ctas + 3) & ~3ll);
+    return set_cuda_error(otf::launch_pdl(otf::k_verify, dim3((unsigned)(batch * ctas)), dim3(otf::kVerifyThreads), 0, s,
+                                          (unsigned)ctas, a, ctas));
+  }
+  a.segs = (int)((vocab + otf::kVerifySeg - 1) / otf::kVerifySeg);
+  a.picks = static_cast<otf::Pick*>(workspace);
+  a.parts = reinterpret_cast<otf::RowPart*>(static_cast<char*>(workspace) +
+                                            otf::align_up(batch * (int64_t)sizeof(otf::Pick), 256));
   // row groups: one per row while all of their CTAs fit the GPU at once, else 4
-  const int64_t rows = drafts + 1 + (a.draft ? drafts : 0);
-  const int64_t blocks = (segs + 7) / 8;
+  const int64_t rows = drafts + 1 + (draft ? drafts : 0), blocks = (a.segs + otf::kVerifyWarps - 1) / otf::kVerifyWarps;
   const int64_t groups = std::min<int64_t>(rows, batch * blocks * rows <= 4 * 148 ? rows : 4);
   cudaError_t e = otf::launch_pdl(otf::k_verify_rows, dim3((unsigned)blocks, (unsigned)groups, (unsigned)batch),
                                   dim3(otf::kVerifyThreads), 0, s, 1u, a);
@@ -467,6 +598,6 @@ extern "C" OTF_API int otf_verify_drafts(const float* target, int64_t target_seq
   // CTAs per sequence: as many as all run at once, two on an SM
   int ctas = otf::kRaceCluster;
   while (ctas > 1 && batch * ctas > 2 * 148) ctas /= 2;
-  return set_cuda_error(otf::launch_pdl(otf::k_verify_race, dim3((unsigned)(batch * ctas)), dim3(otf::kRaceThreads), 0, s,
+  return set_cuda_error(otf::launch_pdl(otf::k_verify_race, dim3((unsigned)(batch * ctas)), dim3(otf::kVerifyThreads), 0, s,
                                         (unsigned)ctas, a, ctas));
 }

@@ -229,7 +229,7 @@ def lib() -> ctypes.CDLL:
     L.otf_paged_attn.restype = i32
     L.otf_paged_evict.argtypes = [cache, cache, vp, i64, vp, i64, i64, i64, vp, vp, vp]
     L.otf_paged_evict.restype = i32
-    L.otf_verify_workspace_bytes.argtypes = [i64, i64, i64]
+    L.otf_verify_workspace_bytes.argtypes = [i64, i64, i64, i32]
     L.otf_verify_workspace_bytes.restype = i64
     L.otf_verify_drafts.argtypes = [vp, i64, i64, vp, i64, i64, vp, i64, vp, i64, vp, i64, vp, ctypes.c_float, vp, vp,
                                     vp, i64, i64, i64, vp, i64, vp]

@@ -67,9 +67,10 @@ def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, *,
         pc = _vector(counts, "counts", torch.int32, batch, dev)
     tokens = torch.empty((batch, drafts + 1), dtype=torch.int64, device=dev)
     accepted = torch.empty(batch, dtype=torch.int32, device=dev)
-    ws = torch.empty(bytes_, dtype=torch.uint8, device=dev)     # for this call alone, on its stream
+    # a large call's scratch, for this call alone and on its stream
+    ws = torch.empty(bytes_, dtype=torch.uint8, device=dev) if bytes_ else None
     _call("otf_verify_drafts", dev, pt, seq_t, ld_t, pd, seq_d, ld_d, ptok, ld_tok, pu, ld_u, pn, ld_n, each, one, pc,
-          tokens.data_ptr(), accepted.data_ptr(), batch, drafts, vocab, ws.data_ptr(), bytes_)
+          tokens.data_ptr(), accepted.data_ptr(), batch, drafts, vocab, ws.data_ptr() if bytes_ else None, bytes_)
     return tokens, accepted
 
 
@@ -117,7 +118,7 @@ def _plan(target: torch.Tensor, tokens: torch.Tensor, draft: Optional[torch.Tens
         ld_u, = _rows(uniforms, "uniforms", (batch, drafts))
     if noise is not None:
         ld_n, = _rows(noise, "noise", (batch, vocab))
-    n = _native.lib().otf_verify_workspace_bytes(batch, drafts, vocab)
+    n = _native.lib().otf_verify_workspace_bytes(batch, drafts, vocab, 0 if draft is None or drafts == 0 else 1)
     if n < 0:
         raise ValueError("shape not supported by otf_verify_drafts")
     return target.device, batch, drafts, vocab, seq_t, ld_t, ld_tok, seq_d, ld_d, ld_u, ld_n, n

@@ -130,18 +130,22 @@ def test_abi_refuses_bad_arguments():
 def test_abi_refuses_bad_verifications():
     from otf_llm import _native as N
     L = N.lib()
-    n = L.otf_verify_workspace_bytes(2, 3, 100)
+    assert L.otf_verify_workspace_bytes(2, 3, 100, 1) == 0
+    n = L.otf_verify_workspace_bytes(64, 5, 128256, 1)
     assert n > 0
-    for bad in ((0, 3, 100), (2, -1, 100), (2, 33, 100), (2, 3, 0)):
+    for bad in ((0, 3, 100, 0), (2, -1, 100, 0), (2, 33, 100, 0), (2, 3, 0, 0), (65536, 3, 100, 0), (2, 3, (1 << 30) + 1, 0)):
         assert L.otf_verify_workspace_bytes(*bad) == -1
 
     def verify(t=FAKE, ts=400, ldt=100, d=None, ds=0, ldd=0, tok=FAKE, ldtok=3, u=FAKE, ldu=3, e=FAKE, lde=100, temp=1.0,
-               out=FAKE, acc=FAKE, batch=2, drafts=3, vocab=100, ws=FAKE, size=n):
+               out=FAKE, acc=FAKE, batch=2, drafts=3, vocab=100, ws=None, size=0):
         return L.otf_verify_drafts(t, ts, ldt, d, ds, ldd, tok, ldtok, u, ldu, e, lde, None, temp, None, out, acc, batch,
                                    drafts, vocab, ws, size, None)
     for bad in (dict(t=None), dict(ldt=99), dict(d=FAKE, ldd=99), dict(tok=None), dict(ldtok=2), dict(u=None),
                 dict(ldu=2), dict(e=None), dict(lde=99), dict(temp=-1.0), dict(temp=float("nan")),
                 dict(temp=float("inf")), dict(temp=1e-30), dict(out=None), dict(acc=None), dict(batch=0),
-                dict(drafts=-1), dict(vocab=0), dict(ws=None), dict(ws=FAKE + 8), dict(size=n - 1)):
+                dict(drafts=-1), dict(vocab=0)):
         assert verify(**bad) == INVALID, bad
     assert verify(drafts=33, ldtok=33, ldu=33) == UNSUPPORTED
+    large = dict(ldt=128256, d=FAKE, ldd=128256, ldtok=5, ldu=5, lde=128256, batch=64, drafts=5, vocab=128256)
+    for bad in (dict(ws=None, size=n), dict(ws=FAKE + 8, size=n), dict(ws=FAKE, size=n - 1)):
+        assert verify(**large, **bad) == INVALID, bad
