@@ -29,6 +29,7 @@ import torch
 
 from . import _native
 from .decoder_stack import shard_linear
+from .paged import rope_frequencies
 from .symmetric_2bit_engine import QuantizedEmbedding, QuantizedLinearHead, SymmetricOTF2BitLinear
 
 PROJ = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj")
@@ -46,6 +47,7 @@ class ModelConfig:
     rope_theta: float = 500000.0
     rms_eps: float = 1e-5
     max_pos: int = 2048
+    rope_scaling: Optional[dict] = None   # as HF's rope_scaling: see otf_llm.paged.rope_frequencies
 
 
 LLAMA32_3B = ModelConfig(layers=28, hidden=3072, intermediate=8192, heads=24, kv_heads=8, head_dim=128,
@@ -77,9 +79,16 @@ def shard_layers(layers: Sequence[Dict[str, SymmetricOTF2BitLinear]], cfg: Model
 
 
 def rope_table(cfg: ModelConfig, device) -> torch.Tensor:
-    """fp16 [max_pos, 2, head_dim]: HF's default rotary cos and sin rows (fp32 angles
-    pos * theta^(-2i/d), both halves duplicated, rounded to fp16 as HF casts them)."""
+    """fp16 [max_pos, 2, head_dim]: HF's rotary cos and sin rows (fp32 angles
+    pos * theta^(-2i/d), both halves duplicated, rounded to fp16 as HF casts them).  With
+    ``cfg.rope_scaling`` the frequencies are the scaled ones, the angles in 64 bits, and the rows
+    are multiplied by the scaling's attention factor."""
     d = cfg.head_dim
+    if cfg.rope_scaling is not None:
+        freqs, factor = rope_frequencies(d, cfg.rope_theta, cfg.rope_scaling)
+        ang = torch.arange(cfg.max_pos, dtype=torch.float64, device=device)[:, None] * freqs.to(device)[None, :]
+        emb = torch.cat((ang, ang), dim=-1)
+        return torch.stack((emb.cos() * factor, emb.sin() * factor), dim=1).to(torch.float16).contiguous()
     inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, d, 2, dtype=torch.int64, device=device).float() / d))
     pos = torch.arange(cfg.max_pos, device=device, dtype=torch.float32)
     freqs = pos[:, None] * inv[None, :]

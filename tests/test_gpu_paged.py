@@ -239,6 +239,10 @@ def test_attend_peaked_and_flat_scores(dtype, cuda_dev):
 def test_attend_many_sequences_and_long_ones(cuda_dev):
     check_attend(cuda_dev, [1 + (37 * b) % 90 for b in range(150)], 1, 16, 4, 2, 64, torch.float16)
     check_attend(cuda_dev, [9000, 1, 40], 1, 64, 4, 1, 64, torch.float16, weights=True)
+    # runs that cross short, long and missing sequences
+    check_attend(cuda_dev, [(1 + (97 * b) % 701) * (b % 11 != 5) for b in range(70)], 1, 16, 4, 2, 64, torch.bfloat16,
+                 weights=True)
+    check_attend(cuda_dev, [3 + (61 * b) % 400 for b in range(40)], 3, 20, 12, 2, 64, torch.float16, "head", weights=True)
 
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])

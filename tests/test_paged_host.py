@@ -42,6 +42,33 @@ def test_frequencies_refuse_what_they_do_not_know():
     assert rope_frequencies(0)[0].numel() == 0
 
 
+def test_decoders_take_scaled_rotary_tables():
+    """rope_table without scaling is HF's default table bit for bit; with it HF's scaled one, within the fp32
+    angles that HF computes (an ulp of the angle, and one fp16 rounding)."""
+    from transformers import LlamaConfig
+    from transformers.models.llama.modeling_llama import LlamaRotaryEmbedding
+
+    from otf_llm.decode_model import ModelConfig, rope_table
+    base = dict(layers=1, hidden=256, intermediate=256, heads=2, kv_heads=2, head_dim=128, vocab=10, rope_theta=500000.0,
+                max_pos=300)
+    scalings = [None, {"rope_type": "linear", "factor": 4.0},
+                {"rope_type": "llama3", "factor": 32.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+                 "original_max_position_embeddings": 8192},
+                {"rope_type": "yarn", "factor": 16.0, "original_max_position_embeddings": 4096}]
+    for scaling in scalings:
+        hf = LlamaConfig(hidden_size=256, num_attention_heads=2, head_dim=128, max_position_embeddings=131072,
+                         rope_parameters=dict(scaling or {"rope_type": "default"}, rope_theta=500000.0))
+        x = torch.zeros(1, 300, 256, dtype=torch.float32)
+        cos, sin = LlamaRotaryEmbedding(hf)(x, torch.arange(300)[None])
+        got = rope_table(ModelConfig(**base, rope_scaling=scaling), "cpu")
+        want = torch.stack((cos[0], sin[0]), dim=1)
+        if scaling is None:
+            assert torch.equal(got, want.half())
+        # frequencies of HF within 2e-5 of ours, angles below 300: 6e-3 at most
+        assert float((got.float() - want).abs().max()) <= 6.5e-3
+    assert torch.equal(rope_table(ModelConfig(**base), "cpu"), rope_table(ModelConfig(**base, rope_scaling=None), "cpu"))
+
+
 def test_no_cpu_cache():
     from otf_llm.paged import PagedKVCache
     from otf_llm.speculative import verify_drafts
