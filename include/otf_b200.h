@@ -452,7 +452,7 @@ OTF_API int otf_attn_decode_noalloc(const void* q, const void* k_cache, const vo
  * [head, token, dim].  lengths[b] counts the tokens cached before a call; a negative length
  * marks a place of the batch without a sequence, which every call leaves as it is.
  * dtype: OTF_DTYPE_F16 or OTF_DTYPE_BF16 (queries and outputs have the cache's type).
- * head_dim 64 or 128; at most 4096 sequences; max_pages * page_size below 2^31.
+ * head_dim 64 or 128; at most 4096 sequences; max_pages * page_size at most 2^30.
  * A sequence whose tokens do not fit in max_pages pages, or (in otf_paged_append and
  * otf_paged_evict) a token whose page is not in [0, n_pages), is left out: nothing of it is
  * written and the otf_device_error flag is raised.  In otf_paged_attn tokens of such a page
@@ -526,7 +526,8 @@ OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* q, int64_t 
  * The order stays.  kept: int32 [batch, kv_heads, budget], the places kept, then -1.  The kept
  * keys and values go to the same head's tokens 0, 1, ... of `to`, whose page_table holds pages
  * that hold nothing of `from` (in the same pools or others); or from's pools, table, weights and
- * lengths are given again, and the cache is cut in place.  `to` has from's geometry
+ * lengths are given again, and the cache is cut in place (its pages then belong to one sequence
+ * each).  `to` has from's geometry
  * (kv_heads, head_dim, batch, dtype, page_size) and room for budget tokens.  weights (fp32
  * [batch, kv_heads, ldw]) go along to weights_out ([batch, kv_heads, ldw_out], may be weights),
  * zero behind the kept ones (in place: up to the old length).  lengths_out[b] = min(lengths[b],

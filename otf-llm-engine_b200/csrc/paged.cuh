@@ -3,6 +3,8 @@
 
 #include <cuda_bf16.h>
 
+#include <atomic>
+
 #include "otf_common.cuh"
 
 namespace otf {
@@ -46,6 +48,17 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
             : __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
 
+// Whether a kernel's attributes still have to be set on the current device (done: per kernel, per device;
+// setting them twice does no harm).
+inline cudaError_t needs_opt_in(std::atomic<bool> (&done)[64], int& dev, bool& needs) {
+  const cudaError_t e = cudaGetDevice(&dev);
+  needs = e == cudaSuccess && (dev < 0 || dev >= 64 || !done[dev].load(std::memory_order_acquire));
+  return e;
+}
+inline void opted_in(std::atomic<bool> (&done)[64], int dev) {
+  if (dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_release);
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // The view of a cache, or why there is none.
@@ -56,7 +69,7 @@ inline int view_of(const otf_paged_cache* c, PagedView& v) {
   if (c->batch <= 0 || c->kv_heads <= 0 || c->page_size <= 0 || c->max_pages <= 0 || c->n_pages <= 0)
     return OTF_ERR_INVALID;
   if (c->batch > kPagedMaxBatch || c->kv_heads > 1024 || c->n_pages > INT32_MAX || c->page_size > INT32_MAX ||
-      c->max_pages > INT32_MAX || c->max_pages * c->page_size > INT32_MAX)
+      c->max_pages > INT32_MAX || c->max_pages * c->page_size > (1ll << 30))
     return OTF_ERR_UNSUPPORTED;
   if (c->ld_table < c->max_pages) return OTF_ERR_INVALID;
   if (!aligned16(c->k_pages) || !aligned16(c->v_pages) || c->page_stride % 8 || c->token_stride % 8 ||

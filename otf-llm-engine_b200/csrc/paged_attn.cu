@@ -24,9 +24,6 @@
 // plain arithmetic, so that the loop needs no causal mask and a row cannot be reached by what
 // later tokens hold.
 #include <algorithm>
-#include <map>
-#include <mutex>
-#include <utility>
 
 #include "paged.cuh"
 
@@ -211,7 +208,8 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
       }
       const int64_t first = base + inc - mine;
       if (u0 >= first && u0 < first + mine) {
-        const int at = (int)(u0 - first), per = n * a.chunk_units + a.item_units, item = at / per, x = at - item * per;
+        const int per = n * a.chunk_units + a.item_units, item = (int)((u0 - first) / per);
+        const int x = (int)(u0 - first - (int64_t)item * per);
         s_walk = a.chunk_units ? Walk{b, item, max(0, x - kPaItemUnits), n, u1 - u0 - max(0, kPaItemUnits - x)}
                                : Walk{b, item, 0, n, u1 - u0};
       }
@@ -796,32 +794,32 @@ static cudaError_t launch_join(const AttnArgs& a, int RB, cudaStream_t s) {
                     s, 1u, a, RB);
 }
 
+template <bool BF, int D, int MT, bool ALIGNED>
+static cudaError_t launch_attn_kernel(const AttnArgs& a, size_t dyn, cudaStream_t s) {
+  auto* k = k_paged_attn<BF, D, MT, ALIGNED>;
+  static std::atomic<bool> done[64];  // the shared-memory opt-in, for the largest batch
+  int dev;
+  bool needs;
+  cudaError_t e = needs_opt_in(done, dev, needs);
+  if (e != cudaSuccess) return e;
+  if (needs) {
+    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kPaWarps * kPaStages * kPaStage + kPaWarps * 16 * 12 + 32 * D * 2 +
+                                 (kPagedMaxTokens - 1) * 4 * D + kPagedMaxBatch * 4);
+    if (e != cudaSuccess) return e;
+    opted_in(done, dev);
+  }
+  return launch_pdl(k, dim3(kPaGrid), dim3(kPaThreads), dyn, s, 1u, a);
+}
+
 template <bool BF, int D>
 static cudaError_t launch_attn(const AttnArgs& a, float* weights, int64_t ldw, cudaStream_t s) {
   const int RB = a.rows <= 16 ? 16 : 32;
-  const bool aligned = a.c.page_size % 16 == 0;
-  auto* k = RB == 16 ? (aligned ? k_paged_attn<BF, D, 1, true> : k_paged_attn<BF, D, 1, false>)
-                     : (aligned ? k_paged_attn<BF, D, 2, true> : k_paged_attn<BF, D, 2, false>);
   const size_t dyn = (size_t)kPaWarps * kPaStages * kPaStage + (size_t)kPaWarps * 16 * 12 + (RB > 16 ? RB * D * 2 : 0) +
                      (size_t)(a.tokens - 1) * 4 * D + (size_t)a.c.batch * 4;
-  {
-    // the shared-memory opt-in, once per kernel and device, for the largest batch
-    static std::mutex mu;
-    static std::map<std::pair<const void*, int>, bool> done;
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    std::lock_guard<std::mutex> lock(mu);
-    bool& have = done[std::make_pair(reinterpret_cast<const void*>(k), dev)];
-    if (!have) {
-      e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               kPaWarps * kPaStages * kPaStage + kPaWarps * 16 * 12 + 32 * D * 2 + (kPagedMaxTokens - 1) * 4 * D +
-                                   kPagedMaxBatch * 4);
-      if (e != cudaSuccess) return e;
-      have = true;
-    }
-  }
-  cudaError_t e = launch_pdl(k, dim3(kPaGrid), dim3(kPaThreads), dyn, s, 1u, a);
+  const bool aligned = a.c.page_size % 16 == 0;
+  cudaError_t e = RB == 16 ? (aligned ? launch_attn_kernel<BF, D, 1, true>(a, dyn, s) : launch_attn_kernel<BF, D, 1, false>(a, dyn, s))
+                           : (aligned ? launch_attn_kernel<BF, D, 2, true>(a, dyn, s) : launch_attn_kernel<BF, D, 2, false>(a, dyn, s));
   if (e != cudaSuccess) return e;
   if (a.chunk_units) e = launch_join<BF, D>(a, RB, s);
   if (e != cudaSuccess || !weights) return e;

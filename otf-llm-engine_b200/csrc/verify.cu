@@ -17,9 +17,8 @@
 // fill the GPU in every step whatever the sequences' drafts are: k_verify_rows, k_verify_pick,
 // k_verify_race.  What a step computes is shared, and so is the order of its sums within a row.
 #include <algorithm>
-#include <mutex>
 
-#include "otf_common.cuh"
+#include "paged.cuh"
 
 namespace otf {
 
@@ -561,19 +560,15 @@ extern "C" OTF_API int otf_verify_drafts(const float* target, int64_t target_seq
   a.drafts = (int)drafts;
   a.vocab = (int)vocab;
   if (bytes == 0) {
-    {
-      // clusters of 16 are beyond the portable size: allowed once per device
-      static std::mutex mu;
-      static bool done[64] = {};
-      int dev = 0;
-      cudaError_t e = cudaGetDevice(&dev);
+    static std::atomic<bool> done[64];  // clusters of 16 are beyond the portable size
+    int dev;
+    bool needs;
+    cudaError_t e = otf::needs_opt_in(done, dev, needs);
+    if (e != cudaSuccess) return set_cuda_error(e);
+    if (needs) {
+      e = cudaFuncSetAttribute(otf::k_verify, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
       if (e != cudaSuccess) return set_cuda_error(e);
-      std::lock_guard<std::mutex> lock(mu);
-      if (dev < 0 || dev >= 64 || !done[dev]) {
-        e = cudaFuncSetAttribute(otf::k_verify, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return set_cuda_error(e);
-        if (dev >= 0 && dev < 64) done[dev] = true;
-      }
+      otf::opted_in(done, dev);
     }
     // CTAs per sequence: 16 (of such clusters 14 run at once), 8, or as many as all run at once, three
     // on an SM; no more than the vocabulary has segments

@@ -74,6 +74,8 @@ def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling: Optional[dic
     def place(turns: float) -> float:                       # the pair that turns so often over the context
         return rot_dim * math.log(context / (turns * 2 * math.pi)) / (2 * math.log(theta))
 
+    if not theta > 1 or not context > 0:
+        raise ValueError("yarn needs a theta above 1 and a positive original_max_position_embeddings")
     low = max(math.floor(place(float(scaling.get("beta_fast") or 32.0))), 0)
     high = min(math.ceil(place(float(scaling.get("beta_slow") or 1.0))), rot_dim - 1)
     ramp = ((i / 2 - low) / ((high - low) if high != low else 0.001)).clamp(0, 1)
@@ -107,8 +109,8 @@ class PagedKVCache:
     and unit inner stride (a transposed view of [n_pages, kv_heads, page_size, head_dim] will do);
     page_table: int32 [batch, max_pages], whose row b names the pages of sequence b in order;
     lengths: int32 [batch], the tokens that each sequence has cached, negative for a place
-    without a sequence (left as it is by every call).  The tensors stay the caller's: pages are
-    handed out by writing the table, and ``advance`` counts a step's tokens once every layer has
+    without a sequence (left as it is by every call).  The tensors stay the caller's and are
+    changed in place: pages are handed out by writing the table, and ``advance`` counts a step's tokens once every layer has
     appended them (layers may share table and lengths).
 
     Sequences that do not fit, and pages outside the pool, are left out on the device and raise
@@ -138,7 +140,7 @@ class PagedKVCache:
             raise ValueError("page_table must be a row-major [batch, max_pages] tensor")
         if lengths.shape != page_table.shape[:1] or lengths.shape[0] == 0 or not lengths.is_contiguous():
             raise ValueError(f"lengths must be a contiguous [{page_table.shape[0]}] vector")
-        self.k_pages, self.v_pages, self.page_table, self.lengths = k_pages, v_pages, page_table, lengths
+        self._k_pages, self._v_pages, self._page_table, self._lengths = k_pages, v_pages, page_table, lengths
         self.device, self.dtype = k_pages.device, k_pages.dtype
         self.page_size, self.kv_heads, self.head_dim = page, heads, dim
         self.batch, self.max_pages = page_table.shape
@@ -157,6 +159,23 @@ class PagedKVCache:
         # loop's calls differ in addresses alone
         self._append_plans: dict = {}
         self._attend_plans: dict = {}
+
+    # the tensors are changed in place, never replaced: the native side holds their addresses
+    @property
+    def k_pages(self) -> torch.Tensor:
+        return self._k_pages
+
+    @property
+    def v_pages(self) -> torch.Tensor:
+        return self._v_pages
+
+    @property
+    def page_table(self) -> torch.Tensor:
+        return self._page_table
+
+    @property
+    def lengths(self) -> torch.Tensor:
+        return self._lengths
 
     @classmethod
     def allocate(cls, n_pages: int, page_size: int, kv_heads: int, head_dim: int, page_table: torch.Tensor,
@@ -312,8 +331,8 @@ class PagedKVCache:
         by itself: the ``recent`` last tokens stay, and of the others those of the largest
         ``weights`` (as ``attend`` adds them up; ties: the earlier token), in their order.
 
-        In place by default: pages, ``weights`` and ``lengths`` of this cache are cut, and a
-        sequence's pages behind its first budget / page_size (rounded up) may be handed on.  With
+        In place by default: pages (of one sequence each), ``weights`` and ``lengths`` of this cache are
+        cut, and a sequence's pages behind its first budget / page_size (rounded up) may be handed on.  With
         ``to``, a cache of the same geometry whose table names other pages, the kept tokens go there
         (its ``lengths`` are set, and ``weights_out``, fp32 [batch, kv_heads, at least budget], is
         written), and this one stays as it is.  Returns int32 [batch, kv_heads, budget]: the

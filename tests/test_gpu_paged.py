@@ -291,6 +291,94 @@ def test_attend_reads_bad_pages_as_zeros_and_raises_the_flag(cuda_dev):
     assert bool((out[0] == 7.0).all()) and not bool((out[1] == 7.0).any())
 
 
+def test_attend_without_any_sequence(cuda_dev):
+    cache, pools, table, g = make(cuda_dev, [-1, -5, -1], 16, 2, 64, torch.float16, room=[300, 16, 16])
+    q = torch.randn(3, 4, 64, generator=g).half().to(cuda_dev)
+    out, w = torch.full_like(q, 7.0), torch.zeros(3, 2, cache.capacity, device=cuda_dev)
+    cache.attend(q, out=out, weights=w)
+    cache.append(q, q[:, :2], q[:, :2], q_out=out)
+    assert flag() == 0 and bool((out == 7.0).all()) and not bool(w.any())
+
+
+def test_refusals_of_the_python_surface(cuda_dev):
+    from otf_llm.paged import PagedKVCache, Rotary
+    cache, pools, table, g = make(cuda_dev, [20, 30], 16, 2, 64, torch.float16)
+    q = torch.zeros(2, 4, 64, dtype=torch.float16, device=cuda_dev)
+    kv = q[:, :2]
+    w = torch.zeros(2, 2, cache.capacity, device=cuda_dev)
+    bad = [lambda: cache.attend(q.bfloat16()), lambda: cache.attend(q.cpu()), lambda: cache.attend(q[:1]),
+           lambda: cache.attend(q[:, :3]), lambda: cache.attend(q[..., :32]), lambda: cache.attend(q.transpose(0, 1)),
+           lambda: cache.attend(q.new_zeros(2, 17, 4, 64)), lambda: cache.attend(q, out=q),
+           lambda: cache.attend(q, out=q.new_zeros(2, 8, 64)), lambda: cache.attend(q, weights=w[..., :-1]),
+           lambda: cache.attend(q, weights=w.half()), lambda: cache.attend(q.new_zeros(4, 4, 64)[::2][:, ::2]),
+           lambda: cache.append(q, kv, kv[:1]), lambda: cache.append(q[:1], kv, kv), lambda: cache.append(q, q, kv),
+           lambda: cache.append(q, kv[:1], kv[:1]), lambda: cache.append(None, kv[:1], kv[:1]),
+           lambda: cache.append(None, kv, kv, q_out=q), lambda: cache.append(q, kv, kv, Rotary(128, device=cuda_dev)),
+           lambda: cache.append(q, kv, kv, Rotary(64, device="cpu")),
+           lambda: cache.append(q, kv, kv, starts=torch.zeros(3, dtype=torch.int64, device=cuda_dev)),
+           lambda: cache.append(q, kv, kv, starts=torch.zeros(2, dtype=torch.int32, device=cuda_dev)),
+           lambda: cache.append(q, kv, kv, positions=torch.zeros(3, dtype=torch.int32, device=cuda_dev)),
+           lambda: cache.evict(w, 0, 0), lambda: cache.evict(w, 8, 9), lambda: cache.evict(w, cache.capacity + 1, 0),
+           lambda: cache.evict(w[..., :-1].contiguous(), 8, 2), lambda: cache.evict(w, 8, 2, weights_out=w.clone()),
+           lambda: cache.evict(w, 8, 2, to=cache, weights_out=w.clone()), lambda: cache.evict(w, 8, 2, to=cache),
+           lambda: Rotary(64, rot_dim=66), lambda: Rotary(64, rot_dim=7),
+           lambda: PagedKVCache(cache.k_pages, cache.v_pages, cache.page_table.long(), cache.lengths),
+           lambda: PagedKVCache(cache.k_pages, cache.v_pages, cache.page_table, cache.lengths[:1]),
+           lambda: PagedKVCache(cache.k_pages, cache.v_pages[:, :8], cache.page_table, cache.lengths),
+           lambda: PagedKVCache(cache.k_pages.float(), cache.v_pages.float(), cache.page_table, cache.lengths),
+           lambda: PagedKVCache(cache.k_pages[..., :32], cache.v_pages[..., :32], cache.page_table, cache.lengths)]
+    for i, call in enumerate(bad):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            call()
+            pytest.fail(f"refusal {i}")
+    with pytest.raises(AttributeError):
+        cache.lengths = cache.lengths + 1
+    assert flag() == 0
+
+
+FIRST_IN_CAPTURE = """
+import torch
+from otf_llm.paged import PagedKVCache, Rotary
+from otf_llm.speculative import verify_drafts
+dev = torch.device("cuda:0")
+table = torch.arange(80, dtype=torch.int32, device=dev).view(2, 40)
+cache = PagedKVCache.allocate(80, 16, 2, 64, table, torch.zeros(2, dtype=torch.int32, device=dev))
+rotary = Rotary(64, device=dev)
+q = torch.randn(2, 4, 64, device=dev).half()
+w = torch.zeros(2, 2, cache.capacity, device=dev)
+logits = torch.randn(2, 3, 500, device=dev)
+tokens = logits[:, :2].argmax(2)
+uniforms, noise = torch.rand(2, 2, device=dev), torch.empty(2, 500, device=dev).exponential_()
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    t = cache.append(q, q[:, :2], q[:, 2:], rotary)
+    out = cache.attend(t, weights=w)
+    cache.advance()
+    cache.evict(w, 8, 2)
+    got = verify_drafts(logits, tokens, uniforms=uniforms, noise=noise)
+for _ in range(12):
+    g.replay()
+torch.cuda.synchronize()
+assert cache.lengths.tolist() == [8, 8] and torch.isfinite(out).all()
+assert torch.allclose(out[:, :2], q[:, 2:3].expand(2, 2, 64), atol=1e-2)      # one value in every place
+want = verify_drafts(logits, tokens, uniforms=uniforms, noise=noise)
+assert all(torch.equal(a, b) for a, b in zip(got, want))
+print("captured")
+"""
+
+
+def test_first_call_of_a_process_may_be_captured(cuda_dev):
+    import os
+    import subprocess
+    import sys
+
+    from conftest import PKG
+    env = dict(os.environ, PYTHONPATH=PKG + os.pathsep + os.environ.get("PYTHONPATH", ""))
+    r = subprocess.run([sys.executable, "-c", FIRST_IN_CAPTURE], env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
 def test_attend_strided_queries_and_outputs(cuda_dev):
     cache, pools, table, g = make(cuda_dev, [33, 50], 16, 2, 64, torch.float16)
     cache.lengths.sub_(3)
