@@ -20,10 +20,10 @@
 // across items, and runs q k and p v on m16n8k16 matrix instructions, the row block's queries
 // held in registers.  The warps meet only at an item's end.
 //
-// The tokens - 1 newest keys, which not every row sees, are added row by row at the item's end on
-// plain arithmetic, so that the loop needs no causal mask and a row cannot be reached by what
-// later tokens hold.
+// The newest keys, which not every row sees, are masked in the steps that hold them; what they hold
+// cannot reach the other rows (see the loop).
 #include <algorithm>
+#include <cmath>
 
 #include "paged.cuh"
 
@@ -96,6 +96,24 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t& r0, u
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr) : "memory");
 }
+__device__ __forceinline__ void lds128(uint32_t addr, uint32_t (&v)[4]) {
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint16_t lds16(uint32_t addr) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts128_zero(uint32_t addr) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(addr), "r"(0) : "memory");
+}
+// The transposed 8 x 8 matrix of 16-bit values, a row in the lanes 4 i .. 4 i + 3.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
 // PL consecutive values of a row to fp32, and back.
 template <bool BF, int PL>
 __device__ __forceinline__ void load_row(const uint16_t* x, float (&v)[PL]) {
@@ -144,27 +162,29 @@ struct Tile {
   static constexpr int rows = 32 / pieces;          // rows that a warp's copy instruction covers
 };
 
+// `end`: a sequence's tokens, the new ones among them; 0 for a place without one.
 template <int D>
-__device__ __forceinline__ int chunks_of(int len) {
-  return (len + 1 + Tile<D>::chunk - 1) / Tile<D>::chunk;  // none when len is -1
+__device__ __forceinline__ int chunks_of(int end) {
+  return (end + Tile<D>::chunk - 1) / Tile<D>::chunk;
 }
 template <int D>
-__device__ __forceinline__ int64_t units_of(const AttnArgs& a, int len, int items) {
-  return len < 0 ? 0 : (int64_t)(chunks_of<D>(len) * a.chunk_units + a.item_units) * items;
+__device__ __forceinline__ int64_t units_of(const AttnArgs& a, int end, int items) {
+  return end == 0 ? 0 : (int64_t)(chunks_of<D>(end) * a.chunk_units + a.item_units) * items;
 }
 
 // ALIGNED: a page holds a multiple of 16 tokens, so that 16 neighbours from a multiple of 16 on lie
 // in one page and one look-up serves them; otherwise every lane looks up its own token.
-template <bool BF, int D, int MT, bool ALIGNED>
+// NT: the block's rows in eights.
+template <bool BF, int D, int NT, bool ALIGNED>
 __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
-  constexpr int KT = Tile<D>::keys, CH = Tile<D>::chunk, NS = kPaStages, RB = 16 * MT, G = Tile<D>::groups;
+  constexpr int KT = Tile<D>::keys, CH = Tile<D>::chunk, NS = kPaStages, RB = 8 * NT, G = Tile<D>::groups;
+  constexpr bool QS = NT > 3;  // queries in shared memory: the outputs take the registers
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char* s_q = smem + kPaWarps * NS * kPaStage;  // [RB][D] when it does not fit the registers
-  float* s_m = reinterpret_cast<float*>(s_q + (MT > 1 ? RB * D * 2 : 0));
+  float* s_m = reinterpret_cast<float*>(s_q + (QS ? RB * D * 2 : 0));
   float* s_l = s_m + kPaWarps * 16;
   float* s_exact = s_l + kPaWarps * 16;
-  uint16_t* s_tail = reinterpret_cast<uint16_t*>(s_exact + kPaWarps * 16);  // [tokens - 1][keys, values][D]
-  int* s_len = reinterpret_cast<int*>(s_tail + (a.tokens - 1) * 2 * D);
+  int* s_end = reinterpret_cast<int*>(s_exact + kPaWarps * 16);
   __shared__ int64_t s_sum[kPaWarps];
   __shared__ Walk s_walk;
   pdl_trigger();
@@ -176,13 +196,14 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
   // the lengths, and this CTA's run of units [u0, u1)
   int64_t sum = 0;
   for (int b = tid; b < c.batch; b += kPaThreads) {
-    int len = max(c.lengths[b], -1);
-    if ((int64_t)len + a.tokens > c.capacity) {
-      if (blockIdx.x == 0) report_bad_attn_page();
-      len = -1;
+    const int len = c.lengths[b];
+    int end = 0;
+    if (len >= 0) {
+      if ((int64_t)len + a.tokens <= c.capacity) end = len + a.tokens;
+      else if (blockIdx.x == 0) report_bad_attn_page();
     }
-    s_len[b] = len;
-    sum += units_of<D>(a, len, items);
+    s_end[b] = end;
+    sum += units_of<D>(a, end, items);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -198,8 +219,8 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
     int64_t base = 0;
     for (int b0 = 0; b0 < c.batch; b0 += 32) {
       const int b = b0 + lane;
-      const int n = b < c.batch ? chunks_of<D>(s_len[b]) : 0;
-      const int64_t mine = b < c.batch ? units_of<D>(a, s_len[b], items) : 0;
+      const int n = b < c.batch ? chunks_of<D>(s_end[b]) : 0;
+      const int64_t mine = b < c.batch ? units_of<D>(a, s_end[b], items) : 0;
       int64_t inc = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -231,8 +252,8 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
     if (++w.item < items || w.left <= 0) return;
     w.item = 0;
     do ++w.b;
-    while (w.b < c.batch && s_len[w.b] < 0);
-    if (w.b < c.batch) w.chunks = chunks_of<D>(s_len[w.b]);
+    while (w.b < c.batch && s_end[w.b] == 0);
+    if (w.b < c.batch) w.chunks = chunks_of<D>(s_end[w.b]);
   };
 
   // Offsets in the pools of the walk's chunk for this warp: of each group of 16 tokens (ALIGNED), or
@@ -246,7 +267,7 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
     for (int g = 0; g < (ALIGNED ? G : 1); ++g) {
       const int key = w.chunk * CH + warp * KT + (ALIGNED ? g * 16 : lane);
       p.at[g] = -1;
-      if (w.left > 0 && (ALIGNED || lane < KT) && key <= s_len[w.b]) {
+      if (w.left > 0 && (ALIGNED || lane < KT) && key < s_end[w.b]) {
         const uint32_t in = (uint32_t)key / a.page;
         const int page = c.table[w.b * c.ld_table + in];
         if (page >= 0 && page < c.n_pages)
@@ -263,7 +284,7 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
   auto fetch = [&](const Walk& w, const Places& p, int slot) {
     const int64_t head = (int64_t)(w.item / a.blocks) * c.head_stride;
     const uint32_t dst = ring + slot * kPaStage;
-    const int there = s_len[w.b] + 1 - (w.chunk * CH + warp * KT);  // tokens of the tile that there are
+    const int there = s_end[w.b] - (w.chunk * CH + warp * KT);  // tokens of the tile that there are
 #pragma unroll
     for (int i = 0; i < KT / Tile<D>::rows; ++i) {
       const int r = i * Tile<D>::rows + my_row;
@@ -297,38 +318,41 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
     cp_async_commit();
   }
 
-  uint32_t qf[D / 16][4];
-  float o[MT][D / 8][4], m[MT][2], l[MT][4], exact[MT][2];
-  // a column of ones beside the values: l is the sum of the probabilities as they were rounded, so that a
+  // Everything is transposed, so that the few rows are the narrow side of the matrix instruction: the
+  // products are keys x rows (16 x 8), the outputs dims x rows, both m16n8k16; the probabilities
+  // change sides by an 8 x 8 transposition.  Lane l holds rows 2 (l % 4) and the next of each eight.
+  uint32_t qf[QS ? 1 : D / 16][NT][2];
+  float o[D / 16][NT][4], m[NT][2], l[NT][4], exact[NT][2];
+  // a row of ones beside the values: l is the sum of the probabilities as they were rounded, so that a
   // rounding common to both cancels (one key with all the weight comes out exactly); `exact` sums them
   // unrounded, for the weights
-  const uint32_t ones = BF ? 0x3F803F80u : 0x3C003C00u;
+  const uint32_t one2 = BF ? 0x3F803F80u : 0x3C003C00u;
+  const uint32_t ones[4] = {one2, one2, one2, one2};
   const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;  // on q, so that a larger product weighs more
-  const float scale = fabsf(a.scale);
+  const float scale = fmaxf(fabsf(a.scale), 1e-30f);  // a masked -inf stays one under a scale of 0
   const int lrow = lane & 7, lmat = lane >> 3;
-  const uint32_t k_lane = ((lmat >> 1) * 8 + lrow) * (D * 2) + (((lmat & 1) ^ lrow) << 4);
-  const uint32_t v_lane = ((lmat & 1) * 8 + lrow) * (D * 2) + (((lmat >> 1) ^ lrow) << 4);
-  const uint32_t q_lane = smem_u32(s_q) + v_lane;  // a query's fragment has the values' order of matrices
+  // a 16 x 16 tile's four 8 x 8 matrices, rows first and columns first
+  const uint32_t rows_first = ((lmat & 1) * 8 + lrow) * (D * 2) + (((lmat >> 1) ^ lrow) << 4);
+  const uint32_t cols_first = ((lmat >> 1) * 8 + lrow) * (D * 2) + (((lmat & 1) ^ lrow) << 4);
+  const uint32_t q_lane = smem_u32(s_q) + cols_first;
   int parts = 0, began = get.chunk, slot = 0;
   bool fresh = true;
   while (get.left > 0) {
     const int g = get.item / a.blocks, rb = get.item - g * a.blocks;
-    const int len = s_len[get.b];
+    const int end = s_end[get.b], len = end - a.tokens;  // row t sees the keys 0 .. len + t
     if (fresh) {
       fresh = false;
-      // the row block's queries: matrix fragments in registers, or (two matrices high, where the
-      // outputs take the registers) rows in shared memory for ldmatrix
-      if (MT == 1) {
+      // the row block's queries: matrix fragments in registers, or rows in shared memory for ldmatrix
+      if (!QS) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = rb * RB + h * 8 + (lane >> 2);
-          const int tok = r / a.rep;
+        for (int n = 0; n < NT; ++n) {
+          const int r = rb * RB + n * 8 + (lane >> 2), tok = r / a.rep;
           const uint32_t* x = reinterpret_cast<const uint32_t*>(a.q + ((int64_t)get.b * a.tokens + tok) * a.ldq +
                                                                 (int64_t)(g * a.rep + r - tok * a.rep) * D) + (lane & 3);
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            qf[k][h] = r < a.rows ? x[k * 8] ^ sign : 0u;
-            qf[k][h + 2] = r < a.rows ? x[k * 8 + 4] ^ sign : 0u;
+          for (int k = 0; k < (QS ? 1 : D / 16); ++k) {
+            qf[k][n][0] = r < a.rows ? x[k * 8] ^ sign : 0u;
+            qf[k][n][1] = r < a.rows ? x[k * 8 + 4] ^ sign : 0u;
           }
         }
       } else {
@@ -345,13 +369,13 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
         __syncthreads();
       }
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        m[t][0] = m[t][1] = -INFINITY;
-        l[t][0] = l[t][1] = l[t][2] = l[t][3] = exact[t][0] = exact[t][1] = 0.0f;
+      for (int n = 0; n < NT; ++n) {
+        m[n][0] = m[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = l[n][2] = l[n][3] = exact[n][0] = exact[n][1] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j)
+        for (int j = 0; j < D / 16; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[t][j][i] = 0.0f;
+          for (int i = 0; i < 4; ++i) o[j][n][i] = 0.0f;
       }
     }
     cp_async_wait<NS - 2>();
@@ -364,131 +388,183 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
     }
     cp_async_commit();
     const int key0 = get.chunk * CH + warp * KT;
-    if (key0 <= len) {
-      const uint32_t kb = ring + slot * kPaStage + k_lane, vb = ring + slot * kPaStage + KT * D * 2 + v_lane;
-      float s[MT][KT / 8][4];
+    if (key0 < end) {
+      const uint32_t kb = ring + slot * kPaStage + rows_first, vb = ring + slot * kPaStage + KT * D * 2 + cols_first;
+      float s[KT / 16][NT][4];  // 16 keys x 8 rows: keys lane / 4 and 8 on, two rows each
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+      for (int h = 0; h < KT / 16; ++h)
 #pragma unroll
-        for (int n = 0; n < KT / 8; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[t][n][i] = 0.0f;
+          for (int i = 0; i < 4; ++i) s[h][n][i] = 0.0f;
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
-        uint32_t qk[MT][4];
+        uint32_t qk[NT][2];
+        if (QS) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
-          if (MT == 1)
+          for (int n = 0; n + 1 < NT; n += 2)
+            ldmatrix_x4((q_lane ^ (k << 5)) + n * 8 * D * 2, qk[n][0], qk[n][1], qk[n + 1][0], qk[n + 1][1]);
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) qk[t][i] = qf[k][i];
-          else
-            ldmatrix_x4((q_lane ^ (k << 5)) + t * 16 * D * 2, qk[t][0], qk[t][1], qk[t][2], qk[t][3]);
-#pragma unroll
-        for (int n = 0; n < KT / 16; ++n) {
-          uint32_t b0, b1, b2, b3;
-          ldmatrix_x4((kb ^ (k << 5)) + n * 16 * D * 2, b0, b1, b2, b3);
-#pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            mma16816<BF>(s[t][2 * n], qk[t], b0, b1);
-            mma16816<BF>(s[t][2 * n + 1], qk[t], b2, b3);
+          for (int n = 0; n < NT; ++n) {
+            qk[n][0] = qf[QS ? 0 : k][n][0];
+            qk[n][1] = qf[QS ? 0 : k][n][1];
           }
         }
+#pragma unroll
+        for (int h = 0; h < KT / 16; ++h) {
+          uint32_t ka[4];
+          ldmatrix_x4((kb ^ (k << 5)) + h * 16 * D * 2, ka[0], ka[1], ka[2], ka[3]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816<BF>(s[h][n], ka, qk[n][0], qk[n][1]);
+        }
       }
-      if (key0 + KT > len + 1) {
+      const bool edge = key0 + KT > len + 1;  // not every row sees every key
+      if (edge) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int n = 0; n < KT / 8; ++n)
+          for (int i = 0; i < 2; ++i) {
+            const int seen = len + (rb * RB + n * 8 + (lane & 3) * 2 + i) / a.rep;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (key0 + n * 8 + (lane & 3) * 2 + (i & 1) > len) s[t][n][i] = -INFINITY;
+            for (int h = 0; h < KT / 16; ++h) {
+              if (key0 + h * 16 + (lane >> 2) > seen) s[h][n][i] = -INFINITY;
+              if (key0 + h * 16 + (lane >> 2) + 8 > seen) s[h][n][i + 2] = -INFINITY;
+            }
+          }
       }
       if (a.scores) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
+        for (int n = 0; n < NT; ++n) {
+          const int r = rb * RB + n * 8 + (lane & 3) * 2;
+          float* to = a.scores + (((int64_t)get.b * c.kv_heads + g) * a.rows + r) * a.ld_scores + key0 + (lane >> 2);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int r = rb * RB + t * 16 + h * 8 + (lane >> 2);
-            if (r < a.rows) {
-              float* to = a.scores + (((int64_t)get.b * c.kv_heads + g) * a.rows + r) * a.ld_scores + key0 + (lane & 3) * 2;
+          for (int h = 0; h < KT / 16; ++h)
 #pragma unroll
-              for (int n = 0; n < KT / 8; ++n)
-                if (key0 + n * 8 <= len)  // ld_scores covers whole groups of 8
-                  *reinterpret_cast<float2*>(to + n * 8) = make_float2(s[t][n][2 * h] * scale, s[t][n][2 * h + 1] * scale);
-            }
-          }
+            for (int i = 0; i < 4; ++i)
+              if (r + (i & 1) < a.rows && key0 + h * 16 + (i >> 1) * 8 + (lane >> 2) < end)
+                to[(i & 1) * a.ld_scores + h * 16 + (i >> 1) * 8] = s[h][n][i] * scale;
+        }
       }
-      uint32_t p[MT][KT / 16][4];
+      uint32_t p[KT / 16][NT][2];
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
+      for (int n = 0; n < NT; ++n) {
         // the exponents scale s - m + shift against the reference m; where one of them leaves the
         // headroom (or a row has no reference yet) m becomes the true maximum so far
-        float e[KT / 8][4], top[2] = {-INFINITY, -INFINITY};
+        float e[KT / 16][4];
         auto exponents = [&] {
-          const float z[2] = {kProbShift<BF> - (m[t][0] == -INFINITY ? 0.0f : m[t][0]),
-                              kProbShift<BF> - (m[t][1] == -INFINITY ? 0.0f : m[t][1])};
+          const float z[2] = {kProbShift<BF> - (m[n][0] == -INFINITY ? 0.0f : m[n][0]),
+                              kProbShift<BF> - (m[n][1] == -INFINITY ? 0.0f : m[n][1])};
 #pragma unroll
-          for (int n = 0; n < KT / 8; ++n)
+          for (int h = 0; h < KT / 16; ++h)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) e[n][i] = fmaf(s[t][n][i], scale, z[i >> 1]);
+            for (int i = 0; i < 4; ++i) e[h][i] = fmaf(s[h][n][i], scale, z[i & 1]);
         };
         exponents();
+        float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int n = 0; n < KT / 8; ++n) {
-          top[0] = fmaxf(top[0], fmaxf(e[n][0], e[n][1]));
-          top[1] = fmaxf(top[1], fmaxf(e[n][2], e[n][3]));
+        for (int h = 0; h < KT / 16; ++h) {
+          top[0] = fmaxf(top[0], fmaxf(e[h][0], e[h][2]));
+          top[1] = fmaxf(top[1], fmaxf(e[h][1], e[h][3]));
         }
-        const bool grow = top[0] > (m[t][0] == -INFINITY ? -INFINITY : kProbShift<BF> + kHeadroom) ||
-                          top[1] > (m[t][1] == -INFINITY ? -INFINITY : kProbShift<BF> + kHeadroom);
+        const bool grow = top[0] > (m[n][0] == -INFINITY ? -INFINITY : kProbShift<BF> + kHeadroom) ||
+                          top[1] > (m[n][1] == -INFINITY ? -INFINITY : kProbShift<BF> + kHeadroom);
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int i = 0; i < 2; ++i) {
             float mx = -INFINITY;
 #pragma unroll
-            for (int n = 0; n < KT / 8; ++n) mx = fmaxf(mx, fmaxf(s[t][n][2 * h], s[t][n][2 * h + 1]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            mx = fmaxf(mx * scale, m[t][h]);
-            const float f = m[t][h] == -INFINITY ? 0.0f : ex2(m[t][h] - mx);
-            l[t][2 * h] *= f;
-            l[t][2 * h + 1] *= f;
-            exact[t][h] *= f;
+            for (int h = 0; h < KT / 16; ++h) mx = fmaxf(mx, fmaxf(s[h][n][i], s[h][n][i + 2]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            mx = fmaxf(mx * scale, m[n][i]);
+            const float f = m[n][i] == -INFINITY ? 0.0f : ex2(m[n][i] - mx);
+            l[n][i] *= f;
+            l[n][i + 2] *= f;
+            exact[n][i] *= f;
 #pragma unroll
-            for (int j = 0; j < D / 8; ++j) {
-              o[t][j][2 * h] *= f;
-              o[t][j][2 * h + 1] *= f;
+            for (int j = 0; j < D / 16; ++j) {
+              o[j][n][i] *= f;
+              o[j][n][i + 2] *= f;
             }
-            m[t][h] = mx;
+            m[n][i] = mx;
           }
           exponents();
         }
 #pragma unroll
-        for (int n = 0; n < KT / 8; ++n) {
+        for (int h = 0; h < KT / 16; ++h) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) e[n][i] = ex2(e[n][i]);
-          p[t][n >> 1][(n & 1) * 2] = pack2<BF>(e[n][0], e[n][1]);
-          p[t][n >> 1][(n & 1) * 2 + 1] = pack2<BF>(e[n][2], e[n][3]);
-        }
-#pragma unroll
-        for (int n = 0; n < KT / 16; ++n) mma16816<BF>(l[t], p[t][n], ones, ones);
-        if (a.scores)
-#pragma unroll
-          for (int n = 0; n < KT / 8; ++n) {
-            exact[t][0] += e[n][0] + e[n][1];
-            exact[t][1] += e[n][2] + e[n][3];
+          for (int i = 0; i < 4; ++i) e[h][i] = ex2(e[h][i]);
+          if (a.scores) {
+            exact[n][0] += e[h][0] + e[h][2];
+            exact[n][1] += e[h][1] + e[h][3];
           }
+          p[h][n][0] = transpose8x8(pack2<BF>(e[h][0], e[h][1]));
+          p[h][n][1] = transpose8x8(pack2<BF>(e[h][2], e[h][3]));
+          mma16816<BF>(l[n], ones, p[h][n][0], p[h][n][1]);
+        }
+      }
+      if (edge && a.tokens > 1) {
+        // A weight of 0 does not keep an infinity or NaN among the newest values from the rows that do
+        // not see them: where there is one, its key's values are added row by row on plain arithmetic
+        // and taken out of the stage.
+        uint32_t bad = 0;
+        const uint32_t v0 = ring + slot * kPaStage + KT * D * 2;
+        const int first = max(0, len + 1 - key0), behind = min(KT, end - key0);
+        for (int r = first; r < behind; ++r) {
+          bool odd = false;
+          if (lane < D / 8) {
+            uint32_t x[4];
+            lds128(v0 + r * (D * 2) + (lane << 4), x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              constexpr uint32_t e = BF ? 0x7F80u : 0x7C00u;
+              odd |= (x[i] & e) == e || (x[i] & (e << 16)) == e << 16;
+            }
+          }
+          if (__any_sync(0xffffffffu, odd)) bad |= 1u << r;
+        }
+        for (; bad; bad &= bad - 1) {
+          const int r = __ffs((int)bad) - 1;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int w = (lane & 3) * 2 + i;  // its probability lies transposed, in lane 4 w + key / 2
+              uint32_t x = 0;
+#pragma unroll
+              for (int h = 0; h < KT / 16; ++h)
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                  const uint32_t y = __shfl_sync(0xffffffffu, p[h][n][z], w * 4 + ((r & 7) >> 1));
+                  if (r >> 3 == 2 * h + z) x = y;
+                }
+              const float2 two = unpack2<BF>(x);
+              const float pr = r & 1 ? two.y : two.x;
+              if (key0 + r <= len + (rb * RB + n * 8 + w) / a.rep)
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+                  for (int z = 0; z < 2; ++z) {
+                    const int d = j * 16 + z * 8 + (lane >> 2);
+                    const uint16_t v = lds16(v0 + r * (D * 2) + (((d >> 3) ^ (r & 7)) << 4) + (d & 7) * 2);
+                    o[j][n][i + 2 * z] = fmaf(pr, to_f<BF>(v), o[j][n][i + 2 * z]);
+                  }
+            }
+          __syncwarp();
+          if (lane < D / 8) sts128_zero(v0 + r * (D * 2) + (lane << 4));
+          __syncwarp();
+        }
       }
 #pragma unroll
       for (int j = 0; j < D / 16; ++j)
 #pragma unroll
-        for (int n = 0; n < KT / 16; ++n) {
-          uint32_t b0, b1, b2, b3;
-          ldmatrix_x4_trans((vb ^ (j << 5)) + n * 16 * D * 2, b0, b1, b2, b3);
+        for (int h = 0; h < KT / 16; ++h) {
+          uint32_t va[4];
+          ldmatrix_x4_trans((vb ^ (j << 5)) + h * 16 * D * 2, va[0], va[1], va[2], va[3]);
 #pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            mma16816<BF>(o[t][2 * j], p[t][n], b0, b1);
-            mma16816<BF>(o[t][2 * j + 1], p[t][n], b2, b3);
-          }
+          for (int n = 0; n < NT; ++n) mma16816<BF>(o[j][n], va, p[h][n][0], p[h][n][1]);
         }
     }
     const Walk now = get;
@@ -499,47 +575,37 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
       // of a block at once: 8 threads per row, each the 4 values from j * 32 + 4 * part on.
       const bool whole = last && began == 0;
       float* mine = reinterpret_cast<float*>(smem + warp * NS * kPaStage + slot * kPaStage);
-      if (last)  // the newest tokens
-        for (int e = tid; e < (a.tokens - 1) * 2 * (D / 8); e += kPaThreads) {
-          const int piece = e % (D / 8), side = e / (D / 8) & 1, i = e / (D / 4);
-          const int key = len + 1 + i;
-          const uint32_t at = (uint32_t)key / a.page;
-          const int page = c.table[now.b * c.ld_table + at];
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (page >= 0 && page < c.n_pages)
-            x = *reinterpret_cast<const uint4*>((side ? c.v : c.k) + page * c.page_stride +
-                                                (int64_t)(key - (int)(at * a.page.d)) * c.token_stride +
-                                                g * c.head_stride + piece * 8);
-          else
-            report_bad_attn_page();
-          *reinterpret_cast<uint4*>(s_tail + (i * 2 + side) * D + piece * 8) = x;
-        }
       const int r = tid >> 3, part = tid & 7;
+      auto turn = [](int row) { return ((row >> 1) & 3) << 3; };
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
+      for (int t = 0; t < (NT + 1) / 2; ++t) {
         const int rr = rb * RB + t * 16 + r;
+        const bool there = t * 16 + r < RB && rr < a.rows;
         const int tok = rr / a.rep, head = g * a.rep + rr - tok * a.rep;
         const int64_t row = (int64_t)now.b * a.tokens + tok;
-        float qv[D / 32][4];
-        if (last && a.tokens > 1 && rr < a.rows)
-#pragma unroll
-          for (int j = 0; j < D / 32; ++j) load_row<BF, 4>(a.q + row * a.ldq + (int64_t)head * D + j * 32 + part * 4, qv[j]);
         __syncwarp();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int w = h * 8 + (lane >> 2);
-          float x = exact[t][h];
-          x += __shfl_xor_sync(0xffffffffu, x, 1);
-          x += __shfl_xor_sync(0xffffffffu, x, 2);
-          if ((lane & 3) == 0) {
-            s_exact[warp * 16 + w] = x;
-            s_m[warp * 16 + w] = m[t][h];
-            s_l[warp * 16 + w] = l[t][2 * h];
-          }
+          const int n = 2 * t + h;
+          if (n < NT)
 #pragma unroll
-          for (int j = 0; j < D / 8; ++j)  // columns turned by the row, against bank conflicts
-            *reinterpret_cast<float2*>(mine + w * D + ((j * 8 + (lane & 3) * 2) ^ ((w & 3) << 3))) =
-                make_float2(o[t][j][2 * h], o[t][j][2 * h + 1]);
+            for (int i = 0; i < 2; ++i) {
+              const int w = h * 8 + (lane & 3) * 2 + i;
+              float x = exact[n < NT ? n : 0][i];
+              x += __shfl_xor_sync(0xffffffffu, x, 4);
+              x += __shfl_xor_sync(0xffffffffu, x, 8);
+              x += __shfl_xor_sync(0xffffffffu, x, 16);
+              if (lane < 4) {
+                s_exact[warp * 16 + w] = x;
+                s_m[warp * 16 + w] = m[n < NT ? n : 0][i];
+                s_l[warp * 16 + w] = l[n < NT ? n : 0][i];
+              }
+#pragma unroll
+              for (int j = 0; j < D / 16; ++j) {  // columns turned by the row, against bank conflicts
+                mine[w * D + ((j * 16 + (lane >> 2)) ^ turn(w))] = o[j][n < NT ? n : 0][i];
+                mine[w * D + ((j * 16 + 8 + (lane >> 2)) ^ turn(w))] = o[j][n < NT ? n : 0][i + 2];
+              }
+            }
         }
         __syncthreads();
         float M = -INFINITY, L = 0.0f, E = 0.0f, acc[D / 32][4];
@@ -559,7 +625,7 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
             E = fmaf(s_exact[w * 16 + r], f, E);
 #pragma unroll
             for (int j = 0; j < D / 32; ++j) {
-              const float4 y = *reinterpret_cast<const float4*>(x + ((j * 32 + part * 4) ^ ((r & 3) << 3)));
+              const float4 y = *reinterpret_cast<const float4*>(x + ((j * 32 + part * 4) ^ turn(r)));
               acc[j][0] = fmaf(y.x, f, acc[j][0]);
               acc[j][1] = fmaf(y.y, f, acc[j][1]);
               acc[j][2] = fmaf(y.z, f, acc[j][2]);
@@ -567,37 +633,7 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
             }
           }
         }
-        if (last && a.tokens > 1) {  // the newest tokens, as far as a row sees them
-          float* sc = a.scores && rr < a.rows && part == 0
-                          ? a.scores + (((int64_t)now.b * c.kv_heads + g) * a.rows + rr) * a.ld_scores + len + 1
-                          : nullptr;
-          for (int i = 0; i < a.tokens - 1; ++i) {
-            float d = 0.0f, vv[D / 32][4];
-#pragma unroll
-            for (int j = 0; j < D / 32; ++j) {
-              float kv[4];
-              load_row<BF, 4>(s_tail + i * 2 * D + j * 32 + part * 4, kv);
-              load_row<BF, 4>(s_tail + (i * 2 + 1) * D + j * 32 + part * 4, vv[j]);
-#pragma unroll
-              for (int z = 0; z < 4; ++z) d = fmaf(qv[j][z], kv[z], d);
-            }
-#pragma unroll
-            for (int x = 4; x > 0; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
-            d = i < tok ? d * a.scale : -INFINITY;
-            if (sc) sc[i] = d;
-            if (d != -INFINITY) {
-              const float mn = fmaxf(M, d), f = M == -INFINITY ? 0.0f : ex2(M - mn), pr = ex2(d - mn + kProbShift<BF>);
-              L = L * f + pr;
-              E = E * f + pr;
-#pragma unroll
-              for (int j = 0; j < D / 32; ++j)
-#pragma unroll
-                for (int z = 0; z < 4; ++z) acc[j][z] = fmaf(pr, vv[j][z], acc[j][z] * f);
-              M = mn;
-            }
-          }
-        }
-        if (rr < a.rows) {
+        if (there) {
           if (whole) {
 #pragma unroll
             for (int j = 0; j < D / 32; ++j)
@@ -769,10 +805,12 @@ struct AttnSpace {
   int64_t prefix, part, part_ml, lse, scores, ld_scores;
   int64_t bytes() const { return prefix + part + part_ml + lse + scores; }
 };
+// Rows of a block: eights, 32 at most.
+static int block_rows(int64_t rows) { return rows >= 32 ? 32 : (int)((rows + 7) / 8 * 8); }
 static AttnSpace attn_space(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t tokens, int64_t max_tokens,
                             bool weights) {
   AttnSpace s;
-  const int64_t rows = heads / kv_heads * tokens, RB = rows <= 16 ? 16 : 32;
+  const int64_t rows = heads / kv_heads * tokens, RB = block_rows(rows);
   s.prefix = align_up((batch + 1) * 8, 256);
   s.part = align_up(2 * kPaGrid * RB * D * 4, 256);
   s.part_ml = align_up(2 * kPaGrid * RB * 16, 256);
@@ -794,9 +832,9 @@ static cudaError_t launch_join(const AttnArgs& a, int RB, cudaStream_t s) {
                     s, 1u, a, RB);
 }
 
-template <bool BF, int D, int MT, bool ALIGNED>
+template <bool BF, int D, int NT, bool ALIGNED>
 static cudaError_t launch_attn_kernel(const AttnArgs& a, size_t dyn, cudaStream_t s) {
-  auto* k = k_paged_attn<BF, D, MT, ALIGNED>;
+  auto* k = k_paged_attn<BF, D, NT, ALIGNED>;
   static std::atomic<bool> done[64];  // the shared-memory opt-in, for the largest batch
   int dev;
   bool needs;
@@ -805,7 +843,7 @@ static cudaError_t launch_attn_kernel(const AttnArgs& a, size_t dyn, cudaStream_
   if (needs) {
     e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              kPaWarps * kPaStages * kPaStage + kPaWarps * 16 * 12 + 32 * D * 2 +
-                                 (kPagedMaxTokens - 1) * 4 * D + kPagedMaxBatch * 4);
+                                 kPagedMaxBatch * 4);
     if (e != cudaSuccess) return e;
     opted_in(done, dev);
   }
@@ -814,12 +852,14 @@ static cudaError_t launch_attn_kernel(const AttnArgs& a, size_t dyn, cudaStream_
 
 template <bool BF, int D>
 static cudaError_t launch_attn(const AttnArgs& a, float* weights, int64_t ldw, cudaStream_t s) {
-  const int RB = a.rows <= 16 ? 16 : 32;
-  const size_t dyn = (size_t)kPaWarps * kPaStages * kPaStage + (size_t)kPaWarps * 16 * 12 + (RB > 16 ? RB * D * 2 : 0) +
-                     (size_t)(a.tokens - 1) * 4 * D + (size_t)a.c.batch * 4;
+  const int RB = block_rows(a.rows);
+  const size_t dyn = (size_t)kPaWarps * kPaStages * kPaStage + (size_t)kPaWarps * 16 * 12 + (RB > 24 ? RB * D * 2 : 0) +
+                     (size_t)a.c.batch * 4;
   const bool aligned = a.c.page_size % 16 == 0;
-  cudaError_t e = RB == 16 ? (aligned ? launch_attn_kernel<BF, D, 1, true>(a, dyn, s) : launch_attn_kernel<BF, D, 1, false>(a, dyn, s))
-                           : (aligned ? launch_attn_kernel<BF, D, 2, true>(a, dyn, s) : launch_attn_kernel<BF, D, 2, false>(a, dyn, s));
+  cudaError_t e = RB == 8    ? (aligned ? launch_attn_kernel<BF, D, 1, true>(a, dyn, s) : launch_attn_kernel<BF, D, 1, false>(a, dyn, s))
+                  : RB == 16 ? (aligned ? launch_attn_kernel<BF, D, 2, true>(a, dyn, s) : launch_attn_kernel<BF, D, 2, false>(a, dyn, s))
+                  : RB == 24 ? (aligned ? launch_attn_kernel<BF, D, 3, true>(a, dyn, s) : launch_attn_kernel<BF, D, 3, false>(a, dyn, s))
+                             : (aligned ? launch_attn_kernel<BF, D, 4, true>(a, dyn, s) : launch_attn_kernel<BF, D, 4, false>(a, dyn, s));
   if (e != cudaSuccess) return e;
   if (a.chunk_units) e = launch_join<BF, D>(a, RB, s);
   if (e != cudaSuccess || !weights) return e;
@@ -864,7 +904,7 @@ extern "C" OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* 
   int st = otf::view_of(cache, a.c);
   if (st != OTF_OK) return st;
   const int64_t D = cache->head_dim;
-  if (heads <= 0 || heads % a.c.kv_heads || tokens <= 0) return OTF_ERR_INVALID;
+  if (heads <= 0 || heads % a.c.kv_heads || tokens <= 0 || !(std::fabs(scale) <= 3.4e38f)) return OTF_ERR_INVALID;
   if (tokens > otf::kPagedMaxTokens || heads > 65535) return OTF_ERR_UNSUPPORTED;
   if (!otf::rows16(q, ldq, heads * D) || !otf::rows16(out, ldo, heads * D)) return OTF_ERR_INVALID;
   if (weights && ldw < a.c.capacity) return OTF_ERR_INVALID;
@@ -885,7 +925,7 @@ extern "C" OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* 
   const bool whole = a.c.capacity <= otf::kPaWholeTokens;
   a.chunk_units = whole ? 0 : 1;
   a.item_units = whole ? 1 : otf::kPaItemUnits;
-  a.blocks = a.rows <= 16 ? 1 : (a.rows + 31) / 32;
+  a.blocks = (a.rows + 31) / 32;
   char* w = static_cast<char*>(workspace);
   a.prefix = reinterpret_cast<int64_t*>(w);
   a.part = reinterpret_cast<float*>(w += space.prefix);

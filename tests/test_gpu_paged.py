@@ -234,6 +234,7 @@ def test_attend_peaked_and_flat_scores(dtype, cuda_dev):
     check_attend(cuda_dev, [500, 33], 1, 16, 8, 2, 128, TYPES[dtype], spread=30.0)      # one key takes nearly all
     check_attend(cuda_dev, [3000], 2, 16, 8, 2, 64, TYPES[dtype], spread=0.0, weights=True)  # all equal
     check_attend(cuda_dev, [90], 1, 16, 8, 2, 128, TYPES[dtype], scale=-0.3)
+    check_attend(cuda_dev, [90, 9], 3, 16, 8, 2, 64, TYPES[dtype], scale=0.0, weights=True)
 
 
 def test_attend_many_sequences_and_long_ones(cuda_dev):
@@ -249,8 +250,12 @@ def test_attend_many_sequences_and_long_ones(cuda_dev):
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 def test_attend_rows_do_not_see_later_tokens(bad, dtype, cuda_dev):
     """The newest tokens hold `bad`: rows before them stay finite and right, rows that see them do not."""
-    dt = TYPES[dtype]
-    totals, tokens, page, heads, kv, dim = [40, 5, 129], 4, 16, 6, 2, 64
+    for totals, tokens, page, heads, kv, dim in (([40, 5, 129], 4, 16, 6, 2, 64), ([33, 7, 66, 400], 5, 20, 28, 4, 128),
+                                                 ([64, 80, 17], 16, 16, 4, 4, 128), ([40, 31], 8, 8, 32, 2, 64)):
+        check_later_tokens(bad, TYPES[dtype], cuda_dev, totals, tokens, page, heads, kv, dim)
+
+
+def check_later_tokens(bad, dt, cuda_dev, totals, tokens, page, heads, kv, dim):
     cache, pools, table, g = make(cuda_dev, totals, page, kv, dim, dt)
     for b, n in enumerate(totals):
         for pool, on in zip(pools, (cache.k_pages, cache.v_pages)):
