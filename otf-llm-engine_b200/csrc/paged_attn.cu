@@ -70,9 +70,10 @@ struct AttnArgs {
   int64_t* prefix;     // [batch + 1] units before each sequence
   float* part;         // [2 x grid][rows of a block][head_dim]: o of a part
   float4* part_ml;     // [2 x grid][rows of a block]: its m, l and unrounded l
-  float* lse;          // [batch, kv_heads, rows] log2 of the sum, when weights are wanted
-  float* scores;       // [batch, kv_heads, rows, ld_scores] likewise
-  int64_t ld_scores;
+  float* lse;          // [batch, kv_heads, ld_scores] log2 of the sum, when weights are wanted
+  float* scores;       // [batch, kv_heads, max_keys, ld_scores] likewise, a row's score in each column
+  int64_t max_keys;
+  int ld_scores;       // rows, rounded up to 4
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -437,13 +438,15 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const int r = rb * RB + n * 8 + (lane & 3) * 2;
-          float* to = a.scores + (((int64_t)get.b * c.kv_heads + g) * a.rows + r) * a.ld_scores + key0 + (lane >> 2);
+          float* to = a.scores + (((int64_t)get.b * c.kv_heads + g) * a.max_keys + key0 + (lane >> 2)) * a.ld_scores + r;
+          if (r < a.ld_scores)  // an odd row's neighbour is padding
 #pragma unroll
-          for (int h = 0; h < KT / 16; ++h)
+            for (int h = 0; h < KT / 16; ++h)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (r + (i & 1) < a.rows && key0 + h * 16 + (i >> 1) * 8 + (lane >> 2) < end)
-                to[(i & 1) * a.ld_scores + h * 16 + (i >> 1) * 8] = s[h][n][i] * scale;
+              for (int z = 0; z < 2; ++z)
+                if (key0 + h * 16 + z * 8 + (lane >> 2) < end)
+                  *reinterpret_cast<float2*>(to + (int64_t)(h * 16 + z * 8) * a.ld_scores) =
+                      make_float2(s[h][n][2 * z] * scale, s[h][n][2 * z + 1] * scale);
         }
       }
       uint32_t p[KT / 16][NT][2];
@@ -639,7 +642,7 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
             for (int j = 0; j < D / 32; ++j)
               store_row<BF, 4>(a.out + row * a.ldo + (int64_t)head * D + j * 32 + part * 4, acc[j], 1.0f / L);
             if (a.lse && part == 0)
-              a.lse[((int64_t)now.b * c.kv_heads + g) * a.rows + rr] = M + log2f(E) - kProbShift<BF>;
+              a.lse[((int64_t)now.b * c.kv_heads + g) * a.ld_scores + rr] = M + log2f(E) - kProbShift<BF>;
           } else {
             const int64_t at = (int64_t)(2 * blockIdx.x + (parts > 0 ? 1 : 0)) * RB + t * 16 + r;
 #pragma unroll
@@ -764,40 +767,34 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_paged_attn_join(AttnArgs a,
   }
   const int tok = rr / a.rep, head = g * a.rep + rr - tok * a.rep;
   store_row<BF, PL>(a.out + ((int64_t)b * a.tokens + tok) * a.ldo + (int64_t)head * D + lane * PL, acc, 1.0f / L);
-  if (a.lse && lane == 0) a.lse[((int64_t)b * c.kv_heads + g) * a.rows + rr] = M + log2f(E) - kProbShift<BF>;
+  if (a.lse && lane == 0) a.lse[((int64_t)b * c.kv_heads + g) * a.ld_scores + rr] = M + log2f(E) - kProbShift<BF>;
 }
 
-// weights[b, g, s] += sum over the item's rows of 2^(score - lse): a thread takes 4 tokens, rows in
-// order.  Memory-bound: the scores are read once, mostly from L2.
+// weights[b, g, s] += sum over the item's rows of 2^(score - lse): a thread per token, rows in order.
+// Memory-bound: the scores are read once, mostly from L2.
 constexpr int kWeightThreads = 128;
 
 __global__ void __launch_bounds__(kWeightThreads) k_paged_attn_weights(AttnArgs a, float* weights, int64_t ldw) {
   pdl_trigger();
   pdl_wait();
   const PagedView& c = a.c;
-  const int g = blockIdx.y, b = blockIdx.z, s = 4 * (blockIdx.x * kWeightThreads + threadIdx.x);
+  const int g = blockIdx.y, b = blockIdx.z, s = blockIdx.x * kWeightThreads + threadIdx.x;
   const int len = c.lengths[b];
   if (len < 0 || (int64_t)len + a.tokens > c.capacity || s >= len + a.tokens) return;
   const int64_t item = (int64_t)b * c.kv_heads + g;
-  const float* x = a.scores + item * a.rows * a.ld_scores + s;
-  const float* lse = a.lse + item * a.rows;
-  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  const float* x = a.scores + (item * a.max_keys + s) * a.ld_scores;
+  const float* lse = a.lse + item * a.ld_scores;
+  float sum = 0.0f;
   auto term = [](float v, float l) { return v == -INFINITY ? 0.0f : ex2(v - l); };
 #pragma unroll 4
-  for (int r = 0; r < a.rows; ++r) {
-    const float4 v = *reinterpret_cast<const float4*>(x + r * a.ld_scores);
-    const float l = lse[r];
-    sum.x += term(v.x, l);
-    sum.y += term(v.y, l);
-    sum.z += term(v.z, l);
-    sum.w += term(v.w, l);
+  for (int r = 0; r < a.rows; r += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(x + r), l = *reinterpret_cast<const float4*>(lse + r);
+    sum += term(v.x, l.x);
+    if (r + 1 < a.rows) sum += term(v.y, l.y);
+    if (r + 2 < a.rows) sum += term(v.z, l.z);
+    if (r + 3 < a.rows) sum += term(v.w, l.w);
   }
-  float* w = weights + item * ldw + s;
-  const int n = len + a.tokens - s;  // what lies behind the last token was not written
-  w[0] += sum.x;
-  if (n > 1) w[1] += sum.y;
-  if (n > 2) w[2] += sum.z;
-  if (n > 3) w[3] += sum.w;
+  weights[item * ldw + s] += sum;
 }
 
 // Bytes of the workspace's parts, in order.
@@ -814,9 +811,9 @@ static AttnSpace attn_space(int64_t batch, int64_t heads, int64_t kv_heads, int6
   s.prefix = align_up((batch + 1) * 8, 256);
   s.part = align_up(2 * kPaGrid * RB * D * 4, 256);
   s.part_ml = align_up(2 * kPaGrid * RB * 16, 256);
-  s.ld_scores = align_up(max_tokens, 8);
-  s.lse = weights ? align_up(batch * kv_heads * rows * 4, 256) : 0;
-  s.scores = weights ? align_up(batch * kv_heads * rows * s.ld_scores * 4, 256) : 0;
+  s.ld_scores = align_up(rows, 4);
+  s.lse = weights ? align_up(batch * kv_heads * s.ld_scores * 4, 256) : 0;
+  s.scores = weights ? align_up(batch * kv_heads * s.ld_scores * max_tokens * 4, 256) : 0;
   return s;
 }
 
@@ -864,7 +861,7 @@ static cudaError_t launch_attn(const AttnArgs& a, float* weights, int64_t ldw, c
   if (a.chunk_units) e = launch_join<BF, D>(a, RB, s);
   if (e != cudaSuccess || !weights) return e;
   return launch_pdl(k_paged_attn_weights,
-                    dim3((unsigned)((a.c.capacity + 4 * kWeightThreads - 1) / (4 * kWeightThreads)), (unsigned)a.c.kv_heads,
+                    dim3((unsigned)((a.c.capacity + kWeightThreads - 1) / kWeightThreads), (unsigned)a.c.kv_heads,
                          (unsigned)a.c.batch),
                     dim3(kWeightThreads), 0,
                     s, 1u, a, weights, ldw);
@@ -934,7 +931,8 @@ extern "C" OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* 
   if (weights) {
     a.lse = reinterpret_cast<float*>(w);
     a.scores = reinterpret_cast<float*>(w + space.lse);
-    a.ld_scores = space.ld_scores;
+    a.ld_scores = (int)space.ld_scores;
+    a.max_keys = a.c.capacity;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = cache->dtype == OTF_DTYPE_BF16;
