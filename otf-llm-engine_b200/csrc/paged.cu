@@ -202,23 +202,25 @@ constexpr int kEvictThreads = 512;
 constexpr int kEvictKeys = 16;       // weights of a thread
 constexpr int kEvictStrip = kEvictThreads * kEvictKeys;
 constexpr int kEvictCluster = 8;     // CTAs that may share one (sequence, KV head)
-constexpr int kEvictBins = 2048;     // 11, 11 and 10 bits in three rounds
 
 // Which places stay: a cluster per (sequence, KV head), each CTA a contiguous slice of the n
-// weights that are not among the recent ones, a thread 16 neighbours.  Three rounds of 11,
-// 11 and 10 bits find the k-th largest key (each round: counts of the slice's keys in shared memory,
-// summed over the cluster through distributed shared memory); then every CTA, knowing how many kept keys
-// lie before its slice, writes its places in order.  Of the keys equal to the k-th largest the
-// first ones stay.  Bound by the rounds' latencies, not by bytes: ONE holds the keys of a
-// slice of up to kEvictStrip in registers through all rounds, longer ones are read again (from L2).
-template <bool ONE>
+// weights that are not among the recent ones, a thread 16 neighbours.  Rounds of BITS bits find the
+// k-th largest key (each round: counts of the slice's keys in shared memory, summed over the cluster
+// through distributed shared memory), and what the CTAs before this one count above the limit and at
+// it is where its own places begin.  Of the keys equal to the k-th largest the first ones stay.
+// Bound by the rounds' latencies, not by bytes: ONE holds the keys of a slice of up to kEvictStrip
+// in registers through all rounds, longer ones are read again (from L2).  BITS 11 (three rounds) for
+// a CTA by itself, 8 (four) in a cluster, whose CTAs read one another's counts: 65536 weights of 8
+// heads, with the copy, 26.1 us with 11, 21.6 us with 8.
+template <bool ONE, int BITS>
 __global__ void __launch_bounds__(kEvictThreads) k_evict_select(const int* lengths, int kv_heads, int capacity,
                                                                 const float* weights, int64_t ldw, int budget,
                                                                 int recent, int* kept, int ctas) {
-  constexpr int W = kEvictThreads / 32, V = kEvictKeys;
-  __shared__ __align__(16) int s_hist[3][kEvictBins];
+  constexpr int W = kEvictThreads / 32, V = kEvictKeys, BINS = 1 << BITS, ROUNDS = (31 + BITS) / BITS;
+  constexpr int ND = BINS > kEvictThreads ? BINS / kEvictThreads : 1;  // digits of a thread, of the first BINS / ND
+  __shared__ __align__(16) int s_hist[ROUNDS][BINS];
   __shared__ int s_cut[2];    // this round's digit, and how many keys of it are needed
-  __shared__ int s_count[2];  // the slice's keys above and at the limit
+  __shared__ int s_count[2];  // kept keys above the limit, and keys at it, in the slices before
   __shared__ int s_warp[W];
   pdl_trigger();
   pdl_wait();
@@ -264,16 +266,17 @@ __global__ void __launch_bounds__(kEvictThreads) k_evict_select(const int* lengt
     return there;
   };
   int there = ONE ? load(i0) : 0;
-  for (int i = tid; i < 3 * kEvictBins / 4; i += kEvictThreads)
+  for (int i = tid; i < ROUNDS * BINS / 4; i += kEvictThreads)
     reinterpret_cast<int4*>(&s_hist[0][0])[i] = make_int4(0, 0, 0, 0);
   if (tid < 2) s_count[tid] = 0;
   __syncthreads();
   uint32_t limit = 0u, mask = 0u;
   int need = k;
+  int g0 = 0, e0 = 0;  // this thread's digits' share of the keys above the limit, and at it, in the slices before
 #pragma unroll 1
-  for (int round = 0; round < 3; ++round) {
-    const int shift = round == 0 ? 21 : round == 1 ? 10 : 0;
-    const uint32_t bits = round == 2 ? 1023u : 2047u;
+  for (int round = 0; round < ROUNDS; ++round) {
+    const int shift = max(0, 32 - BITS * (round + 1));
+    const uint32_t bits = round == ROUNDS - 1 ? (1u << (32 - BITS * (ROUNDS - 1))) - 1u : BINS - 1u;
     for (int base = i0; base < i1; base += kEvictStrip) {
       if (!ONE) there = load(base);
 #pragma unroll
@@ -281,23 +284,30 @@ __global__ void __launch_bounds__(kEvictThreads) k_evict_select(const int* lengt
         if (z < there && (u[z] & mask) == limit) atomicAdd(&s_hist[round][(u[z] >> shift) & bits], 1);
     }
     if (ctas > 1) cluster_sync_all(); else __syncthreads();
-    // thread t: the 4 digits from kEvictBins - 1 - 4 t downwards
-    int4 c = make_int4(0, 0, 0, 0);
-    const int* mine = &s_hist[round][kEvictBins - 4 - 4 * tid];
-    if (ctas > 1) {
+    // thread t: the ND digits from high - ND + 1 to high, of the cluster and of the CTAs before this one
+    const int high = BINS - 1 - ND * tid;
+    int c[ND], lower[ND], all = 0;
 #pragma unroll
-      for (int r = 0; r < kEvictCluster; ++r)
-        if (r < ctas) {
-          const int4 x = ld_cluster_v4(mapa_shared(smem_u32(mine), r));
-          c.x += x.x;
-          c.y += x.y;
-          c.z += x.z;
-          c.w += x.w;
-        }
-    } else {
-      c = *reinterpret_cast<const int4*>(mine);
+    for (int i = 0; i < ND; ++i) c[i] = lower[i] = 0;
+    if (high >= 0) {
+      const int* mine = &s_hist[round][high - ND + 1];
+      if (ctas > 1) {
+#pragma unroll
+        for (int r = 0; r < kEvictCluster; ++r)
+          if (r < ctas)
+#pragma unroll
+            for (int i = 0; i < ND; ++i) {
+              const int x = ld_cluster_s32(mapa_shared(smem_u32(mine + i), r));
+              c[i] += x;
+              if (r < rank) lower[i] += x;
+            }
+      } else {
+#pragma unroll
+        for (int i = 0; i < ND; ++i) c[i] = mine[i];
+      }
     }
-    const int all = (c.x + c.y) + (c.z + c.w);
+#pragma unroll
+    for (int i = 0; i < ND; ++i) all += c[i];
     int before = all;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -311,22 +321,41 @@ __global__ void __launch_bounds__(kEvictThreads) k_evict_select(const int* lengt
     for (int x = 0; x < W; ++x)
       if (x < warp) before += s_warp[x];
     if (before < need && before + all >= need) {  // one thread's
-      const int d[4] = {c.w, c.z, c.y, c.x};
       bool found = false;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (!found && before + d[i] >= need) {
+      for (int i = ND - 1; i >= 0; --i) {
+        if (!found && before + c[i] >= need) {
           found = true;
-          s_cut[0] = kEvictBins - 1 - 4 * tid - i;
+          s_cut[0] = high - ND + 1 + i;
           s_cut[1] = need - before;
         }
-        before += d[i];
+        before += c[i];
       }
     }
     __syncthreads();
-    limit |= (uint32_t)s_cut[0] << shift;
+    // every thread has used what it read: after the last round the others may leave (waited for at the end)
+    if (ctas > 1 && round == ROUNDS - 1) cluster_arrive_relaxed();
+    const int cut = s_cut[0];
+    limit |= (uint32_t)cut << shift;
     need = s_cut[1];
     mask |= bits << shift;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) {
+      const int digit = high - ND + 1 + i;
+      if (digit > cut) g0 += lower[i];
+      if (round == ROUNDS - 1 && digit == cut) e0 += lower[i];
+    }
+  }
+  if (ctas > 1) {  // the threads' shares as one sum
+    g0 = __reduce_add_sync(0xffffffffu, g0);
+    e0 = __reduce_add_sync(0xffffffffu, e0);
+    if (lane == 0) {
+      atomicAdd(&s_count[0], g0);
+      atomicAdd(&s_count[1], e0);
+    }
+    __syncthreads();
+    g0 = s_count[0];
+    e0 = s_count[1];
   }
   // keys above the limit in the low, at it in the high half
   auto count = [&] {
@@ -336,32 +365,9 @@ __global__ void __launch_bounds__(kEvictThreads) k_evict_select(const int* lengt
       if (z < there) c += u[z] > limit ? 1u : u[z] == limit ? 0x10000u : 0u;
     return c;
   };
-  uint32_t mine = 0;
-  int g0 = 0, e0 = 0;  // kept keys above the limit, and keys at it, before this strip
-  if (ctas > 1) {
-    int above = 0, equal = 0;
-    for (int base = i0; base < i1; base += kEvictStrip) {
-      if (!ONE) there = load(base);
-      mine = count();
-      above += mine & 0xffffu;
-      equal += mine >> 16;
-    }
-    above = __reduce_add_sync(0xffffffffu, above);
-    equal = __reduce_add_sync(0xffffffffu, equal);
-    if (lane == 0) {
-      atomicAdd(&s_count[0], above);
-      atomicAdd(&s_count[1], equal);
-    }
-    __syncwarp();
-    cluster_sync_all();
-    for (int r = 0; r < rank; ++r) {
-      g0 += ld_cluster_s32(mapa_shared(smem_u32(&s_count[0]), r));
-      e0 += ld_cluster_s32(mapa_shared(smem_u32(&s_count[1]), r));
-    }
-  }
   for (int base = i0; base < i1; base += kEvictStrip) {
     if (!ONE) there = load(base);
-    mine = count();
+    const uint32_t mine = count();
     uint32_t inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -390,7 +396,8 @@ __global__ void __launch_bounds__(kEvictThreads) k_evict_select(const int* lengt
     e0 += (int)(all >> 16);
     __syncthreads();
   }
-  if (ctas > 1) cluster_sync_all();  // no CTA leaves while another reads its counts
+  __syncwarp();
+  if (ctas > 1) cluster_wait();  // no CTA leaves while another reads its counts
 }
 
 // The kept rows' keys, values and weights, where source and target are apart: grid (pairs, tiles
@@ -647,7 +654,9 @@ extern "C" OTF_API int otf_paged_evict(const otf_paged_cache* from, const otf_pa
   int ctas = 1;
   while (ctas < otf::kEvictCluster && (int64_t)ctas * otf::kEvictStrip < f.capacity && pairs * ctas <= 148) ctas *= 2;
   const bool one = (((f.capacity + ctas - 1) / ctas + 3) & ~3) <= otf::kEvictStrip;
-  cudaError_t e = otf::launch_pdl(one ? otf::k_evict_select<true> : otf::k_evict_select<false>, dim3((unsigned)(pairs * ctas)), dim3(otf::kEvictThreads), 0, s,
+  auto* select = ctas > 1 ? (one ? otf::k_evict_select<true, 8> : otf::k_evict_select<false, 8>)
+                          : (one ? otf::k_evict_select<true, 11> : otf::k_evict_select<false, 11>);
+  cudaError_t e = otf::launch_pdl(select, dim3((unsigned)(pairs * ctas)), dim3(otf::kEvictThreads), 0, s,
                                   (unsigned)ctas, f.lengths, f.kv_heads, f.capacity, weights, ldw, (int)budget,
                                   (int)recent, kept, ctas);
   if (e != cudaSuccess) return set_cuda_error(e);

@@ -509,6 +509,44 @@ def test_evict_long_sequence(cuda_dev):
     check_evict(cuda_dev, [5000], 700, 100, 64, 2, 64, torch.float16, "token", False)
 
 
+@pytest.mark.parametrize("batch,kv,lengths,budget,recent", [
+    (1, 3, [20001], 3000, 17), (1, 2, [70003], 9000, 0), (2, 8, [33000, 8193], 8192, 8000), (50, 4, [9000, 100, 8200], 500, 60),
+    (1, 1, [300000], 1000, 999)])
+@pytest.mark.parametrize("kind", ["spread", "ties", "equal"])
+def test_evict_selects_from_many_weights(batch, kv, lengths, budget, recent, kind, cuda_dev):
+    """Selections over several CTAs and over more weights than they hold, against a stable sort.  The source's
+    tables name one page again and again."""
+    from otf_llm.paged import PagedKVCache
+    g = torch.Generator(device=cuda_dev).manual_seed(budget)
+    lens = [lengths[b % len(lengths)] for b in range(batch)]
+    room = max(lens) + 40
+    pages = torch.randn(1, 64, kv, 64, generator=g, device=cuda_dev).half()
+    cache = PagedKVCache(pages, pages.clone(), torch.zeros(batch, -(-room // 64), dtype=torch.int32, device=cuda_dev),
+                         torch.tensor(lens, dtype=torch.int32, device=cuda_dev))
+    w = torch.rand(batch, kv, cache.capacity, generator=g, device=cuda_dev) ** 5
+    if kind == "ties":
+        w = (w * 12).round()
+    elif kind == "equal":
+        w.fill_(-1.5)
+    each = -(-budget // 64)
+    to = PagedKVCache.allocate(batch * each, 64, kv, 64, torch.arange(batch * each, dtype=torch.int32, device=cuda_dev).view(batch, each),
+                               torch.zeros(batch, dtype=torch.int32, device=cuda_dev))
+    wo = torch.empty(batch, kv, budget, device=cuda_dev)
+    kept = cache.evict(w, budget, recent, to=to, weights_out=wo)
+    assert flag() == 0 and to.lengths.tolist() == [min(n, budget) for n in lens]
+    for b, n in enumerate(lens):
+        if n <= budget:
+            want = torch.arange(n, device=cuda_dev).expand(kv, n)
+        else:
+            old = w[b, :, :n - recent].sort(dim=1, descending=True, stable=True).indices[:, :budget - recent]
+            want = torch.cat([old.sort(dim=1).values, torch.arange(n - recent, n, device=cuda_dev).expand(kv, recent)], 1)
+        m = want.shape[1]
+        assert torch.equal(kept[b, :, :m].long(), want) and bool((kept[b, :, m:] == -1).all())
+        assert torch.equal(wo[b, :, :m], w[b].gather(1, want)) and not bool(wo[b, :, m:].any())
+        got = to.k_pages.view(batch, each * 64, kv, 64)[b, :m]
+        assert torch.equal(got, torch.stack([cache.k_pages[0, want[h] % 64, h] for h in range(kv)], 1))
+
+
 # ---- graphs, streams, all together ----------------------------------------------------------------
 
 
