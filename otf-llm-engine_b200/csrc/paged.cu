@@ -44,95 +44,105 @@ struct AppendArgs {
   int per;    // rows of a sequence, without starts
 };
 
-// Where a row goes: the offset of its token's page row, or -1 (all threads agree).  The rotary
-// position's sines and cosines go to s_c and s_s.
-__device__ __forceinline__ int64_t append_place(const AppendArgs& a, float* s_c, float* s_s) {
+// Where a row goes: the offset of its token's page row, or -1 (all its threads agree; `t` of `threads`).
+// The rotary position's sines and cosines go to s_c and s_s.
+__device__ __forceinline__ int64_t append_place(const AppendArgs& a, int row, int t, int threads, float* s_c, float* s_s) {
   const PagedView& c = a.c;
-  const int row = blockIdx.x, tid = threadIdx.x;
   const int b = a.starts ? sequence_of(a.starts, c.batch, row) : row / a.per;
   if (b >= c.batch) return -1;  // behind the last sequence
-  const int t = row - (a.starts ? a.starts[b] : b * a.per);
+  const int i = row - (a.starts ? a.starts[b] : b * a.per);
   const int len = c.lengths[b];
   if (len < 0) return -1;  // no sequence in this place
-  const int64_t slot = (int64_t)len + t;
-  if (t < 0 || slot >= c.capacity) {
-    if (tid == 0) report_bad_page();
+  const int64_t slot = (int64_t)len + i;
+  if (i < 0 || slot >= c.capacity) {
+    if (t == 0) report_bad_page();
     return -1;
   }
-  const int page = c.table[b * c.ld_table + slot / c.page_size];
+  const int in = (int)slot / c.page_size;
+  const int page = c.table[b * c.ld_table + in];
   if (page < 0 || page >= c.n_pages) {
-    if (tid == 0) report_bad_page();
+    if (t == 0) report_bad_page();
     return -1;
   }
-  if (tid < a.rot / 2) {
+  const int position = a.positions ? a.positions[row] : (int)slot;
+  for (int p = t; p < a.rot / 2; p += threads) {
     // the angle in turns, 64 bits until the whole turns are gone: what is left keeps 2^-25 of a turn
-    double turn = (double)(a.positions ? a.positions[row] : (int)slot) * a.turns[tid];
+    double turn = (double)position * a.turns[p];
     turn -= rint(turn);
     float sn, cs;
     sincospif(2.0f * (float)turn, &sn, &cs);
-    s_c[tid] = cs * a.factor;
-    s_s[tid] = sn * a.factor;
+    s_c[p] = cs * a.factor;
+    s_s[p] = sn * a.factor;
   }
-  return page * c.page_stride + (slot % c.page_size) * c.token_stride;
+  return page * c.page_stride + (int64_t)((int)slot - in * c.page_size) * c.token_stride;
 }
 
-// Rotary positions and the cache write, one CTA per row, in units of two 16-byte pieces whose
-// values turn together: pieces i and i + rot / 16 of a head (half layout), or 2i and 2i + 1.
-// Memory-bound: a row is read and written once.  The values are requested before the row's place
-// in the cache and its angles are known, kAppendBatch units at a time; a thread has the same i in
-// every head, whose 8 sines and cosines it keeps in registers.
+// Where head h of a row is read from and goes to: queries, keys, values in this order.
+template <int D>
+__device__ __forceinline__ const uint16_t* append_source(const AppendArgs& a, int64_t row, int h) {
+  const int k = h - a.heads, v = k - a.c.kv_heads;
+  return k < 0 ? a.q + row * a.ldq + (int64_t)h * D : v < 0 ? a.k + row * a.ldk + (int64_t)k * D : a.v + row * a.ldv + (int64_t)v * D;
+}
+template <int D>
+__device__ __forceinline__ uint16_t* append_target(const AppendArgs& a, int64_t row, int64_t at, int h) {
+  const int k = h - a.heads, v = k - a.c.kv_heads;
+  return k < 0   ? a.qo + row * a.ldqo + (int64_t)h * D
+         : v < 0 ? a.c.k + at + (int64_t)k * a.c.head_stride
+                 : a.c.v + at + (int64_t)v * a.c.head_stride;
+}
+
+// Rotary positions and the cache write in units of two 16-byte pieces whose values turn together:
+// pieces i and i + rot / 16 of a head (half layout), or 2i and 2i + 1.  Memory-bound: a row is read
+// and written once.  The values are requested before the row's place in the cache and its angles are
+// known, kAppendBatch units at a time; a thread has the same i in every head, whose 8 sines and
+// cosines it keeps in registers.  WR warps a row: 4, or 1 for rows that a warp holds at once (27500 rows
+// of 18 heads of 64: 62.5 us with 4, 37.6 with 1; of 80 heads of 128: 168.6 with 4, 171.8 with 1; 256
+// of them 5.1 and 8.3).
 constexpr int kAppendThreads = 128;
 constexpr int kAppendBatch = 5;
 
-template <bool BF, int D>
-__global__ void __launch_bounds__(kAppendThreads) k_paged_append(AppendArgs a) {
-  constexpr int UH = D / 16;  // units of a head
-  __shared__ __align__(16) float s_c[64], s_s[64];
+template <bool BF, int D, int WR>
+__global__ void __launch_bounds__(kAppendThreads) k_paged_append(AppendArgs a, int n) {
+  constexpr int UH = D / 16, T = 32 * WR, R = kAppendThreads / T;  // units of a head, threads of a row, rows of the CTA
+  __shared__ __align__(16) float s_c[R][64], s_s[R][64];
   pdl_trigger();
   pdl_wait();
-  const PagedView& c = a.c;
-  const int64_t row = blockIdx.x;
-  const int heads = a.heads + 2 * c.kv_heads, i = threadIdx.x % UH;
+  const int mine = threadIdx.x / T, t = threadIdx.x % T, row = blockIdx.x * R + mine;
+  if (row >= n) return;  // a whole warp's, and with more warps a row there is one row
+  const int turning = a.heads + a.c.kv_heads, heads = turning + a.c.kv_heads, i = t % UH;
   const bool turns = i < a.rot / 16, halves = turns && !a.interleaved;
   const int p0 = halves ? i * 8 : i * 16, p1 = halves ? i * 8 + a.rot / 2 : i * 16 + 8;
-  const int v0 = i * 16;  // values never turn: whole 32-byte units
   float cs[8], sn[8];
   int64_t at = 0;
-  constexpr int HC = kAppendThreads / UH;  // heads that the CTA covers at once
+  constexpr int HC = T / UH;  // heads that the row's threads cover at once
   for (int h0 = 0; h0 < heads; h0 += kAppendBatch * HC) {
     uint4 x[kAppendBatch][2];
 #pragma unroll
     for (int j = 0; j < kAppendBatch; ++j) {
-      const int h = h0 + j * HC + (int)threadIdx.x / UH;
+      const int h = h0 + j * HC + t / UH;
       if (h < heads) {
-        const bool is_v = h >= a.heads + c.kv_heads;
-        const uint16_t* src = h < a.heads ? a.q + row * a.ldq + (int64_t)h * D
-                              : is_v      ? a.v + row * a.ldv + (int64_t)(h - a.heads - c.kv_heads) * D
-                                          : a.k + row * a.ldk + (int64_t)(h - a.heads) * D;
-        x[j][0] = *reinterpret_cast<const uint4*>(src + (is_v ? v0 : p0));
-        x[j][1] = *reinterpret_cast<const uint4*>(src + (is_v ? v0 + 8 : p1));
+        const uint16_t* src = append_source<D>(a, row, h);
+        x[j][0] = *reinterpret_cast<const uint4*>(src + (h < turning ? p0 : i * 16));  // values never turn
+        x[j][1] = *reinterpret_cast<const uint4*>(src + (h < turning ? p1 : i * 16 + 8));
       }
     }
     if (h0 == 0) {
-      at = append_place(a, s_c, s_s);
+      at = append_place(a, row, t, T, s_c[mine], s_s[mine]);
       if (at < 0) return;
-      __syncthreads();
+      if (WR > 1) __syncthreads(); else __syncwarp();
       if (turns)
 #pragma unroll
         for (int z = 0; z < 8; ++z) {
-          cs[z] = s_c[8 * i + z];
-          sn[z] = s_s[8 * i + z];
+          cs[z] = s_c[mine][8 * i + z];
+          sn[z] = s_s[mine][8 * i + z];
         }
     }
 #pragma unroll
     for (int j = 0; j < kAppendBatch; ++j) {
-      const int h = h0 + j * HC + (int)threadIdx.x / UH;
+      const int h = h0 + j * HC + t / UH;
       if (h >= heads) break;
-      const bool is_v = h >= a.heads + c.kv_heads;
-      uint16_t* dst = h < a.heads ? a.qo + row * a.ldqo + (int64_t)h * D
-                      : is_v      ? c.v + at + (int64_t)(h - a.heads - c.kv_heads) * c.head_stride
-                                  : c.k + at + (int64_t)(h - a.heads) * c.head_stride;
-      if (turns && !is_v) {
+      uint16_t* dst = append_target<D>(a, row, at, h);
+      if (turns && h < turning) {
         uint32_t* w0 = reinterpret_cast<uint32_t*>(&x[j][0]);
         uint32_t* w1 = reinterpret_cast<uint32_t*>(&x[j][1]);
 #pragma unroll
@@ -148,43 +158,61 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(AppendArgs a) {
           }
         }
       }
-      *reinterpret_cast<uint4*>(dst + (is_v ? v0 : p0)) = x[j][0];
-      *reinterpret_cast<uint4*>(dst + (is_v ? v0 + 8 : p1)) = x[j][1];
+      *reinterpret_cast<uint4*>(dst + (h < turning ? p0 : i * 16)) = x[j][0];
+      *reinterpret_cast<uint4*>(dst + (h < turning ? p1 : i * 16 + 8)) = x[j][1];
     }
   }
 }
 
-// The same for a rot that is no multiple of 16, value by value.
-template <bool BF>
-__global__ void __launch_bounds__(256) k_paged_append_any(AppendArgs a, int D) {
+// The same for a rot that is no multiple of 16, where the partners of a 16-byte piece lie across two
+// others: the heads go through shared memory, kAppendHeads at a time, whose threads share out the pairs.
+constexpr int kAppendHeads = 32;
+
+template <bool BF, int D>
+__global__ void __launch_bounds__(kAppendThreads) k_paged_append_any(AppendArgs a) {
+  constexpr int P = D / 8, N = kAppendHeads * P / kAppendThreads;  // pieces of a head, of a thread
   __shared__ float s_c[64], s_s[64];
+  __shared__ __align__(16) uint16_t s_x[kAppendHeads][D];
   pdl_trigger();
   pdl_wait();
-  const PagedView& c = a.c;
   const int64_t row = blockIdx.x;
-  const int64_t at = append_place(a, s_c, s_s);
-  if (at < 0) return;
-  __syncthreads();
-  const int pairs = D / 2, half = a.rot / 2;
-  for (int e = threadIdx.x; e < (a.heads + c.kv_heads) * pairs; e += blockDim.x) {
-    const int h = e / pairs, i = e - h * pairs;
-    const uint16_t* x = h < a.heads ? a.q + row * a.ldq + (int64_t)h * D : a.k + row * a.ldk + (int64_t)(h - a.heads) * D;
-    uint16_t* y = h < a.heads ? a.qo + row * a.ldqo + (int64_t)h * D : c.k + at + (h - a.heads) * c.head_stride;
-    const bool halves = i < half && !a.interleaved;
-    const int i0 = halves ? i : 2 * i, i1 = halves ? i + half : 2 * i + 1;
-    const uint16_t xa = x[i0], xb = x[i1];
-    if (i < half) {
-      const float fa = to_f<BF>(xa), fb = to_f<BF>(xb);
-      y[i0] = from_f<BF>(fa * s_c[i] - fb * s_s[i]);
-      y[i1] = from_f<BF>(fb * s_c[i] + fa * s_s[i]);
-    } else {
-      y[i0] = xa;
-      y[i1] = xb;
+  const int half = a.rot / 2, turning = a.heads + a.c.kv_heads, heads = turning + a.c.kv_heads;
+  int64_t at = 0;
+  for (int h0 = 0; h0 < heads; h0 += kAppendHeads) {
+    uint4 x[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int e = j * kAppendThreads + threadIdx.x, h = h0 + e / P;
+      if (h < heads) x[j] = *reinterpret_cast<const uint4*>(append_source<D>(a, row, h) + e % P * 8);
     }
-  }
-  for (int e = threadIdx.x; e < c.kv_heads * D; e += blockDim.x) {
-    const int h = e / D, i = e - h * D;
-    c.v[at + h * c.head_stride + i] = a.v[row * a.ldv + (int64_t)h * D + i];
+    if (h0 == 0) {
+      at = append_place(a, (int)row, threadIdx.x, kAppendThreads, s_c, s_s);
+      if (at < 0) return;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int e = j * kAppendThreads + threadIdx.x;
+      if (h0 + e / P < turning) *reinterpret_cast<uint4*>(&s_x[e / P][e % P * 8]) = x[j];
+    }
+    __syncthreads();
+    const int pairs = min(kAppendHeads, turning - h0) * half;
+    for (int e = threadIdx.x; e < pairs; e += kAppendThreads) {
+      const int h = e / half, p = e - h * half;
+      uint16_t& u = s_x[h][a.interleaved ? 2 * p : p];
+      uint16_t& v = s_x[h][a.interleaved ? 2 * p + 1 : p + half];
+      const float fu = to_f<BF>(u), fv = to_f<BF>(v);
+      u = from_f<BF>(fu * s_c[p] - fv * s_s[p]);
+      v = from_f<BF>(fv * s_c[p] + fu * s_s[p]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int e = j * kAppendThreads + threadIdx.x, h = h0 + e / P;
+      if (h >= heads) break;
+      if (h < turning && e % P * 8 < a.rot) x[j] = *reinterpret_cast<const uint4*>(&s_x[e / P][e % P * 8]);
+      *reinterpret_cast<uint4*>(append_target<D>(a, row, at, h) + e % P * 8) = x[j];
+    }
+    __syncthreads();  // before the next heads
   }
 }
 
@@ -621,11 +649,17 @@ extern "C" OTF_API int otf_paged_append(const otf_paged_cache* cache, const otf_
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const dim3 grid((unsigned)n);
   if (rot % 16)
-    return set_cuda_error(otf::launch_pdl(bf ? otf::k_paged_append_any<true> : otf::k_paged_append_any<false>, grid,
-                                          dim3(256), 0, s, 1u, a, (int)D));
-  auto* kern = D == 128 ? (bf ? otf::k_paged_append<true, 128> : otf::k_paged_append<false, 128>)
-                        : (bf ? otf::k_paged_append<true, 64> : otf::k_paged_append<false, 64>);
-  return set_cuda_error(otf::launch_pdl(kern, grid, dim3(otf::kAppendThreads), 0, s, 1u, a));
+    return set_cuda_error(otf::launch_pdl(D == 128 ? (bf ? otf::k_paged_append_any<true, 128> : otf::k_paged_append_any<false, 128>)
+                                                   : (bf ? otf::k_paged_append_any<true, 64> : otf::k_paged_append_any<false, 64>),
+                                          grid, dim3(otf::kAppendThreads), 0, s, 1u, a));
+  // a warp per row where its threads hold the whole row at once
+  const bool short_rows = ((q ? heads : 0) + 2 * c.kv_heads) * (D / 16) <= 32 * otf::kAppendBatch;
+  auto* kern = D == 128 ? (short_rows ? (bf ? otf::k_paged_append<true, 128, 1> : otf::k_paged_append<false, 128, 1>)
+                                : (bf ? otf::k_paged_append<true, 128, 4> : otf::k_paged_append<false, 128, 4>))
+                        : (short_rows ? (bf ? otf::k_paged_append<true, 64, 1> : otf::k_paged_append<false, 64, 1>)
+                                : (bf ? otf::k_paged_append<true, 64, 4> : otf::k_paged_append<false, 64, 4>));
+  return set_cuda_error(otf::launch_pdl(kern, dim3((unsigned)(short_rows ? (n + 3) / 4 : n)), dim3(otf::kAppendThreads), 0, s, 1u,
+                                        a, (int)n));
 }
 
 extern "C" OTF_API int otf_paged_evict(const otf_paged_cache* from, const otf_paged_cache* to, const float* weights,
