@@ -200,12 +200,19 @@ class PagedKVCache:
             raise ValueError(f"{name} needs 16-byte aligned rows that do not overlap, got strides {t.stride()}")
         return row
 
-    def _values(self, t: torch.Tensor, name: str) -> int:
-        """The address of values of the cache's type on its device."""
-        p = t.data_ptr()
-        if t.dtype is not self.dtype or t.device != self.device or p & 15:
-            raise ValueError(f"{name} must be 16-byte aligned {self.dtype} on {self.device}, got {t.dtype} on {t.device}")
-        return p
+    def _refuse(self, **given: torch.Tensor) -> None:
+        for name, t in given.items():
+            if t.dtype is not self.dtype or t.device != self.device or t.data_ptr() & 15:
+                raise ValueError(f"{name} must be 16-byte aligned {self.dtype} on {self.device}, got {t.dtype} on "
+                                 f"{t.device}")
+
+    def _output(self, out: torch.Tensor, name: str, like: torch.Tensor) -> Tuple[int, int]:
+        """The row stride and address of an output of like's shape."""
+        if out.shape != like.shape:
+            raise ValueError(f"{name} must have q's shape {tuple(like.shape)}, got {tuple(out.shape)}")
+        self._refuse(**{name: out})
+        rows = self._flat(out, name)
+        return self._heads(rows, name, rows.shape[1]), out.data_ptr()
 
     def _vector(self, t: torch.Tensor, name: str, n: int) -> int:
         if t.device != self.device or t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
@@ -229,18 +236,21 @@ class PagedKVCache:
         if plan is None:
             plan = self._remember(self._append_plans, key, self._plan_append(q, k, v))
         n, heads, ldq, ldk, ldv = plan
-        pk, pv = self._values(k, "k"), self._values(v, "v")
+        dtype, dev = self.dtype, self.device
+        pk, pv = k.data_ptr(), v.data_ptr()
+        if k.dtype is not dtype or v.dtype is not dtype or k.device != dev or v.device != dev or (pk | pv) & 15:
+            self._refuse(k=k, v=v)
         pq = po = ps = pp = None
         ldo = 0
         if q is not None:
-            pq, ldo = self._values(q, "q"), heads * self.head_dim
+            pq = q.data_ptr()
+            if q.dtype is not dtype or q.device != dev or pq & 15:
+                self._refuse(q=q)
             if q_out is None:
-                q_out = torch.empty_like(q)
+                q_out = torch.empty_like(q)         # heads next to one another, rows without gaps
+                ldo, po = heads * self.head_dim, q_out.data_ptr()
             else:
-                if q_out.shape != q.shape:
-                    raise ValueError(f"q_out must have q's shape {tuple(q.shape)}, got {tuple(q_out.shape)}")
-                ldo = self._heads(q_out, "q_out", heads)
-            po = self._values(q_out, "q_out")
+                ldo, po = self._output(q_out, "q_out", q)
         elif q_out is not None:
             raise ValueError("q_out without q")
         if starts is not None:
@@ -252,8 +262,8 @@ class PagedKVCache:
         if rotary is not None and (rotary.head_dim != self.head_dim or rotary.device != self.device):
             raise ValueError(f"rotary is for heads of {rotary.head_dim} on {rotary.device}")
         if n:
-            _call("otf_paged_append", self.device, self._ref, None if rotary is None else rotary._ref, pq, ldq, po, ldo,
-                  heads, pk, ldk, pv, ldv, ps, pp, n)
+            _call(_native.lib().otf_paged_append, dev, self._ref, None if rotary is None else rotary._ref, pq, ldq, po,
+                  ldo, heads, pk, ldk, pv, ldv, ps, pp, n)
         return q_out
 
     def _plan_append(self, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor) -> tuple:
@@ -288,24 +298,24 @@ class PagedKVCache:
         if plan is None:
             plan = self._remember(self._attend_plans, key, self._plan_attend(q, weights))
         tokens, heads, ldq, bytes_ = plan
-        pq, ldo = self._values(q, "q"), heads * self.head_dim
+        pq, dev = q.data_ptr(), self.device
+        if q.dtype is not self.dtype or q.device != dev or pq & 15:
+            self._refuse(q=q)
         if out is None:
             out = torch.empty_like(q)
+            ldo, po = heads * self.head_dim, out.data_ptr()
         else:
-            if out.shape != q.shape:
-                raise ValueError(f"out must have q's shape {tuple(q.shape)}, got {tuple(out.shape)}")
-            ldo = self._heads(self._flat(out, "out"), "out", heads)
-        po = self._values(out, "out")
-        if po == pq:
-            raise ValueError("out must not be q")
+            ldo, po = self._output(out, "out", q)
+            if po == pq:
+                raise ValueError("out must not be q")
         pw, ldw = None, 0
         if weights is not None:
             ldw = self._weights(weights, "weights", self.capacity)
             pw = weights.data_ptr()
         # from the caching allocator, for this call alone: calls on two streams, or in two captured
         # graphs, share nothing
-        ws = torch.empty(bytes_, dtype=torch.uint8, device=self.device)
-        _call("otf_paged_attn", self.device, self._ref, pq, ldq, heads, tokens,
+        ws = torch.empty(bytes_, dtype=torch.uint8, device=dev)
+        _call(_native.lib().otf_paged_attn, dev, self._ref, pq, ldq, heads, tokens,
               self._scale if scale is None else float(scale), po, ldo, pw, ldw, ws.data_ptr(), bytes_)
         return out
 
@@ -355,7 +365,7 @@ class PagedKVCache:
             raise ValueError(f"budget {budget} (of {to.capacity}) and recent {recent} do not fit")
         ldo = self._weights(weights_out, "weights_out", budget)
         kept = torch.empty((self.batch, self.kv_heads, budget), dtype=torch.int32, device=self.device)
-        _call("otf_paged_evict", self.device, self._ref, to._ref, weights.data_ptr(), ldw, weights_out.data_ptr(), ldo,
+        _call(_native.lib().otf_paged_evict, self.device, self._ref, to._ref, weights.data_ptr(), ldw, weights_out.data_ptr(), ldo,
               budget, recent, kept.data_ptr(), to.lengths.data_ptr())
         return kept
 
@@ -381,10 +391,9 @@ class PagedKVCache:
         return t.as_strided((t.shape[0] * t.shape[1], t.shape[2], t.shape[3]), (row, t.stride(2), t.stride(3)))
 
 
-def _call(name: str, dev: torch.device, *args) -> None:
+def _call(fn, dev: torch.device, *args) -> None:
     """An entry point of the library with the device current and its current stream as the last
     argument (the raw handle: torch.cuda.current_stream would make a Stream object)."""
-    fn = getattr(_native.lib(), name)
     index = dev.index
     if torch.cuda.current_device() == index:
         st = fn(*args, torch._C._cuda_getCurrentRawStream(index))
@@ -392,4 +401,4 @@ def _call(name: str, dev: torch.device, *args) -> None:
         with torch.cuda.device(index):
             st = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if st:
-        _native._check(st, name)
+        _native._check(st, fn.__name__)

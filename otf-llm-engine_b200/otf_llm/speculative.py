@@ -69,7 +69,7 @@ def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, *,
     accepted = torch.empty(batch, dtype=torch.int32, device=dev)
     # a large call's scratch, for this call alone and on its stream
     ws = torch.empty(bytes_, dtype=torch.uint8, device=dev) if bytes_ else None
-    _call("otf_verify_drafts", dev, pt, seq_t, ld_t, pd, seq_d, ld_d, ptok, ld_tok, pu, ld_u, pn, ld_n, each, one, pc,
+    _call(_native.lib().otf_verify_drafts, dev, pt, seq_t, ld_t, pd, seq_d, ld_d, ptok, ld_tok, pu, ld_u, pn, ld_n, each, one, pc,
           tokens.data_ptr(), accepted.data_ptr(), batch, drafts, vocab, ws.data_ptr() if bytes_ else None, bytes_)
     return tokens, accepted
 
