@@ -525,9 +525,9 @@ OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* q, int64_t 
  * budget - recent of the largest weights (ties: the lower place; a NaN counts as the largest).
  * The order stays.  kept: int32 [batch, kv_heads, budget], the places kept, then -1.  The kept
  * keys and values go to the same head's tokens 0, 1, ... of `to`, whose page_table holds pages
- * that hold nothing of `from` (in the same pools or others); or from's pools, table, weights and
- * lengths are given again, and the cache is cut in place (its pages then belong to one sequence
- * each).  `to` has from's geometry
+ * that hold nothing of `from` (in the same pools or others); or from's pools, table and
+ * weights are given again, and the cache is cut in place (its pages then belong to one sequence
+ * each; lengths_out may be from's lengths, or another vector while other layers still need those).  `to` has from's geometry
  * (kv_heads, head_dim, batch, dtype, page_size) and room for budget tokens.  weights (fp32
  * [batch, kv_heads, ldw]) go along to weights_out ([batch, kv_heads, ldw_out], may be weights),
  * zero behind the kept ones (in place: up to the old length).  lengths_out[b] = min(lengths[b],

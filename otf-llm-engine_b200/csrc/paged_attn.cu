@@ -9,16 +9,22 @@
 // products are 4 x head_dim x rows flops on them, below the matrix pipe's rate up to some tens
 // of rows.  So the aim is to keep enough loads in flight on every SM.
 //
-// Split.  An item is a (sequence, KV head, block of 16 or 32 query rows); its tokens that every
-// row sees (0 .. length) are cut into chunks, and all items' chunks, in order, are dealt out evenly
-// to a fixed grid in contiguous runs, whatever the lengths are: a run may cross items, and an
-// item may be shared by several CTAs, which then leave parts that a second kernel joins in order.
-// Neither launch depends on lengths (they are read on the device), so a step can be captured.
+// Split.  An item is a (sequence, KV head, block of up to 32 query rows); its tokens are cut into
+// chunks, and all items' chunks, in order, are dealt out evenly to a fixed grid in contiguous runs,
+// whatever the lengths are: a run may cross items, and an item may be shared by several CTAs, which
+// then leave parts that a second kernel joins in order.  Neither launch depends on lengths (they are
+// read on the device), so a step can be captured.
 //
 // Inside a CTA each warp is on its own: it takes 16 (head_dim 64: 32) tokens of every chunk through its
 // own ring of shared-memory stages, filled by 16-byte asynchronous copies some chunks ahead and
-// across items, and runs q k and p v on m16n8k16 matrix instructions, the row block's queries
-// held in registers.  The warps meet only at an item's end.
+// across items, and runs q k and p v on m16n8k16 matrix instructions.  The warps meet only at an
+// item's end.  The asynchronous 5th-generation products (128 rows at least) would be used to a
+// sixteenth here; these keep pace with the loads up to 16 rows.
+//
+// Measured (16-bit, head_dim 128, 8 KV heads; the whole call in a graph): one sequence of 131071
+// tokens, 64 heads, 537 MB, 87.8 us = 6.1 TB/s (k_paged_attn by itself 83 us, 6.4 TB/s); 64 sequences
+// of 127 to 8190 tokens, 1.09 GB, 181.7 us = 6.0 TB/s; one of 700 tokens 8.3 us, of which the joining
+// launch is 3; 16 of 62 to 4001 tokens, 20 rows an item, 39 us without and 55.6 us with weights.
 //
 // The newest keys, which not every row sees, are masked in the steps that hold them; what they hold
 // cannot reach the other rows (see the loop).

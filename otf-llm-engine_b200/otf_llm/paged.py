@@ -336,7 +336,8 @@ class PagedKVCache:
         return tokens, heads, ldq, n
 
     def evict(self, weights: torch.Tensor, budget: int, recent: int, *, to: Optional["PagedKVCache"] = None,
-              weights_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+              weights_out: Optional[torch.Tensor] = None, lengths_out: Optional[torch.Tensor] = None
+              ) -> torch.Tensor:
         """Cut every sequence longer than ``budget`` tokens to it (otf_paged_evict), for each KV head
         by itself: the ``recent`` last tokens stay, and of the others those of the largest
         ``weights`` (as ``attend`` adds them up; ties: the earlier token), in their order.
@@ -345,7 +346,10 @@ class PagedKVCache:
         cut, and a sequence's pages behind its first budget / page_size (rounded up) may be handed on.  With
         ``to``, a cache of the same geometry whose table names other pages, the kept tokens go there
         (its ``lengths`` are set, and ``weights_out``, fp32 [batch, kv_heads, at least budget], is
-        written), and this one stays as it is.  Returns int32 [batch, kv_heads, budget]: the
+        written), and this one stays as it is.
+
+        ``lengths_out`` (int32 [batch]) takes the new lengths instead of the cut cache's ``lengths``:
+        layers that share one lengths vector give another one for all but the last.  Returns int32 [batch, kv_heads, budget]: the
         places that were kept, then -1."""
         ldw = self._weights(weights, "weights", self.capacity)
         budget, recent = int(budget), int(recent)
@@ -364,9 +368,13 @@ class PagedKVCache:
         if not 0 < budget <= to.capacity or not 0 <= recent <= budget:
             raise ValueError(f"budget {budget} (of {to.capacity}) and recent {recent} do not fit")
         ldo = self._weights(weights_out, "weights_out", budget)
+        if lengths_out is None:
+            lengths_out = to.lengths
+        elif to is not self and lengths_out.data_ptr() == self.lengths.data_ptr():
+            raise ValueError("lengths_out must not be the source's lengths with to")
         kept = torch.empty((self.batch, self.kv_heads, budget), dtype=torch.int32, device=self.device)
         _call(_native.lib().otf_paged_evict, self.device, self._ref, to._ref, weights.data_ptr(), ldw, weights_out.data_ptr(), ldo,
-              budget, recent, kept.data_ptr(), to.lengths.data_ptr())
+              budget, recent, kept.data_ptr(), self._vector(lengths_out, "lengths_out", self.batch))
         return kept
 
     def advance(self, tokens: int = 1) -> None:

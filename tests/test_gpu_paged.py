@@ -509,6 +509,25 @@ def test_evict_long_sequence(cuda_dev):
     check_evict(cuda_dev, [5000], 700, 100, 64, 2, 64, torch.float16, "token", False)
 
 
+def test_evict_layers_that_share_their_lengths(cuda_dev):
+    from otf_llm.paged import PagedKVCache
+    first, pools, table, g = make(cuda_dev, [90, 20, 41], 16, 2, 64, torch.float16)
+    second = PagedKVCache(first.k_pages.clone(), first.v_pages.clone(), first.page_table, first.lengths)
+    spare = torch.zeros(3, dtype=torch.int32, device=cuda_dev)
+    weights = [torch.rand(3, 2, first.capacity, generator=g).to(cuda_dev) for _ in range(2)]
+    want = [[[ref.evict(w[b, h].cpu(), n, 40, 8) for h in range(2)] for b, n in enumerate((90, 20, 41))] for w in weights]
+    for i, cache in enumerate((first, second)):
+        kept = cache.evict(weights[i], 40, 8, lengths_out=spare if i == 0 else None).cpu()
+        assert first.lengths.tolist() == ([90, 20, 41] if i == 0 else [40, 20, 40])
+        for b in range(3):
+            for h in range(2):
+                assert kept[b, h, :len(want[i][b][h])].tolist() == want[i][b][h]
+                for j, s in enumerate(want[i][b][h]):
+                    at, src = ref.place(table, 16, b, j), ref.place(table, 16, b, s)
+                    assert torch.equal(cache.k_pages[at][h].cpu(), pools[0][src][h])
+    assert spare.tolist() == [40, 20, 40] and flag() == 0
+
+
 @pytest.mark.parametrize("batch,kv,lengths,budget,recent", [
     (1, 3, [20001], 3000, 17), (1, 2, [70003], 9000, 0), (2, 8, [33000, 8193], 8192, 8000), (50, 4, [9000, 100, 8200], 500, 60),
     (1, 1, [300000], 1000, 999)])
