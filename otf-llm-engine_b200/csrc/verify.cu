@@ -74,15 +74,15 @@ __device__ __forceinline__ float ex2(float x) {
 // 0, or from 1e-20 on (log2(e) / T and its product with a difference of logits stay finite).
 __host__ __device__ __forceinline__ bool temperature_ok(float T) { return T == 0.0f || (T >= 1e-20f && T <= 1e20f); }
 
-// Four consecutive logits of a row, -inf behind its end.  Rows that are not 16-byte aligned are read
+// Four consecutive values of a row, `pad` behind its end.  Rows that are not 16-byte aligned are read
 // value by value by the same threads, so that a row's sums do not depend on where it lies.
-__device__ __forceinline__ float4 logits4(const float* x, int i, int end, bool aligned) {
+__device__ __forceinline__ float4 logits4(const float* x, int i, int end, bool aligned, float pad = -INFINITY) {
   if (aligned && i + 4 <= end) return __ldcs(reinterpret_cast<const float4*>(x + i));
   float4 v;
-  v.x = i < end ? __ldcs(x + i) : -INFINITY;
-  v.y = i + 1 < end ? __ldcs(x + i + 1) : -INFINITY;
-  v.z = i + 2 < end ? __ldcs(x + i + 2) : -INFINITY;
-  v.w = i + 3 < end ? __ldcs(x + i + 3) : -INFINITY;
+  v.x = i < end ? __ldcs(x + i) : pad;
+  v.y = i + 1 < end ? __ldcs(x + i + 1) : pad;
+  v.z = i + 2 < end ? __ldcs(x + i + 2) : pad;
+  v.w = i + 3 < end ? __ldcs(x + i + 3) : pad;
   return v;
 }
 
@@ -277,8 +277,9 @@ struct __align__(8) Leader {
 
 // A warp's part of the race over entries [i0, end) in pieces of 128, `step` apart, U of them
 // requested at a time.  An entry is weighed with the hardware's exponential first, whose error is
-// far below the margin 2^-16; only what may beat the warp's leader by then is computed with care
-// (some 10 entries), so the loop stays near 25 instructions per entry.  y null: p alone.
+// below the margin 2^-15 (2^-23 of the exponent, which is 127 at most); only what may beat the warp's
+// leader by then is computed with care (some 10 entries), so the loop takes 14 instructions per entry.
+// Behind the end the noise is infinite.  y null: p alone.
 template <int U>
 __device__ __forceinline__ Leader race(const Sequence& q, const Pick& k, const float* y, int out_of, int i0, int end, int step) {
   const int lane = threadIdx.x & 31;
@@ -294,7 +295,7 @@ __device__ __forceinline__ Leader race(const Sequence& q, const Pick& k, const f
     for (int j = 0; j < U; ++j) {
       const int i = min(i0 + j * step, end) + 4 * lane;  // behind the end: -inf without a read
       vx[j] = logits4(x, i, end, ax);
-      ve[j] = logits4(e, i, end, ae);
+      ve[j] = logits4(e, i, end, ae, INFINITY);
       vy[j] = y ? logits4(y, i, end, ay) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
 #pragma unroll
@@ -306,16 +307,15 @@ __device__ __forceinline__ Leader race(const Sequence& q, const Pick& k, const f
 #pragma unroll
       for (int z = 0; z < 4; ++z) {
         const float dx = fx[z] - k.xm, dy = fy[z] - k.ym;
-        const float p = ex2(fmaxf(fmaf(dx, q.c_hi, dx * q.c_lo), -200.0f)) * k.xi;
-        float r = 0.0f;
-        if (y) r = ex2(fmaxf(fmaf(dy, q.c_hi, dy * q.c_lo), -200.0f)) * k.yi;
-        may[z] = fmaf(p + r, 0x1p-16f, p - r) > bar * fe[z] && i + z != out_of && i + z < end;
+        const float p = ex2(dx * q.c_hi) * k.xi;                 // a NaN is never taken
+        const float r = y ? fmaxf(ex2(dy * q.c_hi), 0.0f) * k.yi : 0.0f;  // and counts as 0 here
+        may[z] = fmaf(p + r, 0x1p-15f, p - r) > bar * fe[z];
         any |= may[z];
       }
       if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
         for (int z = 0; z < 4; ++z)
-          if (may[z]) {
+          if (may[z] && i + z != out_of) {
             // products that round by themselves: equal rows leave exactly nothing
             float w = __fmul_rn(exp_scaled(fx[z] - k.xm, q.c_hi, q.c_lo), k.xi);
             if (y) w = __fsub_rn(w, __fmul_rn(exp_scaled(fy[z] - k.ym, q.c_hi, q.c_lo), k.yi));
