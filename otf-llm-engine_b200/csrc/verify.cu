@@ -34,11 +34,14 @@ constexpr int kVerifyWarps = kVerifyThreads / 32;
 constexpr int kVerifyCluster = 16;   // CTAs of a sequence at most (k_verify)
 constexpr int kPickThreads = 512;
 constexpr int kRaceCluster = 8;      // CTAs of a sequence at most (k_verify_race)
-// Logits of all rows up to which one launch is taken.  Measured, eager calls one after another, one launch
-// against three: 16 sequences x 5 rows of 32000 (2.4M) 14.2 us against 21.0, 32 sequences (4.9M) 16.5
-// against 21.1, 64 (9.8M) 24.2 against 24.4; 4 x 11 rows of 128256 (5.4M) 30.8 against 26.6, 16 x 8
-// (15.7M) 24.9 against 18.4.
-constexpr int64_t kVerifyOneLaunch = 4 << 20;
+// One launch is taken up to 6M logits in all rows, or 8M of at most kVerifyFew sequences; its CTAs then
+// have 32 warps where a CTA's slice of the rows is large (kVerifyLarge logits), else 8.  Measured,
+// eager calls one after another, one launch against three: 16 sequences x 5 rows of 32000 (2.4M) 14.1 us
+// against 20.8, 32 sequences (4.9M) 16.1 against 21.0, 64 (9.8M) 23.7 against 24.0; 4 x 11 rows of 128256
+// (5.4M) 19.8 against 25.8, 8 x 11 (10.8M) 37.3 against 30.1, 16 x 8 (15.7M) 25.0 against 18.3.  32 warps
+// against 8: one sequence, 9 rows of 128256, 17.4 us against 22.5; 8 x 5 rows of 32000 19.0 against 14.1.
+constexpr int kVerifyFew = 4;
+constexpr int64_t kVerifyLarge = 1 << 14;
 
 // Set when a sequence has no token to draw, or an argument on the device is out of range.
 __device__ int g_verify_device_error;
@@ -336,9 +339,8 @@ __device__ __forceinline__ Leader race(const Sequence& q, const Pick& k, const f
 
 // The race over a cluster: CTA `rank` of `ctas` runs over entries [i0 of its warps, end), the leaders
 // meet in every CTA.  Returns the winner, or -1.  The caller's cluster runs by now.
-template <int U>
+template <int U, int W>
 __device__ __forceinline__ int64_t race_cluster(const Sequence& q, const Pick& k, int i0, int end, int step, int rank, int ctas) {
-  constexpr int W = kVerifyWarps;
   __shared__ Leader s_lead[W];
   __shared__ Leader s_all[2][kVerifyCluster];
   const int tid = threadIdx.x;
@@ -364,9 +366,10 @@ __device__ __forceinline__ int64_t race_cluster(const Sequence& q, const Pick& k
 }
 
 // All in one launch: a cluster of `ctas` CTAs per sequence.
-__global__ void __launch_bounds__(kVerifyThreads, 3) k_verify(VerifyArgs a, int ctas) {
-  constexpr int W = kVerifyWarps;
-  __shared__ RowPart s_part[kVerifyMaxRows][W];              // this slice's rows, by warp
+template <int W>
+__global__ void __launch_bounds__(32 * W, 1024 / (32 * W) < 3 ? 1024 / (32 * W) : 3) k_verify(VerifyArgs a, int ctas) {
+  constexpr int kSlots = 8;
+  __shared__ RowPart s_part[kVerifyMaxRows][kSlots];         // this slice's rows, by slot
   __shared__ RowPart s_cta[kVerifyMaxRows][kVerifyCluster];  // the rows, by CTA
   __shared__ RowPart s_row[kVerifyMaxRows];
   __shared__ Pick s_pick;
@@ -376,7 +379,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 3) k_verify(VerifyArgs a, int 
   const Sequence q(a, b);
   const int rows = q.rows();
   if (rows == 0) {
-    if (rank == 0) write_tokens(q, 0, -1, tid, kVerifyThreads);
+    if (rank == 0) write_tokens(q, 0, -1, tid, 32 * W);
     return;  // as the whole cluster does
   }
   cluster_arrive_relaxed();
@@ -386,7 +389,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 3) k_verify(VerifyArgs a, int 
   // The slice's segments go round `slots` warps, the same ones in every row; several rows at once
   // where the slice has few segments.
   const int segs = (a.slice + kVerifySeg - 1) / kVerifySeg;
-  const int slots = segs >= 8 ? 8 : segs >= 4 ? 4 : segs >= 2 ? 2 : 1;
+  const int slots = segs >= kSlots ? kSlots : segs >= 4 ? 4 : segs >= 2 ? 2 : 1;
   for (int r = warp / slots; r < rows; r += W / slots) {
     const float* x = q.row(r);
     RowPart p = no_part();
@@ -413,8 +416,8 @@ __global__ void __launch_bounds__(kVerifyThreads, 3) k_verify(VerifyArgs a, int 
   __syncthreads();
   const Pick k = s_pick;
   const int64_t last = q.T == 0.0f ? greedy(s_row[k.taken])
-                                   : race_cluster<2>(q, k, s0 + 128 * warp, s1, 128 * W, rank, ctas);
-  if (rank == 0) write_tokens(q, k.taken, last, tid, kVerifyThreads);
+                                   : race_cluster<2, W>(q, k, s0 + 128 * warp, s1, 128 * W, rank, ctas);
+  if (rank == 0) write_tokens(q, k.taken, last, tid, 32 * W);
 }
 
 // Step 1 alone: grid (blocks of 8 segments, row groups, batch), a warp per segment.  64 sequences of 1
@@ -481,13 +484,30 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) k_verify_race(VerifyArgs a,
   cluster_arrive_relaxed();
   const Sequence q(a, b);
   cluster_wait();  // all CTAs of the cluster run
-  const int64_t last = race_cluster<4>(q, k, 4 * (rank * kVerifyThreads + (threadIdx.x & ~31)), a.vocab,
+  const int64_t last = race_cluster<4, kVerifyWarps>(q, k, 4 * (rank * kVerifyThreads + (threadIdx.x & ~31)), a.vocab,
                                        4 * kVerifyThreads * ctas, rank, ctas);
   if (rank == 0) write_tokens(q, k.taken, last, threadIdx.x, kVerifyThreads);
 }
 
+template <int W>
+static cudaError_t launch_verify(const VerifyArgs& a, int batch, int ctas, cudaStream_t s) {
+  static std::atomic<bool> done[64];  // clusters of 16 are beyond the portable size
+  int dev;
+  bool needs;
+  cudaError_t e = needs_opt_in(done, dev, needs);
+  if (e != cudaSuccess) return e;
+  if (needs) {
+    e = cudaFuncSetAttribute(k_verify<W>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    opted_in(done, dev);
+  }
+  return launch_pdl(k_verify<W>, dim3((unsigned)(batch * ctas)), dim3(32 * W), 0, s, (unsigned)ctas, a, ctas);
+}
+
 // One launch, or the workspace of three.
-static bool one_launch(int64_t batch, int64_t rows, int64_t vocab) { return batch * rows <= kVerifyOneLaunch / vocab; }
+static bool one_launch(int64_t batch, int64_t rows, int64_t vocab) {
+  return batch * rows * vocab <= (batch <= kVerifyFew ? 8ll << 20 : 6ll << 20);
+}
 
 }  // namespace otf
 
@@ -559,31 +579,22 @@ extern "C" OTF_API int otf_verify_drafts(const float* target, int64_t target_seq
   a.accepted = accepted;
   a.drafts = (int)drafts;
   a.vocab = (int)vocab;
+  const int64_t rows = drafts + 1 + (draft ? drafts : 0);
   if (bytes == 0) {
-    static std::atomic<bool> done[64];  // clusters of 16 are beyond the portable size
-    int dev;
-    bool needs;
-    cudaError_t e = otf::needs_opt_in(done, dev, needs);
-    if (e != cudaSuccess) return set_cuda_error(e);
-    if (needs) {
-      e = cudaFuncSetAttribute(otf::k_verify, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      if (e != cudaSuccess) return set_cuda_error(e);
-      otf::opted_in(done, dev);
-    }
     // CTAs per sequence: 16 (of such clusters 14 run at once), 8, or as many as all run at once, three
     // on an SM; no more than the vocabulary has segments
     int ctas = batch <= 8 ? 16 : 8;
     while (ctas > 1 && (batch * ctas > 3 * 148 || (int64_t)(ctas - 1) * otf::kVerifySeg >= vocab)) ctas /= 2;
     a.slice = (int)(((vocab + ctas - 1) / ctas + 3) & ~3ll);
-    return set_cuda_error(otf::launch_pdl(otf::k_verify, dim3((unsigned)(batch * ctas)), dim3(otf::kVerifyThreads), 0, s,
-                                          (unsigned)ctas, a, ctas));
+    const bool large = batch <= otf::kVerifyFew && rows * a.slice >= otf::kVerifyLarge;
+    return set_cuda_error(large ? otf::launch_verify<32>(a, (int)batch, ctas, s) : otf::launch_verify<8>(a, (int)batch, ctas, s));
   }
   a.segs = (int)((vocab + otf::kVerifySeg - 1) / otf::kVerifySeg);
   a.picks = static_cast<otf::Pick*>(workspace);
   a.parts = reinterpret_cast<otf::RowPart*>(static_cast<char*>(workspace) +
                                             otf::align_up(batch * (int64_t)sizeof(otf::Pick), 256));
   // row groups: one per row while all of their CTAs fit the GPU at once, else 4
-  const int64_t rows = drafts + 1 + (draft ? drafts : 0), blocks = (a.segs + otf::kVerifyWarps - 1) / otf::kVerifyWarps;
+  const int64_t blocks = (a.segs + otf::kVerifyWarps - 1) / otf::kVerifyWarps;
   const int64_t groups = std::min<int64_t>(rows, batch * blocks * rows <= 4 * 148 ? rows : 4);
   cudaError_t e = otf::launch_pdl(otf::k_verify_rows, dim3((unsigned)blocks, (unsigned)groups, (unsigned)batch),
                                   dim3(otf::kVerifyThreads), 0, s, 1u, a);

@@ -51,6 +51,16 @@ def test_verify_matches_definition(batch, drafts, vocab, drafted, temperature, c
     check(cuda_dev, *inputs(batch, drafts, vocab, drafted, seed=batch * 100 + drafts + vocab), temperature)
 
 
+@pytest.mark.parametrize("temperature", [0.0, 0.8])
+@pytest.mark.parametrize("batch,drafts,vocab,drafted", [(1, 4, 128256, True), (3, 2, 100001, False), (40, 2, 40001, True),
+                                                        (9, 1, 300000, False), (700, 1, 50, True), (2, 32, 70000, False)])
+def test_verify_large_calls(batch, drafts, vocab, drafted, temperature, cuda_dev):
+    """Calls on either side of the switches between one launch and three, and between cluster sizes."""
+    args = inputs(batch, drafts, vocab, drafted, seed=vocab)
+    counts = [(3 * b) % (drafts + 1) for b in range(batch)]
+    check(cuda_dev, *args, temperature, counts=None if batch % 2 else counts)
+
+
 def test_verify_counts_and_temperatures_of_each_sequence(cuda_dev):
     args = inputs(6, 4, 3001, True, seed=5)
     check(cuda_dev, *args, [0.0, 1.0, 0.3, 0.0, 2.0, 1.0], counts=[4, 0, 2, 3, 1, 4])
