@@ -453,10 +453,11 @@ OTF_API int otf_attn_decode_noalloc(const void* q, const void* k_cache, const vo
  * marks a place of the batch without a sequence, which every call leaves as it is.
  * dtype: OTF_DTYPE_F16 or OTF_DTYPE_BF16 (queries and outputs have the cache's type).
  * head_dim 64 or 128; at most 4096 sequences; max_pages * page_size at most 2^30.
- * A sequence whose tokens do not fit in max_pages pages, or (in otf_paged_append and
- * otf_paged_evict) a token whose page is not in [0, n_pages), is left out: nothing of it is
- * written and the otf_device_error flag is raised.  In otf_paged_attn tokens of such a page
- * read as zeros, and the flag is raised.
+ * What does not fit raises the otf_device_error flag.  otf_paged_append leaves out each new
+ * token behind the last of max_pages pages or of a page not in [0, n_pages), with its query;
+ * otf_paged_attn and otf_paged_evict leave out a sequence of more than max_pages pages whole;
+ * tokens of a page not in [0, n_pages) read as zeros in otf_paged_attn and stay where they are
+ * in otf_paged_evict.
  */
 typedef struct otf_paged_cache {
   void* k_pages;

@@ -110,11 +110,11 @@ class PagedKVCache:
     page_table: int32 [batch, max_pages], whose row b names the pages of sequence b in order;
     lengths: int32 [batch], the tokens that each sequence has cached, negative for a place
     without a sequence (left as it is by every call).  The tensors stay the caller's and are
-    changed in place: pages are handed out by writing the table, and ``advance`` counts a step's tokens once every layer has
-    appended them (layers may share table and lengths).
+    changed in place: pages are handed out by writing the table, and ``advance`` counts a step's
+    tokens once every layer has appended them (layers may share table and lengths).
 
-    Sequences that do not fit, and pages outside the pool, are left out on the device and raise
-    the ``_native.device_error`` flag (see include/otf_b200.h)."""
+    Tokens and sequences that do not fit, and pages outside the pool, are left out on the device
+    and raise the ``_native.device_error`` flag (see include/otf_b200.h)."""
 
     def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor):
         for name, t in (("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table), ("lengths", lengths)):
@@ -349,8 +349,8 @@ class PagedKVCache:
         written), and this one stays as it is.
 
         ``lengths_out`` (int32 [batch]) takes the new lengths instead of the cut cache's ``lengths``:
-        layers that share one lengths vector give another one for all but the last.  Returns int32 [batch, kv_heads, budget]: the
-        places that were kept, then -1."""
+        layers that share one lengths vector give another one for all but the last.  Returns int32
+        [batch, kv_heads, budget]: the places that were kept, then -1."""
         ldw = self._weights(weights, "weights", self.capacity)
         budget, recent = int(budget), int(recent)
         if to is None:
