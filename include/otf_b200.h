@@ -553,10 +553,10 @@ OTF_API int otf_paged_evict(const otf_paged_cache* from, const otf_paged_cache* 
  * counts: device int32 [batch], the drafted tokens of each sequence (0..drafts), or NULL: all
  * have `drafts` (0..32).  out_tokens: int64 [batch, drafts + 1], the taken tokens, the drawn
  * one, then -1; accepted: int32 [batch].  Temperatures are 0 or in 1e-20 .. 1e20; a NaN among
- * the logits counts as -inf.  A sequence without a token of positive weight, or
- * with a count or temperature out of range, gets -1 and raises the otf_device_error flag; so
- * does a drafted token outside the vocabulary, which is refused.  Where max(p - q, 0) holds
- * nothing, p is drawn from.  At most 65535 sequences and a vocabulary of 2^30.  workspace:
+ * the logits counts as -inf.  A sequence without a token of positive weight (temperature 0: of a
+ * logit above -inf), or with a count or temperature out of range, gets -1 and raises the
+ * otf_device_error flag; so does a drafted token outside the vocabulary, which is refused.  Where
+ * max(p - q, 0) holds nothing, p is drawn from.  At most 65535 sequences and a vocabulary of 2^30.  workspace:
  * otf_verify_workspace_bytes(...) (0 for small calls, then it may be NULL), 256-byte aligned, need
  * not be cleared; two calls that may run at the same time need one each.  Beside
  * otf_i8_head_argmax, the greedy pick of one row.

@@ -164,13 +164,13 @@ __device__ __forceinline__ RowPart read_segment(const Sequence& q, const float* 
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   float s = 0.0f;
   int at = INT_MAX;
-  if (q.T == 0.0f) {  // the first of the largest
+  if (q.T == 0.0f) {  // the first of the largest, none among -inf alone
 #pragma unroll
     for (int z = N - 1; z >= 0; --z) {
       const float e[4] = {v[z].x, v[z].y, v[z].z, v[z].w};
 #pragma unroll
       for (int w = 3; w >= 0; --w)
-        if (e[w] == m && i0 + z * 128 + w < end) at = i0 + z * 128 + w;
+        if (e[w] == m && m > -INFINITY) at = i0 + z * 128 + w;
     }
     at = __reduce_min_sync(0xffffffffu, at);
   } else {

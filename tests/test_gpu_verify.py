@@ -107,6 +107,22 @@ def test_verify_nan_logits_count_as_masked(cuda_dev):
         assert flag() == 0 and all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("vocab", [1, 500, 700001])
+def test_verify_greedy_of_nothing_but_masked_logits(vocab, cuda_dev):
+    """A row of -inf, or of NaN, or of both holds no token at temperature 0 either: a drafted one is refused
+    there, and none follows; sequences with a logit above them are as without masks."""
+    from otf_llm.speculative import verify_drafts
+    target = torch.full((4, 3, vocab), -float("inf"))
+    target[1, :, ::2] = float("nan")
+    target[2] = float("nan")
+    target[3, :, vocab // 2] = -1e30
+    tokens = torch.full((4, 2), vocab // 2)
+    tokens[:3] = 0
+    got, accepted = verify_drafts(target.to(cuda_dev), tokens.to(cuda_dev), temperature=0.0)
+    assert flag() == 1
+    assert got.tolist() == [[-1] * 3] * 3 + [[vocab // 2] * 3] and accepted.tolist() == [0, 0, 0, 2]
+
+
 def test_verify_equal_distributions(cuda_dev):
     """Draft and target the same: all taken; one refused all the same (u = 1 cannot be below) leaves nothing
     of p - q, and p is drawn from."""
