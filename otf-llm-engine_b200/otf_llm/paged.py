@@ -52,6 +52,8 @@ def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling: Optional[dic
     unknown = [k for k in scaling if k not in need + may + ("rope_type", "type", "rope_theta")]
     if missing or unknown:
         raise ValueError(f"rope_type {kind!r}: missing {missing}, not supported {unknown}")
+    if scaling.get("rope_theta") not in (None, theta):
+        raise ValueError(f"scaling's rope_theta is {scaling['rope_theta']}, theta {theta}")
     if kind == "default":
         return f, 1.0
     factor = float(scaling["factor"])

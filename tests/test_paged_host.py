@@ -42,6 +42,17 @@ def test_frequencies_refuse_what_they_do_not_know():
     assert rope_frequencies(0)[0].numel() == 0
 
 
+def test_frequencies_refuse_two_thetas():
+    """Dicts that carry rope_theta beside the scaling: it has to be the theta given."""
+    from otf_llm.paged import rope_frequencies
+    linear = {"rope_type": "linear", "factor": 2.0}
+    want = rope_frequencies(64, 500000.0, linear)[0]
+    assert torch.equal(rope_frequencies(64, 500000.0, dict(linear, rope_theta=500000))[0], want)
+    for kind in (linear, {"rope_type": "default"}):
+        with pytest.raises(ValueError, match="rope_theta"):
+            rope_frequencies(64, 10000.0, dict(kind, rope_theta=500000.0))
+
+
 def test_decoders_take_scaled_rotary_tables():
     """rope_table without scaling is HF's default table bit for bit; with it HF's scaled one, within the fp32
     angles that HF computes (an ulp of the angle, and one fp16 rounding)."""
