@@ -16,6 +16,8 @@
 // the steps' results exchanged through distributed shared memory.  Many take three, whose grids
 // fill the GPU in every step whatever the sequences' drafts are: k_verify_rows, k_verify_pick,
 // k_verify_race.  What a step computes is shared, and so is the order of its sums within a row.
+#include <cfloat>
+
 #include <algorithm>
 
 #include "paged.cuh"
@@ -33,7 +35,8 @@ constexpr int kVerifyThreads = 256;
 constexpr int kVerifyWarps = kVerifyThreads / 32;
 constexpr int kVerifyCluster = 16;   // CTAs of a sequence at most (k_verify)
 constexpr int kPickThreads = 512;
-constexpr int kRaceCluster = 8;      // CTAs of a sequence at most (k_verify_race)
+constexpr int kRaceResident = 148 * 4;  // CTAs of k_verify_race that run at once
+constexpr int kRaceLeast = 1024;     // entries of a CTA at least (k_verify_race)
 // One launch is taken up to 6M logits in all rows, or 8M of at most kVerifyFew sequences; its CTAs then
 // have 32 warps where a CTA's slice of the rows is large (kVerifyLarge logits), else 8.  Measured,
 // eager calls one after another, one launch against three: 16 sequences x 5 rows of 32000 (2.4M) 14.1 us
@@ -57,6 +60,8 @@ struct __align__(16) RowPart {
 struct __align__(16) Pick {
   int taken, refused, drafted, out_of;  // taken -1: nothing to draw
   float xm, xi, ym, yi;
+  unsigned long long lead;  // k_verify_race: the leader so far (see packed), 0 at first
+  int done, pad;            // and its CTAs that are done
 };
 
 // exp(d / T) for d <= 0, with c = log2(e) / T in two floats: the exponent is split into its
@@ -280,18 +285,19 @@ struct __align__(8) Leader {
 
 // A warp's part of the race over entries [i0, end) in pieces of 128, `step` apart, U of them
 // requested at a time.  An entry is weighed with the hardware's exponential first, whose error is
-// below the margin 2^-15 (2^-23 of the exponent, which is 127 at most); only what may beat the warp's
-// leader by then is computed with care (some 10 entries), so the loop takes 14 instructions per entry.
-// Behind the end the noise is infinite.  y null: p alone.
+// below the margin 2^-15 (2^-23 of the exponent, which is 127 at most); only what may beat the
+// bar, a score that some entry of the CTA's has at least (shared_bar, 0 at first), is computed with care, so
+// the loop takes 14 instructions per entry.  Behind the end the noise is infinite.  y null: p alone.
 template <int U>
-__device__ __forceinline__ Leader race(const Sequence& q, const Pick& k, const float* y, int out_of, int i0, int end, int step) {
+__device__ __forceinline__ Leader race(const Sequence& q, const Pick& k, const float* y, int out_of, int i0, int end, int step,
+                                       uint32_t* shared_bar) {
   const int lane = threadIdx.x & 31;
   const float* x = q.row(k.taken);
   const float* e = q.a.noise + q.b * q.a.ldn;
   const bool ax = (reinterpret_cast<uintptr_t>(x) & 15) == 0, ay = (reinterpret_cast<uintptr_t>(y) & 15) == 0,
              ae = (reinterpret_cast<uintptr_t>(e) & 15) == 0;
   Leader lead = {0.0f, INT_MAX};
-  float bar = 0.0f;  // the warp's leader
+  float bar = 0.0f;
   for (; i0 < end; i0 += U * step) {
     float4 vx[U], ve[U], vy[U];
 #pragma unroll
@@ -301,30 +307,44 @@ __device__ __forceinline__ Leader race(const Sequence& q, const Pick& k, const f
       ve[j] = logits4(e, i, end, ae, INFINITY);
       vy[j] = y ? logits4(y, i, end, ay) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
+    bar = fmaxf(bar, __uint_as_float(*(volatile uint32_t*)shared_bar));
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       const int i = min(i0 + j * step, end) + 4 * lane;
       const float fx[4] = {vx[j].x, vx[j].y, vx[j].z, vx[j].w}, fy[4] = {vy[j].x, vy[j].y, vy[j].z, vy[j].w},
                   fe[4] = {ve[j].x, ve[j].y, ve[j].z, ve[j].w};
-      bool may[4], any = false;
+      float high[4], width[4];
+      bool any = false;
 #pragma unroll
       for (int z = 0; z < 4; ++z) {
         const float dx = fx[z] - k.xm, dy = fy[z] - k.ym;
         const float p = ex2(dx * q.c_hi) * k.xi;                 // a NaN is never taken
         const float r = y ? fmaxf(ex2(dy * q.c_hi), 0.0f) * k.yi : 0.0f;  // and counts as 0 here
-        may[z] = fmaf(p + r, 0x1p-15f, p - r) > bar * fe[z];
-        any |= may[z];
+        width[z] = p + r;
+        high[z] = fmaf(width[z], 0x1p-15f, p - r);
+        any |= high[z] > bar * fe[z];
       }
       if (__any_sync(0xffffffffu, any)) {
+        // what these entries score at least raises the bar, which few of them pass then
+        float least = 0.0f;
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          const float low = fmaf(width[z], -0x1p-14f, high[z]);
+          if (low > 0.0f && i + z != out_of) least = fmaxf(least, low / fe[z]);
+        }
+        least = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fminf(least, FLT_MAX))));
+        if (least > bar) {
+          bar = least;
+          if (lane == 0) atomicMax(shared_bar, __float_as_uint(bar));
+        }
 #pragma unroll
         for (int z = 0; z < 4; ++z)
-          if (may[z] && i + z != out_of) {
+          if (high[z] > bar * fe[z] && i + z != out_of) {
             // products that round by themselves: equal rows leave exactly nothing
             float w = __fmul_rn(exp_scaled(fx[z] - k.xm, q.c_hi, q.c_lo), k.xi);
             if (y) w = __fsub_rn(w, __fmul_rn(exp_scaled(fy[z] - k.ym, q.c_hi, q.c_lo), k.yi));
             if (w > 0.0f) lead.take(w / fe[z], i + z);
           }
-        bar = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(lead.best)));
       }
     }
   }
@@ -343,11 +363,14 @@ template <int U, int W>
 __device__ __forceinline__ int64_t race_cluster(const Sequence& q, const Pick& k, int i0, int end, int step, int rank, int ctas) {
   __shared__ Leader s_lead[W];
   __shared__ Leader s_all[2][kVerifyCluster];
+  __shared__ uint32_t s_bar;
   const int tid = threadIdx.x;
   const float* y = k.drafted ? q.row(q.n + 1 + k.taken) : nullptr;
   int out_of = k.out_of;
+  if (tid == 0) s_bar = 0u;  // and so it is in a second pass: nothing scored in the first
+  __syncthreads();
   for (int pass = 0;; ++pass) {  // a second one where nothing of p - q is left: p itself
-    Leader lead = race<U>(q, k, y, out_of, i0, end, step);
+    Leader lead = race<U>(q, k, y, out_of, i0, end, step, &s_bar);
     if ((tid & 31) == 0) s_lead[tid >> 5] = lead;
     __syncthreads();
     if (tid < ctas) {
@@ -471,22 +494,60 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_verify_pick(VerifyArgs a) {
     write_tokens(q, k.taken, greedy(s_row[k.taken]), lane, 32);
     k.taken = -1;
   }
+  k.lead = 0ull;
+  k.done = 0;
   if (lane == 0) a.picks[q.b] = k;
 }
 
-// Step 3 alone: a cluster of `ctas` CTAs per sequence.  Three rows of 64 x 128256, 98 MB: 20 us in the call.
-__global__ void __launch_bounds__(kVerifyThreads, 2) k_verify_race(VerifyArgs a, int ctas) {
+// A leader as one number, the larger the better: its score, then the lower index; 0 for none.
+__device__ __forceinline__ unsigned long long packed(const Leader& l) {
+  return l.at == INT_MAX ? 0ull : (unsigned long long)__float_as_uint(l.best) << 32 | (uint32_t)~l.at;
+}
+
+// Step 3 alone: grid (CTAs of a sequence, batch), a CTA `per` entries.  The leaders meet in the
+// sequence's Pick by a maximum, which no order of the CTAs changes; the last CTA writes.  All CTAs run
+// at once, four on an SM: a second wave pays the start again (some 4 us: 64 sequences of 128256 entries 61 us
+// a call with 592 CTAs, 65 with 1184; 65 with two on an SM that request four pieces at a time; 64.7 with a
+// cluster of 4 per sequence, which left SMs with one CTA beside SMs with two).
+__global__ void __launch_bounds__(kVerifyThreads, 4) k_verify_race(VerifyArgs a, int per) {
+  constexpr int U = 2, W = kVerifyWarps;
+  __shared__ unsigned long long s_lead[W], s_best;
+  __shared__ int s_last;
+  __shared__ uint32_t s_bar;
   pdl_trigger();
+  if (threadIdx.x == 0) s_bar = 0u;
+  __syncthreads();
   pdl_wait();
-  const int b = blockIdx.x / ctas, rank = blockIdx.x - b * ctas;
-  const Pick k = a.picks[b];
-  if (k.taken < 0) return;  // done already; the whole cluster returns
-  cluster_arrive_relaxed();
-  const Sequence q(a, b);
-  cluster_wait();  // all CTAs of the cluster run
-  const int64_t last = race_cluster<4, kVerifyWarps>(q, k, 4 * (rank * kVerifyThreads + (threadIdx.x & ~31)), a.vocab,
-                                       4 * kVerifyThreads * ctas, rank, ctas);
-  if (rank == 0) write_tokens(q, k.taken, last, threadIdx.x, kVerifyThreads);
+  const Sequence q(a, blockIdx.y);
+  Pick* pick = a.picks + blockIdx.y;
+  const Pick k = *pick;
+  if (k.taken < 0) return;  // done already
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const float* y = k.drafted ? q.row(q.n + 1 + k.taken) : nullptr;
+  auto best = [&](const Leader& lead) {  // of the CTA, in thread 0
+    if (lane == 0) s_lead[warp] = packed(lead);
+    __syncthreads();
+    unsigned long long x = s_lead[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) x = max(x, s_lead[w]);
+    return x;
+  };
+  const int i0 = blockIdx.x * per, end = min(a.vocab, i0 + per);
+  unsigned long long all = best(race<U>(q, k, y, k.out_of, i0 + 128 * warp, end, 128 * W, &s_bar));
+  if (tid == 0) {
+    if (all) atomicMax(&pick->lead, all);
+    __threadfence();
+    s_last = atomicAdd(&pick->done, 1) == (int)gridDim.x - 1;
+    if (s_last) {
+      __threadfence();
+      s_best = atomicMax(&pick->lead, 0ull);
+    }
+  }
+  __syncthreads();
+  if (!s_last) return;
+  all = s_best;
+  if (!all && k.refused) all = best(race<U>(q, k, nullptr, -1, 128 * warp, a.vocab, 128 * W, &s_bar));  // nothing of p - q: p itself
+  write_tokens(q, k.taken, all ? (int64_t)(uint32_t)~(uint32_t)all : -1, tid, kVerifyThreads);
 }
 
 template <int W>
@@ -601,9 +662,9 @@ extern "C" OTF_API int otf_verify_drafts(const float* target, int64_t target_seq
   if (e != cudaSuccess) return set_cuda_error(e);
   e = otf::launch_pdl(otf::k_verify_pick, dim3((unsigned)batch), dim3(otf::kPickThreads), 0, s, 1u, a);
   if (e != cudaSuccess || (!temperatures && temperature == 0.0f)) return set_cuda_error(e);
-  // CTAs per sequence: as many as all run at once, two on an SM
-  int ctas = otf::kRaceCluster;
-  while (ctas > 1 && batch * ctas > 2 * 148) ctas /= 2;
-  return set_cuda_error(otf::launch_pdl(otf::k_verify_race, dim3((unsigned)(batch * ctas)), dim3(otf::kVerifyThreads), 0, s,
-                                        (unsigned)ctas, a, ctas));
+  // CTAs per sequence: as many as all run at once
+  const int64_t ctas = std::max<int64_t>(1, std::min(otf::kRaceResident / batch, vocab / otf::kRaceLeast));
+  const int per = (int)(((vocab + ctas - 1) / ctas + 127) & ~127ll);
+  return set_cuda_error(otf::launch_pdl(otf::k_verify_race, dim3((unsigned)((vocab + per - 1) / per), (unsigned)batch),
+                                        dim3(otf::kVerifyThreads), 0, s, 1u, a, per));
 }

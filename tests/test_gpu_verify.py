@@ -199,3 +199,21 @@ def test_verify_draws_from_the_target(cuda_dev):
     seen = torch.bincount(got[:, 0].cpu(), minlength=vocab).double()
     p = torch.softmax(p_log.double(), 0)
     assert bool(((seen - n * p).abs() <= 5 * (n * p * (1 - p)).sqrt()).all())
+
+
+def test_verify_large_equal_distributions(cuda_dev):
+    """As above, over several CTAs of a race: nothing of p - q is left, p is drawn from."""
+    target, tokens, _, uniforms, noise = inputs(8, 2, 200003, True, seed=31)
+    uniforms = uniforms.clone()
+    uniforms[::2, 1] = 1.0
+    got, accepted = check(cuda_dev, target, tokens, target[:, :2].clone(), uniforms, noise, 1.0)
+    assert accepted.tolist() == [1, 2] * 4
+
+
+def test_verify_large_ties_go_to_the_lowest_index(cuda_dev):
+    batch, vocab = 6, 600000
+    target, tokens = torch.zeros(batch, 2, vocab), torch.zeros(batch, 1, dtype=torch.int64)
+    target[:, :, :1000] = -float("inf")
+    tokens[::2] = 1000
+    got, accepted = check(cuda_dev, target, tokens, None, torch.full((batch, 1), 0.5), torch.ones(batch, vocab), 1.0)
+    assert got.tolist() == [[1001, -1], [1000, -1]] * 3 and accepted.tolist() == [0] * batch
