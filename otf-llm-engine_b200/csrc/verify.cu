@@ -34,15 +34,16 @@ constexpr int kVerifySeg = 1024;     // logits that a warp holds at once, 32 a l
 constexpr int kVerifyThreads = 256;
 constexpr int kVerifyWarps = kVerifyThreads / 32;
 constexpr int kVerifyCluster = 16;   // CTAs of a sequence at most (k_verify)
-constexpr int kPickThreads = 512;
+constexpr int kPickThreads = 1024;   // of k_verify_pick at most
 constexpr int kRaceResident = 148 * 4;  // CTAs of k_verify_race that run at once
 constexpr int kRaceLeast = 1024;     // entries of a CTA at least (k_verify_race)
-// One launch is taken up to 6M logits in all rows, or 8M of at most kVerifyFew sequences; its CTAs then
-// have 32 warps where a CTA's slice of the rows is large (kVerifyLarge logits), else 8.  Measured,
-// eager calls one after another, one launch against three: 16 sequences x 5 rows of 32000 (2.4M) 14.1 us
-// against 20.8, 32 sequences (4.9M) 16.1 against 21.0, 64 (9.8M) 23.7 against 24.0; 4 x 11 rows of 128256
-// (5.4M) 19.8 against 25.8, 8 x 11 (10.8M) 37.3 against 30.1, 16 x 8 (15.7M) 25.0 against 18.3.  32 warps
-// against 8: one sequence, 9 rows of 128256, 17.4 us against 22.5; 8 x 5 rows of 32000 19.0 against 14.1.
+// One launch is taken up to 6M logits in all rows and 512K of a sequence (1.5M of at most kVerifyFew
+// sequences); its CTAs then have 32 warps where a CTA's slice of the rows is large (kVerifyLarge
+// logits), else 8.  Measured, eager calls one after another, one launch against three: 16 sequences x 5
+// rows of 32000 (2.4M) 13.8 us against 20.4, x 9 rows (4.4M) 18.8 against 21.0, 32 x 9 (8.8M) 22.5 against
+// 22.0; 8 x 5 rows of 128256 (641K each) 22.5 against 21.2; 4 x 11 (1.4M each) 18.8 against 21.2, 4 x 17
+// (2.2M) 23.7 against 21.2, one of 33 (4.2M) 31.9 against 21.3.  32 warps against 8: one sequence, 9 rows of
+// 128256, 17.4 us against 22.5; 8 x 5 rows of 32000 19.0 against 14.1.
 constexpr int kVerifyFew = 4;
 constexpr int64_t kVerifyLarge = 1 << 14;
 
@@ -459,8 +460,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) k_verify_rows(VerifyArgs a)
   }
 }
 
-// Step 2 alone: a CTA per sequence, a warp per row.  Latency-bound: 7 us for those 64 sequences.
-__global__ void __launch_bounds__(kPickThreads, 2) k_verify_pick(VerifyArgs a) {
+// Step 2 alone: a CTA per sequence, a warp per row.  Latency-bound, 7 us for those 64 sequences: 32 warps
+// where there are more than 16 rows (4 sequences x 17 rows of 128256 21.0 us a call with 16, 19.5 with 32),
+// but not for more sequences than SMs (250 x 3 rows of 10000 23.1 and 26.5).
+__global__ void __launch_bounds__(kPickThreads, 1) k_verify_pick(VerifyArgs a) {
   __shared__ RowPart s_row[kVerifyMaxRows];
   pdl_trigger();
   pdl_wait();
@@ -469,12 +472,12 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_verify_pick(VerifyArgs a) {
   const int rows = q.rows();
   if (rows == 0) {
     if (tid == 0) a.picks[q.b].taken = -1;
-    write_tokens(q, 0, -1, tid, kPickThreads);
+    write_tokens(q, 0, -1, tid, blockDim.x);
     return;
   }
   Drafted d = {-1, 0.0f, 0.0f, 0.0f};
   if (warp == 0) d = ask_drafted(q, lane);
-  for (int r = warp; r < rows; r += kPickThreads / 32) {
+  for (int r = warp; r < rows; r += blockDim.x / 32) {
     constexpr int U = 4;  // a lane's parts of 128 segments, requested together
     const RowPart* p = q.part(r);
     RowPart x[U];
@@ -567,7 +570,7 @@ static cudaError_t launch_verify(const VerifyArgs& a, int batch, int ctas, cudaS
 
 // One launch, or the workspace of three.
 static bool one_launch(int64_t batch, int64_t rows, int64_t vocab) {
-  return batch * rows * vocab <= (batch <= kVerifyFew ? 8ll << 20 : 6ll << 20);
+  return batch * rows * vocab <= 6ll << 20 && rows * vocab <= (batch <= kVerifyFew ? 3ll << 19 : 1ll << 19);
 }
 
 }  // namespace otf
@@ -654,13 +657,15 @@ extern "C" OTF_API int otf_verify_drafts(const float* target, int64_t target_seq
   a.picks = static_cast<otf::Pick*>(workspace);
   a.parts = reinterpret_cast<otf::RowPart*>(static_cast<char*>(workspace) +
                                             otf::align_up(batch * (int64_t)sizeof(otf::Pick), 256));
-  // row groups: one per row while all of their CTAs fit the GPU at once, else 4
+  // row groups: as many as all of their CTAs run at once, at least 4 (one sequence x 65 rows of 128256
+  // 42.5 us a call with 4, 24.6 with 37)
   const int64_t blocks = (a.segs + otf::kVerifyWarps - 1) / otf::kVerifyWarps;
-  const int64_t groups = std::min<int64_t>(rows, batch * blocks * rows <= 4 * 148 ? rows : 4);
+  const int64_t groups = std::min(rows, std::max<int64_t>(4, 4 * 148 / (batch * blocks)));
   cudaError_t e = otf::launch_pdl(otf::k_verify_rows, dim3((unsigned)blocks, (unsigned)groups, (unsigned)batch),
                                   dim3(otf::kVerifyThreads), 0, s, 1u, a);
   if (e != cudaSuccess) return set_cuda_error(e);
-  e = otf::launch_pdl(otf::k_verify_pick, dim3((unsigned)batch), dim3(otf::kPickThreads), 0, s, 1u, a);
+  e = otf::launch_pdl(otf::k_verify_pick, dim3((unsigned)batch),
+                      dim3(rows > 16 && batch <= 148 ? otf::kPickThreads : otf::kPickThreads / 2), 0, s, 1u, a);
   if (e != cudaSuccess || (!temperatures && temperature == 0.0f)) return set_cuda_error(e);
   // CTAs per sequence: as many as all run at once
   const int64_t ctas = std::max<int64_t>(1, std::min(otf::kRaceResident / batch, vocab / otf::kRaceLeast));

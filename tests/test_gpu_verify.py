@@ -217,3 +217,9 @@ def test_verify_large_ties_go_to_the_lowest_index(cuda_dev):
     tokens[::2] = 1000
     got, accepted = check(cuda_dev, target, tokens, None, torch.full((batch, 1), 0.5), torch.ones(batch, vocab), 1.0)
     assert got.tolist() == [[1001, -1], [1000, -1]] * 3 and accepted.tolist() == [0] * batch
+
+
+@pytest.mark.parametrize("batch,drafts,vocab,drafted", [(1, 12, 128256, True), (4, 5, 128256, True), (5, 2, 110001, True),
+                                                        (2, 32, 60000, True), (150, 16, 4001, False)])
+def test_verify_on_either_side_of_the_switches(batch, drafts, vocab, drafted, cuda_dev):
+    check(cuda_dev, *inputs(batch, drafts, vocab, drafted, seed=vocab + batch), 0.9)
