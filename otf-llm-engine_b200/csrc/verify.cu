@@ -15,7 +15,7 @@
 // Few logits take one launch, k_verify: a cluster of CTAs per sequence, the vocabulary cut among them,
 // the steps' results exchanged through distributed shared memory.  Many take three, whose grids
 // fill the GPU in every step whatever the sequences' drafts are: k_verify_rows, k_verify_pick,
-// k_verify_race.  What a step computes is shared, and so is the order of its sums within a row.
+// k_verify_race.  What a step computes is shared.
 #include <cfloat>
 
 #include <algorithm>
@@ -444,9 +444,10 @@ __global__ void __launch_bounds__(32 * W, 1024 / (32 * W) < 3 ? 1024 / (32 * W) 
   if (rank == 0) write_tokens(q, k.taken, last, tid, 32 * W);
 }
 
-// Step 1 alone: grid (blocks of 8 segments, row groups, batch), a warp per segment.  64 sequences of 1
-// to 11 rows of 128256, 197 MB: 38 us, 5.2 TB/s.  The warps of a CTA never meet.  A CTA goes through its group's rows, so that rows that a sequence with fewer
-// drafted tokens does not have cost nothing.
+// Step 1 alone: grid (blocks of 8 segments, row groups, batch), a warp per segment; the warps of a CTA
+// never meet.  64 sequences of 1 to 11 rows of 128256 and their draft's, 229 MB: 41 us by itself, 5.6 TB/s.  A
+// CTA goes through its group's rows, so that rows that a sequence with fewer drafted tokens does not
+// have cost nothing.
 __global__ void __launch_bounds__(kVerifyThreads, 4) k_verify_rows(VerifyArgs a) {
   pdl_trigger();
   pdl_wait();
@@ -511,7 +512,7 @@ __device__ __forceinline__ unsigned long long packed(const Leader& l) {
 // sequence's Pick by a maximum, which no order of the CTAs changes; the last CTA writes.  All CTAs run
 // at once, four on an SM: a second wave pays the start again (some 4 us: 64 sequences of 128256 entries 61 us
 // a call with 592 CTAs, 65 with 1184; 65 with two on an SM that request four pieces at a time; 64.7 with a
-// cluster of 4 per sequence, which left SMs with one CTA beside SMs with two).
+// cluster of 4 per sequence, which left SMs with one CTA beside SMs with two).  By itself 23 us, 85 MB.
 __global__ void __launch_bounds__(kVerifyThreads, 4) k_verify_race(VerifyArgs a, int per) {
   constexpr int U = 2, W = kVerifyWarps;
   __shared__ unsigned long long s_lead[W], s_best;
