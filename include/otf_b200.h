@@ -556,7 +556,10 @@ OTF_API int otf_paged_evict(const otf_paged_cache* from, const otf_paged_cache* 
  * the logits counts as -inf.  A sequence without a token of positive weight (temperature 0: of a
  * logit above -inf), or with a count or temperature out of range, gets -1 and raises the
  * otf_device_error flag; so does a drafted token outside the vocabulary, which is refused.  Where
- * max(p - q, 0) holds nothing, p is drawn from.  At most 65535 sequences and a vocabulary of 2^30.  workspace:
+ * max(p - q, 0) holds nothing, p is drawn from.  p and q are fp32, so rounding decides where they
+ * differ by less than some 2^-21 of p (a draft is refused with the probability that max(p - q, 0)
+ * sums to: a residue as small is drawn from as rarely).  At most 65535 sequences and a vocabulary of
+ * 2^30.  workspace:
  * otf_verify_workspace_bytes(...) (0 for small calls, then it may be NULL), 256-byte aligned, need
  * not be cleared; two calls that may run at the same time need one each.  Beside
  * otf_i8_head_argmax, the greedy pick of one row.
