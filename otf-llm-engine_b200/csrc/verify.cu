@@ -80,7 +80,7 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// 0, or from 1e-20 on (log2(e) / T and its product with a difference of logits stay finite).
+// 0, or from 1e-20 on (log2(e) / T stays finite; its product with a difference of logits need not).
 __host__ __device__ __forceinline__ bool temperature_ok(float T) { return T == 0.0f || (T >= 1e-20f && T <= 1e20f); }
 
 // Four consecutive values of a row, `pad` behind its end.  Rows that are not 16-byte aligned are read
@@ -181,9 +181,12 @@ __device__ __forceinline__ RowPart read_segment(const Sequence& q, const float* 
     at = __reduce_min_sync(0xffffffffu, at);
   } else {
     const float mt = m == -INFINITY ? 0.0f : m;  // nothing but -inf: the sum is 0
-    auto term = [&](float x) {                   // 0 for -inf and NaN
-      const float d = x - mt;
-      return ex2(fmaxf(fmaf(d, q.c_hi, d * q.c_lo), -200.0f));
+    // 0 for -inf and NaN.  Bounded before the products: the lowest finite logit times a negative c_lo
+    // of a small T is +inf.
+    const float low = -138.629436f * q.T;  // its exponential is 2^-200, 0 in fp32
+    auto term = [&](float x) {
+      const float d = fmaxf(x - mt, low);
+      return ex2(fmaf(d, q.c_hi, d * q.c_lo));
     };
 #pragma unroll
     for (int z = 0; z < N; ++z) s += (term(v[z].x) + term(v[z].y)) + (term(v[z].z) + term(v[z].w));

@@ -223,3 +223,18 @@ def test_verify_large_ties_go_to_the_lowest_index(cuda_dev):
                                                         (2, 32, 60000, True), (150, 16, 4001, False)])
 def test_verify_on_either_side_of_the_switches(batch, drafts, vocab, drafted, cuda_dev):
     check(cuda_dev, *inputs(batch, drafts, vocab, drafted, seed=vocab + batch), 0.9)
+
+
+@pytest.mark.parametrize("temperature", [1e-6, 1e-8, 1e-10, 3e-10, 1e-12, 1e-20])
+@pytest.mark.parametrize("drafted", [False, True])
+@pytest.mark.parametrize("batch,vocab", [(2, 3001), (8, 200003)])
+def test_verify_lowest_finite_masks_at_small_temperatures(batch, vocab, drafted, temperature, cuda_dev):
+    """Logits masked with the lowest finite number, down to the smallest temperature, in one launch and in
+    three: the masked ones weigh nothing, and the largest of the others is taken and drawn."""
+    target, tokens, draft, uniforms, noise = inputs(batch, 3, vocab, drafted, seed=vocab)
+    target[:, :, 1::2] = torch.finfo(torch.float32).min
+    if drafted:
+        draft[:, :, ::3] = torch.finfo(torch.float32).min
+    tokens = (draft if drafted else target[:, :3]).argmax(2)
+    tokens[0, 1] = 1                                        # a masked one
+    check(cuda_dev, target, tokens, draft, uniforms, noise, temperature)
