@@ -817,10 +817,17 @@ __global__ void __launch_bounds__(kWeightThreads) k_paged_attn_weights(AttnArgs 
   weights[item * ldw + s] += sum;
 }
 
+// The sizes that there are limits for.  Within them a head's scores take 2^52 bytes at most, a
+// sequence's 2^62.
+static bool attn_limits(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t tokens, int64_t max_tokens) {
+  return batch <= kPagedMaxBatch && heads <= 65535 && kv_heads <= 1024 && (D == 64 || D == 128) &&
+         tokens <= kPagedMaxTokens && max_tokens <= 1ll << 30;
+}
+
 // Bytes of the workspace's parts, in order.
 struct AttnSpace {
   int64_t prefix, part, part_ml, lse, scores, ld_scores;
-  int64_t bytes() const { return prefix + part + part_ml + lse + scores; }
+  int64_t bytes() const { return scores < 0 ? -1 : prefix + part + part_ml + lse + scores; }  // -1: beyond 2^62
 };
 // Rows of a block: eights, 32 at most.
 static int block_rows(int64_t rows) { return rows >= 32 ? 32 : (int)((rows + 7) / 8 * 8); }
@@ -833,7 +840,8 @@ static AttnSpace attn_space(int64_t batch, int64_t heads, int64_t kv_heads, int6
   s.part_ml = align_up(2 * kPaGrid * RB * 16, 256);
   s.ld_scores = align_up(rows, 4);
   s.lse = weights ? align_up(batch * kv_heads * s.ld_scores * 4, 256) : 0;
-  s.scores = weights ? align_up(batch * kv_heads * s.ld_scores * max_tokens * 4, 256) : 0;
+  const int64_t each = kv_heads * s.ld_scores * max_tokens * 4;  // of a sequence
+  s.scores = !weights ? 0 : each > (1ll << 62) / batch ? -1 : align_up(batch * each, 256);
   return s;
 }
 
@@ -908,8 +916,8 @@ int otf::paged_attn_device_error(int clear) {
 extern "C" OTF_API int64_t otf_paged_attn_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads,
                                                           int64_t head_dim, int64_t tokens, int64_t max_tokens,
                                                           int with_weights) {
-  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || head_dim <= 0 || tokens <= 0 ||
-      tokens > otf::kPagedMaxTokens || max_tokens <= 0)
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || tokens <= 0 || max_tokens <= 0 ||
+      !otf::attn_limits(batch, heads, kv_heads, head_dim, tokens, max_tokens))
     return -1;
   return otf::attn_space(batch, heads, kv_heads, head_dim, tokens, max_tokens, with_weights != 0).bytes();
 }
@@ -922,10 +930,11 @@ extern "C" OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* 
   if (st != OTF_OK) return st;
   const int64_t D = cache->head_dim;
   if (heads <= 0 || heads % a.c.kv_heads || tokens <= 0 || !(std::fabs(scale) <= 3.4e38f)) return OTF_ERR_INVALID;
-  if (tokens > otf::kPagedMaxTokens || heads > 65535) return OTF_ERR_UNSUPPORTED;
+  if (!otf::attn_limits(a.c.batch, heads, a.c.kv_heads, D, tokens, a.c.capacity)) return OTF_ERR_UNSUPPORTED;
   if (!otf::rows16(q, ldq, heads * D) || !otf::rows16(out, ldo, heads * D)) return OTF_ERR_INVALID;
   if (weights && ldw < a.c.capacity) return OTF_ERR_INVALID;
   const otf::AttnSpace space = otf::attn_space(a.c.batch, heads, a.c.kv_heads, D, tokens, a.c.capacity, weights != nullptr);
+  if (space.bytes() < 0) return OTF_ERR_UNSUPPORTED;
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < space.bytes())
     return OTF_ERR_INVALID;
   st = check_device();

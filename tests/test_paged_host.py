@@ -187,3 +187,23 @@ def test_abi_refuses_bad_verifications():
     large = dict(ldt=128256, d=FAKE, ldd=128256, ldtok=5, ldu=5, lde=128256, batch=64, drafts=5, vocab=128256)
     for bad in (dict(ws=None, size=n), dict(ws=FAKE + 8, size=n), dict(ws=FAKE, size=n - 1)):
         assert verify(**large, **bad) == INVALID, bad
+
+
+def test_attention_workspace_does_not_wrap():
+    """The scores' scratch of the largest tables passes 64 bits as a product: it is refused, or so large that
+    no small workspace is taken for it."""
+    from otf_llm import _native as N
+    L = N.lib()
+    for batch, heads, kv, tokens, most in ((4096, 65535, 1, 16, 1 << 30), (4096, 64512, 1024, 16, 1 << 30),
+                                           (4095, 65535, 1, 16, 1 << 29), (4096, 32768, 512, 16, 1 << 30)):
+        n = L.otf_paged_attn_workspace_bytes(batch, heads, kv, 64, tokens, most, 1)
+        assert n == -1 or n >= heads // kv * tokens * most * 4
+        c = cache(batch=batch, kv_heads=kv, token_stride=kv * 64, page_stride=16 * kv * 64, max_pages=most // 16,
+                  ld_table=most // 16)
+        for size in (0, 1 << 20, 1 << 30):
+            # (device memory of this size is never read: no GPU, or refused before)
+            assert L.otf_paged_attn(ctypes.byref(c), FAKE, heads * 64, heads, tokens, 1.0, FAKE, heads * 64, FAKE, most, FAKE,
+                                    size, None) in (INVALID, UNSUPPORTED)
+    for bad in ((4097, 4, 2, 64, 1, 64, 0), (1, 65536, 1, 64, 1, 64, 0), (1, 1025, 1025, 64, 1, 64, 0),
+                (1, 4, 2, 96, 1, 64, 0), (1, 4, 2, 64, 1, (1 << 30) + 1, 0), (1 << 40, 1 << 40, 1, 64, 1, 1 << 40, 1)):
+        assert L.otf_paged_attn_workspace_bytes(*bad) == -1, bad
