@@ -507,7 +507,8 @@ OTF_API int otf_paged_append(const otf_paged_cache* cache, const otf_rotary* rot
  * b * tokens + t of q ([batch * tokens, heads, head_dim], row stride ldq) sees the tokens
  * 0 .. lengths[b] + t (its own key among them: otf_paged_append ran before, lengths not yet
  * advanced) and out (row stride ldo) = softmax(scale q k) v, query head j reading KV head
- * j / (heads / kv_heads).  What a row does not see does not reach it, whatever it holds.
+ * j / (heads / kv_heads).  What a row does not see does not reach it, whatever it holds.  scale
+ * is finite, and so is scale log2(e) in fp32.
  * weights (fp32 [batch, kv_heads, ldw], may be NULL; ldw >= max_pages * page_size):
  * weights[b, h, s] += the softmax weight that token s received from the rows and query heads of
  * KV head h, for otf_paged_evict.  Scores, sums and outputs in fp32, joined over the parts of

@@ -44,6 +44,7 @@ constexpr int kPaThreads = kPaWarps * 32;
 constexpr int kPaStages = 3;
 constexpr int kPaStage = 8192;  // bytes of a warp's stage: its tokens' keys, then values
 constexpr int kPaGrid = 296;    // two CTAs on each of 148 SMs
+constexpr float kLog2e = 1.4426950408889634f;
 
 // Set when a sequence does not fit its pages or names a page outside the pool.
 __device__ int g_paged_attn_device_error;
@@ -338,7 +339,8 @@ __global__ void __launch_bounds__(kPaThreads, 2) k_paged_attn(AttnArgs a) {
   const uint32_t one2 = BF ? 0x3F803F80u : 0x3C003C00u;
   const uint32_t ones[4] = {one2, one2, one2, one2};
   const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;  // on q, so that a larger product weighs more
-  const float scale = fmaxf(fabsf(a.scale), 1e-30f);  // a masked -inf stays one under a scale of 0
+  // a masked -inf stays one under a scale of 0, and no finite score counts under 2^-149
+  const float scale = fmaxf(fabsf(a.scale), 0x1p-149f);
   const int lrow = lane & 7, lmat = lane >> 3;
   // a 16 x 16 tile's four 8 x 8 matrices, rows first and columns first
   const uint32_t rows_first = ((lmat & 1) * 8 + lrow) * (D * 2) + (((lmat >> 1) ^ lrow) << 4);
@@ -929,7 +931,7 @@ extern "C" OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* 
   int st = otf::view_of(cache, a.c);
   if (st != OTF_OK) return st;
   const int64_t D = cache->head_dim;
-  if (heads <= 0 || heads % a.c.kv_heads || tokens <= 0 || !(std::fabs(scale) <= 3.4e38f)) return OTF_ERR_INVALID;
+  if (heads <= 0 || heads % a.c.kv_heads || tokens <= 0 || !std::isfinite(scale * otf::kLog2e)) return OTF_ERR_INVALID;
   if (!otf::attn_limits(a.c.batch, heads, a.c.kv_heads, D, tokens, a.c.capacity)) return OTF_ERR_UNSUPPORTED;
   if (!otf::rows16(q, ldq, heads * D) || !otf::rows16(out, ldo, heads * D)) return OTF_ERR_INVALID;
   if (weights && ldw < a.c.capacity) return OTF_ERR_INVALID;
@@ -944,7 +946,7 @@ extern "C" OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* 
   a.ldq = ldq;
   a.out = static_cast<uint16_t*>(out);
   a.ldo = ldo;
-  a.scale = scale * 1.4426950408889634f;
+  a.scale = scale * otf::kLog2e;
   a.rep = (int)(heads / a.c.kv_heads);
   a.tokens = (int)tokens;
   a.rows = (int)(a.rep * tokens);

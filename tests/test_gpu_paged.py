@@ -670,3 +670,10 @@ def test_prompt_decode_evict_verify_together(dtype, cuda_dev):
     assert got[1].tolist() == [int(tokens[1, 0]), int(best[1, 1]), -1, -1]
     assert got[0].tolist() == tokens[0].tolist() + [int(best[0, 3])]
     assert flag() == 0
+
+
+@pytest.mark.parametrize("scale", [1e-35, -3e-36, 0.0, 1e-44])
+def test_attend_scales_below_the_smallest_normal_products(scale, cuda_dev):
+    """Scores of up to 1e35 under scales that bring them back to some units, and to nothing."""
+    check_attend(cuda_dev, [90, 9], 3, 16, 8, 2, 64, torch.bfloat16, spread=1e34, scale=scale, weights=True)
+    check_attend(cuda_dev, [700], 1, 16, 40, 1, 128, torch.bfloat16, spread=1e34, scale=scale)

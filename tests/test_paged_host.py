@@ -207,3 +207,11 @@ def test_attention_workspace_does_not_wrap():
     for bad in ((4097, 4, 2, 64, 1, 64, 0), (1, 65536, 1, 64, 1, 64, 0), (1, 1025, 1025, 64, 1, 64, 0),
                 (1, 4, 2, 96, 1, 64, 0), (1, 4, 2, 64, 1, (1 << 30) + 1, 0), (1 << 40, 1 << 40, 1, 64, 1, 1 << 40, 1)):
         assert L.otf_paged_attn_workspace_bytes(*bad) == -1, bad
+
+
+def test_abi_refuses_scales_that_are_not_finite():
+    """Nor finite times log2(e), which the scores' exponents are taken with."""
+    from otf_llm import _native as N
+    L, c = N.lib(), ctypes.byref(cache())
+    for scale in (float("inf"), -float("inf"), float("nan"), 3e38, -2.4e38):
+        assert L.otf_paged_attn(c, FAKE, 256, 4, 1, scale, FAKE, 256, None, 0, FAKE, 1 << 40, None) == INVALID
