@@ -513,7 +513,11 @@ OTF_API int otf_paged_append(const otf_paged_cache* cache, const otf_rotary* rot
  * weights[b, h, s] += the softmax weight that token s received from the rows and query heads of
  * KV head h, for otf_paged_evict.  Scores, sums and outputs in fp32, joined over the parts of
  * the cache in a fixed order.  workspace: otf_paged_attn_workspace_bytes(...), 256-byte aligned,
- * need not be cleared; two calls that may run at the same time need one each.
+ * need not be cleared; two calls that may run at the same time need one each.  max_tokens:
+ * max_pages * page_size.  With weights the workspace holds a score for every row, KV head and token
+ * that the table has room for, whatever the lengths are: 4 batch heads tokens max_tokens bytes, of
+ * which 2 GiB at a time (or one KV head's, if those are more), so that larger calls take several
+ * passes.  A caller that knows shorter lengths gives a smaller max_pages with the same ld_table.
  */
 OTF_API int64_t otf_paged_attn_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                                int64_t tokens, int64_t max_tokens, int with_weights);

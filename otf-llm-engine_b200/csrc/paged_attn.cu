@@ -793,43 +793,55 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_paged_attn_join(AttnArgs a,
 }
 
 // weights[b, g, s] += sum over the item's rows of 2^(score - lse): a thread per token, rows in order.
-// Memory-bound: the scores are read once, mostly from L2.
+// Memory-bound: the scores are read once, mostly from L2.  The grid covers all tokens that the table has room
+// for only up to kWeightCtas CTAs, which then go on to further tokens, so that room for long sequences costs
+// short ones little: whole calls, 64 sequences of 100 tokens, 8 KV heads, room for 8192 tokens, 22.8 us with
+// 8192 CTAs, 31 with 16384, 48 with all 32768 (for 131072 tokens the same, and 554 with all); 64 of 4000
+// tokens, 32 rows, room for 4096, 435 us with 8192, 428 with 16384, 426 with all.
 constexpr int kWeightThreads = 128;
+constexpr int64_t kWeightCtas = 16384;
 
-__global__ void __launch_bounds__(kWeightThreads) k_paged_attn_weights(AttnArgs a, float* weights, int64_t ldw) {
+__global__ void __launch_bounds__(kWeightThreads, 16) k_paged_attn_weights(AttnArgs a, float* weights, int64_t ldw) {
   pdl_trigger();
   pdl_wait();
   const PagedView& c = a.c;
-  const int g = blockIdx.y, b = blockIdx.z, s = blockIdx.x * kWeightThreads + threadIdx.x;
-  const int len = c.lengths[b];
-  if (len < 0 || (int64_t)len + a.tokens > c.capacity || s >= len + a.tokens) return;
+  const int g = blockIdx.y, b = blockIdx.z, len = c.lengths[b];
+  if (len < 0 || (int64_t)len + a.tokens > c.capacity) return;
   const int64_t item = (int64_t)b * c.kv_heads + g;
-  const float* x = a.scores + (item * a.max_keys + s) * a.ld_scores;
   const float* lse = a.lse + item * a.ld_scores;
-  float sum = 0.0f;
   auto term = [](float v, float l) { return v == -INFINITY ? 0.0f : ex2(v - l); };
+#pragma unroll 1
+  for (int s = blockIdx.x * kWeightThreads + threadIdx.x; s < len + a.tokens; s += gridDim.x * kWeightThreads) {
+    const float* x = a.scores + (item * a.max_keys + s) * a.ld_scores;
+    float sum = 0.0f;
 #pragma unroll 4
-  for (int r = 0; r < a.rows; r += 4) {
-    const float4 v = *reinterpret_cast<const float4*>(x + r), l = *reinterpret_cast<const float4*>(lse + r);
-    sum += term(v.x, l.x);
-    if (r + 1 < a.rows) sum += term(v.y, l.y);
-    if (r + 2 < a.rows) sum += term(v.z, l.z);
-    if (r + 3 < a.rows) sum += term(v.w, l.w);
+    for (int r = 0; r < a.rows; r += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(x + r), l = *reinterpret_cast<const float4*>(lse + r);
+      sum += term(v.x, l.x);
+      if (r + 1 < a.rows) sum += term(v.y, l.y);
+      if (r + 2 < a.rows) sum += term(v.z, l.z);
+      if (r + 3 < a.rows) sum += term(v.w, l.w);
+    }
+    weights[item * ldw + s] += sum;
   }
-  weights[item * ldw + s] += sum;
 }
 
-// The sizes that there are limits for.  Within them a head's scores take 2^52 bytes at most, a
-// sequence's 2^62.
+// The sizes that there are limits for.  Within them a head's scores take 2^52 bytes at most.
 static bool attn_limits(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t tokens, int64_t max_tokens) {
   return batch <= kPagedMaxBatch && heads <= 65535 && kv_heads <= 1024 && (D == 64 || D == 128) &&
          tokens <= kPagedMaxTokens && max_tokens <= 1ll << 30;
 }
 
-// Bytes of the workspace's parts, in order.
+// With weights, the scores that one pass may keep: rows x capacity x 4 bytes of a KV head, whatever the
+// lengths are.  Calls with more of them go through several passes, one after another, of as many sequences
+// as fit, or of as many KV heads of one sequence (one at least).
+constexpr int64_t kPaScoreBytes = 2ll << 30;
+
+// Bytes of the workspace's parts, in order, and the sequences and KV heads of a pass.
 struct AttnSpace {
   int64_t prefix, part, part_ml, lse, scores, ld_scores;
-  int64_t bytes() const { return scores < 0 ? -1 : prefix + part + part_ml + lse + scores; }  // -1: beyond 2^62
+  int64_t batch, kv_heads;
+  int64_t bytes() const { return prefix + part + part_ml + lse + scores; }
 };
 // Rows of a block: eights, 32 at most.
 static int block_rows(int64_t rows) { return rows >= 32 ? 32 : (int)((rows + 7) / 8 * 8); }
@@ -841,9 +853,16 @@ static AttnSpace attn_space(int64_t batch, int64_t heads, int64_t kv_heads, int6
   s.part = align_up(2 * kPaGrid * RB * D * 4, 256);
   s.part_ml = align_up(2 * kPaGrid * RB * 16, 256);
   s.ld_scores = align_up(rows, 4);
-  s.lse = weights ? align_up(batch * kv_heads * s.ld_scores * 4, 256) : 0;
-  const int64_t each = kv_heads * s.ld_scores * max_tokens * 4;  // of a sequence
-  s.scores = !weights ? 0 : each > (1ll << 62) / batch ? -1 : align_up(batch * each, 256);
+  s.batch = batch;
+  s.kv_heads = kv_heads;
+  s.lse = s.scores = 0;
+  if (weights) {
+    const int64_t each = s.ld_scores * max_tokens * 4, fit = std::max<int64_t>(1, kPaScoreBytes / each);
+    s.kv_heads = std::min(kv_heads, fit);
+    s.batch = std::min(batch, std::max<int64_t>(1, fit / kv_heads));
+    s.lse = align_up(s.batch * s.kv_heads * s.ld_scores * 4, 256);
+    s.scores = align_up(s.batch * s.kv_heads * each, 256);
+  }
   return s;
 }
 
@@ -890,11 +909,11 @@ static cudaError_t launch_attn(const AttnArgs& a, float* weights, int64_t ldw, c
   if (e != cudaSuccess) return e;
   if (a.chunk_units) e = launch_join<BF, D>(a, RB, s);
   if (e != cudaSuccess || !weights) return e;
+  const int64_t blocks = (a.c.capacity + kWeightThreads - 1) / kWeightThreads;
+  const int64_t most = std::max<int64_t>(1, kWeightCtas / ((int64_t)a.c.kv_heads * a.c.batch));
   return launch_pdl(k_paged_attn_weights,
-                    dim3((unsigned)((a.c.capacity + kWeightThreads - 1) / kWeightThreads), (unsigned)a.c.kv_heads,
-                         (unsigned)a.c.batch),
-                    dim3(kWeightThreads), 0,
-                    s, 1u, a, weights, ldw);
+                    dim3((unsigned)std::min(blocks, most), (unsigned)a.c.kv_heads, (unsigned)a.c.batch),
+                    dim3(kWeightThreads), 0, s, 1u, a, weights, ldw);
 }
 
 }  // namespace otf
@@ -936,7 +955,6 @@ extern "C" OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* 
   if (!otf::rows16(q, ldq, heads * D) || !otf::rows16(out, ldo, heads * D)) return OTF_ERR_INVALID;
   if (weights && ldw < a.c.capacity) return OTF_ERR_INVALID;
   const otf::AttnSpace space = otf::attn_space(a.c.batch, heads, a.c.kv_heads, D, tokens, a.c.capacity, weights != nullptr);
-  if (space.bytes() < 0) return OTF_ERR_UNSUPPORTED;
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < space.bytes())
     return OTF_ERR_INVALID;
   st = check_device();
@@ -967,7 +985,21 @@ extern "C" OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* 
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = cache->dtype == OTF_DTYPE_BF16;
-  const cudaError_t e = D == 128 ? (bf ? otf::launch_attn<true, 128>(a, weights, ldw, s) : otf::launch_attn<false, 128>(a, weights, ldw, s))
-                                 : (bf ? otf::launch_attn<true, 64>(a, weights, ldw, s) : otf::launch_attn<false, 64>(a, weights, ldw, s));
-  return set_cuda_error(e);
+  auto* launch = D == 128 ? (bf ? otf::launch_attn<true, 128> : otf::launch_attn<false, 128>)
+                          : (bf ? otf::launch_attn<true, 64> : otf::launch_attn<false, 64>);
+  for (int64_t b = 0; b < a.c.batch; b += space.batch)
+    for (int64_t g = 0; g < a.c.kv_heads; g += space.kv_heads) {  // more than one only with one sequence a pass
+      otf::AttnArgs p = a;
+      p.c.batch = (int)std::min(space.batch, a.c.batch - b);
+      p.c.kv_heads = (int)std::min(space.kv_heads, a.c.kv_heads - g);
+      p.c.table += b * a.c.ld_table;
+      p.c.lengths += b;
+      p.c.k += g * a.c.head_stride;
+      p.c.v += g * a.c.head_stride;
+      p.q += b * tokens * ldq + g * a.rep * D;
+      p.out += b * tokens * ldo + g * a.rep * D;
+      const cudaError_t e = launch(p, weights ? weights + (b * a.c.kv_heads + g) * ldw : nullptr, ldw, s);
+      if (e != cudaSuccess) return set_cuda_error(e);
+    }
+  return OTF_OK;
 }

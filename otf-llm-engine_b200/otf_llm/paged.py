@@ -294,7 +294,10 @@ class PagedKVCache:
         sequence b sees the tokens 0 .. lengths[b] + t.  ``scale`` defaults to head_dim ** -0.5.
         ``weights`` (fp32 [batch, kv_heads, at least capacity], contiguous): to every token's entry
         is added the softmax weight that it received from the rows and the query heads of that KV
-        head.  Returns ``out``, of q's shape (rows of negative lengths are left as they were)."""
+        head.  Scratch for them grows with the table's room, not the lengths: 4 bytes x batch x heads x
+        tokens x capacity, at most 2 GiB at a time (the call then takes several passes).  A cache made
+        over fewer columns of a large table, ``page_table[:, :n]``, needs and walks less.  Returns ``out``,
+        of q's shape (rows of negative lengths are left as they were)."""
         key = (q.shape, q.stride(), weights is None)
         plan = self._attend_plans.get(key)
         if plan is None:

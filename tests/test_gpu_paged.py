@@ -677,3 +677,67 @@ def test_attend_scales_below_the_smallest_normal_products(scale, cuda_dev):
     """Scores of up to 1e35 under scales that bring them back to some units, and to nothing."""
     check_attend(cuda_dev, [90, 9], 3, 16, 8, 2, 64, torch.bfloat16, spread=1e34, scale=scale, weights=True)
     check_attend(cuda_dev, [700], 1, 16, 40, 1, 128, torch.bfloat16, spread=1e34, scale=scale)
+
+
+@pytest.mark.parametrize("totals,tokens,heads,kv", [
+    ([40, 300, 0, 17, 90], 16, 16, 2),                      # a pass of two sequences, and the last by itself
+    ([70, 33], 16, 32, 2),                                  # a sequence a pass
+    ([45, 130, 2000], 16, 51, 3),                           # a KV head a pass
+])
+def test_attend_with_weights_under_a_table_with_much_room(totals, tokens, heads, kv, cuda_dev):
+    """Short sequences under a table for 2^20 tokens, whose scores would not fit the scratch at once: in passes,
+    with the results of the definition, and nothing added elsewhere."""
+    from otf_llm.paged import PagedKVCache
+    page, dim, dt = 64, 64, torch.float16
+    small, pools, table, g = make(cuda_dev, totals, page, kv, dim, dt)
+    wide = torch.full((len(totals), (1 << 20) // page), -7, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    lengths = torch.tensor([n - tokens if n > 0 else -1 for n in totals], dtype=torch.int32, device=cuda_dev)
+    cache = PagedKVCache(small.k_pages, small.v_pages, wide.to(cuda_dev), lengths)
+    q = torch.randn(len(totals), tokens, heads, dim, generator=g).to(dt)
+    out = torch.full_like(q, 7.0).to(cuda_dev)
+    w = torch.full((len(totals), kv, cache.capacity + 3), 0.5, device=cuda_dev)
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    cache.attend(q.to(cuda_dev), weights=w, out=out)
+    assert flag() == 0 and torch.cuda.max_memory_allocated() - before < (2 << 30) + (64 << 20)
+    out = out.cpu().double()
+    for b, n in enumerate(totals):
+        if n == 0:
+            assert bool((out[b] == 7.0).all()) and bool((w[b] == 0.5).all())
+            continue
+        k, v = (ref.gather(p, table, b, n) for p in pools)
+        want, tol = torch.zeros(kv, n, dtype=torch.float64), torch.full((kv, n), 2.0 ** -22, dtype=torch.float64)
+        for t in range(tokens):
+            m = n - tokens + t + 1
+            y, p, mass, size = ref.attend(q[b, t], k[:m], v[:m], dim ** -0.5)
+            assert bool(((out[b, t] - y).abs() <= ref.attend_tolerance(y, mass, size, dim, dt)).all()), (b, t)
+            want[:, :m] += p.view(kv, -1, m).sum(1)
+            # the scores' and the sums' roundings, and those of adding up in fp32
+            tol[:, :m] += (p * (size * 2.0 ** -14 + 2.0 ** -18)).view(kv, -1, m).sum(1) + 2.0 ** -22
+        assert bool(((w[b, :, :n].cpu().double() - 0.5 - want).abs() <= tol).all()), b
+        assert bool((w[b, :, n:] == 0.5).all())
+
+
+def test_attend_walks_long_sequences_under_a_bounded_grid(cuda_dev):
+    """Weights of more tokens than the weights' grid covers at once: one sequence of 300,000 tokens among 63
+    missing ones over 8 KV heads, whose weights sum to the rows."""
+    from otf_llm.paged import PagedKVCache
+    g = torch.Generator(device=cuda_dev).manual_seed(5)
+    n, kv, heads, page = 300000, 8, 16, 64
+    room = -(-n // page)
+    k, v = (torch.randn(40, page, kv, 64, generator=g, device=cuda_dev).half() for _ in range(2))
+    table = torch.randint(0, 40, (64, room), dtype=torch.int32, generator=g, device=cuda_dev)
+    lengths = torch.full((64,), -1, dtype=torch.int32, device=cuda_dev)
+    lengths[37] = n - 1
+    cache = PagedKVCache(k, v, table, lengths)
+    q = torch.randn(64, heads, 64, generator=g, device=cuda_dev).half()
+    w = torch.zeros(64, kv, cache.capacity, device=cuda_dev)
+    cache.attend(q, weights=w)
+    assert flag() == 0
+    keys = k[table[37].long()].flatten(0, 1)[:n].double()
+    p = torch.softmax(torch.einsum("hd,nhd->hn", q[37].double(), keys.repeat_interleave(2, 1)) / 8, -1).view(kv, 2, n).sum(1)
+    # a score is off by 68 roundings of 2^-24 of at most 64 x 25 / 8
+    assert bool(((w[37, :, :n].double() - p).abs() <= p * 2.0 ** -8 + 2.0 ** -40).all())
+    w[37, :, :n] = 0
+    assert not bool(w.any())

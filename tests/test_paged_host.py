@@ -215,3 +215,17 @@ def test_abi_refuses_scales_that_are_not_finite():
     L, c = N.lib(), ctypes.byref(cache())
     for scale in (float("inf"), -float("inf"), float("nan"), 3e38, -2.4e38):
         assert L.otf_paged_attn(c, FAKE, 256, 4, 1, scale, FAKE, 256, None, 0, FAKE, 1 << 40, None) == INVALID
+
+
+def test_attention_workspace_is_bounded():
+    """Scratch for the scores of tables with much room: 2 GiB at most, or one KV head's; small calls as before."""
+    from otf_llm import _native as N
+    f = N.lib().otf_paged_attn_workspace_bytes
+    for batch, heads, kv, tokens, most in ((64, 64, 8, 16, 131072), (64, 64, 8, 1, 131072), (4096, 8, 8, 5, 8192),
+                                           (1, 128, 8, 16, 1 << 20), (3, 128, 4, 16, 1 << 20)):
+        one = heads // kv * tokens * most * 4
+        plain = f(batch, heads, kv, 128, tokens, most, 0)
+        assert plain <= 16 << 20
+        assert plain + one <= f(batch, heads, kv, 128, tokens, most, 1) <= plain + max(one, 2 << 30) + (8 << 20)
+    n = f(16, 32, 8, 128, 5, 4020, 1) - f(16, 32, 8, 128, 5, 4020, 0)
+    assert 16 * 8 * 20 * 4020 * 4 <= n <= 16 * 8 * 20 * 4020 * 4 + 16 * 8 * 20 * 4 + 512
