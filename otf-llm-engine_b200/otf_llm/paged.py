@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 
@@ -113,7 +113,8 @@ class PagedKVCache:
     lengths: int32 [batch], the tokens that each sequence has cached, negative for a place
     without a sequence (left as it is by every call).  The tensors stay the caller's and are
     changed in place: pages are handed out by writing the table, and ``advance`` counts a step's
-    tokens once every layer has appended them (layers may share table and lengths).
+    tokens, a prompt's too, once every layer has appended and attended them (layers may share
+    table and lengths).
 
     Tokens and sequences that do not fit, and pages outside the pool, are left out on the device
     and raise the ``_native.device_error`` flag (see include/otf_b200.h)."""
@@ -382,9 +383,15 @@ class PagedKVCache:
               budget, recent, kept.data_ptr(), self._vector(lengths_out, "lengths_out", self.batch))
         return kept
 
-    def advance(self, tokens: int = 1) -> None:
-        """lengths += tokens, where there is a sequence."""
-        self.lengths.add_(self.lengths.ge(0).to(torch.int32), alpha=int(tokens))
+    def advance(self, tokens: Union[int, torch.Tensor] = 1) -> None:
+        """lengths += tokens, where there is a sequence: a number, or int32 [batch] on the device where the
+        sequences differ (``starts.diff()`` after prompts, ``accepted + 1`` after a pass over drafts)."""
+        there = self.lengths.ge(0).to(torch.int32)
+        if isinstance(tokens, torch.Tensor):
+            self._vector(tokens, "tokens", self.batch)
+            self.lengths.add_(there.mul_(tokens))
+        else:
+            self.lengths.add_(there, alpha=int(tokens))
 
     def _weights(self, t: torch.Tensor, name: str, least: int) -> int:
         if t.device != self.device or t.dtype != torch.float32 or t.dim() != 3 or not t.is_contiguous() or \

@@ -741,3 +741,92 @@ def test_attend_walks_long_sequences_under_a_bounded_grid(cuda_dev):
     assert bool(((w[37, :, :n].double() - p).abs() <= p * 2.0 ** -8 + 2.0 ** -40).all())
     w[37, :, :n] = 0
     assert not bool(w.any())
+
+
+def test_documented_flow_of_ragged_prompts_and_drafts(cuda_dev):
+    """Prompts of different lengths, decoded tokens, drafts of which each sequence keeps its own number, and
+    a cut, over two layers that share table and lengths, through ``advance`` alone: every attention is that
+    over the tokens that each sequence has kept."""
+    from otf_llm.paged import PagedKVCache, Rotary
+    from otf_llm.speculative import verify_drafts
+    dt, heads, kv, dim, page, batch, K, vocab = torch.float16, 4, 2, 64, 16, 4, 3, 300
+    g = torch.Generator().manual_seed(21)
+    prompts = [50, 9, 0, 31]                                # the third place has no sequence
+    table = torch.randperm(40, generator=g)[:32].to(torch.int32).view(batch, 8)
+    lengths = torch.tensor([0, 0, -1, 0], dtype=torch.int32, device=cuda_dev)
+    caches = [PagedKVCache.allocate(40, page, kv, dim, table.to(cuda_dev), lengths) for _ in range(2)]
+    rotary = Rotary(dim, device=cuda_dev)
+    kept = [[[] for _ in range(batch)] for _ in caches]     # the (key, value) rows of each layer and sequence
+    turned = list(prompts)                                  # tokens so far
+
+    def rows(n):
+        return [torch.randn(n, h, dim, generator=g).to(dt) for h in (heads, kv, kv)]
+
+    def turn(x, position):
+        return ref.rotate(x, position, rotary.frequencies, 1.0, dim, False)
+
+    def step(T):
+        """T rows of every sequence through both layers; what they are, kept in full by the caller."""
+        new, outs = [], []
+        for cache, have in zip(caches, kept):
+            q, k, v = rows(batch * T)
+            out = cache.attend(cache.append(q.to(cuda_dev), k.to(cuda_dev), v.to(cuda_dev), rotary).view(batch, T, heads, dim))
+            for b in range(batch):
+                if b == 2:
+                    continue
+                mine = [(turn(k[b * T + t], turned[b] + t).to(dt).double(), v[b * T + t].double()) for t in range(T)]
+                for t in range(T):
+                    seen = have[b] + mine[:t + 1]
+                    kk, vv = (torch.stack([pair[i] for pair in seen]) for i in (0, 1))
+                    y, p, mass, size = ref.attend(turn(q[b * T + t], turned[b] + t).to(dt), kk, vv, dim ** -0.5)
+                    # keys and queries turned in 64 bits may round to the other neighbour: an eps of either, so
+                    # 2 eps size of a score, which count in the product and in the sum below it
+                    tol = ref.attend_tolerance(y, mass, size, dim, dt) + 4 * torch.finfo(dt).eps * size * mass
+                    assert bool(((out[b, t].cpu().double() - y).abs() <= tol).all()), (b, t)
+                new.append((have[b], mine))
+            outs.append(out)
+        return new, outs
+
+    starts = torch.tensor([0] + prompts).cumsum(0).to(torch.int32)
+    for cache, have in zip(caches, kept):
+        q, k, v = rows(sum(prompts))
+        cache.append(q.to(cuda_dev), k.to(cuda_dev), v.to(cuda_dev), rotary, starts=starts.to(cuda_dev))
+        for b in range(batch):
+            have[b] += [(turn(k[starts[b] + t], t).to(dt).double(), v[starts[b] + t].double()) for t in range(prompts[b])]
+    caches[0].advance(starts.to(cuda_dev).diff())
+    assert lengths.tolist() == [50, 9, -1, 31]
+
+    for _ in range(2):
+        new, _ = step(1)
+        caches[0].advance()
+        for have, mine in new:
+            have += mine
+        turned[:] = [n + 1 for n in turned]
+    assert lengths.tolist() == [52, 11, -1, 33]
+    for want in ([3, 0, 0, 1], [1, 2, 0, 3]):               # drafts taken
+        new, outs = step(K + 1)
+        logits = torch.randn(batch, K + 1, vocab, generator=g).to(cuda_dev)
+        drafts = logits[:, :K].argmax(2)
+        for b in range(batch):
+            if want[b] < K:
+                drafts[b, want[b]] = (drafts[b, want[b]] + 1) % vocab
+        _, accepted = verify_drafts(logits, drafts, temperature=0.0)
+        assert accepted.tolist() == want
+        caches[0].advance(accepted + 1)
+        n = [b for b in range(batch) if b != 2] * 2
+        for b, (have, mine) in zip(n, new):
+            have += mine[:want[b] + 1]
+        turned[:] = [m + w + 1 for m, w in zip(turned, want)]
+        assert [x for x in lengths.tolist() if x >= 0] == [turned[b] for b in (0, 1, 3)] and int(lengths[2]) == -1
+    step(1)
+    assert flag() == 0
+
+
+def test_advance_refuses_what_is_no_number_for_each_sequence(cuda_dev):
+    cache, *_ = make(cuda_dev, [20, 30], 16, 2, 64, torch.float16)
+    for bad in (torch.ones(2, dtype=torch.int64, device=cuda_dev), torch.ones(3, dtype=torch.int32, device=cuda_dev),
+                torch.ones(2, dtype=torch.int32), torch.ones(4, dtype=torch.int32, device=cuda_dev)[::2],
+                torch.ones((), dtype=torch.int32, device=cuda_dev), torch.ones(2, device=cuda_dev)):
+        with pytest.raises(ValueError):
+            cache.advance(bad)
+    assert cache.lengths.tolist() == [20, 30]
