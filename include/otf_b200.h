@@ -503,6 +503,17 @@ OTF_API int otf_paged_append(const otf_paged_cache* cache, const otf_rotary* rot
                              int64_t ldv, const int32_t* starts, const int32_t* positions, int64_t n, void* stream);
 
 /*
+ * The same, and the new tokens' entries of weights (fp32 [batch, kv_heads, ldw], as otf_paged_attn adds
+ * them up; ldw >= max_pages * page_size; NULL: otf_paged_append) are set to 0: what drafted tokens
+ * that were refused, or an earlier sequence of the same place of the batch, received there is not
+ * the new tokens'.  What the rows of refused tokens gave to the tokens before them stays.
+ */
+OTF_API int otf_paged_append_weights(const otf_paged_cache* cache, const otf_rotary* rotary, const void* q,
+                                     int64_t ldq, void* q_out, int64_t ldqo, int64_t heads, const void* k,
+                                     int64_t ldk, const void* v, int64_t ldv, const int32_t* starts,
+                                     const int32_t* positions, int64_t n, float* weights, int64_t ldw, void* stream);
+
+/*
  * Attention of the `tokens` (1..16) newest tokens of every sequence over its pages: row
  * b * tokens + t of q ([batch * tokens, heads, head_dim], row stride ldq) sees the tokens
  * 0 .. lengths[b] + t (its own key among them: otf_paged_append ran before, lengths not yet

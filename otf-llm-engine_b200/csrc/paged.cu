@@ -42,6 +42,8 @@ struct AppendArgs {
   const int* starts;
   const int* positions;
   int per;    // rows of a sequence, without starts
+  float* weights;  // or null: their entries of the new tokens are cleared
+  int64_t ldw;
 };
 
 // Where a row goes: the offset of its token's page row, or -1 (all its threads agree; `t` of `threads`).
@@ -64,6 +66,8 @@ __device__ __forceinline__ int64_t append_place(const AppendArgs& a, int row, in
     if (t == 0) report_bad_page();
     return -1;
   }
+  if (a.weights)
+    for (int g = t; g < c.kv_heads; g += threads) a.weights[((int64_t)b * c.kv_heads + g) * a.ldw + slot] = 0.0f;
   const int position = a.positions ? a.positions[row] : (int)slot;
   for (int p = t; p < a.rot / 2; p += threads) {
     // the angle in turns, 64 bits until the whole turns are gone: what is left keeps 2^-25 of a turn
@@ -612,6 +616,15 @@ extern "C" OTF_API int otf_paged_append(const otf_paged_cache* cache, const otf_
                                         int64_t ldq, void* q_out, int64_t ldqo, int64_t heads, const void* k,
                                         int64_t ldk, const void* v, int64_t ldv, const int32_t* starts,
                                         const int32_t* positions, int64_t n, void* stream) {
+  return otf_paged_append_weights(cache, rotary, q, ldq, q_out, ldqo, heads, k, ldk, v, ldv, starts, positions, n,
+                                  nullptr, 0, stream);
+}
+
+extern "C" OTF_API int otf_paged_append_weights(const otf_paged_cache* cache, const otf_rotary* rotary, const void* q,
+                                                int64_t ldq, void* q_out, int64_t ldqo, int64_t heads, const void* k,
+                                                int64_t ldk, const void* v, int64_t ldv, const int32_t* starts,
+                                                const int32_t* positions, int64_t n, float* weights, int64_t ldw,
+                                                void* stream) {
   otf::PagedView c;
   int st = otf::view_of(cache, c);
   if (st != OTF_OK) return st;
@@ -621,6 +634,7 @@ extern "C" OTF_API int otf_paged_append(const otf_paged_cache* cache, const otf_
   if (!otf::rows16(k, ldk, c.kv_heads * D) || !otf::rows16(v, ldv, c.kv_heads * D)) return OTF_ERR_INVALID;
   if (q && (heads <= 0 || heads > 65535 || !otf::rows16(q, ldq, heads * D) || !otf::rows16(q_out, ldqo, heads * D)))
     return OTF_ERR_INVALID;
+  if (weights && ldw < c.capacity) return OTF_ERR_INVALID;
   int rot = 0;
   if (rotary) {
     if (rotary->rot_dim < 0 || rotary->rot_dim > D || rotary->rot_dim % 2 || (rotary->rot_dim && !rotary->turns))
@@ -645,7 +659,9 @@ extern "C" OTF_API int otf_paged_append(const otf_paged_cache* cache, const otf_
                        q ? (int)heads : 0,
                        starts,
                        positions,
-                       (int)(n / c.batch)};
+                       (int)(n / c.batch),
+                       weights,
+                       ldw};
   const bool bf = cache->dtype == OTF_DTYPE_BF16;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const dim3 grid((unsigned)n);

@@ -128,6 +128,7 @@ EXPORTS = (
     "otf_pos_advance_batch",
     "otf_attn_prefill",
     "otf_paged_append",
+    "otf_paged_append_weights",
     "otf_paged_attn_workspace_bytes",
     "otf_paged_attn",
     "otf_paged_evict",
@@ -223,6 +224,8 @@ def lib() -> ctypes.CDLL:
     L.otf_paged_append.argtypes = [cache, ctypes.POINTER(RotaryArgs), vp, i64, vp, i64, i64, vp, i64, vp, i64, vp, vp,
                                    i64, vp]
     L.otf_paged_append.restype = i32
+    L.otf_paged_append_weights.argtypes = L.otf_paged_append.argtypes[:-1] + [vp, i64, vp]
+    L.otf_paged_append_weights.restype = i32
     L.otf_paged_attn_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i64, i32]
     L.otf_paged_attn_workspace_bytes.restype = i64
     L.otf_paged_attn.argtypes = [cache, vp, i64, i64, i64, ctypes.c_float, vp, i64, vp, i64, vp, i64, vp]

@@ -224,7 +224,8 @@ class PagedKVCache:
 
     def append(self, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, rotary: Optional[Rotary] = None, *,
                starts: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
-               q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+               q_out: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None
+               ) -> Optional[torch.Tensor]:
         """New tokens enter the cache (otf_paged_append).
 
         q [n, heads, head_dim] (or None), k and v [n, kv_heads, head_dim]: rows of new tokens, e.g.
@@ -233,7 +234,11 @@ class PagedKVCache:
         and turns by that position, or by positions[row] (int32 [n]) where places and positions
         differ (after ``evict``).  Returns the turned queries, in ``q_out`` (which may be q) or a new
         tensor.  Rows behind the last sequence are left as they were, as are those of a negative
-        length.  ``lengths`` is not advanced."""
+        length.  ``lengths`` is not advanced.
+
+        ``weights``, as ``attend`` adds them up: the new tokens' entries are set to 0.  Give them wherever
+        earlier tokens may have held these places: drafted ones that were refused, or those of the
+        sequence before in this place of the batch."""
         key = (None if q is None else (q.shape, q.stride()), k.shape, k.stride(), v.shape, v.stride())
         plan = self._append_plans.get(key)
         if plan is None:
@@ -264,7 +269,12 @@ class PagedKVCache:
             pp = self._vector(positions, "positions", n)
         if rotary is not None and (rotary.head_dim != self.head_dim or rotary.device != self.device):
             raise ValueError(f"rotary is for heads of {rotary.head_dim} on {rotary.device}")
-        if n:
+        if weights is not None:
+            ldw = self._weights(weights, "weights", self.capacity)
+            if n:
+                _call(_native.lib().otf_paged_append_weights, dev, self._ref, None if rotary is None else rotary._ref, pq, ldq,
+                      po, ldo, heads, pk, ldk, pv, ldv, ps, pp, n, weights.data_ptr(), ldw)
+        elif n:
             _call(_native.lib().otf_paged_append, dev, self._ref, None if rotary is None else rotary._ref, pq, ldq, po,
                   ldo, heads, pk, ldk, pv, ldv, ps, pp, n)
         return q_out
@@ -295,7 +305,7 @@ class PagedKVCache:
         sequence b sees the tokens 0 .. lengths[b] + t.  ``scale`` defaults to head_dim ** -0.5.
         ``weights`` (fp32 [batch, kv_heads, at least capacity], contiguous): to every token's entry
         is added the softmax weight that it received from the rows and the query heads of that KV
-        head.  Scratch for them grows with the table's room, not the lengths: 4 bytes x batch x heads x
+        head (rows of drafted tokens that are refused afterwards have added theirs).  Scratch for them grows with the table's room, not the lengths: 4 bytes x batch x heads x
         tokens x capacity, at most 2 GiB at a time (the call then takes several passes).  A cache made
         over fewer columns of a large table, ``page_table[:, :n]``, needs and walks less.  Returns ``out``,
         of q's shape (rows of negative lengths are left as they were)."""

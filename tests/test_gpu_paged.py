@@ -830,3 +830,81 @@ def test_advance_refuses_what_is_no_number_for_each_sequence(cuda_dev):
         with pytest.raises(ValueError):
             cache.advance(bad)
     assert cache.lengths.tolist() == [20, 30]
+
+
+@pytest.mark.parametrize("heads,kv,dim,rot,page", [(4, 2, 64, 64, 16), (32, 8, 128, 128, 20), (28, 4, 128, 24, 3), (0, 3, 64, 0, 16)])
+def test_append_clears_the_weights_of_new_tokens(heads, kv, dim, rot, page, cuda_dev):
+    """Nothing else of the weights changes, and what is appended is what it is without them."""
+    from otf_llm.paged import PagedKVCache, Rotary
+    lengths, new = [5, 0, -1, 33, 7], [3, 40, 2, 1, 5]
+    cache, pools, table, g = make(cuda_dev, lengths, page, kv, dim, torch.float16, room=[80] * 5)
+    cache.page_table[4] = -1                                # its tokens are left out
+    other = PagedKVCache(cache.k_pages.clone(), cache.v_pages.clone(), cache.page_table, cache.lengths)
+    rotary = Rotary(dim, rot_dim=rot, device=cuda_dev)
+    n = sum(new) + 2
+    q, k, v = (torch.randn(n, h, dim, generator=g).half().to(cuda_dev) if h else None for h in (heads, kv, kv))
+    starts = torch.tensor([0] + new).cumsum(0).to(torch.int32).to(cuda_dev)
+    w0 = torch.rand(5, kv, cache.capacity + 7, generator=g) + 0.5
+    w = w0.to(cuda_dev)
+    out = None if q is None else torch.zeros_like(q)
+    cache.append(q, k, v, rotary, starts=starts, q_out=out, weights=w)
+    assert flag() == 1
+    want = None if q is None else torch.zeros_like(q)
+    other.append(q, k, v, rotary, starts=starts, q_out=want)
+    assert flag() == 1 and same(cache.k_pages, other.k_pages) and same(cache.v_pages, other.v_pages)
+    assert q is None or torch.equal(out, want)
+    for b in (0, 1, 3):
+        w0[b, :, lengths[b]:lengths[b] + new[b]] = 0
+    assert torch.equal(w.cpu(), w0)
+    for bad in (w[..., :cache.capacity - 1].contiguous(), w.half(), w[:4], w.cpu(), w[..., 1:]):
+        with pytest.raises(ValueError):
+            cache.append(q, k, v, rotary, starts=starts, weights=bad)
+
+
+def test_weights_after_refused_drafts_and_a_new_sequence(cuda_dev):
+    """Drafts attended with weights, some refused, the next tokens in their places, a cut: the weights are those
+    of the tokens that there are, from all rows that attended; and a new sequence in a place starts at 0."""
+    dt, heads, kv, dim, page, T = torch.float16, 4, 2, 64, 16, 5
+    cache, pools, table, g = make(cuda_dev, [0, 0, 0], page, kv, dim, dt, room=[96] * 3, fill=0.0)
+    weights = torch.zeros(3, kv, cache.capacity, device=cuda_dev)
+    have = [0, 0, 0]
+    want, tol = (torch.zeros(3, kv, cache.capacity, dtype=torch.float64) for _ in range(2))
+
+    def step(tokens, taken):
+        q, k, v = (torch.randn(3 * tokens, h, dim, generator=g).to(dt) for h in (heads, kv, kv))
+        cache.append(None, k.to(cuda_dev), v.to(cuda_dev), weights=weights)
+        cache.attend(q.view(3, tokens, heads, dim).to(cuda_dev), weights=weights)
+        pages = cache.k_pages.cpu()
+        for b in range(3):
+            kk = ref.gather(pages, table, b, have[b] + tokens)
+            want[b, :, have[b]:have[b] + tokens] = tol[b, :, have[b]:have[b] + tokens] = 0
+            for t in range(tokens):
+                m = have[b] + t + 1
+                _, p, _, size = ref.attend(q[b * tokens + t], kk[:m], kk[:m], dim ** -0.5)
+                want[b, :, :m] += p.view(kv, -1, m).sum(1)
+                tol[b, :, :m] += (p * (size * 2.0 ** -14 + 2.0 ** -18)).view(kv, -1, m).sum(1) + 2.0 ** -22
+            have[b] += taken[b]
+        cache.advance(torch.tensor(taken, dtype=torch.int32, device=cuda_dev))
+
+    def check():
+        assert cache.lengths.tolist() == have
+        for b, n in enumerate(have):
+            # the roundings of the scores (68 of 2^-24 of their size, twice), of the exponentials and of the sums
+            assert bool(((weights[b, :, :n].cpu().double() - want[b, :, :n]).abs() <= tol[b, :, :n]).all()), b
+
+    for taken in ([5, 1, 3], [1, 5, 2], [4, 4, 1], [5, 5, 5], [2, 1, 5], [5, 5, 3]):
+        step(T, taken)
+        check()
+    step(1, [1, 1, 1])
+    check()
+    cache.lengths[1] = have[1] = 0                          # another sequence takes the second place
+    step(9, [9, 9, 9])
+    step(1, [1, 1, 1])
+    check()
+    before = weights.cpu()
+    kept = cache.evict(weights, 12, 4).cpu()
+    for b in range(3):
+        for h in range(kv):
+            keep = ref.evict(before[b, h], have[b], 12, 4)
+            assert kept[b, h].tolist() == keep + [-1] * (12 - len(keep))
+    assert flag() == 0

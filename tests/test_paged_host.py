@@ -229,3 +229,13 @@ def test_attention_workspace_is_bounded():
         assert plain + one <= f(batch, heads, kv, 128, tokens, most, 1) <= plain + max(one, 2 << 30) + (8 << 20)
     n = f(16, 32, 8, 128, 5, 4020, 1) - f(16, 32, 8, 128, 5, 4020, 0)
     assert 16 * 8 * 20 * 4020 * 4 <= n <= 16 * 8 * 20 * 4020 * 4 + 16 * 8 * 20 * 4 + 512
+
+
+def test_abi_append_with_weights_refuses():
+    from otf_llm import _native as N
+    L, c = N.lib(), ctypes.byref(cache())
+
+    def append(w=FAKE, ldw=64, n=3, k=FAKE):
+        return L.otf_paged_append_weights(c, None, None, 0, None, 0, 0, k, 128, FAKE, 128, None, None, n, w, ldw, None)
+    assert append(n=0) == 0
+    assert append(ldw=63) == INVALID and append(n=4) == INVALID and append(k=None) == INVALID
