@@ -495,7 +495,9 @@ typedef struct otf_rotary {
  * (device int32 [n], may be NULL): the rows' rotary positions, where they are not those
  * tokens' places (after otf_paged_evict).  rotary may be NULL (nothing turns).  The pointers
  * are 16-byte aligned, the strides multiples of 8.  lengths is not advanced.  Arithmetic in
- * fp32, one rounding.  The pages that new tokens enter belong to one sequence each.
+ * fp32, one rounding.  The pages that new tokens enter belong to one sequence each.  q_out is q itself, with
+ * ldqo = ldq, or shares no memory with q, k and v (columns beside one another in one buffer share none);
+ * the rows lie outside the pools.
  * Beside otf_rope_kv, which turns whole heads of one position by fp16 tables.
  */
 OTF_API int otf_paged_append(const otf_paged_cache* cache, const otf_rotary* rotary, const void* q, int64_t ldq,
@@ -519,7 +521,8 @@ OTF_API int otf_paged_append_weights(const otf_paged_cache* cache, const otf_rot
  * 0 .. lengths[b] + t (its own key among them: otf_paged_append ran before, lengths not yet
  * advanced) and out (row stride ldo) = softmax(scale q k) v, query head j reading KV head
  * j / (heads / kv_heads).  What a row does not see does not reach it, whatever it holds.  scale
- * is finite, and so is scale log2(e) in fp32.
+ * is finite, and so is scale log2(e) in fp32.  out shares no memory with q (columns beside one another in
+ * one buffer share none).
  * weights (fp32 [batch, kv_heads, ldw], may be NULL; ldw >= max_pages * page_size):
  * weights[b, h, s] += the softmax weight that token s received from the rows and query heads of
  * KV head h, for otf_paged_evict.  Scores, sums and outputs in fp32, joined over the parts of
@@ -548,7 +551,8 @@ OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* q, int64_t 
  * (kv_heads, head_dim, batch, dtype, page_size) and room for budget tokens.  weights (fp32
  * [batch, kv_heads, ldw]) go along to weights_out ([batch, kv_heads, ldw_out], may be weights),
  * zero behind the kept ones (in place: up to the old length).  lengths_out[b] = min(lengths[b],
- * budget).  Sequences within the budget are carried over whole.
+ * budget).  Sequences within the budget are carried over whole.  Beyond that, weights_out shares no memory
+ * with weights, nor lengths_out with from's lengths.
  */
 OTF_API int otf_paged_evict(const otf_paged_cache* from, const otf_paged_cache* to, const float* weights, int64_t ldw,
                             float* weights_out, int64_t ldw_out, int64_t budget, int64_t recent, int32_t* kept,

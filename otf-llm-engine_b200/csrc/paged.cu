@@ -635,6 +635,10 @@ extern "C" OTF_API int otf_paged_append_weights(const otf_paged_cache* cache, co
   if (q && (heads <= 0 || heads > 65535 || !otf::rows16(q, ldq, heads * D) || !otf::rows16(q_out, ldqo, heads * D)))
     return OTF_ERR_INVALID;
   if (weights && ldw < c.capacity) return OTF_ERR_INVALID;
+  if (q && (((q_out != q || ldqo != ldq) && otf::rows_overlap(q, ldq, heads * D, q_out, ldqo, heads * D, n)) ||
+            otf::rows_overlap(k, ldk, c.kv_heads * D, q_out, ldqo, heads * D, n) ||
+            otf::rows_overlap(v, ldv, c.kv_heads * D, q_out, ldqo, heads * D, n)))
+    return OTF_ERR_INVALID;
   int rot = 0;
   if (rotary) {
     if (rotary->rot_dim < 0 || rotary->rot_dim > D || rotary->rot_dim % 2 || (rotary->rot_dim && !rotary->turns))
@@ -692,14 +696,17 @@ extern "C" OTF_API int otf_paged_evict(const otf_paged_cache* from, const otf_pa
     return OTF_ERR_INVALID;
   if (budget <= 0 || recent < 0 || recent > budget || budget > t.capacity) return OTF_ERR_INVALID;
   if (ldw < f.capacity || ldw_out < budget || (weights == weights_out && ldw != ldw_out)) return OTF_ERR_INVALID;
-  st = check_device();
-  if (st != OTF_OK) return st;
   if (budget > 65535ll * otf::kMoveRows) return OTF_ERR_UNSUPPORTED;
   // cut in place: the same pools under the same table, and the weights with them
   const bool in_place = to->page_table == from->page_table && to->k_pages == from->k_pages && to->v_pages == from->v_pages;
   if (in_place != (weights == weights_out) || (!in_place && lengths_out == from->lengths)) return OTF_ERR_INVALID;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t pairs = f.batch * (int64_t)f.kv_heads;
+  if (!in_place && otf::bytes_overlap(weights, pairs * ldw * 4, weights_out, pairs * ldw_out * 4)) return OTF_ERR_INVALID;
+  if (lengths_out != from->lengths && otf::bytes_overlap(lengths_out, f.batch * 4, from->lengths, f.batch * 4))
+    return OTF_ERR_INVALID;
+  st = check_device();
+  if (st != OTF_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
   // CTAs per (sequence, KV head): as many as hold the weights that there can be in registers, while
   // that leaves less than two CTAs per SM
   int ctas = 1;

@@ -81,6 +81,27 @@ inline int view_of(const otf_paged_cache* c, PagedView& v) {
   return OTF_OK;
 }
 
+// Whether `rows` rows of 16-bit values share memory with as many others (strides and columns of each).
+// Views of one buffer whose columns lie beside one another share none.
+inline bool rows_overlap(const void* x, int64_t ldx, int64_t colx, const void* y, int64_t ldy, int64_t coly, int64_t rows) {
+  const int64_t at = (int64_t)(reinterpret_cast<intptr_t>(y) - reinterpret_cast<intptr_t>(x)) / 2;  // of y, from x on
+  if (at >= (rows - 1) * ldx + colx || -at >= (rows - 1) * ldy + coly) return false;
+  if (ldx == ldy) {
+    const int64_t col = (at % ldx + ldx) % ldx;
+    return col < colx || col + coly > ldx;
+  }
+  for (int64_t i = 0; i < rows; ++i) {  // the first of y's rows that ends behind the start of x's row i
+    const int64_t ahead = i * ldx - at - coly, j = ahead < 0 ? 0 : ahead / ldy + 1;
+    if (j < rows && at + j * ldy < i * ldx + colx) return true;
+  }
+  return false;
+}
+// The same of bytes that lie together.
+inline bool bytes_overlap(const void* x, int64_t nx, const void* y, int64_t ny) {
+  const intptr_t a = reinterpret_cast<intptr_t>(x), b = reinterpret_cast<intptr_t>(y);
+  return a < b + ny && b < a + nx;
+}
+
 inline bool rows16(const void* p, int64_t ld, int64_t cols) { return p && aligned16(p) && ld % 8 == 0 && ld >= cols; }
 
 }  // namespace otf

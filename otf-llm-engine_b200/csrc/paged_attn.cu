@@ -953,6 +953,7 @@ extern "C" OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* 
   if (heads <= 0 || heads % a.c.kv_heads || tokens <= 0 || !std::isfinite(scale * otf::kLog2e)) return OTF_ERR_INVALID;
   if (!otf::attn_limits(a.c.batch, heads, a.c.kv_heads, D, tokens, a.c.capacity)) return OTF_ERR_UNSUPPORTED;
   if (!otf::rows16(q, ldq, heads * D) || !otf::rows16(out, ldo, heads * D)) return OTF_ERR_INVALID;
+  if (otf::rows_overlap(q, ldq, heads * D, out, ldo, heads * D, a.c.batch * tokens)) return OTF_ERR_INVALID;
   if (weights && ldw < a.c.capacity) return OTF_ERR_INVALID;
   const otf::AttnSpace space = otf::attn_space(a.c.batch, heads, a.c.kv_heads, D, tokens, a.c.capacity, weights != nullptr);
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < space.bytes())

@@ -232,8 +232,8 @@ class PagedKVCache:
         parts of a fused projection's output.  Sequence b has the rows starts[b] .. starts[b + 1] - 1
         (int32 [batch + 1] on the device), or n / batch each; its t-th becomes token lengths[b] + t,
         and turns by that position, or by positions[row] (int32 [n]) where places and positions
-        differ (after ``evict``).  Returns the turned queries, in ``q_out`` (which may be q) or a new
-        tensor.  Rows behind the last sequence are left as they were, as are those of a negative
+        differ (after ``evict``).  Returns the turned queries, in ``q_out`` (which may be q, and else shares no
+        memory with q, k and v) or a new tensor.  Rows behind the last sequence are left as they were, as are those of a negative
         length.  ``lengths`` is not advanced.
 
         ``weights``, as ``attend`` adds them up: the new tokens' entries are set to 0.  Give them wherever
@@ -308,7 +308,7 @@ class PagedKVCache:
         head (rows of drafted tokens that are refused afterwards have added theirs).  Scratch for them grows with the table's room, not the lengths: 4 bytes x batch x heads x
         tokens x capacity, at most 2 GiB at a time (the call then takes several passes).  A cache made
         over fewer columns of a large table, ``page_table[:, :n]``, needs and walks less.  Returns ``out``,
-        of q's shape (rows of negative lengths are left as they were)."""
+        of q's shape, which shares no memory with q (rows of negative lengths are left as they were)."""
         key = (q.shape, q.stride(), weights is None)
         plan = self._attend_plans.get(key)
         if plan is None:

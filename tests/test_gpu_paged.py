@@ -908,3 +908,55 @@ def test_weights_after_refused_drafts_and_a_new_sequence(cuda_dev):
             keep = ref.evict(before[b, h], have[b], 12, 4)
             assert kept[b, h].tolist() == keep + [-1] * (12 - len(keep))
     assert flag() == 0
+
+
+def test_outputs_in_one_buffer_with_their_inputs(cuda_dev):
+    """Queries and outputs as views of one buffer: refused where they share an element, and otherwise right."""
+    import random
+
+    from test_paged_host import overlaps
+    cache, pools, table, g = make(cuda_dev, [20, 5, 33, 9, 17], 16, 2, 64, torch.float16, room=[48] * 5)
+    rng, seen = random.Random(4), [0, 0]
+    room = torch.randn(12000, generator=g).half().to(cuda_dev)
+    k, v = (torch.randn(5, 2, 64, generator=g).half().to(cuda_dev) for _ in range(2))
+    for _ in range(150):
+        ldq = ldo = 8 * rng.randint(32, 80)
+        if rng.random() < 0.4:
+            ldo = 8 * rng.randint(32, 80)
+        delta = 8 * rng.randint(-5 * 60, 5 * 60)
+        buf = room.clone()
+        q, out = (buf.as_strided((5, 4, 64), (ld, 64, 1), at) for ld, at in ((ldq, 4000), (ldo, 4000 + delta)))
+        over = overlaps(0, ldq, 256, delta, ldo, 256, 5)
+        seen[over] += 1
+        if over:
+            with pytest.raises((RuntimeError, ValueError)):
+                cache.attend(q, out=out)
+            if delta or ldq != ldo:
+                with pytest.raises((RuntimeError, ValueError)):
+                    cache.append(q, k, v, q_out=out)
+            assert torch.equal(buf, room)
+            continue
+        for call in (lambda o: cache.append(q, k, v, q_out=o), lambda o: cache.attend(q, out=o)):
+            call(out)
+            got = out.clone()
+            want = room.clone()
+            want.as_strided((5, 4, 64), (ldo, 64, 1), 4000 + delta).copy_(got)
+            assert torch.equal(buf, want) and torch.equal(got, call(None))
+    assert min(seen) > 20 and flag() == 0
+    # keys and values beside queries that are turned in place, as a fused projection leaves them
+    qkv = torch.randn(5, 8, 64, generator=g).half().to(cuda_dev)
+    q, k, v = qkv.split([4, 2, 2], dim=1)
+    want = cache.append(q, k, v).clone()
+    assert torch.equal(cache.append(q, k, v, q_out=q), want)
+    with pytest.raises(RuntimeError):
+        cache.append(q, k, v, q_out=qkv[:, 1:5])
+    # weights, and where they go to, beside one another
+    other, *_ = make(cuda_dev, [0] * 5, 16, 2, 64, torch.float16, room=[16] * 5, seed=9)
+    w = torch.rand(5 * 2 * (cache.capacity + 16), generator=g).to(cuda_dev)
+    cut = 5 * 2 * cache.capacity
+    weights, wo = w[:cut].view(5, 2, cache.capacity), w[cut:].view(5, 2, 16)
+    kept = cache.evict(weights, 16, 4, to=other, weights_out=wo)
+    assert bool((wo == torch.where(kept >= 0, weights.gather(2, kept.clamp(min=0).long()), 0.0)).all())
+    with pytest.raises(RuntimeError):
+        cache.evict(weights, 16, 4, to=other, weights_out=w[cut - 1:cut - 1 + 160].view(5, 2, 16))
+    assert flag() == 0

@@ -239,3 +239,53 @@ def test_abi_append_with_weights_refuses():
         return L.otf_paged_append_weights(c, None, None, 0, None, 0, 0, k, 128, FAKE, 128, None, None, n, w, ldw, None)
     assert append(n=0) == 0
     assert append(ldw=63) == INVALID and append(n=4) == INVALID and append(k=None) == INVALID
+
+
+def overlaps(x, ldx, colx, y, ldy, coly, rows):
+    """Element by element."""
+    return bool({x + i * ldx + c for i in range(rows) for c in range(colx)} &
+                {y + i * ldy + c for i in range(rows) for c in range(coly)})
+
+
+def test_abi_refuses_outputs_over_inputs():
+    """Queries and outputs in one buffer that share an element, as counted one by one (those that share none
+    are called on a GPU)."""
+    import random
+
+    from otf_llm import _native as N
+    L, c = N.lib(), cache(batch=5)
+    base, far, rng, seen = 1 << 40, 1 << 41, random.Random(3), 0
+    for _ in range(600):
+        ldq = ldo = 8 * rng.randint(32, 80)
+        if rng.random() < 0.4:
+            ldo = 8 * rng.randint(32, 80)
+        delta = 8 * rng.randint(-5 * 60, 5 * 60)
+        if overlaps(0, ldq, 256, delta, ldo, 256, 5):
+            seen += 1
+            assert L.otf_paged_attn(ctypes.byref(c), base, ldq, 4, 1, 1.0, base + 2 * delta, ldo, None, 0, FAKE, 1 << 40,
+                                    None) == INVALID, (ldq, ldo, delta)
+            if delta or ldq != ldo:                         # append's q_out may be q
+                assert L.otf_paged_append(ctypes.byref(c), None, base, ldq, base + 2 * delta, ldo, 4, far, 128, far, 128, None,
+                                          None, 5, None) == INVALID, (ldq, ldo, delta)
+        if overlaps(0, ldq, 128, delta, ldo, 256, 5):       # keys and values have 128 columns
+            for k, v in ((base, far), (far, base)):
+                assert L.otf_paged_append(ctypes.byref(c), None, far, 256, base + 2 * delta, ldo, 4, k, ldq, v, ldq, None, None, 5,
+                                          None) == INVALID, (ldq, ldo, delta)
+    assert seen > 200
+
+
+def test_abi_refuses_evictions_over_their_inputs():
+    from otf_llm import _native as N
+    L, c = N.lib(), cache()
+    to = cache(page_table=FAKE + 4096)
+    w, far = 1 << 40, 1 << 41                               # weights: 3 x 2 x 64 numbers
+
+    def evict(t, wo, ldwo=64, out=far):
+        return L.otf_paged_evict(ctypes.byref(c), ctypes.byref(t), w, 64, wo, ldwo, 8, 2, far + (1 << 20), out, None)
+    for wo in (w + 4, w - 4, w + 4 * 3 * 2 * 64 - 4, w - 4 * 3 * 2 * 64 + 4):
+        assert evict(to, wo) == INVALID
+    assert evict(to, w - 4 * 3 * 2 * 40 + 4, 40) == INVALID
+    for out in (FAKE + 4, FAKE - 8, FAKE):
+        assert evict(to, far + 4096, out=out) == INVALID
+    for out in (FAKE + 4, FAKE - 8):
+        assert evict(c, w, out=out) == INVALID
