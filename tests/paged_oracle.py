@@ -98,3 +98,35 @@ def verify(target, tokens, draft, uniforms, noise, temperature, count):
                 w = p
         last = int((w / noise.double()).argmax())
     return [int(x) for x in tokens[:taken]] + [last] + [-1] * (drafts - taken), taken
+
+
+def attend_tolerance_two(ref, mass, size, dim, dtype, n, largest):
+    """How far an output over n tokens (values of `largest` size at most) may be where probabilities go into the
+    products as two 16-bit numbers, hi and the rounded rest: the result's own rounding, half a step, and
+    - the scores' fp32 sums, as in attend_tolerance, twice (product and denominator);
+    - hi + rest: half a step of half a step of each probability, twice; 2^-22 for the exponential, twice;
+    - fp32 sums of 16 products at a time: (n / 16 + 32) roundings of 2^-23 (some hardware truncates), twice;
+    - fp16 alone: rests below its smallest number, 2^-33 of the largest probability for each token."""
+    u = torch.finfo(dtype).eps / 2
+    score = (dim + 4) * 2.0 ** -24 * size + size * 2.0 ** -22
+    rel = 2 * score + 2 * u * u + 2 * 2.0 ** -22 + 2 * (n / 16 + 32) * 2.0 ** -23
+    off = rel * mass + (n * 2.0 ** -33 * largest if dtype == torch.float16 else 0.0)
+    return u * (ref.abs() + off) + off + torch.finfo(dtype).tiny * u
+
+
+def attend_as_products_see(q, k, v, scale, dtype, rest=True, turned=False, lost=None):
+    """attend's output in float64 from probabilities rounded as the products take them: as two numbers of dtype, or
+    (planted mistakes) without the rest, with neighbours' rests exchanged, or without one token."""
+    rep = q.shape[0] // k.shape[1]
+    kk, vv = k.repeat_interleave(rep, 1), v.repeat_interleave(rep, 1)
+    s = torch.einsum("hd,nhd->hn", q.double(), kk) * scale
+    p = torch.exp(s - s.amax(-1, keepdim=True)) * (256 if dtype == torch.float16 else 1)
+    hi = p.to(dtype).double()
+    lo = (p - hi).to(dtype).double()
+    if turned:
+        m = lo.shape[1] // 2 * 2
+        lo[:, :m] = lo[:, :m].view(lo.shape[0], -1, 2).flip(-1).reshape(lo.shape[0], m)
+    p = hi + lo if rest else hi
+    if lost is not None:
+        p[:, lost] = 0
+    return (torch.einsum("hn,nhd->hd", p, vv) / p.sum(-1)[:, None]).to(dtype).double()

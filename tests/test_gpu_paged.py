@@ -960,3 +960,24 @@ def test_outputs_in_one_buffer_with_their_inputs(cuda_dev):
     with pytest.raises(RuntimeError):
         cache.evict(weights, 16, 4, to=other, weights_out=w[cut - 1:cut - 1 + 160].view(5, 2, 16))
     assert flag() == 0
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("tokens,heads,kv,dim,page", [(1, 8, 2, 64, 16), (1, 16, 2, 128, 16), (2, 24, 3, 64, 20), (5, 16, 4, 128, 16),
+                                                      (3, 8, 1, 128, 8), (16, 4, 2, 64, 32)])
+def test_attend_as_exact_as_its_output(tokens, heads, kv, dim, page, dtype, cuda_dev):
+    """Probabilities in two 16-bit numbers: the bound that tells a lost rest, and a lost token among hundreds, for
+    every number of row eights."""
+    dt, totals = TYPES[dtype], [2 + tokens, 5 + tokens, 17, 40, 300, 611]
+    cache, pools, table, g = make(cuda_dev, totals, page, kv, dim, dt, seed=tokens)
+    cache.lengths.sub_(tokens)
+    q = (0.3 * torch.randn(len(totals), tokens, heads, dim, generator=g)).to(dt)
+    out = cache.attend(q.to(cuda_dev)).cpu().double()
+    assert flag() == 0
+    for b, n in enumerate(totals):
+        k, v = (ref.gather(p, table, b, n) for p in pools)
+        for t in range(tokens):
+            m = n - tokens + t + 1
+            y, p, mass, size = ref.attend(q[b, t], k[:m], v[:m], dim ** -0.5)
+            tol = ref.attend_tolerance_two(y, mass, size, dim, dt, m, float(v.abs().max()))
+            assert bool(((out[b, t] - y).abs() <= tol).all()), (b, t, float(((out[b, t] - y).abs() / tol).max()))

@@ -289,3 +289,35 @@ def test_abi_refuses_evictions_over_their_inputs():
         assert evict(to, far + 4096, out=out) == INVALID
     for out in (FAKE + 4, FAKE - 8):
         assert evict(c, w, out=out) == INVALID
+
+
+# lengths, query heads, KV heads, head size: few tokens, where a probability's rounding shows, and some hundred
+# nearly equal ones, where a lost one does
+SHARP = [(2, 8, 2, 64), (5, 16, 4, 128), (17, 8, 1, 64), (300, 8, 2, 64), (611, 16, 2, 128)]
+
+
+def sharp_inputs(n, heads, kv, dim, dtype):
+    g = torch.Generator().manual_seed(n)
+    q = (0.3 * torch.randn(heads, dim, generator=g)).to(dtype)
+    k, v = (torch.randn(n, kv, dim, generator=g).to(dtype) for _ in range(2))
+    return q, k, v
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,heads,kv,dim", SHARP)
+def test_attention_tolerance_tells_mistakes(n, heads, kv, dim, dtype):
+    """The bound that the attention is held to admits probabilities of two 16-bit numbers, and not a rest left
+    out or exchanged (where few tokens share the mass) nor a token lost."""
+    import paged_oracle as ref
+    q, k, v = sharp_inputs(n, heads, kv, dim, dtype)
+    k, v = k.double(), v.double()
+    y, p, mass, size = ref.attend(q, k, v, dim ** -0.5)
+    tol = ref.attend_tolerance_two(y, mass, size, dim, dtype, n, float(v.abs().max()))
+
+    def off(**mistake):
+        return float(((ref.attend_as_products_see(q, k, v, dim ** -0.5, dtype, **mistake) - y).abs() / tol).max())
+    assert off() <= 1
+    for lost in (0, n // 2, n - 1):
+        assert off(lost=lost) > 2
+    if n <= 17:
+        assert off(rest=False) > 2 and off(turned=True) > 2
