@@ -242,9 +242,9 @@ constexpr int kEvictCluster = 8;     // CTAs that may share one (sequence, KV he
 // it is where its own places begin.  Of the keys equal to the k-th largest the first ones stay.
 // Bound by the rounds' latencies, not by bytes: ONE holds the keys of a slice of up to kEvictStrip
 // in registers through all rounds, longer ones are read again (from L2).  16 x 8 heads of 8191 weights
-// take 11 us.  BITS 11 (three rounds) for
-// a CTA by itself, 8 (four) in a cluster, whose CTAs read one another's counts: 65536 weights of 8
-// heads, with the copy, 26.1 us with 11, 21.6 us with 8.
+// take 11.3 us (12.9 after a flush of the caches).  BITS 11 (three rounds) for a CTA by itself, 8 (four) in
+// a cluster, whose CTAs read one another's counts: 65536 weights of 8 heads, with the copy, 26.1 us with
+// 11, 21.6 us with 8.
 template <bool ONE, int BITS>
 __global__ void __launch_bounds__(kEvictThreads) k_evict_select(const int* lengths, int kv_heads, int capacity,
                                                                 const float* weights, int64_t ldw, int budget,
@@ -434,8 +434,8 @@ __global__ void __launch_bounds__(kEvictThreads) k_evict_select(const int* lengt
 }
 
 // The kept rows' keys, values and weights, where source and target are apart: grid (pairs, tiles
-// of kMoveRows kept places).  One pass, memory-bound: 16 x 8 heads, 2048 rows kept, 233 MB in 38 us,
-// 6.1 TB/s.
+// of kMoveRows kept places).  One pass, memory-bound: 16 x 8 heads, 2048 rows kept, 233 MB in 39 us after
+// a flush of the caches, 6.0 TB/s, 42 us behind other calls, whose writes are still to leave L2.
 constexpr int kMoveRows = 64;
 
 struct MoveArgs {

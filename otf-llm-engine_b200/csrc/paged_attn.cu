@@ -18,13 +18,16 @@
 // Inside a CTA each warp is on its own: it takes 16 (head_dim 64: 32) tokens of every chunk through its
 // own ring of shared-memory stages, filled by 16-byte asynchronous copies some chunks ahead and
 // across items, and runs q k and p v on m16n8k16 matrix instructions.  The warps meet only at an
-// item's end.  The asynchronous 5th-generation products (128 rows at least) would be used to a
-// sixteenth here; these keep pace with the loads up to 16 rows.
+// item's end.  Up to 8 rows the loads decide (94 to 97% of the measured copy rate), and other products
+// would change nothing; at 20 rows memory is at 48%, held back by starts, item ends and 255 registers a
+// thread.  The asynchronous 5th-generation products would fit that side (keys, then dims, as their 128
+// rows, the query rows as the narrow side, outputs in tensor memory); they are not tried here.
 //
-// Measured (16-bit, head_dim 128, 8 KV heads; the whole call in a graph): one sequence of 131071
+// Measured (16-bit, head_dim 128, 8 KV heads; the whole call in a graph, calls on different inputs one
+// after another, caches as they leave them): one sequence of 131071
 // tokens, 64 heads, 537 MB, 87.8 us = 6.1 TB/s (k_paged_attn by itself 83 us, 6.4 TB/s); 64 sequences
 // of 127 to 8190 tokens, 1.09 GB, 181.7 us = 6.0 TB/s; one of 700 tokens 8.3 us, of which the joining
-// launch is 3; 16 of 62 to 4001 tokens, 20 rows an item, 39 us without and 55.6 us with weights.
+// launch, 4.1 by itself, is 3; 16 of 62 to 4001 tokens, 20 rows an item, 39 us without and 56.3 us with weights.
 //
 // The newest keys, which not every row sees, are masked in the steps that hold them; what they hold
 // cannot reach the other rows (see the loop).

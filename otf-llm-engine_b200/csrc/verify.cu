@@ -448,9 +448,9 @@ __global__ void __launch_bounds__(32 * W, 1024 / (32 * W) < 3 ? 1024 / (32 * W) 
 }
 
 // Step 1 alone: grid (blocks of 8 segments, row groups, batch), a warp per segment; the warps of a CTA
-// never meet.  64 sequences of 1 to 11 rows of 128256 and their draft's, 229 MB: 41 us by itself, 5.6 TB/s.  A
-// CTA goes through its group's rows, so that rows that a sequence with fewer drafted tokens does not
-// have cost nothing.
+// never meet.  64 sequences of 1 to 11 rows of 128256 and their draft's, 229 MB: 38.5 us by itself, 6.0 TB/s (41.6
+// after a flush of the caches).  A CTA goes through its group's rows, so that rows that a sequence with
+// fewer drafted tokens does not have cost nothing.
 __global__ void __launch_bounds__(kVerifyThreads, 4) k_verify_rows(VerifyArgs a) {
   pdl_trigger();
   pdl_wait();
@@ -464,9 +464,9 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) k_verify_rows(VerifyArgs a)
   }
 }
 
-// Step 2 alone: a CTA per sequence, a warp per row.  Latency-bound, 7 us for those 64 sequences: 32 warps
-// where there are more than 16 rows (4 sequences x 17 rows of 128256 21.0 us a call with 16, 19.5 with 32),
-// but not for more sequences than SMs (250 x 3 rows of 10000 23.1 and 26.5).
+// Step 2 alone: a CTA per sequence, a warp per row.  Latency-bound, 6.6 us for those 64 sequences (8.8 after a
+// flush of the caches): 32 warps where there are more than 16 rows (4 sequences x 17 rows of 128256 21.0 us
+// a call with 16, 19.5 with 32), but not for more sequences than SMs (250 x 3 rows of 10000 23.1 and 26.5).
 __global__ void __launch_bounds__(kPickThreads, 1) k_verify_pick(VerifyArgs a) {
   __shared__ RowPart s_row[kVerifyMaxRows];
   pdl_trigger();
@@ -515,7 +515,8 @@ __device__ __forceinline__ unsigned long long packed(const Leader& l) {
 // sequence's Pick by a maximum, which no order of the CTAs changes; the last CTA writes.  All CTAs run
 // at once, four on an SM: a second wave pays the start again (some 4 us: 64 sequences of 128256 entries 61 us
 // a call with 592 CTAs, 65 with 1184; 65 with two on an SM that request four pieces at a time; 64.7 with a
-// cluster of 4 per sequence, which left SMs with one CTA beside SMs with two).  By itself 23 us, 85 MB.
+// cluster of 4 per sequence, which left SMs with one CTA beside SMs with two).  By itself 20 us, 23 after a
+// flush of the caches, 85 MB.
 __global__ void __launch_bounds__(kVerifyThreads, 4) k_verify_race(VerifyArgs a, int per) {
   constexpr int U = 2, W = kVerifyWarps;
   __shared__ unsigned long long s_lead[W], s_best;

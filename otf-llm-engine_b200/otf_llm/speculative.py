@@ -29,8 +29,9 @@ def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, *,
     [batch, drafts, vocab], the logits that they were drawn from, or None where the draft was
     certain of them.  uniforms (fp32 [batch, drafts], in [0, 1)) decide which are taken, noise
     (fp32 [batch, vocab], exponentially distributed, e.g. ``torch.empty(...).exponential_()``)
-    which token follows; a temperature of 0 needs neither and takes what the target would have
-    picked greedily.  temperature: a number, or fp32 [batch] on the device.  counts: int32
+    which token follows; a temperature of 0 takes what the target would have picked greedily, and
+    needs neither where it is given as a number.  temperature: a number, or fp32 [batch] on the
+    device, which is not looked at beforehand: it needs both.  counts: int32
     [batch], how many drafted tokens each sequence has, where not all.
 
     Returns (tokens int64 [batch, drafts + 1]: the taken ones, the one that follows, then -1;
