@@ -540,6 +540,33 @@ OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* q, int64_t 
                            int64_t workspace_bytes, void* stream);
 
 /*
+ * Attention of rows of any number per sequence over its pages: prompts, decoded tokens and trees of drafted
+ * tokens, through a sliding window or not.  Sequence b has the rows [starts[b], starts[b + 1]) of q ([n, heads,
+ * head_dim], row stride ldq; starts: device int32 [batch + 1], or NULL: n / batch rows each), as
+ * otf_paged_append took them: row t is token lengths[b] + t, lengths not yet advanced.  out (row stride ldo, no
+ * memory shared with q) = softmax(scale q k) v over the tokens that a row sees, in fp32 with one rounding
+ * (and, where sequences have more than 128 rows of a KV head on average, one of each probability); what it does not see does not reach it, whatever it holds.
+ * parents NULL: row t, at place p = lengths[b] + t, sees the tokens s <= p, with a window (0: none) only those
+ * with s > p - window, and the first `sinks` tokens (sinks without a window: OTF_ERR_INVALID).
+ * parents (device int32 [n]): the rows of a sequence, 64 at most, are nodes of a tree (or of several); node t
+ * hangs on node parents[row] < t of the same sequence, or with -1 on the cached tokens alone.  It sees them,
+ * the nodes above it and itself; its place for the window is p = lengths[b] + the number of nodes above it.  A
+ * window then is 64 at least.  A parent out of range raises the otf_device_error flag and counts as -1.
+ * Sequences with a negative length are left as they are, and so are, with the flag raised, those whose rows do
+ * not lie in [0, n], do not fit the pages or are more than 64 nodes; rows behind the last sequence, too.  Tokens
+ * of a page not in [0, n_pages) read as zeros and raise the flag.  scale as in otf_paged_attn.  n heads /
+ * kv_heads at most 2^31 - 1.  workspace: otf_paged_attn_rows_workspace_bytes(...), 256-byte aligned, need not be
+ * cleared; two calls that may run at the same time need one each.  Beside otf_paged_attn, which takes as many
+ * newest tokens, 16 at most, of every sequence and adds up weights.
+ */
+OTF_API int64_t otf_paged_attn_rows_workspace_bytes(int64_t batch, int64_t n, int64_t heads, int64_t kv_heads,
+                                                    int64_t head_dim);
+OTF_API int otf_paged_attn_rows(const otf_paged_cache* cache, const void* q, int64_t ldq, int64_t heads,
+                                const int32_t* starts, int64_t n, const int32_t* parents, int64_t window,
+                                int64_t sinks, float scale, void* out, int64_t ldo, void* workspace,
+                                int64_t workspace_bytes, void* stream);
+
+/*
  * Eviction: every sequence longer than `budget` tokens is cut to it, for each KV head by
  * itself: the `recent` last tokens stay (0 <= recent <= budget), and of the others the
  * budget - recent of the largest weights (ties: the lower place; a NaN counts as the largest).

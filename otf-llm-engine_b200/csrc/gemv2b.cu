@@ -1926,6 +1926,7 @@ int attn_device_error(int clear);               // attention.cu
 int head_device_error(int clear);               // int8_ops.cu
 int paged_device_error(int clear);              // paged.cu
 int paged_attn_device_error(int clear);         // paged_attn.cu
+int paged_rows_device_error(int clear);         // paged_rows.cu
 int verify_device_error(int clear);             // verify.cu
 
 static int num_sms() {
@@ -2525,6 +2526,7 @@ extern "C" OTF_API int otf_device_error(int clear) {
   const int p = paged_device_error(clear);
   const int c = paged_attn_device_error(clear);
   const int d = verify_device_error(clear);
-  if (w < 0 || x < 0 || a < 0 || h < 0 || p < 0 || c < 0 || d < 0) return -1;
-  return v | w | x | a | h | p | c | d;
+  const int r = paged_rows_device_error(clear);
+  if (w < 0 || x < 0 || a < 0 || h < 0 || p < 0 || c < 0 || d < 0 || r < 0) return -1;
+  return v | w | x | a | h | p | c | d | r;
 }

@@ -48,6 +48,19 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
             : __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
 
+// Division of numbers below 2^31 by a fixed one.
+struct FastDiv {
+  uint32_t mul, shift, d;
+};
+inline FastDiv fast_div(uint32_t d) {
+  uint32_t l = 0;
+  while ((1ull << l) < d) ++l;
+  return FastDiv{(uint32_t)(((1ull << 32) * ((1ull << l) - d)) / d + 1), l, d};
+}
+__device__ __forceinline__ uint32_t operator/(uint32_t n, const FastDiv& f) {
+  return (__umulhi(f.mul, n) + n) >> f.shift;
+}
+
 // Whether a kernel's attributes still have to be set on the current device (done: per kernel, per device;
 // setting them twice does no harm).
 inline cudaError_t needs_opt_in(std::atomic<bool> (&done)[64], int& dev, bool& needs) {

@@ -53,19 +53,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 __device__ int g_paged_attn_device_error;
 __device__ __forceinline__ void report_bad_attn_page() { atomicExch(&g_paged_attn_device_error, 1); }
 
-// Division of numbers below 2^31 by a fixed one.
-struct FastDiv {
-  uint32_t mul, shift, d;
-};
-static FastDiv fast_div(uint32_t d) {
-  uint32_t l = 0;
-  while ((1ull << l) < d) ++l;
-  return FastDiv{(uint32_t)(((1ull << 32) * ((1ull << l) - d)) / d + 1), l, d};
-}
-__device__ __forceinline__ uint32_t operator/(uint32_t n, const FastDiv& f) {
-  return (__umulhi(f.mul, n) + n) >> f.shift;
-}
-
 struct AttnArgs {
   PagedView c;
   FastDiv page;

@@ -132,6 +132,8 @@ EXPORTS = (
     "otf_paged_attn_workspace_bytes",
     "otf_paged_attn",
     "otf_paged_evict",
+    "otf_paged_attn_rows_workspace_bytes",
+    "otf_paged_attn_rows",
     "otf_verify_workspace_bytes",
     "otf_verify_drafts",
 )
@@ -232,6 +234,10 @@ def lib() -> ctypes.CDLL:
     L.otf_paged_attn.restype = i32
     L.otf_paged_evict.argtypes = [cache, cache, vp, i64, vp, i64, i64, i64, vp, vp, vp]
     L.otf_paged_evict.restype = i32
+    L.otf_paged_attn_rows_workspace_bytes.argtypes = [i64, i64, i64, i64, i64]
+    L.otf_paged_attn_rows_workspace_bytes.restype = i64
+    L.otf_paged_attn_rows.argtypes = [cache, vp, i64, i64, vp, i64, vp, i64, i64, ctypes.c_float, vp, i64, vp, i64, vp]
+    L.otf_paged_attn_rows.restype = i32
     L.otf_verify_workspace_bytes.argtypes = [i64, i64, i64, i32]
     L.otf_verify_workspace_bytes.restype = i64
     L.otf_verify_drafts.argtypes = [vp, i64, i64, vp, i64, i64, vp, i64, vp, i64, vp, i64, vp, ctypes.c_float, vp, vp,

@@ -21,6 +21,7 @@ from . import _native
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 MAX_NEW_TOKENS = 16
+MAX_NODES = 64
 
 _SCALING_KEYS = {
     "default": (),
@@ -162,6 +163,7 @@ class PagedKVCache:
         # loop's calls differ in addresses alone
         self._append_plans: dict = {}
         self._attend_plans: dict = {}
+        self._rows_plans: dict = {}
 
     # the tensors are changed in place, never replaced: the native side holds their addresses
     @property
@@ -350,6 +352,83 @@ class PagedKVCache:
         if n < 0:
             raise ValueError("shape not supported by otf_paged_attn")
         return tokens, heads, ldq, n
+
+    def attend_rows(self, q: torch.Tensor, *, starts: Optional[torch.Tensor] = None, window: Optional[int] = None,
+                    sinks: int = 0, scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of rows of any number per sequence over the cache (otf_paged_attn_rows): prompts and
+        decoded tokens.
+
+        q [n, heads, head_dim]: the rows as ``append`` took them, sequence b's from starts[b] on (int32
+        [batch + 1] on the device) or n / batch each; all appended, ``lengths`` not yet advanced.  Row t of
+        sequence b, at place p = lengths[b] + t, sees the tokens up to its own; with a ``window`` only the last
+        ``window`` of them, places above p - window, and the first ``sinks`` of the sequence.  ``scale`` defaults
+        to head_dim ** -0.5.  Returns ``out``, of q's shape, which shares no memory with q (rows behind the
+        last sequence and of negative lengths are left as they were)."""
+        return self._attend_rows(q, None, starts, window, sinks, scale, out)
+
+    def attend_tree(self, q: torch.Tensor, parents: torch.Tensor, *, starts: Optional[torch.Tensor] = None,
+                    window: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of the nodes of drafted trees over the cache (otf_paged_attn_rows).
+
+        q [n, heads, head_dim]: the nodes' rows, up to 64 of a sequence, appended at the places lengths[b] + t
+        with the positions lengths[b] + depth.  parents (int32 [n] on the device): node t hangs on node
+        parents[row] < t of its sequence, or with -1 on the cached tokens alone.  A node sees the cached tokens
+        (with a ``window``, 64 at least, those within it by position, and the first ``sinks``), the nodes above
+        it and itself.  ``verify_tree`` chooses a way through the tree, and ``keep`` moves its nodes together.
+        The rest is as in ``attend_rows``."""
+        return self._attend_rows(q, parents, starts, window, sinks, scale, out)
+
+    def _attend_rows(self, q: torch.Tensor, parents: Optional[torch.Tensor], starts: Optional[torch.Tensor],
+                     window: Optional[int], sinks: int, scale: Optional[float], out: Optional[torch.Tensor]
+                     ) -> torch.Tensor:
+        key = (q.shape, q.stride())
+        plan = self._rows_plans.get(key)
+        if plan is None:
+            plan = self._remember(self._rows_plans, key, self._plan_rows(q))
+        n, heads, ldq, bytes_ = plan
+        pq, dev = q.data_ptr(), self.device
+        if q.dtype is not self.dtype or q.device != dev or pq & 15:
+            self._refuse(q=q)
+        least = 1 if parents is None else MAX_NODES
+        if window is not None and (int(window) != window or window < least):
+            raise ValueError(f"window must be a whole number from {least} on, got {window}")
+        if int(sinks) != sinks or sinks < 0 or (sinks and window is None):
+            raise ValueError(f"sinks must not be negative, and need a window, got {sinks}")
+        if out is None:
+            out = torch.empty_like(q)
+            ldo, po = heads * self.head_dim, out.data_ptr()
+        else:
+            ldo, po = self._output(out, "out", q)
+            if po == pq and n:
+                raise ValueError("out must not be q")
+        ps = pp = None
+        if starts is not None:
+            ps = self._vector(starts, "starts", self.batch + 1)
+        elif n % self.batch:
+            raise ValueError(f"{n} rows do not divide among {self.batch} sequences; give starts")
+        elif parents is not None and n // self.batch > MAX_NODES:
+            raise ValueError(f"a tree has at most {MAX_NODES} nodes, got {n // self.batch}")
+        if parents is not None:
+            pp = self._vector(parents, "parents", n)
+        if n:
+            # for this call alone, as in attend
+            ws = torch.empty(bytes_, dtype=torch.uint8, device=dev)
+            _call(_native.lib().otf_paged_attn_rows, dev, self._ref, pq, ldq, heads, ps, n, pp,
+                  0 if window is None else min(int(window), 1 << 40), min(int(sinks), 1 << 40),
+                  self._scale if scale is None else float(scale), po, ldo, ws.data_ptr(), bytes_)
+        return out
+
+    def _plan_rows(self, q: torch.Tensor) -> tuple:
+        ldq, n, heads = self._heads(q, "q"), q.shape[0], q.shape[1]
+        if heads % self.kv_heads:
+            raise ValueError(f"{heads} query heads over {self.kv_heads} KV heads")
+        size = 0
+        if n:
+            size = _native.lib().otf_paged_attn_rows_workspace_bytes(self.batch, n, heads, self.kv_heads, self.head_dim)
+            if size < 0:
+                raise ValueError("shape not supported by otf_paged_attn_rows")
+        return n, heads, ldq, size
 
     def evict(self, weights: torch.Tensor, budget: int, recent: int, *, to: Optional["PagedKVCache"] = None,
               weights_out: Optional[torch.Tensor] = None, lengths_out: Optional[torch.Tensor] = None
