@@ -567,6 +567,17 @@ OTF_API int otf_paged_attn_rows(const otf_paged_cache* cache, const void* q, int
                                 int64_t workspace_bytes, void* stream);
 
 /*
+ * The taken nodes of a tree move together: for j < accepted[b] (device int32 [batch], 0..depth) the keys and
+ * values of place lengths[b] + path[b, j] (device int32 [batch, ld_path], as otf_verify_tree gives it) go to place
+ * lengths[b] + 1 + j, behind the root at lengths[b]; lengths is not advanced.  All of a KV head's are read before the
+ * first is written, so that the ways may cross, but each sequence's pages are its own.  A path entry that is negative or whose
+ * place is outside the pages is left out and raises the otf_device_error flag; so is a sequence with a count
+ * out of range.  depth at most 63.
+ */
+OTF_API int otf_paged_keep(const otf_paged_cache* cache, const int32_t* path, int64_t ld_path,
+                           const int32_t* accepted, int64_t depth, void* stream);
+
+/*
  * Eviction: every sequence longer than `budget` tokens is cut to it, for each KV head by
  * itself: the `recent` last tokens stay (0 <= recent <= budget), and of the others the
  * budget - recent of the largest weights (ties: the lower place; a NaN counts as the largest).
@@ -618,6 +629,44 @@ OTF_API int otf_verify_drafts(const float* target, int64_t target_seq, int64_t l
                               const float* temperatures, float temperature, const int32_t* counts,
                               int64_t* out_tokens, int32_t* accepted, int64_t batch, int64_t drafts, int64_t vocab,
                               void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * A way through a tree of drafted tokens: at each node, from node 0 on, a token is drawn from the target's
+ * distribution behind it, softmax(target / T), as the i of the largest p_i / noise[b, step, i] (noise: exponentially
+ * distributed random numbers, not negative; ties: the lower index), and if a child holds that token (the first
+ * of several) the walk goes on there, else it ends; with `depth` children taken it ends behind the last one.
+ * T = 0: the first largest logit.  So every token is distributed as the target alone draws it.
+ * target: fp32 [n, ld_target], row of each node; tokens: int64 [n]; parents: int32 [n]; sequence b has the nodes
+ * [starts[b], starts[b + 1]) (device int32 [batch + 1], or NULL: n / batch each), 1 to 64, as in otf_paged_attn_rows:
+ * node 0 is the root, the last token that is certain (its own token is not looked at), and parents[i] < i.  noise:
+ * fp32, row (b, step) at noise + b * noise_seq + step * ld_noise, depth + 1 rows of a sequence (may be NULL when every
+ * temperature is 0).  temperatures: device fp32 [batch], or NULL: `temperature` for all; 0 or in 1e-20 .. 1e20.
+ * out_tokens: int64 [batch, depth + 1], the taken nodes' tokens and the one that follows, then -1; path: int32
+ * [batch, depth], the taken nodes, then -1; accepted: int32 [batch], how many.  A NaN among the logits counts as
+ * -inf; a token of weight 0 is never drawn.  A sequence without a token to draw, with rows not in [0, n], a number of
+ * nodes or a temperature out of range gets -1, 0 accepted, and raises the otf_device_error flag; so does a parent out of
+ * range, whose node hangs nowhere.  Scores that decide are compared in 64 bits.  depth 0..63; at most 65535
+ * sequences and a vocabulary of 2^30.  No workspace.  Beside otf_verify_drafts, for drafts in a line.
+ */
+OTF_API int otf_verify_tree(const float* target, int64_t ld_target, const int64_t* tokens, const int32_t* parents,
+                            const int32_t* starts, int64_t n, const float* noise, int64_t noise_seq, int64_t ld_noise,
+                            const float* temperatures, double temperature, int64_t* out_tokens, int32_t* path,
+                            int32_t* accepted, int64_t batch, int64_t depth, int64_t vocab, void* stream);
+
+/*
+ * Log probabilities: logits [n, vocab] (row stride ld; dtype OTF_DTYPE_F32, _F16 or _BF16), p = softmax of a row.
+ * tokens: int64 [n].  logprobs: fp32 [n], log p of the row's token; ranks: int32 [n], how many entries come before
+ * it (by logit, equal ones by the lower index; 0: the likeliest); entropy: fp32 [n], -sum p log p.  top (0..32):
+ * top_tokens int64 [n, top] and top_logprobs fp32 [n, top], the likeliest tokens in that order (may be NULL when top
+ * is 0).  A negative token asks for nothing: log probability 0, rank -1.  One that is not below vocab gets a NaN, rank
+ * -1, and raises the otf_device_error flag.  A NaN among the logits counts as -inf, +inf as the largest finite
+ * number.  Entries of -inf have no weight and are no alternatives: behind the last one -1 and -inf follow (a row of
+ * nothing else has log probability -inf and entropy 0).  Sums in fp32, without the largest entry, so that small
+ * entropies and log probabilities near 0 keep their precision.  A vocabulary of 2^30 at most, 2^26 rows.
+ */
+OTF_API int otf_token_logprobs(const void* logits, int64_t ld, int32_t dtype, const int64_t* tokens, int64_t n,
+                               int64_t vocab, int64_t top, float* logprobs, float* entropy, int32_t* ranks,
+                               int64_t* top_tokens, float* top_logprobs, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1928,6 +1928,8 @@ int paged_device_error(int clear);              // paged.cu
 int paged_attn_device_error(int clear);         // paged_attn.cu
 int paged_rows_device_error(int clear);         // paged_rows.cu
 int verify_device_error(int clear);             // verify.cu
+int verify_tree_device_error(int clear);        // verify_tree.cu
+int logprobs_device_error(int clear);           // logprobs.cu
 
 static int num_sms() {
   static thread_local int cached[64] = {};
@@ -2527,6 +2529,8 @@ extern "C" OTF_API int otf_device_error(int clear) {
   const int c = paged_attn_device_error(clear);
   const int d = verify_device_error(clear);
   const int r = paged_rows_device_error(clear);
-  if (w < 0 || x < 0 || a < 0 || h < 0 || p < 0 || c < 0 || d < 0 || r < 0) return -1;
-  return v | w | x | a | h | p | c | d | r;
+  const int t = verify_tree_device_error(clear);
+  const int l = logprobs_device_error(clear);
+  if (w < 0 || x < 0 || a < 0 || h < 0 || p < 0 || c < 0 || d < 0 || r < 0 || t < 0 || l < 0) return -1;
+  return v | w | x | a | h | p | c | d | r | t | l;
 }

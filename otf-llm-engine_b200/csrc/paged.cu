@@ -594,6 +594,63 @@ __global__ void k_evict_lengths(MoveArgs a) {
   for (int b = blockIdx.x * blockDim.x + threadIdx.x; b < a.from.batch; b += gridDim.x * blockDim.x) set_length(a, b);
 }
 
+// The taken nodes of a tree (otf_paged_keep): keys and values of the places lengths + path[j] move to
+// lengths + 1 + j.  A CTA per sequence and KV head fetches all of them before it writes the first, so that
+// the ways may cross; latency-bound: a chain of the path, the table, the rows.
+constexpr int kKeepThreads = 128;
+constexpr int kKeepMost = 63;
+
+template <int D>
+__global__ void __launch_bounds__(kKeepThreads) k_paged_keep(PagedView c, const int* path, int64_t ldp, const int* accepted, int depth) {
+  constexpr int P = D / 8;  // 16-byte pieces of a row
+  __shared__ int64_t s_from[kKeepMost], s_to[kKeepMost];
+  extern __shared__ uint4 s_rows[];  // [2 n P]
+  pdl_trigger();
+  pdl_wait();
+  const int g = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const int len = c.lengths[b], n = accepted[b];
+  if (len < 0 || n == 0) return;
+  if (n < 0 || n > depth) {
+    if (tid == 0 && g == 0) report_bad_page();
+    return;
+  }
+  auto place = [&](int64_t s) -> int64_t {
+    if (s >= c.capacity) return -1;
+    const int page = c.table[b * c.ld_table + s / c.page_size];
+    return page < 0 || page >= c.n_pages ? -1 : page * c.page_stride + s % c.page_size * c.token_stride;
+  };
+  if (tid < n) {
+    const int from = path[b * ldp + tid];
+    int64_t x = -1, y = -1;
+    if (from >= 0) {
+      x = place((int64_t)len + from);
+      y = place((int64_t)len + 1 + tid);
+    }
+    if (x < 0 || y < 0) {
+      report_bad_page();
+      x = -1;
+    } else if (x == y) {
+      x = -1;  // there already
+    }
+    s_from[tid] = x;
+    s_to[tid] = y;
+  }
+  __syncthreads();
+  const int64_t head = g * c.head_stride;
+#pragma unroll 4
+  for (int i = tid; i < 2 * n * P; i += kKeepThreads) {
+    const int j = i / (2 * P), piece = i % P;
+    const int64_t x = s_from[j];
+    if (x >= 0) s_rows[i] = *reinterpret_cast<const uint4*>((i / P & 1 ? c.v : c.k) + x + head + piece * 8);
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int i = tid; i < 2 * n * P; i += kKeepThreads) {
+    const int j = i / (2 * P), piece = i % P;
+    if (s_from[j] >= 0) *reinterpret_cast<uint4*>((i / P & 1 ? c.v : c.k) + s_to[j] + head + piece * 8) = s_rows[i];
+  }
+}
+
 }  // namespace otf
 
 using otf::check_device;
@@ -728,4 +785,19 @@ extern "C" OTF_API int otf_paged_evict(const otf_paged_cache* from, const otf_pa
   const int64_t tiles = (budget + otf::kMoveRows - 1) / otf::kMoveRows;
   return set_cuda_error(otf::launch_pdl(from->head_dim == 128 ? otf::k_evict_copy<128> : otf::k_evict_copy<64>,
                                         dim3((unsigned)pairs, (unsigned)tiles), dim3(256), 0, s, 1u, a));
+}
+
+extern "C" OTF_API int otf_paged_keep(const otf_paged_cache* cache, const int32_t* path, int64_t ld_path,
+                                      const int32_t* accepted, int64_t depth, void* stream) {
+  otf::PagedView c;
+  int st = otf::view_of(cache, c);
+  if (st != OTF_OK) return st;
+  if (!accepted || depth < 0 || (depth && (!path || ld_path < depth))) return OTF_ERR_INVALID;
+  if (depth > otf::kKeepMost) return OTF_ERR_UNSUPPORTED;
+  st = check_device();
+  if (st != OTF_OK || depth == 0) return st;
+  const int64_t bytes = 2 * depth * cache->head_dim * 2;
+  return set_cuda_error(otf::launch_pdl(cache->head_dim == 128 ? otf::k_paged_keep<128> : otf::k_paged_keep<64>,
+                                        dim3((unsigned)c.kv_heads, (unsigned)c.batch), dim3(otf::kKeepThreads), (size_t)bytes,
+                                        static_cast<cudaStream_t>(stream), 1u, c, path, ld_path, accepted, (int)depth));
 }

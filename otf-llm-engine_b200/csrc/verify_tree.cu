@@ -1,0 +1,262 @@
+// A way through a tree of drafted tokens (otf_verify_tree).
+//
+// At each node, from the root on, the token that follows is drawn from the target's own distribution behind
+// that node, p = softmax(target / T), as argmax_i p_i / e_i with e_i ~ Exp(1) given; a child that holds it is
+// taken and the walk goes on there, else it ends.  Whatever the tree holds, every token is one of the
+// target's distribution.  In logarithms the leader is the largest x_i / T - log e_i, which needs no sum:
+// a step is one pass over one row of logits and one of noise, and only the rows on the way are read.
+//
+// An entry is weighed in fp32 with a bound on its error; only those that may lead are computed in 64 bits.
+//
+// A sequence is walked by a cluster of CTAs that cut the vocabulary among them; a step's leaders meet in
+// distributed shared memory.  Bound: a step's rows are 8 bytes per entry, but a step cannot start before the
+// one before it has ended, so few sequences are bound by latency.
+#include <algorithm>
+#include <cfloat>
+
+#include "logits.cuh"
+#include "paged.cuh"
+
+namespace otf {
+
+int set_cuda_error(cudaError_t e);        // capi.cu
+int check_device();                       // capi.cu
+int verify_tree_device_error(int clear);  // read (and optionally clear) the flag below
+
+constexpr int kTreeMaxNodes = 64;
+constexpr int kTreeThreads = 512;
+constexpr int kTreeWarps = kTreeThreads / 32;
+constexpr int kTreeCluster = 16;
+constexpr int kTreeResident = 148 * 4;  // CTAs that run at once
+
+// Set when a sequence has no token to draw, or an argument on the device is out of range.
+__device__ int g_verify_tree_device_error;
+
+struct TreeArgs {
+  const float* target;
+  int64_t ldt;
+  const int64_t* tokens;
+  const int* parents;
+  const int* starts;  // or null: `per` nodes each
+  const float* noise;
+  int64_t nseq, ldn;
+  const float* temperatures;
+  double temperature;
+  int64_t* out;       // [batch][depth + 1]
+  int* path;          // [batch][depth]
+  int* accepted;
+  int per, n, depth, vocab;
+};
+
+struct TreeLeader {
+  double score;
+  int at, pad;
+};
+__device__ __forceinline__ bool leads(double s, int i, const TreeLeader& l) { return s > l.score || (s == l.score && i < l.at); }
+
+// x / T - log e in 64 bits, or x at temperature 0.
+__device__ __forceinline__ double tree_score(float x, float e, double T) {
+  return T == 0.0 ? (double)x : (double)x / T - log((double)e);
+}
+
+__global__ void __launch_bounds__(kTreeThreads, 2) k_verify_tree(TreeArgs a, int ctas) {
+  __shared__ TreeLeader s_warp[kTreeWarps], s_all[2][kTreeCluster];
+  __shared__ float s_bar[kTreeWarps];
+  __shared__ int64_t s_tokens[kTreeMaxNodes + 1];
+  __shared__ int s_path[kTreeMaxNodes], s_at, s_taken;
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.x / ctas, rank = blockIdx.x - b * ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int r0 = a.starts ? a.starts[b] : b * a.per, r1 = a.starts ? a.starts[b + 1] : r0 + a.per, nodes = r1 - r0;
+  const double T = a.temperatures ? (double)a.temperatures[b] : a.temperature;
+  const bool ok = r0 >= 0 && r1 <= a.n && nodes > 0 && nodes <= kTreeMaxNodes && temperature_ok((float)T) && (T == 0.0 || a.noise);
+  cluster_arrive_relaxed();
+  // the nodes, two in each lane of the first warp
+  int64_t token[2] = {-1, -1};
+  int parent[2] = {-1, -1};
+  if (ok && warp == 0)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (lane + 32 * h < nodes) {
+        token[h] = a.tokens[r0 + lane + 32 * h];
+        parent[h] = a.parents[r0 + lane + 32 * h];
+        // not a node before it: it hangs nowhere
+        if (parent[h] >= lane + 32 * h || parent[h] < -1) {
+          if (rank == 0) atomicExch(&g_verify_tree_device_error, 1);
+          parent[h] = -1;
+        }
+      }
+  int at = 0, taken = 0;
+  bool failed = !ok;
+  const float c = T > 0.0 ? (float)(1.4426950408889634 / T) : 0.0f;
+  cluster_wait();  // all CTAs of the cluster run
+  for (int step = 0; !failed; ++step) {
+    const float* x = a.target + (int64_t)(r0 + at) * a.ldt;
+    const float* e = T > 0.0 ? a.noise + b * a.nseq + step * a.ldn : nullptr;
+    const bool ax = (reinterpret_cast<uintptr_t>(x) & 15) == 0, ae = (reinterpret_cast<uintptr_t>(e) & 15) == 0;
+    // a thread's first entry of the largest upper bound, the largest of the others, and what its entries score at least
+    float high = -INFINITY, next = -INFINITY, bar = -INFINITY, lead_x = 0.0f, lead_e = 1.0f;
+    int lead = INT_MAX;
+    constexpr int U = 4;
+    const int stride = 4 * kTreeThreads * ctas;
+    for (int i0 = 4 * (rank * kTreeThreads + tid); i0 < a.vocab; i0 += U * stride) {
+      float4 vx[U], ve[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = (int)min((int64_t)i0 + (int64_t)u * stride, (int64_t)a.vocab);  // behind the end: -inf without a read
+        vx[u] = logits4(x, i, a.vocab, ax);
+        if (e) ve[u] = logits4(e, i, a.vocab, ae, INFINITY);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float fx[4] = {vx[u].x, vx[u].y, vx[u].z, vx[u].w};
+        const float fe[4] = {ve[u].x, ve[u].y, ve[u].z, ve[u].w};
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          float up = fx[z], low = fx[z];
+          if (e) {
+            // two roundings of each term, and the logarithm's error, are below 2^-20 of them, and of 1
+            const float p = fx[z] * c, l = __log2f(fe[z]), d = p - l, w = 0x1p-20f * (fabsf(p) + fabsf(l) + 1.0f);
+            up = d + w;
+            low = d - w;
+            if (fabsf(p) == INFINITY) up = fx[z] == -INFINITY ? -INFINITY : fx[z] > 0.0f || fe[z] == 0.0f ? INFINITY : -FLT_MAX;
+          }
+          if (up > high) {
+            next = fmaxf(next, high);
+            high = up;
+            lead = i0 + u * stride + z;
+            lead_x = fx[z];
+            lead_e = e ? fe[z] : 1.0f;
+          } else if (up == up) {
+            next = fmaxf(next, up);
+          }
+          bar = fmaxf(bar, low);
+        }
+      }
+    }
+    float most = bar;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (lane == 0) s_bar[warp] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kTreeWarps; ++w) most = fmaxf(most, s_bar[w]);
+    TreeLeader mine = {-INFINITY, INT_MAX, 0};
+    if (high >= most && lead != INT_MAX) {
+      const double s = tree_score(lead_x, lead_e, T);
+      if (s > -INFINITY) mine = {s, lead, 0};
+      if (e && next >= most)  // another one of the thread's may lead: all of them in 64 bits
+        for (int i0 = 4 * (rank * kTreeThreads + tid); i0 < a.vocab; i0 += min(stride, a.vocab - i0))
+          for (int i = i0; i < min(i0 + 4, a.vocab); ++i) {
+            const double y = tree_score(x[i], e[i], T);
+            if (y > -INFINITY && leads(y, i, mine)) mine = {y, i, 0};
+          }
+    }
+    auto shared = [&](TreeLeader l) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const double s = __shfl_xor_sync(0xffffffffu, l.score, o);
+        const int i = __shfl_xor_sync(0xffffffffu, l.at, o);
+        if (i != INT_MAX && leads(s, i, l)) l = {s, i, 0};
+      }
+      return l;
+    };
+    mine = shared(mine);
+    if (lane == 0) s_warp[warp] = mine;
+    __syncthreads();
+    if (warp == 0) {
+      mine = shared(lane < kTreeWarps ? s_warp[lane] : TreeLeader{-INFINITY, INT_MAX, 0});
+      if (lane < ctas) {
+        const long long bits = __double_as_longlong(mine.score);
+        st_cluster_v4(mapa_shared(smem_u32(&s_all[step & 1][rank]), lane), __uint_as_float((uint32_t)bits),
+                      __uint_as_float((uint32_t)(bits >> 32)), mine.at);
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();
+    if (warp == 0) {
+      const TreeLeader all = shared(lane < ctas ? s_all[step & 1][lane] : TreeLeader{-INFINITY, INT_MAX, 0});
+      int child = -1;  // goes on there; -1: ends, -2: nothing to draw
+      if (all.at == INT_MAX) {
+        child = -2;
+      } else {
+        if (step < a.depth) {
+          const uint32_t h0 = __ballot_sync(0xffffffffu, lane > 0 && parent[0] == at && token[0] == all.at);
+          const uint32_t h1 = __ballot_sync(0xffffffffu, parent[1] == at && token[1] == all.at);
+          child = h0 ? __ffs((int)h0) - 1 : h1 ? 31 + __ffs((int)h1) : -1;
+        }
+        if (lane == 0) {
+          s_tokens[step] = all.at;
+          if (child >= 0) s_path[step] = child;
+        }
+      }
+      if (lane == 0) s_at = child;
+    }
+    __syncthreads();
+    at = s_at;
+    if (at == -2) failed = true;
+    if (at < 0) break;
+    ++taken;
+  }
+  if (rank) return;
+  __syncthreads();
+  for (int j = tid; j <= a.depth; j += kTreeThreads) {
+    a.out[(int64_t)b * (a.depth + 1) + j] = !failed && j <= taken ? s_tokens[j] : -1;
+    if (j < a.depth) a.path[(int64_t)b * a.depth + j] = !failed && j < taken ? s_path[j] : -1;
+  }
+  if (tid == 0) {
+    a.accepted[b] = failed ? 0 : taken;
+    if (failed) atomicExch(&g_verify_tree_device_error, 1);
+  }
+}
+
+}  // namespace otf
+
+using otf::check_device;
+using otf::set_cuda_error;
+
+int otf::verify_tree_device_error(int clear) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, otf::g_verify_tree_device_error, sizeof(int)) != cudaSuccess) {
+    set_cuda_error(cudaGetLastError());
+    return -1;
+  }
+  if (clear && v) {
+    const int z = 0;
+    cudaMemcpyToSymbol(otf::g_verify_tree_device_error, &z, sizeof(int));
+  }
+  return v;
+}
+
+extern "C" OTF_API int otf_verify_tree(const float* target, int64_t ld_target, const int64_t* tokens,
+                                       const int32_t* parents, const int32_t* starts, int64_t n, const float* noise,
+                                       int64_t noise_seq, int64_t ld_noise, const float* temperatures,
+                                       double temperature, int64_t* out_tokens, int32_t* path, int32_t* accepted,
+                                       int64_t batch, int64_t depth, int64_t vocab, void* stream) {
+  if (!target || !tokens || !parents || !out_tokens || (!path && depth) || !accepted) return OTF_ERR_INVALID;
+  if (batch <= 0 || depth < 0 || vocab <= 0 || n <= 0 || (!starts && n % batch) || ld_target < vocab) return OTF_ERR_INVALID;
+  if (!temperatures && !otf::temperature_ok((float)temperature)) return OTF_ERR_INVALID;
+  if (!noise && (temperatures || temperature > 0.0)) return OTF_ERR_INVALID;
+  if (noise && (ld_noise < vocab || noise_seq < 0)) return OTF_ERR_INVALID;
+  if (batch > 65535 || depth >= otf::kTreeMaxNodes || vocab > (1ll << 30) || n > INT32_MAX ||
+      (!starts && n / batch > otf::kTreeMaxNodes))
+    return OTF_ERR_UNSUPPORTED;
+  const int st = check_device();
+  if (st != OTF_OK) return st;
+  otf::TreeArgs a = {target, ld_target, tokens, parents, starts, noise, noise_seq, ld_noise, temperatures, temperature,
+                     out_tokens, path, accepted, starts ? 0 : (int)(n / batch), (int)n, (int)depth, (int)vocab};
+  static std::atomic<bool> done[64];
+  int dev;
+  bool needs;
+  cudaError_t e = otf::needs_opt_in(done, dev, needs);
+  if (e != cudaSuccess) return set_cuda_error(e);
+  if (needs) {
+    e = cudaFuncSetAttribute(otf::k_verify_tree, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return set_cuda_error(e);
+    otf::opted_in(done, dev);
+  }
+  int ctas = otf::kTreeCluster;
+  while (ctas > 1 && (batch * ctas > otf::kTreeResident / 2 || (int64_t)(ctas / 2) * otf::kTreeThreads * 4 >= vocab)) ctas /= 2;
+  return set_cuda_error(otf::launch_pdl(otf::k_verify_tree, dim3((unsigned)(batch * ctas)), dim3(otf::kTreeThreads), 0,
+                                        static_cast<cudaStream_t>(stream), (unsigned)ctas, a, ctas));
+}

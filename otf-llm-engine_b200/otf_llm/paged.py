@@ -430,6 +430,24 @@ class PagedKVCache:
                 raise ValueError("shape not supported by otf_paged_attn_rows")
         return n, heads, ldq, size
 
+    def keep(self, path: torch.Tensor, accepted: torch.Tensor) -> None:
+        """The taken nodes of a tree move together (otf_paged_keep): for j < accepted[b] the keys and values of
+        place lengths[b] + path[b, j] go to lengths[b] + 1 + j, behind the root's.
+
+        path (int32 [batch, depth], 63 deep at most) and accepted (int32 [batch]) as ``verify_tree`` gives them.
+        Every layer's cache is kept before ``advance(accepted + 1)`` counts the root and the taken nodes."""
+        if path.device != self.device or path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != self.batch or \
+                (path.stride(1) != 1 and path.shape[1] > 1):
+            raise ValueError(f"path must be int32 [{self.batch}, depth] with a unit inner stride on {self.device}, got "
+                             f"{path.dtype} {list(path.shape)} on {path.device}")
+        depth = path.shape[1]
+        if depth >= MAX_NODES:
+            raise ValueError(f"a path has at most {MAX_NODES - 1} nodes, got {depth}")
+        pa = self._vector(accepted, "accepted", self.batch)
+        if depth:
+            _call(_native.lib().otf_paged_keep, self.device, self._ref, path.data_ptr(),
+                  path.stride(0) if self.batch > 1 else depth, pa, depth)
+
     def evict(self, weights: torch.Tensor, budget: int, recent: int, *, to: Optional["PagedKVCache"] = None,
               weights_out: Optional[torch.Tensor] = None, lengths_out: Optional[torch.Tensor] = None
               ) -> torch.Tensor:

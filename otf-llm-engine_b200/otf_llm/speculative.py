@@ -13,7 +13,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _native
-from .paged import _call
+from .paged import MAX_NODES, _call
 
 MAX_DRAFTS = 32
 
@@ -73,6 +73,69 @@ def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, *,
     _call(_native.lib().otf_verify_drafts, dev, pt, seq_t, ld_t, pd, seq_d, ld_d, ptok, ld_tok, pu, ld_u, pn, ld_n, each, one, pc,
           tokens.data_ptr(), accepted.data_ptr(), batch, drafts, vocab, ws.data_ptr() if bytes_ else None, bytes_)
     return tokens, accepted
+
+
+def verify_tree(target_logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, *,
+                starts: Optional[torch.Tensor] = None, batch: Optional[int] = None, depth: Optional[int] = None,
+                noise: Optional[torch.Tensor] = None, temperature: Union[float, torch.Tensor] = 1.0
+                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Choose a way through trees of drafted tokens (otf_verify_tree).
+
+    target_logits: fp32 [n, vocab], the target's logits behind every node; tokens (int64 [n]) and parents (int32
+    [n]) of the nodes, sequence b's from starts[b] on (int32 [batch + 1] on the device), or n / ``batch`` each (one
+    sequence by default), 64 at most, as ``PagedKVCache.attend_tree`` takes them: node 0 is the root, the last token
+    that is certain, and a node's parent comes before it.  At each node, from the root on, the target draws the token
+    that follows, with noise (fp32 [batch, depth + 1, vocab], exponentially distributed) at a temperature above 0,
+    else its first largest logit; the walk goes on at a child that holds the token, the first of several, until
+    there is none or ``depth`` (noise.shape[1] - 1, or 63) are taken.  Every token is so distributed as the target
+    alone draws it, whatever was drafted.  temperature: a number, or fp32 [batch] on the device.
+
+    Returns (tokens int64 [batch, depth + 1]: the taken ones, the one that follows, then -1; path int32 [batch,
+    depth]: the taken nodes, then -1, for ``PagedKVCache.keep``; accepted int32 [batch])."""
+    _native._need_cuda(target_logits, "target_logits")
+    dev = target_logits.device
+    if target_logits.dim() != 2 or target_logits.shape[0] == 0 or target_logits.shape[1] == 0:
+        raise ValueError(f"target_logits must be [n, vocab], got {list(target_logits.shape)}")
+    n, vocab = target_logits.shape
+    ld, = _rows(target_logits, "target_logits", (n, vocab))
+    pt = _address(target_logits, "target_logits", _F32, dev)
+    ptok, pp = _vector(tokens, "tokens", torch.int64, n, dev), _vector(parents, "parents", torch.int32, n, dev)
+    ps = None
+    if starts is not None:
+        if starts.dim() != 1 or starts.shape[0] < 2 or (batch is not None and batch != starts.shape[0] - 1):
+            raise ValueError(f"starts must be a [batch + 1] vector, got {list(starts.shape)}")
+        batch = starts.shape[0] - 1
+        ps = _vector(starts, "starts", torch.int32, batch + 1, dev)
+    else:
+        batch = 1 if batch is None else int(batch)
+        if batch < 1 or n % batch or n // batch > MAX_NODES:
+            raise ValueError(f"{n} nodes do not divide among {batch} sequences of {MAX_NODES} at most; give starts")
+    if depth is None:
+        depth = MAX_NODES - 1 if noise is None or noise.dim() != 3 else noise.shape[1] - 1
+    if int(depth) != depth or not 0 <= depth < MAX_NODES:
+        raise ValueError(f"depth must be 0 to {MAX_NODES - 1}, got {depth}")
+    pn = each = None
+    seq_n = ld_n = 0
+    if noise is not None:
+        seq_n, ld_n = _rows(noise, "noise", (batch, depth + 1, vocab))
+        pn = _address(noise, "noise", _F32, dev)
+        if min(seq_n, ld_n) < 0:
+            raise ValueError(f"noise needs strides that are not negative, got {noise.stride()}")
+    one = 0.0
+    if isinstance(temperature, torch.Tensor):
+        each = _vector(temperature, "temperature", _F32, batch, dev)
+    else:
+        one = float(temperature)
+        if not (one == 0.0 or 1e-20 <= one <= 1e20):
+            raise ValueError(f"temperature must be 0, or positive and finite, got {one}")
+    if pn is None and (each is not None or one > 0):
+        raise ValueError("a temperature above 0 needs noise")
+    out = torch.empty((batch, depth + 1), dtype=torch.int64, device=dev)
+    path = torch.empty((batch, depth), dtype=torch.int32, device=dev)
+    accepted = torch.empty(batch, dtype=torch.int32, device=dev)
+    _call(_native.lib().otf_verify_tree, dev, pt, ld, ptok, pp, ps, n, pn, seq_n, ld_n, each, one, out.data_ptr(),
+          path.data_ptr() if depth else None, accepted.data_ptr(), batch, depth, vocab)
+    return out, path, accepted
 
 
 _F32 = torch.float32

@@ -75,16 +75,17 @@ def logprobs(x, tokens, top):
     rows = []
     for r in range(x.shape[0]):
         y = torch.where(x[r].isnan(), -math.inf, x[r].double())
-        m = float(y.max())
-        e = torch.exp(y - m)
-        lse = m + math.log(float(e.sum()))
-        p = e / e.sum()
-        h = float(-(torch.where(p > 0, p * (y - lse), 0.0)).sum())
+        d = y - y.max()
+        e = torch.exp(d)
+        rest = e.clone()
+        rest[int(y.argmax())] = 0.0
+        more = math.log1p(float(rest.sum()))            # of the sum of exponentials, without the largest's 1
+        h = more - float(torch.where(e > 0, e * d, 0.0).sum() / e.sum())
         order = sorted(range(y.shape[0]), key=lambda i: (-float(y[i]), i))
         order = [i for i in order[:top] if float(y[i]) > -math.inf]
         t = int(tokens[r])
-        lp = float(y[t]) - lse if t >= 0 else 0.0
+        lp = float(d[t]) - more if t >= 0 else 0.0
         rank = int(((y > y[t]) | ((y == y[t]) & (torch.arange(y.shape[0]) < t))).sum()) if t >= 0 else -1
         rows.append((lp, h, rank, order + [-1] * (top - len(order)),
-                     [float(y[i]) - lse for i in order] + [-math.inf] * (top - len(order))))
+                     [float(d[i]) - more for i in order] + [-math.inf] * (top - len(order))))
     return rows
