@@ -33,7 +33,7 @@ int paged_rows_device_error(int clear);  // read (and optionally clear) the flag
 
 constexpr int kPrKeys = 128;      // keys of a chunk
 constexpr int kPrGrid = 148;      // a CTA on each SM
-constexpr int kPrMma = 8, kPrQuery = 9, kPrLoad = 12;  // warps that issue products, fetch queries, and the first of four that fetch keys
+constexpr int kPrMma = 8, kPrQuery = 9, kPrScan = 10, kPrLoad = 12;  // that issue products, fetch queries, look values through (2), fetch keys (4)
 constexpr int kPrThreads = 512;
 // Registers: 128 a thread at launch, of which half of the threads give 32 to the others, which hold rows.
 constexpr int kPrRowRegs = 160, kPrOtherRegs = 96;
@@ -133,6 +133,12 @@ __device__ __forceinline__ int first_key(const Keys& k, int v) {
   return (v < k.sink_chunks ? v : k.low_chunk + v - k.sink_chunks) * kPrKeys;
 }
 
+// Whether a chunk has keys that some of the block's rows see and others do not, beyond a single token's.
+__device__ __forceinline__ bool some_do_not_see(const Keys& k, int v, int sinks) {
+  const int k0 = first_key(k, v);
+  return k.t1 > k.t0 && (k0 + kPrKeys > k.full || (k0 < k.low_full && k0 + kPrKeys > sinks));
+}
+
 // What one row sees.
 struct RowView {
   int lo, hi;  // keys lo .. hi; trees: lo .. hi and the nodes of `nodes` behind them
@@ -211,7 +217,6 @@ struct RowsShape {
   static constexpr int rows = 128 * TILES;
   static constexpr int tile = 128 * D * 2;               // bytes of 128 queries, keys or values
   static constexpr int slots = D == 128 ? 5 : 10;        // of the ring
-  static constexpr int lag = slots - 2;                  // fills in flight; the oldest slot's release may need the one after the next
   static constexpr int meet = TILES == 1 ? 128 * 64 * 4 : 0;  // where the groups' outputs meet, 64 columns at a time
   static constexpr int ring = TILES * tile + meet;
   static constexpr int small = ring + slots * tile;      // barriers and the like
@@ -220,7 +225,7 @@ struct RowsShape {
 
 // The small part of the shared memory, behind the ring.
 struct RowsSmall {
-  uint64_t kv_full[10], kv_empty[10];
+  uint64_t kv_full[10], kv_empty[10], v_landed[10];
   uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_done[2];
   RunStart run;
   int64_t sums[16];
@@ -247,13 +252,16 @@ __device__ __forceinline__ void rows_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
+__device__ __forceinline__ void mbar_arrive_n(uint32_t addr, uint32_t n) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(addr), "r"(n) : "memory");
+}
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// 32 lanes x 32 consecutive 32-bit columns of tensor memory, and back.
+// 32 lanes x 32 consecutive 32-bit columns of tensor memory, complete on return, and back.
 __device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
         "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
         "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
@@ -308,8 +316,8 @@ template <bool BF, int D, bool TREE, int ROWS>
 __device__ __noinline__ void add_odd(const Item<TREE, ROWS>& it, const RowView& view, float* o, int col) {
   const RowsArgs& a = it.a;
   for (int v = it.c0; v < it.c1; ++v) {
+    if (!some_do_not_see(it.k, v, a.sinks)) continue;
     const int k0 = first_key(it.k, v);
-    if (k0 + kPrKeys <= it.k.full && (k0 >= it.k.low_full || k0 + kPrKeys <= a.sinks)) continue;
     for (int s = k0; s < min(k0 + kPrKeys, it.k.end); ++s) {
       if (s < it.k.low && s >= a.sinks) continue;
       const int64_t at = key_place(a, it.b, s);
@@ -332,7 +340,7 @@ template <bool BF, int D, int TILES, bool TREE>
 __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_constant__ RowsArgs a) {
   using S = RowsShape<D, TILES>;
   using It = Item<TREE, S::rows>;
-  constexpr int NS = S::slots, LAG = S::lag;
+  constexpr int NS = S::slots;
   constexpr uint32_t kFormat = (1u << 4) | (BF ? 1u << 7 | 1u << 10 : 0u) | ((uint32_t)(128 >> 4) << 24);
   constexpr uint32_t kScores = kFormat | ((uint32_t)(kPrKeys >> 3) << 17);
   constexpr uint32_t kOutputs = kFormat | ((uint32_t)(D >> 3) << 17) | (1u << 16);  // values: keys across
@@ -344,7 +352,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
   pdl_trigger();
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(smem_u32(&sm.kv_full[i]), 4);
+      mbar_init(smem_u32(&sm.kv_full[i]), 128);
+      mbar_init(smem_u32(&sm.v_landed[i]), 128);
       mbar_init(smem_u32(&sm.kv_empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -453,31 +462,12 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
     const int w = warp - kPrLoad, piece = lane % P, sub = lane / P;
     const uint32_t ring = smem_u32(smem + S::ring);
     const uint32_t to = (uint32_t)((piece >> 3) * 128 * 128 + (32 * w + sub) * 128);
-    uint32_t fill = 0, scan = 0;  // scan: which of the last fills are values that not every row sees
+    uint32_t fill = 0;
     auto places = [&](int v) -> int64_t {
       const int s = first_key(it.k, v) + 32 * w + lane;
       return s < it.k.end && (s >= it.k.low || s < a.sinks) ? key_place(a, it.b, s) : -1;
     };
-    // Slot f - LAG, or with the last fills all that are still in flight, one by one.
-    auto publish = [&](uint32_t f, bool odd) {
-      const uint32_t slot = f % NS;
-      if (odd) {
-#pragma unroll 1
-        for (int i = 0; i < 32 / R; ++i) {
-          const int key = sub + i * R;
-          uint4* x = reinterpret_cast<uint4*>(smem + S::ring + slot * S::tile + to + i * R * 128 + (((piece & 7) ^ (key & 7)) << 4));
-          const uint4 y = *x;
-          if (odd2<BF>(y.x) || odd2<BF>(y.y) || odd2<BF>(y.z) || odd2<BF>(y.w)) {
-            *x = make_uint4(without_odd2<BF>(y.x), without_odd2<BF>(y.y), without_odd2<BF>(y.z), without_odd2<BF>(y.w));
-            *(volatile int*)&sm.odd = 1;
-          }
-        }
-      }
-      fence_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sm.kv_full[slot]));
-    };
-    auto put = [&](const uint16_t* base, int64_t place, bool odd) {
+    auto put = [&](const uint16_t* base, int64_t place, uint64_t* full) {
       const uint32_t slot = fill % NS;
       if (fill >= NS) rows_wait(&sm.kv_empty[slot], (fill / NS - 1) & 1u, gave_up);
       const uint32_t dst = ring + slot * S::tile + to;
@@ -486,20 +476,14 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
         const int64_t at = __shfl_sync(0xffffffffu, place, sub + i * R);
         cp_async16(dst + i * R * 128 + (((piece & 7) ^ ((sub + i * R) & 7)) << 4), base + (at >= 0 ? at : 0), at >= 0 ? 16u : 0u);
       }
-      cp_async_commit();
-      scan = scan << 1 | (odd ? 1u : 0u);
-      if (fill >= LAG) {
-        cp_async_wait<LAG>();
-        publish(fill - LAG, scan >> LAG & 1u);
-      }
+      cp_async_mbar_arrive(smem_u32(full + slot));  // when they have landed
       ++fill;
     };
     if (it.begin()) {
       int64_t place = places(it.c0);
       int v = it.c0;
       for (;;) {
-        const int k0 = first_key(it.k, v);
-        const bool odd = it.k.t1 > it.k.t0 && (k0 + kPrKeys > it.k.full || (k0 < it.k.low_full && k0 + kPrKeys > a.sinks));
+        const bool odd = some_do_not_see(it.k, v, a.sinks);
         const int64_t head = it.g * a.c.head_stride + piece * 8, now = place;
         bool more = true;
         if (++v == it.c1) {
@@ -507,15 +491,38 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
           v = it.c0;
         }
         if (more) place = places(v);
-        put(a.c.k + head, now, false);
-        put(a.c.v + head, now, odd);
+        put(a.c.k + head, now, sm.kv_full);
+        put(a.c.v + head, now, odd ? sm.v_landed : sm.kv_full);
         if (!more) break;
       }
-      const uint32_t left = min(fill, (uint32_t)LAG);
-      cp_async_wait<0>();
-      for (uint32_t f = fill - left; f < fill; ++f) publish(f, scan >> (fill - 1 - f) & 1u);
     }
     cp_async_wait<0>();
+  } else if (warp >= kPrScan) {
+    // Values that not every row of the block sees: a weight of 0 does not keep an infinity or NaN from a row, so
+    // they are taken out before the products (and given back at the item's end).  A warp has half of a slot.
+    const int h = warp - kPrScan;
+    uint32_t fill = 0;
+    uint32_t turns = 0;  // how often each slot's landing came around, a bit per slot
+    for (bool more = it.begin(); more; more = it.next())
+      for (int v = it.c0; v < it.c1; ++v, fill += 2) {
+        if (!some_do_not_see(it.k, v, a.sinks)) continue;
+        const uint32_t slot = (fill + 1) % NS;
+        rows_wait(&sm.v_landed[slot], turns >> slot & 1u, gave_up);
+        turns ^= 1u << slot;
+        uint4* x = reinterpret_cast<uint4*>(smem + S::ring + slot * S::tile + h * (S::tile / 2));
+        bool odd = false;
+#pragma unroll 4
+        for (int i = lane; i < S::tile / 32; i += 32) {
+          const uint4 y = x[i];
+          if (odd2<BF>(y.x) || odd2<BF>(y.y) || odd2<BF>(y.z) || odd2<BF>(y.w)) {
+            x[i] = make_uint4(without_odd2<BF>(y.x), without_odd2<BF>(y.y), without_odd2<BF>(y.z), without_odd2<BF>(y.w));
+            odd = true;
+          }
+        }
+        if (odd) *(volatile int*)&sm.odd = 1;
+        __syncwarp();
+        if (lane == 0) mbar_arrive_n(smem_u32(&sm.kv_full[slot]), 64);
+      }
   } else if (warp == kPrQuery) {
     // Queries: rows that there are, 128 of a tile; the others' scores are never looked at.
     constexpr int P = D / 8, R = 32 / P;
@@ -567,7 +574,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
           }
         }
       };
-      auto filled = [&](uint32_t f) { rows_wait(&sm.kv_full[f % NS], f / NS & 1u, gave_up); };
+      auto filled = [&](uint32_t f) {
+        rows_wait(&sm.kv_full[f % NS], f / NS & 1u, gave_up);
+        fence_async_shared();  // the copies are of the generic proxy, the products of the other
+      };
       auto release = [&](uint32_t f) { tc_commit(smem_u32(&sm.kv_empty[f % NS])); };
       auto ready = [&](int w) {
         rows_wait(&sm.p_full[w], probs[w] & 1u, gave_up);
@@ -684,7 +694,6 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
           auto load = [&](int c, float (&s)[32]) {
             uint32_t x[32];
             tmem_ld32(s_at + 32 * c, x);
-            tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(x[i]);
             if (edge)
@@ -701,7 +710,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
             for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i]);
           }
           top *= a.scale;
-          if (__any_sync(0xffffffffu, top > (m == -INFINITY ? -INFINITY : m + kPrHeadroom))) {
+          // lanes without a row hold what happens to lie there
+          if (__any_sync(0xffffffffu, there && top > (m == -INFINITY ? -INFINITY : m + kPrHeadroom))) {
             const float mx = fmaxf(m, top), f = m == -INFINITY ? 0.0f : pr_ex2(m - mx);
             m = mx;
             l *= f;
@@ -711,7 +721,6 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
               for (int c = 0; c < D; c += 32) {
                 uint32_t x[32];
                 tmem_ld32(o_at + c, x);
-                tmem_wait_ld();
 #pragma unroll
                 for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
                 tmem_st32(o_at + c, x);
@@ -773,7 +782,6 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
             for (int c = 0; c < 64; c += 32) {
               uint32_t x[32];
               tmem_ld32(o_at + half * 64 + c, x);
-              tmem_wait_ld();
               if (there)
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
@@ -800,7 +808,6 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
             uint32_t x[32];
             float o[32];
             tmem_ld32(o_at + c, x);
-            tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(x[i]);
             if (two && there) {
