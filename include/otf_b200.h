@@ -545,7 +545,7 @@ OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* q, int64_t 
  * head_dim], row stride ldq; starts: device int32 [batch + 1], or NULL: n / batch rows each), as
  * otf_paged_append took them: row t is token lengths[b] + t, lengths not yet advanced.  out (row stride ldo, no
  * memory shared with q) = softmax(scale q k) v over the tokens that a row sees, in fp32 with one rounding
- * (and, where sequences have more than 128 rows of a KV head on average, one of each probability); what it does not see does not reach it, whatever it holds.
+ * (and, in blocks of 256 rows (tokens x query heads of a KV head) that have more than 128, one of each probability); what it does not see does not reach it, whatever it holds.
  * parents NULL: row t, at place p = lengths[b] + t, sees the tokens s <= p, with a window (0: none) only those
  * with s > p - window, and the first `sinks` tokens (sinks without a window: OTF_ERR_INVALID).
  * parents (device int32 [n]): the rows of a sequence, 64 at most, are nodes of a tree (or of several); node t

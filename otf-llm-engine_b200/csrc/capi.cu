@@ -36,13 +36,7 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// A 2-D tiled tensor map over a row-major array of `rows` rows of `inner` elements of
-// `elem_bytes` bytes, rows `row_bytes` apart, copied in boxes of box_inner x box_rows;
-// reads past either extent come back as zeros.  cuTensorMapEncodeTiled is reached through
-// the runtime's driver entry point, so the library does not link libcuda.  `map` points at
-// a CUtensorMap (64-byte aligned, 128 bytes).
-bool encode_tiled_2d(void* map, int elem_bytes, const void* base, uint64_t inner, uint64_t rows, uint64_t row_bytes,
-                     uint32_t box_inner, uint32_t box_rows, bool swizzle128) {
+static EncodeTiledFn encode_tiled() {
   static EncodeTiledFn fn = [] {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
@@ -52,6 +46,17 @@ bool encode_tiled_2d(void* map, int elem_bytes, const void* base, uint64_t inner
     cudaGetLastError();
     return reinterpret_cast<EncodeTiledFn>(p);
   }();
+  return fn;
+}
+
+// A 2-D tiled tensor map over a row-major array of `rows` rows of `inner` elements of
+// `elem_bytes` bytes, rows `row_bytes` apart, copied in boxes of box_inner x box_rows;
+// reads past either extent come back as zeros.  cuTensorMapEncodeTiled is reached through
+// the runtime's driver entry point, so the library does not link libcuda.  `map` points at
+// a CUtensorMap (64-byte aligned, 128 bytes).
+bool encode_tiled_2d(void* map, int elem_bytes, const void* base, uint64_t inner, uint64_t rows, uint64_t row_bytes,
+                     uint32_t box_inner, uint32_t box_rows, bool swizzle128) {
+  const EncodeTiledFn fn = encode_tiled();
   if (!fn) return false;
   const CUtensorMapDataType dt = elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                  : elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
@@ -63,6 +68,19 @@ bool encode_tiled_2d(void* map, int elem_bytes, const void* base, uint64_t inner
   return fn(static_cast<CUtensorMap*>(map), dt, 2, const_cast<void*>(base), dims, strides, box, es,
             CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// A 4-D tiled tensor map over 16-bit values: dims[0] next to one another, the others strides[0..2] bytes apart,
+// copied in boxes of box[0..3] with the 128-byte swizzle; reads past an extent come back as zeros.
+bool encode_tiled_4d_swizzled(void* map, const void* base, const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
+  const EncodeTiledFn fn = encode_tiled();
+  if (!fn) return false;
+  const cuuint32_t es[4] = {1, 1, 1, 1};
+  const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]}, st[3] = {strides[0], strides[1], strides[2]};
+  const cuuint32_t b[4] = {box[0], box[1], box[2], box[3]};
+  return fn(static_cast<CUtensorMap*>(map), CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), d, st, b, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace otf

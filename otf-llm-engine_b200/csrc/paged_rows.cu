@@ -18,10 +18,15 @@
 // issues the matrix products (tcgen05, 128 rows x 128 keys and 128 rows x head_dim, scores, probabilities
 // and outputs in tensor memory); a warp that fetches queries, and four that fetch keys and values through
 // a ring of shared-memory slots by 16-byte asynchronous copies, page by page, whatever the page size is.
-// TILES 2, for many rows: the groups have 128 rows each and share every chunk.  TILES 1, for few rows:
-// the groups have the same rows and every other chunk each, and join at the item's end.
+// Blocks of more than 128 rows: the groups have 128 rows each and share every chunk.  Blocks of fewer: the
+// groups have the same rows and every other chunk each, and join at the item's end; and where there are 64 rows
+// or fewer they lie there two or four times, each copy with its own keys of a chunk (its other probabilities are 0),
+// so that all warps have work.
+#include <cuda.h>
+
 #include <algorithm>
 #include <cmath>
+#include <numeric>
 
 #include "paged.cuh"
 
@@ -30,13 +35,13 @@ namespace otf {
 int set_cuda_error(cudaError_t e);       // capi.cu
 int check_device();                      // capi.cu
 int paged_rows_device_error(int clear);  // read (and optionally clear) the flag below
+bool encode_tiled_4d_swizzled(void* map, const void* base, const uint64_t* dims, const uint64_t* strides, const uint32_t* box);  // capi.cu
 
 constexpr int kPrKeys = 128;      // keys of a chunk
+constexpr int kPrRows = 256;      // rows of a block
 constexpr int kPrGrid = 148;      // a CTA on each SM
-constexpr int kPrMma = 8, kPrQuery = 9, kPrScan = 10, kPrLoad = 12;  // that issue products, fetch queries, look values through (2), fetch keys (4)
-constexpr int kPrThreads = 512;
-// Registers: 128 a thread at launch, of which half of the threads give 32 to the others, which hold rows.
-constexpr int kPrRowRegs = 160, kPrOtherRegs = 96;
+constexpr int kPrMma = 8, kPrQuery = 9, kPrLoad = 10;  // warps that issue products, fetch queries, and two that fetch keys and values
+constexpr int kPrThreads = 384;
 constexpr int kPrMaxNodes = 64;
 constexpr int kPrItemUnits = 2;   // what an item's start and end cost, in chunks
 constexpr float kPrLog2e = 1.4426950408889634f;
@@ -52,6 +57,9 @@ struct __align__(16) SharedItem {
 };
 
 struct RowsArgs {
+  CUtensorMap kmap, vmap;  // boxes of 64 dims of `box` tokens of a page, as the ring holds them
+  CUtensorMap qmap;        // boxes of 64 dims of 32 rows: a KV head's query heads of some tokens
+  int box, q_box;          // 0: no tensor copies; tokens of a box
   PagedView c;
   FastDiv page, rep_div;
   const uint16_t* q;
@@ -64,8 +72,9 @@ struct RowsArgs {
   int window, sinks;   // window 0: none
   float scale;         // |scale| log2(e)
   uint32_t sign;       // of the scale, on two 16-bit queries
-  float* part;         // [2 x grid][rows of a block][head_dim]: o of a part
-  float2* part_ml;     // [2 x grid][rows of a block]: its m and l
+  int part_rows;       // rows of a block that there can be
+  float* part;         // [2 x grid][part_rows][head_dim]: o of a part
+  float2* part_ml;     // [2 x grid][part_rows]: its m and l
   SharedItem* shared;  // [grid]
 };
 
@@ -110,10 +119,10 @@ struct Keys {
   int t0, t1;  // its first and last token
   int low, low_full, full, end, sink_chunks, low_chunk, chunks;
 };
-template <bool TREE, int ROWS>
+template <bool TREE>
 __device__ __forceinline__ Keys keys_of(const RowsArgs& a, const RowRange& s, int rb) {
   Keys k;
-  const int row0 = rb * ROWS, row1 = min(s.tokens * a.rep, row0 + ROWS);
+  const int row0 = rb * kPrRows, row1 = min(s.tokens * a.rep, row0 + kPrRows);
   k.t0 = (uint32_t)row0 / a.rep_div;
   k.t1 = (uint32_t)(row1 - 1) / a.rep_div;
   k.low = k.low_full = k.sink_chunks = k.low_chunk = 0;
@@ -164,7 +173,7 @@ struct RunStart {
 };
 
 // An item of a run, with the chunks [c0, c1) that the run has of it.
-template <bool TREE, int ROWS>
+template <bool TREE>
 struct Item {
   const RowsArgs& a;
   const int64_t u0, u1;
@@ -184,7 +193,7 @@ struct Item {
   __device__ __forceinline__ bool begin() {
     if (u0 >= u1) return false;
     s = range_of<TREE>(a, b, false);
-    k = keys_of<TREE, ROWS>(a, s, rb);
+    k = keys_of<TREE>(a, s, rb);
     return clip() || next_with_chunks();
   }
   __device__ __forceinline__ bool next() {
@@ -197,36 +206,39 @@ struct Item {
       if (at + kPrItemUnits >= u1) return false;
       if (++g == a.c.kv_heads) {
         g = 0;
-        if ((int64_t)(++rb) * ROWS >= (int64_t)s.tokens * a.rep) {
+        if ((int64_t)(++rb) * kPrRows >= (int64_t)s.tokens * a.rep) {
           rb = 0;
           do {
             if (++b >= a.c.batch) return false;
             s = range_of<TREE>(a, b, false);
           } while (s.tokens == 0);
         }
-        k = keys_of<TREE, ROWS>(a, s, rb);
+        k = keys_of<TREE>(a, s, rb);
       }
     } while (!clip());
     return true;
   }
   __device__ __forceinline__ bool whole() const { return c0 == 0 && c1 == k.chunks; }
+  __device__ __forceinline__ int rows() const { return min(kPrRows, s.tokens * a.rep - rb * kPrRows); }
+  // Copies of the rows: 1 << fold.
+  __device__ __forceinline__ int fold() const { return rows() <= 32 ? 2 : rows() <= 64 ? 1 : 0; }
 };
 
-template <int D, int TILES>
+template <int D>
 struct RowsShape {
-  static constexpr int rows = 128 * TILES;
   static constexpr int tile = 128 * D * 2;               // bytes of 128 queries, keys or values
   static constexpr int slots = D == 128 ? 5 : 10;        // of the ring
-  static constexpr int meet = TILES == 1 ? 128 * 64 * 4 : 0;  // where the groups' outputs meet, 64 columns at a time
-  static constexpr int ring = TILES * tile + meet;
+  static constexpr int ring = D == 128 ? 2 * tile : tile + 128 * 64 * 4;  // behind two tiles of queries, or one and `meet`
   static constexpr int small = ring + slots * tile;      // barriers and the like
   static constexpr int bytes = 1024 + small + 2048;
 };
+// Behind the first tile of queries, where there is no second one: 64 columns of the outputs of 128 rows, where
+// the groups and copies meet.
 
 // The small part of the shared memory, behind the ring.
 struct RowsSmall {
   uint64_t kv_full[10], kv_empty[10], v_landed[10];
-  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_done[2];
+  uint64_t q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_done[2];
   RunStart run;
   int64_t sums[16];
   float2 ml[128];
@@ -252,20 +264,58 @@ __device__ __forceinline__ void rows_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int x, int y, int z, int u, uint32_t mbar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      ::"r"(dst), "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(u), "r"(mbar) : "memory");
+}
+// True in one lane of a warp that runs together.
+__device__ __forceinline__ bool one_lane() {
+  uint32_t x;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(x));
+  return x != 0;
+}
 __device__ __forceinline__ void mbar_arrive_n(uint32_t addr, uint32_t n) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(addr), "r"(n) : "memory");
 }
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// 32 lanes x 32 consecutive 32-bit columns of tensor memory, complete on return, and back.
+// 32 lanes x 32 consecutive 32-bit columns of tensor memory, asked for and, with tmem_have, there; 32 or 16 columns
+// complete on return; and back.
+__device__ __forceinline__ void tmem_ask32(uint32_t at, float (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%1"
+      "7,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(at) : "memory");
+}
+template <int NC>
+__device__ __forceinline__ void tmem_have(float (&v)[NC][32]) {
+  tmem_wait_ld();
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[c][i]));  // no use of them before the wait
+}
 __device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&v)[32]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%1"
+      "7,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
         "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
         "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
         "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(at) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
       : "r"(at) : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&v)[32]) {
@@ -285,12 +335,7 @@ __device__ __forceinline__ uint64_t values_desc(uint32_t at) {
          ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
 }
 
-// Whether one of two 16-bit values is an infinity or NaN.
-template <bool BF>
-__device__ __forceinline__ bool odd2(uint32_t x) {
-  constexpr uint32_t e = BF ? 0x7F80u : 0x7C00u;
-  return (x & e) == e || (x & (e << 16)) == e << 16;
-}
+// Two 16-bit values, an infinity or NaN as 0.
 template <bool BF>
 __device__ __forceinline__ uint32_t without_odd2(uint32_t x) {
   constexpr uint32_t e = BF ? 0x7F80u : 0x7C00u;
@@ -299,47 +344,211 @@ __device__ __forceinline__ uint32_t without_odd2(uint32_t x) {
   return x;
 }
 
-// Offset of key s of sequence b in the pools, -1 where its page lies outside.
-__device__ __forceinline__ int64_t key_place(const RowsArgs& a, int b, int s) {
+// The page of a key, as the table names it (0 where there is no key), and the key's offset in the pools under it: -1
+// where the page lies outside.
+struct KeyPlace {
+  int page, rest;
+  bool there;
+};
+__device__ __forceinline__ KeyPlace ask_key(const RowsArgs& a, int b, int s, bool there) {
   const uint32_t in = (uint32_t)s / a.page;
-  const int page = a.c.table[b * a.c.ld_table + in];
-  if (page < 0 || page >= a.c.n_pages) {
+  return KeyPlace{there ? a.c.table[b * a.c.ld_table + in] : 0, s - (int)(in * a.page.d), there};
+}
+__device__ __forceinline__ int64_t offset_of(const RowsArgs& a, const KeyPlace& k) {
+  if (!k.there) return -1;
+  if (k.page < 0 || k.page >= a.c.n_pages) {
     report_bad_rows();
     return -1;
   }
-  return page * a.c.page_stride + (int64_t)(s - (int)(in * a.page.d)) * a.c.token_stride;
+  return k.page * a.c.page_stride + (int64_t)k.rest * a.c.token_stride;
 }
 
 // The infinities and NaN that were taken out of a block's values, given back to the rows that see them:
-// columns [col, col + 32) of the outputs o that a warp's lanes hold a row of each.
-template <bool BF, int D, bool TREE, int ROWS>
-__device__ __noinline__ void add_odd(const Item<TREE, ROWS>& it, const RowView& view, float* o, int col) {
+// columns [col, col + N) of the outputs o that a warp's lanes hold a row of each (the same columns).
+template <bool BF, int D, bool TREE, int N>
+__device__ __noinline__ void add_odd(const Item<TREE>& it, const RowView& view, float* o, int col) {
   const RowsArgs& a = it.a;
   for (int v = it.c0; v < it.c1; ++v) {
     if (!some_do_not_see(it.k, v, a.sinks)) continue;
     const int k0 = first_key(it.k, v);
     for (int s = k0; s < min(k0 + kPrKeys, it.k.end); ++s) {
       if (s < it.k.low && s >= a.sinks) continue;
-      const int64_t at = key_place(a, it.b, s);
+      const int64_t at = offset_of(a, ask_key(a, it.b, s, true));
       if (at < 0) continue;
-      const uint16_t* x = a.c.v + at + it.g * a.c.head_stride + col;
-      const float mine = to_f<BF>(x[threadIdx.x & 31]);
+      const float mine = to_f<BF>(a.c.v[at + it.g * a.c.head_stride + col + (threadIdx.x & (N - 1))]);
       if (!__any_sync(0xffffffffu, !isfinite(mine))) continue;
       const bool sees = (seen32<TREE>(a, view, s & ~31) >> (s & 31)) & 1u;
-      for (int i = 0; i < 32; ++i) {
+      for (int i = 0; i < N; ++i) {
         const float y = __shfl_sync(0xffffffffu, mine, i);
         if (sees && !isfinite(y)) o[i] += y;
       }
     }
   }
 }
+template <bool BF, int D, bool TREE, int N>
+__device__ __forceinline__ void give_back(const Item<TREE>& it, const RowView& view, float (&o)[N], int col) {
+  const Item<TREE> here = it;  // copies: what lies in memory for the call
+  const RowView mine = view;
+  float y[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) y[i] = o[i];
+  add_odd<BF, D, TREE, N>(here, mine, y, col);
+#pragma unroll
+  for (int i = 0; i < N; ++i) o[i] = y[i];
+}
+
+// ---- scores to probabilities ------------------------------------------------------------------
+
+// Two fp32 operations in one.
+__device__ __forceinline__ void fma_two(float& x, float& y, float m, float z) {
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\tmov.b64 c, {%3, %3};\n\t"
+      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(x), "+f"(y) : "f"(m), "f"(z));
+}
+__device__ __forceinline__ void add_two(float& x, float& y, float u, float v) {
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+      "add.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(x), "+f"(y) : "f"(u), "f"(v));
+}
+// p = p f + c.
+__device__ __forceinline__ void fma_by(float& px, float& py, float fx, float fy, float c) {
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tmov.b64 c, {%4, %4};\n\t"
+      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(px), "+f"(py) : "f"(fx), "f"(fy), "f"(c));
+}
+__device__ __forceinline__ float max_three(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+
+// 2^x of two numbers without the exponential unit: x = n + f with n whole and |f| <= 1/2, a polynomial of degree 4
+// for 2^f (least relative error with 1 at f = 0, 2^-18.4, by linear programming), n added to its exponent.  0 from
+// -127 down, where the exponent's bits run out.  The unit makes 16 a cycle on an SM, so 128 x 128 scores take as long as their two products; some of
+// them go this way (kPrPoly of each 8).
+constexpr int kPrPoly = 2;
+__device__ __forceinline__ void exp2_two(float& x, float& y) {
+  constexpr float big = 12582912.0f;  // 1.5 2^23: its sum's last bits are n
+  x = fmaxf(x, -127.0f);
+  y = fmaxf(y, -127.0f);
+  float nx = x, ny = y, px = 0.009582576341927052f, py = px;
+  add_two(nx, ny, big, big);
+  float fx = nx, fy = ny;
+  add_two(fx, fy, -big, -big);
+  fma_two(fx, fy, -1.0f, 0.0f);
+  add_two(fx, fy, x, y);
+  fma_by(px, py, fx, fy, 0.05590682849287987f);
+  fma_by(px, py, fx, fy, 0.24024106562137604f);
+  fma_by(px, py, fx, fy, 0.6931241154670715f);
+  fma_by(px, py, fx, fy, 1.0f);
+  x = __int_as_float(__float_as_int(px) + (__float_as_int(nx) << 23));
+  y = __int_as_float(__float_as_int(py) + (__float_as_int(ny) << 23));
+}
+
+// A row's state.
+struct RowState {
+  float m, l;
+  bool any;  // a chunk came before
+};
+
+// The scores of 32 NC keys from column s_at on become probabilities: one 16-bit number each, the columns packed
+// from p_at on, or (TWO) the rounding and the rest, 16 columns of each in the place of 32 scores.
+template <bool BF, int D, bool TWO, int NC>
+__device__ __forceinline__ void turn(uint32_t s_at, uint32_t p_at, uint32_t o_at, float scale, bool edge, const uint32_t (&see)[NC],
+                                     bool there, RowState& r, uint64_t* half_bar) {
+  float s[NC][32];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) tmem_ask32(s_at + 32 * c, s[c]);
+  tmem_have(s);
+  if (edge)
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (!(see[c] >> i & 1u)) s[c][i] = -INFINITY;
+  float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) tops[(i >> 1) & 3] = max_three(tops[(i >> 1) & 3], s[c][i], s[c][i + 1]);
+  const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * scale;
+  // lanes without a row hold what happens to lie there
+  if (__any_sync(0xffffffffu, there && top > (r.m == -INFINITY ? -INFINITY : r.m + kPrHeadroom))) {
+    const float mx = fmaxf(r.m, top), f = r.m == -INFINITY ? 0.0f : pr_ex2(r.m - mx);
+    r.m = mx;
+    r.l *= f;
+    // the scores of a chunk are complete after the outputs of the one before it
+    if (r.any)
+#pragma unroll 1
+      for (int c = 0; c < D; c += 16) {
+        uint32_t x[16];
+        tmem_ld16(o_at + c, x);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
+        tmem_st16(o_at + c, x);
+      }
+  }
+  const float z = kPrShift<BF> - (r.m == -INFINITY ? 0.0f : r.m);
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      fma_two(s[c][i], s[c][i + 1], scale, z);
+      if (!TWO && (i & 7) >= 8 - kPrPoly) {
+        exp2_two(s[c][i], s[c][i + 1]);
+      } else {
+        s[c][i] = pr_ex2(s[c][i]);
+        s[c][i + 1] = pr_ex2(s[c][i + 1]);
+      }
+      add_two(sum[i & 2], sum[(i & 2) + 1], s[c][i], s[c][i + 1]);
+    }
+    if (TWO) {
+      uint32_t p[32];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        p[i] = pack2<BF>(s[c][2 * i], s[c][2 * i + 1]);
+        const float2 y = unpack2<BF>(p[i]);
+        p[16 + i] = pack2<BF>(s[c][2 * i] - y.x, s[c][2 * i + 1] - y.y);
+      }
+      tmem_st32(p_at + 32 * c, p);
+    } else {
+      uint32_t p[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) p[i] = pack2<BF>(s[c][2 * i], s[c][2 * i + 1]);
+      tmem_st16(p_at + 16 * c, p);
+    }
+    if (NC == 4 && c == 1) {  // the products with the first half of the keys' values may begin
+      tmem_wait_st();
+      tc_fence_before_sync();
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(half_bar));
+    }
+  }
+  r.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+// The same for a copy that has the 32 NC keys from 32 c0 on: its other probabilities are 0.
+template <bool BF, int D, int NC>
+__device__ __forceinline__ void turn_part(uint32_t s_at, uint32_t o_at, int c0, float scale, bool edge, const uint32_t (&see)[4],
+                                          bool there, RowState& r) {
+  uint32_t mine[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) mine[c] = see[0];
+#pragma unroll
+  for (int k = 1; k < 4; ++k)
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      if (c0 + c == k) mine[c] = see[k];
+  turn<BF, D, true, NC>(s_at + 32 * c0, s_at + 32 * c0, o_at, scale, edge, mine, there, r, nullptr);
+  const uint32_t none[32] = {};
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c)
+    if (c < c0 || c >= c0 + NC) tmem_st32(s_at + 32 * c, none);
+}
 
 // ---- the kernel -------------------------------------------------------------------------------
 
-template <bool BF, int D, int TILES, bool TREE>
+template <bool BF, int D, bool TREE>
 __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_constant__ RowsArgs a) {
-  using S = RowsShape<D, TILES>;
-  using It = Item<TREE, S::rows>;
+  using S = RowsShape<D>;
+  using It = Item<TREE>;
   constexpr int NS = S::slots;
   constexpr uint32_t kFormat = (1u << 4) | (BF ? 1u << 7 | 1u << 10 : 0u) | ((uint32_t)(128 >> 4) << 24);
   constexpr uint32_t kScores = kFormat | ((uint32_t)(kPrKeys >> 3) << 17);
@@ -352,14 +561,15 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
   pdl_trigger();
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(smem_u32(&sm.kv_full[i]), 128);
-      mbar_init(smem_u32(&sm.v_landed[i]), 128);
+      mbar_init(smem_u32(&sm.kv_full[i]), 64);
+      mbar_init(smem_u32(&sm.v_landed[i]), 64);
       mbar_init(smem_u32(&sm.kv_empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&sm.q_full[i]), 1);
       mbar_init(smem_u32(&sm.q_empty[i]), 1);
       mbar_init(smem_u32(&sm.s_full[i]), 1);
+      mbar_init(smem_u32(&sm.p_half[i]), 4);
       mbar_init(smem_u32(&sm.p_full[i]), 4);
       mbar_init(smem_u32(&sm.o_done[i]), 1);
     }
@@ -379,8 +589,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
     for (int b = warp; b < a.c.batch; b += kPrThreads / 32) {
       const RowRange s = range_of<TREE>(a, b, blockIdx.x == 0 && lane == 0);
       int64_t x = 0;
-      for (int rb = lane; (int64_t)rb * S::rows < (int64_t)s.tokens * a.rep; rb += 32)
-        x += keys_of<TREE, S::rows>(a, s, rb).chunks + kPrItemUnits;
+      for (int rb = lane; (int64_t)rb * kPrRows < (int64_t)s.tokens * a.rep; rb += 32)
+        x += keys_of<TREE>(a, s, rb).chunks + kPrItemUnits;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
       x *= a.c.kv_heads;
@@ -421,8 +631,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
       if (found >= 0) {
         const RowRange s = range_of<TREE>(a, found, false);
         for (int r0 = 0;; r0 += 32) {
-          const int per = (int64_t)(r0 + lane) * S::rows < (int64_t)s.tokens * a.rep
-                              ? keys_of<TREE, S::rows>(a, s, r0 + lane).chunks + kPrItemUnits : 0;
+          const int per = (int64_t)(r0 + lane) * kPrRows < (int64_t)s.tokens * a.rep
+                              ? keys_of<TREE>(a, s, r0 + lane).chunks + kPrItemUnits : 0;
           const int64_t mine = (int64_t)per * a.c.kv_heads;
           int64_t inc = mine;
 #pragma unroll
@@ -451,191 +661,278 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
   It it(a, run);
   volatile int* gave_up = &sm.gave_up;
 
-  if (warp >= 8)
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPrOtherRegs));
-  else
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPrRowRegs));
-
   if (warp >= kPrLoad) {
-    // Keys and values: chunk after chunk a slot of keys, then one of values, 32 rows a warp.
+    // Keys and values: chunk after chunk a slot of keys, then one of values, 64 rows a warp.
     constexpr int P = D / 8, R = 32 / P;  // 16-byte pieces of a row, rows of a copy instruction
     const int w = warp - kPrLoad, piece = lane % P, sub = lane / P;
     const uint32_t ring = smem_u32(smem + S::ring);
-    const uint32_t to = (uint32_t)((piece >> 3) * 128 * 128 + (32 * w + sub) * 128);
+    const uint32_t to = (uint32_t)((piece >> 3) * 128 * 128 + (64 * w + sub) * 128);
     uint32_t fill = 0;
-    auto places = [&](int v) -> int64_t {
-      const int s = first_key(it.k, v) + 32 * w + lane;
-      return s < it.k.end && (s >= it.k.low || s < a.sinks) ? key_place(a, it.b, s) : -1;
+    constexpr int H = D / 64;  // boxes that a group of tokens takes
+    // What a chunk's copies need to know, asked for a chunk ahead: of two of the warp's keys, 32 apart, or where all
+    // keys are there and tensor copies are open, of a lane's two boxes.
+    struct Asked {
+      KeyPlace key[2];
+      bool boxes;
     };
-    auto put = [&](const uint16_t* base, int64_t place, uint64_t* full) {
-      const uint32_t slot = fill % NS;
-      if (fill >= NS) rows_wait(&sm.kv_empty[slot], (fill / NS - 1) & 1u, gave_up);
-      const uint32_t dst = ring + slot * S::tile + to;
+    auto ask = [&](int v) {
+      const int k0 = first_key(it.k, v);
+      Asked x;
+      x.boxes = a.box && k0 + kPrKeys <= it.k.end && (k0 >= it.k.low || k0 + kPrKeys <= a.sinks);
+      if (x.boxes) {
 #pragma unroll
-      for (int i = 0; i < 32 / R; ++i) {
-        const int64_t at = __shfl_sync(0xffffffffu, place, sub + i * R);
-        cp_async16(dst + i * R * 128 + (((piece & 7) ^ ((sub + i * R) & 7)) << 4), base + (at >= 0 ? at : 0), at >= 0 ? 16u : 0u);
+        for (int h = 0; h < 2; ++h) {
+          const int s = (lane + 32 * h) / H * a.box;
+          x.key[h] = ask_key(a, it.b, k0 + s, s < kPrKeys);
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int s = k0 + 64 * w + 32 * h + lane;
+          x.key[h] = ask_key(a, it.b, s, s < it.k.end && (s >= it.k.low || s < a.sinks));
+        }
       }
-      cp_async_mbar_arrive(smem_u32(full + slot));  // when they have landed
-      ++fill;
+      return x;
+    };
+    auto empty = [&](uint32_t f) {
+      if (f >= NS) rows_wait(&sm.kv_empty[f % NS], (f / NS - 1) & 1u, gave_up);
     };
     if (it.begin()) {
-      int64_t place = places(it.c0);
-      int v = it.c0;
-      for (;;) {
+      const int64_t v_from_k = a.c.v - a.c.k;
+      Asked next = ask(it.c0);
+      for (int v = it.c0;; fill += 2) {
         const bool odd = some_do_not_see(it.k, v, a.sinks);
-        const int64_t head = it.g * a.c.head_stride + piece * 8, now = place;
+        const int g = it.g;
+        const Asked x = next;
         bool more = true;
         if (++v == it.c1) {
           more = it.next();
           v = it.c0;
         }
-        if (more) place = places(v);
-        put(a.c.k + head, now, sm.kv_full);
-        put(a.c.v + head, now, odd ? sm.v_landed : sm.kv_full);
+        if (more) next = ask(v);
+        const uint32_t ks = fill % NS, vs = (fill + 1) % NS;
+        if (x.boxes) {
+          // the first warp the keys, the second one the values
+          const uint32_t slot = w ? vs : ks, bar = smem_u32(w && odd ? &sm.v_landed[slot] : &sm.kv_full[slot]);
+          empty(fill + w);
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive_expect_tx(bar, S::tile);
+            mbar_arrive_n(bar, 63);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (x.key[h].there) {
+              int page = x.key[h].page;
+              if (page < 0 || page >= a.c.n_pages) {
+                report_bad_rows();
+                page = a.c.n_pages;  // reads as zeros
+              }
+              tma_load_4d(ring + slot * S::tile + lane % H * (128 * 128) + (lane + 32 * h) / H * a.box * 128, w ? &a.vmap : &a.kmap,
+                          lane % H * 64, g, x.key[h].rest, page, bar);
+            }
+        } else {
+          empty(fill);
+          empty(fill + 1);
+          const uint16_t* const base = a.c.k + g * a.c.head_stride + piece * 8;
+          const uint32_t dst = ring + ks * S::tile + to, across = (vs - ks) * S::tile;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int64_t mine = offset_of(a, x.key[h]);
+#pragma unroll
+            for (int i = 0; i < 32 / R; ++i) {
+              const int64_t at = __shfl_sync(0xffffffffu, mine, sub + i * R);
+              const uint16_t* y = base + (at >= 0 ? at : 0);  // an address, not read where there is no key
+              const uint32_t to_key = dst + (32 * h + i * R) * 128 + (((piece & 7) ^ ((sub + i * R) & 7)) << 4), bytes = at >= 0 ? 16u : 0u;
+              cp_async16(to_key, y, bytes);
+              cp_async16(to_key + across, y + v_from_k, bytes);
+            }
+          }
+          cp_async_mbar_arrive(smem_u32(&sm.kv_full[ks]));  // when they have landed
+          cp_async_mbar_arrive(smem_u32(odd ? &sm.v_landed[vs] : &sm.kv_full[vs]));
+        }
         if (!more) break;
       }
     }
     cp_async_wait<0>();
-  } else if (warp >= kPrScan) {
-    // Values that not every row of the block sees: a weight of 0 does not keep an infinity or NaN from a row, so
-    // they are taken out before the products (and given back at the item's end).  A warp has half of a slot.
-    const int h = warp - kPrScan;
-    uint32_t fill = 0;
+  } else if (warp == kPrQuery) {
+    // Queries: rows that there are, 128 of a tile; the others' scores are never looked at.  Then, once they have
+    // landed, the item's values that not every row of the block sees: a weight of 0 does not keep an infinity or NaN
+    // from a row, so they are taken out before the products (and given back at the item's end).
+    constexpr int P = D / 8, R = 32 / P;
+    const int piece = lane % P, sub = lane / P;
+    uint32_t n[2] = {0, 0}, fill = 0;
     uint32_t turns = 0;  // how often each slot's landing came around, a bit per slot
-    for (bool more = it.begin(); more; more = it.next())
+    for (bool more = it.begin(); more; more = it.next()) {
+      const int all = it.rows(), fold = it.fold();
+      for (int w = 0; w < (all > 128 ? 2 : 1); ++w) {
+        if (n[w] > 0) rows_wait(&sm.q_empty[w], (n[w] - 1) & 1u, gave_up);
+        ++n[w];
+        const int row0 = it.rb * kPrRows + w * 128, rows = min(128, all - w * 128);
+        unsigned char* tile = smem + w * S::tile + (piece >> 3) * 128 * 128;
+        auto at = [&](int r) { return reinterpret_cast<uint4*>(tile + r * 128 + (((piece & 7) ^ (r & 7)) << 4)); };
+        if (a.q_box) {
+          constexpr int H = D / 64;
+          const int from = lane / H & ((4 >> fold) - 1);  // a lane's box, which lies there 1 << fold times
+          const bool mine = lane < 4 * H && from * 32 < rows;
+          const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, mine)), bar = smem_u32(&sm.q_full[w]);
+          if (lane == 0) mbar_arrive_expect_tx(bar, boxes * 32 * 128);
+          __syncwarp();
+          if (mine)
+            tma_load_4d(smem_u32(smem + w * S::tile) + lane % H * (128 * 128) + lane / H * (32 * 128), &a.qmap, lane % H * 64,
+                        it.g * a.rep, it.s.r0 + (int)((uint32_t)row0 / a.rep_div) + from * a.q_box, 0, bar);
+          continue;
+        }
+        for (int r = sub; r < rows; r += R) {
+          const uint32_t row = row0 + r, t = row / a.rep_div;
+          const uint16_t* x = a.q + (it.s.r0 + (int64_t)t) * a.ldq + (int64_t)(it.g * a.rep + row - t * a.rep) * D + piece * 8;
+          for (int c = 0; c < 128; c += 128 >> fold) cp_async16(smem_u32(at(c + r)), x, 16u);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        if (a.sign)  // a negative scale's, so that a larger product weighs more
+          for (int r = sub; r < rows; r += R)
+            for (int c = 0; c < 128; c += 128 >> fold) {
+              const uint4 y = *at(c + r);
+              *at(c + r) = make_uint4(y.x ^ a.sign, y.y ^ a.sign, y.z ^ a.sign, y.w ^ a.sign);
+            }
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sm.q_full[w]));
+      }
       for (int v = it.c0; v < it.c1; ++v, fill += 2) {
         if (!some_do_not_see(it.k, v, a.sinks)) continue;
         const uint32_t slot = (fill + 1) % NS;
         rows_wait(&sm.v_landed[slot], turns >> slot & 1u, gave_up);
         turns ^= 1u << slot;
-        uint4* x = reinterpret_cast<uint4*>(smem + S::ring + slot * S::tile + h * (S::tile / 2));
-        bool odd = false;
-#pragma unroll 4
-        for (int i = lane; i < S::tile / 32; i += 32) {
+        uint4* x = reinterpret_cast<uint4*>(smem + S::ring + slot * S::tile);
+        uint32_t high = 0;  // an exponent of ones plus one carries into the sign's place
+#pragma unroll 16
+        for (int i = lane; i < S::tile / 16; i += 32) {
+          constexpr uint32_t e = BF ? 0x7F807F80u : 0x7C007C00u, one = BF ? 0x00800080u : 0x04000400u;
           const uint4 y = x[i];
-          if (odd2<BF>(y.x) || odd2<BF>(y.y) || odd2<BF>(y.z) || odd2<BF>(y.w)) {
-            x[i] = make_uint4(without_odd2<BF>(y.x), without_odd2<BF>(y.y), without_odd2<BF>(y.z), without_odd2<BF>(y.w));
-            odd = true;
-          }
+          high |= ((y.x & e) + one) | ((y.y & e) + one) | ((y.z & e) + one) | ((y.w & e) + one);
         }
-        if (odd) *(volatile int*)&sm.odd = 1;
+        if (high & 0x80008000u) {
+          for (int i = lane; i < S::tile / 16; i += 32) {
+            const uint4 y = x[i];
+            x[i] = make_uint4(without_odd2<BF>(y.x), without_odd2<BF>(y.y), without_odd2<BF>(y.z), without_odd2<BF>(y.w));
+          }
+          *(volatile int*)&sm.odd = 1;
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive_n(smem_u32(&sm.kv_full[slot]), 64);
       }
-  } else if (warp == kPrQuery) {
-    // Queries: rows that there are, 128 of a tile; the others' scores are never looked at.
-    constexpr int P = D / 8, R = 32 / P;
-    const int piece = lane % P, sub = lane / P;
-    uint32_t n = 0;
-    for (bool more = it.begin(); more; more = it.next(), ++n)
-      for (int w = 0; w < TILES; ++w) {
-        if (n > 0) rows_wait(&sm.q_empty[w], (n - 1) & 1u, gave_up);
-        const int row0 = it.rb * S::rows + w * 128, rows = min(128, it.s.tokens * a.rep - row0);
-        unsigned char* tile = smem + w * S::tile + (piece >> 3) * 128 * 128;
-        for (int r = sub; r < rows; r += R) {
-          const uint32_t row = row0 + r, t = row / a.rep_div;
-          const uint16_t* x = a.q + (it.s.r0 + (int64_t)t) * a.ldq + (int64_t)(it.g * a.rep + row - t * a.rep) * D + piece * 8;
-          cp_async16(smem_u32(tile + r * 128 + (((piece & 7) ^ (r & 7)) << 4)), x, 16u);
-        }
-        cp_async_commit();
-        cp_async_wait<0>();
-        if (a.sign)  // a negative scale's, so that a larger product weighs more
-          for (int r = sub; r < rows; r += R) {
-            uint4* x = reinterpret_cast<uint4*>(tile + r * 128 + (((piece & 7) ^ (r & 7)) << 4));
-            const uint4 y = *x;
-            *x = make_uint4(y.x ^ a.sign, y.y ^ a.sign, y.z ^ a.sign, y.w ^ a.sign);
-          }
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sm.q_full[w]));
-      }
+    }
   } else if (warp == kPrMma) {
-    if (lane == 0) {
-      uint32_t items = 0, fill = 0, probs[2] = {0, 0};
-      const uint32_t q0 = smem_u32(smem), ring = smem_u32(smem + S::ring);
-      auto scores = [&](int w, uint32_t f) {  // of group w, from the keys of fill f
-        const uint32_t q = q0 + (TILES == 2 ? w : 0) * S::tile, k = ring + f % NS * S::tile;
+    // The whole warp keeps count, one lane issues: descriptors then are a warp's, not a lane's.
+    uint32_t fill = 0, probs[2] = {0, 0}, items[2] = {0, 0};
+    const uint32_t q0 = smem_u32(smem), ring = smem_u32(smem + S::ring);
+    auto scores = [&](int w, uint32_t q, uint32_t f) {  // of group w, from the keys of fill f
+      const uint64_t qd = tc_desc_sw128(q), kd = tc_desc_sw128(ring + f % NS * S::tile);
+      if (one_lane()) {
 #pragma unroll
         for (int x = 0; x < D / 16; ++x)
-          tc_mma_f16(tmem + w * 128, tc_desc_sw128(q + (x >> 2) * 128 * 128 + (x & 3) * 32),
-                     tc_desc_sw128(k + (x >> 2) * 128 * 128 + (x & 3) * 32), kScores, x > 0);
+          tc_mma_f16(tmem + w * 128, qd + (x >> 2) * (128 * 128 / 16) + (x & 3) * 2, kd + (x >> 2) * (128 * 128 / 16) + (x & 3) * 2,
+                     kScores, x > 0);
         tc_commit(smem_u32(&sm.s_full[w]));
-      };
-      auto outputs = [&](int w, uint32_t f, bool add) {  // of group w, from the values of fill f
-        const uint32_t v = ring + f % NS * S::tile, p = tmem + w * 128;
+      }
+    };
+    // Outputs of group w from the values of fill f, the keys of the chunk's first or second half.
+    auto outputs = [&](int w, uint32_t f, int half, uint32_t add) {
+      const uint64_t vd = values_desc(ring + f % NS * S::tile) + half * (64 * 128 / 16);
+      const uint32_t p = tmem + w * 128 + 32 * half, o = tmem + kOut + w * 128;
+      if (one_lane())
 #pragma unroll
-        for (int x = 0; x < kPrKeys / 16; ++x) {
-          if (TILES == 2) {
-            tc_mma_f16_ta(tmem + kOut + w * 128, p + 8 * x, values_desc(v + x * 2048), kOutputs, add || x > 0);
+        for (int x = 0; x < 4; ++x) tc_mma_f16_ta(o, p + 8 * x, vd + x * (2048 / 16), kOutputs, x > 0 ? 1u : add);
+    };
+    auto outputs_two = [&](int w, uint32_t f, int half, uint32_t add) {  // the same from probabilities of two numbers
+      const uint64_t vd = values_desc(ring + f % NS * S::tile) + half * (64 * 128 / 16);
+      const uint32_t p = tmem + w * 128 + 64 * half, o = tmem + kOut + w * 128;
+      if (one_lane())
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          tc_mma_f16_ta(o, p + 32 * (x >> 1) + 8 * (x & 1), vd + x * (2048 / 16), kOutputs, x > 0 ? 1u : add);
+          tc_mma_f16_ta(o, p + 32 * (x >> 1) + 8 * (x & 1) + 16, vd + x * (2048 / 16), kOutputs, 1u);
+        }
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (one_lane()) tc_commit(smem_u32(bar));
+    };
+    auto filled = [&](uint32_t f) {
+      rows_wait(&sm.kv_full[f % NS], f / NS & 1u, gave_up);
+      fence_async_shared();  // the copies are of the generic proxy, the products of the other
+      __syncwarp();
+    };
+    auto release = [&](uint32_t f) { commit(&sm.kv_empty[f % NS]); };
+    auto ready = [&](int w, int half) {
+      rows_wait(half ? &sm.p_full[w] : &sm.p_half[w], probs[w] & 1u, gave_up);
+      probs[w] += half;
+      tc_fence_after_sync();
+      __syncwarp();
+    };
+    for (bool more = it.begin(); more; more = it.next()) {
+      const int m = it.c1 - it.c0;
+      const bool pair = it.rows() > 128;
+      for (int w = 0; w < (pair ? 2 : 1); ++w) rows_wait(&sm.q_full[w], items[w]++ & 1u, gave_up);
+      tc_fence_after_sync();
+      __syncwarp();
+      if (pair) {
+        filled(fill);
+        scores(0, q0, fill);
+        scores(1, q0 + S::tile, fill);
+        release(fill);
+#pragma unroll 1
+        for (int j = 0; j < m; ++j, fill += 2) {
+          filled(fill + 1);
+          if (j + 1 < m) filled(fill + 2);
+          ready(0, 0);
+          outputs(0, fill + 1, 0, j > 0);
+          ready(0, 1);
+          outputs(0, fill + 1, 1, 1u);
+          if (j + 1 < m) {
+            scores(0, q0, fill + 2);
           } else {
-            tc_mma_f16_ta(tmem + kOut + w * 128, p + 32 * (x >> 1) + 8 * (x & 1), values_desc(v + x * 2048), kOutputs, add || x > 0);
-            tc_mma_f16_ta(tmem + kOut + w * 128, p + 32 * (x >> 1) + 8 * (x & 1) + 16, values_desc(v + x * 2048), kOutputs, 1u);
+            commit(&sm.q_empty[0]);
+            commit(&sm.o_done[0]);
+          }
+          ready(1, 0);
+          outputs(1, fill + 1, 0, j > 0);
+          ready(1, 1);
+          outputs(1, fill + 1, 1, 1u);
+          release(fill + 1);
+          if (j + 1 < m) {
+            scores(1, q0 + S::tile, fill + 2);
+            release(fill + 2);
+          } else {
+            commit(&sm.q_empty[1]);
+            commit(&sm.o_done[1]);
           }
         }
-      };
-      auto filled = [&](uint32_t f) {
-        rows_wait(&sm.kv_full[f % NS], f / NS & 1u, gave_up);
-        fence_async_shared();  // the copies are of the generic proxy, the products of the other
-      };
-      auto release = [&](uint32_t f) { tc_commit(smem_u32(&sm.kv_empty[f % NS])); };
-      auto ready = [&](int w) {
-        rows_wait(&sm.p_full[w], probs[w] & 1u, gave_up);
-        ++probs[w];
-        tc_fence_after_sync();
-      };
-      for (bool more = it.begin(); more; more = it.next(), ++items) {
-        const int m = it.c1 - it.c0;
-        for (int w = 0; w < TILES; ++w) rows_wait(&sm.q_full[w], items & 1u, gave_up);
-        tc_fence_after_sync();
-        if (TILES == 2) {
-          filled(fill);
-          scores(0, fill);
-          scores(1, fill);
-          release(fill);
-          for (int j = 0; j < m; ++j, fill += 2) {
-            filled(fill + 1);
-            ready(0);
-            outputs(0, fill + 1, j > 0);
-            if (j + 1 < m) {
-              filled(fill + 2);
-              scores(0, fill + 2);
-            } else {
-              tc_commit(smem_u32(&sm.q_empty[0]));
-              tc_commit(smem_u32(&sm.o_done[0]));
-            }
-            ready(1);
-            outputs(1, fill + 1, j > 0);
-            release(fill + 1);
-            if (j + 1 < m) {
-              scores(1, fill + 2);
-              release(fill + 2);
-            } else {
-              tc_commit(smem_u32(&sm.q_empty[1]));
-              tc_commit(smem_u32(&sm.o_done[1]));
-            }
-          }
-        } else {
-          for (int j = 0; j < min(m, 2); ++j) {
-            filled(fill + 2 * j);
-            scores(j, fill + 2 * j);
-            release(fill + 2 * j);
-          }
-          if (m <= 2) tc_commit(smem_u32(&sm.q_empty[0]));
-          for (int j = 0; j < m; ++j, fill += 2) {
-            const int w = j & 1;
-            filled(fill + 1);
-            ready(w);
-            outputs(w, fill + 1, j > 1);
-            release(fill + 1);
-            if (j + 2 < m) {
-              filled(fill + 4);
-              scores(w, fill + 4);
-              release(fill + 4);
-              if (j + 3 == m) tc_commit(smem_u32(&sm.q_empty[0]));
-            } else {
-              tc_commit(smem_u32(&sm.o_done[w]));
-            }
+      } else {
+        for (int j = 0; j < min(m, 2); ++j) {
+          filled(fill + 2 * j);
+          scores(j, q0, fill + 2 * j);
+          release(fill + 2 * j);
+        }
+        if (m <= 2) commit(&sm.q_empty[0]);
+#pragma unroll 1
+        for (int j = 0; j < m; ++j, fill += 2) {
+          const int w = j & 1;
+          filled(fill + 1);
+          ready(w, 0);
+          outputs_two(w, fill + 1, 0, j > 1);
+          ready(w, 1);
+          outputs_two(w, fill + 1, 1, 1u);
+          release(fill + 1);
+          if (j + 2 < m) {
+            filled(fill + 4);
+            scores(w, q0, fill + 4);
+            release(fill + 4);
+            if (j + 3 == m) commit(&sm.q_empty[0]);
+          } else {
+            commit(&sm.o_done[w]);
           }
         }
       }
@@ -648,7 +945,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
     const uint32_t s_at = tmem + lanes + w * 128, o_at = tmem + lanes + kOut + w * 128;
     uint32_t chunk_count = 0, item_count = 0;
     for (bool more = it.begin(); more; more = it.next()) {
-      const int row = it.rb * S::rows + (TILES == 2 ? w * 128 : 0) + r, rows = it.s.tokens * a.rep;
+      const bool pair = it.rows() > 128;
+      const int fold = it.fold(), size = 128 >> fold, copy = r >> (7 - fold);
+      const int row = it.rb * kPrRows + (pair ? w * 128 : 0) + (r & (size - 1)), rows = it.s.tokens * a.rep;
       const bool there = row < rows, warp_there = row - lane < rows;
       const int t = there ? (int)((uint32_t)row / a.rep_div) : it.k.t1;
       RowView view;
@@ -679,9 +978,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
         view.lo = a.window ? view.hi - a.window + 1 : 0;
         view.nodes = 0;
       }
-      float m = -INFINITY, l = 0.0f;
-      bool any = false;  // a chunk of this group came before
-      for (int v = it.c0 + (TILES == 1 ? w : 0); v < it.c1; v += TILES == 1 ? 2 : 1) {
+      RowState state = {-INFINITY, 0.0f, false};
+#pragma unroll 1
+      for (int v = it.c0 + (pair ? 0 : w); v < it.c1; v += pair ? 1 : 2) {
         rows_wait(&sm.s_full[w], chunk_count & 1u, gave_up);
         ++chunk_count;
         tc_fence_after_sync();
@@ -691,162 +990,163 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
           uint32_t see[4];
 #pragma unroll
           for (int c = 0; c < 4; ++c) see[c] = edge ? seen32<TREE>(a, view, k0 + 32 * c) : 0xffffffffu;
-          auto load = [&](int c, float (&s)[32]) {
-            uint32_t x[32];
-            tmem_ld32(s_at + 32 * c, x);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(x[i]);
-            if (edge)
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!(see[c] >> i & 1u)) s[i] = -INFINITY;
-          };
-          float top = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float s[32];
-            load(c, s);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i]);
-          }
-          top *= a.scale;
-          // lanes without a row hold what happens to lie there
-          if (__any_sync(0xffffffffu, there && top > (m == -INFINITY ? -INFINITY : m + kPrHeadroom))) {
-            const float mx = fmaxf(m, top), f = m == -INFINITY ? 0.0f : pr_ex2(m - mx);
-            m = mx;
-            l *= f;
-            // the scores of a chunk are complete after the outputs of the one before it
-            if (any)
-#pragma unroll 1
-              for (int c = 0; c < D; c += 32) {
-                uint32_t x[32];
-                tmem_ld32(o_at + c, x);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
-                tmem_st32(o_at + c, x);
-              }
-          }
-          const float z = kPrShift<BF> - (m == -INFINITY ? 0.0f : m);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float s[32];
-            load(c, s);
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              s[i] = pr_ex2(fmaf(s[i], a.scale, z));
-              sum[i & 3] += s[i];
-            }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            if (TILES == 2) {
-              uint32_t p[16];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) p[i] = pack2<BF>(s[2 * i], s[2 * i + 1]);
-              tmem_st16(s_at + 16 * c, p);
-            } else {
-              uint32_t p[32];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                p[i] = pack2<BF>(s[2 * i], s[2 * i + 1]);
-                const float2 y = unpack2<BF>(p[i]);
-                p[16 + i] = pack2<BF>(s[2 * i] - y.x, s[2 * i + 1] - y.y);
-              }
-              tmem_st32(s_at + 32 * c, p);
-            }
-          }
+          if (pair)
+            turn<BF, D, false, 4>(s_at, s_at, o_at, a.scale, edge, see, there, state, &sm.p_half[w]);
+          else if (fold == 0)
+            turn<BF, D, true, 4>(s_at, s_at, o_at, a.scale, edge, see, there, state, &sm.p_half[w]);
+          else if (fold == 1)
+            turn_part<BF, D, 2>(s_at, o_at, 2 * copy, a.scale, edge, see, there, state);
+          else
+            turn_part<BF, D, 1>(s_at, o_at, copy, a.scale, edge, see, there, state);
           tmem_wait_st();
         }
-        any = true;
+        state.any = true;
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sm.p_full[w]));
+        if (lane == 0) {
+          if (fold || !warp_there) mbar_arrive(smem_u32(&sm.p_half[w]));
+          mbar_arrive(smem_u32(&sm.p_full[w]));
+        }
       }
 
       // The item's end in this run.
-      if (any) {
+      if (state.any) {
         rows_wait(&sm.o_done[w], item_count & 1u, gave_up);
         ++item_count;
         tc_fence_after_sync();
       }
-      const bool two = TILES == 1 && it.c1 - it.c0 > 1;  // the groups meet
-      float f0 = 1.0f, f1 = 0.0f;
-      const bool whole = it.whole();
-      const int64_t part = (int64_t)(2 * blockIdx.x + (it.first ? 0 : 1)) * S::rows + (TILES == 2 ? w * 128 : 0) + r;
-      const bool odd = *(volatile int*)&sm.odd;
-#pragma unroll 1
-      for (int half = 0; half < (TILES == 1 ? D / 64 : 1); ++half) {
-        float* meet = reinterpret_cast<float*>(smem + TILES * S::tile) + r * 64;
-        if (two) {
-          if (w == 1 && warp_there) {
-#pragma unroll 1
-            for (int c = 0; c < 64; c += 32) {
-              uint32_t x[32];
-              tmem_ld32(o_at + half * 64 + c, x);
-              if (there)
+      const bool whole = it.whole(), odd = *(volatile int*)&sm.odd;
+      const int64_t part = (int64_t)(2 * blockIdx.x + (it.first ? 0 : 1)) * a.part_rows + (row - it.rb * kPrRows);
+      uint16_t* const to = a.out + (it.s.r0 + (int64_t)t) * a.ldo + (int64_t)(it.g * a.rep + row - t * a.rep) * D;
+      auto store = [&](auto& o, int c, float l) {  // columns from c on
+        constexpr int N = sizeof(o) / sizeof(float);
+        if (odd) give_back<BF, D, TREE, N>(it, view, o, c);
+        if (!there) return;
+        if (whole) {
+          const float inv = 1.0f / l;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                  *reinterpret_cast<uint4*>(meet + ((((c >> 2) + i) ^ (r & 15)) << 2)) =
-                      make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-            }
-            if (half == 0) sm.ml[r] = make_float2(m, l);
-          }
-          named_barrier_sync(1, 256);
-          if (w == 0 && half == 0) {
-            const float2 ml = sm.ml[r];
-            const float mx = fmaxf(m, ml.x);
-            f0 = m == -INFINITY ? 0.0f : pr_ex2(m - mx);
-            f1 = ml.x == -INFINITY ? 0.0f : pr_ex2(ml.x - mx);
-            m = mx;
-            l = l * f0 + ml.y * f1;
-          }
+          for (int i = 0; i < N; i += 8)
+            *reinterpret_cast<uint4*>(to + c + i) =
+                make_uint4(pack2<BF>(o[i] * inv, o[i + 1] * inv), pack2<BF>(o[i + 2] * inv, o[i + 3] * inv),
+                           pack2<BF>(o[i + 4] * inv, o[i + 5] * inv), pack2<BF>(o[i + 6] * inv, o[i + 7] * inv));
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; i += 4)
+            *reinterpret_cast<float4*>(a.part + part * D + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
-        if ((TILES == 2 || w == 0) && warp_there) {
-          const float inv = whole ? 1.0f / l : 1.0f;
-          const int head = it.g * a.rep + row - t * a.rep;
+      };
+      if (pair) {
+        if (warp_there) {
 #pragma unroll 1
-          for (int c = TILES == 1 ? half * 64 : 0; c < (TILES == 1 ? half * 64 + 64 : D); c += 32) {
+          for (int c = 0; c < D; c += 32) {
             uint32_t x[32];
             float o[32];
             tmem_ld32(o_at + c, x);
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(x[i]);
-            if (two && there) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float4 y = *reinterpret_cast<const float4*>(meet + (((((c & 63) >> 2) + i) ^ (r & 15)) << 2));
-                o[4 * i] = fmaf(o[4 * i], f0, y.x * f1);
-                o[4 * i + 1] = fmaf(o[4 * i + 1], f0, y.y * f1);
-                o[4 * i + 2] = fmaf(o[4 * i + 2], f0, y.z * f1);
-                o[4 * i + 3] = fmaf(o[4 * i + 3], f0, y.w * f1);
-              }
-            }
-            if (odd) {
-              const It here = it;  // copies: what lies in memory for the call
-              const RowView mine = view;
-              float y[32];
-#pragma unroll
-              for (int i = 0; i < 32; ++i) y[i] = o[i];
-              add_odd<BF, D>(here, mine, y, c);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = y[i];
-            }
-            if (there) {
-              if (whole) {
-                uint4* to = reinterpret_cast<uint4*>(a.out + (it.s.r0 + (int64_t)t) * a.ldo + (int64_t)head * D + c);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  to[i] = make_uint4(pack2<BF>(o[8 * i] * inv, o[8 * i + 1] * inv), pack2<BF>(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
-                                     pack2<BF>(o[8 * i + 4] * inv, o[8 * i + 5] * inv), pack2<BF>(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
-              } else {
-                float4* to = reinterpret_cast<float4*>(a.part + part * D + c);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-              }
-            }
+            store(o, c, state.l);
           }
-          if (!whole && there && half == 0) a.part_ml[part] = make_float2(m, l);
+          if (!whole && there) a.part_ml[part] = make_float2(state.m, state.l);
         }
-        if (two) named_barrier_sync(1, 256);  // before the columns are written again
+      } else {
+        const bool two = it.c1 - it.c0 > 1;  // both groups have chunks
+        if (w == 0 || two) {
+          float* const meet = reinterpret_cast<float*>(smem + S::tile);
+          auto place = [&](int row, int c) {  // of four columns, turned by the row against bank conflicts
+            return reinterpret_cast<float4*>(meet + row * 64 + (((c >> 2) ^ (row & 15)) << 2));
+          };
+          float f0 = 1.0f, f1 = 0.0f;
+#pragma unroll 1
+          for (int half = 0; half < D; half += 64) {
+            if (w == 1) {
+              if (warp_there)
+#pragma unroll 1
+                for (int c = 0; c < 64; c += 32) {
+                  uint32_t x[32];
+                  tmem_ld32(o_at + half + c, x);
+                  if (there)
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                      *place(r, c + i) = make_float4(__uint_as_float(x[i]), __uint_as_float(x[i + 1]),
+                                                     __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+                }
+              if (half == 0) sm.ml[r] = make_float2(state.m, state.l);
+            }
+            if (two) named_barrier_sync(1, 256);
+            if (w == 0) {
+              if (half == 0) {
+                if (two) {
+                  const float2 ml = sm.ml[r];
+                  const float mx = fmaxf(state.m, ml.x);
+                  f0 = state.m == -INFINITY ? 0.0f : pr_ex2(state.m - mx);
+                  f1 = ml.x == -INFINITY ? 0.0f : pr_ex2(ml.x - mx);
+                  state.m = mx;
+                  state.l = state.l * f0 + ml.y * f1;
+                }
+                sm.ml[r] = make_float2(state.m, state.l);
+              }
+              if (warp_there)
+#pragma unroll 1
+                for (int c = 0; c < 64; c += 32) {
+                  uint32_t x[32];
+                  float o[32];
+                  tmem_ld32(o_at + half + c, x);
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(x[i]);
+                  if (two && there)
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                      const float4 y = *place(r, c + i);
+                      o[i] = fmaf(o[i], f0, y.x * f1);
+                      o[i + 1] = fmaf(o[i + 1], f0, y.y * f1);
+                      o[i + 2] = fmaf(o[i + 2], f0, y.z * f1);
+                      o[i + 3] = fmaf(o[i + 3], f0, y.w * f1);
+                    }
+                  if (fold == 0) {
+                    store(o, half + c, state.l);
+                  } else if (there) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) *place(r, c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                  }
+                }
+              if (fold) {
+                // the copies: a thread has some of its row's columns, of all copies
+                named_barrier_sync(2, 128);
+                const int lr = r & (size - 1);
+                float mx = -INFINITY, l = 0.0f, f[4];
+                for (int k = 0; k < 1 << fold; ++k) mx = fmaxf(mx, sm.ml[lr + k * size].x);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const float2 ml = sm.ml[(lr + k * size) & 127];
+                  f[k] = k >= 1 << fold || ml.x == -INFINITY ? 0.0f : pr_ex2(ml.x - mx);
+                  l = fmaf(ml.y, f[k], l);
+                }
+#pragma unroll 1
+                for (int c = copy * (64 >> fold); c < (copy + 1) * (64 >> fold); c += 16) {
+                  float o[16] = {};
+                  if (there)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                      if (f[k] != 0.0f)
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) {
+                          const float4 y = *place(lr + k * size, c + i);
+                          o[i] = fmaf(y.x, f[k], o[i]);
+                          o[i + 1] = fmaf(y.y, f[k], o[i + 1]);
+                          o[i + 2] = fmaf(y.z, f[k], o[i + 2]);
+                          o[i + 3] = fmaf(y.w, f[k], o[i + 3]);
+                        }
+                  store(o, half + c, l);
+                }
+                if (!whole && there && half == 0 && copy == 0) a.part_ml[part] = make_float2(mx, l);
+                if (half + 64 < D || !two) named_barrier_sync(2, 128);  // before the columns are written again
+              } else if (!whole && there && half == 0) {
+                a.part_ml[part] = make_float2(state.m, state.l);
+              }
+            }
+            if (two) named_barrier_sync(1, 256);
+          }
+        }
       }
     }
   }
@@ -871,18 +1171,18 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
 
 // The parts of an item that several CTAs shared, joined in the keys' order: grid (CTAs, rows / 8), a warp
 // per row.
-template <bool BF, int D, int TILES, bool TREE>
+template <bool BF, int D, bool TREE>
 __global__ void __launch_bounds__(256) k_paged_rows_join(const __grid_constant__ RowsArgs a) {
-  constexpr int ROWS = 128 * TILES, PL = D / 32;
+  constexpr int PL = D / 32;
   pdl_trigger();
   pdl_wait();
   const SharedItem x = a.shared[blockIdx.x];
   if (!x.there) return;
   const RowRange s = range_of<TREE>(a, x.b, false);
-  const int lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5), row = x.rb * ROWS + r;
+  const int lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5), row = x.rb * kPrRows + r;
   if (row >= s.tokens * a.rep) return;
   const int n = x.last_cta - (int)blockIdx.x + 1;
-  auto part = [&](int i) { return (int64_t)(i == 0 ? x.first_part : 2 * ((int)blockIdx.x + i)) * ROWS + r; };
+  auto part = [&](int i) { return (int64_t)(i == 0 ? x.first_part : 2 * ((int)blockIdx.x + i)) * a.part_rows + r; };
   float M = -INFINITY, L = 0.0f, acc[PL] = {};
   for (int i = lane; i < n; i += 32) M = fmaxf(M, a.part_ml[part(i)].x);
 #pragma unroll
@@ -903,44 +1203,39 @@ __global__ void __launch_bounds__(256) k_paged_rows_join(const __grid_constant__
   for (int j = 0; j < PL / 2; ++j) to[j] = pack2<BF>(acc[2 * j] / L, acc[2 * j + 1] / L);
 }
 
-// Blocks of 256 rows where sequences have more than 128 rows of a KV head on average.
-static int rows_tiles(int64_t n, int64_t rep, int64_t batch) { return n * rep > 128 * batch ? 2 : 1; }
-
 struct RowsSpace {
-  int64_t part, part_ml, shared;
+  int64_t rows, part, part_ml, shared;
   int64_t bytes() const { return part + part_ml + shared; }
 };
-static RowsSpace rows_space(int64_t n, int64_t heads, int64_t kv_heads, int64_t D, int64_t batch) {
-  const int64_t rows = 128 * rows_tiles(n, heads / kv_heads, batch);
-  return RowsSpace{2 * kPrGrid * rows * D * 4, 2 * kPrGrid * rows * 8, align_up(kPrGrid * (int64_t)sizeof(SharedItem), 256)};
+static RowsSpace rows_space(int64_t n, int64_t rep, int64_t D) {
+  RowsSpace s;
+  s.rows = std::min<int64_t>(kPrRows, align_up(n * rep, 8));
+  s.part = align_up(2 * kPrGrid * s.rows * D * 4, 256);
+  s.part_ml = align_up(2 * kPrGrid * s.rows * 8, 256);
+  s.shared = align_up(kPrGrid * (int64_t)sizeof(SharedItem), 256);
+  return s;
 }
 static bool rows_limits(int64_t batch, int64_t n, int64_t heads, int64_t kv_heads, int64_t D) {
   return batch <= kPagedMaxBatch && heads <= 65535 && kv_heads <= 1024 && (D == 64 || D == 128) && n <= INT32_MAX &&
          n * (heads / kv_heads) <= INT32_MAX;
 }
 
-template <bool BF, int D, int TILES, bool TREE>
+template <bool BF, int D, bool TREE>
 static cudaError_t launch_rows(const RowsArgs& a, cudaStream_t s) {
-  auto* k = k_paged_rows<BF, D, TILES, TREE>;
-  constexpr int bytes = RowsShape<D, TILES>::bytes;
+  auto* k = k_paged_rows<BF, D, TREE>;
   static std::atomic<bool> done[64];
   int dev;
   bool needs;
   cudaError_t e = needs_opt_in(done, dev, needs);
   if (e != cudaSuccess) return e;
   if (needs) {
-    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsShape<D>::bytes);
     if (e != cudaSuccess) return e;
     opted_in(done, dev);
   }
-  e = launch_pdl(k, dim3(kPrGrid), dim3(kPrThreads), bytes, s, 1u, a);
+  e = launch_pdl(k, dim3(kPrGrid), dim3(kPrThreads), RowsShape<D>::bytes, s, 1u, a);
   if (e != cudaSuccess) return e;
-  return launch_pdl(k_paged_rows_join<BF, D, TILES, TREE>, dim3(kPrGrid, 16 * TILES), dim3(256), 0, s, 1u, a);
-}
-template <bool BF, int D>
-static cudaError_t launch_rows_of(const RowsArgs& a, int tiles, cudaStream_t s) {
-  if (a.parents) return tiles == 2 ? launch_rows<BF, D, 2, true>(a, s) : launch_rows<BF, D, 1, true>(a, s);
-  return tiles == 2 ? launch_rows<BF, D, 2, false>(a, s) : launch_rows<BF, D, 1, false>(a, s);
+  return launch_pdl(k_paged_rows_join<BF, D, TREE>, dim3(kPrGrid, (unsigned)(a.part_rows / 8)), dim3(256), 0, s, 1u, a);
 }
 
 }  // namespace otf
@@ -966,7 +1261,7 @@ extern "C" OTF_API int64_t otf_paged_attn_rows_workspace_bytes(int64_t batch, in
   if (batch <= 0 || n <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads ||
       !otf::rows_limits(batch, n, heads, kv_heads, head_dim))
     return -1;
-  return otf::rows_space(n, heads, kv_heads, head_dim, batch).bytes();
+  return otf::rows_space(n, heads / kv_heads, head_dim).bytes();
 }
 
 extern "C" OTF_API int otf_paged_attn_rows(const otf_paged_cache* cache, const void* q, int64_t ldq, int64_t heads,
@@ -984,7 +1279,7 @@ extern "C" OTF_API int otf_paged_attn_rows(const otf_paged_cache* cache, const v
     return OTF_ERR_UNSUPPORTED;
   if (!otf::rows16(q, ldq, heads * D) || !otf::rows16(out, ldo, heads * D)) return OTF_ERR_INVALID;
   if (otf::rows_overlap(q, ldq, heads * D, out, ldo, heads * D, n)) return OTF_ERR_INVALID;
-  const otf::RowsSpace space = otf::rows_space(n, heads, a.c.kv_heads, D, a.c.batch);
+  const otf::RowsSpace space = otf::rows_space(n, heads / a.c.kv_heads, D);
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < space.bytes())
     return OTF_ERR_INVALID;
   st = check_device();
@@ -1006,13 +1301,33 @@ extern "C" OTF_API int otf_paged_attn_rows(const otf_paged_cache* cache, const v
   // a masked -inf stays one under a scale of 0, and no finite score counts under 2^-149
   a.scale = fmaxf(fabsf(scale * otf::kPrLog2e), 0x1p-149f);
   a.sign = scale < 0.0f ? 0x80008000u : 0u;
+  // Tensor copies where groups of 4 tokens or more lie in one page; else, and for the chunks that are not all there,
+  // 16-byte copies.
+  const int box = std::gcd((int)a.c.page_size, otf::kPrKeys);
+  if (box >= 4) {
+    const uint64_t dims[4] = {(uint64_t)D, (uint64_t)a.c.kv_heads, (uint64_t)a.c.page_size, (uint64_t)a.c.n_pages};
+    const uint64_t strides[3] = {(uint64_t)a.c.head_stride * 2, (uint64_t)a.c.token_stride * 2, (uint64_t)a.c.page_stride * 2};
+    const uint32_t boxes[4] = {64, 1, (uint32_t)box, 1};
+    if (otf::encode_tiled_4d_swizzled(&a.kmap, a.c.k, dims, strides, boxes) &&
+        otf::encode_tiled_4d_swizzled(&a.vmap, a.c.v, dims, strides, boxes))
+      a.box = box;
+  }
+  if (a.rep <= 32 && 32 % a.rep == 0 && !a.sign) {
+    const uint64_t dims[4] = {(uint64_t)D, (uint64_t)heads, (uint64_t)n, 1};
+    const uint64_t strides[3] = {(uint64_t)D * 2, (uint64_t)ldq * 2, (uint64_t)ldq * 2};
+    const uint32_t boxes[4] = {64, (uint32_t)a.rep, (uint32_t)(32 / a.rep), 1};
+    if (otf::encode_tiled_4d_swizzled(&a.qmap, a.q, dims, strides, boxes)) a.q_box = 32 / a.rep;
+  }
   char* w = static_cast<char*>(workspace);
   a.part = reinterpret_cast<float*>(w);
   a.part_ml = reinterpret_cast<float2*>(w + space.part);
   a.shared = reinterpret_cast<otf::SharedItem*>(w + space.part + space.part_ml);
-  const int tiles = otf::rows_tiles(n, a.rep, a.c.batch);
+  a.part_rows = (int)space.rows;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = cache->dtype == OTF_DTYPE_BF16;
-  return set_cuda_error(D == 128 ? (bf ? otf::launch_rows_of<true, 128>(a, tiles, s) : otf::launch_rows_of<false, 128>(a, tiles, s))
-                                 : (bf ? otf::launch_rows_of<true, 64>(a, tiles, s) : otf::launch_rows_of<false, 64>(a, tiles, s)));
+  auto* launch = parents ? (D == 128 ? (bf ? otf::launch_rows<true, 128, true> : otf::launch_rows<false, 128, true>)
+                                     : (bf ? otf::launch_rows<true, 64, true> : otf::launch_rows<false, 64, true>))
+                         : (D == 128 ? (bf ? otf::launch_rows<true, 128, false> : otf::launch_rows<false, 128, false>)
+                                     : (bf ? otf::launch_rows<true, 64, false> : otf::launch_rows<false, 64, false>));
+  return set_cuda_error(launch(a, s));
 }
