@@ -172,57 +172,73 @@ struct RunStart {
   int b, rb, g, pad;
 };
 
-// An item of a run, with the chunks [c0, c1) that the run has of it.
-template <bool TREE>
-struct Item {
-  const RowsArgs& a;
-  const int64_t u0, u1;
-  int64_t at;
-  int b, rb, g, c0, c1;
+// What a run has of an item: the chunks [c0, c1).  Without any it is the run's end.
+struct __align__(16) Portion {
+  int b, rb, g, rows;  // rows of the block
+  int c0, c1, first;   // first: of the run
   RowRange s;
   Keys k;
-  bool first = true;  // of the run
+  int pad;
+  __device__ __forceinline__ bool whole() const { return c0 == 0 && c1 == k.chunks; }
+  // Copies of the rows: 1 << fold.
+  __device__ __forceinline__ int fold() const { return rows <= 32 ? 2 : rows <= 64 ? 1 : 0; }
+};
+static_assert(sizeof(Portion) == 80, "");
 
-  __device__ __forceinline__ Item(const RowsArgs& args, const RunStart& r)
-      : a(args), u0(r.u0), u1(r.u1), at(r.at), b(r.b), rb(r.rb), g(r.g) {}
+// The portions of a run, one after another.
+template <bool TREE>
+struct Walk {
+  const RowsArgs& a;
+  const int64_t u0, u1;
+  int64_t at;  // the item's first unit
+  Portion p;
+
+  __device__ __forceinline__ Walk(const RowsArgs& args, const RunStart& r) : a(args), u0(r.u0), u1(r.u1), at(r.at) {
+    p.b = r.b;
+    p.rb = r.rb;
+    p.g = r.g;
+    p.first = 1;
+  }
+  __device__ __forceinline__ void block() {
+    p.k = keys_of<TREE>(a, p.s, p.rb);
+    p.rows = min(kPrRows, p.s.tokens * a.rep - p.rb * kPrRows);
+  }
   __device__ __forceinline__ bool clip() {
-    c0 = (int)max((int64_t)0, u0 - at - kPrItemUnits);
-    c1 = (int)min((int64_t)k.chunks, u1 - at - kPrItemUnits);
-    return c1 > c0;
+    p.c0 = (int)max((int64_t)0, u0 - at - kPrItemUnits);
+    p.c1 = (int)min((int64_t)p.k.chunks, u1 - at - kPrItemUnits);
+    return p.c1 > p.c0;
   }
   __device__ __forceinline__ bool begin() {
     if (u0 >= u1) return false;
-    s = range_of<TREE>(a, b, false);
-    k = keys_of<TREE>(a, s, rb);
-    return clip() || next_with_chunks();
+    p.s = range_of<TREE>(a, p.b, false);
+    block();
+    return clip() || find();
   }
   __device__ __forceinline__ bool next() {
-    first = false;
-    return next_with_chunks();
+    p.first = 0;
+    return find();
   }
-  __device__ __forceinline__ bool next_with_chunks() {
+  __device__ __forceinline__ bool find() {
     do {
-      at += k.chunks + kPrItemUnits;
+      at += p.k.chunks + kPrItemUnits;
       if (at + kPrItemUnits >= u1) return false;
-      if (++g == a.c.kv_heads) {
-        g = 0;
-        if ((int64_t)(++rb) * kPrRows >= (int64_t)s.tokens * a.rep) {
-          rb = 0;
+      if (++p.g == a.c.kv_heads) {
+        p.g = 0;
+        if ((int64_t)(++p.rb) * kPrRows >= (int64_t)p.s.tokens * a.rep) {
+          p.rb = 0;
           do {
-            if (++b >= a.c.batch) return false;
-            s = range_of<TREE>(a, b, false);
-          } while (s.tokens == 0);
+            if (++p.b >= a.c.batch) return false;
+            p.s = range_of<TREE>(a, p.b, false);
+          } while (p.s.tokens == 0);
         }
-        k = keys_of<TREE>(a, s, rb);
+        block();
       }
     } while (!clip());
     return true;
   }
-  __device__ __forceinline__ bool whole() const { return c0 == 0 && c1 == k.chunks; }
-  __device__ __forceinline__ int rows() const { return min(kPrRows, s.tokens * a.rep - rb * kPrRows); }
-  // Copies of the rows: 1 << fold.
-  __device__ __forceinline__ int fold() const { return rows() <= 32 ? 2 : rows() <= 64 ? 1 : 0; }
 };
+
+constexpr int kPrSmall = 3072;
 
 template <int D>
 struct RowsShape {
@@ -230,7 +246,7 @@ struct RowsShape {
   static constexpr int slots = D == 128 ? 5 : 10;        // of the ring
   static constexpr int ring = D == 128 ? 2 * tile : tile + 128 * 64 * 4;  // behind two tiles of queries, or one and `meet`
   static constexpr int small = ring + slots * tile;      // barriers and the like
-  static constexpr int bytes = 1024 + small + 2048;
+  static constexpr int bytes = small + kPrSmall;  // the runtime's own kilobyte lies before a 1024-byte border
 };
 // Behind the first tile of queries, where there is no second one: 64 columns of the outputs of 128 rows, where
 // the groups and copies meet.
@@ -239,14 +255,16 @@ struct RowsShape {
 struct RowsSmall {
   uint64_t kv_full[10], kv_empty[10], v_landed[10];
   uint64_t q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_done[2];
+  uint64_t item_full[4], item_empty[4];
+  Portion items[4];  // the run's next ones, from the warp that fetches keys to all others
   RunStart run;
   int64_t sums[16];
-  float2 ml[128];
+  float2 ml[256];
   uint32_t tmem;
   int gave_up;   // a wait ran out: no more waiting
   int odd;       // an infinity or NaN was taken out of some values
 };
-static_assert(sizeof(RowsSmall) <= 2048, "");
+static_assert(sizeof(RowsSmall) <= kPrSmall, "");
 
 // A bounded wait: after a second the CTA gives up, raises the flag and runs to its end without waiting.
 __device__ __forceinline__ void rows_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
@@ -275,30 +293,38 @@ __device__ __forceinline__ bool one_lane() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(x));
   return x != 0;
 }
+// A warp's view of the run's portions.
+struct Feed {
+  RowsSmall& sm;
+  volatile int* gave_up;
+  uint32_t n = 0;
+  __device__ __forceinline__ Feed(RowsSmall& small) : sm(small), gave_up(&small.gave_up) {}
+  __device__ __forceinline__ bool next(Portion& p) {
+    const uint32_t slot = n & 3;
+    rows_wait(&sm.item_full[slot], n >> 2 & 1u, gave_up);
+    p = sm.items[slot];
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&sm.item_empty[slot]));
+    ++n;
+    return p.c1 > p.c0 && !*gave_up;
+  }
+};
+
 __device__ __forceinline__ void mbar_arrive_n(uint32_t addr, uint32_t n) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(addr), "r"(n) : "memory");
 }
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// 32 lanes x 32 consecutive 32-bit columns of tensor memory, asked for and, with tmem_have, there; 32 or 16 columns
-// complete on return; and back.
-__device__ __forceinline__ void tmem_ask32(uint32_t at, float (&v)[32]) {
+// 32 lanes x 32 or 16 consecutive 32-bit columns of tensor memory, complete on return, and back.
+__device__ __forceinline__ void tmem_ld32(uint32_t at, float (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%1"
-      "7,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      "7,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
       : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
         "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
         "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
         "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
       : "r"(at) : "memory");
-}
-template <int NC>
-__device__ __forceinline__ void tmem_have(float (&v)[NC][32]) {
-  tmem_wait_ld();
-#pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[c][i]));  // no use of them before the wait
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&v)[32]) {
   asm volatile(
@@ -366,8 +392,7 @@ __device__ __forceinline__ int64_t offset_of(const RowsArgs& a, const KeyPlace& 
 // The infinities and NaN that were taken out of a block's values, given back to the rows that see them:
 // columns [col, col + N) of the outputs o that a warp's lanes hold a row of each (the same columns).
 template <bool BF, int D, bool TREE, int N>
-__device__ __noinline__ void add_odd(const Item<TREE>& it, const RowView& view, float* o, int col) {
-  const RowsArgs& a = it.a;
+__device__ __noinline__ void add_odd(const RowsArgs& a, const Portion& it, const RowView& view, float* o, int col) {
   for (int v = it.c0; v < it.c1; ++v) {
     if (!some_do_not_see(it.k, v, a.sinks)) continue;
     const int k0 = first_key(it.k, v);
@@ -386,13 +411,13 @@ __device__ __noinline__ void add_odd(const Item<TREE>& it, const RowView& view, 
   }
 }
 template <bool BF, int D, bool TREE, int N>
-__device__ __forceinline__ void give_back(const Item<TREE>& it, const RowView& view, float (&o)[N], int col) {
-  const Item<TREE> here = it;  // copies: what lies in memory for the call
+__device__ __forceinline__ void give_back(const RowsArgs& a, const Portion& it, const RowView& view, float (&o)[N], int col) {
+  const Portion here = it;  // copies: what lies in memory for the call
   const RowView mine = view;
   float y[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) y[i] = o[i];
-  add_odd<BF, D, TREE, N>(here, mine, y, col);
+  add_odd<BF, D, TREE, N>(a, here, mine, y, col);
 #pragma unroll
   for (int i = 0; i < N; ++i) o[i] = y[i];
 }
@@ -448,27 +473,32 @@ struct RowState {
   bool any;  // a chunk came before
 };
 
-// The scores of 32 NC keys from column s_at on become probabilities: one 16-bit number each, the columns packed
-// from p_at on, or (TWO) the rounding and the rest, 16 columns of each in the place of 32 scores.
-template <bool BF, int D, bool TWO, int NC>
-__device__ __forceinline__ void turn(uint32_t s_at, uint32_t p_at, uint32_t o_at, float scale, bool edge, const uint32_t (&see)[NC],
+// The scores of the keys' groups of 32, c0 .. c1 - 1 of a chunk's four, become probabilities: one 16-bit number each,
+// 16 columns a group, or (TWO) the rounding and the rest, 16 columns of each in the place of 32 scores.  Loops over
+// the groups, the scores fetched twice: with all 128 in registers the code was four times as long and its fetching
+// took more time than the second look (prompts 2.94 ms against FIGURE).
+template <bool BF, int D, bool TWO, bool TREE>
+__device__ __forceinline__ void turn(const RowsArgs& a, uint32_t s_at, uint32_t o_at, int c0, int c1, bool edge, const RowView& view, int k0,
                                      bool there, RowState& r, uint64_t* half_bar) {
-  float s[NC][32];
-#pragma unroll
-  for (int c = 0; c < NC; ++c) tmem_ask32(s_at + 32 * c, s[c]);
-  tmem_have(s);
-  if (edge)
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
+  const float scale = a.scale;
+  auto fetch = [&](int c, float (&s)[32]) {
+    tmem_ld32(s_at + 32 * c, s);
+    if (edge) {
+      const uint32_t see = seen32<TREE>(a, view, k0 + 32 * c);
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        if (!(see[c] >> i & 1u)) s[c][i] = -INFINITY;
-  float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (!(see >> i & 1u)) s[i] = -INFINITY;
+    }
+  };
+  float tops[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
+  for (int c = c0; c < c1; ++c) {
+    float s[32];
+    fetch(c, s);
 #pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int i = 0; i < 32; i += 2) tops[(i >> 1) & 3] = max_three(tops[(i >> 1) & 3], s[c][i], s[c][i + 1]);
-  const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * scale;
+    for (int i = 0; i < 32; i += 2) tops[(i >> 1) & 1] = max_three(tops[(i >> 1) & 1], s[i], s[i + 1]);
+  }
+  const float top = fmaxf(tops[0], tops[1]) * scale;
   // lanes without a row hold what happens to lie there
   if (__any_sync(0xffffffffu, there && top > (r.m == -INFINITY ? -INFINITY : r.m + kPrHeadroom))) {
     const float mx = fmaxf(r.m, top), f = r.m == -INFINITY ? 0.0f : pr_ex2(r.m - mx);
@@ -487,60 +517,50 @@ __device__ __forceinline__ void turn(uint32_t s_at, uint32_t p_at, uint32_t o_at
   }
   const float z = kPrShift<BF> - (r.m == -INFINITY ? 0.0f : r.m);
   float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
+#pragma unroll 1
+  for (int c = c0; c < c1; ++c) {
+    float s[32];
+    fetch(c, s);
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
-      fma_two(s[c][i], s[c][i + 1], scale, z);
+      fma_two(s[i], s[i + 1], scale, z);
       if (!TWO && (i & 7) >= 8 - kPrPoly) {
-        exp2_two(s[c][i], s[c][i + 1]);
+        exp2_two(s[i], s[i + 1]);
       } else {
-        s[c][i] = pr_ex2(s[c][i]);
-        s[c][i + 1] = pr_ex2(s[c][i + 1]);
+        s[i] = pr_ex2(s[i]);
+        s[i + 1] = pr_ex2(s[i + 1]);
       }
-      add_two(sum[i & 2], sum[(i & 2) + 1], s[c][i], s[c][i + 1]);
+      add_two(sum[i & 2], sum[(i & 2) + 1], s[i], s[i + 1]);
     }
     if (TWO) {
       uint32_t p[32];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        p[i] = pack2<BF>(s[c][2 * i], s[c][2 * i + 1]);
+        p[i] = pack2<BF>(s[2 * i], s[2 * i + 1]);
         const float2 y = unpack2<BF>(p[i]);
-        p[16 + i] = pack2<BF>(s[c][2 * i] - y.x, s[c][2 * i + 1] - y.y);
+        p[16 + i] = pack2<BF>(s[2 * i] - y.x, s[2 * i + 1] - y.y);
       }
-      tmem_st32(p_at + 32 * c, p);
+      tmem_st32(s_at + 32 * c, p);
     } else {
       uint32_t p[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) p[i] = pack2<BF>(s[c][2 * i], s[c][2 * i + 1]);
-      tmem_st16(p_at + 16 * c, p);
+      for (int i = 0; i < 16; ++i) p[i] = pack2<BF>(s[2 * i], s[2 * i + 1]);
+      tmem_st16(s_at + 16 * c, p);
     }
-    if (NC == 4 && c == 1) {  // the products with the first half of the keys' values may begin
+    if (c == 1 && c1 - c0 == 4) {  // the products with the first half of the keys' values may begin
       tmem_wait_st();
       tc_fence_before_sync();
       __syncwarp();
       if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(half_bar));
     }
   }
-  r.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-}
-// The same for a copy that has the 32 NC keys from 32 c0 on: its other probabilities are 0.
-template <bool BF, int D, int NC>
-__device__ __forceinline__ void turn_part(uint32_t s_at, uint32_t o_at, int c0, float scale, bool edge, const uint32_t (&see)[4],
-                                          bool there, RowState& r) {
-  uint32_t mine[NC];
-#pragma unroll
-  for (int c = 0; c < NC; ++c) mine[c] = see[0];
-#pragma unroll
-  for (int k = 1; k < 4; ++k)
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-      if (c0 + c == k) mine[c] = see[k];
-  turn<BF, D, true, NC>(s_at + 32 * c0, s_at + 32 * c0, o_at, scale, edge, mine, there, r, nullptr);
-  const uint32_t none[32] = {};
+  if (TWO && c1 - c0 < 4) {  // a copy's other keys
+    const uint32_t none[32] = {};
 #pragma unroll 1
-  for (int c = 0; c < 4; ++c)
-    if (c < c0 || c >= c0 + NC) tmem_st32(s_at + 32 * c, none);
+    for (int c = 0; c < 4; ++c)
+      if (c < c0 || c >= c1) tmem_st32(s_at + 32 * c, none);
+  }
+  r.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 // ---- the kernel -------------------------------------------------------------------------------
@@ -548,17 +568,19 @@ __device__ __forceinline__ void turn_part(uint32_t s_at, uint32_t o_at, int c0, 
 template <bool BF, int D, bool TREE>
 __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_constant__ RowsArgs a) {
   using S = RowsShape<D>;
-  using It = Item<TREE>;
   constexpr int NS = S::slots;
   constexpr uint32_t kFormat = (1u << 4) | (BF ? 1u << 7 | 1u << 10 : 0u) | ((uint32_t)(128 >> 4) << 24);
   constexpr uint32_t kScores = kFormat | ((uint32_t)(kPrKeys >> 3) << 17);
   constexpr uint32_t kOutputs = kFormat | ((uint32_t)(D >> 3) << 17) | (1u << 16);  // values: keys across
   constexpr uint32_t kOut = 256;  // tensor memory: 128 columns of scores for each group, then its outputs
-  extern __shared__ unsigned char smem_raw[];
-  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  extern __shared__ __align__(1024) unsigned char smem[];
   RowsSmall& sm = *reinterpret_cast<RowsSmall*>(smem + S::small);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_trigger();
+  if (smem_u32(smem) & 1023u) {  // the swizzles count on it
+    report_bad_rows();
+    return;
+  }
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(smem_u32(&sm.kv_full[i]), 64);
@@ -572,6 +594,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
       mbar_init(smem_u32(&sm.p_half[i]), 4);
       mbar_init(smem_u32(&sm.p_full[i]), 4);
       mbar_init(smem_u32(&sm.o_done[i]), 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(smem_u32(&sm.item_full[i]), 1);
+      mbar_init(smem_u32(&sm.item_empty[i]), kPrThreads / 32 - 1);
     }
     mbar_fence_init();
     sm.gave_up = sm.odd = 0;
@@ -658,8 +684,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
   tc_fence_after_sync();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sm.tmem);
   const RunStart run = sm.run;
-  It it(a, run);
   volatile int* gave_up = &sm.gave_up;
+  Feed feed(sm);
+  Portion it;
 
   if (warp >= kPrLoad) {
     // Keys and values: chunk after chunk a slot of keys, then one of values, 64 rows a warp.
@@ -697,7 +724,32 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
     auto empty = [&](uint32_t f) {
       if (f >= NS) rows_wait(&sm.kv_empty[f % NS], (f / NS - 1) & 1u, gave_up);
     };
-    if (it.begin()) {
+    // The first of the two warps finds the run's portions for all.
+    Walk<TREE> walk(a, run);
+    SharedItem over = {};
+    uint32_t found = 0;
+    auto next_portion = [&](bool begin) -> bool {
+      if (w) return feed.next(it);
+      const bool more = begin ? walk.begin() : walk.next();
+      if (!more) walk.p.c0 = walk.p.c1 = 0;
+      it = walk.p;
+      if (it.c0 == 0 && it.c1 > 0 && it.c1 < it.k.chunks) {
+        // begins in this run and goes on behind it: what the joining kernel needs to know
+        const int64_t end = walk.at + kPrItemUnits + it.k.chunks - 1;  // the unit of its last chunk
+        over = SharedItem{1, it.b, it.rb, it.g, 2 * (int)blockIdx.x + (it.first ? 0 : 1),
+                          (int)(((end + 1) * run.ctas - 1) / run.total), {0, 0}};
+      }
+      const uint32_t slot = found & 3;
+      if (found >= 4) rows_wait(&sm.item_empty[slot], ((found >> 2) - 1) & 1u, gave_up);
+      __syncwarp();
+      if (lane == 0) {
+        sm.items[slot] = it;
+        mbar_arrive(smem_u32(&sm.item_full[slot]));
+      }
+      ++found;
+      return more;
+    };
+    if (next_portion(true)) {
       const int64_t v_from_k = a.c.v - a.c.k;
       Asked next = ask(it.c0);
       for (int v = it.c0;; fill += 2) {
@@ -706,7 +758,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
         const Asked x = next;
         bool more = true;
         if (++v == it.c1) {
-          more = it.next();
+          more = next_portion(false);
           v = it.c0;
         }
         if (more) next = ask(v);
@@ -755,6 +807,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
         if (!more) break;
       }
     }
+    if (w == 0 && lane == 0) a.shared[blockIdx.x] = over;
     cp_async_wait<0>();
   } else if (warp == kPrQuery) {
     // Queries: rows that there are, 128 of a tile; the others' scores are never looked at.  Then, once they have
@@ -764,8 +817,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
     const int piece = lane % P, sub = lane / P;
     uint32_t n[2] = {0, 0}, fill = 0;
     uint32_t turns = 0;  // how often each slot's landing came around, a bit per slot
-    for (bool more = it.begin(); more; more = it.next()) {
-      const int all = it.rows(), fold = it.fold();
+    while (feed.next(it)) {
+      const int all = it.rows, fold = it.fold();
       for (int w = 0; w < (all > 128 ? 2 : 1); ++w) {
         if (n[w] > 0) rows_wait(&sm.q_empty[w], (n[w] - 1) & 1u, gave_up);
         ++n[w];
@@ -872,9 +925,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
       tc_fence_after_sync();
       __syncwarp();
     };
-    for (bool more = it.begin(); more; more = it.next()) {
+    while (feed.next(it)) {
       const int m = it.c1 - it.c0;
-      const bool pair = it.rows() > 128;
+      const bool pair = it.rows > 128;
       for (int w = 0; w < (pair ? 2 : 1); ++w) rows_wait(&sm.q_full[w], items[w]++ & 1u, gave_up);
       tc_fence_after_sync();
       __syncwarp();
@@ -944,8 +997,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
     const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
     const uint32_t s_at = tmem + lanes + w * 128, o_at = tmem + lanes + kOut + w * 128;
     uint32_t chunk_count = 0, item_count = 0;
-    for (bool more = it.begin(); more; more = it.next()) {
-      const bool pair = it.rows() > 128;
+    while (feed.next(it)) {
+      const bool pair = it.rows > 128;
       const int fold = it.fold(), size = 128 >> fold, copy = r >> (7 - fold);
       const int row = it.rb * kPrRows + (pair ? w * 128 : 0) + (r & (size - 1)), rows = it.s.tokens * a.rep;
       const bool there = row < rows, warp_there = row - lane < rows;
@@ -987,17 +1040,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
         if (warp_there) {
           const int k0 = first_key(it.k, v);
           const bool edge = k0 + kPrKeys > it.k.full || (k0 < it.k.low_full && k0 + kPrKeys > a.sinks);
-          uint32_t see[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) see[c] = edge ? seen32<TREE>(a, view, k0 + 32 * c) : 0xffffffffu;
           if (pair)
-            turn<BF, D, false, 4>(s_at, s_at, o_at, a.scale, edge, see, there, state, &sm.p_half[w]);
-          else if (fold == 0)
-            turn<BF, D, true, 4>(s_at, s_at, o_at, a.scale, edge, see, there, state, &sm.p_half[w]);
-          else if (fold == 1)
-            turn_part<BF, D, 2>(s_at, o_at, 2 * copy, a.scale, edge, see, there, state);
+            turn<BF, D, false, TREE>(a, s_at, o_at, 0, 4, edge, view, k0, there, state, &sm.p_half[w]);
           else
-            turn_part<BF, D, 1>(s_at, o_at, copy, a.scale, edge, see, there, state);
+            turn<BF, D, true, TREE>(a, s_at, o_at, copy * (4 >> fold), (copy + 1) * (4 >> fold), edge, view, k0, there, state, &sm.p_half[w]);
           tmem_wait_st();
         }
         state.any = true;
@@ -1015,12 +1061,13 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
         ++item_count;
         tc_fence_after_sync();
       }
+      if (!pair && it.c1 - it.c0 > 1) named_barrier_sync(1, 256);  // the other group's values have been looked through, too
       const bool whole = it.whole(), odd = *(volatile int*)&sm.odd;
       const int64_t part = (int64_t)(2 * blockIdx.x + (it.first ? 0 : 1)) * a.part_rows + (row - it.rb * kPrRows);
       uint16_t* const to = a.out + (it.s.r0 + (int64_t)t) * a.ldo + (int64_t)(it.g * a.rep + row - t * a.rep) * D;
       auto store = [&](auto& o, int c, float l) {  // columns from c on
         constexpr int N = sizeof(o) / sizeof(float);
-        if (odd) give_back<BF, D, TREE, N>(it, view, o, c);
+        if (odd) give_back<BF, D, TREE, N>(a, it, view, o, c);
         if (!there) return;
         if (whole) {
           const float inv = 1.0f / l;
@@ -1050,8 +1097,65 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
         }
       } else {
         const bool two = it.c1 - it.c0 > 1;  // both groups have chunks
-        if (w == 0 || two) {
-          float* const meet = reinterpret_cast<float*>(smem + S::tile);
+        float* const meet = reinterpret_cast<float*>(smem + S::tile);
+        if (fold) {
+          // The groups' and copies' parts of each row: as many columns at a time as `meet` has room for, then all
+          // threads add up four columns of a row at a time.
+          const int rows_here = it.rows, parts = (two ? 2 : 1) << fold, mine = (w << fold) + copy;
+          const int wide = rows_here <= 8 ? 7 : rows_here <= 16 ? 6 : 5, cols = min(D, 1 << wide);  // 8 parts x rows x cols <= 8192
+          const int lr = r & (size - 1);
+          if (state.any && there) sm.ml[(mine * size + lr) & 255] = make_float2(state.m, state.l);
+#pragma unroll 1
+          for (int c0 = 0; c0 < D; c0 += cols) {
+            if (state.any && warp_there)
+#pragma unroll 1
+              for (int c = 0; c < cols; c += 32) {
+                uint32_t x[32];
+                float o[32];
+                tmem_ld32(o_at + c0 + c, x);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(x[i]);
+                if (odd && mine == 0) give_back<BF, D, TREE, 32>(a, it, view, o, c0 + c);
+                if (there)
+#pragma unroll
+                  for (int i = 0; i < 32; i += 4)  // turned by the row against bank conflicts
+                    *reinterpret_cast<float4*>(meet + (mine * rows_here + lr) * cols + ((c + i) ^ ((lr & 7) << 2))) =
+                        make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+              }
+            named_barrier_sync(1, 256);
+#pragma unroll 1
+            for (int e = tid * 4; e < rows_here * cols; e += 256 * 4) {
+              const int rr = e / cols, c = e - rr * cols;
+              float mx = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+              for (int k = 0; k < parts; ++k) mx = fmaxf(mx, sm.ml[k * size + rr].x);
+#pragma unroll 4
+              for (int k = 0; k < parts; ++k) {
+                const float2 ml = sm.ml[k * size + rr];
+                const float f = ml.x == -INFINITY ? 0.0f : pr_ex2(ml.x - mx);
+                if (f != 0.0f || odd) {
+                  const float4 y = *reinterpret_cast<const float4*>(meet + (k * rows_here + rr) * cols + (c ^ ((rr & 7) << 2)));
+                  l = fmaf(ml.y, f, l);
+                  o[0] = fmaf(y.x, f, o[0]);
+                  o[1] = fmaf(y.y, f, o[1]);
+                  o[2] = fmaf(y.z, f, o[2]);
+                  o[3] = fmaf(y.w, f, o[3]);
+                }
+              }
+              if (whole) {
+                const int rt = (uint32_t)(it.rb * kPrRows + rr) / a.rep_div, head = it.g * a.rep + it.rb * kPrRows + rr - rt * a.rep;
+                const float inv = 1.0f / l;
+                *reinterpret_cast<uint2*>(a.out + (it.s.r0 + (int64_t)rt) * a.ldo + (int64_t)head * D + c0 + c) =
+                    make_uint2(pack2<BF>(o[0] * inv, o[1] * inv), pack2<BF>(o[2] * inv, o[3] * inv));
+              } else {
+                const int64_t at = (int64_t)(2 * blockIdx.x + (it.first ? 0 : 1)) * a.part_rows + rr;
+                *reinterpret_cast<float4*>(a.part + at * D + c0 + c) = make_float4(o[0], o[1], o[2], o[3]);
+                if (c0 + c == 0) a.part_ml[at] = make_float2(mx, l);
+              }
+            }
+            named_barrier_sync(1, 256);  // before the columns are written again
+          }
+        } else if (w == 0 || two) {
           auto place = [&](int row, int c) {  // of four columns, turned by the row against bank conflicts
             return reinterpret_cast<float4*>(meet + row * 64 + (((c >> 2) ^ (row & 15)) << 2));
           };
@@ -1074,16 +1178,13 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
             }
             if (two) named_barrier_sync(1, 256);
             if (w == 0) {
-              if (half == 0) {
-                if (two) {
-                  const float2 ml = sm.ml[r];
-                  const float mx = fmaxf(state.m, ml.x);
-                  f0 = state.m == -INFINITY ? 0.0f : pr_ex2(state.m - mx);
-                  f1 = ml.x == -INFINITY ? 0.0f : pr_ex2(ml.x - mx);
-                  state.m = mx;
-                  state.l = state.l * f0 + ml.y * f1;
-                }
-                sm.ml[r] = make_float2(state.m, state.l);
+              if (half == 0 && two) {
+                const float2 ml = sm.ml[r];
+                const float mx = fmaxf(state.m, ml.x);
+                f0 = state.m == -INFINITY ? 0.0f : pr_ex2(state.m - mx);
+                f1 = ml.x == -INFINITY ? 0.0f : pr_ex2(ml.x - mx);
+                state.m = mx;
+                state.l = state.l * f0 + ml.y * f1;
               }
               if (warp_there)
 #pragma unroll 1
@@ -1102,67 +1203,17 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
                       o[i + 2] = fmaf(o[i + 2], f0, y.z * f1);
                       o[i + 3] = fmaf(o[i + 3], f0, y.w * f1);
                     }
-                  if (fold == 0) {
-                    store(o, half + c, state.l);
-                  } else if (there) {
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4) *place(r, c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                  }
+                  store(o, half + c, state.l);
                 }
-              if (fold) {
-                // the copies: a thread has some of its row's columns, of all copies
-                named_barrier_sync(2, 128);
-                const int lr = r & (size - 1);
-                float mx = -INFINITY, l = 0.0f, f[4];
-                for (int k = 0; k < 1 << fold; ++k) mx = fmaxf(mx, sm.ml[lr + k * size].x);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const float2 ml = sm.ml[(lr + k * size) & 127];
-                  f[k] = k >= 1 << fold || ml.x == -INFINITY ? 0.0f : pr_ex2(ml.x - mx);
-                  l = fmaf(ml.y, f[k], l);
-                }
-#pragma unroll 1
-                for (int c = copy * (64 >> fold); c < (copy + 1) * (64 >> fold); c += 16) {
-                  float o[16] = {};
-                  if (there)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                      if (f[k] != 0.0f)
-#pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                          const float4 y = *place(lr + k * size, c + i);
-                          o[i] = fmaf(y.x, f[k], o[i]);
-                          o[i + 1] = fmaf(y.y, f[k], o[i + 1]);
-                          o[i + 2] = fmaf(y.z, f[k], o[i + 2]);
-                          o[i + 3] = fmaf(y.w, f[k], o[i + 3]);
-                        }
-                  store(o, half + c, l);
-                }
-                if (!whole && there && half == 0 && copy == 0) a.part_ml[part] = make_float2(mx, l);
-                if (half + 64 < D || !two) named_barrier_sync(2, 128);  // before the columns are written again
-              } else if (!whole && there && half == 0) {
-                a.part_ml[part] = make_float2(state.m, state.l);
-              }
+              if (!whole && there && half == 0) a.part_ml[part] = make_float2(state.m, state.l);
             }
-            if (two) named_barrier_sync(1, 256);
+            if (two) named_barrier_sync(1, 256);  // before the columns are written again
           }
         }
       }
     }
   }
 
-  // what the joining kernel needs of this run: the item that begins in it and goes on behind it
-  if (tid == 0) {
-    SharedItem x = {};
-    It last(a, run);
-    for (bool more = last.begin(); more; more = last.next())
-      if (last.c0 == 0 && last.c1 < last.k.chunks) {
-        const int64_t end = last.at + kPrItemUnits + last.k.chunks - 1;  // the unit of its last chunk
-        x = SharedItem{1, last.b, last.rb, last.g, 2 * (int)blockIdx.x + (last.first ? 0 : 1),
-                       (int)(((end + 1) * run.ctas - 1) / run.total), {0, 0}};
-      }
-    a.shared[blockIdx.x] = x;
-  }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
