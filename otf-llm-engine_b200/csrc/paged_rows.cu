@@ -57,9 +57,10 @@ struct __align__(16) SharedItem {
 };
 
 struct RowsArgs {
-  CUtensorMap kmap, vmap;  // boxes of 64 dims of `box` tokens of a page, as the ring holds them
+  // Boxes of 64 dims of `box` tokens of a page, as the ring holds them, and of `rest` tokens for what is left of it.
+  CUtensorMap kmap, vmap, kmap_rest, vmap_rest;
   CUtensorMap qmap;        // boxes of 64 dims of 32 rows: a KV head's query heads of some tokens
-  int box, q_box;          // 0: no tensor copies; tokens of a box
+  int box, rest, q_box;    // box, q_box: 0 for no tensor copies
   PagedView c;
   FastDiv page, rep_div;
   const uint16_t* q;
@@ -433,38 +434,27 @@ __device__ __forceinline__ void add_two(float& x, float& y, float u, float v) {
   asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
       "add.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(x), "+f"(y) : "f"(u), "f"(v));
 }
-// p = p f + c.
-__device__ __forceinline__ void fma_by(float& px, float& py, float fx, float fy, float c) {
-  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tmov.b64 c, {%4, %4};\n\t"
-      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(px), "+f"(py) : "f"(fx), "f"(fy), "f"(c));
-}
 __device__ __forceinline__ float max_three(float x, float y, float z) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
   return r;
 }
 
-// 2^x of two numbers without the exponential unit: x = n + f with n whole and |f| <= 1/2, a polynomial of degree 4
-// for 2^f (least relative error with 1 at f = 0, 2^-18.4, by linear programming), n added to its exponent.  0 from
-// -127 down, where the exponent's bits run out.  The unit makes 16 a cycle on an SM, so 128 x 128 scores take as long as their two products; some of
-// them go this way (kPrPoly of each 8).
-constexpr int kPrPoly = 2;
-__device__ __forceinline__ void exp2_two(float& x, float& y) {
-  constexpr float big = 12582912.0f;  // 1.5 2^23: its sum's last bits are n
-  x = fmaxf(x, -127.0f);
-  y = fmaxf(y, -127.0f);
-  float nx = x, ny = y, px = 0.009582576341927052f, py = px;
-  add_two(nx, ny, big, big);
-  float fx = nx, fy = ny;
-  add_two(fx, fy, -big, -big);
-  fma_two(fx, fy, -1.0f, 0.0f);
-  add_two(fx, fy, x, y);
-  fma_by(px, py, fx, fy, 0.05590682849287987f);
-  fma_by(px, py, fx, fy, 0.24024106562137604f);
-  fma_by(px, py, fx, fy, 0.6931241154670715f);
-  fma_by(px, py, fx, fy, 1.0f);
-  x = __int_as_float(__float_as_int(px) + (__float_as_int(nx) << 23));
-  y = __int_as_float(__float_as_int(py) + (__float_as_int(ny) << 23));
+// 4 x 4 16-byte pieces across four lanes: lane q's piece i becomes lane i's piece q.
+__device__ __forceinline__ void turn_pieces(uint32_t (&x)[4][4]) {
+#pragma unroll
+  for (int step = 1; step <= 2; step <<= 1) {
+    const bool upper = threadIdx.x & step;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (!(i & step))
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? x[i][k] : x[i + step][k], step);
+          if (upper) x[i][k] = got;
+          else x[i + step][k] = got;
+        }
+  }
 }
 
 // A row's state.
@@ -477,13 +467,13 @@ struct RowState {
 // 16 columns a group, or (TWO) the rounding and the rest, 16 columns of each in the place of 32 scores.  Loops over
 // the groups, the scores fetched twice: with all 128 in registers the code was four times as long and its fetching
 // took more time than the second look (prompts 2.94 ms against FIGURE).
-template <bool BF, int D, bool TWO, bool TREE>
-__device__ __forceinline__ void turn(const RowsArgs& a, uint32_t s_at, uint32_t o_at, int c0, int c1, bool edge, const RowView& view, int k0,
+template <bool BF, int D, bool TWO, bool TREE, bool EDGE>
+__device__ __forceinline__ void turn_chunk(const RowsArgs& a, uint32_t s_at, uint32_t o_at, int c0, int c1, const RowView& view, int k0,
                                      bool there, RowState& r, uint64_t* half_bar) {
   const float scale = a.scale;
   auto fetch = [&](int c, float (&s)[32]) {
     tmem_ld32(s_at + 32 * c, s);
-    if (edge) {
+    if (EDGE) {
       const uint32_t see = seen32<TREE>(a, view, k0 + 32 * c);
 #pragma unroll
       for (int i = 0; i < 32; ++i)
@@ -524,12 +514,8 @@ __device__ __forceinline__ void turn(const RowsArgs& a, uint32_t s_at, uint32_t 
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
       fma_two(s[i], s[i + 1], scale, z);
-      if (!TWO && (i & 7) >= 8 - kPrPoly) {
-        exp2_two(s[i], s[i + 1]);
-      } else {
-        s[i] = pr_ex2(s[i]);
-        s[i + 1] = pr_ex2(s[i + 1]);
-      }
+      s[i] = pr_ex2(s[i]);
+      s[i + 1] = pr_ex2(s[i + 1]);
       add_two(sum[i & 2], sum[(i & 2) + 1], s[i], s[i + 1]);
     }
     if (TWO) {
@@ -561,6 +547,15 @@ __device__ __forceinline__ void turn(const RowsArgs& a, uint32_t s_at, uint32_t 
       if (c < c0 || c >= c1) tmem_st32(s_at + 32 * c, none);
   }
   r.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
+template <bool BF, int D, bool TWO, bool TREE>
+__device__ __forceinline__ void turn(const RowsArgs& a, uint32_t s_at, uint32_t o_at, int c0, int c1, bool edge, const RowView& view, int k0,
+                                     bool there, RowState& r, uint64_t* half_bar) {
+  if (edge)
+    turn_chunk<BF, D, TWO, TREE, true>(a, s_at, o_at, c0, c1, view, k0, there, r, half_bar);
+  else
+    turn_chunk<BF, D, TWO, TREE, false>(a, s_at, o_at, c0, c1, view, k0, there, r, half_bar);
 }
 
 // ---- the kernel -------------------------------------------------------------------------------
@@ -695,9 +690,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
     const uint32_t ring = smem_u32(smem + S::ring);
     const uint32_t to = (uint32_t)((piece >> 3) * 128 * 128 + (64 * w + sub) * 128);
     uint32_t fill = 0;
-    constexpr int H = D / 64;  // boxes that a group of tokens takes
     // What a chunk's copies need to know, asked for a chunk ahead: of two of the warp's keys, 32 apart, or where all
-    // keys are there and tensor copies are open, of a lane's two boxes.
+    // keys are there and tensor copies are open, of the first key in a lane's page (one page a lane).
     struct Asked {
       KeyPlace key[2];
       bool boxes;
@@ -707,11 +701,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
       Asked x;
       x.boxes = a.box && k0 + kPrKeys <= it.k.end && (k0 >= it.k.low || k0 + kPrKeys <= a.sinks);
       if (x.boxes) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int s = (lane + 32 * h) / H * a.box;
-          x.key[h] = ask_key(a, it.b, k0 + s, s < kPrKeys);
-        }
+        const int s = max(k0, (int)((uint32_t)k0 / a.page + lane) * (int)a.page.d);
+        x.key[0] = ask_key(a, it.b, s, s < k0 + kPrKeys);
       } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -773,17 +764,28 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
             mbar_arrive_n(bar, 63);
           }
           __syncwarp();
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (x.key[h].there) {
-              int page = x.key[h].page;
-              if (page < 0 || page >= a.c.n_pages) {
-                report_bad_rows();
-                page = a.c.n_pages;  // reads as zeros
-              }
-              tma_load_4d(ring + slot * S::tile + lane % H * (128 * 128) + (lane + 32 * h) / H * a.box * 128, w ? &a.vmap : &a.kmap,
-                          lane % H * 64, g, x.key[h].rest, page, bar);
+          if (x.key[0].there) {
+            int page = x.key[0].page, from = x.key[0].rest;
+            if (page < 0 || page >= a.c.n_pages) {
+              report_bad_rows();
+              page = a.c.n_pages;  // reads as zeros
             }
+            // the first lane's page may have begun before the chunk, the last one's may go on behind it
+            const int first = __shfl_sync(__activemask(), from, 0), d = (int)a.page.d;
+            int row = lane ? lane * d - first : 0;
+            const int end = min(kPrKeys, (lane + 1) * d - first);
+            uint32_t dst = ring + slot * S::tile + row * 128;
+            while (row < end) {
+              const bool big = end - row >= a.box;
+              const CUtensorMap* map = w ? (big ? &a.vmap : &a.vmap_rest) : (big ? &a.kmap : &a.kmap_rest);
+#pragma unroll
+              for (int h = 0; h < D / 64; ++h) tma_load_4d(dst + h * (128 * 128), map, h * 64, g, from, page, bar);
+              const int n = big ? a.box : a.rest;
+              row += n;
+              from += n;
+              dst += n * 128;
+            }
+          }
         } else {
           empty(fill);
           empty(fill + 1);
@@ -792,7 +794,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int64_t mine = offset_of(a, x.key[h]);
-#pragma unroll
+#pragma unroll 4
             for (int i = 0; i < 32 / R; ++i) {
               const int64_t at = __shfl_sync(0xffffffffu, mine, sub + i * R);
               const uint16_t* y = base + (at >= 0 ? at : 0);  // an address, not read where there is no key
@@ -1065,21 +1067,37 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
       const bool whole = it.whole(), odd = *(volatile int*)&sm.odd;
       const int64_t part = (int64_t)(2 * blockIdx.x + (it.first ? 0 : 1)) * a.part_rows + (row - it.rb * kPrRows);
       uint16_t* const to = a.out + (it.s.r0 + (int64_t)t) * a.ldo + (int64_t)(it.g * a.rep + row - t * a.rep) * D;
-      auto store = [&](auto& o, int c, float l) {  // columns from c on
-        constexpr int N = sizeof(o) / sizeof(float);
-        if (odd) give_back<BF, D, TREE, N>(a, it, view, o, c);
-        if (!there) return;
+      // Columns [c, c + 32) of the warp's rows.  Four lanes turn their rows' 16-byte pieces, so that they write 64 bytes of
+      // one row together.
+      auto store = [&](float (&o)[32], int c, float l) {
+        if (odd) give_back<BF, D, TREE, 32>(a, it, view, o, c);
         if (whole) {
           const float inv = 1.0f / l;
+          uint32_t x[4][4];
 #pragma unroll
-          for (int i = 0; i < N; i += 8)
-            *reinterpret_cast<uint4*>(to + c + i) =
-                make_uint4(pack2<BF>(o[i] * inv, o[i + 1] * inv), pack2<BF>(o[i + 2] * inv, o[i + 3] * inv),
-                           pack2<BF>(o[i + 4] * inv, o[i + 5] * inv), pack2<BF>(o[i + 6] * inv, o[i + 7] * inv));
+          for (int i = 0; i < 16; ++i) x[i >> 2][i & 3] = pack2<BF>(o[2 * i] * inv, o[2 * i + 1] * inv);
+          turn_pieces(x);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int from = (lane & 28) + i;
+            uint16_t* y = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, (unsigned long long)to, from)) + c + (lane & 3) * 8;
+            if (row - lane + from < rows) *reinterpret_cast<uint4*>(y) = make_uint4(x[i][0], x[i][1], x[i][2], x[i][3]);
+          }
         } else {
 #pragma unroll
-          for (int i = 0; i < N; i += 4)
-            *reinterpret_cast<float4*>(a.part + part * D + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          for (int h = 0; h < 2; ++h) {
+            uint32_t x[4][4];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i >> 2][i & 3] = __float_as_uint(o[16 * h + i]);
+            turn_pieces(x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int from = (lane & 28) + i;
+              if (row - lane + from < rows)
+                *reinterpret_cast<uint4*>(a.part + (part - lane + from) * D + c + 16 * h + (lane & 3) * 4) =
+                    make_uint4(x[i][0], x[i][1], x[i][2], x[i][3]);
+            }
+          }
         }
       };
       if (pair) {
@@ -1352,16 +1370,23 @@ extern "C" OTF_API int otf_paged_attn_rows(const otf_paged_cache* cache, const v
   // a masked -inf stays one under a scale of 0, and no finite score counts under 2^-149
   a.scale = fmaxf(fabsf(scale * otf::kPrLog2e), 0x1p-149f);
   a.sign = scale < 0.0f ? 0x80008000u : 0u;
-  // Tensor copies where groups of 4 tokens or more lie in one page; else, and for the chunks that are not all there,
-  // 16-byte copies.
-  const int box = std::gcd((int)a.c.page_size, otf::kPrKeys);
-  if (box >= 4) {
+  // Tensor copies where chunks cut pages into groups of 4 tokens or more (`rest`), in larger boxes as far as they go:
+  // a box costs the copy unit some 40 cycles whatever is in it (pages of 20: 128 boxes of 4 a chunk 5500 cycles, with boxes
+  // of 16 FIGURE).  Else, and for the chunks that are not all there, 16-byte copies.
+  const int rest = std::gcd((int)a.c.page_size, otf::kPrKeys);
+  if (rest >= 4) {
+    int box = rest;
+    while (rest < 16 && box * 2 <= std::min(16, a.c.page_size)) box *= 2;
     const uint64_t dims[4] = {(uint64_t)D, (uint64_t)a.c.kv_heads, (uint64_t)a.c.page_size, (uint64_t)a.c.n_pages};
     const uint64_t strides[3] = {(uint64_t)a.c.head_stride * 2, (uint64_t)a.c.token_stride * 2, (uint64_t)a.c.page_stride * 2};
-    const uint32_t boxes[4] = {64, 1, (uint32_t)box, 1};
+    const uint32_t boxes[4] = {64, 1, (uint32_t)box, 1}, rests[4] = {64, 1, (uint32_t)rest, 1};
     if (otf::encode_tiled_4d_swizzled(&a.kmap, a.c.k, dims, strides, boxes) &&
-        otf::encode_tiled_4d_swizzled(&a.vmap, a.c.v, dims, strides, boxes))
+        otf::encode_tiled_4d_swizzled(&a.vmap, a.c.v, dims, strides, boxes) &&
+        (rest == box || (otf::encode_tiled_4d_swizzled(&a.kmap_rest, a.c.k, dims, strides, rests) &&
+                         otf::encode_tiled_4d_swizzled(&a.vmap_rest, a.c.v, dims, strides, rests)))) {
       a.box = box;
+      a.rest = rest;
+    }
   }
   if (a.rep <= 32 && 32 % a.rep == 0 && !a.sign) {
     const uint64_t dims[4] = {(uint64_t)D, (uint64_t)heads, (uint64_t)n, 1};
