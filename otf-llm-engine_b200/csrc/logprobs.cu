@@ -5,8 +5,10 @@
 // m + log1p(l), a token's log probability is d - log1p(l), and the entropy log1p(l) - t / (1 + l), two terms
 // that are not negative: both keep their relative precision where one token has nearly all of the weight.
 // Parts join as l = l_a + (1 + l_b) f, t = t_a + f (t_b + (1 + l_b) (m_b - m_a)) with f = e^(m_b - m_a), m_b <= m_a.
-// The likeliest tokens are kept as a sorted list of 32 in a warp's lanes, value before index, which takes
-// few insertions once it is full.
+// The likeliest tokens are kept as a sorted list of 32 in a warp's lanes, value before index.  What may belong to
+// them gathers in a buffer of 32 that is sorted into the list when it is full; a bar that the warps share (each one's
+// last listed value, and at first the top-th largest of its lanes' first maxima) keeps all but a few hundred
+// entries of a row out.
 //
 // Bound: the logits are read once.  A row is cut among the warps of a cluster of CTAs (one CTA where there
 // are enough rows), 512 logits at a time, 16 in each lane; their parts meet in the cluster's first CTA.
@@ -14,6 +16,7 @@
 #include <cfloat>
 
 #include "paged.cuh"
+#include "pairs.cuh"
 
 namespace otf {
 
@@ -138,14 +141,70 @@ __device__ __forceinline__ void lp_load(const void* row, int i0, int vocab, bool
     }
   }
 }
-// The largest float below x (x itself for -inf and NaN).
+// The largest float below x, the smallest above it (x itself for infinities and NaN).
 __device__ __forceinline__ float lp_below(float x) { return x > -INFINITY ? nextafterf(x, -INFINITY) : x; }
+__device__ __forceinline__ float lp_above(float x) { return x < INFINITY ? nextafterf(x, INFINITY) : x; }
+// 1 where x > y, else 0.
+__device__ __forceinline__ float lp_greater(float x, float y) {
+  float r;
+  asm("set.gt.f32.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float lp_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 32 values over the lanes, the largest first.
+__device__ __forceinline__ float lp_sort_values(float x) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int n = 2; n <= 32; n <<= 1)
+#pragma unroll
+    for (int o = n / 2; o > 0; o >>= 1) {
+      const float y = __shfl_xor_sync(0xffffffffu, x, o);
+      x = (!(lane & o) == !(lane & n)) ? fmaxf(x, y) : fminf(x, y);
+    }
+  return x;
+}
+
+// A warp's list of the likeliest, and what may belong to it.
+struct LpList {
+  unsigned long long best;     // the lane's entry of the sorted list
+  unsigned long long* buffer;  // [32]
+  uint32_t* bar;               // the row's, as the upper half of a key: an entry below it is not among the likeliest
+  int held, top;
+  float least;                 // entries below it need not be looked at
+
+  // The buffer into the list.
+  __device__ __forceinline__ void sort_in() {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+    best = lp_both(best, lp_sort(lane < held ? buffer[lane] : 0ull));
+    held = 0;
+    raise();
+    __syncwarp();
+  }
+  // Later entries of the warp have higher indexes: those as large as the list's last one come behind it.
+  __device__ __forceinline__ void raise() {
+    const unsigned long long last = __shfl_sync(0xffffffffu, best, top - 1);
+    if (last) {
+      least = fmaxf(least, lp_above(lp_value(last)));
+      if ((threadIdx.x & 31) == 0) atomicMax(bar, (uint32_t)(last >> 32));
+    }
+  }
+};
 
 template <int T, bool TOP>
 __global__ void __launch_bounds__(kLpThreads, 4) k_token_logprobs(LogprobArgs a, int ctas) {
   __shared__ LpPart s_part[kLpWarps], s_cta[kLpCluster];
   __shared__ unsigned long long s_list[TOP ? kLpWarps : 1][32], s_cta_list[TOP ? kLpCluster : 1][32];
+  __shared__ uint32_t s_bar;
   pdl_trigger();
+  if (TOP) {
+    if (threadIdx.x == 0) s_bar = 0;
+    __syncthreads();
+  }
   pdl_wait();
   if (ctas > 1) cluster_arrive_relaxed();
   const int row = blockIdx.x / ctas, rank = blockIdx.x - row * ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -160,9 +219,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_token_logprobs(LogprobArgs a,
   }
   const float mine_below = lp_below(mine);
   float m = -INFINITY, l = 0.0f, t = 0.0f;  // m of the warp, l and t of the lane
-  int before = 0;
-  unsigned long long list = 0;
-  float least = -INFINITY;  // of the list's first `top`, once it is full
+  float ahead[2] = {0.0f, 0.0f};  // entries before the token, whole numbers below 2^24 in a lane
+  LpList list = {0ull, s_list[TOP ? warp : 0], &s_bar, 0, a.top, -FLT_MAX};  // an entry of -inf is none
   for (int64_t g = (int64_t)(rank * kLpWarps + warp) * kLpGroup; g < a.vocab; g += (int64_t)ctas * kLpWarps * kLpGroup) {
     const int i0 = (int)g;
     float v[16];
@@ -179,37 +237,61 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_token_logprobs(LogprobArgs a,
     if (token >= i0 + kLpGroup || token < i0) {
       const float than = token >= i0 ? mine_below : mine;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) before += v[j] > than;
+      for (int j = 0; j < 16; j += 2) add_two(ahead[0], ahead[1], lp_greater(v[j], than), lp_greater(v[j + 1], than));
       if (token >= i0 && mine == -INFINITY)  // all of them, NaN too
 #pragma unroll
-        for (int j = 0; j < 16; ++j) before += !(v[j] > -INFINITY);
+        for (int j = 0; j < 16; ++j) ahead[0] += !(v[j] > -INFINITY);
     } else {
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const int i = i0 + lp_index<T>(j);
-        before += v[j] > mine || (i < token && !(v[j] < mine) && (v[j] == mine || mine == -INFINITY));
+        ahead[0] += v[j] > mine || (i < token && !(v[j] < mine) && (v[j] == mine || mine == -INFINITY));
       }
     }
-    if (TOP && __any_sync(0xffffffffu, top > least)) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        uint32_t in = __ballot_sync(0xffffffffu, v[j] > least);
-        if (__popc(in) > 4) {
-          list = lp_both(list, lp_sort(v[j] > least ? lp_key(v[j], i0 + lp_index<T>(j)) : 0ull));
-        } else {
-          for (; in; in &= in - 1) {
-            const unsigned long long k = __shfl_sync(0xffffffffu, lp_key(v[j], i0 + lp_index<T>(j)), __ffs((int)in) - 1);
-            const unsigned long long up = __shfl_up_sync(0xffffffffu, list, 1);
-            const int pos = __popc(__ballot_sync(0xffffffffu, list > k));
-            list = lane < pos ? list : lane == pos ? k : up;
+    if (TOP) {
+      const uint32_t bar = *(volatile uint32_t*)&s_bar;
+      if (bar) list.least = fmaxf(list.least, lp_value((unsigned long long)bar << 32));
+      if (__any_sync(0xffffffffu, top >= list.least)) {
+        if (list.least == -FLT_MAX) {
+          // nothing known yet: a.top lanes have an entry that is their a.top-th largest maximum at least
+          const float first = __shfl_sync(0xffffffffu, lp_sort_values(top == top ? top : -INFINITY), a.top - 1);
+          if (first > -INFINITY) {
+            list.least = first;
+            if (lane == 0) atomicMax(&s_bar, (uint32_t)(lp_key(first, 0) >> 32));
           }
         }
-        // entries of one group come in no order, so equal ones may still pass
-        const unsigned long long last = __shfl_sync(0xffffffffu, list, a.top - 1);
-        if (last) least = lp_below(lp_value(last));
+        const float limit = list.least;  // sorting in may raise it before the entries counted here are taken
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) n += v[j] >= limit;
+        int at = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, at, o);
+          if (lane >= o) at += y;
+        }
+        const int all = __shfl_sync(0xffffffffu, at, 31);
+        if (all <= 32) {
+          if (list.held + all > 32) list.sort_in();
+          at += list.held - n;
+          if (n)
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (v[j] >= limit) list.buffer[at++] = lp_key(v[j], i0 + lp_index<T>(j));
+          list.held += all;
+        } else {
+          if (list.held) list.sort_in();
+#pragma unroll 1
+          for (int j = 0; j < 16; ++j) {
+            float x = v[0];
+#pragma unroll
+            for (int k = 1; k < 16; ++k) x = j == k ? v[k] : x;
+            if (__any_sync(0xffffffffu, x >= list.least))
+              list.best = lp_both(list.best, lp_sort(x >= list.least ? lp_key(x, i0 + lp_index<T>(j)) : 0ull));
+          }
+          list.raise();
+        }
       }
-      const unsigned long long last = __shfl_sync(0xffffffffu, list, a.top - 1);
-      if (last) least = lp_value(last);
     }
     // the warp's maximum, and the entry that l leaves out
     if (__any_sync(0xffffffffu, top > m)) {
@@ -241,14 +323,23 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_token_logprobs(LogprobArgs a,
     // e^-200 is 0 in fp32; so -inf and NaN weigh nothing
     float sl[2] = {0.0f, 0.0f}, st[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float d = fmaxf(v[j] - m, -200.0f), e = __expf(d);
-      sl[j & 1] += e;
-      st[j & 1] = fmaf(e, d, st[j & 1]);
+    for (int j = 0; j < 16; j += 2) {
+      float d = v[j], e = v[j + 1];
+      add_two(d, e, -m, -m);
+      d = fmaxf(d, -200.0f);
+      e = fmaxf(e, -200.0f);
+      float p = d, q = e;
+      fma_two(p, q, 1.4426950408889634f, 0.0f);
+      p = lp_ex2(p);
+      q = lp_ex2(q);
+      add_two(sl[0], sl[1], p, q);
+      fma_pair(st[0], st[1], p, q, d, e);
     }
     l += sl[0] + sl[1];
     t += st[0] + st[1];
   }
+  int before = (int)ahead[0] + (int)ahead[1];
+  if (TOP && list.held) list.sort_in();
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     l += __shfl_xor_sync(0xffffffffu, l, o);
@@ -256,14 +347,14 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_token_logprobs(LogprobArgs a,
     before += __shfl_xor_sync(0xffffffffu, before, o);
   }
   if (lane == 0) s_part[warp] = LpPart{m, l, t, before};
-  if (TOP) s_list[warp][lane] = list;
+  if (TOP) s_list[warp][lane] = list.best;
   __syncthreads();
   if (ctas > 1) cluster_wait();  // all CTAs of the cluster run
   LpPart p = s_part[0];
   if (warp == 0) {
     for (int w = 1; w < kLpWarps; ++w) {
       p = lp_join(p, s_part[w]);
-      if (TOP) list = lp_both(list, s_list[w][lane]);
+      if (TOP) list.best = lp_both(list.best, s_list[w][lane]);
     }
     if (ctas > 1) {
       if (lane == 0) {
@@ -271,7 +362,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_token_logprobs(LogprobArgs a,
         st_cluster_v2(to, __float_as_uint(p.m), __float_as_uint(p.l));
         st_cluster_v2(to + 8, __float_as_uint(p.t), (uint32_t)p.before);
       }
-      if (TOP) st_cluster_v2(mapa_shared(smem_u32(&s_cta_list[rank][lane]), 0), (uint32_t)list, (uint32_t)(list >> 32));
+      if (TOP) st_cluster_v2(mapa_shared(smem_u32(&s_cta_list[rank][lane]), 0), (uint32_t)list.best, (uint32_t)(list.best >> 32));
     }
   }
   if (ctas > 1) {
@@ -282,7 +373,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_token_logprobs(LogprobArgs a,
       p = s_cta[0];
       for (int r = 1; r < ctas; ++r) {
         p = lp_join(p, s_cta[r]);
-        if (TOP) list = lp_both(list, s_cta_list[r][lane]);
+        if (TOP) list.best = lp_both(list.best, s_cta_list[r][lane]);
       }
     }
   }
@@ -296,8 +387,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_token_logprobs(LogprobArgs a,
     a.entropy[row] = (float)(lse - (double)p.t / (1.0 + (double)p.l));
   }
   if (TOP && lane < a.top) {
-    a.top_tokens[(int64_t)row * a.top + lane] = list ? (int64_t)(int)~(uint32_t)list : -1;
-    a.top_logprobs[(int64_t)row * a.top + lane] = list ? logprob(lp_value(list)) : -INFINITY;
+    a.top_tokens[(int64_t)row * a.top + lane] = list.best ? (int64_t)(int)~(uint32_t)list.best : -1;
+    a.top_logprobs[(int64_t)row * a.top + lane] = list.best ? logprob(lp_value(list.best)) : -INFINITY;
   }
 }
 

@@ -29,6 +29,7 @@
 #include <numeric>
 
 #include "paged.cuh"
+#include "pairs.cuh"
 
 namespace otf {
 
@@ -425,21 +426,6 @@ __device__ __forceinline__ void give_back(const RowsArgs& a, const Portion& it, 
 
 // ---- scores to probabilities ------------------------------------------------------------------
 
-// Two fp32 operations in one.
-__device__ __forceinline__ void fma_two(float& x, float& y, float m, float z) {
-  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\tmov.b64 c, {%3, %3};\n\t"
-      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(x), "+f"(y) : "f"(m), "f"(z));
-}
-__device__ __forceinline__ void add_two(float& x, float& y, float u, float v) {
-  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
-      "add.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(x), "+f"(y) : "f"(u), "f"(v));
-}
-__device__ __forceinline__ float max_three(float x, float y, float z) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
-  return r;
-}
-
 // 4 x 4 16-byte pieces across four lanes: lane q's piece i becomes lane i's piece q.
 __device__ __forceinline__ void turn_pieces(uint32_t (&x)[4][4]) {
 #pragma unroll
@@ -764,6 +750,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
             mbar_arrive_n(bar, 63);
           }
           __syncwarp();
+          const int first = __shfl_sync(0xffffffffu, x.key[0].rest, 0);
           if (x.key[0].there) {
             int page = x.key[0].page, from = x.key[0].rest;
             if (page < 0 || page >= a.c.n_pages) {
@@ -771,7 +758,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
               page = a.c.n_pages;  // reads as zeros
             }
             // the first lane's page may have begun before the chunk, the last one's may go on behind it
-            const int first = __shfl_sync(__activemask(), from, 0), d = (int)a.page.d;
+            const int d = (int)a.page.d;
             int row = lane ? lane * d - first : 0;
             const int end = min(kPrKeys, (lane + 1) * d - first);
             uint32_t dst = ring + slot * S::tile + row * 128;
