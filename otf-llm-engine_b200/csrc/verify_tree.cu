@@ -24,7 +24,7 @@ int check_device();                       // capi.cu
 int verify_tree_device_error(int clear);  // read (and optionally clear) the flag below
 
 constexpr int kTreeMaxNodes = 64;
-constexpr int kTreeThreads = 512;
+constexpr int kTreeThreads = 256;
 constexpr int kTreeWarps = kTreeThreads / 32;
 constexpr int kTreeCluster = 16;
 constexpr int kTreeResident = 148 * 4;  // CTAs that run at once
@@ -59,7 +59,7 @@ __device__ __forceinline__ double tree_score(float x, float e, double T) {
   return T == 0.0 ? (double)x : (double)x / T - log((double)e);
 }
 
-__global__ void __launch_bounds__(kTreeThreads, 2) k_verify_tree(TreeArgs a, int ctas) {
+__global__ void __launch_bounds__(kTreeThreads, 4) k_verify_tree(TreeArgs a, int ctas) {
   __shared__ TreeLeader s_warp[kTreeWarps], s_all[2][kTreeCluster];
   __shared__ float s_bar[kTreeWarps];
   __shared__ int64_t s_tokens[kTreeMaxNodes + 1];
@@ -256,7 +256,7 @@ extern "C" OTF_API int otf_verify_tree(const float* target, int64_t ld_target, c
     otf::opted_in(done, dev);
   }
   int ctas = otf::kTreeCluster;
-  while (ctas > 1 && (batch * ctas > otf::kTreeResident / 2 || (int64_t)(ctas / 2) * otf::kTreeThreads * 4 >= vocab)) ctas /= 2;
+  while (ctas > 1 && (batch * ctas > otf::kTreeResident || (int64_t)(ctas / 2) * otf::kTreeThreads * 4 >= vocab)) ctas /= 2;
   return set_cuda_error(otf::launch_pdl(otf::k_verify_tree, dim3((unsigned)(batch * ctas)), dim3(otf::kTreeThreads), 0,
                                         static_cast<cudaStream_t>(stream), (unsigned)ctas, a, ctas));
 }
