@@ -53,8 +53,8 @@ __device__ __forceinline__ void report_bad_rows() { atomicExch(&g_paged_rows_dev
 
 // The item that several CTAs share and that begins in a CTA's run.
 struct __align__(16) SharedItem {
-  int there, b, rb, g;
-  int first_part, last_cta, pad[2];
+  int there, g, row0, rows;  // row0: of the sequence's; rows of the block
+  int first_part, last_cta, r0, pad;
 };
 
 struct RowsArgs {
@@ -612,7 +612,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
       for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
       RunStart r = {};
       r.total = total;
-      r.ctas = max((int64_t)1, min((int64_t)kPrGrid, total / (kPrItemUnits + 1)));
+      r.ctas = max((int64_t)1, min((int64_t)kPrGrid, total));
       r.u0 = blockIdx.x < r.ctas ? blockIdx.x * total / r.ctas : total;
       r.u1 = blockIdx.x < r.ctas ? (blockIdx.x + 1) * total / r.ctas : total;
       if (lane == 0) sm.run = r;
@@ -713,8 +713,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
       if (it.c0 == 0 && it.c1 > 0 && it.c1 < it.k.chunks) {
         // begins in this run and goes on behind it: what the joining kernel needs to know
         const int64_t end = walk.at + kPrItemUnits + it.k.chunks - 1;  // the unit of its last chunk
-        over = SharedItem{1, it.b, it.rb, it.g, 2 * (int)blockIdx.x + (it.first ? 0 : 1),
-                          (int)(((end + 1) * run.ctas - 1) / run.total), {0, 0}};
+        over = SharedItem{1, it.g, it.rb * kPrRows, it.rows, 2 * (int)blockIdx.x + (it.first ? 0 : 1),
+                          (int)(((end + 1) * run.ctas - 1) / run.total), it.s.r0, 0};
       }
       const uint32_t slot = found & 3;
       if (found >= 4) rows_wait(&sm.item_empty[slot], ((found >> 2) - 1) & 1u, gave_up);
@@ -750,6 +750,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
             mbar_arrive_n(bar, 63);
           }
           __syncwarp();
+          const int first = __shfl_sync(0xffffffffu, x.key[0].rest, 0);
           const int first = __shfl_sync(0xffffffffu, x.key[0].rest, 0);
           if (x.key[0].there) {
             int page = x.key[0].page, from = x.key[0].rest;
@@ -1226,35 +1227,55 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
 }
 
 // The parts of an item that several CTAs shared, joined in the keys' order: grid (CTAs, rows / 8), a warp
-// per row.
-template <bool BF, int D, bool TREE>
+// per row.  Latency-bound: what the item is, then all parts' m and l and, eight at a time, their o.
+template <bool BF, int D>
 __global__ void __launch_bounds__(256) k_paged_rows_join(const __grid_constant__ RowsArgs a) {
-  constexpr int PL = D / 32;
+  constexpr int PL = D / 32, U = 8;
   pdl_trigger();
   pdl_wait();
   const SharedItem x = a.shared[blockIdx.x];
-  if (!x.there) return;
-  const RowRange s = range_of<TREE>(a, x.b, false);
-  const int lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5), row = x.rb * kPrRows + r;
-  if (row >= s.tokens * a.rep) return;
+  const int lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
+  if (!x.there || r >= x.rows) return;
   const int n = x.last_cta - (int)blockIdx.x + 1;
   auto part = [&](int i) { return (int64_t)(i == 0 ? x.first_part : 2 * ((int)blockIdx.x + i)) * a.part_rows + r; };
   float M = -INFINITY, L = 0.0f, acc[PL] = {};
-  for (int i = lane; i < n; i += 32) M = fmaxf(M, a.part_ml[part(i)].x);
+  float2 ml = lane < n ? a.part_ml[part(lane)] : make_float2(-INFINITY, 0.0f);  // of the lane's part among 32
+  M = ml.x;
+  for (int i = lane + 32; i < n; i += 32) M = fmaxf(M, a.part_ml[part(i)].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const float2 ml = a.part_ml[part(i)];
-    const float f = ml.x == -INFINITY ? 0.0f : pr_ex2(ml.x - M);
-    const float* y = a.part + part(i) * D + lane * PL;
-    L = fmaf(ml.y, f, L);
-    if (ml.x != -INFINITY)
+  for (int base = 0; base < n; base += U) {
+    float y[U][PL];
 #pragma unroll
-      for (int j = 0; j < PL; ++j) acc[j] = fmaf(y[j], f, acc[j]);
+    for (int k = 0; k < U; ++k) {
+      const float* z = a.part + part(min(base + k, n - 1)) * D + lane * PL;
+      if (D == 128) {
+        const float4 v = *reinterpret_cast<const float4*>(z);
+        y[k][0] = v.x;
+        y[k][1] = v.y;
+        y[k][PL - 2] = v.z;
+        y[k][PL - 1] = v.w;
+      } else {
+        const float2 v = *reinterpret_cast<const float2*>(z);
+        y[k][0] = v.x;
+        y[k][1] = v.y;
+      }
+    }
+    if (base && (base & 31) == 0) ml = base + lane < n ? a.part_ml[part(base + lane)] : make_float2(-INFINITY, 0.0f);
+    const float mine = ml.x == -INFINITY ? 0.0f : pr_ex2(ml.x - M);
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const float f = __shfl_sync(0xffffffffu, mine, (base + k) & 31), l = __shfl_sync(0xffffffffu, ml.y, (base + k) & 31);
+      const float m = __shfl_sync(0xffffffffu, ml.x, (base + k) & 31);
+      if (base + k < n && m != -INFINITY) {
+        L = fmaf(l, f, L);
+#pragma unroll
+        for (int j = 0; j < PL; ++j) acc[j] = fmaf(y[k][j], f, acc[j]);
+      }
+    }
   }
-  const int t = (uint32_t)row / a.rep_div, head = x.g * a.rep + row - t * a.rep;
-  uint32_t* to = reinterpret_cast<uint32_t*>(a.out + (s.r0 + (int64_t)t) * a.ldo + (int64_t)head * D + lane * PL);
+  const int row = x.row0 + r, t = (uint32_t)row / a.rep_div, head = x.g * a.rep + row - t * a.rep;
+  uint32_t* to = reinterpret_cast<uint32_t*>(a.out + (x.r0 + (int64_t)t) * a.ldo + (int64_t)head * D + lane * PL);
 #pragma unroll
   for (int j = 0; j < PL / 2; ++j) to[j] = pack2<BF>(acc[2 * j] / L, acc[2 * j + 1] / L);
 }
@@ -1291,7 +1312,7 @@ static cudaError_t launch_rows(const RowsArgs& a, cudaStream_t s) {
   }
   e = launch_pdl(k, dim3(kPrGrid), dim3(kPrThreads), RowsShape<D>::bytes, s, 1u, a);
   if (e != cudaSuccess) return e;
-  return launch_pdl(k_paged_rows_join<BF, D, TREE>, dim3(kPrGrid, (unsigned)(a.part_rows / 8)), dim3(256), 0, s, 1u, a);
+  return launch_pdl(k_paged_rows_join<BF, D>, dim3(kPrGrid, (unsigned)(a.part_rows / 8)), dim3(256), 0, s, 1u, a);
 }
 
 }  // namespace otf
