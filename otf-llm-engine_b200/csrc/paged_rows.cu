@@ -751,7 +751,6 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
           }
           __syncwarp();
           const int first = __shfl_sync(0xffffffffu, x.key[0].rest, 0);
-          const int first = __shfl_sync(0xffffffffu, x.key[0].rest, 0);
           if (x.key[0].there) {
             int page = x.key[0].page, from = x.key[0].rest;
             if (page < 0 || page >= a.c.n_pages) {
