@@ -646,12 +646,16 @@ OTF_API int otf_verify_drafts(const float* target, int64_t target_seq, int64_t l
  * -inf; a token of weight 0 is never drawn.  A sequence without a token to draw, with rows not in [0, n], a number of
  * nodes or a temperature out of range gets -1, 0 accepted, and raises the otf_device_error flag; so does a parent out of
  * range, whose node hangs nowhere.  Scores that decide are compared in 64 bits.  depth 0..63; at most 65535
- * sequences and a vocabulary of 2^30.  No workspace.  Beside otf_verify_drafts, for drafts in a line.
+ * sequences and a vocabulary of 2^30.  workspace: otf_verify_tree_workspace_bytes(...) (0 for many logits, then it may be
+ * NULL), 16-byte aligned, need not be cleared; two calls that may run at the same time need one each.  Beside
+ * otf_verify_drafts, for drafts in a line.
  */
+OTF_API int64_t otf_verify_tree_workspace_bytes(int64_t n, int64_t vocab);
 OTF_API int otf_verify_tree(const float* target, int64_t ld_target, const int64_t* tokens, const int32_t* parents,
                             const int32_t* starts, int64_t n, const float* noise, int64_t noise_seq, int64_t ld_noise,
                             const float* temperatures, double temperature, int64_t* out_tokens, int32_t* path,
-                            int32_t* accepted, int64_t batch, int64_t depth, int64_t vocab, void* stream);
+                            int32_t* accepted, int64_t batch, int64_t depth, int64_t vocab, void* workspace,
+                            int64_t workspace_bytes, void* stream);
 
 /*
  * Log probabilities: logits [n, vocab] (row stride ld; dtype OTF_DTYPE_F32, _F16 or _BF16), p = softmax of a row.

@@ -8,9 +8,10 @@
 //
 // An entry is weighed in fp32 with a bound on its error; only those that may lead are computed in 64 bits.
 //
-// A sequence is walked by a cluster of CTAs that cut the vocabulary among them; a step's leaders meet in
-// distributed shared memory.  Bound: a step's rows are 8 bytes per entry, but a step cannot start before the
-// one before it has ended, so few sequences are bound by latency.
+// Many logits: a sequence is walked by a cluster of CTAs that cut the vocabulary among them (k_verify_tree); a step's
+// leaders meet in distributed shared memory.  A step's rows are 8 bytes per entry, but a step cannot start before the
+// one before it has ended: some 4 us.  Few logits: every node's leader is found at once by the whole GPU, with the
+// noise of the node's depth, and the way is then followed in a second launch (k_tree_leaders, k_tree_walk).
 #include <algorithm>
 #include <cfloat>
 
@@ -28,6 +29,9 @@ constexpr int kTreeThreads = 256;
 constexpr int kTreeWarps = kTreeThreads / 32;
 constexpr int kTreeCluster = 16;
 constexpr int kTreeResident = 148 * 4;  // CTAs that run at once
+constexpr int kTreeSlice = 8192;        // entries of a CTA of k_tree_leaders
+// Logits of all nodes up to which they are looked at at once.  Measured: FIGURE.
+constexpr int64_t kTreeAtOnce = 12ll << 20;
 
 // Set when a sequence has no token to draw, or an argument on the device is out of range.
 __device__ int g_verify_tree_device_error;
@@ -46,6 +50,8 @@ struct TreeArgs {
   int* path;          // [batch][depth]
   int* accepted;
   int per, n, depth, vocab;
+  int batch, slices;
+  struct TreeLeader* leaders;  // [n][slices], k_tree_leaders alone
 };
 
 struct TreeLeader {
@@ -59,11 +65,88 @@ __device__ __forceinline__ double tree_score(float x, float e, double T) {
   return T == 0.0 ? (double)x : (double)x / T - log((double)e);
 }
 
+// The leader of two lanes' at every lane.
+__device__ __forceinline__ TreeLeader tree_leader_of_warp(TreeLeader l) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const double s = __shfl_xor_sync(0xffffffffu, l.score, o);
+    const int i = __shfl_xor_sync(0xffffffffu, l.at, o);
+    if (i != INT_MAX && leads(s, i, l)) l = {s, i, 0};
+  }
+  return l;
+}
+
+// The leader among entries i0, i0 + 1 .. 3 and so on, `stride` apart, below `end`, of a row of logits x and of noise e (null
+// at temperature 0) that the CTA's threads cut among them: of the warp, at every lane.  `bar`: [kTreeWarps] of the CTA.
+__device__ __forceinline__ TreeLeader tree_leader(const float* x, const float* e, double T, float c, int first, int stride, int end,
+                                                  float* s_bar) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool ax = (reinterpret_cast<uintptr_t>(x) & 15) == 0, ae = (reinterpret_cast<uintptr_t>(e) & 15) == 0;
+  // a thread's first entry of the largest upper bound, the largest of the others, and what its entries score at least
+  float high = -INFINITY, next = -INFINITY, bar = -INFINITY, lead_x = 0.0f, lead_e = 1.0f;
+  int lead = INT_MAX;
+  constexpr int U = 4;
+  for (int i0 = first; i0 < end; i0 += U * stride) {
+    float4 vx[U], ve[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = (int)min((int64_t)i0 + (int64_t)u * stride, (int64_t)end);  // behind the end: -inf without a read
+      vx[u] = logits4(x, i, end, ax);
+      if (e) ve[u] = logits4(e, i, end, ae, INFINITY);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float fx[4] = {vx[u].x, vx[u].y, vx[u].z, vx[u].w};
+      const float fe[4] = {ve[u].x, ve[u].y, ve[u].z, ve[u].w};
+#pragma unroll
+      for (int z = 0; z < 4; ++z) {
+        float up = fx[z], low = fx[z];
+        if (e) {
+          // two roundings of each term, and the logarithm's error, are below 2^-20 of them, and of 1
+          const float p = fx[z] * c, l = __log2f(fe[z]), d = p - l, w = 0x1p-20f * (fabsf(p) + fabsf(l) + 1.0f);
+          up = d + w;
+          low = d - w;
+          if (fabsf(p) == INFINITY) up = fx[z] == -INFINITY ? -INFINITY : fx[z] > 0.0f || fe[z] == 0.0f ? INFINITY : -FLT_MAX;
+        }
+        if (up > high) {
+          next = fmaxf(next, high);
+          high = up;
+          lead = i0 + u * stride + z;
+          lead_x = fx[z];
+          lead_e = e ? fe[z] : 1.0f;
+        } else if (up == up) {
+          next = fmaxf(next, up);
+        }
+        bar = fmaxf(bar, low);
+      }
+    }
+  }
+  float most = bar;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  if (lane == 0) s_bar[warp] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kTreeWarps; ++w) most = fmaxf(most, s_bar[w]);
+  TreeLeader mine = {-INFINITY, INT_MAX, 0};
+  if (high >= most && lead != INT_MAX) {
+    const double s = tree_score(lead_x, lead_e, T);
+    if (s > -INFINITY) mine = {s, lead, 0};
+    if (e && next >= most)  // another one of the thread's may lead: all of them in 64 bits
+      for (int i0 = first; i0 < end; i0 += min(stride, end - i0))
+        for (int i = i0; i < min(i0 + 4, end); ++i) {
+          const double y = tree_score(x[i], e[i], T);
+          if (y > -INFINITY && leads(y, i, mine)) mine = {y, i, 0};
+        }
+  }
+  return tree_leader_of_warp(mine);
+}
+
 __global__ void __launch_bounds__(kTreeThreads, 4) k_verify_tree(TreeArgs a, int ctas) {
   __shared__ TreeLeader s_warp[kTreeWarps], s_all[2][kTreeCluster];
   __shared__ float s_bar[kTreeWarps];
   __shared__ int64_t s_tokens[kTreeMaxNodes + 1];
-  __shared__ int s_path[kTreeMaxNodes], s_at, s_taken;
+  __shared__ int s_path[kTreeMaxNodes], s_at;
   pdl_trigger();
   pdl_wait();
   const int b = blockIdx.x / ctas, rank = blockIdx.x - b * ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -93,79 +176,11 @@ __global__ void __launch_bounds__(kTreeThreads, 4) k_verify_tree(TreeArgs a, int
   for (int step = 0; !failed; ++step) {
     const float* x = a.target + (int64_t)(r0 + at) * a.ldt;
     const float* e = T > 0.0 ? a.noise + b * a.nseq + step * a.ldn : nullptr;
-    const bool ax = (reinterpret_cast<uintptr_t>(x) & 15) == 0, ae = (reinterpret_cast<uintptr_t>(e) & 15) == 0;
-    // a thread's first entry of the largest upper bound, the largest of the others, and what its entries score at least
-    float high = -INFINITY, next = -INFINITY, bar = -INFINITY, lead_x = 0.0f, lead_e = 1.0f;
-    int lead = INT_MAX;
-    constexpr int U = 4;
-    const int stride = 4 * kTreeThreads * ctas;
-    for (int i0 = 4 * (rank * kTreeThreads + tid); i0 < a.vocab; i0 += U * stride) {
-      float4 vx[U], ve[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = (int)min((int64_t)i0 + (int64_t)u * stride, (int64_t)a.vocab);  // behind the end: -inf without a read
-        vx[u] = logits4(x, i, a.vocab, ax);
-        if (e) ve[u] = logits4(e, i, a.vocab, ae, INFINITY);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const float fx[4] = {vx[u].x, vx[u].y, vx[u].z, vx[u].w};
-        const float fe[4] = {ve[u].x, ve[u].y, ve[u].z, ve[u].w};
-#pragma unroll
-        for (int z = 0; z < 4; ++z) {
-          float up = fx[z], low = fx[z];
-          if (e) {
-            // two roundings of each term, and the logarithm's error, are below 2^-20 of them, and of 1
-            const float p = fx[z] * c, l = __log2f(fe[z]), d = p - l, w = 0x1p-20f * (fabsf(p) + fabsf(l) + 1.0f);
-            up = d + w;
-            low = d - w;
-            if (fabsf(p) == INFINITY) up = fx[z] == -INFINITY ? -INFINITY : fx[z] > 0.0f || fe[z] == 0.0f ? INFINITY : -FLT_MAX;
-          }
-          if (up > high) {
-            next = fmaxf(next, high);
-            high = up;
-            lead = i0 + u * stride + z;
-            lead_x = fx[z];
-            lead_e = e ? fe[z] : 1.0f;
-          } else if (up == up) {
-            next = fmaxf(next, up);
-          }
-          bar = fmaxf(bar, low);
-        }
-      }
-    }
-    float most = bar;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if (lane == 0) s_bar[warp] = most;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kTreeWarps; ++w) most = fmaxf(most, s_bar[w]);
-    TreeLeader mine = {-INFINITY, INT_MAX, 0};
-    if (high >= most && lead != INT_MAX) {
-      const double s = tree_score(lead_x, lead_e, T);
-      if (s > -INFINITY) mine = {s, lead, 0};
-      if (e && next >= most)  // another one of the thread's may lead: all of them in 64 bits
-        for (int i0 = 4 * (rank * kTreeThreads + tid); i0 < a.vocab; i0 += min(stride, a.vocab - i0))
-          for (int i = i0; i < min(i0 + 4, a.vocab); ++i) {
-            const double y = tree_score(x[i], e[i], T);
-            if (y > -INFINITY && leads(y, i, mine)) mine = {y, i, 0};
-          }
-    }
-    auto shared = [&](TreeLeader l) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const double s = __shfl_xor_sync(0xffffffffu, l.score, o);
-        const int i = __shfl_xor_sync(0xffffffffu, l.at, o);
-        if (i != INT_MAX && leads(s, i, l)) l = {s, i, 0};
-      }
-      return l;
-    };
-    mine = shared(mine);
+    TreeLeader mine = tree_leader(x, e, T, c, 4 * (rank * kTreeThreads + tid), 4 * kTreeThreads * ctas, a.vocab, s_bar);
     if (lane == 0) s_warp[warp] = mine;
     __syncthreads();
     if (warp == 0) {
-      mine = shared(lane < kTreeWarps ? s_warp[lane] : TreeLeader{-INFINITY, INT_MAX, 0});
+      mine = tree_leader_of_warp(lane < kTreeWarps ? s_warp[lane] : TreeLeader{-INFINITY, INT_MAX, 0});
       if (lane < ctas) {
         const long long bits = __double_as_longlong(mine.score);
         st_cluster_v4(mapa_shared(smem_u32(&s_all[step & 1][rank]), lane), __uint_as_float((uint32_t)bits),
@@ -175,7 +190,7 @@ __global__ void __launch_bounds__(kTreeThreads, 4) k_verify_tree(TreeArgs a, int
     __syncwarp();
     cluster_sync_all();
     if (warp == 0) {
-      const TreeLeader all = shared(lane < ctas ? s_all[step & 1][lane] : TreeLeader{-INFINITY, INT_MAX, 0});
+      const TreeLeader all = tree_leader_of_warp(lane < ctas ? s_all[step & 1][lane] : TreeLeader{-INFINITY, INT_MAX, 0});
       int child = -1;  // goes on there; -1: ends, -2: nothing to draw
       if (all.at == INT_MAX) {
         child = -2;
@@ -210,6 +225,133 @@ __global__ void __launch_bounds__(kTreeThreads, 4) k_verify_tree(TreeArgs a, int
   }
 }
 
+// The leaders of all nodes' rows, grid (slices, n).
+__global__ void __launch_bounds__(kTreeThreads, 4) k_tree_leaders(TreeArgs a) {
+  __shared__ float s_bar[kTreeWarps];
+  __shared__ TreeLeader s_warp[kTreeWarps];
+  __shared__ int s_seq, s_level;
+  pdl_trigger();
+  pdl_wait();
+  const int row = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (warp == 0) {
+    int b = 0, level = 0;
+    if (a.starts) {
+      for (int i = 0; i < a.batch; i += 32)
+        b += __popc(__ballot_sync(0xffffffffu, i + lane < a.batch && a.starts[i + lane + 1] <= row));
+    } else {
+      b = row / a.per;
+    }
+    // the node's depth, up through its parents in the lanes
+    const int r0 = b < a.batch ? (a.starts ? a.starts[b] : b * a.per) : 0, r1 = b < a.batch ? (a.starts ? a.starts[b + 1] : r0 + a.per) : 0;
+    if (b >= a.batch || r0 < 0 || r1 > a.n || row < r0 || r1 - r0 > kTreeMaxNodes) {
+      b = -1;
+    } else {
+      int up[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int i = lane + 32 * h;
+        up[h] = r0 + i < r1 ? a.parents[r0 + i] : -1;
+        if (up[h] >= i || up[h] < -1) up[h] = -1;
+      }
+      for (int at = row - r0;;) {
+        const int p = at < 32 ? __shfl_sync(0xffffffffu, up[0], at) : __shfl_sync(0xffffffffu, up[1], at - 32);
+        if (p < 0) {
+          if (at) b = -1;  // does not hang on the root: never reached
+          break;
+        }
+        at = p;
+        ++level;
+      }
+      if (level > a.depth) b = -1;
+    }
+    if (lane == 0) {
+      s_seq = b;
+      s_level = level;
+    }
+  }
+  __syncthreads();
+  const int b = s_seq;
+  if (b < 0) return;
+  const double T = a.temperatures ? (double)a.temperatures[b] : a.temperature;
+  if (!temperature_ok((float)T) || (T > 0.0 && !a.noise)) return;  // k_tree_walk reports it
+  const float c = T > 0.0 ? (float)(1.4426950408889634 / T) : 0.0f;
+  const float* x = a.target + (int64_t)row * a.ldt;
+  const float* e = T > 0.0 ? a.noise + b * a.nseq + s_level * a.ldn : nullptr;
+  const int i0 = blockIdx.x * kTreeSlice, end = min(a.vocab, i0 + kTreeSlice);
+  const TreeLeader mine = tree_leader(x, e, T, c, i0 + 4 * tid, 4 * kTreeThreads, end, s_bar);
+  if (lane == 0) s_warp[warp] = mine;
+  __syncthreads();
+  if (warp == 0) {
+    const TreeLeader all = tree_leader_of_warp(lane < kTreeWarps ? s_warp[lane] : TreeLeader{-INFINITY, INT_MAX, 0});
+    if (lane == 0) a.leaders[(int64_t)row * a.slices + blockIdx.x] = all;
+  }
+}
+
+// And the ways through them: a warp per sequence.
+__global__ void __launch_bounds__(32) k_tree_walk(TreeArgs a) {
+  __shared__ int64_t s_tokens[kTreeMaxNodes];
+  __shared__ int s_path[kTreeMaxNodes];
+  __shared__ int s_drawn[kTreeMaxNodes];
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.x, lane = threadIdx.x;
+  const int r0 = a.starts ? a.starts[b] : b * a.per, r1 = a.starts ? a.starts[b + 1] : r0 + a.per, nodes = r1 - r0;
+  const double T = a.temperatures ? (double)a.temperatures[b] : a.temperature;
+  bool failed = !(r0 >= 0 && r1 <= a.n && nodes > 0 && nodes <= kTreeMaxNodes && temperature_ok((float)T) && (T == 0.0 || a.noise));
+  int64_t token[2] = {-1, -1};
+  int parent[2] = {-1, -1};
+  if (!failed) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (lane + 32 * h < nodes) {
+        token[h] = a.tokens[r0 + lane + 32 * h];
+        parent[h] = a.parents[r0 + lane + 32 * h];
+        if (parent[h] >= lane + 32 * h || parent[h] < -1) {
+          atomicExch(&g_verify_tree_device_error, 1);
+          parent[h] = -1;
+        }
+      }
+    // a lane's nodes' leaders (those that cannot be reached hold what happens to lie there)
+#pragma unroll 1
+    for (int i = lane; i < nodes; i += 32) {
+      const TreeLeader* l = a.leaders + (int64_t)(r0 + i) * a.slices;
+      TreeLeader all = {-INFINITY, INT_MAX, 0};
+#pragma unroll 4
+      for (int k = 0; k < a.slices; ++k) {
+        const TreeLeader y = l[k];
+        if (y.at != INT_MAX && leads(y.score, y.at, all)) all = y;
+      }
+      s_drawn[i] = all.at;
+    }
+  }
+  __syncwarp();
+  int at = 0, taken = 0;
+  while (!failed) {
+    const int drawn = s_drawn[at];
+    if (drawn == INT_MAX) {
+      failed = true;
+      break;
+    }
+    if (lane == 0) s_tokens[taken] = drawn;
+    if (taken == a.depth) break;
+    const uint32_t h0 = __ballot_sync(0xffffffffu, lane > 0 && parent[0] == at && token[0] == drawn);
+    const uint32_t h1 = __ballot_sync(0xffffffffu, parent[1] == at && token[1] == drawn);
+    if (!(h0 | h1)) break;
+    at = h0 ? __ffs((int)h0) - 1 : 31 + __ffs((int)h1);
+    if (lane == 0) s_path[taken] = at;
+    ++taken;
+  }
+  __syncwarp();
+  for (int j = lane; j <= a.depth; j += 32) {
+    a.out[(int64_t)b * (a.depth + 1) + j] = !failed && j <= taken ? s_tokens[j] : -1;
+    if (j < a.depth) a.path[(int64_t)b * a.depth + j] = !failed && j < taken ? s_path[j] : -1;
+  }
+  if (lane == 0) {
+    a.accepted[b] = failed ? 0 : taken;
+    if (failed) atomicExch(&g_verify_tree_device_error, 1);
+  }
+}
+
 }  // namespace otf
 
 using otf::check_device;
@@ -228,11 +370,18 @@ int otf::verify_tree_device_error(int clear) {
   return v;
 }
 
+extern "C" OTF_API int64_t otf_verify_tree_workspace_bytes(int64_t n, int64_t vocab) {
+  if (n <= 0 || vocab <= 0 || n > INT32_MAX || vocab > (1ll << 30)) return -1;
+  if (n > 65535 || n * vocab > otf::kTreeAtOnce) return 0;
+  return n * ((vocab + otf::kTreeSlice - 1) / otf::kTreeSlice) * (int64_t)sizeof(otf::TreeLeader);
+}
+
 extern "C" OTF_API int otf_verify_tree(const float* target, int64_t ld_target, const int64_t* tokens,
                                        const int32_t* parents, const int32_t* starts, int64_t n, const float* noise,
                                        int64_t noise_seq, int64_t ld_noise, const float* temperatures,
                                        double temperature, int64_t* out_tokens, int32_t* path, int32_t* accepted,
-                                       int64_t batch, int64_t depth, int64_t vocab, void* stream) {
+                                       int64_t batch, int64_t depth, int64_t vocab, void* workspace,
+                                       int64_t workspace_bytes, void* stream) {
   if (!target || !tokens || !parents || !out_tokens || (!path && depth) || !accepted) return OTF_ERR_INVALID;
   if (batch <= 0 || depth < 0 || vocab <= 0 || n <= 0 || (!starts && n % batch) || ld_target < vocab) return OTF_ERR_INVALID;
   if (!temperatures && !otf::temperature_ok((float)temperature)) return OTF_ERR_INVALID;
@@ -241,10 +390,19 @@ extern "C" OTF_API int otf_verify_tree(const float* target, int64_t ld_target, c
   if (batch > 65535 || depth >= otf::kTreeMaxNodes || vocab > (1ll << 30) || n > INT32_MAX ||
       (!starts && n / batch > otf::kTreeMaxNodes))
     return OTF_ERR_UNSUPPORTED;
+  const int64_t bytes = otf_verify_tree_workspace_bytes(n, vocab);
+  if (bytes && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < bytes)) return OTF_ERR_INVALID;
   const int st = check_device();
   if (st != OTF_OK) return st;
   otf::TreeArgs a = {target, ld_target, tokens, parents, starts, noise, noise_seq, ld_noise, temperatures, temperature,
-                     out_tokens, path, accepted, starts ? 0 : (int)(n / batch), (int)n, (int)depth, (int)vocab};
+                     out_tokens, path, accepted, starts ? 0 : (int)(n / batch), (int)n, (int)depth, (int)vocab,
+                     (int)batch, (int)((vocab + otf::kTreeSlice - 1) / otf::kTreeSlice), static_cast<otf::TreeLeader*>(workspace)};
+  if (bytes) {
+    const cudaError_t e = otf::launch_pdl(otf::k_tree_leaders, dim3((unsigned)a.slices, (unsigned)n), dim3(otf::kTreeThreads), 0,
+                                          static_cast<cudaStream_t>(stream), 1u, a);
+    if (e != cudaSuccess) return set_cuda_error(e);
+    return set_cuda_error(otf::launch_pdl(otf::k_tree_walk, dim3((unsigned)batch), dim3(32), 0, static_cast<cudaStream_t>(stream), 1u, a));
+  }
   static std::atomic<bool> done[64];
   int dev;
   bool needs;

@@ -137,6 +137,7 @@ EXPORTS = (
     "otf_paged_keep",
     "otf_verify_workspace_bytes",
     "otf_verify_drafts",
+    "otf_verify_tree_workspace_bytes",
     "otf_verify_tree",
     "otf_token_logprobs",
 )
@@ -243,7 +244,10 @@ def lib() -> ctypes.CDLL:
     L.otf_paged_attn_rows.restype = i32
     L.otf_paged_keep.argtypes = [cache, vp, i64, vp, i64, vp]
     L.otf_paged_keep.restype = i32
-    L.otf_verify_tree.argtypes = [vp, i64, vp, vp, vp, i64, vp, i64, i64, vp, ctypes.c_double, vp, vp, vp, i64, i64, i64, vp]
+    L.otf_verify_tree_workspace_bytes.argtypes = [i64, i64]
+    L.otf_verify_tree_workspace_bytes.restype = i64
+    L.otf_verify_tree.argtypes = [vp, i64, vp, vp, vp, i64, vp, i64, i64, vp, ctypes.c_double, vp, vp, vp, i64, i64, i64, vp,
+                                  i64, vp]
     L.otf_verify_tree.restype = i32
     L.otf_token_logprobs.argtypes = [vp, i64, i32, vp, i64, i64, i64, vp, vp, vp, vp, vp, vp]
     L.otf_token_logprobs.restype = i32

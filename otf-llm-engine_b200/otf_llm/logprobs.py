@@ -13,7 +13,7 @@ import torch
 
 from . import _native
 from .paged import _call
-from .speculative import _rows, _vector
+from .speculative import _rows
 
 MAX_TOP = 32
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
@@ -34,6 +34,31 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     nothing (log probability 0, rank -1).  ``top``: how many of the likeliest tokens to list, 32 at most, equal ones
     by the lower index; where fewer have a logit above -inf, -1 and -inf follow.  NaN counts as -inf, +inf as the
     largest finite number.  A token outside the vocabulary gets a NaN and raises the ``_native.device_error`` flag."""
+    key = (logits.device, logits.dtype, logits.shape, logits.stride(), tokens.shape, top)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _plan(logits, tokens, top)
+        if len(_plans) >= 256:
+            _plans.clear()
+        _plans[key] = plan
+    dev, n, vocab, ld, dtype, top = plan
+    if tokens.dtype is not torch.int64 or tokens.device != dev or not tokens.is_contiguous():
+        raise ValueError(f"tokens must be contiguous int64 on {dev}, got {tokens.dtype} on {tokens.device}")
+    values, ranks = torch.empty((2, n), dtype=torch.float32, device=dev), torch.empty(n, dtype=torch.int32, device=dev)
+    logprobs, entropy = values.unbind()
+    top_tokens, top_logprobs = torch.empty((n, top), dtype=torch.int64, device=dev), torch.empty((n, top), device=dev, dtype=torch.float32)
+    if n:
+        at = values.data_ptr()
+        _call(_native.lib().otf_token_logprobs, dev, logits.data_ptr(), ld, dtype, tokens.data_ptr(), n, vocab, top, at, at + 4 * n,
+              ranks.data_ptr(), top_tokens.data_ptr() if top else None, top_logprobs.data_ptr() if top else None)
+    return TokenLogprobs(logprobs, entropy, ranks, top_tokens, top_logprobs)
+
+
+# shapes and strides of earlier calls' arguments, with what their checks found
+_plans: dict = {}
+
+
+def _plan(logits: torch.Tensor, tokens: torch.Tensor, top: int) -> tuple:
     _native._need_cuda(logits, "logits")
     if logits.dtype not in _DTYPES:
         raise TypeError(f"logits must be fp32, fp16 or bf16, got {logits.dtype}")
@@ -42,16 +67,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     n, vocab = logits.shape
     if int(top) != top or not 0 <= top <= MAX_TOP:
         raise ValueError(f"top must be 0 to {MAX_TOP}, got {top}")
-    top, dev = int(top), logits.device
     ld, = _rows(logits, "logits", (n, vocab))
     if ld < vocab:
         raise ValueError(f"logits needs rows that do not overlap, got strides {logits.stride()}")
-    pt = _vector(tokens, "tokens", torch.int64, n, dev)
-    out = TokenLogprobs(torch.empty(n, dtype=torch.float32, device=dev), torch.empty(n, dtype=torch.float32, device=dev),
-                        torch.empty(n, dtype=torch.int32, device=dev), torch.empty((n, top), dtype=torch.int64, device=dev),
-                        torch.empty((n, top), dtype=torch.float32, device=dev))
-    if n:
-        _call(_native.lib().otf_token_logprobs, dev, logits.data_ptr(), ld, _DTYPES[logits.dtype], pt, n, vocab, top,
-              out.logprobs.data_ptr(), out.entropy.data_ptr(), out.ranks.data_ptr(),
-              out.top_tokens.data_ptr() if top else None, out.top_logprobs.data_ptr() if top else None)
-    return out
+    if tokens.shape != (n,):
+        raise ValueError(f"tokens must be a contiguous [{n}] vector, got {list(tokens.shape)}")
+    return logits.device, n, vocab, ld, _DTYPES[logits.dtype], int(top)

@@ -92,35 +92,23 @@ def verify_tree(target_logits: torch.Tensor, tokens: torch.Tensor, parents: torc
 
     Returns (tokens int64 [batch, depth + 1]: the taken ones, the one that follows, then -1; path int32 [batch,
     depth]: the taken nodes, then -1, for ``PagedKVCache.keep``; accepted int32 [batch])."""
-    _native._need_cuda(target_logits, "target_logits")
-    dev = target_logits.device
-    if target_logits.dim() != 2 or target_logits.shape[0] == 0 or target_logits.shape[1] == 0:
-        raise ValueError(f"target_logits must be [n, vocab], got {list(target_logits.shape)}")
-    n, vocab = target_logits.shape
-    ld, = _rows(target_logits, "target_logits", (n, vocab))
+    key = (target_logits.device, target_logits.shape, target_logits.stride(), tokens.shape, parents.shape,
+           None if starts is None else starts.shape, batch, depth, None if noise is None else (noise.shape, noise.stride()))
+    plan = _tree_plans.get(key)
+    if plan is None:
+        plan = _plan_tree(target_logits, tokens, parents, starts, batch, depth, noise)
+        if len(_tree_plans) >= 256:
+            _tree_plans.clear()
+        _tree_plans[key] = plan
+    dev, n, vocab, ld, batch, depth, seq_n, ld_n, bytes_ = plan
     pt = _address(target_logits, "target_logits", _F32, dev)
-    ptok, pp = _vector(tokens, "tokens", torch.int64, n, dev), _vector(parents, "parents", torch.int32, n, dev)
-    ps = None
-    if starts is not None:
-        if starts.dim() != 1 or starts.shape[0] < 2 or (batch is not None and batch != starts.shape[0] - 1):
-            raise ValueError(f"starts must be a [batch + 1] vector, got {list(starts.shape)}")
-        batch = starts.shape[0] - 1
-        ps = _vector(starts, "starts", torch.int32, batch + 1, dev)
-    else:
-        batch = 1 if batch is None else int(batch)
-        if batch < 1 or n % batch or n // batch > MAX_NODES:
-            raise ValueError(f"{n} nodes do not divide among {batch} sequences of {MAX_NODES} at most; give starts")
-    if depth is None:
-        depth = MAX_NODES - 1 if noise is None or noise.dim() != 3 else noise.shape[1] - 1
-    if int(depth) != depth or not 0 <= depth < MAX_NODES:
-        raise ValueError(f"depth must be 0 to {MAX_NODES - 1}, got {depth}")
+    ptok, pp = _address(tokens, "tokens", torch.int64, dev), _address(parents, "parents", torch.int32, dev)
+    ps = None if starts is None else _vector(starts, "starts", torch.int32, batch + 1, dev)
+    if not (tokens.is_contiguous() and parents.is_contiguous()):
+        raise ValueError("tokens and parents must be contiguous")
     pn = each = None
-    seq_n = ld_n = 0
     if noise is not None:
-        seq_n, ld_n = _rows(noise, "noise", (batch, depth + 1, vocab))
         pn = _address(noise, "noise", _F32, dev)
-        if min(seq_n, ld_n) < 0:
-            raise ValueError(f"noise needs strides that are not negative, got {noise.stride()}")
     one = 0.0
     if isinstance(temperature, torch.Tensor):
         each = _vector(temperature, "temperature", _F32, batch, dev)
@@ -133,14 +121,52 @@ def verify_tree(target_logits: torch.Tensor, tokens: torch.Tensor, parents: torc
     out = torch.empty((batch, depth + 1), dtype=torch.int64, device=dev)
     path = torch.empty((batch, depth), dtype=torch.int32, device=dev)
     accepted = torch.empty(batch, dtype=torch.int32, device=dev)
+    # a small call's scratch, for this call alone and on its stream
+    ws = torch.empty(bytes_, dtype=torch.uint8, device=dev) if bytes_ else None
     _call(_native.lib().otf_verify_tree, dev, pt, ld, ptok, pp, ps, n, pn, seq_n, ld_n, each, one, out.data_ptr(),
-          path.data_ptr() if depth else None, accepted.data_ptr(), batch, depth, vocab)
+          path.data_ptr() if depth else None, accepted.data_ptr(), batch, depth, vocab, ws.data_ptr() if bytes_ else None, bytes_)
     return out, path, accepted
+
+
+def _plan_tree(target: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, starts: Optional[torch.Tensor],
+               batch: Optional[int], depth: Optional[int], noise: Optional[torch.Tensor]) -> tuple:
+    _native._need_cuda(target, "target_logits")
+    if target.dim() != 2 or target.shape[0] == 0 or target.shape[1] == 0:
+        raise ValueError(f"target_logits must be [n, vocab], got {list(target.shape)}")
+    n, vocab = target.shape
+    ld, = _rows(target, "target_logits", (n, vocab))
+    if ld < vocab:
+        raise ValueError(f"target_logits needs rows that do not overlap, got strides {target.stride()}")
+    for name, t in (("tokens", tokens), ("parents", parents)):
+        if t.shape != (n,):
+            raise ValueError(f"{name} must be a contiguous [{n}] vector, got {list(t.shape)}")
+    if starts is not None:
+        if starts.dim() != 1 or starts.shape[0] < 2 or (batch is not None and batch != starts.shape[0] - 1):
+            raise ValueError(f"starts must be a [batch + 1] vector, got {list(starts.shape)}")
+        batch = starts.shape[0] - 1
+    else:
+        batch = 1 if batch is None else int(batch)
+        if batch < 1 or n % batch or n // batch > MAX_NODES:
+            raise ValueError(f"{n} nodes do not divide among {batch} sequences of {MAX_NODES} at most; give starts")
+    if depth is None:
+        depth = MAX_NODES - 1 if noise is None or noise.dim() != 3 else noise.shape[1] - 1
+    if int(depth) != depth or not 0 <= depth < MAX_NODES:
+        raise ValueError(f"depth must be 0 to {MAX_NODES - 1}, got {depth}")
+    depth, seq_n, ld_n = int(depth), 0, 0
+    if noise is not None:
+        seq_n, ld_n = _rows(noise, "noise", (batch, depth + 1, vocab))
+        if seq_n < 0 or ld_n < vocab:
+            raise ValueError(f"noise needs rows that do not overlap, got strides {noise.stride()}")
+    size = _native.lib().otf_verify_tree_workspace_bytes(n, vocab)
+    if size < 0:
+        raise ValueError("shape not supported by otf_verify_tree")
+    return target.device, n, vocab, ld, batch, depth, seq_n, ld_n, size
 
 
 _F32 = torch.float32
 # shapes and strides of earlier calls' arguments, with what their checks found
 _plans: dict = {}
+_tree_plans: dict = {}
 
 
 def _address(t: torch.Tensor, name: str, dtype: torch.dtype, dev: torch.device) -> int:
