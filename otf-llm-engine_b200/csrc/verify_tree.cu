@@ -6,14 +6,13 @@
 // target's distribution.  In logarithms the leader is the largest x_i / T - log e_i, which needs no sum:
 // a step is one pass over one row of logits and one of noise, and only the rows on the way are read.
 //
-// An entry is weighed in fp32 with a bound on its error; only those that may lead are computed in 64 bits.
+// An entry is weighed in fp32, 5 instructions, with a bound on the error; only those that may lead are computed in 64 bits.
 //
 // Many logits: a sequence is walked by a cluster of CTAs that cut the vocabulary among them (k_verify_tree); a step's
 // leaders meet in distributed shared memory.  A step's rows are 8 bytes per entry, but a step cannot start before the
 // one before it has ended: some 4 us.  Few logits: every node's leader is found at once by the whole GPU, with the
 // noise of the node's depth, and the way is then followed in a second launch (k_tree_leaders, k_tree_walk).
 #include <algorithm>
-#include <cfloat>
 
 #include "logits.cuh"
 #include "paged.cuh"
@@ -76,16 +75,18 @@ __device__ __forceinline__ TreeLeader tree_leader_of_warp(TreeLeader l) {
   return l;
 }
 
-// The leader among entries i0, i0 + 1 .. 3 and so on, `stride` apart, below `end`, of a row of logits x and of noise e (null
-// at temperature 0) that the CTA's threads cut among them: of the warp, at every lane.  `bar`: [kTreeWarps] of the CTA.
+// The leader among entries first .. first + 3 and so on, `stride` apart, below `end`, of a row of logits x and of noise e
+// (null at temperature 0) that the CTA's threads cut among them: of the warp, at every lane.  s_top: [kTreeWarps].
+// In fp32 a score d = x c - log2 e is off by 2^-20 (|x c| + |log2 e| + 1) at most (two roundings, the logarithm's error), and
+// |log2 e| <= 150 where d is finite, so what lies 2^-19 (|d| + 304) below the largest d cannot lead.  The entries of a
+// thread that has one above are looked at again, by its warp, in 64 bits.
 __device__ __forceinline__ TreeLeader tree_leader(const float* x, const float* e, double T, float c, int first, int stride, int end,
-                                                  float* s_bar) {
+                                                  float* s_top) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool ax = (reinterpret_cast<uintptr_t>(x) & 15) == 0, ae = (reinterpret_cast<uintptr_t>(e) & 15) == 0;
-  // a thread's first entry of the largest upper bound, the largest of the others, and what its entries score at least
-  float high = -INFINITY, next = -INFINITY, bar = -INFINITY, lead_x = 0.0f, lead_e = 1.0f;
-  int lead = INT_MAX;
+  auto weigh = [&](float fx, float fe) { return e ? fmaf(fx, c, -__log2f(fe)) : fx; };
   constexpr int U = 4;
+  float top = -INFINITY;  // of the thread; a NaN is none
   for (int i0 = first; i0 < end; i0 += U * stride) {
     float4 vx[U], ve[U];
 #pragma unroll
@@ -95,49 +96,34 @@ __device__ __forceinline__ TreeLeader tree_leader(const float* x, const float* e
       if (e) ve[u] = logits4(e, i, end, ae, INFINITY);
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const float fx[4] = {vx[u].x, vx[u].y, vx[u].z, vx[u].w};
-      const float fe[4] = {ve[u].x, ve[u].y, ve[u].z, ve[u].w};
-#pragma unroll
-      for (int z = 0; z < 4; ++z) {
-        float up = fx[z], low = fx[z];
-        if (e) {
-          // two roundings of each term, and the logarithm's error, are below 2^-20 of them, and of 1
-          const float p = fx[z] * c, l = __log2f(fe[z]), d = p - l, w = 0x1p-20f * (fabsf(p) + fabsf(l) + 1.0f);
-          up = d + w;
-          low = d - w;
-          if (fabsf(p) == INFINITY) up = fx[z] == -INFINITY ? -INFINITY : fx[z] > 0.0f || fe[z] == 0.0f ? INFINITY : -FLT_MAX;
-        }
-        if (up > high) {
-          next = fmaxf(next, high);
-          high = up;
-          lead = i0 + u * stride + z;
-          lead_x = fx[z];
-          lead_e = e ? fe[z] : 1.0f;
-        } else if (up == up) {
-          next = fmaxf(next, up);
-        }
-        bar = fmaxf(bar, low);
-      }
-    }
+    for (int u = 0; u < U; ++u)
+      top = fmaxf(top, fmaxf(fmaxf(weigh(vx[u].x, ve[u].x), weigh(vx[u].y, ve[u].y)), fmaxf(weigh(vx[u].z, ve[u].z), weigh(vx[u].w, ve[u].w))));
   }
-  float most = bar;
+  float most = top;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-  if (lane == 0) s_bar[warp] = most;
+  if (lane == 0) s_top[warp] = most;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kTreeWarps; ++w) most = fmaxf(most, s_bar[w]);
+  for (int w = 0; w < kTreeWarps; ++w) most = fmaxf(most, s_top[w]);
+  // an infinity (a logit's, a noise of 0, or a product's) and -inf alone (small temperatures) are weighed in 64 bits as they are
+  const float bar = !e || fabsf(most) == INFINITY ? most : most - 0x1p-19f * (fabsf(most) + 304.0f);
   TreeLeader mine = {-INFINITY, INT_MAX, 0};
-  if (high >= most && lead != INT_MAX) {
-    const double s = tree_score(lead_x, lead_e, T);
-    if (s > -INFINITY) mine = {s, lead, 0};
-    if (e && next >= most)  // another one of the thread's may lead: all of them in 64 bits
-      for (int i0 = first; i0 < end; i0 += min(stride, end - i0))
-        for (int i = i0; i < min(i0 + 4, end); ++i) {
-          const double y = tree_score(x[i], e[i], T);
-          if (y > -INFINITY && leads(y, i, mine)) mine = {y, i, 0};
-        }
+  for (uint32_t in = __ballot_sync(0xffffffffu, top >= bar); in; in &= in - 1) {
+    const int64_t from = __shfl_sync(0xffffffffu, first, __ffs((int)in) - 1);
+    for (int k = lane;; k += 32) {
+      const int64_t i = from + (int64_t)(k >> 2) * stride + (k & 3);
+      if (i >= end) {
+        if ((k & 3) == 0 || from + (int64_t)(k >> 2) * stride >= end) break;
+        continue;
+      }
+      const float fx = x[i], fe = e ? e[i] : 1.0f;
+      if (weigh(fx, fe) >= bar) {
+        const double s = tree_score(fx, fe, T);
+        if (s > -INFINITY && leads(s, (int)i, mine)) mine = {s, (int)i, 0};
+      }
+    }
+    __syncwarp();
   }
   return tree_leader_of_warp(mine);
 }
