@@ -637,13 +637,13 @@ OTF_API int otf_verify_drafts(const float* target, int64_t target_seq, int64_t l
  * of several) the walk goes on there, else it ends; with `depth` children taken it ends behind the last one.
  * T = 0: the first largest logit.  So every token is distributed as the target alone draws it.
  * target: fp32 [n, ld_target], row of each node; tokens: int64 [n]; parents: int32 [n]; sequence b has the nodes
- * [starts[b], starts[b + 1]) (device int32 [batch + 1], or NULL: n / batch each), 1 to 64, as in otf_paged_attn_rows:
+ * [starts[b], starts[b + 1]) (device int32 [batch + 1], or NULL: n / batch each), 64 at most, as in otf_paged_attn_rows:
  * node 0 is the root, the last token that is certain (its own token is not looked at), and parents[i] < i.  noise:
  * fp32, row (b, step) at noise + b * noise_seq + step * ld_noise, depth + 1 rows of a sequence (may be NULL when every
  * temperature is 0).  temperatures: device fp32 [batch], or NULL: `temperature` for all; 0 or in 1e-20 .. 1e20.
  * out_tokens: int64 [batch, depth + 1], the taken nodes' tokens and the one that follows, then -1; path: int32
  * [batch, depth], the taken nodes, then -1; accepted: int32 [batch], how many.  A NaN among the logits counts as
- * -inf; a token of weight 0 is never drawn.  A sequence without a token to draw, with rows not in [0, n], a number of
+ * -inf; a token of weight 0 is never drawn.  A sequence without nodes gets -1 and 0 accepted.  One without a token to draw, with rows not in [0, n], a number of
  * nodes or a temperature out of range gets -1, 0 accepted, and raises the otf_device_error flag; so does a parent out of
  * range, whose node hangs nowhere.  Scores that decide are compared in 64 bits.  depth 0..63; at most 65535
  * sequences and a vocabulary of 2^30.  workspace: otf_verify_tree_workspace_bytes(...) (0 for many logits, then it may be

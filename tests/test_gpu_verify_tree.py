@@ -67,6 +67,10 @@ def test_walks_of_many_sequences_go_down(cuda_dev):
     assert int(taken.max()) >= 3
     check(cuda_dev, [(7 * b) % 20 + 1 for b in range(600)], 64, 4, 0.8, seed=4)
     check(cuda_dev, [9, 12, 3], 2000, 4, [0.0, 0.9, 1.4], seed=5)
+    # more logits than are looked at at once: clusters of several sizes, unaligned rows
+    check(cuda_dev, [40, 3, 64], 140001, 4, 0.9, seed=6)
+    check(cuda_dev, [30] * 90, 6003, 3, [0.0, 1.1, 0.7] * 30, seed=7)
+    check(cuda_dev, [25] * 700, 1001, 2, 0.8, seed=8)
 
 
 def test_the_first_of_equal_children_and_of_equal_logits(cuda_dev):
@@ -121,6 +125,9 @@ def test_sequences_that_cannot_be_walked(cuda_dev):
     bad = [[-1, 1, 0], [-1, 0, -5], [-1, 0, 2]]
     run(cuda_dev, target.clamp(min=-5), tokens, bad, [3] * 3, 2, noise, 0.5)
     assert flag() == 1
+    # none is no mistake: a place of the batch without a sequence
+    out, path, accepted = run(cuda_dev, target.clamp(min=-5)[:6], tokens[:6], [[-1, 0, 1], [], [-1, 0, 0]], [3, 0, 3], 2, noise, 0.5)
+    assert flag() == 0 and out[1].eq(-1).all() and path[1].eq(-1).all() and int(accepted[1]) == 0 and out[::2, 0].ge(0).all()
     # 65 nodes, and rows that lie outside
     target, tokens, parents, noise = trees([65, 1], 50, 2, 2)
     out, _, accepted = run(cuda_dev, target, tokens, parents, [65, 1], 2, noise, 0.0)
