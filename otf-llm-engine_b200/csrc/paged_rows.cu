@@ -257,7 +257,7 @@ struct RowsShape {
 struct RowsSmall {
   uint64_t kv_full[10], kv_empty[10], v_landed[10];
   uint64_t q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_done[2];
-  uint64_t item_full[4], item_empty[4];
+  uint64_t item_full[4], item_empty[4], meet_free[2];
   Portion items[4];  // the run's next ones, from the warp that fetches keys to all others
   RunStart run;
   int64_t sums[16];
@@ -452,7 +452,7 @@ struct RowState {
 // The scores of the keys' groups of 32, c0 .. c1 - 1 of a chunk's four, become probabilities: one 16-bit number each,
 // 16 columns a group, or (TWO) the rounding and the rest, 16 columns of each in the place of 32 scores.  Loops over
 // the groups, the scores fetched twice: with all 128 in registers the code was four times as long and its fetching
-// took more time than the second look (prompts 2.94 ms against FIGURE).
+// took more time than the second look (prompts of 64 heads, some 16400 rows, 2.94 ms against 2.69).
 template <bool BF, int D, bool TWO, bool TREE, bool EDGE>
 __device__ __forceinline__ void turn_chunk(const RowsArgs& a, uint32_t s_at, uint32_t o_at, int c0, int c1, const RowView& view, int k0,
                                      bool there, RowState& r, uint64_t* half_bar) {
@@ -576,6 +576,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
       mbar_init(smem_u32(&sm.p_full[i]), 4);
       mbar_init(smem_u32(&sm.o_done[i]), 1);
     }
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&sm.meet_free[i]), 8);
     for (int i = 0; i < 4; ++i) {
       mbar_init(smem_u32(&sm.item_full[i]), 1);
       mbar_init(smem_u32(&sm.item_empty[i]), kPrThreads / 32 - 1);
@@ -660,6 +661,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
       }
     }
   }
+  fence_async_shared();  // the units lie where tensor copies go
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -806,9 +808,21 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
     const int piece = lane % P, sub = lane / P;
     uint32_t n[2] = {0, 0}, fill = 0;
     uint32_t turns = 0;  // how often each slot's landing came around, a bit per slot
+    uint32_t meets = 0;
+    bool met = false;    // the portion before uses `meet`
     while (feed.next(it)) {
       const int all = it.rows, fold = it.fold();
-      for (int w = 0; w < (all > 128 ? 2 : 1); ++w) {
+      for (int w = 0; w < 2; ++w) {
+        if (w == 1) {
+          // The second tile lies where the groups of the portion before may still be meeting.  Two barriers in turn:
+          // with one the portion at hand, whose first tile is there, might be through before this warp has looked.
+          if (met) {
+            rows_wait(&sm.meet_free[meets & 1], meets >> 1 & 1u, gave_up);
+            ++meets;
+          }
+          met = all <= 128;
+          if (met) break;
+        }
         if (n[w] > 0) rows_wait(&sm.q_empty[w], (n[w] - 1) & 1u, gave_up);
         ++n[w];
         const int row0 = it.rb * kPrRows + w * 128, rows = min(128, all - w * 128);
@@ -985,7 +999,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
     const int w = warp >> 2, r = tid & 127, quarter = warp & 3;
     const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
     const uint32_t s_at = tmem + lanes + w * 128, o_at = tmem + lanes + kOut + w * 128;
-    uint32_t chunk_count = 0, item_count = 0;
+    uint32_t chunk_count = 0, item_count = 0, meets = 0;
     while (feed.next(it)) {
       const bool pair = it.rows > 128;
       const int fold = it.fold(), size = 128 >> fold, copy = r >> (7 - fold);
@@ -1215,6 +1229,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
             if (two) named_barrier_sync(1, 256);  // before the columns are written again
           }
         }
+        fence_async_shared();  // before the tensor copies that may follow there
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sm.meet_free[meets & 1]));
+        ++meets;
       }
     }
   }
@@ -1378,8 +1396,8 @@ extern "C" OTF_API int otf_paged_attn_rows(const otf_paged_cache* cache, const v
   a.scale = fmaxf(fabsf(scale * otf::kPrLog2e), 0x1p-149f);
   a.sign = scale < 0.0f ? 0x80008000u : 0u;
   // Tensor copies where chunks cut pages into groups of 4 tokens or more (`rest`), in larger boxes as far as they go:
-  // a box costs the copy unit some 40 cycles whatever is in it (pages of 20: 128 boxes of 4 a chunk 5500 cycles, with boxes
-  // of 16 FIGURE).  Else, and for the chunks that are not all there, 16-byte copies.
+  // a box costs the copy unit some 40 cycles whatever is in it (pages of 20, trees of 32 sequences: boxes of 4 alone
+  // 321 us, with boxes of 16 277).  Else, and for the chunks that are not all there, 16-byte copies.
   const int rest = std::gcd((int)a.c.page_size, otf::kPrKeys);
   if (rest >= 4) {
     int box = rest;

@@ -326,3 +326,11 @@ def test_a_tree_as_it_is_used(cuda_dev):
                 x = embed[torch.tensor([trees[b][row - first]], device=dev)].view(1, heads + 2 * kv, dim)
                 assert same(cache.v_pages[at].cpu(), x[0, heads + kv:].cpu())
     assert flag() == 0
+
+
+@pytest.mark.parametrize("dim,dtype", [(128, "fp16"), (64, "bf16")])
+def test_large_and_small_blocks_in_one_run(dim, dtype, cuda_dev):
+    """Blocks of 256 rows, of more and fewer than 128 and of a few, several of each on every SM one after another: what
+    one leaves behind must not reach the next one's queries."""
+    new = [130, 5, 200, 64, 33, 129, 1]
+    check(cuda_dev, [20, 150, 0, 33, 260, 7, 300], new, 16, 192, 96, dim, TYPES[dtype], window=140, sinks=1)
