@@ -1255,17 +1255,12 @@ __global__ void __launch_bounds__(256) k_paged_rows_join(const __grid_constant__
   if (!x.there || r >= x.rows) return;
   const int n = x.last_cta - (int)blockIdx.x + 1;
   auto part = [&](int i) { return (int64_t)(i == 0 ? x.first_part : 2 * ((int)blockIdx.x + i)) * a.part_rows + r; };
-  float M = -INFINITY, L = 0.0f, acc[PL] = {};
-  float2 ml = lane < n ? a.part_ml[part(lane)] : make_float2(-INFINITY, 0.0f);  // of the lane's part among 32
-  M = ml.x;
-  for (int i = lane + 32; i < n; i += 32) M = fmaxf(M, a.part_ml[part(i)].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  for (int base = 0; base < n; base += U) {
-    float y[U][PL];
+  float y[U][PL];
+  auto fetch = [&](int base) {
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const float* z = a.part + part(min(base + k, n - 1)) * D + lane * PL;
+      if (base + k >= n) break;
+      const float* z = a.part + part(base + k) * D + lane * PL;
       if (D == 128) {
         const float4 v = *reinterpret_cast<const float4*>(z);
         y[k][0] = v.x;
@@ -1278,13 +1273,23 @@ __global__ void __launch_bounds__(256) k_paged_rows_join(const __grid_constant__
         y[k][1] = v.y;
       }
     }
+  };
+  fetch(0);  // on their way while the maxima are found
+  float2 ml = lane < n ? a.part_ml[part(lane)] : make_float2(-INFINITY, 0.0f);  // of the lane's part among 32
+  float M = ml.x, L = 0.0f, acc[PL] = {};
+  for (int i = lane + 32; i < n; i += 32) M = fmaxf(M, a.part_ml[part(i)].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  for (int base = 0; base < n; base += U) {
+    if (base) fetch(base);
     if (base && (base & 31) == 0) ml = base + lane < n ? a.part_ml[part(base + lane)] : make_float2(-INFINITY, 0.0f);
     const float mine = ml.x == -INFINITY ? 0.0f : pr_ex2(ml.x - M);
 #pragma unroll
     for (int k = 0; k < U; ++k) {
+      if (base + k >= n) break;
       const float f = __shfl_sync(0xffffffffu, mine, (base + k) & 31), l = __shfl_sync(0xffffffffu, ml.y, (base + k) & 31);
       const float m = __shfl_sync(0xffffffffu, ml.x, (base + k) & 31);
-      if (base + k < n && m != -INFINITY) {
+      if (m != -INFINITY) {  // else nothing that the row sees, or nothing at all, lies there
         L = fmaf(l, f, L);
 #pragma unroll
         for (int j = 0; j < PL; ++j) acc[j] = fmaf(y[k][j], f, acc[j]);
