@@ -182,6 +182,12 @@ struct __align__(16) Portion {
   Keys k;
   int pad;
   __device__ __forceinline__ bool whole() const { return c0 == 0 && c1 == k.chunks; }
+  // The ring's order, that of the products: of m chunks the j-th one's keys and values are these fills.  With groups that
+  // share chunks K0 V0 K1 V1 ..., with groups that take turns K0 K1 V0 K2 V1 ...: what is fetched later is held shorter.
+  __device__ __forceinline__ uint32_t key_fill(int j) const { return rows > 128 || j == 0 ? 2 * j : 2 * j - 1; }
+  __device__ __forceinline__ uint32_t value_fill(int j) const {
+    return rows > 128 || j + 1 == c1 - c0 ? 2 * j + 1 : 2 * j + 2;
+  }
   // Copies of the rows: 1 << fold.
   __device__ __forceinline__ int fold() const { return rows <= 32 ? 2 : rows <= 64 ? 1 : 0; }
 };
@@ -731,21 +737,23 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
     if (next_portion(true)) {
       const int64_t v_from_k = a.c.v - a.c.k;
       Asked next = ask(it.c0);
-      for (int v = it.c0;; fill += 2) {
+      for (int v = it.c0;;) {
         const bool odd = some_do_not_see(it.k, v, a.sinks);
         const int g = it.g;
         const Asked x = next;
+        const uint32_t kf = fill + it.key_fill(v - it.c0), vf = fill + it.value_fill(v - it.c0);
         bool more = true;
         if (++v == it.c1) {
+          fill += 2 * (it.c1 - it.c0);
           more = next_portion(false);
           v = it.c0;
         }
         if (more) next = ask(v);
-        const uint32_t ks = fill % NS, vs = (fill + 1) % NS;
+        const uint32_t ks = kf % NS, vs = vf % NS;
         if (x.boxes) {
           // the first warp the keys, the second one the values
           const uint32_t slot = w ? vs : ks, bar = smem_u32(w && odd ? &sm.v_landed[slot] : &sm.kv_full[slot]);
-          empty(fill + w);
+          empty(w ? vf : kf);
           __syncwarp();
           if (lane == 0) {
             mbar_arrive_expect_tx(bar, S::tile);
@@ -776,8 +784,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
             }
           }
         } else {
-          empty(fill);
-          empty(fill + 1);
+          empty(kf);
+          empty(vf);
           const uint16_t* const base = a.c.k + g * a.c.head_stride + piece * 8;
           const uint32_t dst = ring + ks * S::tile + to, across = (vs - ks) * S::tile;
 #pragma unroll
@@ -857,9 +865,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sm.q_full[w]));
       }
-      for (int v = it.c0; v < it.c1; ++v, fill += 2) {
+      for (int v = it.c0; v < it.c1; ++v) {
         if (!some_do_not_see(it.k, v, a.sinks)) continue;
-        const uint32_t slot = (fill + 1) % NS;
+        const uint32_t slot = (fill + it.value_fill(v - it.c0)) % NS;
         rows_wait(&sm.v_landed[slot], turns >> slot & 1u, gave_up);
         turns ^= 1u << slot;
         uint4* x = reinterpret_cast<uint4*>(smem + S::ring + slot * S::tile);
@@ -880,6 +888,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
         __syncwarp();
         if (lane == 0) mbar_arrive_n(smem_u32(&sm.kv_full[slot]), 64);
       }
+      fill += 2 * (it.c1 - it.c0);
     }
   } else if (warp == kPrMma) {
     // The whole warp keeps count, one lane issues: descriptors then are a warp's, not a lane's.
@@ -967,30 +976,33 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
           }
         }
       } else {
-        for (int j = 0; j < min(m, 2); ++j) {
-          filled(fill + 2 * j);
-          scores(j, q0, fill + 2 * j);
-          release(fill + 2 * j);
-        }
+        auto next_scores = [&](int j) {
+          const uint32_t f = fill + it.key_fill(j);
+          filled(f);
+          scores(j & 1, q0, f);
+          release(f);
+        };
+        next_scores(0);
+        if (m > 1) next_scores(1);
         if (m <= 2) commit(&sm.q_empty[0]);
 #pragma unroll 1
-        for (int j = 0; j < m; ++j, fill += 2) {
+        for (int j = 0; j < m; ++j) {
           const int w = j & 1;
-          filled(fill + 1);
+          const uint32_t f = fill + it.value_fill(j);
+          filled(f);
           ready(w, 0);
-          outputs_two(w, fill + 1, 0, j > 1);
+          outputs_two(w, f, 0, j > 1);
           ready(w, 1);
-          outputs_two(w, fill + 1, 1, 1u);
-          release(fill + 1);
+          outputs_two(w, f, 1, 1u);
+          release(f);
           if (j + 2 < m) {
-            filled(fill + 4);
-            scores(w, q0, fill + 4);
-            release(fill + 4);
+            next_scores(j + 2);
             if (j + 3 == m) commit(&sm.q_empty[0]);
           } else {
             commit(&sm.o_done[w]);
           }
         }
+        fill += 2 * m;
       }
     }
     __syncwarp();
