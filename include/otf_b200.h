@@ -555,7 +555,7 @@ OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* q, int64_t 
  * Sequences with a negative length are left as they are, and so are, with the flag raised, those whose rows do
  * not lie in [0, n], do not fit the pages or are more than 64 nodes; rows behind the last sequence, too.  Tokens
  * of a page not in [0, n_pages) read as zeros and raise the flag.  scale as in otf_paged_attn.  n heads /
- * kv_heads at most 2^31 - 1.  workspace: otf_paged_attn_rows_workspace_bytes(...), 256-byte aligned, need not be
+ * kv_heads below 2^31 - 256.  workspace: otf_paged_attn_rows_workspace_bytes(...), 256-byte aligned, need not be
  * cleared; two calls that may run at the same time need one each.  Beside otf_paged_attn, which takes as many
  * newest tokens, 16 at most, of every sequence and adds up weights.
  */

@@ -118,7 +118,7 @@ __device__ __forceinline__ RowRange range_of(const RowsArgs& a, int b, bool repo
 // key on, then those from chunk `low_chunk` on.  From key `full` on a row may not see a key that another does,
 // and so below key `low_full`, from the sinks on.
 struct Keys {
-  int t0, t1;  // its first and last token
+  int t0, t1;  // the first and last token whose keys and rows it has
   int low, low_full, full, end, sink_chunks, low_chunk, chunks;
 };
 template <bool TREE>
@@ -136,6 +136,10 @@ __device__ __forceinline__ Keys keys_of(const RowsArgs& a, const RowRange& s, in
   }
   k.full = TREE ? s.len : s.len + k.t0 + 1;
   k.end = TREE ? s.len + s.tokens : s.len + k.t1 + 1;
+  if (TREE) {  // all nodes' keys are there for every block
+    k.t0 = 0;
+    k.t1 = s.tokens - 1;
+  }
   k.chunks = k.sink_chunks + (k.end + kPrKeys - 1) / kPrKeys - k.low_chunk;
   return k;
 }
@@ -263,7 +267,7 @@ struct RowsShape {
 struct RowsSmall {
   uint64_t kv_full[10], kv_empty[10], v_landed[10];
   uint64_t q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_done[2];
-  uint64_t item_full[4], item_empty[4], meet_free[2];
+  uint64_t item_full[4], item_empty[4], meet_free[2], both;
   Portion items[4];  // the run's next ones, from the warp that fetches keys to all others
   RunStart run;
   int64_t sums[16];
@@ -565,7 +569,11 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_trigger();
   if (smem_u32(smem) & 1023u) {  // the swizzles count on it
-    report_bad_rows();
+    pdl_wait();
+    if (tid == 0) {
+      report_bad_rows();
+      a.shared[blockIdx.x] = SharedItem{};
+    }
     return;
   }
   if (tid == 0) {
@@ -583,6 +591,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
       mbar_init(smem_u32(&sm.o_done[i]), 1);
     }
     for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&sm.meet_free[i]), 8);
+    mbar_init(smem_u32(&sm.both), 8);
     for (int i = 0; i < 4; ++i) {
       mbar_init(smem_u32(&sm.item_full[i]), 1);
       mbar_init(smem_u32(&sm.item_empty[i]), kPrThreads / 32 - 1);
@@ -1011,7 +1020,14 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
     const int w = warp >> 2, r = tid & 127, quarter = warp & 3;
     const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
     const uint32_t s_at = tmem + lanes + w * 128, o_at = tmem + lanes + kOut + w * 128;
-    uint32_t chunk_count = 0, item_count = 0, meets = 0;
+    uint32_t chunk_count = 0, item_count = 0, meets = 0, boths = 0;
+    // The groups' eight warps meet (a wait that ends, as all others).
+    auto both = [&] {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sm.both));
+      rows_wait(&sm.both, boths++ & 1u, gave_up);
+      __syncwarp();
+    };
     while (feed.next(it)) {
       const bool pair = it.rows > 128;
       const int fold = it.fold(), size = 128 >> fold, copy = r >> (7 - fold);
@@ -1076,7 +1092,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
         ++item_count;
         tc_fence_after_sync();
       }
-      if (!pair && it.c1 - it.c0 > 1) named_barrier_sync(1, 256);  // the other group's values have been looked through, too
+      if (!pair && it.c1 - it.c0 > 1) both();  // the other group's values have been looked through, too
       const bool whole = it.whole(), odd = *(volatile int*)&sm.odd;
       const int64_t part = (int64_t)(2 * blockIdx.x + (it.first ? 0 : 1)) * a.part_rows + (row - it.rb * kPrRows);
       uint16_t* const to = a.out + (it.s.r0 + (int64_t)t) * a.ldo + (int64_t)(it.g * a.rep + row - t * a.rep) * D;
@@ -1153,7 +1169,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
                     *reinterpret_cast<float4*>(meet + (mine * rows_here + lr) * cols + ((c + i) ^ ((lr & 7) << 2))) =
                         make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
               }
-            named_barrier_sync(1, 256);
+            both();
 #pragma unroll 1
             for (int e = tid * 4; e < rows_here * cols; e += 256 * 4) {
               const int rr = e / cols, c = e - rr * cols;
@@ -1184,7 +1200,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
                 if (c0 + c == 0) a.part_ml[at] = make_float2(mx, l);
               }
             }
-            named_barrier_sync(1, 256);  // before the columns are written again
+            both();  // before the columns are written again
           }
         } else if (w == 0 || two) {
           auto place = [&](int row, int c) {  // of four columns, turned by the row against bank conflicts
@@ -1207,7 +1223,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
                 }
               if (half == 0) sm.ml[r] = make_float2(state.m, state.l);
             }
-            if (two) named_barrier_sync(1, 256);
+            if (two) both();
             if (w == 0) {
               if (half == 0 && two) {
                 const float2 ml = sm.ml[r];
@@ -1238,7 +1254,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
                 }
               if (!whole && there && half == 0) a.part_ml[part] = make_float2(state.m, state.l);
             }
-            if (two) named_barrier_sync(1, 256);  // before the columns are written again
+            if (two) both();  // before the columns are written again
           }
         }
         fence_async_shared();  // before the tensor copies that may follow there
@@ -1249,6 +1265,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
     }
   }
 
+  if (*gave_up) {  // what is still on its way ends within microseconds
+    const uint64_t t0 = global_ns();
+    while (global_ns() - t0 < 2000000ull) __nanosleep(1000);
+  }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -1328,7 +1348,7 @@ static RowsSpace rows_space(int64_t n, int64_t rep, int64_t D) {
 }
 static bool rows_limits(int64_t batch, int64_t n, int64_t heads, int64_t kv_heads, int64_t D) {
   return batch <= kPagedMaxBatch && heads <= 65535 && kv_heads <= 1024 && (D == 64 || D == 128) && n <= INT32_MAX &&
-         n * (heads / kv_heads) <= INT32_MAX;
+         n * (heads / kv_heads) <= INT32_MAX - kPrRows;
 }
 
 template <bool BF, int D, bool TREE>

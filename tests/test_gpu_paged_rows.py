@@ -334,3 +334,21 @@ def test_large_and_small_blocks_in_one_run(dim, dtype, cuda_dev):
     one leaves behind must not reach the next one's queries."""
     new = [130, 5, 200, 64, 33, 129, 1]
     check(cuda_dev, [20, 150, 0, 33, 260, 7, 300], new, 16, 192, 96, dim, TYPES[dtype], window=140, sinks=1)
+
+
+def test_a_block_of_one_node_does_not_see_its_siblings(cuda_dev):
+    """33 nodes of 8 query heads: the last block has one node's rows alone, and the others' values are odd."""
+    cache, _, table, g = make(cuda_dev, [100 + 33], 16, 1, 128, torch.float16, room=[140], seed=9)
+    cache.lengths.fill_(100)
+    q = torch.randn(33, 8, 128, generator=g).half().to(cuda_dev)
+    parents = torch.full((33,), -1, dtype=torch.int32, device=cuda_dev)
+    plain = cache.attend_tree(q, parents)
+    for place in (100, 131):
+        at = ref.place(table, 16, 0, place)
+        kept = cache.v_pages[at].clone()
+        cache.v_pages[at][:] = float("nan")
+        got = cache.attend_tree(q, parents)
+        cache.v_pages[at] = kept
+        others = [t for t in range(33) if t != place - 100]
+        assert same(got[others], plain[others]) and bool(got[place - 100].isnan().all())
+    assert flag() == 0

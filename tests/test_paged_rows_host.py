@@ -35,7 +35,7 @@ BAD_ROWS = [(dict(cache=None), INVALID), (dict(q=None), INVALID), (dict(out=None
             (dict(parents=FAKE, window=63), INVALID), (dict(scale=float("nan")), INVALID), (dict(scale=float("inf")), INVALID),
             (dict(scale=3e38), INVALID), (dict(starts=None, n=13), INVALID), (dict(ws=None), INVALID), (dict(ws=FAKE + 16), INVALID),
             (dict(bytes=1000), INVALID), (dict(starts=None, parents=FAKE, n=195), UNSUPPORTED), (dict(n=1 << 31), UNSUPPORTED),
-            (dict(n=(1 << 31) // 4, out=FAKE << 30), UNSUPPORTED), (dict(c_head_dim=96), UNSUPPORTED), (dict(c_batch=4097), UNSUPPORTED),
+            (dict(n=(1 << 31) // 4 - 60, out=FAKE << 30), UNSUPPORTED), (dict(c_head_dim=96), UNSUPPORTED), (dict(c_batch=4097), UNSUPPORTED),
             (dict(c_dtype=2), UNSUPPORTED), (dict(c_lengths=None), INVALID)]
 
 
