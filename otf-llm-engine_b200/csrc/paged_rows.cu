@@ -278,8 +278,10 @@ struct RowsSmall {
 };
 static_assert(sizeof(RowsSmall) <= kPrSmall, "");
 
-// A bounded wait: after a second the CTA gives up, raises the flag and runs to its end without waiting.
-__device__ __forceinline__ void rows_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
+// A bounded wait: after a second the CTA gives up, raises the flag and runs to its end without waiting.  The warp that
+// fetches queries waits for whole items, of up to millions of chunks: a minute.
+constexpr uint64_t kPrWait = 1000000000ull, kPrLongWait = 60 * kPrWait;
+__device__ __forceinline__ void rows_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up, uint64_t most = kPrWait) {
   const uint32_t at = smem_u32(bar);
   if (mbar_try_wait(at, parity)) return;
   const uint64_t t0 = global_ns();
@@ -287,7 +289,7 @@ __device__ __forceinline__ void rows_wait(uint64_t* bar, uint32_t parity, volati
 #pragma unroll 1
     for (int i = 0; i < 32; ++i)
       if (mbar_try_wait(at, parity)) return;
-    if (global_ns() - t0 > 1000000000ull) {
+    if (global_ns() - t0 > most) {
       *gave_up = 1;
       report_bad_rows();
     }
@@ -311,9 +313,9 @@ struct Feed {
   volatile int* gave_up;
   uint32_t n = 0;
   __device__ __forceinline__ Feed(RowsSmall& small) : sm(small), gave_up(&small.gave_up) {}
-  __device__ __forceinline__ bool next(Portion& p) {
+  __device__ __forceinline__ bool next(Portion& p, uint64_t most = kPrWait) {
     const uint32_t slot = n & 3;
-    rows_wait(&sm.item_full[slot], n >> 2 & 1u, gave_up);
+    rows_wait(&sm.item_full[slot], n >> 2 & 1u, gave_up, most);
     p = sm.items[slot];
     __syncwarp();
     if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&sm.item_empty[slot]));
@@ -704,8 +706,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
       Asked x;
       x.boxes = a.box && k0 + kPrKeys <= it.k.end && (k0 >= it.k.low || k0 + kPrKeys <= a.sinks);
       if (x.boxes) {
-        const int s = max(k0, (int)((uint32_t)k0 / a.page + lane) * (int)a.page.d);
-        x.key[0] = ask_key(a, it.b, s, s < k0 + kPrKeys);
+        const int64_t first = ((int64_t)((uint32_t)k0 / a.page) + lane) * a.page.d;
+        const bool there = first < k0 + kPrKeys;
+        x.key[0] = ask_key(a, it.b, there ? max(k0, (int)first) : 0, there);
       } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -827,20 +830,20 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
     uint32_t turns = 0;  // how often each slot's landing came around, a bit per slot
     uint32_t meets = 0;
     bool met = false;    // the portion before uses `meet`
-    while (feed.next(it)) {
+    while (feed.next(it, kPrLongWait)) {
       const int all = it.rows, fold = it.fold();
       for (int w = 0; w < 2; ++w) {
         if (w == 1) {
           // The second tile lies where the groups of the portion before may still be meeting.  Two barriers in turn:
           // with one the portion at hand, whose first tile is there, might be through before this warp has looked.
           if (met) {
-            rows_wait(&sm.meet_free[meets & 1], meets >> 1 & 1u, gave_up);
+            rows_wait(&sm.meet_free[meets & 1], meets >> 1 & 1u, gave_up, kPrLongWait);
             ++meets;
           }
           met = all <= 128;
           if (met) break;
         }
-        if (n[w] > 0) rows_wait(&sm.q_empty[w], (n[w] - 1) & 1u, gave_up);
+        if (n[w] > 0) rows_wait(&sm.q_empty[w], (n[w] - 1) & 1u, gave_up, kPrLongWait);
         ++n[w];
         const int row0 = it.rb * kPrRows + w * 128, rows = min(128, all - w * 128);
         unsigned char* tile = smem + w * S::tile + (piece >> 3) * 128 * 128;
@@ -877,7 +880,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
       for (int v = it.c0; v < it.c1; ++v) {
         if (!some_do_not_see(it.k, v, a.sinks)) continue;
         const uint32_t slot = (fill + it.value_fill(v - it.c0)) % NS;
-        rows_wait(&sm.v_landed[slot], turns >> slot & 1u, gave_up);
+        rows_wait(&sm.v_landed[slot], turns >> slot & 1u, gave_up, kPrLongWait);
         turns ^= 1u << slot;
         uint4* x = reinterpret_cast<uint4*>(smem + S::ring + slot * S::tile);
         uint32_t high = 0;  // an exponent of ones plus one carries into the sign's place

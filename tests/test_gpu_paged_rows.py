@@ -352,3 +352,40 @@ def test_a_block_of_one_node_does_not_see_its_siblings(cuda_dev):
         others = [t for t in range(33) if t != place - 100]
         assert same(got[others], plain[others]) and bool(got[place - 100].isnan().all())
     assert flag() == 0
+
+
+@pytest.mark.parametrize("page", [2, 4, 6, 12, 24, 40, 48, 96, 136, 200, 256, 1000])
+def test_page_sizes(page, cuda_dev):
+    """Chunks that cut pages into groups of 4, 8, 16 and more, of fewer, and pages longer than chunks."""
+    check(cuda_dev, [700, 13], [3, 140], page, 4, 2, 64, torch.float16, window=400, sinks=5)
+    check(cuda_dev, [530], [7], page, 4, 1, 128, torch.bfloat16, order="head", trees=True)
+
+
+def test_offsets_beyond_32_bits(cuda_dev):
+    """Pools of more than 2^31 values: the same bits as from a small pool."""
+    from otf_llm.paged import PagedKVCache
+    small, _, table, g = make(cuda_dev, [700], 16, 8, 128, torch.float16, room=[720], fill=0.0)
+    small.lengths.fill_(690)
+    n = 140000
+    big = [torch.empty(n, 16, 8, 128, dtype=torch.float16, device=cuda_dev) for _ in range(2)]
+    far = torch.arange(n - 1, n - 1 - 2 * table.shape[1], -2, dtype=torch.int32, device=cuda_dev)[None].contiguous()
+    for pool, of in zip(big, (small.k_pages, small.v_pages)):
+        for j in range(-(-720 // 16)):
+            pool[int(far[0, j])] = of[int(table[0, j])]
+    cache = PagedKVCache(big[0], big[1], far, torch.full((1,), 690, dtype=torch.int32, device=cuda_dev))
+    q = torch.randn(10, 16, 128, generator=g).half().to(cuda_dev)
+    assert same(cache.attend_rows(q, window=500, sinks=20), small.attend_rows(q, window=500, sinks=20))
+    parents = torch.tensor([-1, 0, 1, 0, 3, 3, 2, 0, 1, 8], dtype=torch.int32, device=cuda_dev)
+    assert same(cache.attend_tree(q, parents), small.attend_tree(q, parents))
+    path, accepted = torch.tensor([[1, 8, 9]], dtype=torch.int32, device=cuda_dev), torch.tensor([3], dtype=torch.int32, device=cuda_dev)
+    for c in (cache, small):
+        c.keep(path, accepted)
+        c.lengths.fill_(684)
+    assert same(cache.attend_rows(q), small.attend_rows(q)) and flag() == 0
+
+
+@pytest.mark.parametrize("heads,kv", [(40, 1), (300, 1), (9, 3), (64, 2)])
+def test_head_layouts(heads, kv, cuda_dev):
+    """Ratios of query to KV heads that no tensor copy of queries takes, and more rows of one token than a block."""
+    check(cuda_dev, [150, 3], [2, 9], 16, heads, kv, 64, torch.float16, window=100, sinks=2)
+    check(cuda_dev, [90], [5], 16, heads, kv, 64, torch.bfloat16, trees=True)
