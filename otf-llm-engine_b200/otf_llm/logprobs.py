@@ -44,13 +44,16 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     dev, n, vocab, ld, dtype, top = plan
     if tokens.dtype is not torch.int64 or tokens.device != dev or not tokens.is_contiguous():
         raise ValueError(f"tokens must be contiguous int64 on {dev}, got {tokens.dtype} on {tokens.device}")
-    values, ranks = torch.empty((2, n), dtype=torch.float32, device=dev), torch.empty(n, dtype=torch.int32, device=dev)
-    logprobs, entropy = values.unbind()
-    top_tokens, top_logprobs = torch.empty((n, top), dtype=torch.int64, device=dev), torch.empty((n, top), device=dev, dtype=torch.float32)
+    # the three numbers of a row in one piece of memory
+    values = torch.empty((3, n), dtype=torch.float32, device=dev)
+    logprobs, entropy, ranks = values.unbind()
+    ranks = ranks.view(torch.int32)
+    top_tokens = tokens.new_empty((n, top))
+    top_logprobs = values.new_empty((n, top))
     if n:
         at = values.data_ptr()
         _call(_native.lib().otf_token_logprobs, dev, logits.data_ptr(), ld, dtype, tokens.data_ptr(), n, vocab, top, at, at + 4 * n,
-              ranks.data_ptr(), top_tokens.data_ptr() if top else None, top_logprobs.data_ptr() if top else None)
+              at + 8 * n, top_tokens.data_ptr() if top else None, top_logprobs.data_ptr() if top else None)
     return TokenLogprobs(logprobs, entropy, ranks, top_tokens, top_logprobs)
 
 

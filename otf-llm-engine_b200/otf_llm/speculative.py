@@ -118,11 +118,9 @@ def verify_tree(target_logits: torch.Tensor, tokens: torch.Tensor, parents: torc
             raise ValueError(f"temperature must be 0, or positive and finite, got {one}")
     if pn is None and (each is not None or one > 0):
         raise ValueError("a temperature above 0 needs noise")
-    out = torch.empty((batch, depth + 1), dtype=torch.int64, device=dev)
-    path = torch.empty((batch, depth), dtype=torch.int32, device=dev)
-    accepted = torch.empty(batch, dtype=torch.int32, device=dev)
+    out, path, accepted = tokens.new_empty((batch, depth + 1)), parents.new_empty((batch, depth)), parents.new_empty(batch)
     # a small call's scratch, for this call alone and on its stream
-    ws = torch.empty(bytes_, dtype=torch.uint8, device=dev) if bytes_ else None
+    ws = tokens.new_empty(bytes_ // 8) if bytes_ else None
     _call(_native.lib().otf_verify_tree, dev, pt, ld, ptok, pp, ps, n, pn, seq_n, ld_n, each, one, out.data_ptr(),
           path.data_ptr() if depth else None, accepted.data_ptr(), batch, depth, vocab, ws.data_ptr() if bytes_ else None, bytes_)
     return out, path, accepted
