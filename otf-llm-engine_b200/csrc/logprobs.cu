@@ -13,6 +13,10 @@
 //
 // Bound: the logits are read once.  A row is cut among the warps of a cluster of CTAs (one CTA where there
 // are enough rows), 512 logits at a time, 16 in each lane; their parts meet in the cluster's first CTA.
+//
+// Measured: 2047 rows of 128256 fp32, 1.05 GB, 164 to 183 us = 5.7 to 6.4 TB/s; 1024 rows of 128256 bf16, 0.26 GB, 78 us
+// without a list and 98 to 111 with twenty alternatives: instructions bound it, some 13 a logit, and twice the logits come
+// with every byte; 4 rows of 32000 with five alternatives 9.5 us.
 #include <algorithm>
 #include <cfloat>
 

@@ -14,14 +14,24 @@
 // may cross items, and an item may be shared by several CTAs, which then leave parts that a second
 // kernel joins in order.  Lengths and row ranges are read on the device, so that a step can be captured.
 //
-// A CTA has two groups of four warps that turn scores into probabilities, a thread per row; a warp that
-// issues the matrix products (tcgen05, 128 rows x 128 keys and 128 rows x head_dim, scores, probabilities
-// and outputs in tensor memory); a warp that fetches queries, and four that fetch keys and values through
-// a ring of shared-memory slots by 16-byte asynchronous copies, page by page, whatever the page size is.
-// Blocks of more than 128 rows: the groups have 128 rows each and share every chunk.  Blocks of fewer: the
-// groups have the same rows and every other chunk each, and join at the item's end; and where there are 64 rows
-// or fewer they lie there two or four times, each copy with its own keys of a chunk (its other probabilities are 0),
-// so that all warps have work.
+// A CTA has two groups of four warps that turn scores into probabilities, a thread per row; a warp that issues the matrix
+// products (tcgen05, 128 rows x 128 keys and 128 rows x head_dim, scores, probabilities and outputs in tensor memory); a warp
+// that fetches queries and looks values through; and two that fetch keys and values through a ring of shared-memory slots:
+// by tensor copies, a page at a time, where all of a chunk's keys are there, else by 16-byte copies.  Blocks of more than 128
+// rows: the groups have 128 rows each and share every chunk.  Blocks of fewer: the groups have the same rows and every other
+// chunk each, and join at the item's end; and where there are 64 rows or fewer they lie there two or four times, each copy
+// with its own keys of a chunk (its other probabilities are 0), so that all warps have work.
+//
+// Bound.  Many rows: 4 head_dim flops a row and key on the matrix pipe and one exponential, of which an SM makes 16 a cycle:
+// a chunk's 256 x 128 scores take it as long as their products, 2048 cycles, and the two overlap in part.  Few rows: keys and
+// values are read once, 4 head_dim bytes a token and KV head.  Measured (head_dim 128, 64 heads over 8): 16,382 prompt rows
+// through a window of 4096, 2.20 TFLOP, 2.3 to 2.5 ms = 880 to 950 TFLOP/s at the power limit; a token of each of 64 sequences
+// through such a window, 0.90 GB, 166 to 208 us = 4.3 to 5.4 TB/s; trees of 8 to 64 nodes of 32 sequences on up to 8190
+// tokens, 0.2 TFLOP and 0.6 GB, 245 to 287 us; one token through a window of 1024 (32 heads) 13.5 us.
+//
+// The products of one thread run in the order of their issue: scores that overwrite a chunk's probabilities wait for its
+// outputs, and a chunk's scores are complete after the outputs of the chunk before (nothing else guards either).
+// Halves of a chunk whose scores are there ahead of time (64 keys a product) were slower: 2.76 against 2.44 ms on the prompts.
 #include <cuda.h>
 
 #include <algorithm>
@@ -44,7 +54,9 @@ constexpr int kPrGrid = 148;      // a CTA on each SM
 constexpr int kPrMma = 8, kPrQuery = 9, kPrLoad = 10;  // warps that issue products, fetch queries, and two that fetch keys and values
 constexpr int kPrThreads = 384;
 constexpr int kPrMaxNodes = 64;
-constexpr int kPrItemUnits = 2;   // what an item's start and end cost, in chunks
+// What an item's start and end cost, in chunks.  With 2, 3 and 4: a batch's step (as above) 194, 188 and 185 us, trees 266,
+// 265 and 268, prompts 2.50, 2.51 and 2.52 ms.
+constexpr int kPrItemUnits = 3;
 constexpr float kPrLog2e = 1.4426950408889634f;
 
 // Set when a sequence does not fit its pages, names a page outside the pool, or has rows or parents out of range.
@@ -492,8 +504,7 @@ __device__ __forceinline__ void turn_chunk(const RowsArgs& a, uint32_t s_at, uin
     const float mx = fmaxf(r.m, top), f = r.m == -INFINITY ? 0.0f : pr_ex2(r.m - mx);
     r.m = mx;
     r.l *= f;
-    // the scores of a chunk are complete after the outputs of the one before it
-    if (r.any)
+    if (r.any)  // the outputs of the chunk before are complete, as this one's scores are
 #pragma unroll 1
       for (int c = 0; c < D; c += 16) {
         uint32_t x[16];
