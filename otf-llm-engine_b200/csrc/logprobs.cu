@@ -167,13 +167,14 @@ __device__ __forceinline__ void lp_values(const LpRaw<T>& raw, float (&v)[16]) {
     }
   }
 }
-// The largest float below x, the smallest above it (x itself for infinities and NaN).
-__device__ __forceinline__ float lp_below(float x) { return x > -INFINITY ? nextafterf(x, -INFINITY) : x; }
+// The smallest float above x (x itself for an infinity or NaN).
 __device__ __forceinline__ float lp_above(float x) { return x < INFINITY ? nextafterf(x, INFINITY) : x; }
-// 1 where x > y, else 0.
+// 1 where x > y, or (EQUAL) x >= y, else 0.
+template <bool EQUAL>
 __device__ __forceinline__ float lp_greater(float x, float y) {
   float r;
-  asm("set.gt.f32.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  if (EQUAL) asm("set.ge.f32.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  else asm("set.gt.f32.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
   return r;
 }
 // How many of a lane's 16 logits are larger than `than`, or (EQUAL) as large: in two halves.
@@ -181,9 +182,8 @@ template <int T, bool EQUAL>
 __device__ __forceinline__ float2 lp_ahead(const LpRaw<T>& raw, const float (&v)[16], float than) {
   float2 n = make_float2(0.0f, 0.0f);
   if (T == 0) {
-    const float y = EQUAL ? lp_below(than) : than;
 #pragma unroll
-    for (int j = 0; j < 16; j += 2) add_two(n.x, n.y, lp_greater(v[j], y), lp_greater(v[j + 1], y));
+    for (int j = 0; j < 16; j += 2) add_two(n.x, n.y, lp_greater<EQUAL>(v[j], than), lp_greater<EQUAL>(v[j + 1], than));
   } else if (T == 1) {
     const __half2 y = __float2half2_rn(than);  // exact: it is one of the row's
     __half2 sum = __float2half2_rn(0.0f);

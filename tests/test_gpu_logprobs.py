@@ -145,3 +145,24 @@ def test_captured_and_on_a_stream(cuda_dev):
     side.synchronize()
     for a, b in zip(held, token_logprobs(y.to(cuda_dev), torch.tensor(other, device=cuda_dev), top=4)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("vocab,at", [(1500, (600, 1400, 0, 511, 512)), (32000, (31999, 17001, 513, 4097, 16384))])
+def test_ranks_of_masked_tokens_behind_the_first_logits(vocab, at, dtype, cuda_dev):
+    """Tokens of -inf and NaN, which counts as -inf, in every part of a row: all that is larger and the masked ones
+    of lower indexes come before them, wherever those lie."""
+    x, _ = logits(len(at), vocab, vocab, ALL[dtype])
+    x[:, 1::2] = -math.inf
+    x[1:, 2::6] = math.nan
+    x[2] = -math.inf
+    for r, token in enumerate(at):
+        x[r, token] = math.nan if r % 2 else -math.inf
+    if not x[2].isfinite().any():
+        x[2, 3] = 1.0
+    check(cuda_dev, x, list(at), 3)
+    # and of tokens that are as large as many others
+    y = torch.full((len(at), vocab), torch.finfo(ALL[dtype]).min, dtype=ALL[dtype])
+    y[:, ::3] = 0.0
+    y[:, 1::3] = -0.0
+    check(cuda_dev, y, list(at), 3)
