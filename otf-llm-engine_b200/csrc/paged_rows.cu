@@ -1193,8 +1193,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
 #pragma unroll 4
               for (int k = 0; k < parts; ++k) {
                 const float2 ml = sm.ml[k * size + rr];
-                const float f = ml.x == -INFINITY ? 0.0f : pr_ex2(ml.x - mx);
-                if (f != 0.0f || odd) {
+                // A part without a key that the row sees holds nothing, whatever its outputs are, but for what the first one
+                // was given back; one whose keys are all NaN has no maximum either, and its sum says so.
+                if (ml.x != -INFINITY || ml.y != 0.0f || (odd && k == 0)) {
+                  const float f = ml.x == -INFINITY ? 0.0f : pr_ex2(ml.x - mx);
                   const float4 y = *reinterpret_cast<const float4*>(meet + (k * rows_here + rr) * cols + (c ^ ((rr & 7) << 2)));
                   l = fmaf(ml.y, f, l);
                   o[0] = fmaf(y.x, f, o[0]);
@@ -1335,7 +1337,7 @@ __global__ void __launch_bounds__(256) k_paged_rows_join(const __grid_constant__
       if (base + k >= n) break;
       const float f = __shfl_sync(0xffffffffu, mine, (base + k) & 31), l = __shfl_sync(0xffffffffu, ml.y, (base + k) & 31);
       const float m = __shfl_sync(0xffffffffu, ml.x, (base + k) & 31);
-      if (m != -INFINITY) {  // else nothing that the row sees, or nothing at all, lies there
+      if (m != -INFINITY || l != 0.0f) {  // else nothing that the row sees, or nothing at all, lies there (l of NaN keys alone is one)
         L = fmaf(l, f, L);
 #pragma unroll
         for (int j = 0; j < PL; ++j) acc[j] = fmaf(y[k][j], f, acc[j]);

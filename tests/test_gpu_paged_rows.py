@@ -389,3 +389,35 @@ def test_head_layouts(heads, kv, cuda_dev):
     """Ratios of query to KV heads that no tensor copy of queries takes, and more rows of one token than a block."""
     check(cuda_dev, [150, 3], [2, 9], 16, heads, kv, 64, torch.float16, window=100, sinks=2)
     check(cuda_dev, [90], [5], 16, heads, kv, 64, torch.bfloat16, trees=True)
+
+
+NAN_KEYS = [
+    # cached tokens, new rows, heads, kv, dim, window, sinks, the odd key's place; 32 keys of a chunk at a time for 32 rows
+    # and fewer, 64 for 64, one CTA or many
+    (96, 1, 4, 1, 128, None, 0, 96), (95, 1, 4, 1, 128, None, 0, 95), (0, 1, 8, 1, 64, None, 0, 0), (32, 1, 1, 1, 64, None, 0, 32),
+    (128, 1, 4, 1, 128, None, 0, 128), (256, 1, 4, 2, 64, None, 0, 256), (64, 9, 4, 1, 128, None, 0, 64), (5888, 1, 8, 1, 128, None, 0, 5888),
+    (5888, 20, 4, 1, 64, None, 0, 5888), (640, 30, 4, 1, 128, None, 0, 640), (384, 60, 4, 1, 64, None, 0, 384),
+    (900, 3, 8, 2, 128, 100, 1, 0), (2000, 9, 8, 1, 64, 33, 1, 0), (700, 40, 4, 1, 128, 64, 1, 0)]
+
+
+@pytest.mark.parametrize("faint", [False, True])
+@pytest.mark.parametrize("length,new,heads,kv,dim,window,sinks,place", NAN_KEYS)
+def test_a_nan_key_reaches_every_row_that_sees_it(length, new, heads, kv, dim, window, sinks, place, faint, cuda_dev):
+    """Also where it is the only key that a row sees of those that are looked at together, or (faint) where the others
+    among them weigh nothing beside the rest."""
+    cache, _, table, g = make(cuda_dev, [length + new], 16, kv, dim, torch.float16, room=[length + new + 1], seed=4)
+    cache.lengths.fill_(length)
+    q = torch.rand(new, heads, dim, generator=g).half() + 1
+    q = q.to(cuda_dev)
+    if faint:
+        for s in range(place // 32 * 32, min(place // 32 * 32 + 32, length + new)):
+            cache.k_pages[ref.place(table, 16, 0, s)] = -120.0
+    plain = cache.attend_rows(q, window=window, sinks=sinks)
+    cache.k_pages[ref.place(table, 16, 0, place)][:, dim // 2] = float("nan")
+    got = cache.attend_rows(q, window=window, sinks=sinks)
+    assert flag() == 0
+    for t in range(new):
+        if place in rows.seen(length, t, window, sinks):
+            assert bool(got[t].isnan().all()), t
+        else:
+            assert same(got[t], plain[t]), t
