@@ -286,7 +286,9 @@ struct RowsSmall {
   float2 ml[256];
   uint32_t tmem;
   int gave_up;   // a wait ran out: no more waiting
-  int odd;       // an infinity or NaN was taken out of some values
+  // Slot n & 7 holds n where an infinity or NaN was taken out of values of the run's n-th portion.  Any warp is at most four
+  // portions ahead of another (`items`), so that no slot is written for a later portion while an earlier one's is read.
+  uint32_t odd[8];
 };
 static_assert(sizeof(RowsSmall) <= kPrSmall, "");
 
@@ -610,7 +612,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
       mbar_init(smem_u32(&sm.item_empty[i]), kPrThreads / 32 - 1);
     }
     mbar_fence_init();
-    sm.gave_up = sm.odd = 0;
+    sm.gave_up = 0;
+    for (int i = 0; i < 8; ++i) sm.odd[i] = 0;
   }
   if (warp == kPrMma) {
     tmem_alloc(smem_u32(&sm.tmem), 512);
@@ -906,7 +909,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
             const uint4 y = x[i];
             x[i] = make_uint4(without_odd2<BF>(y.x), without_odd2<BF>(y.y), without_odd2<BF>(y.z), without_odd2<BF>(y.w));
           }
-          *(volatile int*)&sm.odd = 1;
+          *(volatile uint32_t*)&sm.odd[feed.n & 7] = feed.n;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive_n(smem_u32(&sm.kv_full[slot]), 64);
@@ -1107,7 +1110,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
         tc_fence_after_sync();
       }
       if (!pair && it.c1 - it.c0 > 1) both();  // the other group's values have been looked through, too
-      const bool whole = it.whole(), odd = *(volatile int*)&sm.odd;
+      auto any_odd = [&] { return *(volatile uint32_t*)&sm.odd[feed.n & 7] == feed.n; };
+      const bool whole = it.whole(), odd = __any_sync(0xffffffffu, any_odd());  // the warp goes one way: what it gives back takes all lanes
       const int64_t part = (int64_t)(2 * blockIdx.x + (it.first ? 0 : 1)) * a.part_rows + (row - it.rb * kPrRows);
       uint16_t* const to = a.out + (it.s.r0 + (int64_t)t) * a.ldo + (int64_t)(it.g * a.rep + row - t * a.rep) * D;
       // Columns [c, c + 32) of the warp's rows.  Four lanes turn their rows' 16-byte pieces, so that they write 64 bytes of
@@ -1184,6 +1188,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
                         make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
               }
             both();
+            const bool given = any_odd();  // a group without chunks only now knows
 #pragma unroll 1
             for (int e = tid * 4; e < rows_here * cols; e += 256 * 4) {
               const int rr = e / cols, c = e - rr * cols;
@@ -1195,7 +1200,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
                 const float2 ml = sm.ml[k * size + rr];
                 // A part without a key that the row sees holds nothing, whatever its outputs are, but for what the first one
                 // was given back; one whose keys are all NaN has no maximum either, and its sum says so.
-                if (ml.x != -INFINITY || ml.y != 0.0f || (odd && k == 0)) {
+                if (ml.x != -INFINITY || ml.y != 0.0f || (given && k == 0)) {
                   const float f = ml.x == -INFINITY ? 0.0f : pr_ex2(ml.x - mx);
                   const float4 y = *reinterpret_cast<const float4*>(meet + (k * rows_here + rr) * cols + (c ^ ((rr & 7) << 2)));
                   l = fmaf(ml.y, f, l);

@@ -421,3 +421,33 @@ def test_a_nan_key_reaches_every_row_that_sees_it(length, new, heads, kv, dim, w
             assert bool(got[t].isnan().all()), t
         else:
             assert same(got[t], plain[t]), t
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("lengths,new,heads,kv,dim,window,sinks", [
+    ([(61 * b) % 200 + 60 for b in range(48)], [3] * 48, 8, 4, 128, 40, 0),          # whose first keys no row sees, one chunk or two
+    ([(61 * b) % 300 for b in range(40)], [1 + 7 * b % 40 for b in range(40)], 16, 8, 64, 70, 3),
+    ([(47 * b) % 500 for b in range(30)], [(30, 60, 150, 9)[b % 4] for b in range(30)], 32, 16, 128, 130, 1)])
+def test_odd_values_of_one_sequence_leave_all_others(lengths, new, heads, kv, dim, window, sinks, dtype, cuda_dev):
+    """Many items on every SM, some of them with infinities among values that not all of their rows see."""
+    cache, _, table, g = make(cuda_dev, [n + t for n, t in zip(lengths, new)], 16, kv, dim, TYPES[dtype],
+                              room=[n + t + 1 for n, t in zip(lengths, new)], seed=6)
+    cache.lengths.copy_(torch.tensor(lengths, dtype=torch.int32))
+    q = torch.randn(sum(new), heads, dim, generator=g).to(TYPES[dtype]).to(cuda_dev)
+    starts = torch.tensor([0] + new).cumsum(0).to(torch.int32).to(cuda_dev)
+    plain = cache.attend_rows(q, starts=starts, window=window, sinks=sinks)
+    places = {b: lengths[b] + new[b] // 2 for b in range(0, len(new), 3)}
+    at = {b: ref.place(table, 16, b, s) for b, s in places.items()}
+    for b, (page, place) in at.items():
+        cache.v_pages[page, place, b % kv, b % dim] = float("inf")
+    calls = [cache.attend_rows(q, starts=starts, window=window, sinks=sinks) for _ in range(4)]
+    assert flag() == 0
+    want_odd = torch.zeros_like(plain, dtype=torch.bool)
+    rep = heads // kv
+    for b, s in places.items():
+        for t in range(new[b]):
+            if s in rows.seen(lengths[b], t, window, sinks):
+                want_odd[int(starts[b]) + t, b % kv * rep:(b % kv + 1) * rep, b % dim] = True
+    for got in calls:
+        assert torch.equal(~got.isfinite(), want_odd)
+        assert same(torch.where(want_odd, 0, got), torch.where(want_odd, 0, plain))
