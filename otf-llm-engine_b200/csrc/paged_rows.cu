@@ -293,21 +293,24 @@ struct RowsSmall {
 static_assert(sizeof(RowsSmall) <= kPrSmall, "");
 
 // A bounded wait: after a second the CTA gives up, raises the flag and runs to its end without waiting.  The warp that
-// fetches queries waits for whole items, of up to millions of chunks: a minute.
+// fetches queries waits for whole items, of up to millions of chunks: a minute.  For a whole warp, whose lanes go on together:
+// what follows are instructions of all of them.
 constexpr uint64_t kPrWait = 1000000000ull, kPrLongWait = 60 * kPrWait;
 __device__ __forceinline__ void rows_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up, uint64_t most = kPrWait) {
   const uint32_t at = smem_u32(bar);
-  if (mbar_try_wait(at, parity)) return;
-  const uint64_t t0 = global_ns();
-  while (!*gave_up) {
+  bool there = mbar_try_wait(at, parity);
+  if (!there) {
+    const uint64_t t0 = global_ns();
+    while (!there && !*gave_up) {
 #pragma unroll 1
-    for (int i = 0; i < 32; ++i)
-      if (mbar_try_wait(at, parity)) return;
-    if (global_ns() - t0 > most) {
-      *gave_up = 1;
-      report_bad_rows();
+      for (int i = 0; i < 32 && !there; ++i) there = mbar_try_wait(at, parity);
+      if (!there && global_ns() - t0 > most) {
+        *gave_up = 1;
+        report_bad_rows();
+      }
     }
   }
+  __syncwarp();
 }
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int x, int y, int z, int u, uint32_t mbar) {
@@ -334,7 +337,8 @@ struct Feed {
     __syncwarp();
     if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&sm.item_empty[slot]));
     ++n;
-    return p.c1 > p.c0 && !*gave_up;
+    // one answer for the warp: where a lane has given up, the lanes may hold different portions
+    return !__any_sync(0xffffffffu, *gave_up) && p.c1 > p.c0;
   }
 };
 
@@ -741,7 +745,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_paged_rows(const __grid_const
     uint32_t found = 0;
     auto next_portion = [&](bool begin) -> bool {
       if (w) return feed.next(it);
-      const bool more = begin ? walk.begin() : walk.next();
+      const bool more = (begin ? walk.begin() : walk.next()) && !__any_sync(0xffffffffu, *gave_up);
       if (!more) walk.p.c0 = walk.p.c1 = 0;
       it = walk.p;
       if (it.c0 == 0 && it.c1 > 0 && it.c1 < it.k.chunks) {
