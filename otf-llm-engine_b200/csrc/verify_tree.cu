@@ -61,7 +61,8 @@ struct TreeArgs {
 
 struct TreeLeader {
   double score;
-  int at, pad;
+  int at;
+  int seq;  // in the leaders of k_tree_leaders: whose temperature and noise it was found with, -1: nobody's
 };
 __device__ __forceinline__ bool leads(double s, int i, const TreeLeader& l) { return s > l.score || (s == l.score && i < l.at); }
 
@@ -226,18 +227,25 @@ __global__ void __launch_bounds__(kTreeThreads, 4) k_tree_leaders(TreeArgs a) {
   pdl_wait();
   const int row = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (warp == 0) {
-    int b = 0, level = 0;
+    // the first sequence that has the row, and the node's depth, up through its parents in the lanes
+    int b = -1, level = 0, r0 = 0, r1 = 0;
     if (a.starts) {
-      for (int i = 0; i < a.batch; i += 32)
-        b += __popc(__ballot_sync(0xffffffffu, i + lane < a.batch && a.starts[i + lane + 1] <= row));
+      for (int i = 0; i < a.batch && b < 0; i += 32) {
+        const int x = i + lane < a.batch ? a.starts[i + lane] : 0, y = i + lane < a.batch ? a.starts[i + lane + 1] : 0;
+        const uint32_t in = __ballot_sync(0xffffffffu, x >= 0 && x <= row && row < y && y <= a.n && y - x <= kTreeMaxNodes);
+        if (in) {
+          const int from = __ffs((int)in) - 1;
+          b = i + from;
+          r0 = __shfl_sync(0xffffffffu, x, from);
+          r1 = __shfl_sync(0xffffffffu, y, from);
+        }
+      }
     } else {
       b = row / a.per;
+      r0 = b * a.per;
+      r1 = r0 + a.per;
     }
-    // the node's depth, up through its parents in the lanes
-    const int r0 = b < a.batch ? (a.starts ? a.starts[b] : b * a.per) : 0, r1 = b < a.batch ? (a.starts ? a.starts[b + 1] : r0 + a.per) : 0;
-    if (b >= a.batch || r0 < 0 || r1 > a.n || row < r0 || r1 - r0 > kTreeMaxNodes) {
-      b = -1;
-    } else {
+    if (b >= 0) {
       int up[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -263,9 +271,12 @@ __global__ void __launch_bounds__(kTreeThreads, 4) k_tree_leaders(TreeArgs a) {
   }
   __syncthreads();
   const int b = s_seq;
-  if (b < 0) return;
-  const double T = a.temperatures ? (double)a.temperatures[b] : a.temperature;
-  if (!temperature_ok((float)T) || (T > 0.0 && !a.noise)) return;  // k_tree_walk reports it
+  TreeLeader* const to = a.leaders + (int64_t)row * a.slices + blockIdx.x;
+  const double T = b < 0 ? -1.0 : a.temperatures ? (double)a.temperatures[b] : a.temperature;
+  if (!temperature_ok((float)T) || (T > 0.0 && !a.noise)) {  // k_tree_walk reports a sequence's
+    if (tid == 0) *to = {-INFINITY, INT_MAX, -1};
+    return;
+  }
   const float c = T > 0.0 ? (float)(1.4426950408889634 / T) : 0.0f;
   const float* x = a.target + (int64_t)row * a.ldt;
   const float* e = T > 0.0 ? a.noise + b * a.nseq + s_level * a.ldn : nullptr;
@@ -275,11 +286,12 @@ __global__ void __launch_bounds__(kTreeThreads, 4) k_tree_leaders(TreeArgs a) {
   __syncthreads();
   if (warp == 0) {
     const TreeLeader all = tree_leader_of_warp(lane < kTreeWarps ? s_warp[lane] : TreeLeader{-INFINITY, INT_MAX, 0});
-    if (lane == 0) a.leaders[(int64_t)row * a.slices + blockIdx.x] = all;
+    if (lane == 0) *to = {all.score, all.at, b};
   }
 }
 
-// And the ways through them: a warp per sequence.
+// And the ways through them: a warp per sequence.  Rows that another sequence has too (starts that fall) were looked at
+// for the first of them; the others look for themselves.
 __global__ void __launch_bounds__(32) k_tree_walk(TreeArgs a) {
   __shared__ int64_t s_tokens[kTreeMaxNodes];
   __shared__ int s_path[kTreeMaxNodes];
@@ -303,7 +315,7 @@ __global__ void __launch_bounds__(32) k_tree_walk(TreeArgs a) {
           parent[h] = -1;
         }
       }
-    // a lane's nodes' leaders (those that cannot be reached hold what happens to lie there)
+    // a lane's nodes' leaders
 #pragma unroll 1
     for (int i = lane; i < nodes; i += 32) {
       const TreeLeader* l = a.leaders + (int64_t)(r0 + i) * a.slices;
@@ -313,13 +325,23 @@ __global__ void __launch_bounds__(32) k_tree_walk(TreeArgs a) {
         const TreeLeader y = l[k];
         if (y.at != INT_MAX && leads(y.score, y.at, all)) all = y;
       }
-      s_drawn[i] = all.at;
+      s_drawn[i] = l[0].seq == b ? all.at : -1;
     }
   }
   __syncwarp();
   int at = 0, taken = 0;
   while (!failed) {
-    const int drawn = s_drawn[at];
+    int drawn = s_drawn[at];
+    if (drawn < 0) {
+      const float* x = a.target + (int64_t)(r0 + at) * a.ldt;
+      const float* e = T > 0.0 ? a.noise + b * a.nseq + taken * a.ldn : nullptr;
+      TreeLeader mine = {-INFINITY, INT_MAX, 0};
+      for (int i = lane; i < a.vocab; i += 32) {
+        const double s = tree_score(x[i], e ? e[i] : 1.0f, T);
+        if (s > -INFINITY && leads(s, i, mine)) mine = {s, i, 0};
+      }
+      drawn = tree_leader_of_warp(mine).at;
+    }
     if (drawn == INT_MAX) {
       failed = true;
       break;

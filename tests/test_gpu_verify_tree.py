@@ -170,3 +170,37 @@ def test_keep_leaves_out_what_does_not_fit(cuda_dev):
         cache.keep(torch.tensor(way, dtype=torch.int32, device=cuda_dev), torch.tensor(count, dtype=torch.int32, device=cuda_dev))
         assert flag() == 1
         assert same(cache.k_pages, before[0]) and same(cache.v_pages, before[1])
+
+
+@pytest.mark.parametrize("temperature", [0.0, 0.8])
+@pytest.mark.parametrize("vocab", [700, 200000])
+def test_a_sequence_beside_starts_that_fall(vocab, temperature, cuda_dev):
+    """A sequence whose rows are in order gets its tokens whatever the starts beside it are, few logits or many; also where
+    two sequences have the same rows."""
+    from otf_llm.speculative import verify_tree
+    depth = 3
+    target, tokens, parents, _ = trees([7, 6, 64], vocab, depth, 5)
+    flat = torch.tensor([p for up in parents for p in up], dtype=torch.int32)
+    noise = torch.empty(5, depth + 1, vocab).exponential_(generator=torch.Generator().manual_seed(6))
+
+    def want(b, r0, r1):
+        up = [int(p) for p in flat[r0:r1]]
+        drawn, way, taken = ref.walk(target[r0:r1], tokens[r0:r1], up, noise[b], temperature, depth)
+        return drawn + [-1] * (depth + 1 - len(drawn)), way + [-1] * (depth - taken), taken
+    dev = [t.to(cuda_dev) for t in (target, tokens, flat, noise)]
+    for starts, good in (([0, 7, 3, 3, 3, 3], {0: (0, 7)}), ([7, 13, 7, 13, 13, 13], {0: (7, 13), 2: (7, 13)}),
+                         ([0, 7, 0, 7, 13, 77], {0: (0, 7), 2: (0, 7), 3: (7, 13), 4: (13, 77)}),
+                         ([90, 0, 7, -5, 7, 13], {1: (0, 7), 4: (7, 13)})):
+        for _ in range(2):                              # the second time over what the first one left in the scratch
+            out, path, accepted = verify_tree(dev[0], dev[1], dev[2], starts=torch.tensor(starts, dtype=torch.int32, device=cuda_dev),
+                                              depth=depth, noise=dev[3], temperature=temperature)
+        assert flag() == 1
+        for b in range(5):
+            expect = want(b, *good[b]) if b in good else ([-1] * (depth + 1), [-1] * depth, 0)
+            assert (out[b].tolist(), path[b].tolist(), int(accepted[b])) == expect, (starts, b)
+    # the first sequence with the rows has no temperature to be walked at
+    temps = torch.tensor([-1.0, 1.0, temperature, 1.0, 1.0], device=cuda_dev)
+    for _ in range(2):
+        out, _, accepted = verify_tree(dev[0], dev[1], dev[2], starts=torch.tensor([7, 13, 7, 13, 13, 13], dtype=torch.int32, device=cuda_dev),
+                                       depth=depth, noise=dev[3], temperature=temps)
+        assert flag() == 1 and out[:2].eq(-1).all() and (out[2].tolist(), int(accepted[2])) == (want(2, 7, 13)[0], want(2, 7, 13)[2])
