@@ -5,8 +5,9 @@
 
 namespace otf {
 
-// 0, or from 1e-20 on (log2(e) / T stays finite; its product with a difference of logits need not).
-__host__ __device__ __forceinline__ bool temperature_ok(float T) { return T == 0.0f || (T >= 1e-20f && T <= 1e20f); }
+// 0, or from 1e-20 on (log2(e) / T stays finite; its product with a difference of logits need not).  In 64 bits: a number
+// that fp32 would hold as 0 is none of them.
+__host__ __device__ __forceinline__ bool temperature_ok(double T) { return T == 0.0 || (T >= 1e-20f && T <= 1e20f); }
 
 // Four consecutive values of a row, `pad` behind its end.  Rows that are not 16-byte aligned are read
 // value by value by the same threads, so that a row's sums do not depend on where it lies.

@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kTreeThreads, 4) k_verify_tree(TreeArgs a, int
   const int b = blockIdx.x / ctas, rank = blockIdx.x - b * ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int r0 = a.starts ? a.starts[b] : b * a.per, r1 = a.starts ? a.starts[b + 1] : r0 + a.per, nodes = r1 - r0;
   const double T = a.temperatures ? (double)a.temperatures[b] : a.temperature;
-  const bool ok = r0 >= 0 && r1 <= a.n && nodes > 0 && nodes <= kTreeMaxNodes && temperature_ok((float)T) && (T == 0.0 || a.noise);
+  const bool ok = r0 >= 0 && r1 <= a.n && nodes > 0 && nodes <= kTreeMaxNodes && temperature_ok(T) && (T == 0.0 || a.noise);
   cluster_arrive_relaxed();
   // the nodes, two in each lane of the first warp
   int64_t token[2] = {-1, -1};
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kTreeThreads, 4) k_tree_leaders(TreeArgs a) {
   const int b = s_seq;
   TreeLeader* const to = a.leaders + (int64_t)row * a.slices + blockIdx.x;
   const double T = b < 0 ? -1.0 : a.temperatures ? (double)a.temperatures[b] : a.temperature;
-  if (!temperature_ok((float)T) || (T > 0.0 && !a.noise)) {  // k_tree_walk reports a sequence's
+  if (!temperature_ok(T) || (T > 0.0 && !a.noise)) {  // k_tree_walk reports a sequence's
     if (tid == 0) *to = {-INFINITY, INT_MAX, -1};
     return;
   }
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(32) k_tree_walk(TreeArgs a) {
   const int b = blockIdx.x, lane = threadIdx.x;
   const int r0 = a.starts ? a.starts[b] : b * a.per, r1 = a.starts ? a.starts[b + 1] : r0 + a.per, nodes = r1 - r0;
   const double T = a.temperatures ? (double)a.temperatures[b] : a.temperature;
-  bool failed = !(r0 >= 0 && r1 <= a.n && nodes > 0 && nodes <= kTreeMaxNodes && temperature_ok((float)T) && (T == 0.0 || a.noise));
+  bool failed = !(r0 >= 0 && r1 <= a.n && nodes > 0 && nodes <= kTreeMaxNodes && temperature_ok(T) && (T == 0.0 || a.noise));
   int64_t token[2] = {-1, -1};
   int parent[2] = {-1, -1};
   if (!failed) {
@@ -398,7 +398,7 @@ extern "C" OTF_API int otf_verify_tree(const float* target, int64_t ld_target, c
                                        int64_t workspace_bytes, void* stream) {
   if (!target || !tokens || !parents || !out_tokens || (!path && depth) || !accepted) return OTF_ERR_INVALID;
   if (batch <= 0 || depth < 0 || vocab <= 0 || n <= 0 || (!starts && n % batch) || ld_target < vocab) return OTF_ERR_INVALID;
-  if (!temperatures && !otf::temperature_ok((float)temperature)) return OTF_ERR_INVALID;
+  if (!temperatures && !otf::temperature_ok(temperature)) return OTF_ERR_INVALID;
   if (!noise && (temperatures || temperature > 0.0)) return OTF_ERR_INVALID;
   if (noise && (ld_noise < vocab || noise_seq < 0)) return OTF_ERR_INVALID;
   if (batch > 65535 || depth >= otf::kTreeMaxNodes || vocab > (1ll << 30) || n > INT32_MAX ||

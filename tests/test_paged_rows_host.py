@@ -78,6 +78,12 @@ def test_abi_refuses_bad_trees(other, status):
     assert tree(**other) == status
 
 
+@pytest.mark.parametrize("temperature", [1e-50, 1e-46, 5e-324, 9e-21, 1.1e20, float("inf"), -0.1])
+def test_abi_refuses_temperatures_beside_the_range(temperature):
+    """Also those that fp32 would hold as 0."""
+    assert tree(temperature=temperature) == INVALID
+
+
 def test_tree_workspace():
     from otf_llm import _native as N
     size = N.lib().otf_verify_tree_workspace_bytes
