@@ -435,7 +435,9 @@ class PagedKVCache:
         place lengths[b] + path[b, j] go to lengths[b] + 1 + j, behind the root's.
 
         path (int32 [batch, depth], 63 deep at most) and accepted (int32 [batch]) as ``verify_tree`` gives them.
-        Every layer's cache is kept before ``advance(accepted + 1)`` counts the root and the taken nodes."""
+        Every layer's cache is kept before ``advance`` counts the root and the taken nodes: as many as tokens
+        came out, ``(tokens >= 0).sum(1, dtype=torch.int32)``, which is accepted + 1 and for a sequence that had no nodes,
+        or none to draw from, 0."""
         if path.device != self.device or path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != self.batch or \
                 (path.stride(1) != 1 and path.shape[1] > 1):
             raise ValueError(f"path must be int32 [{self.batch}, depth] with a unit inner stride on {self.device}, got "
@@ -492,7 +494,8 @@ class PagedKVCache:
 
     def advance(self, tokens: Union[int, torch.Tensor] = 1) -> None:
         """lengths += tokens, where there is a sequence: a number, or int32 [batch] on the device where the
-        sequences differ (``starts.diff()`` after prompts, ``accepted + 1`` after a pass over drafts)."""
+        sequences differ (``starts.diff()`` after prompts, ``accepted + 1`` after a pass over drafts that every
+        sequence had, ``(tokens >= 0).sum(1, dtype=torch.int32)`` after one that some had no nodes in)."""
         there = self.lengths.ge(0).to(torch.int32)
         if isinstance(tokens, torch.Tensor):
             self._vector(tokens, "tokens", self.batch)

@@ -451,3 +451,27 @@ def test_odd_values_of_one_sequence_leave_all_others(lengths, new, heads, kv, di
     for got in calls:
         assert torch.equal(~got.isfinite(), want_odd)
         assert same(torch.where(want_odd, 0, got), torch.where(want_odd, 0, plain))
+
+
+def test_a_live_sequence_without_nodes_in_a_step(cuda_dev):
+    """As many places as tokens came out are counted: a sequence that has no nodes in a step, or nothing to draw from, keeps
+    its length, and what it attends afterwards."""
+    from otf_llm.speculative import verify_tree
+    cache, _, table, g = make(cuda_dev, [40, 33, 50], 16, 2, 64, torch.float16, room=[60, 60, 60], seed=12)
+    cache.lengths.copy_(torch.tensor([36, 32, 45], dtype=torch.int32))
+    q = torch.randn(3, 4, 64, generator=g).half().to(cuda_dev)
+    before = cache.attend_rows(q)
+    starts = torch.tensor([0, 3, 3, 7], dtype=torch.int32, device=cuda_dev)
+    parents = torch.tensor([-1, 0, 1, -1, 0, 0, 1], dtype=torch.int32, device=cuda_dev)
+    target = torch.zeros(7, 9, device=cuda_dev)
+    target[0, 4] = target[1, 5] = 1.0
+    target[3] = -float("inf")
+    ids = torch.tensor([0, 4, 7, 0, 1, 2, 3], device=cuda_dev)
+    tokens, path, accepted = verify_tree(target, ids, parents, starts=starts, depth=2, temperature=0.0)
+    assert flag() == 1                                  # the last sequence has nothing to draw from
+    assert tokens.tolist() == [[4, 5, -1], [-1] * 3, [-1] * 3] and accepted.tolist() == [1, 0, 0]
+    cache.keep(path, accepted)
+    cache.advance((tokens >= 0).sum(1, dtype=torch.int32))
+    assert cache.lengths.tolist() == [38, 32, 45] and flag() == 0
+    after = cache.attend_rows(q)
+    assert same(after[1:], before[1:]) and not same(after[0], before[0])
