@@ -122,6 +122,12 @@ template <int T>
 struct LpRaw {
   uint4 x[T == 0 ? 4 : 2];
 };
+// Two 16-bit logits of a lane's 16, z of 8.
+template <int T>
+__device__ __forceinline__ uint32_t lp_word(const LpRaw<T>& raw, int z) {
+  const uint4& x = raw.x[z >> 2];
+  return (z & 3) == 0 ? x.x : (z & 3) == 1 ? x.y : (z & 3) == 2 ? x.z : x.w;
+}
 template <int T>
 __device__ __forceinline__ void lp_load(const void* row, int64_t i0, int vocab, bool aligned, LpRaw<T>& raw) {
   constexpr int N = T == 0 ? 4 : 2, E = 16 / N;
@@ -181,15 +187,15 @@ __device__ __forceinline__ float lp_greater(float x, float y) {
 template <int T, bool EQUAL>
 __device__ __forceinline__ float2 lp_ahead(const LpRaw<T>& raw, const float (&v)[16], float than) {
   float2 n = make_float2(0.0f, 0.0f);
-  if (T == 0) {
+  if constexpr (T == 0) {
 #pragma unroll
     for (int j = 0; j < 16; j += 2) add_two(n.x, n.y, lp_greater<EQUAL>(v[j], than), lp_greater<EQUAL>(v[j + 1], than));
-  } else if (T == 1) {
+  } else if constexpr (T == 1) {
     const __half2 y = __float2half2_rn(than);  // exact: it is one of the row's
     __half2 sum = __float2half2_rn(0.0f);
 #pragma unroll
     for (int z = 0; z < 8; ++z) {
-      const uint32_t w = (&raw.x[z >> 2].x)[z & 3];
+      const uint32_t w = lp_word<T>(raw, z);
       const __half2 x = *reinterpret_cast<const __half2*>(&w);
       sum = __hadd2(sum, EQUAL ? __hge2(x, y) : __hgt2(x, y));
     }
@@ -199,7 +205,7 @@ __device__ __forceinline__ float2 lp_ahead(const LpRaw<T>& raw, const float (&v)
     __nv_bfloat162 sum = __float2bfloat162_rn(0.0f);
 #pragma unroll
     for (int z = 0; z < 8; ++z) {
-      const uint32_t w = (&raw.x[z >> 2].x)[z & 3];
+      const uint32_t w = lp_word<T>(raw, z);
       const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&w);
       sum = __hadd2(sum, EQUAL ? __hge2(x, y) : __hgt2(x, y));
     }
@@ -210,29 +216,30 @@ __device__ __forceinline__ float2 lp_ahead(const LpRaw<T>& raw, const float (&v)
 // The largest of a lane's 16 logits (NaN aside).
 template <int T>
 __device__ __forceinline__ float lp_top(const LpRaw<T>& raw, const float (&v)[16]) {
-  if (T == 0) {
+  if constexpr (T == 0) {
     float top = v[0];
 #pragma unroll
     for (int j = 1; j < 15; j += 2) top = max_three(top, v[j], v[j + 1]);
     return fmaxf(top, v[15]);
-  }
-  uint32_t w[8];
+  } else {
+    uint32_t w[8];
 #pragma unroll
-  for (int z = 0; z < 8; ++z) w[z] = (&raw.x[T == 0 ? 0 : z >> 2].x)[z & 3];
+    for (int z = 0; z < 8; ++z) w[z] = lp_word<T>(raw, z);
 #pragma unroll
-  for (int o = 4; o > 0; o >>= 1)
+    for (int o = 4; o > 0; o >>= 1)
 #pragma unroll
-    for (int z = 0; z < o; ++z) {
-      if (T == 1) {
-        const __half2 y = __hmax2(*reinterpret_cast<const __half2*>(&w[z]), *reinterpret_cast<const __half2*>(&w[z + o]));
-        w[z] = *reinterpret_cast<const uint32_t*>(&y);
-      } else {
-        const __nv_bfloat162 y = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&w[z]), *reinterpret_cast<const __nv_bfloat162*>(&w[z + o]));
-        w[z] = *reinterpret_cast<const uint32_t*>(&y);
+      for (int z = 0; z < o; ++z) {
+        if (T == 1) {
+          const __half2 y = __hmax2(*reinterpret_cast<const __half2*>(&w[z]), *reinterpret_cast<const __half2*>(&w[z + o]));
+          w[z] = *reinterpret_cast<const uint32_t*>(&y);
+        } else {
+          const __nv_bfloat162 y = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&w[z]), *reinterpret_cast<const __nv_bfloat162*>(&w[z + o]));
+          w[z] = *reinterpret_cast<const uint32_t*>(&y);
+        }
       }
-    }
-  const float2 y = unpack2<T == 2>(w[0]);
-  return fmaxf(y.x, y.y);
+    const float2 y = unpack2<T == 2>(w[0]);
+    return fmaxf(y.x, y.y);
+  }
 }
 __device__ __forceinline__ float lp_ex2(float x) {
   float y;
