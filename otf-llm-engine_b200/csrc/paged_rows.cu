@@ -29,6 +29,12 @@
 // through such a window, 0.90 GB, 166 to 208 us = 4.3 to 5.4 TB/s; trees of 8 to 64 nodes of 32 sequences on up to 8190
 // tokens, 0.2 TFLOP and 0.6 GB, 245 to 287 us; one token through a window of 1024 (32 heads) 13.5 us.
 //
+// Probabilities go into the products as 16-bit numbers, as tcgen05 takes them beside 16-bit values.  Blocks of 128 rows or fewer
+// have room on the matrix pipe for two, the rounding and the rest, and outputs off by little but their own rounding.  Blocks of
+// more take one: with two the prompts above take 3.03 in place of 2.45 ms and the trees 324 in place of 269 us, and their
+// root mean square error falls from 2.7e-4 (fp16) and 2.2e-3 (bf16) of the outputs to 2.0e-4 and 1.7e-3, that of the
+// outputs' rounding alone.  Sums are of the probabilities before either.
+//
 // The products of one thread run in the order of their issue: scores that overwrite a chunk's probabilities wait for its
 // outputs, and a chunk's scores are complete after the outputs of the chunk before (nothing else guards either).
 // Halves of a chunk whose scores are there ahead of time (64 keys a product) were slower: 2.76 against 2.44 ms on the prompts.
@@ -54,8 +60,8 @@ constexpr int kPrGrid = 148;      // a CTA on each SM
 constexpr int kPrMma = 8, kPrQuery = 9, kPrLoad = 10;  // warps that issue products, fetch queries, and two that fetch keys and values
 constexpr int kPrThreads = 384;
 constexpr int kPrMaxNodes = 64;
-// What an item's start and end cost, in chunks.  With 2, 3 and 4: a batch's step (as above) 194, 188 and 185 us, trees 266,
-// 265 and 268, prompts 2.50, 2.51 and 2.52 ms.
+// What an item's start and end cost, in chunks.  With 2, 3 and 4 on one GPU: a batch's step (as above) 194, 188 and 185 us,
+// trees 266, 265 and 268, prompts 2.50, 2.51 and 2.52 ms (between GPUs they differ by more).
 constexpr int kPrItemUnits = 3;
 constexpr float kPrLog2e = 1.4426950408889634f;
 
@@ -262,7 +268,7 @@ struct Walk {
   }
 };
 
-constexpr int kPrSmall = 3072;
+constexpr int kPrSmall = 3 * 1024;
 
 template <int D>
 struct RowsShape {
@@ -442,6 +448,7 @@ __device__ __noinline__ void add_odd(const RowsArgs& a, const Portion& it, const
     }
   }
 }
+// (The call keeps some 240 to 430 bytes a thread in local memory; blocks without odd values never make it.)
 template <bool BF, int D, bool TREE, int N>
 __device__ __forceinline__ void give_back(const RowsArgs& a, const Portion& it, const RowView& view, float (&o)[N], int col) {
   const Portion here = it;  // copies: what lies in memory for the call

@@ -13,8 +13,9 @@
 // one before it has ended: some 4 us.  Few logits: every node's leader is found at once by the whole GPU, with the
 // noise of the node's depth, and the way is then followed in a second launch (k_tree_leaders, k_tree_walk).
 //
-// Measured: 64 sequences of 5 to 40 nodes over 128256 at temperature 0.8, some 0.33 GB on the ways, 54 to 67 us; one of 26
-// nodes over 32000, greedy, 7.5 to 7.9 us.
+// Measured: 64 sequences of 5 to 40 nodes over 128256 at temperature 0.8, ways of 2 rows on average and of 6 or 7 the longest,
+// 0.13 to 0.14 GB, 54 to 67 us: 2 to 2.6 TB/s, bound by the longest ways' steps, one after another, while the CTAs of ways
+// that have ended idle; one of 26 nodes over 32000, greedy, 7.5 to 7.9 us.
 #include <algorithm>
 
 #include "logits.cuh"
@@ -32,8 +33,10 @@ constexpr int kTreeWarps = kTreeThreads / 32;
 constexpr int kTreeCluster = 16;
 constexpr int kTreeResident = 148 * 4;  // CTAs that run at once
 constexpr int kTreeSlice = 8192;        // entries of a CTA of k_tree_leaders
-// Logits of all nodes up to which they are looked at at once.  Measured, clusters against at once, greedy and at
-// temperature 0.8: one sequence of 26 nodes over 32000 23.5 against 7.6 us and 9.1 against 7.9 (a way of few steps), of 64
+// Logits of all nodes up to which they are looked at at once.  At once takes as long whatever the way is, clusters some 4 us a
+// step and so less for short ways.  The host does not know how long a way is; the border lies where long ways no longer gain,
+// and below it short ones lose.  Measured, one way each, clusters against at once, greedy (long ways) and at temperature 0.8
+// (shorter ones): one sequence of 26 nodes over 32000 23.5 against 7.6 us and 9.1 against 7.9, of 64
 // over 128256 (8.2M) 27 against 19 and 6.5 against 22, 16 of 26 over 32000 (13.3M) 29 against 16 and 30 against 21, 4 of
 // 40 over 128256 (20.5M) 30 against 29 and 22 against 37, 16 of 26 over 128256 (53M) 38 against 63 and 35 against 76.
 constexpr int64_t kTreeAtOnce = 13ll << 20;

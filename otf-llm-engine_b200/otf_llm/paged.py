@@ -363,7 +363,12 @@ class PagedKVCache:
         sequence b, at place p = lengths[b] + t, sees the tokens up to its own; with a ``window`` only the last
         ``window`` of them, places above p - window, and the first ``sinks`` of the sequence.  ``scale`` defaults
         to head_dim ** -0.5.  Returns ``out``, of q's shape, which shares no memory with q (rows behind the
-        last sequence and of negative lengths are left as they were)."""
+        last sequence and of negative lengths are left as they were).
+
+        Probabilities are rounded where many rows lie together: those of a sequence, tokens times query heads of a KV
+        head, go in blocks of 256, and in a block of more than 128 each probability is one number of the cache's type
+        (an error of the outputs of 1.3 times that of their own rounding, measured), else two.  So a token's last
+        bits may differ between a long prompt and a short one; equal calls give equal bits."""
         return self._attend_rows(q, None, starts, window, sinks, scale, out)
 
     def attend_tree(self, q: torch.Tensor, parents: torch.Tensor, *, starts: Optional[torch.Tensor] = None,
@@ -376,7 +381,8 @@ class PagedKVCache:
         parents[row] < t of its sequence, or with -1 on the cached tokens alone.  A node sees the cached tokens
         (with a ``window``, 64 at least, those within it by position, and the first ``sinks``), the nodes above
         it and itself.  ``verify_tree`` chooses a way through the tree, and ``keep`` moves its nodes together.
-        The rest is as in ``attend_rows``."""
+        The rest is as in ``attend_rows``, the rounding of probabilities too: with 8 query heads a KV head, 16
+        nodes have two numbers for each, 17 to 32 one."""
         return self._attend_rows(q, parents, starts, window, sinks, scale, out)
 
     def _attend_rows(self, q: torch.Tensor, parents: Optional[torch.Tensor], starts: Optional[torch.Tensor],
