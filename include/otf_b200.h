@@ -545,8 +545,8 @@ OTF_API int otf_paged_attn(const otf_paged_cache* cache, const void* q, int64_t 
  * head_dim], row stride ldq; starts: device int32 [batch + 1], or NULL: n / batch rows each), as
  * otf_paged_append took them: row t is token lengths[b] + t, lengths not yet advanced.  out (row stride ldo, no
  * memory shared with q) = softmax(scale q k) v over the tokens that a row sees.  What it does not see does not reach
- * it, whatever it holds; a NaN or infinity among the keys and values that it does see reaches all of its output
- * (keys) or the same column (values), as a NaN or infinity.  Scores, sums and outputs in fp32 with one rounding; each
+ * it, whatever it holds; a NaN among the keys that it does see makes its output NaN, one among the values the same
+ * column, and an infinity among the values makes that column an infinity or NaN.  Scores, sums and outputs in fp32 with one rounding; each
  * probability goes into its product as two 16-bit numbers, or as one, half a step of the cache's type off at most, in
  * those blocks of 256 rows (a sequence's tokens x query heads of a KV head) that have more than 128.
  * parents NULL: row t, at place p = lengths[b] + t, sees the tokens s <= p, with a window (0: none) only those
@@ -648,7 +648,8 @@ OTF_API int otf_verify_drafts(const float* target, int64_t target_seq, int64_t l
  * [batch, depth], the taken nodes, then -1; accepted: int32 [batch], how many.  A NaN among the logits counts as
  * -inf; a token of weight 0 is never drawn.  A sequence without nodes gets -1 and 0 accepted.  One without a token to
  * draw, with rows not in [0, n], a number of nodes or a temperature out of range gets -1, 0 accepted, and raises the
- * otf_device_error flag; so does a parent out of range, whose node hangs nowhere.  Scores that decide are compared in 64 bits.  depth 0..63; at most 65535
+ * otf_device_error flag; so does a parent out of range, whose node hangs nowhere.  Scores that decide are compared in
+ * 64 bits.  depth 0..63; at most 65535
  * sequences and a vocabulary of 2^30.  workspace: otf_verify_tree_workspace_bytes(...) (0 for many logits, then it may be
  * NULL), 16-byte aligned, need not be cleared; two calls that may run at the same time need one each.  Beside
  * otf_verify_drafts, for drafts in a line.
